@@ -271,11 +271,11 @@ def _sample_plain(st):
     temp, k, p, least = st["temperature"], st["top_k"].long(), st["top_p"], st["min_p"]
     warm = temp > 0
     k = torch.where(warm, torch.where((k <= 0) | (k > v), v, k), 1)[:, None]      # temperature 0: the largest logit
-    s = x * torch.where(warm, 1 / temp, 1.0)[:, None]
-    s = torch.where(torch.isnan(s), -math.inf, s)
-    top = s.max(1, keepdim=True)[0]
-    e = torch.where(s == top, 1.0, torch.exp(s - top))
-    e = torch.where(s > -math.inf, e, 0.0)
+    x = torch.where(torch.isnan(x), -math.inf, x)
+    top = x.max(1, keepdim=True)[0]
+    s = torch.where(x == top, 0.0, (x - top) * torch.where(warm, 1 / temp, 1.0)[:, None])
+    s = torch.where((x > -math.inf) & ~torch.isnan(s), s, -math.inf)
+    e = torch.exp(s)
     w = (e * ONE).to(torch.int64)                                   # integer weights: sums that no order changes
     order = torch.sort(s, dim=1, descending=True, stable=True)[1]       # ties to the lowest index
     ws = torch.gather(w, 1, order)
@@ -293,7 +293,7 @@ def _sample_plain(st):
     token = (run_up <= target).sum(1)
     empty = total[:, 0] == 0
     token = torch.where(empty, 0, token)
-    got = torch.gather(s - top, 1, token[:, None])[:, 0] - torch.log(total[:, 0].double() / ONE).float()
+    got = torch.gather(s, 1, token[:, None])[:, 0] - torch.log(total[:, 0].double() / ONE).float()
     return torch.where(empty, -1, token), torch.where(empty, -math.inf, got)
 
 

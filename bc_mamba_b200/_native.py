@@ -54,6 +54,15 @@ ABI_SYMBOLS = (
     "bcm_s6_bwd",
     "bcm_event_params_fwd",
     "bcm_event_params_bwd",
+    "bcm_gated_rec_ckpt_bytes",
+    "bcm_gated_rec_bwd_workspace_bytes",
+    "bcm_gated_rec_fwd",
+    "bcm_gated_rec_bwd",
+    "bcm_gated_rec_step",
+    "bcm_distill_fwd",
+    "bcm_distill_bwd",
+    "bcm_distill_fwd_grad",
+    "bcm_sample_tokens",
 )
 
 _ops = None

@@ -1272,6 +1272,246 @@ std::vector<Tensor> event_params_bwd(const Tensor& A, const Tensor& a0, const Te
     return {dA_log, dW_BC, da0, da1};
 }
 
+// --------------------------------------------- language-model operators ----
+// (no reference bindings; messages name shapes symbolically, see check_status)
+bcm_dtype float_dtype(const Tensor& t, const char* name) {
+    TORCH_CHECK(t.scalar_type() == at::ScalarType::Float || t.scalar_type() == at::ScalarType::Half ||
+                    t.scalar_type() == at::ScalarType::BFloat16,
+                name, " must be float32, float16 or bfloat16");
+    return to_bcm(t.scalar_type(), name);
+}
+
+// x, r, i (or dy): (B, L, D), packed (T, D), or one token (B, D); unit stride of the features
+void check_rows(const char* what, const Tensor& t, const char* name, const Tensor& like) {
+    TORCH_CHECK(t.is_cuda() && t.device() == like.device(), what, ": ", name, " must be on the device of x");
+    TORCH_CHECK(t.scalar_type() == like.scalar_type(), what, ": ", name, " must have the dtype of x");
+    TORCH_CHECK(t.sizes() == like.sizes(), what, ": ", name, " must have the shape of x");
+    TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1, what, ": ", name, " must have unit stride in its last dimension");
+}
+
+const float* fp32_ptr(const char* what, const Tensor& t, const char* name, const Tensor& like, c10::IntArrayRef shape) {
+    TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == at::ScalarType::Float && t.is_contiguous(),
+                what, ": ", name, " must be a contiguous float32 tensor on the device of the input");
+    TORCH_CHECK(t.sizes() == shape, what, ": ", name, " has the wrong shape");
+    return t.data_ptr<float>();
+}
+
+// Sizes, input pointers and strides of a gated recurrence (forward and backward).
+bcm_gated_rec_args gated_rec_args(const char* what, const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& lam,
+                                  const optional<Tensor>& h0, const optional<Tensor>& cu_seqlens, double decay_scale) {
+    TORCH_CHECK(x.is_cuda(), what, ": x must be on CUDA");
+    const bool packed = cu_seqlens.has_value();
+    TORCH_CHECK(x.dim() == (packed ? 2 : 3), what, ": x must be (B, L, D), or (T, D) with cu_seqlens");
+    bcm_gated_rec_args a{};
+    a.dtype = float_dtype(x, "x");
+    check_rows(what, x, "x", x);
+    check_rows(what, r, "r", x);
+    check_rows(what, i, "i", x);
+    if (packed) {
+        const Tensor& cu = *cu_seqlens;
+        TORCH_CHECK(cu.is_cuda() && cu.device() == x.device() && cu.scalar_type() == at::ScalarType::Int &&
+                        cu.is_contiguous() && cu.dim() == 1 && cu.size(0) >= 1,
+                    what, ": cu_seqlens must be a contiguous 1-D int32 tensor on the device of x");
+        a.batch = cu.size(0) - 1;
+        a.seqlen = x.size(0);
+        a.cu_seqlens = cu.data_ptr<int32_t>();
+        TORCH_CHECK(a.batch >= 1 || a.seqlen == 0, what, ": cu_seqlens of no sequence with tokens");
+    } else {
+        a.batch = x.size(0);
+        a.seqlen = x.size(1);
+    }
+    a.dim = x.size(-1);
+    TORCH_CHECK(a.dim >= 1, what, ": x must have features");
+    auto set = [&](const Tensor& t, const void*& p, int64_t& sb, int64_t& st) {
+        p = t.data_ptr();
+        sb = packed ? 0 : t.stride(0);
+        st = t.stride(packed ? 0 : 1);
+    };
+    set(x, a.x, a.x_stride_b, a.x_stride_t);
+    set(r, a.r, a.r_stride_b, a.r_stride_t);
+    set(i, a.i, a.i_stride_b, a.i_stride_t);
+    a.lam = fp32_ptr(what, lam, "lam", x, {a.dim});
+    a.h0 = h0.has_value() ? fp32_ptr(what, *h0, "h0", x, {a.batch, a.dim}) : nullptr;
+    a.decay_scale = (float)decay_scale;
+    return a;
+}
+
+std::vector<Tensor> gated_rec_fwd(const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& lam,
+                                  const optional<Tensor>& h0, const optional<Tensor>& cu_seqlens, double decay_scale,
+                                  bool keep_ckpt) {
+    bcm_gated_rec_args a = gated_rec_args("gated_rec_fwd", x, r, i, lam, h0, cu_seqlens, decay_scale);
+    c10::cuda::CUDAGuard guard(x.device());
+    auto y = torch::empty(x.sizes(), x.options());
+    auto h_last = torch::empty({a.batch, a.dim}, lam.options());
+    a.y = y.data_ptr();
+    a.h_last = h_last.data_ptr<float>();
+    std::vector<Tensor> out = {y, h_last};
+    if (keep_ckpt) {
+        auto ckpt = workspace((int64_t)bcm_gated_rec_ckpt_bytes(&a), x.device());
+        a.ckpt = ckpt.data_ptr();
+        a.ckpt_bytes = (size_t)ckpt.numel();
+        out.push_back(ckpt);
+    }
+    check_status(bcm_gated_rec_fwd(&a, cur_stream()), "gated_rec_fwd");
+    return out;
+}
+
+std::vector<Tensor> gated_rec_bwd(const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& lam,
+                                  const optional<Tensor>& h0, const optional<Tensor>& cu_seqlens, double decay_scale,
+                                  const Tensor& ckpt, const optional<Tensor>& dy, const optional<Tensor>& dh_last) {
+    bcm_gated_rec_args a = gated_rec_args("gated_rec_bwd", x, r, i, lam, h0, cu_seqlens, decay_scale);
+    if (dy.has_value()) {
+        check_rows("gated_rec_bwd", *dy, "dy", x);
+        a.dy = dy->data_ptr();
+        a.dy_stride_b = a.cu_seqlens ? 0 : dy->stride(0);
+        a.dy_stride_t = dy->stride(a.cu_seqlens ? 0 : 1);
+    }
+    if (dh_last.has_value()) a.dh_last = fp32_ptr("gated_rec_bwd", *dh_last, "dh_last", x, {a.batch, a.dim});
+    TORCH_CHECK(ckpt.is_cuda() && ckpt.device() == x.device() && ckpt.is_contiguous(),
+                "gated_rec_bwd: ckpt must be the buffer gated_rec_fwd returned for these inputs");
+    c10::cuda::CUDAGuard guard(x.device());
+    auto dx = torch::empty(x.sizes(), x.options());
+    auto dr = torch::empty(x.sizes(), x.options());
+    auto di = torch::empty(x.sizes(), x.options());
+    auto dlam = torch::empty_like(lam);
+    auto dh0 = torch::empty({a.batch, a.dim}, lam.options());
+    a.dx = dx.data_ptr();
+    a.dr = dr.data_ptr();
+    a.di = di.data_ptr();
+    a.dlam = dlam.data_ptr<float>();
+    a.dh0 = dh0.data_ptr<float>();
+    a.ckpt = ckpt.data_ptr();
+    a.ckpt_bytes = ckpt.nbytes();
+    Tensor ws = workspace((int64_t)bcm_gated_rec_bwd_workspace_bytes(&a), x.device());
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = (size_t)ws.numel();
+    check_status(bcm_gated_rec_bwd(&a, cur_stream()), "gated_rec_bwd");
+    return {dx, dr, di, dlam, dh0};
+}
+
+Tensor gated_rec_step(const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& lam, const Tensor& h,
+                      double decay_scale) {
+    const char* what = "gated_rec_step";
+    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.size(1) >= 1, what, ": x must be a CUDA tensor (B, D)");
+    const bcm_dtype dt = float_dtype(x, "x");
+    check_rows(what, x, "x", x);
+    check_rows(what, r, "r", x);
+    check_rows(what, i, "i", x);
+    fp32_ptr(what, lam, "lam", x, {x.size(1)});
+    fp32_ptr(what, h, "h", x, {x.size(0), x.size(1)});
+    c10::cuda::CUDAGuard guard(x.device());
+    auto y = torch::empty(x.sizes(), x.options());
+    check_status(bcm_gated_rec_step(x.data_ptr(), x.stride(0), r.data_ptr(), r.stride(0), i.data_ptr(), i.stride(0), dt,
+                                    x.size(0), x.size(1), lam.data_ptr<float>(), (float)decay_scale, h.data_ptr<float>(),
+                                    y.data_ptr(), cur_stream()),
+                 what);
+    return y;
+}
+
+bcm_distill_args distill_args(const char* what, const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_ids,
+                              const optional<Tensor>& weight, double temperature) {
+    TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, what, ": logits must be a CUDA tensor (T, V)");
+    bcm_distill_args a{};
+    a.dtype = float_dtype(logits, "logits");
+    TORCH_CHECK(logits.size(1) >= 1 && (logits.size(1) == 1 || logits.stride(1) == 1), what,
+                ": logits must have unit stride in their last dimension");
+    TORCH_CHECK(teacher_logits.is_cuda() && teacher_logits.device() == logits.device() && teacher_logits.dim() == 2 &&
+                    teacher_logits.size(0) == logits.size(0) && teacher_logits.is_contiguous(),
+                what, ": teacher_logits must be a contiguous (T, K) tensor on the device of the logits");
+    a.teacher_dtype = float_dtype(teacher_logits, "teacher_logits");
+    const bool wide = teacher_ids.scalar_type() == at::ScalarType::Long;
+    TORCH_CHECK(wide || teacher_ids.scalar_type() == at::ScalarType::Int, what, ": teacher_ids must be int32 or int64");
+    TORCH_CHECK(teacher_ids.is_cuda() && teacher_ids.device() == logits.device() &&
+                    teacher_ids.sizes() == teacher_logits.sizes() && teacher_ids.is_contiguous(),
+                what, ": teacher_ids must be contiguous, of the shape of teacher_logits, on the device of the logits");
+    a.rows = logits.size(0);
+    a.vocab = logits.size(1);
+    a.k = teacher_logits.size(1);
+    a.ids_are_int64 = wide ? 1 : 0;
+    a.temperature = (float)temperature;
+    a.logits = logits.data_ptr();
+    a.logits_stride = logits.stride(0);
+    a.teacher_logits = teacher_logits.data_ptr();
+    a.teacher_ids = teacher_ids.data_ptr();
+    a.weight = weight.has_value() ? fp32_ptr(what, *weight, "weight", logits, {a.rows}) : nullptr;
+    return a;
+}
+
+// -> [loss, stats], with grad also [dlogits] for an upstream gradient of one
+std::vector<Tensor> distill_fwd(const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_ids,
+                                const optional<Tensor>& weight, double temperature, bool grad) {
+    bcm_distill_args a = distill_args("distill_fwd", logits, teacher_logits, teacher_ids, weight, temperature);
+    c10::cuda::CUDAGuard guard(logits.device());
+    auto opt = logits.options().dtype(at::ScalarType::Float);
+    auto loss = torch::empty({a.rows}, opt), stats = torch::empty({a.rows, 2}, opt);
+    a.loss = loss.data_ptr<float>();
+    a.stats = stats.data_ptr<float>();
+    if (!grad) {
+        check_status(bcm_distill_fwd(&a, cur_stream()), "distill_fwd");
+        return {loss, stats};
+    }
+    auto dlogits = torch::empty({a.rows, a.vocab}, logits.options());
+    a.dlogits = dlogits.data_ptr();
+    check_status(bcm_distill_fwd_grad(&a, cur_stream()), "distill_fwd_grad");
+    return {loss, stats, dlogits};
+}
+
+Tensor distill_bwd(const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_ids,
+                   const optional<Tensor>& weight, double temperature, const Tensor& loss, const Tensor& stats,
+                   const Tensor& dloss) {
+    const char* what = "distill_bwd";
+    bcm_distill_args a = distill_args(what, logits, teacher_logits, teacher_ids, weight, temperature);
+    fp32_ptr(what, loss, "loss", logits, {a.rows});
+    fp32_ptr(what, stats, "stats", logits, {a.rows, 2});
+    a.loss = loss.data_ptr<float>();
+    a.stats = stats.data_ptr<float>();
+    a.dloss = fp32_ptr(what, dloss, "dloss", logits, {a.rows});
+    c10::cuda::CUDAGuard guard(logits.device());
+    auto dlogits = torch::empty({a.rows, a.vocab}, logits.options());
+    a.dlogits = dlogits.data_ptr();
+    check_status(bcm_distill_bwd(&a, cur_stream()), what);
+    return dlogits;
+}
+
+// each setting: the value of every row, and a tensor of one per row that takes its place
+std::vector<Tensor> sample_tokens(const Tensor& logits, const Tensor& u, double temperature, int64_t top_k, double top_p,
+                                  double min_p, const optional<Tensor>& temperatures, const optional<Tensor>& top_ks,
+                                  const optional<Tensor>& top_ps, const optional<Tensor>& min_ps) {
+    const char* what = "sample_tokens";
+    TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, what, ": logits must be a CUDA tensor (B, V)");
+    bcm_sample_args a{};
+    a.dtype = float_dtype(logits, "logits");
+    TORCH_CHECK(logits.size(1) >= 1 && (logits.size(1) == 1 || logits.stride(1) == 1), what,
+                ": logits must have unit stride in their last dimension");
+    const int64_t B = logits.size(0);
+    a.batch = B;
+    a.vocab = logits.size(1);
+    a.logits = logits.data_ptr();
+    a.logits_stride = logits.stride(0);
+    a.u = fp32_ptr(what, u, "u", logits, {B});
+    a.temperature_all = (float)temperature;
+    a.top_k_all = (int32_t)std::min<int64_t>(std::max<int64_t>(top_k, 0), INT32_MAX);
+    a.top_p_all = (float)top_p;
+    a.min_p_all = (float)min_p;
+    if (temperatures.has_value()) a.temperature = fp32_ptr(what, *temperatures, "temperature", logits, {B});
+    if (top_ps.has_value()) a.top_p = fp32_ptr(what, *top_ps, "top_p", logits, {B});
+    if (min_ps.has_value()) a.min_p = fp32_ptr(what, *min_ps, "min_p", logits, {B});
+    if (top_ks.has_value()) {
+        TORCH_CHECK(top_ks->is_cuda() && top_ks->device() == logits.device() &&
+                        top_ks->scalar_type() == at::ScalarType::Int && top_ks->is_contiguous() && top_ks->dim() == 1 &&
+                        top_ks->size(0) == B,
+                    what, ": top_k must be a contiguous int32 tensor (B) on the device of the logits");
+        a.top_k = top_ks->data_ptr<int32_t>();
+    }
+    c10::cuda::CUDAGuard guard(logits.device());
+    auto tokens = torch::empty({B}, logits.options().dtype(at::ScalarType::Long));
+    auto logprob = torch::empty({B}, u.options());
+    a.tokens = tokens.data_ptr<int64_t>();
+    a.logprob = logprob.data_ptr<float>();
+    check_status(bcm_sample_tokens(&a, cur_stream()), what);
+    return {tokens, logprob};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1363,4 +1603,27 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("event_params_bwd", &event_params_bwd, py::arg("A"), py::arg("a0"), py::arg("a1"), py::arg("dA"),
           py::arg("dW_B"), py::arg("dW_C"), py::arg("ddt_idle"), py::arg("ddt_active"),
           "backward of event_params_fwd (None gradients are zero) -> [dA_log, dW_BC, da0, da1]");
+    // language-model operators (no reference bindings)
+    m.def("gated_rec_fwd", &gated_rec_fwd, py::arg("x"), py::arg("r"), py::arg("i"), py::arg("lam"),
+          py::arg("h0") = py::none(), py::arg("cu_seqlens") = py::none(), py::arg("decay_scale") = 8.0,
+          py::arg("keep_ckpt") = false,
+          "Gated linear recurrence over (B, L, D), or packed (T, D) with cu_seqlens -> [y, h_last], with keep_ckpt also "
+          "the buffer gated_rec_bwd reads");
+    m.def("gated_rec_bwd", &gated_rec_bwd, py::arg("x"), py::arg("r"), py::arg("i"), py::arg("lam"), py::arg("h0"),
+          py::arg("cu_seqlens"), py::arg("decay_scale"), py::arg("ckpt"), py::arg("dy"), py::arg("dh_last"),
+          "Backward of gated_rec_fwd (dy or dh_last None: zero) -> [dx, dr, di, dlam, dh0]");
+    m.def("gated_rec_step", &gated_rec_step, py::arg("x"), py::arg("r"), py::arg("i"), py::arg("lam"), py::arg("h"),
+          py::arg("decay_scale") = 8.0, "One token of every sequence; the state h (B, D) is updated in place -> y (B, D)");
+    m.def("distill_fwd", &distill_fwd, py::arg("logits"), py::arg("teacher_logits"), py::arg("teacher_ids"),
+          py::arg("weight") = py::none(), py::arg("temperature") = 1.0, py::arg("grad") = false,
+          "Distillation loss on a teacher's top logits -> [loss (T), stats (T, 2)], with grad also dlogits (T, V) for an "
+          "upstream gradient of one");
+    m.def("distill_bwd", &distill_bwd, py::arg("logits"), py::arg("teacher_logits"), py::arg("teacher_ids"),
+          py::arg("weight"), py::arg("temperature"), py::arg("loss"), py::arg("stats"), py::arg("dloss"),
+          "Backward of distill_fwd -> dlogits (T, V)");
+    m.def("sample_tokens", &sample_tokens, py::arg("logits"), py::arg("u"), py::arg("temperature") = 1.0,
+          py::arg("top_k") = 0, py::arg("top_p") = 1.0, py::arg("min_p") = 0.0, py::arg("temperatures") = py::none(),
+          py::arg("top_ks") = py::none(), py::arg("top_ps") = py::none(), py::arg("min_ps") = py::none(),
+          "One token per row from given uniforms -> [tokens (B) int64, logprob (B)]; a tensor of one setting per row takes "
+          "the place of the number");
 }

@@ -9,6 +9,11 @@ reference's Python layer so callers switch without edits:
 * ``EventParamsFn`` / ``event_params``          (the parameter transforms of
   Mamba.forward, spike_mamba/e_model.py:210-230, 463, 475-476, in one kernel)
 
+and, without a counterpart there, operators of language models: the gated
+linear recurrence (``gated_recurrence``, ``gated_recurrence_step``), the
+distillation loss on a teacher's top logits (``distill_topk``,
+``distill_topk_with_grad``) and token sampling (``sample_tokens``).
+
 All device work goes through the native shim (``bc_mamba_b200._native``);
 there is no Python or CPU fallback.  ``install_shim()`` puts the drop-in
 modules ``selective_scan_cuda``, ``extract_events_cuda`` and
@@ -409,3 +414,139 @@ class EventDecoder:
                                             dt_idle.contiguous(), dt_active.contiguous(), A, W_B.contiguous(),
                                             W_C.contiguous(), D, self.eta, self.counters, self.held,
                                             self.conv_state, conv_weight, conv_bias)
+
+
+# ------------------------------------------------ language-model operators ----
+# (no counterpart in the reference: a sequence mixer, a training loss and a
+# token sampler for models built on this package's scans)
+
+
+def _unit(t):
+    """t, copied only where its last dimension is strided."""
+    return t if t is None or t.size(-1) <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _flat(t):
+    return None if t is None else t.contiguous()
+
+
+class GatedRecurrenceFn(torch.autograd.Function):
+    """Gated linear recurrence; see gated_recurrence."""
+
+    @staticmethod
+    def forward(ctx, x, r, i, lam, h0, cu_seqlens, decay_scale):
+        x, r, i, lam, h0, cu_seqlens = _unit(x), _unit(r), _unit(i), _flat(lam), _flat(h0), _flat(cu_seqlens)
+        keep = any(ctx.needs_input_grad[:5])
+        with cuda_stage("gated_recurrence_forward"):
+            res = load_ops().gated_rec_fwd(x, r, i, lam, h0, cu_seqlens, decay_scale, keep)
+        if keep:
+            ctx.save_for_backward(x, r, i, lam, h0, cu_seqlens, res[2])
+            ctx.decay_scale = decay_scale
+        ctx.set_materialize_grads(False)   # an output without a gradient reaches the kernel as NULL
+        return res[0], res[1]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh_last):
+        if dy is None and dh_last is None:
+            return (None,) * 7
+        x, r, i, lam, h0, cu_seqlens, ckpt = ctx.saved_tensors
+        with cuda_stage("gated_recurrence_backward"):
+            dx, dr, di, dlam, dh0 = load_ops().gated_rec_bwd(x, r, i, lam, h0, cu_seqlens, ctx.decay_scale, ckpt,
+                                                             _unit(dy), _flat(dh_last))
+        return dx, dr, di, dlam, dh0 if h0 is not None else None, None, None
+
+
+def gated_recurrence(x, r, i, lam, h0=None, cu_seqlens=None, decay_scale: float = 8.0):
+    """h_t = a_t h_(t-1) + sqrt(1 - a_t^2) sigmoid(i_t) x_t with the decay
+    a_t = exp(-decay_scale softplus(lam) sigmoid(r_t)), per feature.
+
+    x (values), r (decay gate) and i (input gate) are (B, L, D), or packed
+    (T, D) with cu_seqlens (n + 1,) int32, ascending from 0 to T (sequences may
+    be empty); float32, float16 or bfloat16, any batch and position strides.
+    lam (D,) and the entering states h0 (B, D) (None: zeros) are float32.
+    Returns (y, h_last): y = h in x's dtype, and the float32 states after each
+    sequence's last token, which continue it as h0 of a next call or as the
+    state of gated_recurrence_step.  Differentiable in x, r, i, lam and h0; the
+    state is float32 throughout and gradients are the same from run to run."""
+    return GatedRecurrenceFn.apply(x, r, i, lam, h0, cu_seqlens, float(decay_scale))
+
+
+def gated_recurrence_step(x, r, i, lam, h, decay_scale: float = 8.0):
+    """One token of gated_recurrence for every sequence: x, r, i (B, D), the
+    state h (B, D) float32 contiguous, updated in place.  Returns y (B, D)."""
+    return load_ops().gated_rec_step(_unit(x), _unit(r), _unit(i), lam.contiguous(), h, float(decay_scale))
+
+
+class DistillTopkFn(torch.autograd.Function):
+    """Distillation loss on a teacher's top logits; see distill_topk."""
+
+    @staticmethod
+    def forward(ctx, logits, teacher_logits, teacher_ids, weight, temperature):
+        logits, teacher_logits, teacher_ids, weight = _unit(logits), _flat(teacher_logits), _flat(teacher_ids), _flat(weight)
+        with cuda_stage("distill_forward"):
+            loss, stats = load_ops().distill_fwd(logits, teacher_logits, teacher_ids, weight, temperature)
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(logits, teacher_logits, teacher_ids, weight, loss, stats)
+            ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        logits, teacher_logits, teacher_ids, weight, loss, stats = ctx.saved_tensors
+        with cuda_stage("distill_backward"):
+            dz = load_ops().distill_bwd(logits, teacher_logits, teacher_ids, weight, ctx.temperature, loss, stats,
+                                        dloss.contiguous())
+        return dz, None, None, None, None
+
+
+def distill_topk(logits, teacher_logits, teacher_ids, weight=None, temperature: float = 1.0):
+    """Per-row loss weight tau^2 KL(teacher || student), tau the temperature:
+    the teacher's softmax over its K top logits (T, K) with token ids (T, K)
+    (int32 or int64; K up to 1024) against the student's softmax over the whole
+    vocabulary, logits (T, V) in float32, float16 or bfloat16.  Entries whose
+    id lies outside [0, V) or whose logit is -inf are absent (lists may end
+    early); a row without entries, or of weight 0, has loss and gradient 0
+    whatever its logits hold.  weight (T,) float32.  Differentiable in logits.
+    Returns the losses (T,) float32."""
+    return DistillTopkFn.apply(logits, teacher_logits, teacher_ids, weight, float(temperature))
+
+
+def distill_topk_with_grad(logits, teacher_logits, teacher_ids, weight=None, temperature: float = 1.0):
+    """distill_topk and its gradient in one call: (loss (T,), dlogits (T, V)),
+    dlogits for an upstream gradient of one per row (put a mean's 1/T, or a loss
+    scale, into weight).  It reads the logits from memory once where the
+    autograd pair reads them twice."""
+    with torch.no_grad(), cuda_stage("distill_forward"):
+        loss, _, dz = load_ops().distill_fwd(_unit(logits.detach()), _flat(teacher_logits.detach()), _flat(teacher_ids),
+                                             _flat(weight), float(temperature), True)
+    return loss, dz
+
+
+def _per_row(value, off, dtype):
+    """A setting as (number of every row, tensor of one per row or None)."""
+    if not isinstance(value, torch.Tensor):
+        return (off if value is None else value), None
+    if dtype == torch.int32 and value.dtype != dtype:
+        value = value.clamp(0, 2 ** 31 - 1)
+    return off, value.to(dtype).contiguous()
+
+
+def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One token per row of logits (B, V) from given uniform numbers u (B,) in
+    [0, 1), with temperature, top-k, top-p and min-p, each a number or a tensor
+    of one per row.  Filters apply in that order: top-p to the mass that top-k
+    leaves, min-p relative to the most likely token.  temperature <= 0 is greedy,
+    top_k <= 0, top_p >= 1 and min_p <= 0 are off; ties go to the lowest index.
+    Probabilities are summed as integers, so the token depends on logits, u and
+    the settings alone.  Returns (tokens (B,) int64, log-probabilities among the
+    kept tokens (B,) float32); a row whose logits are all -inf or NaN gives token
+    -1 and log-probability -inf."""
+    t, ts = _per_row(temperature, 1.0, torch.float32)
+    k, ks = _per_row(top_k, 0, torch.int32)
+    p, ps = _per_row(top_p, 1.0, torch.float32)
+    m, ms = _per_row(min_p, 0.0, torch.float32)
+    with torch.no_grad(), cuda_stage("sample_tokens"):
+        tokens, logprob = load_ops().sample_tokens(_unit(logits.detach()), u.contiguous(), t, k, p, m, ts, ks, ps, ms)
+    return tokens, logprob

@@ -574,6 +574,131 @@ BCM_API bcm_status bcm_event_params_bwd(const float* A, const float* a0, const f
                                         int64_t dstate, float* dA_log, float* dW_BC, float* da0,
                                         float* da1, cudaStream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Gated linear recurrence.  No reference binding: a sequence mixer beside the
+ * event scan and the dense S6 scan.  Per feature d, c = decay_scale,
+ * s = softplus(lam[d]) (identity above 20):
+ *   u_t = -c s sigmoid(r_t),  a_t = exp(u_t),  m_t = sqrt(1 - a_t^2),
+ *   h_t = a_t h_{t-1} + m_t sigmoid(i_t) x_t,  y_t = h_t,
+ * h_0 from h0 (NULL: zeros), the state after the last token to h_last.
+ * Dense: batch sequences of seqlen tokens; x, r, i, dy with strides of b and t
+ * and unit stride of d.  Packed (cu_seqlens [batch + 1] int32 on the device,
+ * ascending from 0 to seqlen): batch sequences, some of them possibly empty,
+ * in seqlen tokens; the b strides are not used.  Offsets that are not ascending
+ * or leave [0, seqlen] give undefined values, no access out of range.
+ * x, r, i, y, dy and the gradients dx, dr, di in dtype; y, dx, dr, di
+ * contiguous; lam, dlam [dim], h0, h_last, dh_last, dh0 [batch, dim] fp32,
+ * contiguous.  The state is fp32 throughout.
+ * ckpt (bcm_gated_rec_ckpt_bytes): what the backward needs of the forward's
+ * states; NULL in a forward without a backward.  Backward: dy or dh_last NULL
+ * is a zero gradient, dh0 may be NULL; every output is written, not
+ * accumulated, and sums run in a fixed order.  Where m_t = 0, the term with
+ * 1 / m_t of the gradient is 0.
+ * ------------------------------------------------------------------------- */
+typedef struct bcm_gated_rec_args {
+    int64_t batch, seqlen, dim;
+    const int32_t* cu_seqlens;
+    bcm_dtype dtype;
+    float decay_scale;
+    const void* x; int64_t x_stride_b, x_stride_t;
+    const void* r; int64_t r_stride_b, r_stride_t;
+    const void* i; int64_t i_stride_b, i_stride_t;
+    const float* lam;
+    const float* h0;
+    /* forward outputs */
+    void* y; float* h_last;
+    void* ckpt; size_t ckpt_bytes;      /* written by the forward, read by the backward */
+    /* backward */
+    const void* dy; int64_t dy_stride_b, dy_stride_t;
+    const float* dh_last;
+    void* dx; void* dr; void* di; float* dlam; float* dh0;
+    void* workspace; size_t workspace_bytes;
+} bcm_gated_rec_args;
+
+BCM_API size_t bcm_gated_rec_ckpt_bytes(const bcm_gated_rec_args* args);
+BCM_API size_t bcm_gated_rec_bwd_workspace_bytes(const bcm_gated_rec_args* args);
+BCM_API bcm_status bcm_gated_rec_fwd(const bcm_gated_rec_args* args, cudaStream_t stream);
+BCM_API bcm_status bcm_gated_rec_bwd(const bcm_gated_rec_args* args, cudaStream_t stream);
+
+/* One token of every sequence: x, r, i [batch, dim] (unit stride of d), the
+ * state h [batch, dim] fp32 updated in place, y [batch, dim] contiguous. */
+BCM_API bcm_status bcm_gated_rec_step(const void* x, int64_t x_stride_b, const void* r, int64_t r_stride_b,
+                                      const void* i, int64_t i_stride_b, bcm_dtype dtype, int64_t batch,
+                                      int64_t dim, const float* lam, float decay_scale, float* h, void* y,
+                                      cudaStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Distillation from a teacher's top logits.  No reference binding.
+ * Row t of the student's logits z [rows, vocab] (dtype, row stride, unit
+ * stride of v), the teacher's k logits q [rows, k] (teacher_dtype) with token
+ * ids [rows, k] (int32, or int64 with ids_are_int64), w = weight[t] (NULL: 1),
+ * tau the temperature:
+ *   p = softmax(q / tau) over the entries whose id lies in [0, vocab) and
+ *       whose logit is not -inf,   s = softmax(z / tau),
+ *   loss[t] = w tau^2 sum_j p_j (ln p_j - ln s_{id_j})      (p_j = 0: no term),
+ *   dlogits[t, v] = dloss[t] w tau (s_v - sum over {j: id_j = v} of p_j).
+ * A row without such entries, or with w = 0, has loss 0 and gradient 0 even
+ * where its logits are NaN.  An id that occurs twice adds up.
+ * loss [rows] fp32; stats [rows, 2] fp32 carries (max, sum of exp) of z / tau
+ * from the forward to the backward; dlogits [rows, vocab] contiguous, must not
+ * overlap the logits.  fwd_grad is forward and backward in one call (dloss
+ * NULL: 1).
+ * ------------------------------------------------------------------------- */
+#define BCM_DISTILL_MAX_K 1024
+
+typedef struct bcm_distill_args {
+    int64_t rows, vocab, k;
+    bcm_dtype dtype, teacher_dtype;
+    int ids_are_int64;
+    float temperature;
+    const void* logits; int64_t logits_stride;
+    const void* teacher_logits; const void* teacher_ids;   /* contiguous */
+    const float* weight;
+    float* loss; float* stats;
+    const float* dloss;
+    void* dlogits;
+} bcm_distill_args;
+
+BCM_API bcm_status bcm_distill_fwd(const bcm_distill_args* args, cudaStream_t stream);
+BCM_API bcm_status bcm_distill_bwd(const bcm_distill_args* args, cudaStream_t stream);
+BCM_API bcm_status bcm_distill_fwd_grad(const bcm_distill_args* args, cudaStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * One token per row from given uniform numbers.  No reference binding.
+ * logits [batch, vocab] (dtype, row stride, unit stride of v); u [batch] in
+ * [0, 1) (values outside are clamped, NaN is 0); temperature, top_k, top_p,
+ * min_p [batch], or one value for every row.  T = temperature <= 0, NaN, or so
+ * small that 1/T overflows, is greedy: 1/T taken as 1 and top_k as 1.
+ *   s_v = (logit_v - max logit) (1/T), 0 at the maximum; a NaN logit counts as
+ *   -inf, and s = -inf is never taken;  e_v = exp(s_v);  w_v = floor(e_v 2^40).
+ * In descending order of s, equal s in ascending order of index:
+ *   top_k keeps the first k (k <= 0: all); top_p keeps of these the tokens
+ *   whose preceding weight is below ceil(p * total weight), the first always
+ *   (p >= 1 or NaN: all); min_p keeps of these those with e_v >= min(min_p, 1)
+ *   (<= 0 or NaN: all).
+ * tokens[b] (int64) is the first, in ascending order of index, whose inclusive
+ * kept weight exceeds floor(u * total kept weight); logprob[b] (fp32) its log
+ * probability among the kept.  The weights are integers: sums are exact, and
+ * the token does not depend on their order.  A row whose logits are all -inf
+ * (or NaN) gives token -1 and log probability -inf.
+ * ------------------------------------------------------------------------- */
+#define BCM_SAMPLE_MAX_VOCAB 4194304
+
+typedef struct bcm_sample_args {
+    int64_t batch, vocab;
+    bcm_dtype dtype;
+    const void* logits; int64_t logits_stride;
+    const float* u;
+    /* one value per row, or NULL and the value for every row */
+    const float* temperature; float temperature_all;
+    const int32_t* top_k; int32_t top_k_all;
+    const float* top_p; float top_p_all;
+    const float* min_p; float min_p_all;
+    int64_t* tokens; float* logprob;
+} bcm_sample_args;
+
+BCM_API bcm_status bcm_sample_tokens(const bcm_sample_args* args, cudaStream_t stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

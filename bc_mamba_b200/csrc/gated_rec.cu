@@ -11,6 +11,7 @@
 //   dlam = -c sigmoid(lam) sum_t du_t sigmoid(r_t),  dh0 = a_1 G_1.
 // The second term of du is 0 where m_t = 0 (its limit after the factor u).
 #include <algorithm>
+#include <cstring>
 
 #include "common.cuh"
 
@@ -40,74 +41,542 @@ struct RecPtr {
     int64_t xb, xt, rb, rt, ib, it, gb, gt;
 };
 
-// Rows of sequence b: dense [b*L, (b+1)*L); packed [cu[b], cu[b+1]) within [0, L).
-__device__ __forceinline__ void rows_of(const int32_t* cu, int64_t b, int64_t L, int64_t& t0, int64_t& n) {
-    if (cu == nullptr) {
-        t0 = 0;
-        n = L;
-        return;
+struct RecOut {
+    const float* h0; void* y; float* h_last; float* ckpt;          // forward
+    const float* dh_last; void* dx; void* dr; void* di; float* part; float* dh0;   // backward
+};
+
+// ---- layout of the scan kernels -----------------------------------------------
+// A lane owns VEC neighbouring features of one row, a warp kSteps consecutive
+// tokens, a block kWarps * kSteps = kChunk tokens of a tile of 32 * VEC features.
+// A block's chunks follow one another in a loop that carries the state; P blocks
+// of a cluster take P consecutive chunks per turn, so that few tiles with long
+// sequences still fill the GPU.  Every input is read once: the composition
+// h -> A h + H of a warp's tokens goes to shared memory, the other warps' and
+// blocks' compositions give the state that enters, and the tokens, still in
+// registers, are replayed from it.
+//
+// Mode: kDense, one sequence per block; kGroup, a block takes `per` consecutive
+// dense sequences as one run of tokens (short sequences would leave most of a
+// chunk empty); kPacked, one run of tokens with the sequences' offsets in cu.
+// Where a sequence starts inside a run, nothing passes and its own state enters.
+constexpr int kWarps = 8;
+constexpr int kSteps = 8;
+constexpr int kChunk = kWarps * kSteps;
+constexpr int kMaxCluster = 16;
+constexpr float kCut = -1.0f;   // in place of a product of decays: nothing passes (a sequence starts inside)
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, bool ok, float (&v)[VEC]) {
+    if constexpr (VEC == 1) {
+        v[0] = ok ? to_f32<T>(*p) : 0.0f;
+    } else if constexpr (sizeof(T) == 4) {
+        const float2 w = ok ? __ldg(reinterpret_cast<const float2*>(p)) : make_float2(0.0f, 0.0f);
+        v[0] = w.x;
+        v[1] = w.y;
+    } else {
+        const uint32_t w = ok ? __ldg(reinterpret_cast<const uint32_t*>(p)) : 0u;
+        T e[2];
+        memcpy(e, &w, 4);
+        v[0] = to_f32<T>(e[0]);
+        v[1] = to_f32<T>(e[1]);
     }
-    const int64_t lo = cu[b], hi = cu[b + 1];
-    t0 = lo < 0 ? 0 : (lo > L ? L : lo);
-    const int64_t e = hi < t0 ? t0 : (hi > L ? L : hi);
-    n = e - t0;
 }
 
-template <typename T>
-__global__ void rec_fwd_kernel(RecPtr p, const int32_t* __restrict__ cu, int64_t L, int64_t D, const float* __restrict__ lam,
-                               float c, const float* __restrict__ h0, T* __restrict__ y, float* __restrict__ h_last,
-                               float* __restrict__ hs) {
-    const int64_t d = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int64_t b = blockIdx.y;
-    if (d >= D) return;
-    int64_t t0, n;
-    rows_of(cu, b, L, t0, n);
-    const T* x = static_cast<const T*>(p.x) + (cu ? 0 : b * p.xb) + t0 * p.xt + d;
-    const T* r = static_cast<const T*>(p.r) + (cu ? 0 : b * p.rb) + t0 * p.rt + d;
-    const T* i = static_cast<const T*>(p.i) + (cu ? 0 : b * p.ib) + t0 * p.it + d;
-    const int64_t o = ((cu ? 0 : b * L) + t0) * D + d;
-    const float cs = c * softplus_(lam[d]);
-    float h = h0 ? h0[b * D + d] : 0.0f;
-    for (int64_t t = 0; t < n; ++t) {
-        const Gates g = gates(to_f32<T>(r[t * p.rt]), to_f32<T>(i[t * p.it]), cs);
-        if (hs) hs[o + t * D] = h;
-        h = fmaf(g.a, h, g.m * g.si * to_f32<T>(x[t * p.xt]));
-        y[o + t * D] = from_f32<T>(h);
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
+    if constexpr (VEC == 1) {
+        *p = from_f32<T>(v[0]);
+    } else if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+    } else {
+        const T e[2] = {from_f32<T>(v[0]), from_f32<T>(v[1])};
+        uint32_t w;
+        memcpy(&w, e, 4);
+        *reinterpret_cast<uint32_t*>(p) = w;
     }
-    h_last[b * D + d] = h;
 }
 
-template <typename T>
-__global__ void rec_bwd_kernel(RecPtr p, const int32_t* __restrict__ cu, int64_t L, int64_t D, const float* __restrict__ lam,
-                               float c, const float* __restrict__ hs, const float* __restrict__ dh_last, T* __restrict__ dx,
-                               T* __restrict__ dr, T* __restrict__ di, float* __restrict__ part, float* __restrict__ dh0) {
-    const int64_t d = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int64_t b = blockIdx.y;
-    if (d >= D) return;
-    int64_t t0, n;
-    rows_of(cu, b, L, t0, n);
-    const T* x = static_cast<const T*>(p.x) + (cu ? 0 : b * p.xb) + t0 * p.xt + d;
-    const T* r = static_cast<const T*>(p.r) + (cu ? 0 : b * p.rb) + t0 * p.rt + d;
-    const T* i = static_cast<const T*>(p.i) + (cu ? 0 : b * p.ib) + t0 * p.it + d;
-    const T* dy = p.dy ? static_cast<const T*>(p.dy) + (cu ? 0 : b * p.gb) + t0 * p.gt + d : nullptr;
-    const int64_t o = ((cu ? 0 : b * L) + t0) * D + d;
-    const float cs = c * softplus_(lam[d]);
-    float back = dh_last ? dh_last[b * D + d] : 0.0f, sum = 0.0f;
-    for (int64_t t = n - 1; t >= 0; --t) {
-        const Gates g = gates(to_f32<T>(r[t * p.rt]), to_f32<T>(i[t * p.it]), cs);
-        const float xv = to_f32<T>(x[t * p.xt]);
-        const float G = back + (dy ? to_f32<T>(dy[t * p.gt]) : 0.0f);
-        const float dxv = G * g.m * g.si;
-        dx[o + t * D] = from_f32<T>(dxv);
-        di[o + t * D] = from_f32<T>(dxv * xv * (1.0f - g.si));
-        const float slope = g.m == 0.0f ? 0.0f : g.a * g.a / g.m;
-        const float du = G * (g.a * hs[o + t * D] - slope * g.si * xv);
-        dr[o + t * D] = from_f32<T>(du * g.u * (1.0f - g.sr));
-        sum = fmaf(du, g.sr, sum);
-        back = g.a * G;
+// The sequence that holds token t: the last s with cu[s] <= t, in [0, n).  Called by whole warps; t is uniform.
+__device__ __forceinline__ int seq_of(const int32_t* __restrict__ cu, int n, int t) {
+    int lo = 0, hi = n - 1;                          // the answer lies in [lo, hi]
+    const int lane = threadIdx.x & 31;
+    while (hi > lo) {
+        const int step = (hi - lo + 31) / 32;        // lanes look at lo + step, lo + 2 step, ...
+        const int at = lo + (lane + 1) * step;
+        const unsigned m = __ballot_sync(kFull, at <= hi && cu[at] <= t);
+        const int c = __popc(m);
+        lo += c * step;
+        hi = min(hi, lo + step - 1);
     }
-    if (dh0) dh0[b * D + d] = back;
-    part[b * D + d] = sum;
+    return lo;
+}
+
+enum Mode { kDense, kGroup, kPacked };
+
+// What the kernels know of the sizes: a run holds L tokens (kGroup: its last may hold fewer), a sequence Ls (kDense,
+// kGroup), per sequences make a run (kGroup); n sequences, D features, P blocks in a cluster.
+struct RecDim {
+    const int32_t* cu;
+    int64_t n;
+    int L, Ls, per, D, P;
+};
+
+// The sequence around a token of the run, moved along by a warp: its index s, its first token and its end.
+template <int MODE>
+struct Seq {
+    const int32_t* cu;
+    int n, Ls;
+    int64_t s0, s;
+    int beg, end;
+    __device__ __forceinline__ void at(int t) {
+        if (MODE == kPacked) {
+            const int k = seq_of(cu, n, t);
+            s = k;
+            beg = cu[k];
+            end = cu[k + 1];
+        } else if (MODE == kGroup) {
+            const int k = t / Ls;
+            s = s0 + k;
+            beg = k * Ls;
+            end = beg + Ls;
+        }
+    }
+};
+
+// (A1, H1) followed by (A2, H2)
+template <bool CUTS>
+__device__ __forceinline__ void then(float& A1, float& H1, float A2, float H2) {
+    if (CUTS && A2 < 0.0f) {
+        A1 = kCut;
+        H1 = H2;
+    } else {
+        H1 = fmaf(A2, H1, H2);
+        A1 = CUTS && A1 < 0.0f ? kCut : A1 * A2;
+    }
+}
+
+template <bool CUTS>
+__device__ __forceinline__ float apply(float A, float H, float h) {
+    return CUTS && A < 0.0f ? H : fmaf(A, h, H);
+}
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void st_cluster(uint32_t addr, int rank, float2 v) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(remote), "f"(v.x), "f"(v.y) : "memory");
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <typename T, int VEC, int MODE, bool CLUSTER>
+__global__ void __launch_bounds__(kWarps * 32)
+rec_fwd_kernel(RecPtr p, RecOut o, RecDim n, const float* __restrict__ lam, float c) {
+    constexpr bool CUTS = MODE != kDense;
+    __shared__ float2 ex[2][kWarps][VEC][32];
+    __shared__ float2 pub[CLUSTER ? 2 : 1][CLUSTER ? kMaxCluster : 1][VEC][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int D = n.D, P = n.P, tiles = (D + 32 * VEC - 1) / (32 * VEC);
+    const int rank = CLUSTER ? blockIdx.x % P : 0;
+    const int64_t run_id = blockIdx.x / (CLUSTER ? P : 1) / tiles;
+    const int tile = blockIdx.x / (CLUSTER ? P : 1) - (int)run_id * tiles;
+    // the run's first sequence and its tokens
+    const int64_t b = MODE == kGroup ? run_id * n.per : run_id;
+    const int L = MODE == kGroup ? (int)min((int64_t)n.per, n.n - b) * n.Ls : n.L;
+    const int d = (tile * 32 + lane) * VEC;
+    const bool mine = d < D;
+    const int dd = mine ? d : 0;
+    const T* x = static_cast<const T*>(p.x) + (MODE == kPacked ? 0 : b * p.xb) + dd;
+    const T* r = static_cast<const T*>(p.r) + (MODE == kPacked ? 0 : b * p.rb) + dd;
+    const T* i = static_cast<const T*>(p.i) + (MODE == kPacked ? 0 : b * p.ib) + dd;
+    T* y = static_cast<T*>(o.y) + (MODE == kPacked ? 0 : b * n.Ls * D) + dd;
+    const int chunks = (n.L + kChunk - 1) / kChunk, turns = (chunks + P - 1) / P;   // (of a full run)
+    float* ck = o.ckpt ? o.ckpt + run_id * chunks * D + dd : nullptr;
+    float cs[VEC], run[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        cs[v] = c * softplus_(lam[dd + v]);
+        run[v] = MODE == kDense && o.h0 ? o.h0[b * D + dd + v] : 0.0f;
+    }
+    Seq<MODE> seq{n.cu, (int)n.n, n.Ls, b, 0, 0, 0};
+    if (CLUSTER) cluster_sync();       // every block of the cluster runs before its shared memory is written to
+    for (int turn = 0; turn < turns; ++turn) {
+        const int buf = turn & 1;
+        const int chunk = turn * P + rank;
+        const int t0 = chunk * kChunk + warp * kSteps;
+        float a[kSteps][VEC], e[kSteps][VEC];
+        {
+            float xv[kSteps][VEC], rv[kSteps][VEC], iv[kSteps][VEC];
+            if (MODE == kGroup) seq.at(t0);
+            int64_t sl = seq.s - b;
+            int tl = t0 - seq.beg;
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+                const bool ok = mine && t0 + j < L;
+                const int64_t t = MODE == kGroup ? tl : t0 + j, q = MODE == kGroup ? sl : 0;
+                load_vec<T, VEC>(r + q * p.rb + t * p.rt, ok, rv[j]);
+                load_vec<T, VEC>(i + q * p.ib + t * p.it, ok, iv[j]);
+                load_vec<T, VEC>(x + q * p.xb + t * p.xt, ok, xv[j]);
+                if (MODE == kGroup && ++tl == n.Ls) {
+                    tl = 0;
+                    ++sl;
+                }
+            }
+            if (MODE == kPacked && t0 < L) seq.at(t0);
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    const Gates g = gates(rv[j][v], iv[j][v], cs[v]);
+                    const bool ok = t0 + j < L;
+                    a[j][v] = ok ? g.a : 1.0f;
+                    e[j][v] = ok ? g.m * g.si * xv[j][v] : 0.0f;
+                }
+        }
+        unsigned starts = 0;      // bit j: a sequence starts at token t0 + j (its entering state goes into e)
+        if (CUTS && t0 < L && (seq.beg == t0 || seq.end < t0 + kSteps)) {
+            Seq<MODE> q = seq;
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+                const int t = t0 + j;
+                if (t < L && t == q.end) q.at(t);
+                if (t < L && t == q.beg) {
+                    starts |= 1u << j;
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v)
+                        e[j][v] = fmaf(a[j][v], o.h0 ? o.h0[q.s * D + dd + v] : 0.0f, e[j][v]);
+                }
+            }
+        }
+        float A[VEC], H[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            A[v] = 1.0f;
+            H[v] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            const bool cut = CUTS && (starts >> j & 1u);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) then<CUTS>(A[v], H[v], cut ? kCut : a[j][v], e[j][v]);
+        }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) ex[buf][warp][v][lane] = make_float2(A[v], H[v]);
+        __syncthreads();
+        float preA[VEC], preH[VEC], totA[VEC], totH[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            totA[v] = 1.0f;
+            totH[v] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) {
+                if (k == warp) {
+                    preA[v] = totA[v];
+                    preH[v] = totH[v];
+                }
+                const float2 f = ex[buf][k][v][lane];
+                then<CUTS>(totA[v], totH[v], f.x, f.y);
+            }
+        }
+        float h[VEC];
+        if (CLUSTER) {
+            for (int k = warp; k < P; k += kWarps)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) st_cluster(smem_addr(&pub[buf][rank][v][lane]), k, make_float2(totA[v], totH[v]));
+            cluster_sync();
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                for (int k = 0; k < P; ++k) {
+                    if (k == rank) h[v] = run[v];
+                    const float2 f = pub[buf][k][v][lane];
+                    run[v] = apply<CUTS>(f.x, f.y, run[v]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                h[v] = run[v];
+                run[v] = apply<CUTS>(totA[v], totH[v], run[v]);
+            }
+        }
+        if (ck && warp == 0 && mine && chunk < chunks)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) ck[(int64_t)chunk * D + v] = h[v];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) h[v] = apply<CUTS>(preA[v], preH[v], h[v]);
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            const int t = t0 + j;
+            const bool cut = CUTS && (starts >> j & 1u);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) h[v] = cut ? e[j][v] : fmaf(a[j][v], h[v], e[j][v]);
+            if (mine && t < L) store_vec<T, VEC>(y + (int64_t)t * D, h);
+            if (CUTS && t < L) {
+                if (t == seq.end) seq.at(t);
+                if (t == seq.end - 1 && mine)
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) o.h_last[seq.s * D + d + v] = h[v];
+            }
+        }
+    }
+    if (rank != 0 || !mine) return;
+    if (MODE == kDense) {
+        if (warp == 0)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) o.h_last[b * D + d + v] = run[v];
+    } else if (MODE == kPacked) {
+        for (int64_t s = warp; s < n.n; s += kWarps)       // empty sequences keep their state
+            if (n.cu[s] >= n.cu[s + 1])
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) o.h_last[s * D + d + v] = o.h0 ? o.h0[s * D + d + v] : 0.0f;
+    }
+}
+
+// Chunks from the last to the first.  The states that enter a chunk come from
+// the forward; back_t = a_t G_t passes from right to left by the same products
+// of decays, back -> A back + K.
+template <typename T, int VEC, int MODE, bool CLUSTER>
+__global__ void __launch_bounds__(kWarps * 32)
+rec_bwd_kernel(RecPtr p, RecOut o, RecDim n, const float* __restrict__ lam, float c) {
+    constexpr bool CUTS = MODE != kDense;
+    __shared__ float ex[2][kWarps][3][VEC][32];
+    __shared__ float2 pub[CLUSTER ? 2 : 1][CLUSTER ? kMaxCluster : 1][VEC][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int D = n.D, P = n.P, tiles = (D + 32 * VEC - 1) / (32 * VEC);
+    const int rank = CLUSTER ? blockIdx.x % P : 0;
+    const int64_t run_id = blockIdx.x / (CLUSTER ? P : 1) / tiles;
+    const int tile = blockIdx.x / (CLUSTER ? P : 1) - (int)run_id * tiles;
+    // the run's first sequence and its tokens
+    const int64_t b = MODE == kGroup ? run_id * n.per : run_id;
+    const int L = MODE == kGroup ? (int)min((int64_t)n.per, n.n - b) * n.Ls : n.L;
+    const int d = (tile * 32 + lane) * VEC;
+    const bool mine = d < D;
+    const int dd = mine ? d : 0;
+    const T* x = static_cast<const T*>(p.x) + (MODE == kPacked ? 0 : b * p.xb) + dd;
+    const T* r = static_cast<const T*>(p.r) + (MODE == kPacked ? 0 : b * p.rb) + dd;
+    const T* i = static_cast<const T*>(p.i) + (MODE == kPacked ? 0 : b * p.ib) + dd;
+    const T* dy = static_cast<const T*>(p.dy) + (MODE == kPacked ? 0 : b * p.gb) + dd;
+    const bool has_dy = p.dy != nullptr;
+    const int64_t base = (MODE == kPacked ? 0 : b * n.Ls * D) + dd;
+    T* dx = static_cast<T*>(o.dx) + base;
+    T* dr = static_cast<T*>(o.dr) + base;
+    T* di = static_cast<T*>(o.di) + base;
+    const int chunks = (n.L + kChunk - 1) / kChunk, turns = (chunks + P - 1) / P;   // (of a full run)
+    const float* ck = o.ckpt + run_id * chunks * D + dd;
+    Seq<MODE> seq{n.cu, (int)n.n, n.Ls, b, 0, 0, 0};
+    float cs[VEC], run[VEC], sum[VEC];
+    if (CUTS) seq.at(L - 1);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        cs[v] = c * softplus_(lam[dd + v]);
+        run[v] = o.dh_last ? o.dh_last[(CUTS ? seq.s : b) * D + dd + v] : 0.0f;
+        sum[v] = 0.0f;
+    }
+    if (CLUSTER) cluster_sync();
+    for (int turn = turns - 1; turn >= 0; --turn) {
+        const int buf = turn & 1;
+        const int chunk = turn * P + rank;
+        const int t0 = chunk * kChunk + warp * kSteps;
+        float xv[kSteps][VEC], gv[kSteps][VEC], sr[kSteps][VEC], si[kSteps][VEC], a[kSteps][VEC], m[kSteps][VEC], enter[VEC];
+        {
+            float rv[kSteps][VEC], iv[kSteps][VEC];
+            if (MODE == kGroup) seq.at(t0);
+            int64_t sl = seq.s - b;
+            int tl = t0 - seq.beg;
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+                const bool ok = mine && t0 + j < L;
+                const int64_t t = MODE == kGroup ? tl : t0 + j, q = MODE == kGroup ? sl : 0;
+                load_vec<T, VEC>(r + q * p.rb + t * p.rt, ok, rv[j]);
+                load_vec<T, VEC>(i + q * p.ib + t * p.it, ok, iv[j]);
+                load_vec<T, VEC>(x + q * p.xb + t * p.xt, ok, xv[j]);
+                load_vec<T, VEC>(dy + q * p.gb + t * p.gt, ok && has_dy, gv[j]);
+                if (MODE == kGroup && ++tl == n.Ls) {
+                    tl = 0;
+                    ++sl;
+                }
+            }
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) enter[v] = chunk < chunks ? ck[(int64_t)chunk * D + v] : 0.0f;
+            if (MODE == kPacked && t0 < L) seq.at(t0);
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    const Gates g = gates(rv[j][v], iv[j][v], cs[v]);
+                    sr[j][v] = g.sr;
+                    si[j][v] = g.si;
+                    a[j][v] = t0 + j < L ? g.a : 1.0f;
+                    m[j][v] = g.m;
+                }
+        }
+        // forward composition (A, H), backward composition (A, K) of the warp's tokens
+        unsigned starts = 0;
+        if (CUTS && t0 < L && (seq.beg == t0 || seq.end < t0 + kSteps)) {
+            Seq<MODE> q = seq;
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+                const int t = t0 + j;
+                if (t < L && t == q.end) q.at(t);
+                if (t < L && t == q.beg) starts |= 1u << j;
+            }
+        }
+        auto state0 = [&](int t, int v) -> float {          // the state entering the sequence that starts at t
+            Seq<MODE> q = seq;
+            q.at(t);
+            return o.h0 ? o.h0[q.s * D + dd + v] : 0.0f;
+        };
+        auto back0 = [&](int t, int v) -> float {           // what enters, from the right, the sequence that ends at t
+            if (t < 0) return 0.0f;
+            Seq<MODE> q = seq;
+            q.at(t);
+            return o.dh_last ? o.dh_last[q.s * D + dd + v] : 0.0f;
+        };
+        float A[VEC], H[VEC], K[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            A[v] = 1.0f;
+            H[v] = 0.0f;
+            K[v] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            const bool cut = CUTS && (starts >> j & 1u);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const float e = m[j][v] * si[j][v] * xv[j][v];
+                if (cut) {
+                    A[v] = kCut;
+                    H[v] = fmaf(a[j][v], state0(t0 + j, v), e);
+                } else {
+                    then<CUTS>(A[v], H[v], a[j][v], e);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = kSteps - 1; j >= 0; --j) {
+            const bool cut = CUTS && (starts >> j & 1u);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) K[v] = cut ? back0(t0 + j - 1, v) : a[j][v] * (gv[j][v] + K[v]);
+        }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            ex[buf][warp][0][v][lane] = A[v];
+            ex[buf][warp][1][v][lane] = H[v];
+            ex[buf][warp][2][v][lane] = K[v];
+        }
+        __syncthreads();
+        float sufA[VEC], sufK[VEC], totA[VEC], totK[VEC], h[VEC], back[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            totA[v] = 1.0f;
+            totK[v] = 0.0f;
+#pragma unroll
+            for (int k = kWarps - 1; k >= 0; --k) {
+                if (k == warp) {
+                    sufA[v] = totA[v];
+                    sufK[v] = totK[v];
+                }
+                then<CUTS>(totA[v], totK[v], ex[buf][k][0][v][lane], ex[buf][k][2][v][lane]);
+            }
+            h[v] = enter[v];
+            for (int k = 0; k < warp; ++k) h[v] = apply<CUTS>(ex[buf][k][0][v][lane], ex[buf][k][1][v][lane], h[v]);
+        }
+        if (CLUSTER) {
+            for (int k = warp; k < P; k += kWarps)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) st_cluster(smem_addr(&pub[buf][rank][v][lane]), k, make_float2(totA[v], totK[v]));
+            cluster_sync();
+#pragma unroll
+            for (int v = 0; v < VEC; ++v)
+                for (int k = P - 1; k >= 0; --k) {
+                    if (k == rank) back[v] = run[v];
+                    const float2 f = pub[buf][k][v][lane];
+                    run[v] = apply<CUTS>(f.x, f.y, run[v]);
+                }
+        } else {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                back[v] = run[v];
+                run[v] = apply<CUTS>(totA[v], totK[v], run[v]);
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) back[v] = apply<CUTS>(sufA[v], sufK[v], back[v]);
+        float prev[kSteps][VEC];
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            const bool cut = CUTS && (starts >> j & 1u);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                if (cut) h[v] = state0(t0 + j, v);
+                prev[j][v] = h[v];
+                h[v] = fmaf(a[j][v], h[v], m[j][v] * si[j][v] * xv[j][v]);
+            }
+        }
+#pragma unroll
+        for (int j = kSteps - 1; j >= 0; --j) {
+            const int t = t0 + j;
+            const bool ok = mine && t < L;
+            float ox[VEC], orr[VEC], oi[VEC];
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const float G = gv[j][v] + back[v];
+                ox[v] = G * m[j][v] * si[j][v];
+                oi[v] = ox[v] * xv[j][v] * (1.0f - si[j][v]);
+                const float slope = m[j][v] == 0.0f ? 0.0f : a[j][v] * a[j][v] / m[j][v];
+                const float du = G * (a[j][v] * prev[j][v] - slope * si[j][v] * xv[j][v]);
+                orr[v] = du * (-cs[v] * sr[j][v]) * (1.0f - sr[j][v]);
+                if (t < L) {
+                    sum[v] = fmaf(du, sr[j][v], sum[v]);
+                    back[v] = a[j][v] * G;
+                }
+            }
+            if (ok) {
+                store_vec<T, VEC>(dx + (int64_t)t * D, ox);
+                store_vec<T, VEC>(dr + (int64_t)t * D, orr);
+                store_vec<T, VEC>(di + (int64_t)t * D, oi);
+            }
+            if (CUTS && (starts >> j & 1u)) {
+                Seq<MODE> q = seq;
+                q.at(t);
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    if (o.dh0 && mine) o.dh0[q.s * D + d + v] = back[v];
+                    back[v] = back0(t - 1, v);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    float* red = &ex[0][0][0][0][0];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) red[(warp * VEC + v) * 32 + lane] = sum[v];
+    __syncthreads();
+    if (warp == 0 && mine)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            float s = 0.0f;
+            for (int k = 0; k < kWarps; ++k) s += red[(k * VEC + v) * 32 + lane];
+            o.part[(run_id * P + rank) * D + d + v] = s;
+        }
+    if (rank != 0 || !mine || !o.dh0) return;
+    if (MODE == kDense) {
+        if (warp == 0)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) o.dh0[b * D + d + v] = run[v];
+    } else if (MODE == kPacked) {
+        for (int64_t s = warp; s < n.n; s += kWarps)
+            if (n.cu[s] >= n.cu[s + 1])
+#pragma unroll
+                for (int v = 0; v < VEC; ++v)
+                    o.dh0[s * D + d + v] = o.dh_last ? o.dh_last[s * D + d + v] : 0.0f;
+    }
 }
 
 // dlam[d] = -c sigmoid(lam[d]) * sum of the partials of feature d, in order.
@@ -139,8 +608,8 @@ bcm_status rec_validate(const bcm_gated_rec_args* a, const char* what) {
     BCM_REQUIRE(a != nullptr, "%s: null arguments", what);
     BCM_REQUIRE(dtype_ok(a->dtype), "%s: unsupported dtype %d", what, (int)a->dtype);
     BCM_REQUIRE(a->batch >= 0 && a->seqlen >= 0 && a->dim >= 1, "%s: bad sizes", what);
-    BCM_REQUIRE(a->batch < 65536 && a->seqlen < (1ll << 31) && a->dim < (1ll << 31),
-                "%s: batch must be below 65536, seqlen and dim below 2^31", what);
+    BCM_REQUIRE(a->batch < (1ll << 31) && a->seqlen < (1ll << 31) - 4096 && a->dim < (1ll << 30),
+                "%s: batch must be below 2^31, seqlen below 2^31 - 4096, dim below 2^30", what);
     BCM_REQUIRE(a->decay_scale >= 0.0f, "%s: decay_scale must not be negative", what);
     return BCM_OK;
 }
@@ -156,6 +625,102 @@ RecPtr rec_ptr(const bcm_gated_rec_args* a) {
 }
 
 int64_t rec_rows(const bcm_gated_rec_args* a) { return a->cu_seqlens ? a->seqlen : a->batch * a->seqlen; }
+int rec_chunks(int64_t L) { return (int)((L + kChunk - 1) / kChunk); }
+
+// How the tokens are dealt out.  It goes by sizes alone: forward and backward have to agree on the runs.
+struct Plan {
+    int mode, per, L, vec, P;
+    int64_t runs;
+};
+
+Plan rec_plan(const bcm_gated_rec_args* a, int vec) {
+    Plan pl = {kDense, 1, (int)a->seqlen, vec, 1, a->batch};
+    // in units of the widest tile, so that the runs do not depend on alignment
+    const int64_t wide = (a->dim + 63) / 64, tiles = (a->dim + 32 * vec - 1) / (32 * vec);
+    if (a->cu_seqlens) {
+        pl.mode = kPacked;
+        pl.runs = 1;
+    } else if (a->seqlen < 4 * kChunk && a->batch > 1) {
+        // runs of about 8 chunks (an eighth of the last one empty at most), fewer where that leaves SMs without a block
+        pl.mode = kGroup;
+        int64_t per = (8 * kChunk + a->seqlen - 1) / a->seqlen;
+        while (per > 1 && per * a->seqlen > kChunk && ((a->batch + per - 1) / per) * wide < 4 * (int64_t)sm_count()) per = (per + 1) / 2;
+        pl.per = (int)std::min<int64_t>(per, a->batch);
+        pl.L = (int)(pl.per * a->seqlen);
+        pl.runs = (a->batch + pl.per - 1) / pl.per;
+    }
+    // blocks of a cluster: as many as the chunks allow until the GPU holds three blocks per SM
+    while (pl.P < kMaxCluster && pl.runs * tiles * pl.P < 3 * (int64_t)sm_count() && 2 * pl.P <= rec_chunks(pl.L)) pl.P *= 2;
+    return pl;
+}
+
+// Two features a lane where rows are even and aligned for it.
+int rec_vec(const bcm_gated_rec_args* a, bool bwd) {
+    const size_t s = 2 * dtype_size(a->dtype);
+    int64_t odd = a->dim;
+    uintptr_t at = 0;
+    auto see = [&](const void* p, int64_t sb, int64_t st) {
+        at |= (uintptr_t)p;
+        odd |= (a->cu_seqlens || a->batch == 1 ? 0 : sb) | (a->seqlen == 1 ? 0 : st);
+    };
+    see(a->x, a->x_stride_b, a->x_stride_t);
+    see(a->r, a->r_stride_b, a->r_stride_t);
+    see(a->i, a->i_stride_b, a->i_stride_t);
+    if (bwd) {
+        if (a->dy) see(a->dy, a->dy_stride_b, a->dy_stride_t);
+        at |= (uintptr_t)a->dx | (uintptr_t)a->dr | (uintptr_t)a->di;
+    } else {
+        at |= (uintptr_t)a->y;
+    }
+    return (odd & 1) == 0 && at % s == 0 ? 2 : 1;
+}
+
+template <typename F>
+bcm_status rec_launch_as(F* kernel, const bcm_gated_rec_args* a, const RecOut& o, const Plan& pl, cudaStream_t stream) {
+    const int64_t blocks = ((a->dim + 32 * pl.vec - 1) / (32 * pl.vec)) * pl.runs * pl.P;
+    BCM_REQUIRE(blocks < (1ll << 31), "gated_rec: batch x dim too large");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)pl.P;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pl.P > 1 ? 1 : 0;
+    if (pl.P > 8) BCM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    const RecDim n = {a->cu_seqlens, a->batch, pl.L, (int)a->seqlen, pl.per, (int)a->dim, pl.P};
+    BCM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, rec_ptr(a), o, n, a->lam, a->decay_scale));
+    return BCM_OK;
+}
+
+template <bool BWD, typename T, int VEC, int MODE>
+bcm_status rec_launch_p(const bcm_gated_rec_args* a, const RecOut& o, const Plan& pl, cudaStream_t stream) {
+    if constexpr (BWD) {
+        return pl.P > 1 ? rec_launch_as(rec_bwd_kernel<T, VEC, MODE, true>, a, o, pl, stream)
+                        : rec_launch_as(rec_bwd_kernel<T, VEC, MODE, false>, a, o, pl, stream);
+    } else {
+        return pl.P > 1 ? rec_launch_as(rec_fwd_kernel<T, VEC, MODE, true>, a, o, pl, stream)
+                        : rec_launch_as(rec_fwd_kernel<T, VEC, MODE, false>, a, o, pl, stream);
+    }
+}
+
+template <bool BWD, typename T, int VEC>
+bcm_status rec_launch_v(const bcm_gated_rec_args* a, const RecOut& o, const Plan& pl, cudaStream_t stream) {
+    if (pl.mode == kDense) return rec_launch_p<BWD, T, VEC, kDense>(a, o, pl, stream);
+    if (pl.mode == kGroup) return rec_launch_p<BWD, T, VEC, kGroup>(a, o, pl, stream);
+    return rec_launch_p<BWD, T, VEC, kPacked>(a, o, pl, stream);
+}
+
+template <bool BWD>
+bcm_status rec_launch(const bcm_gated_rec_args* a, const RecOut& o, const Plan& pl, cudaStream_t stream) {
+    return dispatch_dtype(a->dtype, [&](auto tag) -> bcm_status {
+        using T = decltype(tag);
+        return pl.vec == 2 ? rec_launch_v<BWD, T, 2>(a, o, pl, stream) : rec_launch_v<BWD, T, 1>(a, o, pl, stream);
+    });
+}
 
 }  // namespace
 }  // namespace bcm
@@ -164,12 +729,16 @@ using namespace bcm;
 
 extern "C" size_t bcm_gated_rec_ckpt_bytes(const bcm_gated_rec_args* a) {
     if (!a || a->batch < 0 || a->seqlen < 0 || a->dim < 1) return 0;
-    return align_up((size_t)rec_rows(a) * (size_t)a->dim * sizeof(float), 256);
+    if (rec_rows(a) == 0) return 0;
+    const Plan pl = rec_plan(a, 1);
+    return align_up((size_t)pl.runs * (size_t)rec_chunks(pl.L) * (size_t)a->dim * sizeof(float), 256);
 }
 
 extern "C" size_t bcm_gated_rec_bwd_workspace_bytes(const bcm_gated_rec_args* a) {
     if (!a || a->batch < 0 || a->seqlen < 0 || a->dim < 1) return 0;
-    return align_up((size_t)a->batch * (size_t)a->dim * sizeof(float), 256);
+    if (rec_rows(a) == 0) return 0;
+    const Plan pl = rec_plan(a, 2);         // one lane a feature takes no more blocks to a cluster than two
+    return align_up((size_t)pl.runs * (size_t)pl.P * (size_t)a->dim * sizeof(float), 256);
 }
 
 extern "C" bcm_status bcm_gated_rec_fwd(const bcm_gated_rec_args* a, cudaStream_t stream) {
@@ -181,43 +750,43 @@ extern "C" bcm_status bcm_gated_rec_fwd(const bcm_gated_rec_args* a, cudaStream_
         set_error("gated_rec_fwd: ckpt of %zu bytes < required %zu", a->ckpt_bytes, bcm_gated_rec_ckpt_bytes(a));
         return BCM_ERR_WORKSPACE;
     }
-    const dim3 grid((unsigned)ceil_div(a->dim, 128), (unsigned)a->batch);
-    return dispatch_dtype(a->dtype, [&](auto tag) -> bcm_status {
-        using T = decltype(tag);
-        rec_fwd_kernel<T><<<grid, 128, 0, stream>>>(rec_ptr(a), a->cu_seqlens, a->seqlen, a->dim, a->lam, a->decay_scale, a->h0,
-                                                    static_cast<T*>(a->y), a->h_last, static_cast<float*>(a->ckpt));
-        BCM_LAUNCH_CHECK();
+    if (rec_rows(a) == 0) {                 // no token: the states stay
+        const size_t bytes = sizeof(float) * (size_t)a->batch * (size_t)a->dim;
+        if (a->h0) BCM_CUDA_TRY(cudaMemcpyAsync(a->h_last, a->h0, bytes, cudaMemcpyDeviceToDevice, stream));
+        else BCM_CUDA_TRY(cudaMemsetAsync(a->h_last, 0, bytes, stream));
         return BCM_OK;
-    });
+    }
+    RecOut o = {};
+    o.h0 = a->h0; o.y = a->y; o.h_last = a->h_last; o.ckpt = static_cast<float*>(a->ckpt);
+    return rec_launch<false>(a, o, rec_plan(a, rec_vec(a, false)), stream);
 }
 
 extern "C" bcm_status bcm_gated_rec_bwd(const bcm_gated_rec_args* a, cudaStream_t stream) {
     clear_error();
     if (bcm_status st = rec_validate(a, "gated_rec_bwd"); st != BCM_OK) return st;
     BCM_REQUIRE(a->lam && a->dlam, "gated_rec_bwd: null pointer");
-    if (a->batch == 0) {
+    if (rec_rows(a) == 0) {
+        const size_t bytes = sizeof(float) * (size_t)a->batch * (size_t)a->dim;
         BCM_CUDA_TRY(cudaMemsetAsync(a->dlam, 0, sizeof(float) * a->dim, stream));
+        if (a->dh0 && a->dh_last) BCM_CUDA_TRY(cudaMemcpyAsync(a->dh0, a->dh_last, bytes, cudaMemcpyDeviceToDevice, stream));
+        else if (a->dh0) BCM_CUDA_TRY(cudaMemsetAsync(a->dh0, 0, bytes, stream));
         return BCM_OK;
     }
-    BCM_REQUIRE(rec_rows(a) == 0 || (a->x && a->r && a->i && a->dx && a->dr && a->di && a->ckpt), "gated_rec_bwd: null pointer");
+    BCM_REQUIRE(a->batch >= 1 && a->x && a->r && a->i && a->dx && a->dr && a->di && a->ckpt, "gated_rec_bwd: null pointer");
     const size_t need = bcm_gated_rec_bwd_workspace_bytes(a), ck = bcm_gated_rec_ckpt_bytes(a);
     if (!a->workspace || a->workspace_bytes < need || a->ckpt_bytes < ck) {
         set_error("gated_rec_bwd: workspace of %zu bytes or ckpt of %zu bytes < required %zu and %zu", a->workspace_bytes,
                   a->ckpt_bytes, need, ck);
         return BCM_ERR_WORKSPACE;
     }
-    float* part = static_cast<float*>(a->workspace);
-    const dim3 grid((unsigned)ceil_div(a->dim, 128), (unsigned)a->batch);
-    bcm_status st = dispatch_dtype(a->dtype, [&](auto tag) -> bcm_status {
-        using T = decltype(tag);
-        rec_bwd_kernel<T><<<grid, 128, 0, stream>>>(rec_ptr(a), a->cu_seqlens, a->seqlen, a->dim, a->lam, a->decay_scale,
-                                                    static_cast<const float*>(a->ckpt), a->dh_last, static_cast<T*>(a->dx),
-                                                    static_cast<T*>(a->dr), static_cast<T*>(a->di), part, a->dh0);
-        BCM_LAUNCH_CHECK();
-        return BCM_OK;
-    });
-    if (st != BCM_OK) return st;
-    rec_dlam_kernel<<<(unsigned)ceil_div(a->dim, 128), 128, 0, stream>>>(part, a->batch, a->dim, a->lam, a->decay_scale, a->dlam);
+    RecOut o = {};
+    o.h0 = a->h0; o.ckpt = static_cast<float*>(a->ckpt);
+    o.dh_last = a->dh_last; o.dx = a->dx; o.dr = a->dr; o.di = a->di;
+    o.part = static_cast<float*>(a->workspace); o.dh0 = a->dh0;
+    const Plan pl = rec_plan(a, rec_vec(a, true));
+    if (bcm_status st = rec_launch<true>(a, o, pl, stream); st != BCM_OK) return st;
+    rec_dlam_kernel<<<(unsigned)ceil_div(a->dim, 128), 128, 0, stream>>>(o.part, pl.runs * pl.P, a->dim, a->lam, a->decay_scale,
+                                                                        a->dlam);
     BCM_LAUNCH_CHECK();
     return BCM_OK;
 }

@@ -76,6 +76,12 @@ def test_dense(B, L, D, dtype):
     _check(_inputs(B * L, D, B, dtype, seed=B + L + D), range(0, B * L + 1, L), (B, L))
 
 
+@pytest.mark.parametrize("B,L,D", [(3000, 1, 65), (700, 2, 64), (333, 7, 96), (90, 64, 33), (41, 65, 10), (9, 255, 6), (2, 256, 64),
+                                   (1, 20000, 4)])
+def test_many_short_and_one_long(B, L, D):
+    _check(_inputs(B * L, D, B, torch.float32, seed=B + L), range(0, B * L + 1, L), (B, L))
+
+
 def test_half():
     _check(_inputs(2 * 300, 70, 2, torch.float16, seed=3), (0, 300, 600), (2, 300))
 

@@ -21,20 +21,66 @@ namespace {
 __device__ __forceinline__ float sigmoid_(float v) { return 1.0f / (1.0f + expf(-v)); }
 __device__ __forceinline__ float softplus_(float v) { return v > 20.0f ? v : log1pf(expf(v)); }
 
+// ---- two gates at a time ----------------------------------------------------
+// The scan kernels' arithmetic works on pairs (packed fp32 instructions): two
+// neighbouring features of a token, or two tokens of a feature.  What bounds it
+// is the special-function unit (one result per lane every 8 cycles), so:
+//  * a - 1 = expm1(u) is a polynomial for |u| <= kPolyEnd (degree 4 times u,
+//    interpolated at Chebyshev nodes, relative error 1.4e-8): no cancellation in
+//    1 - a^2 = (1 - a)(1 + a) and a correctly rounded a = 1 + (a - 1), so that a
+//    memory of a thousand tokens does not add up a biased decay;
+//  * FAST (every gate of the warp's batch above -40, every cs below kPolyEnd)
+//    shares one reciprocal between the two sigmoids and needs no exponential for
+//    a: 4 results per pair member instead of 6.
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kPolyEnd = 0.35f;
+constexpr float kGateLow = -40.0f;   // below: (1 + e^-r)(1 + e^-i) may overflow
+
+__device__ __forceinline__ float ex2_(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float rcp_(float v) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float rsqrt_(float v) { float r; asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float min_nan_(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
+
 struct Gates {
-    float sr, si, u, a, m;
+    float2 sr, si, w, rs;     // sigmoid(r), sigmoid(i), a - 1, 1 / m (0 where m = 0)
 };
 
-__device__ __forceinline__ Gates gates(float r, float i, float cs) {
+__device__ __forceinline__ float2 one_minus_a2(float2 w) { return __fmul2_rn(w, __ffma2_rn(w, f2(-1.0f), f2(-2.0f))); }
+
+template <bool FAST>
+__device__ __forceinline__ Gates gates(float2 r, float2 i, float2 ncs) {
     Gates g;
-    g.sr = sigmoid_(r);
-    g.si = sigmoid_(i);
-    g.u = -cs * g.sr;
-    const float w = expm1f(g.u);       // a - 1 without cancellation
-    g.a = 1.0f + w;
-    g.m = sqrtf(-w * (2.0f + w));      // 1 - a^2
+    const float2 tr = __fmul2_rn(r, f2(-kLog2e)), ti = __fmul2_rn(i, f2(-kLog2e));
+    const float2 dr = __fadd2_rn(make_float2(ex2_(tr.x), ex2_(tr.y)), f2(1.0f));
+    const float2 di = __fadd2_rn(make_float2(ex2_(ti.x), ex2_(ti.y)), f2(1.0f));
+    if (FAST) {
+        const float2 both = __fmul2_rn(dr, di);
+        const float2 inv = make_float2(rcp_(both.x), rcp_(both.y));
+        g.sr = __fmul2_rn(di, inv);
+        g.si = __fmul2_rn(dr, inv);
+    } else {
+        g.sr = make_float2(rcp_(dr.x), rcp_(dr.y));
+        g.si = make_float2(rcp_(di.x), rcp_(di.y));
+    }
+    const float2 u = __fmul2_rn(ncs, g.sr);
+    float2 q = __ffma2_rn(u, f2(0.007211245596408844f), f2(0.04133187234401703f));
+    q = __ffma2_rn(u, q, f2(0.16662530601024628f));
+    q = __ffma2_rn(u, q, f2(0.49999821186065674f));
+    q = __ffma2_rn(u, q, f2(1.0f));
+    g.w = __fmul2_rn(u, q);
+    if (!FAST) {
+        const float2 t = __fmul2_rn(u, f2(kLog2e));
+        if (!(u.x >= -kPolyEnd)) g.w.x = ex2_(t.x) - 1.0f;
+        if (!(u.y >= -kPolyEnd)) g.w.y = ex2_(t.y) - 1.0f;
+    }
+    const float2 m2 = one_minus_a2(g.w);
+    g.rs.x = m2.x > 1e-37f ? rsqrt_(m2.x) : 0.0f;
+    g.rs.y = m2.y > 1e-37f ? rsqrt_(m2.y) : 0.0f;
     return g;
 }
+
+__device__ __forceinline__ float2 m_of(const Gates& g) { return __fmul2_rn(one_minus_a2(g.w), g.rs); }
 
 struct RecPtr {
     const void* x; const void* r; const void* i; const void* dy;
@@ -47,8 +93,8 @@ struct RecOut {
 };
 
 // ---- layout of the scan kernels -----------------------------------------------
-// A lane owns VEC neighbouring features of one row, a warp kSteps consecutive
-// tokens, a block kWarps * kSteps = kChunk tokens of a tile of 32 * VEC features.
+// A lane owns VEC neighbouring features, a warp a few consecutive tokens, a block
+// kWarps times as many (a chunk) of a tile of 32 * VEC features.
 // A block's chunks follow one another in a loop that carries the state; P blocks
 // of a cluster take P consecutive chunks per turn, so that few tiles with long
 // sequences still fill the GPU.  Every input is read once: the composition
@@ -61,8 +107,8 @@ struct RecOut {
 // chunk empty); kPacked, one run of tokens with the sequences' offsets in cu.
 // Where a sequence starts inside a run, nothing passes and its own state enters.
 constexpr int kWarps = 8;
-constexpr int kSteps = 8;
-constexpr int kChunk = kWarps * kSteps;
+constexpr int kChunkFwd = 64, kChunkBwd = 32;    // tokens of a block's turn: 8 and 4 a warp (the backward keeps 7 values a token)
+constexpr int kCkpt = 32;                        // the forward keeps the state that enters every kCkpt tokens of a run
 constexpr int kMaxCluster = 16;
 constexpr float kCut = -1.0f;   // in place of a product of decays: nothing passes (a sequence starts inside)
 
@@ -95,6 +141,28 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
         memcpy(&w, e, 4);
         *reinterpret_cast<uint32_t*>(p) = w;
     }
+}
+
+// Arrays of pairs hold S tokens of VEC features: pair j = token j's two features, or the tokens 2j, 2j + 1 of one.
+template <int VEC, int N>
+__device__ __forceinline__ float get(const float2 (&p)[N], int j, int v) {
+    if (VEC == 2) return v ? p[j].y : p[j].x;
+    return (j & 1) ? p[j >> 1].y : p[j >> 1].x;
+}
+template <int VEC, int N>
+__device__ __forceinline__ void put(float2 (&p)[N], int j, int v, float e) {
+    if (VEC == 2) {
+        if (v) p[j].y = e;
+        else p[j].x = e;
+    } else {
+        if (j & 1) p[j >> 1].y = e;
+        else p[j >> 1].x = e;
+    }
+}
+template <int VEC, int N>
+__device__ __forceinline__ void put_row(float2 (&p)[N], int j, const float (&e)[VEC]) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) put<VEC>(p, j, v, e[v]);
 }
 
 // The sequence that holds token t: the last s with cu[s] <= t, in [0, n).  Called by whole warps; t is uniform.
@@ -174,10 +242,21 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// Whether a warp's batch of gates can take the shorter form (uniform over the warp; false where a gate is NaN).
+template <int N>
+__device__ __forceinline__ bool fast_batch(bool small, const float2 (&r)[N], const float2 (&i)[N]) {
+    if (!small) return false;
+    float low = 0.0f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) low = min_nan_(min_nan_(low, min_nan_(r[k].x, r[k].y)), min_nan_(i[k].x, i[k].y));
+    return __all_sync(kFull, low >= kGateLow);
+}
+
 template <typename T, int VEC, int MODE, bool CLUSTER>
 __global__ void __launch_bounds__(kWarps * 32)
 rec_fwd_kernel(RecPtr p, RecOut o, RecDim n, const float* __restrict__ lam, float c) {
     constexpr bool CUTS = MODE != kDense;
+    constexpr int kChunk = kChunkFwd, S = kChunk / kWarps, NP = S * VEC / 2;
     __shared__ float2 ex[2][kWarps][VEC][32];
     __shared__ float2 pub[CLUSTER ? 2 : 1][CLUSTER ? kMaxCluster : 1][VEC][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -196,11 +275,12 @@ rec_fwd_kernel(RecPtr p, RecOut o, RecDim n, const float* __restrict__ lam, floa
     const T* i = static_cast<const T*>(p.i) + (MODE == kPacked ? 0 : b * p.ib) + dd;
     T* y = static_cast<T*>(o.y) + (MODE == kPacked ? 0 : b * n.Ls * D) + dd;
     const int chunks = (n.L + kChunk - 1) / kChunk, turns = (chunks + P - 1) / P;   // (of a full run)
-    float* ck = o.ckpt ? o.ckpt + run_id * chunks * D + dd : nullptr;
-    float cs[VEC], run[VEC];
+    float* ck = o.ckpt ? o.ckpt + run_id * ((n.L + kCkpt - 1) / kCkpt) * D + dd : nullptr;
+    float run[VEC];
+    const float2 ncs = make_float2(-c * softplus_(lam[dd]), -c * softplus_(lam[dd + VEC - 1]));
+    const bool small = __all_sync(kFull, -ncs.x <= kPolyEnd && -ncs.y <= kPolyEnd);
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-        cs[v] = c * softplus_(lam[dd + v]);
         run[v] = MODE == kDense && o.h0 ? o.h0[b * D + dd + v] : 0.0f;
     }
     Seq<MODE> seq{n.cu, (int)n.n, n.Ls, b, 0, 0, 0};
@@ -208,48 +288,67 @@ rec_fwd_kernel(RecPtr p, RecOut o, RecDim n, const float* __restrict__ lam, floa
     for (int turn = 0; turn < turns; ++turn) {
         const int buf = turn & 1;
         const int chunk = turn * P + rank;
-        const int t0 = chunk * kChunk + warp * kSteps;
-        float a[kSteps][VEC], e[kSteps][VEC];
+        const int t0 = chunk * kChunk + warp * S;
+        float2 a[NP], e[NP];
         {
-            float xv[kSteps][VEC], rv[kSteps][VEC], iv[kSteps][VEC];
+            float2 xv[NP], rv[NP], iv[NP];
             if (MODE == kGroup) seq.at(t0);
             int64_t sl = seq.s - b;
             int tl = t0 - seq.beg;
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j) {
+            for (int j = 0; j < S; ++j) {
                 const bool ok = mine && t0 + j < L;
                 const int64_t t = MODE == kGroup ? tl : t0 + j, q = MODE == kGroup ? sl : 0;
-                load_vec<T, VEC>(r + q * p.rb + t * p.rt, ok, rv[j]);
-                load_vec<T, VEC>(i + q * p.ib + t * p.it, ok, iv[j]);
-                load_vec<T, VEC>(x + q * p.xb + t * p.xt, ok, xv[j]);
+                float row[VEC];
+                load_vec<T, VEC>(r + q * p.rb + t * p.rt, ok, row);
+                put_row<VEC>(rv, j, row);
+                load_vec<T, VEC>(i + q * p.ib + t * p.it, ok, row);
+                put_row<VEC>(iv, j, row);
+                load_vec<T, VEC>(x + q * p.xb + t * p.xt, ok, row);
+                put_row<VEC>(xv, j, row);
                 if (MODE == kGroup && ++tl == n.Ls) {
                     tl = 0;
                     ++sl;
                 }
             }
             if (MODE == kPacked && t0 < L) seq.at(t0);
+            if (fast_batch(small, rv, iv)) {
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    const Gates g = gates(rv[j][v], iv[j][v], cs[v]);
-                    const bool ok = t0 + j < L;
-                    a[j][v] = ok ? g.a : 1.0f;
-                    e[j][v] = ok ? g.m * g.si * xv[j][v] : 0.0f;
+                for (int k = 0; k < NP; ++k) {
+                    const Gates g = gates<true>(rv[k], iv[k], ncs);
+                    a[k] = __fadd2_rn(g.w, f2(1.0f));
+                    e[k] = __fmul2_rn(__fmul2_rn(m_of(g), g.si), xv[k]);
                 }
+            } else {
+#pragma unroll
+                for (int k = 0; k < NP; ++k) {
+                    const Gates g = gates<false>(rv[k], iv[k], ncs);
+                    a[k] = __fadd2_rn(g.w, f2(1.0f));
+                    e[k] = __fmul2_rn(__fmul2_rn(m_of(g), g.si), xv[k]);
+                }
+            }
+            if (t0 + S > L)               // tokens past the end change nothing
+#pragma unroll
+                for (int j = 0; j < S; ++j)
+                    if (t0 + j >= L)
+#pragma unroll
+                        for (int v = 0; v < VEC; ++v) {
+                            put<VEC>(a, j, v, 1.0f);
+                            put<VEC>(e, j, v, 0.0f);
+                        }
         }
         unsigned starts = 0;      // bit j: a sequence starts at token t0 + j (its entering state goes into e)
-        if (CUTS && t0 < L && (seq.beg == t0 || seq.end < t0 + kSteps)) {
+        if (CUTS && t0 < L && (seq.beg == t0 || seq.end < t0 + S)) {
             Seq<MODE> q = seq;
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j) {
+            for (int j = 0; j < S; ++j) {
                 const int t = t0 + j;
                 if (t < L && t == q.end) q.at(t);
                 if (t < L && t == q.beg) {
                     starts |= 1u << j;
 #pragma unroll
                     for (int v = 0; v < VEC; ++v)
-                        e[j][v] = fmaf(a[j][v], o.h0 ? o.h0[q.s * D + dd + v] : 0.0f, e[j][v]);
+                        put<VEC>(e, j, v, fmaf(get<VEC>(a, j, v), o.h0 ? o.h0[q.s * D + dd + v] : 0.0f, get<VEC>(e, j, v)));
                 }
             }
         }
@@ -260,10 +359,10 @@ rec_fwd_kernel(RecPtr p, RecOut o, RecDim n, const float* __restrict__ lam, floa
             H[v] = 0.0f;
         }
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
+        for (int j = 0; j < S; ++j) {
             const bool cut = CUTS && (starts >> j & 1u);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) then<CUTS>(A[v], H[v], cut ? kCut : a[j][v], e[j][v]);
+            for (int v = 0; v < VEC; ++v) then<CUTS>(A[v], H[v], cut ? kCut : get<VEC>(a, j, v), get<VEC>(e, j, v));
         }
 #pragma unroll
         for (int v = 0; v < VEC; ++v) ex[buf][warp][v][lane] = make_float2(A[v], H[v]);
@@ -304,17 +403,17 @@ rec_fwd_kernel(RecPtr p, RecOut o, RecDim n, const float* __restrict__ lam, floa
                 run[v] = apply<CUTS>(totA[v], totH[v], run[v]);
             }
         }
-        if (ck && warp == 0 && mine && chunk < chunks)
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) ck[(int64_t)chunk * D + v] = h[v];
 #pragma unroll
         for (int v = 0; v < VEC; ++v) h[v] = apply<CUTS>(preA[v], preH[v], h[v]);
+        if (ck && warp * S % kCkpt == 0 && mine && t0 < L)
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
+            for (int v = 0; v < VEC; ++v) ck[(int64_t)(t0 / kCkpt) * D + v] = h[v];
+#pragma unroll
+        for (int j = 0; j < S; ++j) {
             const int t = t0 + j;
             const bool cut = CUTS && (starts >> j & 1u);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) h[v] = cut ? e[j][v] : fmaf(a[j][v], h[v], e[j][v]);
+            for (int v = 0; v < VEC; ++v) h[v] = cut ? get<VEC>(e, j, v) : fmaf(get<VEC>(a, j, v), h[v], get<VEC>(e, j, v));
             if (mine && t < L) store_vec<T, VEC>(y + (int64_t)t * D, h);
             if (CUTS && t < L) {
                 if (t == seq.end) seq.at(t);
@@ -344,6 +443,7 @@ template <typename T, int VEC, int MODE, bool CLUSTER>
 __global__ void __launch_bounds__(kWarps * 32)
 rec_bwd_kernel(RecPtr p, RecOut o, RecDim n, const float* __restrict__ lam, float c) {
     constexpr bool CUTS = MODE != kDense;
+    constexpr int kChunk = kChunkBwd, S = kChunk / kWarps, NP = S * VEC / 2;
     __shared__ float ex[2][kWarps][3][VEC][32];
     __shared__ float2 pub[CLUSTER ? 2 : 1][CLUSTER ? kMaxCluster : 1][VEC][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -367,60 +467,87 @@ rec_bwd_kernel(RecPtr p, RecOut o, RecDim n, const float* __restrict__ lam, floa
     T* dr = static_cast<T*>(o.dr) + base;
     T* di = static_cast<T*>(o.di) + base;
     const int chunks = (n.L + kChunk - 1) / kChunk, turns = (chunks + P - 1) / P;   // (of a full run)
-    const float* ck = o.ckpt + run_id * chunks * D + dd;
+    const float* ck = o.ckpt + run_id * ((n.L + kCkpt - 1) / kCkpt) * D + dd;
     Seq<MODE> seq{n.cu, (int)n.n, n.Ls, b, 0, 0, 0};
-    float cs[VEC], run[VEC], sum[VEC];
+    float run[VEC];
+    float2 sum = f2(0.0f);
+    const float2 ncs = make_float2(-c * softplus_(lam[dd]), -c * softplus_(lam[dd + VEC - 1]));
+    const bool small = __all_sync(kFull, -ncs.x <= kPolyEnd && -ncs.y <= kPolyEnd);
     if (CUTS) seq.at(L - 1);
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-        cs[v] = c * softplus_(lam[dd + v]);
         run[v] = o.dh_last ? o.dh_last[(CUTS ? seq.s : b) * D + dd + v] : 0.0f;
-        sum[v] = 0.0f;
     }
     if (CLUSTER) cluster_sync();
     for (int turn = turns - 1; turn >= 0; --turn) {
         const int buf = turn & 1;
         const int chunk = turn * P + rank;
-        const int t0 = chunk * kChunk + warp * kSteps;
-        float xv[kSteps][VEC], gv[kSteps][VEC], sr[kSteps][VEC], si[kSteps][VEC], a[kSteps][VEC], m[kSteps][VEC], enter[VEC];
+        const int t0 = chunk * kChunk + warp * S;
+        float2 xv[NP], gv[NP], sr[NP], si[NP], w[NP], rs[NP];
+        float enter[VEC];
         {
-            float rv[kSteps][VEC], iv[kSteps][VEC];
+            float2 rv[NP], iv[NP];
             if (MODE == kGroup) seq.at(t0);
             int64_t sl = seq.s - b;
             int tl = t0 - seq.beg;
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j) {
+            for (int j = 0; j < S; ++j) {
                 const bool ok = mine && t0 + j < L;
                 const int64_t t = MODE == kGroup ? tl : t0 + j, q = MODE == kGroup ? sl : 0;
-                load_vec<T, VEC>(r + q * p.rb + t * p.rt, ok, rv[j]);
-                load_vec<T, VEC>(i + q * p.ib + t * p.it, ok, iv[j]);
-                load_vec<T, VEC>(x + q * p.xb + t * p.xt, ok, xv[j]);
-                load_vec<T, VEC>(dy + q * p.gb + t * p.gt, ok && has_dy, gv[j]);
+                float row[VEC];
+                load_vec<T, VEC>(r + q * p.rb + t * p.rt, ok, row);
+                put_row<VEC>(rv, j, row);
+                load_vec<T, VEC>(i + q * p.ib + t * p.it, ok, row);
+                put_row<VEC>(iv, j, row);
+                load_vec<T, VEC>(x + q * p.xb + t * p.xt, ok, row);
+                put_row<VEC>(xv, j, row);
+                load_vec<T, VEC>(dy + q * p.gb + t * p.gt, ok && has_dy, row);
+                put_row<VEC>(gv, j, row);
                 if (MODE == kGroup && ++tl == n.Ls) {
                     tl = 0;
                     ++sl;
                 }
             }
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) enter[v] = chunk < chunks ? ck[(int64_t)chunk * D + v] : 0.0f;
+            for (int v = 0; v < VEC; ++v) enter[v] = chunk * kChunk < L ? ck[(int64_t)chunk * D + v] : 0.0f;
             if (MODE == kPacked && t0 < L) seq.at(t0);
+            if (fast_batch(small, rv, iv)) {
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    const Gates g = gates(rv[j][v], iv[j][v], cs[v]);
-                    sr[j][v] = g.sr;
-                    si[j][v] = g.si;
-                    a[j][v] = t0 + j < L ? g.a : 1.0f;
-                    m[j][v] = g.m;
+                for (int k = 0; k < NP; ++k) {
+                    const Gates g = gates<true>(rv[k], iv[k], ncs);
+                    sr[k] = g.sr; si[k] = g.si; w[k] = g.w; rs[k] = g.rs;
                 }
+            } else {
+#pragma unroll
+                for (int k = 0; k < NP; ++k) {
+                    const Gates g = gates<false>(rv[k], iv[k], ncs);
+                    sr[k] = g.sr; si[k] = g.si; w[k] = g.w; rs[k] = g.rs;
+                }
+            }
+            if (t0 + S > L)               // tokens past the end change nothing
+#pragma unroll
+                for (int j = 0; j < S; ++j)
+                    if (t0 + j >= L)
+#pragma unroll
+                        for (int v = 0; v < VEC; ++v) {
+                            put<VEC>(w, j, v, 0.0f);
+                            put<VEC>(rs, j, v, 0.0f);
+                            put<VEC>(sr, j, v, 0.0f);
+                        }
+        }
+        float2 a[NP], msi[NP], prev[NP];
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            a[k] = __fadd2_rn(w[k], f2(1.0f));
+            msi[k] = __fmul2_rn(__fmul2_rn(one_minus_a2(w[k]), rs[k]), si[k]);
+            prev[k] = __fmul2_rn(msi[k], xv[k]);        // for now what enters at the token
         }
         // forward composition (A, H), backward composition (A, K) of the warp's tokens
         unsigned starts = 0;
-        if (CUTS && t0 < L && (seq.beg == t0 || seq.end < t0 + kSteps)) {
+        if (CUTS && t0 < L && (seq.beg == t0 || seq.end < t0 + S)) {
             Seq<MODE> q = seq;
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j) {
+            for (int j = 0; j < S; ++j) {
                 const int t = t0 + j;
                 if (t < L && t == q.end) q.at(t);
                 if (t < L && t == q.beg) starts |= 1u << j;
@@ -445,24 +572,24 @@ rec_bwd_kernel(RecPtr p, RecOut o, RecDim n, const float* __restrict__ lam, floa
             K[v] = 0.0f;
         }
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
+        for (int j = 0; j < S; ++j) {
             const bool cut = CUTS && (starts >> j & 1u);
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                const float e = m[j][v] * si[j][v] * xv[j][v];
+                const float e = get<VEC>(prev, j, v);
                 if (cut) {
                     A[v] = kCut;
-                    H[v] = fmaf(a[j][v], state0(t0 + j, v), e);
+                    H[v] = fmaf(get<VEC>(a, j, v), state0(t0 + j, v), e);
                 } else {
-                    then<CUTS>(A[v], H[v], a[j][v], e);
+                    then<CUTS>(A[v], H[v], get<VEC>(a, j, v), e);
                 }
             }
         }
 #pragma unroll
-        for (int j = kSteps - 1; j >= 0; --j) {
+        for (int j = S - 1; j >= 0; --j) {
             const bool cut = CUTS && (starts >> j & 1u);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) K[v] = cut ? back0(t0 + j - 1, v) : a[j][v] * (gv[j][v] + K[v]);
+            for (int v = 0; v < VEC; ++v) K[v] = cut ? back0(t0 + j - 1, v) : get<VEC>(a, j, v) * (get<VEC>(gv, j, v) + K[v]);
         }
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
@@ -508,47 +635,61 @@ rec_bwd_kernel(RecPtr p, RecOut o, RecDim n, const float* __restrict__ lam, floa
         }
 #pragma unroll
         for (int v = 0; v < VEC; ++v) back[v] = apply<CUTS>(sufA[v], sufK[v], back[v]);
-        float prev[kSteps][VEC];
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
+        for (int j = 0; j < S; ++j) {
             const bool cut = CUTS && (starts >> j & 1u);
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
                 if (cut) h[v] = state0(t0 + j, v);
-                prev[j][v] = h[v];
-                h[v] = fmaf(a[j][v], h[v], m[j][v] * si[j][v] * xv[j][v]);
+                const float e = get<VEC>(prev, j, v);
+                put<VEC>(prev, j, v, h[v]);
+                h[v] = fmaf(get<VEC>(a, j, v), h[v], e);
             }
         }
 #pragma unroll
-        for (int j = kSteps - 1; j >= 0; --j) {
-            const int t = t0 + j;
-            const bool ok = mine && t < L;
-            float ox[VEC], orr[VEC], oi[VEC];
+        for (int j = S - 1; j >= 0; --j) {              // gv becomes G
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                const float G = gv[j][v] + back[v];
-                ox[v] = G * m[j][v] * si[j][v];
-                oi[v] = ox[v] * xv[j][v] * (1.0f - si[j][v]);
-                const float slope = m[j][v] == 0.0f ? 0.0f : a[j][v] * a[j][v] / m[j][v];
-                const float du = G * (a[j][v] * prev[j][v] - slope * si[j][v] * xv[j][v]);
-                orr[v] = du * (-cs[v] * sr[j][v]) * (1.0f - sr[j][v]);
-                if (t < L) {
-                    sum[v] = fmaf(du, sr[j][v], sum[v]);
-                    back[v] = a[j][v] * G;
-                }
-            }
-            if (ok) {
-                store_vec<T, VEC>(dx + (int64_t)t * D, ox);
-                store_vec<T, VEC>(dr + (int64_t)t * D, orr);
-                store_vec<T, VEC>(di + (int64_t)t * D, oi);
+                const float G = get<VEC>(gv, j, v) + back[v];
+                put<VEC>(gv, j, v, G);
+                back[v] = t0 + j < L ? get<VEC>(a, j, v) * G : back[v];
             }
             if (CUTS && (starts >> j & 1u)) {
                 Seq<MODE> q = seq;
-                q.at(t);
+                q.at(t0 + j);
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
                     if (o.dh0 && mine) o.dh0[q.s * D + d + v] = back[v];
-                    back[v] = back0(t - 1, v);
+                    back[v] = back0(t0 + j - 1, v);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            const float2 G = gv[k];
+            const float2 ox = __fmul2_rn(G, msi[k]);
+            const float2 oi = __fmul2_rn(__fmul2_rn(ox, xv[k]), __ffma2_rn(si[k], f2(-1.0f), f2(1.0f)));
+            // du = G a (prev - (a / m) sigmoid(i) x)
+            const float2 slope = __fmul2_rn(__fmul2_rn(a[k], rs[k]), __fmul2_rn(si[k], xv[k]));
+            const float2 du = __fmul2_rn(__fmul2_rn(G, a[k]), __ffma2_rn(slope, f2(-1.0f), prev[k]));
+            const float2 ds = __fmul2_rn(du, sr[k]);
+            sum = __fadd2_rn(sum, ds);
+            const float2 orr = __fmul2_rn(__fmul2_rn(ds, ncs), __ffma2_rn(sr[k], f2(-1.0f), f2(1.0f)));
+#pragma unroll
+            for (int half = 0; half < 2 / VEC; ++half) {
+                const int t = t0 + (VEC == 2 ? k : 2 * k + half);
+                if (mine && t < L) {
+                    float vx[VEC], vr[VEC], vi[VEC];
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) {
+                        const bool y = VEC == 2 ? v : half;
+                        vx[v] = y ? ox.y : ox.x;
+                        vr[v] = y ? orr.y : orr.x;
+                        vi[v] = y ? oi.y : oi.x;
+                    }
+                    store_vec<T, VEC>(dx + (int64_t)t * D, vx);
+                    store_vec<T, VEC>(dr + (int64_t)t * D, vr);
+                    store_vec<T, VEC>(di + (int64_t)t * D, vi);
                 }
             }
         }
@@ -556,7 +697,7 @@ rec_bwd_kernel(RecPtr p, RecOut o, RecDim n, const float* __restrict__ lam, floa
     __syncthreads();
     float* red = &ex[0][0][0][0][0];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) red[(warp * VEC + v) * 32 + lane] = sum[v];
+    for (int v = 0; v < VEC; ++v) red[(warp * VEC + v) * 32 + lane] = VEC == 2 ? (v ? sum.y : sum.x) : sum.x + sum.y;
     __syncthreads();
     if (warp == 0 && mine)
 #pragma unroll
@@ -596,9 +737,9 @@ __global__ void rec_step_kernel(RecPtr p, int64_t B, int64_t D, const float* __r
     const int64_t n = B * D, stride = (int64_t)gridDim.x * blockDim.x;
     for (int64_t k = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; k < n; k += stride) {
         const int64_t b = k / D, d = k - b * D;
-        const Gates g = gates(to_f32<T>(static_cast<const T*>(p.r)[b * p.rb + d]),
-                              to_f32<T>(static_cast<const T*>(p.i)[b * p.ib + d]), c * softplus_(lam[d]));
-        const float v = fmaf(g.a, h[k], g.m * g.si * to_f32<T>(static_cast<const T*>(p.x)[b * p.xb + d]));
+        const Gates g = gates<false>(f2(to_f32<T>(static_cast<const T*>(p.r)[b * p.rb + d])),
+                                     f2(to_f32<T>(static_cast<const T*>(p.i)[b * p.ib + d])), f2(-c * softplus_(lam[d])));
+        const float v = fmaf(1.0f + g.w.x, h[k], m_of(g).x * g.si.x * to_f32<T>(static_cast<const T*>(p.x)[b * p.xb + d]));
         h[k] = v;
         y[k] = from_f32<T>(v);
     }
@@ -625,7 +766,7 @@ RecPtr rec_ptr(const bcm_gated_rec_args* a) {
 }
 
 int64_t rec_rows(const bcm_gated_rec_args* a) { return a->cu_seqlens ? a->seqlen : a->batch * a->seqlen; }
-int rec_chunks(int64_t L) { return (int)((L + kChunk - 1) / kChunk); }
+int64_t rec_parts(int64_t L, int part) { return (L + part - 1) / part; }
 
 // How the tokens are dealt out.  It goes by sizes alone: forward and backward have to agree on the runs.
 struct Plan {
@@ -640,17 +781,17 @@ Plan rec_plan(const bcm_gated_rec_args* a, int vec) {
     if (a->cu_seqlens) {
         pl.mode = kPacked;
         pl.runs = 1;
-    } else if (a->seqlen < 4 * kChunk && a->batch > 1) {
+    } else if (a->seqlen < 4 * kChunkFwd && a->batch > 1) {
         // runs of about 8 chunks (an eighth of the last one empty at most), fewer where that leaves SMs without a block
         pl.mode = kGroup;
-        int64_t per = (8 * kChunk + a->seqlen - 1) / a->seqlen;
-        while (per > 1 && per * a->seqlen > kChunk && ((a->batch + per - 1) / per) * wide < 4 * (int64_t)sm_count()) per = (per + 1) / 2;
+        int64_t per = (8 * kChunkFwd + a->seqlen - 1) / a->seqlen;
+        while (per > 1 && per * a->seqlen > kChunkFwd && ((a->batch + per - 1) / per) * wide < 4 * (int64_t)sm_count()) per = (per + 1) / 2;
         pl.per = (int)std::min<int64_t>(per, a->batch);
         pl.L = (int)(pl.per * a->seqlen);
         pl.runs = (a->batch + pl.per - 1) / pl.per;
     }
     // blocks of a cluster: as many as the chunks allow until the GPU holds three blocks per SM
-    while (pl.P < kMaxCluster && pl.runs * tiles * pl.P < 3 * (int64_t)sm_count() && 2 * pl.P <= rec_chunks(pl.L)) pl.P *= 2;
+    while (pl.P < kMaxCluster && pl.runs * tiles * pl.P < 3 * (int64_t)sm_count() && 2 * pl.P <= rec_parts(pl.L, kChunkFwd)) pl.P *= 2;
     return pl;
 }
 
@@ -731,7 +872,7 @@ extern "C" size_t bcm_gated_rec_ckpt_bytes(const bcm_gated_rec_args* a) {
     if (!a || a->batch < 0 || a->seqlen < 0 || a->dim < 1) return 0;
     if (rec_rows(a) == 0) return 0;
     const Plan pl = rec_plan(a, 1);
-    return align_up((size_t)pl.runs * (size_t)rec_chunks(pl.L) * (size_t)a->dim * sizeof(float), 256);
+    return align_up((size_t)pl.runs * (size_t)rec_parts(pl.L, kCkpt) * (size_t)a->dim * sizeof(float), 256);
 }
 
 extern "C" size_t bcm_gated_rec_bwd_workspace_bytes(const bcm_gated_rec_args* a) {

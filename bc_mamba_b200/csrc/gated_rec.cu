@@ -21,66 +21,96 @@ namespace {
 __device__ __forceinline__ float sigmoid_(float v) { return 1.0f / (1.0f + expf(-v)); }
 __device__ __forceinline__ float softplus_(float v) { return v > 20.0f ? v : log1pf(expf(v)); }
 
-// ---- two gates at a time ----------------------------------------------------
-// The scan kernels' arithmetic works on pairs (packed fp32 instructions): two
-// neighbouring features of a token, or two tokens of a feature.  What bounds it
-// is the special-function unit (one result per lane every 8 cycles), so:
+// ---- the gates of two features at a time ------------------------------------
+// A lane owns two neighbouring features; its arithmetic is packed fp32 (two
+// results an instruction).  What bounds it then is the special-function unit
+// (8 cycles a warp instruction), so:
 //  * a - 1 = expm1(u) is a polynomial for |u| <= kPolyEnd (degree 4 times u,
-//    interpolated at Chebyshev nodes, relative error 1.4e-8): no cancellation in
-//    1 - a^2 = (1 - a)(1 + a) and a correctly rounded a = 1 + (a - 1), so that a
-//    memory of a thousand tokens does not add up a biased decay;
-//  * FAST (every gate of the warp's batch above -40, every cs below kPolyEnd)
-//    shares one reciprocal between the two sigmoids and needs no exponential for
-//    a: 4 results per pair member instead of 6.
+//    interpolated at Chebyshev nodes, relative error 1.4e-8).  It also gives
+//    1 - a^2 = (1 - a)(1 + a) without cancellation and a correctly rounded
+//    a = 1 + (a - 1), so that a memory of a thousand tokens does not add up a
+//    biased decay;
+//  * FAST shares one reciprocal between the four sigmoids of a pair and needs no
+//    exponential for a: 7 special functions a pair instead of 12.  It holds where
+//    every c s is at most kPolyEnd and the product of a pair's four denominators
+//    (1 + e^-r)(1 + e^-i) stays below kProdEnd; a warp that finds a larger one (a
+//    gate below about -20, infinite, NaN) computes its batch again in the long form.
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPolyEnd = 0.35f;
-constexpr float kGateLow = -40.0f;   // below: (1 + e^-r)(1 + e^-i) may overflow
+constexpr float kProdEnd = 1e36f;
 
 __device__ __forceinline__ float ex2_(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
 __device__ __forceinline__ float rcp_(float v) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
 __device__ __forceinline__ float rsqrt_(float v) { float r; asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
-__device__ __forceinline__ float min_nan_(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float max_nan_(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 mul(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 fma(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 
 struct Gates {
-    float2 sr, si, w, rs;     // sigmoid(r), sigmoid(i), a - 1, 1 / m (0 where m = 0)
+    float2 sr, si, w, rs;     // sigmoid(r), sigmoid(i), a - 1, 1 / m (3e18 where m = 0: it meets a factor 0 then)
 };
 
-__device__ __forceinline__ float2 one_minus_a2(float2 w) { return __fmul2_rn(w, __ffma2_rn(w, f2(-1.0f), f2(-2.0f))); }
+__device__ __forceinline__ float2 a_of(float2 w) { return add(w, f2(1.0f)); }
+// m = (1 - a^2) / sqrt(1 - a^2): exactly 0 for a = 1
+__device__ __forceinline__ float2 m_of(float2 w, float2 rs) { return mul(mul(w, fma(w, f2(-1.0f), f2(-2.0f))), rs); }
 
 template <bool FAST>
-__device__ __forceinline__ Gates gates(float2 r, float2 i, float2 ncs) {
+__device__ __forceinline__ Gates gates(float2 r, float2 i, float2 ncs, float& prod) {
     Gates g;
-    const float2 tr = __fmul2_rn(r, f2(-kLog2e)), ti = __fmul2_rn(i, f2(-kLog2e));
-    const float2 dr = __fadd2_rn(make_float2(ex2_(tr.x), ex2_(tr.y)), f2(1.0f));
-    const float2 di = __fadd2_rn(make_float2(ex2_(ti.x), ex2_(ti.y)), f2(1.0f));
+    const float2 tr = mul(r, f2(-kLog2e)), ti = mul(i, f2(-kLog2e));
+    const float2 dr = add(make_float2(ex2_(tr.x), ex2_(tr.y)), f2(1.0f));
+    const float2 di = add(make_float2(ex2_(ti.x), ex2_(ti.y)), f2(1.0f));
     if (FAST) {
-        const float2 both = __fmul2_rn(dr, di);
-        const float2 inv = make_float2(rcp_(both.x), rcp_(both.y));
-        g.sr = __fmul2_rn(di, inv);
-        g.si = __fmul2_rn(dr, inv);
+        const float2 both = mul(dr, di);
+        const float all = both.x * both.y;
+        prod = max_nan_(prod, all);
+        const float2 inv = mul(make_float2(both.y, both.x), f2(rcp_(all)));
+        g.sr = mul(di, inv);
+        g.si = mul(dr, inv);
     } else {
         g.sr = make_float2(rcp_(dr.x), rcp_(dr.y));
         g.si = make_float2(rcp_(di.x), rcp_(di.y));
     }
-    const float2 u = __fmul2_rn(ncs, g.sr);
-    float2 q = __ffma2_rn(u, f2(0.007211245596408844f), f2(0.04133187234401703f));
-    q = __ffma2_rn(u, q, f2(0.16662530601024628f));
-    q = __ffma2_rn(u, q, f2(0.49999821186065674f));
-    q = __ffma2_rn(u, q, f2(1.0f));
-    g.w = __fmul2_rn(u, q);
+    const float2 u = mul(ncs, g.sr);
+    float2 q = fma(u, f2(0.007211245596408844f), f2(0.04133187234401703f));
+    q = fma(u, q, f2(0.16662530601024628f));
+    q = fma(u, q, f2(0.49999821186065674f));
+    q = fma(u, q, f2(1.0f));
+    g.w = mul(u, q);
     if (!FAST) {
-        const float2 t = __fmul2_rn(u, f2(kLog2e));
+        const float2 t = mul(u, f2(kLog2e));
         if (!(u.x >= -kPolyEnd)) g.w.x = ex2_(t.x) - 1.0f;
         if (!(u.y >= -kPolyEnd)) g.w.y = ex2_(t.y) - 1.0f;
     }
-    const float2 m2 = one_minus_a2(g.w);
-    g.rs.x = m2.x > 1e-37f ? rsqrt_(m2.x) : 0.0f;
-    g.rs.y = m2.y > 1e-37f ? rsqrt_(m2.y) : 0.0f;
+    const float2 m2 = fma(g.w, fma(g.w, f2(-1.0f), f2(-2.0f)), f2(1e-37f));
+    g.rs = make_float2(rsqrt_(m2.x), rsqrt_(m2.y));
     return g;
 }
 
-__device__ __forceinline__ float2 m_of(const Gates& g) { return __fmul2_rn(one_minus_a2(g.w), g.rs); }
+// ---- layout of the scan kernels -----------------------------------------------
+// A warp owns a few consecutive tokens of 64 features, a block kWarps times as
+// many (a chunk).  A block's chunks follow one another in a loop (turns) that
+// carries the state; P blocks of a cluster take P consecutive chunks per turn, so
+// that few features with long sequences still fill the GPU.  Every input is read
+// once: the composition h -> A h + H of a warp's tokens goes to shared memory,
+// the other warps' and blocks' compositions give the state that enters, and the
+// tokens, still in registers, are replayed from it.  Rows arrive by 16-byte
+// cp.async a few turns ahead; a warp copies its own rows only.
+//
+// Mode: kDense, one sequence per block; kGroup, a block takes `per` consecutive
+// dense sequences as one run of tokens (short sequences would leave most of a
+// chunk empty); kPacked, one run of tokens with the sequences' offsets in cu.
+// Where a sequence starts inside a run, nothing passes and its own state enters.
+constexpr int kWarps = 8;
+constexpr int kTile = 64;                        // features of a block
+constexpr int kStepsFwd = 8, kStepsBwd = 4;      // tokens of a warp's turn (the backward keeps 7 values a token)
+constexpr int kCkpt = kWarps * kStepsBwd;        // the forward keeps the state that enters every kCkpt tokens of a run
+constexpr int kMaxCluster = 16;
+constexpr float kCut = -1.0f;                    // in place of a product of decays: nothing passes (a sequence starts inside)
+
+enum Mode { kDense, kGroup, kPacked };
 
 struct RecPtr {
     const void* x; const void* r; const void* i; const void* dy;
@@ -88,82 +118,17 @@ struct RecPtr {
 };
 
 struct RecOut {
-    const float* h0; void* y; float* h_last; float* ckpt;          // forward
+    const float* h0; void* y; float* h_last; float* ckpt;                          // forward
     const float* dh_last; void* dx; void* dr; void* di; float* part; float* dh0;   // backward
 };
 
-// ---- layout of the scan kernels -----------------------------------------------
-// A lane owns VEC neighbouring features, a warp a few consecutive tokens, a block
-// kWarps times as many (a chunk) of a tile of 32 * VEC features.
-// A block's chunks follow one another in a loop that carries the state; P blocks
-// of a cluster take P consecutive chunks per turn, so that few tiles with long
-// sequences still fill the GPU.  Every input is read once: the composition
-// h -> A h + H of a warp's tokens goes to shared memory, the other warps' and
-// blocks' compositions give the state that enters, and the tokens, still in
-// registers, are replayed from it.
-//
-// Mode: kDense, one sequence per block; kGroup, a block takes `per` consecutive
-// dense sequences as one run of tokens (short sequences would leave most of a
-// chunk empty); kPacked, one run of tokens with the sequences' offsets in cu.
-// Where a sequence starts inside a run, nothing passes and its own state enters.
-constexpr int kWarps = 8;
-constexpr int kChunkFwd = 64, kChunkBwd = 32;    // tokens of a block's turn: 8 and 4 a warp (the backward keeps 7 values a token)
-constexpr int kCkpt = 32;                        // the forward keeps the state that enters every kCkpt tokens of a run
-constexpr int kMaxCluster = 16;
-constexpr float kCut = -1.0f;   // in place of a product of decays: nothing passes (a sequence starts inside)
-
-template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const T* p, bool ok, float (&v)[VEC]) {
-    if constexpr (VEC == 1) {
-        v[0] = ok ? to_f32<T>(*p) : 0.0f;
-    } else if constexpr (sizeof(T) == 4) {
-        const float2 w = ok ? __ldg(reinterpret_cast<const float2*>(p)) : make_float2(0.0f, 0.0f);
-        v[0] = w.x;
-        v[1] = w.y;
-    } else {
-        const uint32_t w = ok ? __ldg(reinterpret_cast<const uint32_t*>(p)) : 0u;
-        T e[2];
-        memcpy(e, &w, 4);
-        v[0] = to_f32<T>(e[0]);
-        v[1] = to_f32<T>(e[1]);
-    }
-}
-
-template <typename T, int VEC>
-__device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
-    if constexpr (VEC == 1) {
-        *p = from_f32<T>(v[0]);
-    } else if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
-    } else {
-        const T e[2] = {from_f32<T>(v[0]), from_f32<T>(v[1])};
-        uint32_t w;
-        memcpy(&w, e, 4);
-        *reinterpret_cast<uint32_t*>(p) = w;
-    }
-}
-
-// Arrays of pairs hold S tokens of VEC features: pair j = token j's two features, or the tokens 2j, 2j + 1 of one.
-template <int VEC, int N>
-__device__ __forceinline__ float get(const float2 (&p)[N], int j, int v) {
-    if (VEC == 2) return v ? p[j].y : p[j].x;
-    return (j & 1) ? p[j >> 1].y : p[j >> 1].x;
-}
-template <int VEC, int N>
-__device__ __forceinline__ void put(float2 (&p)[N], int j, int v, float e) {
-    if (VEC == 2) {
-        if (v) p[j].y = e;
-        else p[j].x = e;
-    } else {
-        if (j & 1) p[j >> 1].y = e;
-        else p[j >> 1].x = e;
-    }
-}
-template <int VEC, int N>
-__device__ __forceinline__ void put_row(float2 (&p)[N], int j, const float (&e)[VEC]) {
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) put<VEC>(p, j, v, e[v]);
-}
+// A run holds L tokens (kGroup: its last may hold fewer), a sequence Ls (kDense, kGroup), per sequences make a run
+// (kGroup); n sequences, D features, P blocks in a cluster.
+struct RecDim {
+    const int32_t* cu;
+    int64_t n;
+    int L, Ls, per, D, P;
+};
 
 // The sequence that holds token t: the last s with cu[s] <= t, in [0, n).  Called by whole warps; t is uniform.
 __device__ __forceinline__ int seq_of(const int32_t* __restrict__ cu, int n, int t) {
@@ -171,24 +136,13 @@ __device__ __forceinline__ int seq_of(const int32_t* __restrict__ cu, int n, int
     const int lane = threadIdx.x & 31;
     while (hi > lo) {
         const int step = (hi - lo + 31) / 32;        // lanes look at lo + step, lo + 2 step, ...
-        const int at = lo + (lane + 1) * step;
-        const unsigned m = __ballot_sync(kFull, at <= hi && cu[at] <= t);
-        const int c = __popc(m);
+        const int64_t at = lo + (int64_t)(lane + 1) * step;
+        const int c = __popc(__ballot_sync(kFull, at <= hi && cu[at] <= t));
         lo += c * step;
         hi = min(hi, lo + step - 1);
     }
     return lo;
 }
-
-enum Mode { kDense, kGroup, kPacked };
-
-// What the kernels know of the sizes: a run holds L tokens (kGroup: its last may hold fewer), a sequence Ls (kDense,
-// kGroup), per sequences make a run (kGroup); n sequences, D features, P blocks in a cluster.
-struct RecDim {
-    const int32_t* cu;
-    int64_t n;
-    int L, Ls, per, D, P;
-};
 
 // The sequence around a token of the run, moved along by a warp: its index s, its first token and its end.
 template <int MODE>
@@ -198,12 +152,13 @@ struct Seq {
     int64_t s0, s;
     int beg, end;
     __device__ __forceinline__ void at(int t) {
+        if (MODE == kDense || (beg <= t && t < end)) return;
         if (MODE == kPacked) {
             const int k = seq_of(cu, n, t);
             s = k;
             beg = cu[k];
             end = cu[k + 1];
-        } else if (MODE == kGroup) {
+        } else {
             const int k = t / Ls;
             s = s0 + k;
             beg = k * Ls;
@@ -214,519 +169,602 @@ struct Seq {
 
 // (A1, H1) followed by (A2, H2)
 template <bool CUTS>
-__device__ __forceinline__ void then(float& A1, float& H1, float A2, float H2) {
-    if (CUTS && A2 < 0.0f) {
-        A1 = kCut;
+__device__ __forceinline__ void then(float2& A1, float2& H1, float2 A2, float2 H2) {
+    if (!CUTS) {
+        H1 = fma(A2, H1, H2);
+        A1 = mul(A1, A2);
+    } else if (A2.x < 0.0f) {                        // (cuts lie between tokens: both features have them)
+        A1 = f2(kCut);
         H1 = H2;
     } else {
-        H1 = fmaf(A2, H1, H2);
-        A1 = CUTS && A1 < 0.0f ? kCut : A1 * A2;
+        const bool cut = A1.x < 0.0f;
+        H1 = fma(A2, H1, H2);
+        A1 = cut ? f2(kCut) : mul(A1, A2);
     }
 }
-
 template <bool CUTS>
-__device__ __forceinline__ float apply(float A, float H, float h) {
-    return CUTS && A < 0.0f ? H : fmaf(A, h, H);
+__device__ __forceinline__ float2 apply(float2 A, float2 H, float2 h) {
+    return CUTS && A.x < 0.0f ? H : fma(A, h, H);
 }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-__device__ __forceinline__ void st_cluster(uint32_t addr, int rank, float2 v) {
+__device__ __forceinline__ void st_cluster(uint32_t addr, int rank, float4 v) {
     uint32_t remote;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(remote), "f"(v.x), "f"(v.y) : "memory");
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
-
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-
-// Whether a warp's batch of gates can take the shorter form (uniform over the warp; false where a gate is NaN).
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
-__device__ __forceinline__ bool fast_batch(bool small, const float2 (&r)[N], const float2 (&i)[N]) {
-    if (!small) return false;
-    float low = 0.0f;
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// ---- rows in shared memory -----------------------------------------------------
+// A row of a tile is 64 elements from the tile's first feature on.  EVEN: every
+// row starts on 16 bytes.  Otherwise the copy starts at the 16-byte granule that
+// holds the row's first element and takes one granule more; it reads no granule
+// without an element of the row in it.
+template <typename T, bool EVEN>
+struct Rows {
+    static constexpr int kGran = kTile * (int)sizeof(T) / 16 + (EVEN ? 0 : 1);
+    static constexpr int kPitch = kGran * 16;
+
+    // S rows from token t0 of the run on, those past its end and the features past the last one filled with zeros
+    template <int MODE, int S>
+    static __device__ __forceinline__ void copy(char* dst, const T* base, int64_t sb, int64_t st, int t0, const RecDim& n, int L, int width) {
+        const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int k = 0; k < N; ++k) low = min_nan_(min_nan_(low, min_nan_(r[k].x, r[k].y)), min_nan_(i[k].x, i[k].y));
-    return __all_sync(kFull, low >= kGateLow);
+        for (int q0 = 0; q0 < S * kGran; q0 += 32) {
+            const int q = q0 + lane, row = q / kGran, g = q - row * kGran, t = t0 + row;
+            if (S * kGran % 32 != 0 && q >= S * kGran) continue;
+            int bytes = 0;
+            uintptr_t src = reinterpret_cast<uintptr_t>(base) & ~(uintptr_t)15;
+            if (t < L) {
+                int64_t at = (int64_t)t * st;
+                if (MODE == kGroup) {
+                    const int k = t / n.Ls;
+                    at = k * sb + (int64_t)(t - k * n.Ls) * st;
+                }
+                const uintptr_t first = reinterpret_cast<uintptr_t>(base + at), end = first + width * sizeof(T);
+                const uintptr_t from = (first & ~(uintptr_t)15) + g * 16;
+                if (from < end) {
+                    src = from;
+                    bytes = (int)min((uintptr_t)16, end - from);
+                }
+            }
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst + row * kPitch + g * 16)), "l"(src), "r"(bytes)
+                         : "memory");
+        }
+    }
+
+    // off: bytes of the row's first element past its granule
+    static __device__ __forceinline__ float2 read(const char* row, int off) {
+        const char* p = row + (threadIdx.x & 31) * 2 * sizeof(T) + (EVEN ? 0 : off);
+        if constexpr (sizeof(T) == 4) {
+            if (EVEN) return *reinterpret_cast<const float2*>(p);
+            return make_float2(*reinterpret_cast<const float*>(p), *reinterpret_cast<const float*>(p + 4));
+        } else {
+            const T *e = reinterpret_cast<const T*>(p);
+            if (EVEN) {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+                T v[2];
+                memcpy(v, &w, 4);
+                return make_float2(to_f32<T>(v[0]), to_f32<T>(v[1]));
+            }
+            return make_float2(to_f32<T>(e[0]), to_f32<T>(e[1]));
+        }
+    }
+};
+
+// The granule offset of the rows t0 .. of one array; rows of a run advance by a constant number of bytes (kDense, kPacked).
+template <typename T, int MODE>
+struct Offset {
+    uint32_t first, step, wrap;
+    int Ls;
+    __device__ __forceinline__ Offset(const T* base, int64_t sb, int64_t st, int Ls_)
+        : first((uint32_t)(uintptr_t)base), step((uint32_t)(st * sizeof(T))), wrap((uint32_t)(sb * sizeof(T))), Ls(Ls_) {}
+    __device__ __forceinline__ int at(int t) const {
+        if (MODE == kGroup) {
+            const int k = t / Ls;
+            return (int)((first + k * wrap + (uint32_t)(t - k * Ls) * step) & 15u);
+        }
+        return (int)((first + (uint32_t)t * step) & 15u);
+    }
+};
+
+// one row's two features; pair: both exist and lie on 2 * sizeof(T)
+template <typename T>
+__device__ __forceinline__ void store_row(T* p, float2 v, bool pair, bool one) {
+    if (pair) {
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float2*>(p) = v;
+        } else {
+            const T e[2] = {from_f32<T>(v.x), from_f32<T>(v.y)};
+            uint32_t w;
+            memcpy(&w, e, 4);
+            *reinterpret_cast<uint32_t*>(p) = w;
+        }
+    } else if (one) {
+        p[0] = from_f32<T>(v.x);
+    }
+}
+template <typename T, bool EVEN>
+__device__ __forceinline__ void store_pair(T* p, float2 v, bool even_rows, bool has0, bool has1) {
+    if (EVEN || even_rows) {
+        store_row<T>(p, v, has0, false);
+    } else {
+        if (has0) p[0] = from_f32<T>(v.x);
+        if (has1) p[1] = from_f32<T>(v.y);
+    }
 }
 
-template <typename T, int VEC, int MODE, bool CLUSTER>
-__global__ void __launch_bounds__(kWarps * 32)
-rec_fwd_kernel(RecPtr p, RecOut o, RecDim n, const float* __restrict__ lam, float c) {
-    constexpr bool CUTS = MODE != kDense;
-    constexpr int kChunk = kChunkFwd, S = kChunk / kWarps, NP = S * VEC / 2;
-    __shared__ float2 ex[2][kWarps][VEC][32];
-    __shared__ float2 pub[CLUSTER ? 2 : 1][CLUSTER ? kMaxCluster : 1][VEC][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int D = n.D, P = n.P, tiles = (D + 32 * VEC - 1) / (32 * VEC);
-    const int rank = CLUSTER ? blockIdx.x % P : 0;
-    const int64_t run_id = blockIdx.x / (CLUSTER ? P : 1) / tiles;
-    const int tile = blockIdx.x / (CLUSTER ? P : 1) - (int)run_id * tiles;
-    // the run's first sequence and its tokens
-    const int64_t b = MODE == kGroup ? run_id * n.per : run_id;
-    const int L = MODE == kGroup ? (int)min((int64_t)n.per, n.n - b) * n.Ls : n.L;
-    const int d = (tile * 32 + lane) * VEC;
-    const bool mine = d < D;
-    const int dd = mine ? d : 0;
-    const T* x = static_cast<const T*>(p.x) + (MODE == kPacked ? 0 : b * p.xb) + dd;
-    const T* r = static_cast<const T*>(p.r) + (MODE == kPacked ? 0 : b * p.rb) + dd;
-    const T* i = static_cast<const T*>(p.i) + (MODE == kPacked ? 0 : b * p.ib) + dd;
-    T* y = static_cast<T*>(o.y) + (MODE == kPacked ? 0 : b * n.Ls * D) + dd;
-    const int chunks = (n.L + kChunk - 1) / kChunk, turns = (chunks + P - 1) / P;   // (of a full run)
-    float* ck = o.ckpt ? o.ckpt + run_id * ((n.L + kCkpt - 1) / kCkpt) * D + dd : nullptr;
-    float run[VEC];
-    const float2 ncs = make_float2(-c * softplus_(lam[dd]), -c * softplus_(lam[dd + VEC - 1]));
-    const bool small = __all_sync(kFull, -ncs.x <= kPolyEnd && -ncs.y <= kPolyEnd);
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-        run[v] = MODE == kDense && o.h0 ? o.h0[b * D + dd + v] : 0.0f;
+__device__ __forceinline__ float2 load_state(const float* p, int64_t row, int D, int d, bool has0, bool has1) {
+    if (p == nullptr) return f2(0.0f);
+    return make_float2(has0 ? p[row * D + d] : 0.0f, has1 ? p[row * D + d + 1] : 0.0f);
+}
+__device__ __forceinline__ void store_state(float* p, int64_t row, int D, int d, float2 v, bool has0, bool has1) {
+    if (has0) p[row * D + d] = v.x;
+    if (has1) p[row * D + d + 1] = v.y;
+}
+
+// Where a block works.
+struct Place {
+    int lane, warp, rank, tile, d, L;
+    int64_t run, b;           // the run and its first sequence
+    bool has0, has1;          // the lane's features exist
+};
+template <int MODE, bool CLUSTER>
+__device__ __forceinline__ Place place(const RecDim& n) {
+    Place q;
+    q.lane = threadIdx.x & 31;
+    q.warp = threadIdx.x >> 5;
+    const int P = CLUSTER ? n.P : 1, tiles = (n.D + kTile - 1) / kTile;
+    q.rank = CLUSTER ? blockIdx.x % P : 0;
+    q.run = blockIdx.x / P / tiles;
+    q.tile = (int)(blockIdx.x / P - q.run * tiles);
+    q.b = MODE == kGroup ? q.run * n.per : q.run;
+    q.L = MODE == kGroup ? (int)min((int64_t)n.per, n.n - q.b) * n.Ls : n.L;
+    q.d = q.tile * kTile + q.lane * 2;
+    q.has0 = q.d < n.D;
+    q.has1 = q.d + 1 < n.D;
+    return q;
+}
+
+// Bit j: a sequence starts at token t0 + j.
+template <int MODE, int S>
+__device__ __forceinline__ unsigned starts_in(const Seq<MODE>& seq, int t0, int L) {
+    if (MODE == kDense || t0 >= L || (seq.beg != t0 && seq.end >= t0 + S)) return 0u;
+    unsigned m = 0;
+    Seq<MODE> q = seq;
+    for (int j = 0; j < S && t0 + j < L; ++j) {
+        q.at(t0 + j);
+        if (t0 + j == q.beg) m |= 1u << j;
     }
-    Seq<MODE> seq{n.cu, (int)n.n, n.Ls, b, 0, 0, 0};
+    return m;
+}
+
+template <typename T, int S, bool EVEN, int ARRAYS>
+constexpr int stage_bytes() { return kWarps * ARRAYS * S * Rows<T, EVEN>::kPitch; }
+// turns of rows in flight or in use: what fits two blocks on an SM
+template <typename T>
+constexpr int stages_fwd() { return sizeof(T) == 4 ? 2 : 3; }
+template <typename T>
+constexpr int stages_bwd() { return sizeof(T) == 4 ? 2 : 3; }
+
+template <typename T, int MODE, bool EVEN, bool CLUSTER>
+__global__ void __launch_bounds__(kWarps * 32, 2)
+rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut o, const __grid_constant__ RecDim n,
+               const float* __restrict__ lam, float c) {
+    constexpr bool CUTS = MODE != kDense;
+    constexpr int S = kStepsFwd, kChunk = kWarps * S, ST = stages_fwd<T>();
+    using R = Rows<T, EVEN>;
+    __shared__ float4 ex[2][kWarps][32];
+    __shared__ float4 pub[CLUSTER ? 2 : 1][CLUSTER ? kMaxCluster : 1][32];
+    extern __shared__ __align__(16) char rows[];
+    const Place w = place<MODE, CLUSTER>(n);
+    const int D = n.D, L = w.L, P = CLUSTER ? n.P : 1, width = min(kTile, D - w.tile * kTile);
+    const int64_t f0 = (int64_t)w.tile * kTile;
+    const T* x = static_cast<const T*>(p.x) + (MODE == kPacked ? 0 : w.b * p.xb) + f0;
+    const T* r = static_cast<const T*>(p.r) + (MODE == kPacked ? 0 : w.b * p.rb) + f0;
+    const T* i = static_cast<const T*>(p.i) + (MODE == kPacked ? 0 : w.b * p.ib) + f0;
+    T* y = static_cast<T*>(o.y) + (MODE == kPacked ? 0 : w.b * n.Ls * D) + w.d;
+    const bool even_rows = (D & 1) == 0 && (uintptr_t)o.y % (2 * sizeof(T)) == 0;
+    const int turns = ((n.L + kChunk - 1) / kChunk + P - 1) / P;
+    float* ck = o.ckpt ? o.ckpt + w.run * ((n.L + kCkpt - 1) / kCkpt) * D : nullptr;
+    const float2 l = load_state(lam, 0, D, w.d, w.has0, w.has1);
+    const float2 ncs = make_float2(-c * softplus_(l.x), -c * softplus_(l.y));
+    const bool small = __all_sync(kFull, -ncs.x <= kPolyEnd && -ncs.y <= kPolyEnd);
+    const Offset<T, MODE> ox(x, p.xb, p.xt, n.Ls), orr(r, p.rb, p.rt, n.Ls), oi(i, p.ib, p.it, n.Ls);
+    char* mine = rows + w.warp * (3 * S * R::kPitch);
+    auto fetch = [&](int turn) {
+        if (turn < turns) {
+            char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 3>();
+            const int t0 = (turn * P + w.rank) * kChunk + w.warp * S;
+            R::template copy<MODE, S>(at, r, p.rb, p.rt, t0, n, L, width);
+            R::template copy<MODE, S>(at + S * R::kPitch, i, p.ib, p.it, t0, n, L, width);
+            R::template copy<MODE, S>(at + 2 * S * R::kPitch, x, p.xb, p.xt, t0, n, L, width);
+        }
+        cp_commit();
+    };
+    float2 run = MODE == kDense ? load_state(o.h0, w.b, D, w.d, w.has0, w.has1) : f2(0.0f);
+    Seq<MODE> seq{n.cu, (int)n.n, n.Ls, w.b, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < ST - 1; ++k) fetch(k);
     if (CLUSTER) cluster_sync();       // every block of the cluster runs before its shared memory is written to
     for (int turn = 0; turn < turns; ++turn) {
         const int buf = turn & 1;
-        const int chunk = turn * P + rank;
-        const int t0 = chunk * kChunk + warp * S;
-        float2 a[NP], e[NP];
-        {
-            float2 xv[NP], rv[NP], iv[NP];
-            if (MODE == kGroup) seq.at(t0);
-            int64_t sl = seq.s - b;
-            int tl = t0 - seq.beg;
+        const int t0 = (turn * P + w.rank) * kChunk + w.warp * S;
+        fetch(turn + ST - 1);
+        cp_wait<ST - 1>();
+        __syncwarp();
+        const char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 3>();
+        float2 a[S], e[S];
+        float prod = 0.0f;
+#pragma unroll
+        for (int j = 0; j < S; ++j) {
+            const float2 rv = R::read(at + j * R::kPitch, orr.at(t0 + j)), iv = R::read(at + (S + j) * R::kPitch, oi.at(t0 + j));
+            const float2 xv = R::read(at + (2 * S + j) * R::kPitch, ox.at(t0 + j));
+            const Gates g = gates<true>(rv, iv, ncs, prod);
+            a[j] = a_of(g.w);
+            e[j] = mul(mul(m_of(g.w, g.rs), g.si), xv);
+        }
+        if (!__all_sync(kFull, small && prod < kProdEnd)) {
 #pragma unroll
             for (int j = 0; j < S; ++j) {
-                const bool ok = mine && t0 + j < L;
-                const int64_t t = MODE == kGroup ? tl : t0 + j, q = MODE == kGroup ? sl : 0;
-                float row[VEC];
-                load_vec<T, VEC>(r + q * p.rb + t * p.rt, ok, row);
-                put_row<VEC>(rv, j, row);
-                load_vec<T, VEC>(i + q * p.ib + t * p.it, ok, row);
-                put_row<VEC>(iv, j, row);
-                load_vec<T, VEC>(x + q * p.xb + t * p.xt, ok, row);
-                put_row<VEC>(xv, j, row);
-                if (MODE == kGroup && ++tl == n.Ls) {
-                    tl = 0;
-                    ++sl;
-                }
+                const float2 rv = R::read(at + j * R::kPitch, orr.at(t0 + j)), iv = R::read(at + (S + j) * R::kPitch, oi.at(t0 + j));
+                const float2 xv = R::read(at + (2 * S + j) * R::kPitch, ox.at(t0 + j));
+                const Gates g = gates<false>(rv, iv, ncs, prod);
+                a[j] = a_of(g.w);
+                e[j] = mul(mul(m_of(g.w, g.rs), g.si), xv);
             }
-            if (MODE == kPacked && t0 < L) seq.at(t0);
-            if (fast_batch(small, rv, iv)) {
-#pragma unroll
-                for (int k = 0; k < NP; ++k) {
-                    const Gates g = gates<true>(rv[k], iv[k], ncs);
-                    a[k] = __fadd2_rn(g.w, f2(1.0f));
-                    e[k] = __fmul2_rn(__fmul2_rn(m_of(g), g.si), xv[k]);
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < NP; ++k) {
-                    const Gates g = gates<false>(rv[k], iv[k], ncs);
-                    a[k] = __fadd2_rn(g.w, f2(1.0f));
-                    e[k] = __fmul2_rn(__fmul2_rn(m_of(g), g.si), xv[k]);
-                }
-            }
-            if (t0 + S > L)               // tokens past the end change nothing
-#pragma unroll
-                for (int j = 0; j < S; ++j)
-                    if (t0 + j >= L)
-#pragma unroll
-                        for (int v = 0; v < VEC; ++v) {
-                            put<VEC>(a, j, v, 1.0f);
-                            put<VEC>(e, j, v, 0.0f);
-                        }
         }
-        unsigned starts = 0;      // bit j: a sequence starts at token t0 + j (its entering state goes into e)
-        if (CUTS && t0 < L && (seq.beg == t0 || seq.end < t0 + S)) {
+        if (t0 + S > L)                   // tokens past the end change nothing
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+                if (t0 + j >= L) {
+                    a[j] = f2(1.0f);
+                    e[j] = f2(0.0f);
+                }
+        if (CUTS && t0 < L) seq.at(t0);
+        const unsigned starts = starts_in<MODE, S>(seq, t0, L);
+        float2 A = f2(1.0f), H = f2(0.0f);
+        if (CUTS && starts) {
             Seq<MODE> q = seq;
 #pragma unroll
             for (int j = 0; j < S; ++j) {
-                const int t = t0 + j;
-                if (t < L && t == q.end) q.at(t);
-                if (t < L && t == q.beg) {
-                    starts |= 1u << j;
-#pragma unroll
-                    for (int v = 0; v < VEC; ++v)
-                        put<VEC>(e, j, v, fmaf(get<VEC>(a, j, v), o.h0 ? o.h0[q.s * D + dd + v] : 0.0f, get<VEC>(e, j, v)));
-                }
-            }
-        }
-        float A[VEC], H[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            A[v] = 1.0f;
-            H[v] = 0.0f;
-        }
-#pragma unroll
-        for (int j = 0; j < S; ++j) {
-            const bool cut = CUTS && (starts >> j & 1u);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) then<CUTS>(A[v], H[v], cut ? kCut : get<VEC>(a, j, v), get<VEC>(e, j, v));
-        }
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) ex[buf][warp][v][lane] = make_float2(A[v], H[v]);
-        __syncthreads();
-        float preA[VEC], preH[VEC], totA[VEC], totH[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            totA[v] = 1.0f;
-            totH[v] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < kWarps; ++k) {
-                if (k == warp) {
-                    preA[v] = totA[v];
-                    preH[v] = totH[v];
-                }
-                const float2 f = ex[buf][k][v][lane];
-                then<CUTS>(totA[v], totH[v], f.x, f.y);
-            }
-        }
-        float h[VEC];
-        if (CLUSTER) {
-            for (int k = warp; k < P; k += kWarps)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) st_cluster(smem_addr(&pub[buf][rank][v][lane]), k, make_float2(totA[v], totH[v]));
-            cluster_sync();
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                for (int k = 0; k < P; ++k) {
-                    if (k == rank) h[v] = run[v];
-                    const float2 f = pub[buf][k][v][lane];
-                    run[v] = apply<CUTS>(f.x, f.y, run[v]);
+                if (starts >> j & 1u) {   // the sequence's own state enters
+                    q.at(t0 + j);
+                    e[j] = fma(a[j], load_state(o.h0, q.s, D, w.d, w.has0, w.has1), e[j]);
+                    A = f2(kCut);
+                    H = e[j];
+                } else {
+                    then<CUTS>(A, H, a[j], e[j]);
                 }
             }
         } else {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                h[v] = run[v];
-                run[v] = apply<CUTS>(totA[v], totH[v], run[v]);
+            for (int j = 0; j < S; ++j) then<false>(A, H, a[j], e[j]);
+        }
+        ex[buf][w.warp][w.lane] = make_float4(A.x, A.y, H.x, H.y);
+        __syncthreads();
+        float2 h;
+        if (CLUSTER) {
+            float2 tA = f2(1.0f), tH = f2(0.0f);
+            for (int k = 0; k < w.warp; ++k) {
+                const float4 f = ex[buf][k][w.lane];
+                then<CUTS>(tA, tH, make_float2(f.x, f.y), make_float2(f.z, f.w));
+            }
+            const float2 preA = tA, preH = tH;
+            for (int k = w.warp; k < kWarps; ++k) {
+                const float4 f = ex[buf][k][w.lane];
+                then<CUTS>(tA, tH, make_float2(f.x, f.y), make_float2(f.z, f.w));
+            }
+            for (int k = w.warp; k < P; k += kWarps) st_cluster(smem_addr(&pub[buf][w.rank][w.lane]), k, make_float4(tA.x, tA.y, tH.x, tH.y));
+            cluster_sync();
+            for (int k = 0; k < w.rank; ++k) {
+                const float4 f = pub[buf][k][w.lane];
+                run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
+            }
+            h = apply<CUTS>(preA, preH, run);
+            for (int k = w.rank; k < P; ++k) {
+                const float4 f = pub[buf][k][w.lane];
+                run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
+            }
+        } else {
+            for (int k = 0; k < w.warp; ++k) {
+                const float4 f = ex[buf][k][w.lane];
+                run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
+            }
+            h = run;
+            for (int k = w.warp; k < kWarps; ++k) {
+                const float4 f = ex[buf][k][w.lane];
+                run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
             }
         }
+        if (ck && w.warp % (kCkpt / S) == 0 && t0 < L) store_state(ck, t0 / kCkpt, D, w.d, h, w.has0, w.has1);
+        T* out = y + (int64_t)t0 * D;
+        if (!CUTS || (starts == 0 && seq.end > t0 + S)) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) h[v] = apply<CUTS>(preA[v], preH[v], h[v]);
-        if (ck && warp * S % kCkpt == 0 && mine && t0 < L)
+            for (int j = 0; j < S; ++j) {
+                h = fma(a[j], h, e[j]);
+                if (t0 + j < L) store_pair<T, EVEN>(out, h, even_rows, w.has0, w.has1);
+                out += D;
+            }
+        } else {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) ck[(int64_t)(t0 / kCkpt) * D + v] = h[v];
-#pragma unroll
-        for (int j = 0; j < S; ++j) {
-            const int t = t0 + j;
-            const bool cut = CUTS && (starts >> j & 1u);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) h[v] = cut ? get<VEC>(e, j, v) : fmaf(get<VEC>(a, j, v), h[v], get<VEC>(e, j, v));
-            if (mine && t < L) store_vec<T, VEC>(y + (int64_t)t * D, h);
-            if (CUTS && t < L) {
-                if (t == seq.end) seq.at(t);
-                if (t == seq.end - 1 && mine)
-#pragma unroll
-                    for (int v = 0; v < VEC; ++v) o.h_last[seq.s * D + d + v] = h[v];
+            for (int j = 0; j < S; ++j) {
+                const int t = t0 + j;
+                h = starts >> j & 1u ? e[j] : fma(a[j], h, e[j]);
+                if (t < L) {
+                    store_pair<T, EVEN>(out, h, even_rows, w.has0, w.has1);
+                    seq.at(t);
+                    if (t == seq.end - 1) store_state(o.h_last, seq.s, D, w.d, h, w.has0, w.has1);
+                }
+                out += D;
             }
         }
     }
-    if (rank != 0 || !mine) return;
+    if (w.rank != 0) return;
     if (MODE == kDense) {
-        if (warp == 0)
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) o.h_last[b * D + d + v] = run[v];
+        if (w.warp == 0) store_state(o.h_last, w.b, D, w.d, run, w.has0, w.has1);
     } else if (MODE == kPacked) {
-        for (int64_t s = warp; s < n.n; s += kWarps)       // empty sequences keep their state
+        for (int64_t s = w.warp; s < n.n; s += kWarps)       // empty sequences keep their state
             if (n.cu[s] >= n.cu[s + 1])
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) o.h_last[s * D + d + v] = o.h0 ? o.h0[s * D + d + v] : 0.0f;
+                store_state(o.h_last, s, D, w.d, load_state(o.h0, s, D, w.d, w.has0, w.has1), w.has0, w.has1);
     }
 }
 
 // Chunks from the last to the first.  The states that enter a chunk come from
 // the forward; back_t = a_t G_t passes from right to left by the same products
 // of decays, back -> A back + K.
-template <typename T, int VEC, int MODE, bool CLUSTER>
-__global__ void __launch_bounds__(kWarps * 32)
-rec_bwd_kernel(RecPtr p, RecOut o, RecDim n, const float* __restrict__ lam, float c) {
+template <typename T, int MODE, bool EVEN, bool CLUSTER>
+__global__ void __launch_bounds__(kWarps * 32, 2)
+rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut o, const __grid_constant__ RecDim n,
+               const float* __restrict__ lam, float c) {
     constexpr bool CUTS = MODE != kDense;
-    constexpr int kChunk = kChunkBwd, S = kChunk / kWarps, NP = S * VEC / 2;
-    __shared__ float ex[2][kWarps][3][VEC][32];
-    __shared__ float2 pub[CLUSTER ? 2 : 1][CLUSTER ? kMaxCluster : 1][VEC][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int D = n.D, P = n.P, tiles = (D + 32 * VEC - 1) / (32 * VEC);
-    const int rank = CLUSTER ? blockIdx.x % P : 0;
-    const int64_t run_id = blockIdx.x / (CLUSTER ? P : 1) / tiles;
-    const int tile = blockIdx.x / (CLUSTER ? P : 1) - (int)run_id * tiles;
-    // the run's first sequence and its tokens
-    const int64_t b = MODE == kGroup ? run_id * n.per : run_id;
-    const int L = MODE == kGroup ? (int)min((int64_t)n.per, n.n - b) * n.Ls : n.L;
-    const int d = (tile * 32 + lane) * VEC;
-    const bool mine = d < D;
-    const int dd = mine ? d : 0;
-    const T* x = static_cast<const T*>(p.x) + (MODE == kPacked ? 0 : b * p.xb) + dd;
-    const T* r = static_cast<const T*>(p.r) + (MODE == kPacked ? 0 : b * p.rb) + dd;
-    const T* i = static_cast<const T*>(p.i) + (MODE == kPacked ? 0 : b * p.ib) + dd;
-    const T* dy = static_cast<const T*>(p.dy) + (MODE == kPacked ? 0 : b * p.gb) + dd;
-    const bool has_dy = p.dy != nullptr;
-    const int64_t base = (MODE == kPacked ? 0 : b * n.Ls * D) + dd;
+    constexpr int S = kStepsBwd, kChunk = kWarps * S, ST = stages_bwd<T>();
+    using R = Rows<T, EVEN>;
+    __shared__ float4 ex[2][kWarps][32];          // (A, K)
+    __shared__ float2 exh[2][kWarps][32];         // H
+    __shared__ float4 pub[CLUSTER ? 2 : 1][CLUSTER ? kMaxCluster : 1][32];
+    extern __shared__ __align__(16) char rows[];
+    const Place w = place<MODE, CLUSTER>(n);
+    const int D = n.D, L = w.L, P = CLUSTER ? n.P : 1, width = min(kTile, D - w.tile * kTile);
+    const int64_t f0 = (int64_t)w.tile * kTile;
+    const T* x = static_cast<const T*>(p.x) + (MODE == kPacked ? 0 : w.b * p.xb) + f0;
+    const T* r = static_cast<const T*>(p.r) + (MODE == kPacked ? 0 : w.b * p.rb) + f0;
+    const T* i = static_cast<const T*>(p.i) + (MODE == kPacked ? 0 : w.b * p.ib) + f0;
+    // (without dy, rows of no width: zeros)
+    const T* dy = p.dy ? static_cast<const T*>(p.dy) + (MODE == kPacked ? 0 : w.b * p.gb) + f0 : x;
+    const int64_t base = (MODE == kPacked ? 0 : w.b * n.Ls * D) + w.d;
     T* dx = static_cast<T*>(o.dx) + base;
     T* dr = static_cast<T*>(o.dr) + base;
     T* di = static_cast<T*>(o.di) + base;
-    const int chunks = (n.L + kChunk - 1) / kChunk, turns = (chunks + P - 1) / P;   // (of a full run)
-    const float* ck = o.ckpt + run_id * ((n.L + kCkpt - 1) / kCkpt) * D + dd;
-    Seq<MODE> seq{n.cu, (int)n.n, n.Ls, b, 0, 0, 0};
-    float run[VEC];
-    float2 sum = f2(0.0f);
-    const float2 ncs = make_float2(-c * softplus_(lam[dd]), -c * softplus_(lam[dd + VEC - 1]));
+    const bool even_rows = (D & 1) == 0 && ((uintptr_t)o.dx | (uintptr_t)o.dr | (uintptr_t)o.di) % (2 * sizeof(T)) == 0;
+    const int turns = ((n.L + kChunk - 1) / kChunk + P - 1) / P;
+    const float* ck = o.ckpt + w.run * ((n.L + kCkpt - 1) / kCkpt) * D;
+    const float2 l = load_state(lam, 0, D, w.d, w.has0, w.has1);
+    const float2 ncs = make_float2(-c * softplus_(l.x), -c * softplus_(l.y));
     const bool small = __all_sync(kFull, -ncs.x <= kPolyEnd && -ncs.y <= kPolyEnd);
-    if (CUTS) seq.at(L - 1);
+    const Offset<T, MODE> ox(x, p.xb, p.xt, n.Ls), orr(r, p.rb, p.rt, n.Ls), oi(i, p.ib, p.it, n.Ls), og(dy, p.gb, p.gt, n.Ls);
+    char* mine = rows + w.warp * (4 * S * R::kPitch);
+    auto fetch = [&](int turn) {
+        if (turn >= 0) {
+            char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 4>();
+            const int t0 = (turn * P + w.rank) * kChunk + w.warp * S;
+            R::template copy<MODE, S>(at, r, p.rb, p.rt, t0, n, L, width);
+            R::template copy<MODE, S>(at + S * R::kPitch, i, p.ib, p.it, t0, n, L, width);
+            R::template copy<MODE, S>(at + 2 * S * R::kPitch, x, p.xb, p.xt, t0, n, L, width);
+            R::template copy<MODE, S>(at + 3 * S * R::kPitch, dy, p.gb, p.gt, t0, n, L, p.dy ? width : 0);
+        }
+        cp_commit();
+    };
+    Seq<MODE> seq{n.cu, (int)n.n, n.Ls, w.b, 0, 0, 0};
+    seq.at(L - 1);
+    float2 run = load_state(o.dh_last, CUTS ? seq.s : w.b, D, w.d, w.has0, w.has1), sum = f2(0.0f);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-        run[v] = o.dh_last ? o.dh_last[(CUTS ? seq.s : b) * D + dd + v] : 0.0f;
-    }
+    for (int k = 1; k < ST; ++k) fetch(turns - k);
     if (CLUSTER) cluster_sync();
     for (int turn = turns - 1; turn >= 0; --turn) {
         const int buf = turn & 1;
-        const int chunk = turn * P + rank;
-        const int t0 = chunk * kChunk + warp * S;
-        float2 xv[NP], gv[NP], sr[NP], si[NP], w[NP], rs[NP];
-        float enter[VEC];
-        {
-            float2 rv[NP], iv[NP];
-            if (MODE == kGroup) seq.at(t0);
-            int64_t sl = seq.s - b;
-            int tl = t0 - seq.beg;
+        const int chunk = turn * P + w.rank;
+        const int t0 = chunk * kChunk + w.warp * S;
+        fetch(turn - ST + 1);
+        const float2 enter = chunk * kChunk < L ? load_state(ck, chunk, D, w.d, w.has0, w.has1) : f2(0.0f);
+        cp_wait<ST - 1>();
+        __syncwarp();
+        const char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 4>();
+        float2 sr[S], si[S], wv[S], rs[S];
+        float prod = 0.0f;
+#pragma unroll
+        for (int j = 0; j < S; ++j) {
+            const Gates g = gates<true>(R::read(at + j * R::kPitch, orr.at(t0 + j)), R::read(at + (S + j) * R::kPitch, oi.at(t0 + j)), ncs, prod);
+            sr[j] = g.sr; si[j] = g.si; wv[j] = g.w; rs[j] = g.rs;
+        }
+        if (!__all_sync(kFull, small && prod < kProdEnd)) {
 #pragma unroll
             for (int j = 0; j < S; ++j) {
-                const bool ok = mine && t0 + j < L;
-                const int64_t t = MODE == kGroup ? tl : t0 + j, q = MODE == kGroup ? sl : 0;
-                float row[VEC];
-                load_vec<T, VEC>(r + q * p.rb + t * p.rt, ok, row);
-                put_row<VEC>(rv, j, row);
-                load_vec<T, VEC>(i + q * p.ib + t * p.it, ok, row);
-                put_row<VEC>(iv, j, row);
-                load_vec<T, VEC>(x + q * p.xb + t * p.xt, ok, row);
-                put_row<VEC>(xv, j, row);
-                load_vec<T, VEC>(dy + q * p.gb + t * p.gt, ok && has_dy, row);
-                put_row<VEC>(gv, j, row);
-                if (MODE == kGroup && ++tl == n.Ls) {
-                    tl = 0;
-                    ++sl;
-                }
+                const Gates g = gates<false>(R::read(at + j * R::kPitch, orr.at(t0 + j)), R::read(at + (S + j) * R::kPitch, oi.at(t0 + j)), ncs, prod);
+                sr[j] = g.sr; si[j] = g.si; wv[j] = g.w; rs[j] = g.rs;
             }
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) enter[v] = chunk * kChunk < L ? ck[(int64_t)chunk * D + v] : 0.0f;
-            if (MODE == kPacked && t0 < L) seq.at(t0);
-            if (fast_batch(small, rv, iv)) {
-#pragma unroll
-                for (int k = 0; k < NP; ++k) {
-                    const Gates g = gates<true>(rv[k], iv[k], ncs);
-                    sr[k] = g.sr; si[k] = g.si; w[k] = g.w; rs[k] = g.rs;
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < NP; ++k) {
-                    const Gates g = gates<false>(rv[k], iv[k], ncs);
-                    sr[k] = g.sr; si[k] = g.si; w[k] = g.w; rs[k] = g.rs;
-                }
-            }
-            if (t0 + S > L)               // tokens past the end change nothing
-#pragma unroll
-                for (int j = 0; j < S; ++j)
-                    if (t0 + j >= L)
-#pragma unroll
-                        for (int v = 0; v < VEC; ++v) {
-                            put<VEC>(w, j, v, 0.0f);
-                            put<VEC>(rs, j, v, 0.0f);
-                            put<VEC>(sr, j, v, 0.0f);
-                        }
         }
-        float2 a[NP], msi[NP], prev[NP];
+        if (t0 + S > L)                   // tokens past the end change nothing (their x and dy are zero)
 #pragma unroll
-        for (int k = 0; k < NP; ++k) {
-            a[k] = __fadd2_rn(w[k], f2(1.0f));
-            msi[k] = __fmul2_rn(__fmul2_rn(one_minus_a2(w[k]), rs[k]), si[k]);
-            prev[k] = __fmul2_rn(msi[k], xv[k]);        // for now what enters at the token
+            for (int j = 0; j < S; ++j)
+                if (t0 + j >= L) {
+                    wv[j] = f2(0.0f);
+                    rs[j] = f2(0.0f);
+                    sr[j] = f2(0.0f);
+                }
+        float2 xv[S], G[S], a[S], msi[S], prev[S];
+#pragma unroll
+        for (int j = 0; j < S; ++j) {
+            xv[j] = R::read(at + (2 * S + j) * R::kPitch, ox.at(t0 + j));
+            G[j] = R::read(at + (3 * S + j) * R::kPitch, og.at(t0 + j));        // for now dy
+            a[j] = a_of(wv[j]);
+            msi[j] = mul(m_of(wv[j], rs[j]), si[j]);
+            prev[j] = mul(msi[j], xv[j]);                                       // for now what enters at the token
         }
         // forward composition (A, H), backward composition (A, K) of the warp's tokens
-        unsigned starts = 0;
-        if (CUTS && t0 < L && (seq.beg == t0 || seq.end < t0 + S)) {
+        if (CUTS && t0 < L) seq.at(t0);
+        const unsigned starts = starts_in<MODE, S>(seq, t0, L);
+        auto state0 = [&](int t) -> float2 {                // the state that enters the sequence of token t
             Seq<MODE> q = seq;
+            q.at(t);
+            return load_state(o.h0, q.s, D, w.d, w.has0, w.has1);
+        };
+        auto back0 = [&](int t) -> float2 {                 // what enters, from the right, the sequence of token t
+            if (t < 0) return f2(0.0f);
+            Seq<MODE> q = seq;
+            q.at(t);
+            return load_state(o.dh_last, q.s, D, w.d, w.has0, w.has1);
+        };
+        float2 A = f2(1.0f), H = f2(0.0f), K = f2(0.0f);
+        if (CUTS && starts) {
 #pragma unroll
             for (int j = 0; j < S; ++j) {
-                const int t = t0 + j;
-                if (t < L && t == q.end) q.at(t);
-                if (t < L && t == q.beg) starts |= 1u << j;
-            }
-        }
-        auto state0 = [&](int t, int v) -> float {          // the state entering the sequence that starts at t
-            Seq<MODE> q = seq;
-            q.at(t);
-            return o.h0 ? o.h0[q.s * D + dd + v] : 0.0f;
-        };
-        auto back0 = [&](int t, int v) -> float {           // what enters, from the right, the sequence that ends at t
-            if (t < 0) return 0.0f;
-            Seq<MODE> q = seq;
-            q.at(t);
-            return o.dh_last ? o.dh_last[q.s * D + dd + v] : 0.0f;
-        };
-        float A[VEC], H[VEC], K[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            A[v] = 1.0f;
-            H[v] = 0.0f;
-            K[v] = 0.0f;
-        }
-#pragma unroll
-        for (int j = 0; j < S; ++j) {
-            const bool cut = CUTS && (starts >> j & 1u);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float e = get<VEC>(prev, j, v);
-                if (cut) {
-                    A[v] = kCut;
-                    H[v] = fmaf(get<VEC>(a, j, v), state0(t0 + j, v), e);
+                if (starts >> j & 1u) {
+                    A = f2(kCut);
+                    H = fma(a[j], state0(t0 + j), prev[j]);
                 } else {
-                    then<CUTS>(A[v], H[v], get<VEC>(a, j, v), e);
+                    then<CUTS>(A, H, a[j], prev[j]);
                 }
             }
-        }
 #pragma unroll
-        for (int j = S - 1; j >= 0; --j) {
-            const bool cut = CUTS && (starts >> j & 1u);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) K[v] = cut ? back0(t0 + j - 1, v) : get<VEC>(a, j, v) * (get<VEC>(gv, j, v) + K[v]);
-        }
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            ex[buf][warp][0][v][lane] = A[v];
-            ex[buf][warp][1][v][lane] = H[v];
-            ex[buf][warp][2][v][lane] = K[v];
-        }
-        __syncthreads();
-        float sufA[VEC], sufK[VEC], totA[VEC], totK[VEC], h[VEC], back[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            totA[v] = 1.0f;
-            totK[v] = 0.0f;
-#pragma unroll
-            for (int k = kWarps - 1; k >= 0; --k) {
-                if (k == warp) {
-                    sufA[v] = totA[v];
-                    sufK[v] = totK[v];
-                }
-                then<CUTS>(totA[v], totK[v], ex[buf][k][0][v][lane], ex[buf][k][2][v][lane]);
-            }
-            h[v] = enter[v];
-            for (int k = 0; k < warp; ++k) h[v] = apply<CUTS>(ex[buf][k][0][v][lane], ex[buf][k][1][v][lane], h[v]);
-        }
-        if (CLUSTER) {
-            for (int k = warp; k < P; k += kWarps)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) st_cluster(smem_addr(&pub[buf][rank][v][lane]), k, make_float2(totA[v], totK[v]));
-            cluster_sync();
-#pragma unroll
-            for (int v = 0; v < VEC; ++v)
-                for (int k = P - 1; k >= 0; --k) {
-                    if (k == rank) back[v] = run[v];
-                    const float2 f = pub[buf][k][v][lane];
-                    run[v] = apply<CUTS>(f.x, f.y, run[v]);
-                }
+            for (int j = S - 1; j >= 0; --j) K = starts >> j & 1u ? back0(t0 + j - 1) : mul(a[j], add(G[j], K));
         } else {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                back[v] = run[v];
-                run[v] = apply<CUTS>(totA[v], totK[v], run[v]);
+            for (int j = 0; j < S; ++j) then<false>(A, H, a[j], prev[j]);
+#pragma unroll
+            for (int j = S - 1; j >= 0; --j) K = mul(a[j], add(G[j], K));
+        }
+        ex[buf][w.warp][w.lane] = make_float4(A.x, A.y, K.x, K.y);
+        exh[buf][w.warp][w.lane] = H;
+        __syncthreads();
+        float2 h = enter, back;
+        for (int k = 0; k < w.warp; ++k) {
+            const float4 f = ex[buf][k][w.lane];
+            h = apply<CUTS>(make_float2(f.x, f.y), exh[buf][k][w.lane], h);
+        }
+        if (CLUSTER) {
+            float2 tA = f2(1.0f), tK = f2(0.0f);
+            for (int k = kWarps - 1; k > w.warp; --k) {
+                const float4 f = ex[buf][k][w.lane];
+                then<CUTS>(tA, tK, make_float2(f.x, f.y), make_float2(f.z, f.w));
+            }
+            const float2 sufA = tA, sufK = tK;
+            for (int k = w.warp; k >= 0; --k) {
+                const float4 f = ex[buf][k][w.lane];
+                then<CUTS>(tA, tK, make_float2(f.x, f.y), make_float2(f.z, f.w));
+            }
+            for (int k = w.warp; k < P; k += kWarps) st_cluster(smem_addr(&pub[buf][w.rank][w.lane]), k, make_float4(tA.x, tA.y, tK.x, tK.y));
+            cluster_sync();
+            for (int k = P - 1; k > w.rank; --k) {
+                const float4 f = pub[buf][k][w.lane];
+                run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
+            }
+            back = apply<CUTS>(sufA, sufK, run);
+            for (int k = w.rank; k >= 0; --k) {
+                const float4 f = pub[buf][k][w.lane];
+                run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
+            }
+        } else {
+            for (int k = kWarps - 1; k > w.warp; --k) {
+                const float4 f = ex[buf][k][w.lane];
+                run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
+            }
+            back = run;
+            for (int k = w.warp; k >= 0; --k) {
+                const float4 f = ex[buf][k][w.lane];
+                run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
             }
         }
+        if (!CUTS || starts == 0) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) back[v] = apply<CUTS>(sufA[v], sufK[v], back[v]);
+            for (int j = 0; j < S; ++j) {
+                const float2 e = prev[j];
+                prev[j] = h;
+                h = fma(a[j], h, e);
+            }
+#pragma unroll
+            for (int j = S - 1; j >= 0; --j) {
+                G[j] = add(G[j], back);
+                back = mul(a[j], G[j]);                 // (past the end a is 1 and dy 0)
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < S; ++j) {
+                const float2 e = prev[j];
+                if (starts >> j & 1u) h = state0(t0 + j);
+                prev[j] = h;
+                h = fma(a[j], h, e);
+            }
+#pragma unroll
+            for (int j = S - 1; j >= 0; --j) {
+                G[j] = add(G[j], back);
+                back = mul(a[j], G[j]);
+                if (starts >> j & 1u) {
+                    Seq<MODE> q = seq;
+                    q.at(t0 + j);
+                    if (o.dh0) store_state(o.dh0, q.s, D, w.d, back, w.has0, w.has1);
+                    back = back0(t0 + j - 1);
+                }
+            }
+        }
+        const int64_t out = (int64_t)t0 * D;
 #pragma unroll
         for (int j = 0; j < S; ++j) {
-            const bool cut = CUTS && (starts >> j & 1u);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                if (cut) h[v] = state0(t0 + j, v);
-                const float e = get<VEC>(prev, j, v);
-                put<VEC>(prev, j, v, h[v]);
-                h[v] = fmaf(get<VEC>(a, j, v), h[v], e);
-            }
-        }
-#pragma unroll
-        for (int j = S - 1; j >= 0; --j) {              // gv becomes G
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float G = get<VEC>(gv, j, v) + back[v];
-                put<VEC>(gv, j, v, G);
-                back[v] = t0 + j < L ? get<VEC>(a, j, v) * G : back[v];
-            }
-            if (CUTS && (starts >> j & 1u)) {
-                Seq<MODE> q = seq;
-                q.at(t0 + j);
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    if (o.dh0 && mine) o.dh0[q.s * D + d + v] = back[v];
-                    back[v] = back0(t0 + j - 1, v);
-                }
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < NP; ++k) {
-            const float2 G = gv[k];
-            const float2 ox = __fmul2_rn(G, msi[k]);
-            const float2 oi = __fmul2_rn(__fmul2_rn(ox, xv[k]), __ffma2_rn(si[k], f2(-1.0f), f2(1.0f)));
+            const float2 vx = mul(G[j], msi[j]);
+            const float2 vi = mul(mul(vx, xv[j]), fma(si[j], f2(-1.0f), f2(1.0f)));
             // du = G a (prev - (a / m) sigmoid(i) x)
-            const float2 slope = __fmul2_rn(__fmul2_rn(a[k], rs[k]), __fmul2_rn(si[k], xv[k]));
-            const float2 du = __fmul2_rn(__fmul2_rn(G, a[k]), __ffma2_rn(slope, f2(-1.0f), prev[k]));
-            const float2 ds = __fmul2_rn(du, sr[k]);
-            sum = __fadd2_rn(sum, ds);
-            const float2 orr = __fmul2_rn(__fmul2_rn(ds, ncs), __ffma2_rn(sr[k], f2(-1.0f), f2(1.0f)));
-#pragma unroll
-            for (int half = 0; half < 2 / VEC; ++half) {
-                const int t = t0 + (VEC == 2 ? k : 2 * k + half);
-                if (mine && t < L) {
-                    float vx[VEC], vr[VEC], vi[VEC];
-#pragma unroll
-                    for (int v = 0; v < VEC; ++v) {
-                        const bool y = VEC == 2 ? v : half;
-                        vx[v] = y ? ox.y : ox.x;
-                        vr[v] = y ? orr.y : orr.x;
-                        vi[v] = y ? oi.y : oi.x;
-                    }
-                    store_vec<T, VEC>(dx + (int64_t)t * D, vx);
-                    store_vec<T, VEC>(dr + (int64_t)t * D, vr);
-                    store_vec<T, VEC>(di + (int64_t)t * D, vi);
-                }
+            const float2 slope = mul(mul(a[j], rs[j]), mul(si[j], xv[j]));
+            const float2 du = mul(mul(G[j], a[j]), fma(slope, f2(-1.0f), prev[j]));
+            const float2 ds = mul(du, sr[j]);
+            const float2 vr = mul(mul(ds, ncs), fma(sr[j], f2(-1.0f), f2(1.0f)));
+            if (t0 + j < L) {
+                sum = add(sum, ds);
+                store_pair<T, EVEN>(dx + out + (int64_t)j * D, vx, even_rows, w.has0, w.has1);
+                store_pair<T, EVEN>(dr + out + (int64_t)j * D, vr, even_rows, w.has0, w.has1);
+                store_pair<T, EVEN>(di + out + (int64_t)j * D, vi, even_rows, w.has0, w.has1);
             }
         }
     }
     __syncthreads();
-    float* red = &ex[0][0][0][0][0];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) red[(warp * VEC + v) * 32 + lane] = VEC == 2 ? (v ? sum.y : sum.x) : sum.x + sum.y;
+    exh[0][w.warp][w.lane] = sum;
     __syncthreads();
-    if (warp == 0 && mine)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            float s = 0.0f;
-            for (int k = 0; k < kWarps; ++k) s += red[(k * VEC + v) * 32 + lane];
-            o.part[(run_id * P + rank) * D + d + v] = s;
-        }
-    if (rank != 0 || !mine || !o.dh0) return;
+    if (w.warp == 0) {
+        float2 s = f2(0.0f);
+        for (int k = 0; k < kWarps; ++k) s = add(s, exh[0][k][w.lane]);
+        store_state(o.part, w.run * P + w.rank, D, w.d, s, w.has0, w.has1);
+    }
+    if (w.rank != 0 || !o.dh0) return;
     if (MODE == kDense) {
-        if (warp == 0)
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) o.dh0[b * D + d + v] = run[v];
+        if (w.warp == 0) store_state(o.dh0, w.b, D, w.d, run, w.has0, w.has1);
     } else if (MODE == kPacked) {
-        for (int64_t s = warp; s < n.n; s += kWarps)
+        for (int64_t s = w.warp; s < n.n; s += kWarps)
             if (n.cu[s] >= n.cu[s + 1])
-#pragma unroll
-                for (int v = 0; v < VEC; ++v)
-                    o.dh0[s * D + d + v] = o.dh_last ? o.dh_last[s * D + d + v] : 0.0f;
+                store_state(o.dh0, s, D, w.d, load_state(o.dh_last, s, D, w.d, w.has0, w.has1), w.has0, w.has1);
     }
 }
 
-// dlam[d] = -c sigmoid(lam[d]) * sum of the partials of feature d, in order.
-__global__ void rec_dlam_kernel(const float* __restrict__ part, int64_t n, int64_t D, const float* __restrict__ lam, float c,
-                                float* __restrict__ dlam) {
-    const int64_t d = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (d >= D) return;
+// dlam[d] = -c sigmoid(lam[d]) * sum of the n partials of feature d: a block takes
+// 32 features, a warp every 32nd partial, then the warps' sums in order.
+__global__ void __launch_bounds__(1024)
+rec_dlam_kernel(const float* __restrict__ part, int64_t n, int64_t D, const float* __restrict__ lam, float c, float* __restrict__ dlam) {
+    __shared__ float sums[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t d = (int64_t)blockIdx.x * 32 + lane;
     float s = 0.0f;
-    for (int64_t k = 0; k < n; ++k) s += part[k * D + d];
+    if (d < D)
+        for (int64_t k = warp; k < n; k += 32) s += part[k * D + d];
+    sums[warp][lane] = s;
+    __syncthreads();
+    if (warp != 0 || d >= D) return;
+    s = 0.0f;
+    for (int k = 0; k < 32; ++k) s += sums[k][lane];
     dlam[d] = -c * sigmoid_(lam[d]) * s;
 }
 
@@ -737,9 +775,10 @@ __global__ void rec_step_kernel(RecPtr p, int64_t B, int64_t D, const float* __r
     const int64_t n = B * D, stride = (int64_t)gridDim.x * blockDim.x;
     for (int64_t k = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; k < n; k += stride) {
         const int64_t b = k / D, d = k - b * D;
+        float prod;
         const Gates g = gates<false>(f2(to_f32<T>(static_cast<const T*>(p.r)[b * p.rb + d])),
-                                     f2(to_f32<T>(static_cast<const T*>(p.i)[b * p.ib + d])), f2(-c * softplus_(lam[d])));
-        const float v = fmaf(1.0f + g.w.x, h[k], m_of(g).x * g.si.x * to_f32<T>(static_cast<const T*>(p.x)[b * p.xb + d]));
+                                     f2(to_f32<T>(static_cast<const T*>(p.i)[b * p.ib + d])), f2(-c * softplus_(lam[d])), prod);
+        const float v = fmaf(1.0f + g.w.x, h[k], m_of(g.w, g.rs).x * g.si.x * to_f32<T>(static_cast<const T*>(p.x)[b * p.xb + d]));
         h[k] = v;
         y[k] = from_f32<T>(v);
     }
@@ -770,59 +809,53 @@ int64_t rec_parts(int64_t L, int part) { return (L + part - 1) / part; }
 
 // How the tokens are dealt out.  It goes by sizes alone: forward and backward have to agree on the runs.
 struct Plan {
-    int mode, per, L, vec, P;
-    int64_t runs;
+    int mode, per, L, P;
+    int64_t runs, tiles;
 };
 
-Plan rec_plan(const bcm_gated_rec_args* a, int vec) {
-    Plan pl = {kDense, 1, (int)a->seqlen, vec, 1, a->batch};
-    // in units of the widest tile, so that the runs do not depend on alignment
-    const int64_t wide = (a->dim + 63) / 64, tiles = (a->dim + 32 * vec - 1) / (32 * vec);
+Plan rec_plan(const bcm_gated_rec_args* a) {
+    constexpr int kChunk = kWarps * kStepsFwd;
+    Plan pl = {kDense, 1, (int)a->seqlen, 1, a->batch, rec_parts(a->dim, kTile)};
     if (a->cu_seqlens) {
         pl.mode = kPacked;
         pl.runs = 1;
-    } else if (a->seqlen < 4 * kChunkFwd && a->batch > 1) {
+    } else if (a->seqlen < 4 * kChunk && a->batch > 1) {
         // runs of about 8 chunks (an eighth of the last one empty at most), fewer where that leaves SMs without a block
         pl.mode = kGroup;
-        int64_t per = (8 * kChunkFwd + a->seqlen - 1) / a->seqlen;
-        while (per > 1 && per * a->seqlen > kChunkFwd && ((a->batch + per - 1) / per) * wide < 4 * (int64_t)sm_count()) per = (per + 1) / 2;
+        int64_t per = (8 * kChunk + a->seqlen - 1) / a->seqlen;
+        while (per > 1 && per * a->seqlen > kChunk && rec_parts(a->batch, (int)per) * pl.tiles < 4 * (int64_t)sm_count()) per = (per + 1) / 2;
         pl.per = (int)std::min<int64_t>(per, a->batch);
         pl.L = (int)(pl.per * a->seqlen);
-        pl.runs = (a->batch + pl.per - 1) / pl.per;
+        pl.runs = rec_parts(a->batch, pl.per);
     }
-    // blocks of a cluster: as many as the chunks allow until the GPU holds three blocks per SM
-    while (pl.P < kMaxCluster && pl.runs * tiles * pl.P < 3 * (int64_t)sm_count() && 2 * pl.P <= rec_parts(pl.L, kChunkFwd)) pl.P *= 2;
+    // blocks of a cluster: as many as the chunks allow until the GPU holds its two blocks per SM
+    while (pl.P < kMaxCluster && pl.runs * pl.tiles * pl.P < 2 * (int64_t)sm_count() && 2 * pl.P <= rec_parts(pl.L, kChunk)) pl.P *= 2;
     return pl;
 }
 
-// Two features a lane where rows are even and aligned for it.
-int rec_vec(const bcm_gated_rec_args* a, bool bwd) {
-    const size_t s = 2 * dtype_size(a->dtype);
-    int64_t odd = a->dim;
-    uintptr_t at = 0;
+// Whether every row of every input starts on 16 bytes (and the outputs' rows on two features).
+bool rec_even(const bcm_gated_rec_args* a, bool bwd) {
+    const int64_t s = (int64_t)dtype_size(a->dtype);
+    int64_t bits = 0;
     auto see = [&](const void* p, int64_t sb, int64_t st) {
-        at |= (uintptr_t)p;
-        odd |= (a->cu_seqlens || a->batch == 1 ? 0 : sb) | (a->seqlen == 1 ? 0 : st);
+        bits |= (int64_t)(uintptr_t)p | (a->cu_seqlens || a->batch == 1 ? 0 : sb * s) | (a->seqlen == 1 ? 0 : st * s);
     };
     see(a->x, a->x_stride_b, a->x_stride_t);
     see(a->r, a->r_stride_b, a->r_stride_t);
     see(a->i, a->i_stride_b, a->i_stride_t);
-    if (bwd) {
-        if (a->dy) see(a->dy, a->dy_stride_b, a->dy_stride_t);
-        at |= (uintptr_t)a->dx | (uintptr_t)a->dr | (uintptr_t)a->di;
-    } else {
-        at |= (uintptr_t)a->y;
-    }
-    return (odd & 1) == 0 && at % s == 0 ? 2 : 1;
+    if (bwd && a->dy) see(a->dy, a->dy_stride_b, a->dy_stride_t);
+    bits |= (int64_t)(bwd ? (uintptr_t)a->dx | (uintptr_t)a->dr | (uintptr_t)a->di : (uintptr_t)a->y);
+    return (bits & 15) == 0 && a->dim % 2 == 0;
 }
 
 template <typename F>
-bcm_status rec_launch_as(F* kernel, const bcm_gated_rec_args* a, const RecOut& o, const Plan& pl, cudaStream_t stream) {
-    const int64_t blocks = ((a->dim + 32 * pl.vec - 1) / (32 * pl.vec)) * pl.runs * pl.P;
+bcm_status rec_launch_as(F* kernel, int smem, const bcm_gated_rec_args* a, const RecOut& o, const Plan& pl, cudaStream_t stream) {
+    const int64_t blocks = pl.tiles * pl.runs * pl.P;
     BCM_REQUIRE(blocks < (1ll << 31), "gated_rec: batch x dim too large");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);
     cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -831,35 +864,38 @@ bcm_status rec_launch_as(F* kernel, const bcm_gated_rec_args* a, const RecOut& o
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pl.P > 1 ? 1 : 0;
+    BCM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     if (pl.P > 8) BCM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     const RecDim n = {a->cu_seqlens, a->batch, pl.L, (int)a->seqlen, pl.per, (int)a->dim, pl.P};
     BCM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, rec_ptr(a), o, n, a->lam, a->decay_scale));
     return BCM_OK;
 }
 
-template <bool BWD, typename T, int VEC, int MODE>
+template <bool BWD, typename T, int MODE, bool EVEN>
 bcm_status rec_launch_p(const bcm_gated_rec_args* a, const RecOut& o, const Plan& pl, cudaStream_t stream) {
     if constexpr (BWD) {
-        return pl.P > 1 ? rec_launch_as(rec_bwd_kernel<T, VEC, MODE, true>, a, o, pl, stream)
-                        : rec_launch_as(rec_bwd_kernel<T, VEC, MODE, false>, a, o, pl, stream);
+        constexpr int smem = stages_bwd<T>() * stage_bytes<T, kStepsBwd, EVEN, 4>();
+        return pl.P > 1 ? rec_launch_as(rec_bwd_kernel<T, MODE, EVEN, true>, smem, a, o, pl, stream)
+                        : rec_launch_as(rec_bwd_kernel<T, MODE, EVEN, false>, smem, a, o, pl, stream);
     } else {
-        return pl.P > 1 ? rec_launch_as(rec_fwd_kernel<T, VEC, MODE, true>, a, o, pl, stream)
-                        : rec_launch_as(rec_fwd_kernel<T, VEC, MODE, false>, a, o, pl, stream);
+        constexpr int smem = stages_fwd<T>() * stage_bytes<T, kStepsFwd, EVEN, 3>();
+        return pl.P > 1 ? rec_launch_as(rec_fwd_kernel<T, MODE, EVEN, true>, smem, a, o, pl, stream)
+                        : rec_launch_as(rec_fwd_kernel<T, MODE, EVEN, false>, smem, a, o, pl, stream);
     }
 }
 
-template <bool BWD, typename T, int VEC>
-bcm_status rec_launch_v(const bcm_gated_rec_args* a, const RecOut& o, const Plan& pl, cudaStream_t stream) {
-    if (pl.mode == kDense) return rec_launch_p<BWD, T, VEC, kDense>(a, o, pl, stream);
-    if (pl.mode == kGroup) return rec_launch_p<BWD, T, VEC, kGroup>(a, o, pl, stream);
-    return rec_launch_p<BWD, T, VEC, kPacked>(a, o, pl, stream);
+template <bool BWD, typename T, bool EVEN>
+bcm_status rec_launch_m(const bcm_gated_rec_args* a, const RecOut& o, const Plan& pl, cudaStream_t stream) {
+    if (pl.mode == kDense) return rec_launch_p<BWD, T, kDense, EVEN>(a, o, pl, stream);
+    if (pl.mode == kGroup) return rec_launch_p<BWD, T, kGroup, EVEN>(a, o, pl, stream);
+    return rec_launch_p<BWD, T, kPacked, EVEN>(a, o, pl, stream);
 }
 
 template <bool BWD>
 bcm_status rec_launch(const bcm_gated_rec_args* a, const RecOut& o, const Plan& pl, cudaStream_t stream) {
     return dispatch_dtype(a->dtype, [&](auto tag) -> bcm_status {
         using T = decltype(tag);
-        return pl.vec == 2 ? rec_launch_v<BWD, T, 2>(a, o, pl, stream) : rec_launch_v<BWD, T, 1>(a, o, pl, stream);
+        return rec_even(a, BWD) ? rec_launch_m<BWD, T, true>(a, o, pl, stream) : rec_launch_m<BWD, T, false>(a, o, pl, stream);
     });
 }
 
@@ -871,14 +907,14 @@ using namespace bcm;
 extern "C" size_t bcm_gated_rec_ckpt_bytes(const bcm_gated_rec_args* a) {
     if (!a || a->batch < 0 || a->seqlen < 0 || a->dim < 1) return 0;
     if (rec_rows(a) == 0) return 0;
-    const Plan pl = rec_plan(a, 1);
+    const Plan pl = rec_plan(a);
     return align_up((size_t)pl.runs * (size_t)rec_parts(pl.L, kCkpt) * (size_t)a->dim * sizeof(float), 256);
 }
 
 extern "C" size_t bcm_gated_rec_bwd_workspace_bytes(const bcm_gated_rec_args* a) {
     if (!a || a->batch < 0 || a->seqlen < 0 || a->dim < 1) return 0;
     if (rec_rows(a) == 0) return 0;
-    const Plan pl = rec_plan(a, 2);         // one lane a feature takes no more blocks to a cluster than two
+    const Plan pl = rec_plan(a);
     return align_up((size_t)pl.runs * (size_t)pl.P * (size_t)a->dim * sizeof(float), 256);
 }
 
@@ -899,7 +935,7 @@ extern "C" bcm_status bcm_gated_rec_fwd(const bcm_gated_rec_args* a, cudaStream_
     }
     RecOut o = {};
     o.h0 = a->h0; o.y = a->y; o.h_last = a->h_last; o.ckpt = static_cast<float*>(a->ckpt);
-    return rec_launch<false>(a, o, rec_plan(a, rec_vec(a, false)), stream);
+    return rec_launch<false>(a, o, rec_plan(a), stream);
 }
 
 extern "C" bcm_status bcm_gated_rec_bwd(const bcm_gated_rec_args* a, cudaStream_t stream) {
@@ -924,9 +960,9 @@ extern "C" bcm_status bcm_gated_rec_bwd(const bcm_gated_rec_args* a, cudaStream_
     o.h0 = a->h0; o.ckpt = static_cast<float*>(a->ckpt);
     o.dh_last = a->dh_last; o.dx = a->dx; o.dr = a->dr; o.di = a->di;
     o.part = static_cast<float*>(a->workspace); o.dh0 = a->dh0;
-    const Plan pl = rec_plan(a, rec_vec(a, true));
+    const Plan pl = rec_plan(a);
     if (bcm_status st = rec_launch<true>(a, o, pl, stream); st != BCM_OK) return st;
-    rec_dlam_kernel<<<(unsigned)ceil_div(a->dim, 128), 128, 0, stream>>>(o.part, pl.runs * pl.P, a->dim, a->lam, a->decay_scale,
+    rec_dlam_kernel<<<(unsigned)ceil_div(a->dim, 32), 1024, 0, stream>>>(o.part, pl.runs * pl.P, a->dim, a->lam, a->decay_scale,
                                                                         a->dlam);
     BCM_LAUNCH_CHECK();
     return BCM_OK;

@@ -82,6 +82,14 @@ def test_many_short_and_one_long(B, L, D):
     _check(_inputs(B * L, D, B, torch.float32, seed=B + L), range(0, B * L + 1, L), (B, L))
 
 
+@pytest.mark.parametrize("D", [63, 66, 129, 1001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_rows_off_16_bytes(D, dtype):
+    _check(_inputs(3 * 300, D, 3, dtype, seed=D), (0, 300, 600, 900), (3, 300))
+    _check(_inputs(300, D, 4, dtype, seed=D), (0, 7, 7, 200, 300), None)
+    _check(_inputs(40 * 7, D, 40, dtype, seed=D), range(0, 281, 7), (40, 7))
+
+
 def test_half():
     _check(_inputs(2 * 300, 70, 2, torch.float16, seed=3), (0, 300, 600), (2, 300))
 

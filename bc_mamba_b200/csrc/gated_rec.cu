@@ -259,19 +259,50 @@ struct Rows {
     }
 };
 
-// The granule offset of the rows t0 .. of one array; rows of a run advance by a constant number of bytes (kDense, kPacked).
-template <typename T, int MODE>
-struct Offset {
-    uint32_t first, step, wrap;
-    int Ls;
-    __device__ __forceinline__ Offset(const T* base, int64_t sb, int64_t st, int Ls_)
-        : first((uint32_t)(uintptr_t)base), step((uint32_t)(st * sizeof(T))), wrap((uint32_t)(sb * sizeof(T))), Ls(Ls_) {}
-    __device__ __forceinline__ int at(int t) const {
-        if (MODE == kGroup) {
-            const int k = t / Ls;
-            return (int)((first + k * wrap + (uint32_t)(t - k * Ls) * step) & 15u);
+// One input of a warp: fetches S rows a turn, reads them back.  LINEAR (kDense, kPacked, and kGroup where a sequence
+// follows the one before it at once): rows of a run lie st elements apart.
+template <typename T, int MODE, bool EVEN, int S>
+struct Stream {
+    using R = Rows<T, EVEN>;
+    static constexpr int kLaneRows = 32 / R::kGran;      // rows of a warp's copy instruction (EVEN)
+    const T* base;
+    int64_t sb, st;
+    const char* at;                                      // EVEN: the lane's granule in the rows of the next fetch
+    int bytes, width;
+    bool linear;
+    __device__ __forceinline__ Stream(const T* base_, int64_t sb_, int64_t st_, const RecDim& n, int t0, int width_)
+        : base(base_), sb(sb_), st(st_), width(width_) {
+        const int lane = threadIdx.x & 31, g = EVEN ? lane % R::kGran : 0, row = EVEN ? lane / R::kGran : 0;
+        linear = MODE != kGroup || sb == st * n.Ls;
+        at = reinterpret_cast<const char*>(base + (t0 + row) * st) + g * 16;
+        bytes = max(0, min(16, width * (int)sizeof(T) - g * 16));
+    }
+    // t0: the first row; advance: tokens from this fetch to the next
+    __device__ __forceinline__ void fetch(char* dst, int t0, int advance, const RecDim& n, int L) {
+        if (EVEN && linear && t0 + S <= L) {
+            const uint32_t to = smem_addr(dst) + (threadIdx.x & 31) * 16;
+#pragma unroll
+            for (int k = 0; k < S / kLaneRows; ++k)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * 512), "l"(at + (int64_t)(k * kLaneRows) * st * (int)sizeof(T)),
+                             "r"(bytes)
+                             : "memory");
+        } else {
+            R::template copy<MODE, S>(dst, base, sb, st, t0, n, L, width);
         }
-        return (int)((first + (uint32_t)t * step) & 15u);
+        if (EVEN) at += (int64_t)advance * st * (int)sizeof(T);
+    }
+    // the lane's two features of token t, row j of the fetched ones
+    __device__ __forceinline__ float2 read(const char* from, int j, int t, const RecDim& n) const {
+        uint32_t off = 0;
+        if (!EVEN) {
+            uint32_t e = (uint32_t)t * (uint32_t)st;
+            if (MODE == kGroup) {
+                const int k = t / n.Ls;
+                e = k * (uint32_t)sb + (uint32_t)(t - k * n.Ls) * (uint32_t)st;
+            }
+            off = ((uint32_t)(uintptr_t)base + e * (uint32_t)sizeof(T)) & 15u;
+        }
+        return R::read(from + j * R::kPitch, (int)off);
     }
 };
 
@@ -377,15 +408,16 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
     const float2 l = load_state(lam, 0, D, w.d, w.has0, w.has1);
     const float2 ncs = make_float2(-c * softplus_(l.x), -c * softplus_(l.y));
     const bool small = __all_sync(kFull, -ncs.x <= kPolyEnd && -ncs.y <= kPolyEnd);
-    const Offset<T, MODE> ox(x, p.xb, p.xt, n.Ls), orr(r, p.rb, p.rt, n.Ls), oi(i, p.ib, p.it, n.Ls);
+    const int first = w.rank * kChunk + w.warp * S;
+    Stream<T, MODE, EVEN, S> sx(x, p.xb, p.xt, n, first, width), sr(r, p.rb, p.rt, n, first, width), si(i, p.ib, p.it, n, first, width);
     char* mine = rows + w.warp * (3 * S * R::kPitch);
     auto fetch = [&](int turn) {
         if (turn < turns) {
             char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 3>();
-            const int t0 = (turn * P + w.rank) * kChunk + w.warp * S;
-            R::template copy<MODE, S>(at, r, p.rb, p.rt, t0, n, L, width);
-            R::template copy<MODE, S>(at + S * R::kPitch, i, p.ib, p.it, t0, n, L, width);
-            R::template copy<MODE, S>(at + 2 * S * R::kPitch, x, p.xb, p.xt, t0, n, L, width);
+            const int t0 = turn * P * kChunk + first;
+            sr.fetch(at, t0, P * kChunk, n, L);
+            si.fetch(at + S * R::kPitch, t0, P * kChunk, n, L);
+            sx.fetch(at + 2 * S * R::kPitch, t0, P * kChunk, n, L);
         }
         cp_commit();
     };
@@ -405,8 +437,7 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         float prod = 0.0f;
 #pragma unroll
         for (int j = 0; j < S; ++j) {
-            const float2 rv = R::read(at + j * R::kPitch, orr.at(t0 + j)), iv = R::read(at + (S + j) * R::kPitch, oi.at(t0 + j));
-            const float2 xv = R::read(at + (2 * S + j) * R::kPitch, ox.at(t0 + j));
+            const float2 rv = sr.read(at, j, t0 + j, n), iv = si.read(at, S + j, t0 + j, n), xv = sx.read(at, 2 * S + j, t0 + j, n);
             const Gates g = gates<true>(rv, iv, ncs, prod);
             a[j] = a_of(g.w);
             e[j] = mul(mul(m_of(g.w, g.rs), g.si), xv);
@@ -414,8 +445,7 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         if (!__all_sync(kFull, small && prod < kProdEnd)) {
 #pragma unroll
             for (int j = 0; j < S; ++j) {
-                const float2 rv = R::read(at + j * R::kPitch, orr.at(t0 + j)), iv = R::read(at + (S + j) * R::kPitch, oi.at(t0 + j));
-                const float2 xv = R::read(at + (2 * S + j) * R::kPitch, ox.at(t0 + j));
+                const float2 rv = sr.read(at, j, t0 + j, n), iv = si.read(at, S + j, t0 + j, n), xv = sx.read(at, 2 * S + j, t0 + j, n);
                 const Gates g = gates<false>(rv, iv, ncs, prod);
                 a[j] = a_of(g.w);
                 e[j] = mul(mul(m_of(g.w, g.rs), g.si), xv);
@@ -486,11 +516,11 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         }
         if (ck && w.warp % (kCkpt / S) == 0 && t0 < L) store_state(ck, t0 / kCkpt, D, w.d, h, w.has0, w.has1);
         T* out = y + (int64_t)t0 * D;
-        if (!CUTS || (starts == 0 && seq.end > t0 + S)) {
+        if (t0 + S <= L && (!CUTS || (starts == 0 && seq.end > t0 + S))) {
 #pragma unroll
             for (int j = 0; j < S; ++j) {
                 h = fma(a[j], h, e[j]);
-                if (t0 + j < L) store_pair<T, EVEN>(out, h, even_rows, w.has0, w.has1);
+                store_pair<T, EVEN>(out, h, even_rows, w.has0, w.has1);
                 out += D;
             }
         } else {
@@ -500,8 +530,8 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
                 h = starts >> j & 1u ? e[j] : fma(a[j], h, e[j]);
                 if (t < L) {
                     store_pair<T, EVEN>(out, h, even_rows, w.has0, w.has1);
-                    seq.at(t);
-                    if (t == seq.end - 1) store_state(o.h_last, seq.s, D, w.d, h, w.has0, w.has1);
+                    if (CUTS) seq.at(t);
+                    if (CUTS && t == seq.end - 1) store_state(o.h_last, seq.s, D, w.d, h, w.has0, w.has1);
                 }
                 out += D;
             }
@@ -549,16 +579,18 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
     const float2 l = load_state(lam, 0, D, w.d, w.has0, w.has1);
     const float2 ncs = make_float2(-c * softplus_(l.x), -c * softplus_(l.y));
     const bool small = __all_sync(kFull, -ncs.x <= kPolyEnd && -ncs.y <= kPolyEnd);
-    const Offset<T, MODE> ox(x, p.xb, p.xt, n.Ls), orr(r, p.rb, p.rt, n.Ls), oi(i, p.ib, p.it, n.Ls), og(dy, p.gb, p.gt, n.Ls);
+    const int first = w.rank * kChunk + w.warp * S, last = (turns - 1) * P * kChunk + first;
+    Stream<T, MODE, EVEN, S> sx(x, p.xb, p.xt, n, last, width), sr(r, p.rb, p.rt, n, last, width), si(i, p.ib, p.it, n, last, width),
+        sg(dy, p.gb, p.gt, n, last, p.dy ? width : 0);
     char* mine = rows + w.warp * (4 * S * R::kPitch);
     auto fetch = [&](int turn) {
         if (turn >= 0) {
             char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 4>();
-            const int t0 = (turn * P + w.rank) * kChunk + w.warp * S;
-            R::template copy<MODE, S>(at, r, p.rb, p.rt, t0, n, L, width);
-            R::template copy<MODE, S>(at + S * R::kPitch, i, p.ib, p.it, t0, n, L, width);
-            R::template copy<MODE, S>(at + 2 * S * R::kPitch, x, p.xb, p.xt, t0, n, L, width);
-            R::template copy<MODE, S>(at + 3 * S * R::kPitch, dy, p.gb, p.gt, t0, n, L, p.dy ? width : 0);
+            const int t0 = turn * P * kChunk + first;
+            sr.fetch(at, t0, -P * kChunk, n, L);
+            si.fetch(at + S * R::kPitch, t0, -P * kChunk, n, L);
+            sx.fetch(at + 2 * S * R::kPitch, t0, -P * kChunk, n, L);
+            sg.fetch(at + 3 * S * R::kPitch, t0, -P * kChunk, n, L);
         }
         cp_commit();
     };
@@ -577,18 +609,18 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         cp_wait<ST - 1>();
         __syncwarp();
         const char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 4>();
-        float2 sr[S], si[S], wv[S], rs[S];
+        float2 sgr[S], sgi[S], wv[S], rs[S];
         float prod = 0.0f;
 #pragma unroll
         for (int j = 0; j < S; ++j) {
-            const Gates g = gates<true>(R::read(at + j * R::kPitch, orr.at(t0 + j)), R::read(at + (S + j) * R::kPitch, oi.at(t0 + j)), ncs, prod);
-            sr[j] = g.sr; si[j] = g.si; wv[j] = g.w; rs[j] = g.rs;
+            const Gates g = gates<true>(sr.read(at, j, t0 + j, n), si.read(at, S + j, t0 + j, n), ncs, prod);
+            sgr[j] = g.sr; sgi[j] = g.si; wv[j] = g.w; rs[j] = g.rs;
         }
         if (!__all_sync(kFull, small && prod < kProdEnd)) {
 #pragma unroll
             for (int j = 0; j < S; ++j) {
-                const Gates g = gates<false>(R::read(at + j * R::kPitch, orr.at(t0 + j)), R::read(at + (S + j) * R::kPitch, oi.at(t0 + j)), ncs, prod);
-                sr[j] = g.sr; si[j] = g.si; wv[j] = g.w; rs[j] = g.rs;
+                const Gates g = gates<false>(sr.read(at, j, t0 + j, n), si.read(at, S + j, t0 + j, n), ncs, prod);
+                sgr[j] = g.sr; sgi[j] = g.si; wv[j] = g.w; rs[j] = g.rs;
             }
         }
         if (t0 + S > L)                   // tokens past the end change nothing (their x and dy are zero)
@@ -597,15 +629,15 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
                 if (t0 + j >= L) {
                     wv[j] = f2(0.0f);
                     rs[j] = f2(0.0f);
-                    sr[j] = f2(0.0f);
+                    sgr[j] = f2(0.0f);
                 }
         float2 xv[S], G[S], a[S], msi[S], prev[S];
 #pragma unroll
         for (int j = 0; j < S; ++j) {
-            xv[j] = R::read(at + (2 * S + j) * R::kPitch, ox.at(t0 + j));
-            G[j] = R::read(at + (3 * S + j) * R::kPitch, og.at(t0 + j));        // for now dy
+            xv[j] = sx.read(at, 2 * S + j, t0 + j, n);
+            G[j] = sg.read(at, 3 * S + j, t0 + j, n);        // for now dy
             a[j] = a_of(wv[j]);
-            msi[j] = mul(m_of(wv[j], rs[j]), si[j]);
+            msi[j] = mul(m_of(wv[j], rs[j]), sgi[j]);
             prev[j] = mul(msi[j], xv[j]);                                       // for now what enters at the token
         }
         // forward composition (A, H), backward composition (A, K) of the warp's tokens
@@ -714,22 +746,26 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
                 }
             }
         }
-        const int64_t out = (int64_t)t0 * D;
+        T *px = dx + (int64_t)t0 * D, *pr = dr + (int64_t)t0 * D, *pi = di + (int64_t)t0 * D;
+        const bool full = t0 + S <= L;
 #pragma unroll
         for (int j = 0; j < S; ++j) {
             const float2 vx = mul(G[j], msi[j]);
-            const float2 vi = mul(mul(vx, xv[j]), fma(si[j], f2(-1.0f), f2(1.0f)));
+            const float2 vi = mul(mul(vx, xv[j]), fma(sgi[j], f2(-1.0f), f2(1.0f)));
             // du = G a (prev - (a / m) sigmoid(i) x)
-            const float2 slope = mul(mul(a[j], rs[j]), mul(si[j], xv[j]));
+            const float2 slope = mul(mul(a[j], rs[j]), mul(sgi[j], xv[j]));
             const float2 du = mul(mul(G[j], a[j]), fma(slope, f2(-1.0f), prev[j]));
-            const float2 ds = mul(du, sr[j]);
-            const float2 vr = mul(mul(ds, ncs), fma(sr[j], f2(-1.0f), f2(1.0f)));
-            if (t0 + j < L) {
+            const float2 ds = mul(du, sgr[j]);
+            const float2 vr = mul(mul(ds, ncs), fma(sgr[j], f2(-1.0f), f2(1.0f)));
+            if (full || t0 + j < L) {
                 sum = add(sum, ds);
-                store_pair<T, EVEN>(dx + out + (int64_t)j * D, vx, even_rows, w.has0, w.has1);
-                store_pair<T, EVEN>(dr + out + (int64_t)j * D, vr, even_rows, w.has0, w.has1);
-                store_pair<T, EVEN>(di + out + (int64_t)j * D, vi, even_rows, w.has0, w.has1);
+                store_pair<T, EVEN>(px, vx, even_rows, w.has0, w.has1);
+                store_pair<T, EVEN>(pr, vr, even_rows, w.has0, w.has1);
+                store_pair<T, EVEN>(pi, vi, even_rows, w.has0, w.has1);
             }
+            px += D;
+            pr += D;
+            pi += D;
         }
     }
     __syncthreads();
@@ -828,8 +864,8 @@ Plan rec_plan(const bcm_gated_rec_args* a) {
         pl.L = (int)(pl.per * a->seqlen);
         pl.runs = rec_parts(a->batch, pl.per);
     }
-    // blocks of a cluster: as many as the chunks allow until the GPU holds its two blocks per SM
-    while (pl.P < kMaxCluster && pl.runs * pl.tiles * pl.P < 2 * (int64_t)sm_count() && 2 * pl.P <= rec_parts(pl.L, kChunk)) pl.P *= 2;
+    // blocks of a cluster: as many as the chunks allow and two blocks per SM hold at once
+    while (pl.P < kMaxCluster && pl.runs * pl.tiles * pl.P <= (int64_t)sm_count() && 2 * pl.P <= rec_parts(pl.L, kChunk)) pl.P *= 2;
     return pl;
 }
 

@@ -25,19 +25,19 @@ __device__ __forceinline__ float softplus_(float v) { return v > 20.0f ? v : log
 // A lane owns two neighbouring features; its arithmetic is packed fp32 (two
 // results an instruction).  What bounds it then is the special-function unit
 // (8 cycles a warp instruction), so:
-//  * a - 1 = expm1(u) is a polynomial for |u| <= kPolyEnd (degree 4 times u,
-//    interpolated at Chebyshev nodes, relative error 1.4e-8).  It also gives
-//    1 - a^2 = (1 - a)(1 + a) without cancellation and a correctly rounded
-//    a = 1 + (a - 1), so that a memory of a thousand tokens does not add up a
-//    biased decay;
+//  * v = 1 - a = -expm1(u) is a polynomial for U = -u <= kPolyEnd (degree 4 times
+//    U, interpolated at Chebyshev nodes, relative error 1.4e-8).  It also gives
+//    1 - a^2 = v + v a without cancellation and a correctly rounded a = 1 - v, so
+//    that a memory of a thousand tokens does not add up a biased decay;
 //  * FAST shares one reciprocal between the four sigmoids of a pair and needs no
 //    exponential for a: 7 special functions a pair instead of 12.  It holds where
-//    every c s is at most kPolyEnd and the product of a pair's four denominators
-//    (1 + e^-r)(1 + e^-i) stays below kProdEnd; a warp that finds a larger one (a
-//    gate below about -20, infinite, NaN) computes its batch again in the long form.
+//    every c s lies in [kCsLow, kPolyEnd] and the product of a pair's four
+//    denominators (1 + e^-r)(1 + e^-i) stays below kProdEnd (U is a normal number
+//    then); a warp that finds a larger one (gates below about -10, infinite, NaN)
+//    computes its batch again in the long form.
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kPolyEnd = 0.35f;
-constexpr float kProdEnd = 1e36f;
+constexpr float kPolyEnd = 0.35f, kCsLow = 1e-18f;
+constexpr float kProdEnd = 1e18f;
 
 __device__ __forceinline__ float ex2_(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
 __device__ __forceinline__ float rcp_(float v) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
@@ -48,44 +48,59 @@ __device__ __forceinline__ float2 mul(float2 a, float2 b) { return __fmul2_rn(a,
 __device__ __forceinline__ float2 add(float2 a, float2 b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ float2 fma(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 
-struct Gates {
-    float2 sr, si, w, rs;     // sigmoid(r), sigmoid(i), a - 1, 1 / m (3e18 where m = 0: it meets a factor 0 then)
+// Constants as register pairs: packed instructions take no immediates, and left to itself the compiler sets each pair
+// up again at every use (a quarter of the loop's instructions).
+__device__ __forceinline__ float2 pinned(float v) {
+    float2 r;
+    asm volatile("mov.b32 %0, %2; mov.b32 %1, %2;" : "=f"(r.x), "=f"(r.y) : "f"(v));
+    return r;
+}
+struct Consts {
+    float2 nlog2e, one, c1, c2, c3, c4;
+    __device__ __forceinline__ Consts()
+        : nlog2e(pinned(-kLog2e)), one(pinned(1.0f)), c1(pinned(-0.49999821186065674f)), c2(pinned(0.16662530601024628f)),
+          c3(pinned(-0.04133187234401703f)), c4(pinned(0.007211245596408844f)) {}
 };
 
-__device__ __forceinline__ float2 a_of(float2 w) { return add(w, f2(1.0f)); }
-// m = (1 - a^2) / sqrt(1 - a^2): exactly 0 for a = 1
-__device__ __forceinline__ float2 m_of(float2 w, float2 rs) { return mul(mul(w, fma(w, f2(-1.0f), f2(-2.0f))), rs); }
+struct Gates {
+    float2 sr, si, a, m, rs;     // sigmoid(r), sigmoid(i), a, m, 1 / m (0 where m = 0)
+};
 
 template <bool FAST>
-__device__ __forceinline__ Gates gates(float2 r, float2 i, float2 ncs, float& prod) {
+__device__ __forceinline__ Gates gates(float2 r, float2 i, float2 cs, const Consts& k, float& prod) {
     Gates g;
-    const float2 tr = mul(r, f2(-kLog2e)), ti = mul(i, f2(-kLog2e));
-    const float2 dr = add(make_float2(ex2_(tr.x), ex2_(tr.y)), f2(1.0f));
-    const float2 di = add(make_float2(ex2_(ti.x), ex2_(ti.y)), f2(1.0f));
+    const float2 tr = mul(r, k.nlog2e), ti = mul(i, k.nlog2e);
+    const float2 dr = add(make_float2(ex2_(tr.x), ex2_(tr.y)), k.one);
+    const float2 di = add(make_float2(ex2_(ti.x), ex2_(ti.y)), k.one);
     if (FAST) {
         const float2 both = mul(dr, di);
         const float all = both.x * both.y;
         prod = max_nan_(prod, all);
-        const float2 inv = mul(make_float2(both.y, both.x), f2(rcp_(all)));
-        g.sr = mul(di, inv);
-        g.si = mul(dr, inv);
+        const float inv = rcp_(all);
+        const float2 each = make_float2(both.y * inv, both.x * inv);
+        g.sr = mul(di, each);
+        g.si = mul(dr, each);
     } else {
         g.sr = make_float2(rcp_(dr.x), rcp_(dr.y));
         g.si = make_float2(rcp_(di.x), rcp_(di.y));
     }
-    const float2 u = mul(ncs, g.sr);
-    float2 q = fma(u, f2(0.007211245596408844f), f2(0.04133187234401703f));
-    q = fma(u, q, f2(0.16662530601024628f));
-    q = fma(u, q, f2(0.49999821186065674f));
-    q = fma(u, q, f2(1.0f));
-    g.w = mul(u, q);
+    const float2 U = mul(cs, g.sr);
+    float2 q = fma(U, k.c4, k.c3);
+    q = fma(U, q, k.c2);
+    q = fma(U, q, k.c1);
+    float2 v = fma(mul(U, U), q, U);
     if (!FAST) {
-        const float2 t = mul(u, f2(kLog2e));
-        if (!(u.x >= -kPolyEnd)) g.w.x = ex2_(t.x) - 1.0f;
-        if (!(u.y >= -kPolyEnd)) g.w.y = ex2_(t.y) - 1.0f;
+        if (!(U.x <= kPolyEnd)) v.x = 1.0f - ex2_(U.x * -kLog2e);
+        if (!(U.y <= kPolyEnd)) v.y = 1.0f - ex2_(U.y * -kLog2e);
     }
-    const float2 m2 = fma(g.w, fma(g.w, f2(-1.0f), f2(-2.0f)), f2(1e-37f));
+    g.a = make_float2(1.0f - v.x, 1.0f - v.y);
+    const float2 m2 = fma(v, g.a, v);
     g.rs = make_float2(rsqrt_(m2.x), rsqrt_(m2.y));
+    if (!FAST) {
+        if (m2.x == 0.0f || g.rs.x == __int_as_float(0x7f800000)) g.rs.x = 0.0f;
+        if (m2.y == 0.0f || g.rs.y == __int_as_float(0x7f800000)) g.rs.y = 0.0f;
+    }
+    g.m = mul(m2, g.rs);
     return g;
 }
 
@@ -97,7 +112,10 @@ __device__ __forceinline__ Gates gates(float2 r, float2 i, float2 ncs, float& pr
 // once: the composition h -> A h + H of a warp's tokens goes to shared memory,
 // the other warps' and blocks' compositions give the state that enters, and the
 // tokens, still in registers, are replayed from it.  Rows arrive by 16-byte
-// cp.async a few turns ahead; a warp copies its own rows only.
+// cp.async a few turns ahead; a warp copies its own rows only.  Two blocks share
+// an SM: one computes while the other exchanges.  (Computing the next turn's gates
+// before a turn is replayed, with a split cluster barrier, needs both turns in
+// registers: it spilled and ran 20 to 30 % slower.)
 //
 // Mode: kDense, one sequence per block; kGroup, a block takes `per` consecutive
 // dense sequences as one run of tokens (short sequences would leave most of a
@@ -107,7 +125,7 @@ constexpr int kWarps = 8;
 constexpr int kTile = 64;                        // features of a block
 constexpr int kStepsFwd = 8, kStepsBwd = 4;      // tokens of a warp's turn (the backward keeps 7 values a token)
 constexpr int kCkpt = kWarps * kStepsBwd;        // the forward keeps the state that enters every kCkpt tokens of a run
-constexpr int kMaxCluster = 16;
+constexpr int kMaxCluster = 8;                   // (16 measured no faster: a turn's exchange grew with the blocks)
 constexpr float kCut = -1.0f;                    // in place of a product of decays: nothing passes (a sequence starts inside)
 
 enum Mode { kDense, kGroup, kPacked };
@@ -131,7 +149,7 @@ struct RecDim {
 };
 
 // The sequence that holds token t: the last s with cu[s] <= t, in [0, n).  Called by whole warps; t is uniform.
-__device__ __forceinline__ int seq_of(const int32_t* __restrict__ cu, int n, int t) {
+__device__ __forceinline__ int seq_of(const int32_t* cu, int n, int t) {
     int lo = 0, hi = n - 1;                          // the answer lies in [lo, hi]
     const int lane = threadIdx.x & 31;
     while (hi > lo) {
@@ -194,13 +212,34 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, int rank, float4 v) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Where a block works.
+struct Place {
+    int lane, warp, rank, tile, d, L;
+    int64_t run, b;           // the run and its first sequence
+    bool has0, has1;          // the lane's features exist
+};
+template <int MODE, bool CLUSTER>
+__device__ __forceinline__ Place place(const RecDim& n) {
+    Place q;
+    q.lane = threadIdx.x & 31;
+    q.warp = threadIdx.x >> 5;
+    const int P = CLUSTER ? n.P : 1, tiles = (n.D + kTile - 1) / kTile;
+    q.rank = CLUSTER ? blockIdx.x % P : 0;
+    q.run = blockIdx.x / P / tiles;
+    q.tile = (int)(blockIdx.x / P - q.run * tiles);
+    q.b = MODE == kGroup ? q.run * n.per : q.run;
+    q.L = MODE == kGroup ? (int)min((int64_t)n.per, n.n - q.b) * n.Ls : n.L;
+    q.d = q.tile * kTile + q.lane * 2;
+    q.has0 = q.d < n.D;
+    q.has1 = q.d + 1 < n.D;
+    return q;
+}
 
 // ---- rows in shared memory -----------------------------------------------------
 // A row of a tile is 64 elements from the tile's first feature on.  EVEN: every
@@ -211,34 +250,6 @@ template <typename T, bool EVEN>
 struct Rows {
     static constexpr int kGran = kTile * (int)sizeof(T) / 16 + (EVEN ? 0 : 1);
     static constexpr int kPitch = kGran * 16;
-
-    // S rows from token t0 of the run on, those past its end and the features past the last one filled with zeros
-    template <int MODE, int S>
-    static __device__ __forceinline__ void copy(char* dst, const T* base, int64_t sb, int64_t st, int t0, const RecDim& n, int L, int width) {
-        const int lane = threadIdx.x & 31;
-#pragma unroll
-        for (int q0 = 0; q0 < S * kGran; q0 += 32) {
-            const int q = q0 + lane, row = q / kGran, g = q - row * kGran, t = t0 + row;
-            if (S * kGran % 32 != 0 && q >= S * kGran) continue;
-            int bytes = 0;
-            uintptr_t src = reinterpret_cast<uintptr_t>(base) & ~(uintptr_t)15;
-            if (t < L) {
-                int64_t at = (int64_t)t * st;
-                if (MODE == kGroup) {
-                    const int k = t / n.Ls;
-                    at = k * sb + (int64_t)(t - k * n.Ls) * st;
-                }
-                const uintptr_t first = reinterpret_cast<uintptr_t>(base + at), end = first + width * sizeof(T);
-                const uintptr_t from = (first & ~(uintptr_t)15) + g * 16;
-                if (from < end) {
-                    src = from;
-                    bytes = (int)min((uintptr_t)16, end - from);
-                }
-            }
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst + row * kPitch + g * 16)), "l"(src), "r"(bytes)
-                         : "memory");
-        }
-    }
 
     // off: bytes of the row's first element past its granule
     static __device__ __forceinline__ float2 read(const char* row, int off) {
@@ -259,49 +270,64 @@ struct Rows {
     }
 };
 
-// One input of a warp: fetches S rows a turn, reads them back.  LINEAR (kDense, kPacked, and kGroup where a sequence
-// follows the one before it at once): rows of a run lie st elements apart.
+// One input of a warp: fetches S rows a turn, reads them back.  Where a row of the run follows the one before it by st
+// elements (kDense, kPacked, and kGroup without gaps between sequences) and all S rows are there, the lane's granule
+// (EVEN) only moves along.
+struct Input {
+    const void* p;
+    int64_t sb, st;
+};
 template <typename T, int MODE, bool EVEN, int S>
 struct Stream {
     using R = Rows<T, EVEN>;
-    static constexpr int kLaneRows = 32 / R::kGran;      // rows of a warp's copy instruction (EVEN)
-    const T* base;
-    int64_t sb, st;
-    const char* at;                                      // EVEN: the lane's granule in the rows of the next fetch
-    int bytes, width;
-    bool linear;
-    __device__ __forceinline__ Stream(const T* base_, int64_t sb_, int64_t st_, const RecDim& n, int t0, int width_)
-        : base(base_), sb(sb_), st(st_), width(width_) {
-        const int lane = threadIdx.x & 31, g = EVEN ? lane % R::kGran : 0, row = EVEN ? lane / R::kGran : 0;
-        linear = MODE != kGroup || sb == st * n.Ls;
-        at = reinterpret_cast<const char*>(base + (t0 + row) * st) + g * 16;
-        bytes = max(0, min(16, width * (int)sizeof(T) - g * 16));
+    static constexpr int kLaneRows = EVEN ? 32 / R::kGran : 1;      // rows of a warp's copy instruction
+    const char* at;
+    __device__ __forceinline__ static bool linear(const Input& in, const RecDim& n) { return MODE != kGroup || in.sb == in.st * n.Ls; }
+    // elements from the run's first row to that of token t
+    __device__ __forceinline__ static int64_t row(const Input& in, const RecDim& n, int t) {
+        if (linear(in, n)) return (int64_t)t * in.st;
+        const int k = t / n.Ls;
+        return k * in.sb + (int64_t)(t - k * n.Ls) * in.st;
     }
-    // t0: the first row; advance: tokens from this fetch to the next
-    __device__ __forceinline__ void fetch(char* dst, int t0, int advance, const RecDim& n, int L) {
-        if (EVEN && linear && t0 + S <= L) {
-            const uint32_t to = smem_addr(dst) + (threadIdx.x & 31) * 16;
+    __device__ __forceinline__ static const T* base(const Input& in, const Place& w) {
+        return static_cast<const T*>(in.p) + (MODE == kPacked ? 0 : w.b * in.sb) + (int64_t)w.tile * kTile;
+    }
+    __device__ __forceinline__ Stream(const Input& in, const Place& w, int t0) {
+        if (EVEN) at = reinterpret_cast<const char*>(base(in, w) + (int64_t)(t0 + w.lane / R::kGran) * in.st) + w.lane % R::kGran * 16;
+    }
+    // t0: the first row; advance: tokens from this fetch to the next; rows and features that are not there become zeros
+    __device__ __forceinline__ void fetch(char* dst, const Input& in, const Place& w, const RecDim& n, int t0, int advance, int width) {
+        const uint32_t to = smem_addr(dst);
+        if (EVEN && t0 + S <= w.L && linear(in, n)) {
+            const int bytes = max(0, min(16, width * (int)sizeof(T) - w.lane % R::kGran * 16));
 #pragma unroll
             for (int k = 0; k < S / kLaneRows; ++k)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * 512), "l"(at + (int64_t)(k * kLaneRows) * st * (int)sizeof(T)),
-                             "r"(bytes)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + w.lane * 16 + k * 512),
+                             "l"(at + (int64_t)(k * kLaneRows) * in.st * (int)sizeof(T)), "r"(bytes)
                              : "memory");
         } else {
-            R::template copy<MODE, S>(dst, base, sb, st, t0, n, L, width);
-        }
-        if (EVEN) at += (int64_t)advance * st * (int)sizeof(T);
-    }
-    // the lane's two features of token t, row j of the fetched ones
-    __device__ __forceinline__ float2 read(const char* from, int j, int t, const RecDim& n) const {
-        uint32_t off = 0;
-        if (!EVEN) {
-            uint32_t e = (uint32_t)t * (uint32_t)st;
-            if (MODE == kGroup) {
-                const int k = t / n.Ls;
-                e = k * (uint32_t)sb + (uint32_t)(t - k * n.Ls) * (uint32_t)st;
+            const T* from0 = base(in, w);
+            for (int q = w.lane; q < S * R::kGran; q += 32) {
+                const int j = q / R::kGran, g = q - j * R::kGran;
+                int bytes = 0;
+                uintptr_t src = reinterpret_cast<uintptr_t>(from0) & ~(uintptr_t)15;
+                if (t0 + j < w.L) {
+                    const uintptr_t first = reinterpret_cast<uintptr_t>(from0 + row(in, n, t0 + j)), end = first + width * sizeof(T);
+                    const uintptr_t from = (first & ~(uintptr_t)15) + g * 16;
+                    if (from < end) {
+                        src = from;
+                        bytes = (int)min((uintptr_t)16, end - from);
+                    }
+                }
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + j * R::kPitch + g * 16), "l"(src), "r"(bytes) : "memory");
             }
-            off = ((uint32_t)(uintptr_t)base + e * (uint32_t)sizeof(T)) & 15u;
         }
+        if (EVEN) at += (int64_t)advance * in.st * (int)sizeof(T);
+    }
+    // the lane's two features of token t, in slot j of the fetched rows
+    __device__ __forceinline__ static float2 read(const char* from, const Input& in, const Place& w, const RecDim& n, int j, int t) {
+        uint32_t off = 0;
+        if (!EVEN) off = ((uint32_t)(uintptr_t)base(in, w) + (uint32_t)row(in, n, t) * (uint32_t)sizeof(T)) & 15u;
         return R::read(from + j * R::kPitch, (int)off);
     }
 };
@@ -341,29 +367,6 @@ __device__ __forceinline__ void store_state(float* p, int64_t row, int D, int d,
     if (has1) p[row * D + d + 1] = v.y;
 }
 
-// Where a block works.
-struct Place {
-    int lane, warp, rank, tile, d, L;
-    int64_t run, b;           // the run and its first sequence
-    bool has0, has1;          // the lane's features exist
-};
-template <int MODE, bool CLUSTER>
-__device__ __forceinline__ Place place(const RecDim& n) {
-    Place q;
-    q.lane = threadIdx.x & 31;
-    q.warp = threadIdx.x >> 5;
-    const int P = CLUSTER ? n.P : 1, tiles = (n.D + kTile - 1) / kTile;
-    q.rank = CLUSTER ? blockIdx.x % P : 0;
-    q.run = blockIdx.x / P / tiles;
-    q.tile = (int)(blockIdx.x / P - q.run * tiles);
-    q.b = MODE == kGroup ? q.run * n.per : q.run;
-    q.L = MODE == kGroup ? (int)min((int64_t)n.per, n.n - q.b) * n.Ls : n.L;
-    q.d = q.tile * kTile + q.lane * 2;
-    q.has0 = q.d < n.D;
-    q.has1 = q.d + 1 < n.D;
-    return q;
-}
-
 // Bit j: a sequence starts at token t0 + j.
 template <int MODE, int S>
 __device__ __forceinline__ unsigned starts_in(const Seq<MODE>& seq, int t0, int L) {
@@ -377,13 +380,30 @@ __device__ __forceinline__ unsigned starts_in(const Seq<MODE>& seq, int t0, int 
     return m;
 }
 
+// The sequences' offsets of a packed run, in shared memory where they fit.
+constexpr int kCuMax = 1024;
+template <int MODE>
+__device__ __forceinline__ const int32_t* stage_cu(const RecDim& n, int32_t* room) {
+    if (MODE != kPacked || n.n >= kCuMax) return n.cu;
+    for (int k = threadIdx.x; k <= (int)n.n; k += kWarps * 32) room[k] = n.cu[k];
+    __syncthreads();
+    return room;
+}
+
 template <typename T, int S, bool EVEN, int ARRAYS>
 constexpr int stage_bytes() { return kWarps * ARRAYS * S * Rows<T, EVEN>::kPitch; }
-// turns of rows in flight or in use: what fits two blocks on an SM
+// turns of rows in shared memory, as many as let two blocks share an SM
 template <typename T>
 constexpr int stages_fwd() { return sizeof(T) == 4 ? 2 : 3; }
 template <typename T>
 constexpr int stages_bwd() { return sizeof(T) == 4 ? 2 : 3; }
+
+// A block's (A, H) or (A, K) of a turn goes to every block of the cluster.  Two turns' slots: a block writes those of
+// turn k + 2 only after every block has arrived for turn k + 1, hence has read those of turn k.
+template <bool CLUSTER>
+struct Pub {
+    float4 v[CLUSTER ? 2 : 1][CLUSTER ? kMaxCluster : 1][CLUSTER ? 32 : 1];
+};
 
 template <typename T, int MODE, bool EVEN, bool CLUSTER>
 __global__ void __launch_bounds__(kWarps * 32, 2)
@@ -391,64 +411,75 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
                const float* __restrict__ lam, float c) {
     constexpr bool CUTS = MODE != kDense;
     constexpr int S = kStepsFwd, kChunk = kWarps * S, ST = stages_fwd<T>();
+    using In = Stream<T, MODE, EVEN, S>;
     using R = Rows<T, EVEN>;
     __shared__ float4 ex[2][kWarps][32];
-    __shared__ float4 pub[CLUSTER ? 2 : 1][CLUSTER ? kMaxCluster : 1][32];
+    __shared__ Pub<CLUSTER> pub;
+    __shared__ int32_t cus[MODE == kPacked ? kCuMax : 1];
     extern __shared__ __align__(16) char rows[];
     const Place w = place<MODE, CLUSTER>(n);
     const int D = n.D, L = w.L, P = CLUSTER ? n.P : 1, width = min(kTile, D - w.tile * kTile);
-    const int64_t f0 = (int64_t)w.tile * kTile;
-    const T* x = static_cast<const T*>(p.x) + (MODE == kPacked ? 0 : w.b * p.xb) + f0;
-    const T* r = static_cast<const T*>(p.r) + (MODE == kPacked ? 0 : w.b * p.rb) + f0;
-    const T* i = static_cast<const T*>(p.i) + (MODE == kPacked ? 0 : w.b * p.ib) + f0;
     T* y = static_cast<T*>(o.y) + (MODE == kPacked ? 0 : w.b * n.Ls * D) + w.d;
     const bool even_rows = (D & 1) == 0 && (uintptr_t)o.y % (2 * sizeof(T)) == 0;
     const int turns = ((n.L + kChunk - 1) / kChunk + P - 1) / P;
     float* ck = o.ckpt ? o.ckpt + w.run * ((n.L + kCkpt - 1) / kCkpt) * D : nullptr;
     const float2 l = load_state(lam, 0, D, w.d, w.has0, w.has1);
-    const float2 ncs = make_float2(-c * softplus_(l.x), -c * softplus_(l.y));
-    const bool small = __all_sync(kFull, -ncs.x <= kPolyEnd && -ncs.y <= kPolyEnd);
+    const float2 cs = make_float2(w.has0 ? c * softplus_(l.x) : kPolyEnd, w.has1 ? c * softplus_(l.y) : kPolyEnd);
+    const bool small = __all_sync(kFull, cs.x >= kCsLow && cs.x <= kPolyEnd && cs.y >= kCsLow && cs.y <= kPolyEnd);
+    const Consts consts;
     const int first = w.rank * kChunk + w.warp * S;
-    Stream<T, MODE, EVEN, S> sx(x, p.xb, p.xt, n, first, width), sr(r, p.rb, p.rt, n, first, width), si(i, p.ib, p.it, n, first, width);
+    const Input ix = {p.x, p.xb, p.xt}, ir = {p.r, p.rb, p.rt}, ii = {p.i, p.ib, p.it};
+    In sx(ix, w, first), sr(ir, w, first), si(ii, w, first);
     char* mine = rows + w.warp * (3 * S * R::kPitch);
     auto fetch = [&](int turn) {
         if (turn < turns) {
             char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 3>();
             const int t0 = turn * P * kChunk + first;
-            sr.fetch(at, t0, P * kChunk, n, L);
-            si.fetch(at + S * R::kPitch, t0, P * kChunk, n, L);
-            sx.fetch(at + 2 * S * R::kPitch, t0, P * kChunk, n, L);
+            sr.fetch(at, ir, w, n, t0, P * kChunk, width);
+            si.fetch(at + S * R::kPitch, ii, w, n, t0, P * kChunk, width);
+            sx.fetch(at + 2 * S * R::kPitch, ix, w, n, t0, P * kChunk, width);
         }
         cp_commit();
     };
-    float2 run = MODE == kDense ? load_state(o.h0, w.b, D, w.d, w.has0, w.has1) : f2(0.0f);
-    Seq<MODE> seq{n.cu, (int)n.n, n.Ls, w.b, 0, 0, 0};
 #pragma unroll
     for (int k = 0; k < ST - 1; ++k) fetch(k);
-    if (CLUSTER) cluster_sync();       // every block of the cluster runs before its shared memory is written to
-    for (int turn = 0; turn < turns; ++turn) {
-        const int buf = turn & 1;
-        const int t0 = (turn * P + w.rank) * kChunk + w.warp * S;
+    Seq<MODE> seq{stage_cu<MODE>(n, cus), (int)n.n, n.Ls, w.b, 0, 0, 0};
+    float2 run = MODE == kDense ? load_state(o.h0, w.b, D, w.d, w.has0, w.has1) : f2(0.0f);
+
+    // gates and composition of a turn: h -> a_j h + e_j token by token, h -> A h + H together
+    auto prepare = [&](int turn, float2 (&a)[S], float2 (&e)[S], unsigned& starts) {
+        const int t0 = turn * P * kChunk + first;
         fetch(turn + ST - 1);
+        float2 own[S];                    // the states that enter with the sequences that start here
+        if (CUTS) {
+            if (t0 < L) seq.at(t0);
+            starts = starts_in<MODE, S>(seq, t0, L);
+            if (starts) {
+                Seq<MODE> q = seq;
+#pragma unroll
+                for (int j = 0; j < S; ++j)
+                    if (starts >> j & 1u) {
+                        q.at(t0 + j);
+                        own[j] = load_state(o.h0, q.s, D, w.d, w.has0, w.has1);
+                    }
+            }
+        }
         cp_wait<ST - 1>();
         __syncwarp();
         const char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 3>();
-        float2 a[S], e[S];
         float prod = 0.0f;
 #pragma unroll
         for (int j = 0; j < S; ++j) {
-            const float2 rv = sr.read(at, j, t0 + j, n), iv = si.read(at, S + j, t0 + j, n), xv = sx.read(at, 2 * S + j, t0 + j, n);
-            const Gates g = gates<true>(rv, iv, ncs, prod);
-            a[j] = a_of(g.w);
-            e[j] = mul(mul(m_of(g.w, g.rs), g.si), xv);
+            const Gates g = gates<true>(In::read(at, ir, w, n, j, t0 + j), In::read(at, ii, w, n, S + j, t0 + j), cs, consts, prod);
+            a[j] = g.a;
+            e[j] = mul(mul(g.m, g.si), In::read(at, ix, w, n, 2 * S + j, t0 + j));
         }
         if (!__all_sync(kFull, small && prod < kProdEnd)) {
 #pragma unroll
             for (int j = 0; j < S; ++j) {
-                const float2 rv = sr.read(at, j, t0 + j, n), iv = si.read(at, S + j, t0 + j, n), xv = sx.read(at, 2 * S + j, t0 + j, n);
-                const Gates g = gates<false>(rv, iv, ncs, prod);
-                a[j] = a_of(g.w);
-                e[j] = mul(mul(m_of(g.w, g.rs), g.si), xv);
+                const Gates g = gates<false>(In::read(at, ir, w, n, j, t0 + j), In::read(at, ii, w, n, S + j, t0 + j), cs, consts, prod);
+                a[j] = g.a;
+                e[j] = mul(mul(g.m, g.si), In::read(at, ix, w, n, 2 * S + j, t0 + j));
             }
         }
         if (t0 + S > L)                   // tokens past the end change nothing
@@ -458,16 +489,12 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
                     a[j] = f2(1.0f);
                     e[j] = f2(0.0f);
                 }
-        if (CUTS && t0 < L) seq.at(t0);
-        const unsigned starts = starts_in<MODE, S>(seq, t0, L);
         float2 A = f2(1.0f), H = f2(0.0f);
         if (CUTS && starts) {
-            Seq<MODE> q = seq;
 #pragma unroll
             for (int j = 0; j < S; ++j) {
-                if (starts >> j & 1u) {   // the sequence's own state enters
-                    q.at(t0 + j);
-                    e[j] = fma(a[j], load_state(o.h0, q.s, D, w.d, w.has0, w.has1), e[j]);
+                if (starts >> j & 1u) {
+                    e[j] = fma(a[j], own[j], e[j]);
                     A = f2(kCut);
                     H = e[j];
                 } else {
@@ -478,45 +505,45 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
 #pragma unroll
             for (int j = 0; j < S; ++j) then<false>(A, H, a[j], e[j]);
         }
-        ex[buf][w.warp][w.lane] = make_float4(A.x, A.y, H.x, H.y);
+        ex[turn & 1][w.warp][w.lane] = make_float4(A.x, A.y, H.x, H.y);
         __syncthreads();
-        float2 h;
-        if (CLUSTER) {
-            float2 tA = f2(1.0f), tH = f2(0.0f);
-            for (int k = 0; k < w.warp; ++k) {
-                const float4 f = ex[buf][k][w.lane];
-                then<CUTS>(tA, tH, make_float2(f.x, f.y), make_float2(f.z, f.w));
-            }
-            const float2 preA = tA, preH = tH;
-            for (int k = w.warp; k < kWarps; ++k) {
-                const float4 f = ex[buf][k][w.lane];
-                then<CUTS>(tA, tH, make_float2(f.x, f.y), make_float2(f.z, f.w));
-            }
-            for (int k = w.warp; k < P; k += kWarps) st_cluster(smem_addr(&pub[buf][w.rank][w.lane]), k, make_float4(tA.x, tA.y, tH.x, tH.y));
-            cluster_sync();
-            for (int k = 0; k < w.rank; ++k) {
-                const float4 f = pub[buf][k][w.lane];
-                run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
-            }
-            h = apply<CUTS>(preA, preH, run);
-            for (int k = w.rank; k < P; ++k) {
-                const float4 f = pub[buf][k][w.lane];
-                run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
-            }
-        } else {
-            for (int k = 0; k < w.warp; ++k) {
-                const float4 f = ex[buf][k][w.lane];
-                run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
-            }
-            h = run;
-            for (int k = w.warp; k < kWarps; ++k) {
-                const float4 f = ex[buf][k][w.lane];
-                run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
-            }
+    };
+    // the composition of the block's warps before this one, and the block's, which goes to the cluster
+    auto publish = [&](int turn, float2& preA, float2& preH) {
+        float2 tA = f2(1.0f), tH = f2(0.0f);
+        for (int k = 0; k < w.warp; ++k) {
+            const float4 f = ex[turn & 1][k][w.lane];
+            then<CUTS>(tA, tH, make_float2(f.x, f.y), make_float2(f.z, f.w));
         }
+        preA = tA;
+        preH = tH;
+        for (int k = w.warp; k < kWarps; ++k) {
+            const float4 f = ex[turn & 1][k][w.lane];
+            then<CUTS>(tA, tH, make_float2(f.x, f.y), make_float2(f.z, f.w));
+        }
+        if constexpr (CLUSTER)
+            if (w.warp < P) st_cluster(smem_addr(&pub.v[turn & 1][w.rank][w.lane]), w.warp, make_float4(tA.x, tA.y, tH.x, tH.y));
+    };
+    // the state that enters the warp's tokens; run moves on to the next turn
+    auto enter = [&](const float4 (&from)[CLUSTER ? kMaxCluster : kWarps][32], int count, int here) -> float2 {
+        for (int k = 0; k < here; ++k) {
+            const float4 f = from[k][w.lane];
+            run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
+        }
+        const float2 h = run;
+        for (int k = here; k < count; ++k) {
+            const float4 f = from[k][w.lane];
+            run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
+        }
+        return h;
+    };
+    auto replay = [&](int turn, float2 (&a)[S], float2 (&e)[S], unsigned starts, float2 h) {
+        const int t0 = turn * P * kChunk + first;
         if (ck && w.warp % (kCkpt / S) == 0 && t0 < L) store_state(ck, t0 / kCkpt, D, w.d, h, w.has0, w.has1);
         T* out = y + (int64_t)t0 * D;
-        if (t0 + S <= L && (!CUTS || (starts == 0 && seq.end > t0 + S))) {
+        Seq<MODE> q = seq;
+        if (CUTS && t0 < L) q.at(t0);
+        if (t0 + S <= L && (!CUTS || (starts == 0 && q.end > t0 + S))) {
 #pragma unroll
             for (int j = 0; j < S; ++j) {
                 h = fma(a[j], h, e[j]);
@@ -527,22 +554,42 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
 #pragma unroll
             for (int j = 0; j < S; ++j) {
                 const int t = t0 + j;
-                h = starts >> j & 1u ? e[j] : fma(a[j], h, e[j]);
+                h = CUTS && (starts >> j & 1u) ? e[j] : fma(a[j], h, e[j]);
                 if (t < L) {
                     store_pair<T, EVEN>(out, h, even_rows, w.has0, w.has1);
-                    if (CUTS) seq.at(t);
-                    if (CUTS && t == seq.end - 1) store_state(o.h_last, seq.s, D, w.d, h, w.has0, w.has1);
+                    if (CUTS) q.at(t);
+                    if (CUTS && t == q.end - 1) store_state(o.h_last, q.s, D, w.d, h, w.has0, w.has1);
                 }
                 out += D;
             }
         }
+    };
+
+    if (CLUSTER) {                        // every block of the cluster runs before its shared memory is written to
+        cluster_arrive();
+        cluster_wait();
+    }
+    for (int turn = 0; turn < turns; ++turn) {
+        float2 a[S], e[S], h;
+        unsigned starts = 0;
+        prepare(turn, a, e, starts);
+        if constexpr (CLUSTER) {
+            float2 preA, preH;
+            publish(turn, preA, preH);
+            cluster_arrive();
+            cluster_wait();
+            h = apply<CUTS>(preA, preH, enter(pub.v[turn & 1], P, w.rank));
+        } else {
+            h = enter(ex[turn & 1], kWarps, w.warp);
+        }
+        replay(turn, a, e, starts, h);
     }
     if (w.rank != 0) return;
     if (MODE == kDense) {
         if (w.warp == 0) store_state(o.h_last, w.b, D, w.d, run, w.has0, w.has1);
     } else if (MODE == kPacked) {
         for (int64_t s = w.warp; s < n.n; s += kWarps)       // empty sequences keep their state
-            if (n.cu[s] >= n.cu[s + 1])
+            if (seq.cu[s] >= seq.cu[s + 1])
                 store_state(o.h_last, s, D, w.d, load_state(o.h0, s, D, w.d, w.has0, w.has1), w.has0, w.has1);
     }
 }
@@ -556,207 +603,191 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
                const float* __restrict__ lam, float c) {
     constexpr bool CUTS = MODE != kDense;
     constexpr int S = kStepsBwd, kChunk = kWarps * S, ST = stages_bwd<T>();
+    using In = Stream<T, MODE, EVEN, S>;
     using R = Rows<T, EVEN>;
     __shared__ float4 ex[2][kWarps][32];          // (A, K)
     __shared__ float2 exh[2][kWarps][32];         // H
-    __shared__ float4 pub[CLUSTER ? 2 : 1][CLUSTER ? kMaxCluster : 1][32];
+    __shared__ Pub<CLUSTER> pub;
+    __shared__ int32_t cus[MODE == kPacked ? kCuMax : 1];
     extern __shared__ __align__(16) char rows[];
     const Place w = place<MODE, CLUSTER>(n);
     const int D = n.D, L = w.L, P = CLUSTER ? n.P : 1, width = min(kTile, D - w.tile * kTile);
-    const int64_t f0 = (int64_t)w.tile * kTile;
-    const T* x = static_cast<const T*>(p.x) + (MODE == kPacked ? 0 : w.b * p.xb) + f0;
-    const T* r = static_cast<const T*>(p.r) + (MODE == kPacked ? 0 : w.b * p.rb) + f0;
-    const T* i = static_cast<const T*>(p.i) + (MODE == kPacked ? 0 : w.b * p.ib) + f0;
-    // (without dy, rows of no width: zeros)
-    const T* dy = p.dy ? static_cast<const T*>(p.dy) + (MODE == kPacked ? 0 : w.b * p.gb) + f0 : x;
     const int64_t base = (MODE == kPacked ? 0 : w.b * n.Ls * D) + w.d;
-    T* dx = static_cast<T*>(o.dx) + base;
-    T* dr = static_cast<T*>(o.dr) + base;
-    T* di = static_cast<T*>(o.di) + base;
     const bool even_rows = (D & 1) == 0 && ((uintptr_t)o.dx | (uintptr_t)o.dr | (uintptr_t)o.di) % (2 * sizeof(T)) == 0;
     const int turns = ((n.L + kChunk - 1) / kChunk + P - 1) / P;
     const float* ck = o.ckpt + w.run * ((n.L + kCkpt - 1) / kCkpt) * D;
     const float2 l = load_state(lam, 0, D, w.d, w.has0, w.has1);
-    const float2 ncs = make_float2(-c * softplus_(l.x), -c * softplus_(l.y));
-    const bool small = __all_sync(kFull, -ncs.x <= kPolyEnd && -ncs.y <= kPolyEnd);
+    const float2 cs = make_float2(w.has0 ? c * softplus_(l.x) : kPolyEnd, w.has1 ? c * softplus_(l.y) : kPolyEnd);
+    const bool small = __all_sync(kFull, cs.x >= kCsLow && cs.x <= kPolyEnd && cs.y >= kCsLow && cs.y <= kPolyEnd);
+    const Consts consts;
     const int first = w.rank * kChunk + w.warp * S, last = (turns - 1) * P * kChunk + first;
-    Stream<T, MODE, EVEN, S> sx(x, p.xb, p.xt, n, last, width), sr(r, p.rb, p.rt, n, last, width), si(i, p.ib, p.it, n, last, width),
-        sg(dy, p.gb, p.gt, n, last, p.dy ? width : 0);
+    // (without dy: rows of no width, zeros)
+    const Input ix = {p.x, p.xb, p.xt}, ir = {p.r, p.rb, p.rt}, ii = {p.i, p.ib, p.it}, ig = {p.dy ? p.dy : p.x, p.gb, p.gt};
+    In sx(ix, w, last), sr(ir, w, last), si(ii, w, last), sg(ig, w, last);
     char* mine = rows + w.warp * (4 * S * R::kPitch);
     auto fetch = [&](int turn) {
         if (turn >= 0) {
             char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 4>();
             const int t0 = turn * P * kChunk + first;
-            sr.fetch(at, t0, -P * kChunk, n, L);
-            si.fetch(at + S * R::kPitch, t0, -P * kChunk, n, L);
-            sx.fetch(at + 2 * S * R::kPitch, t0, -P * kChunk, n, L);
-            sg.fetch(at + 3 * S * R::kPitch, t0, -P * kChunk, n, L);
+            sr.fetch(at, ir, w, n, t0, -P * kChunk, width);
+            si.fetch(at + S * R::kPitch, ii, w, n, t0, -P * kChunk, width);
+            sx.fetch(at + 2 * S * R::kPitch, ix, w, n, t0, -P * kChunk, width);
+            sg.fetch(at + 3 * S * R::kPitch, ig, w, n, t0, -P * kChunk, p.dy ? width : 0);
         }
         cp_commit();
     };
-    Seq<MODE> seq{n.cu, (int)n.n, n.Ls, w.b, 0, 0, 0};
+    constexpr int kAhead = ST - 1;                // turns in flight beyond the one being prepared
+#pragma unroll
+    for (int k = 1; k <= kAhead; ++k) fetch(turns - k);
+    Seq<MODE> seq{stage_cu<MODE>(n, cus), (int)n.n, n.Ls, w.b, 0, 0, 0};
     seq.at(L - 1);
     float2 run = load_state(o.dh_last, CUTS ? seq.s : w.b, D, w.d, w.has0, w.has1), sum = f2(0.0f);
+    auto state0 = [&](int t) -> float2 {          // the state that enters the sequence of token t
+        Seq<MODE> q = seq;
+        q.at(t);
+        return load_state(o.h0, q.s, D, w.d, w.has0, w.has1);
+    };
+    auto back0 = [&](int t) -> float2 {           // what enters, from the right, the sequence of token t
+        if (t < 0) return f2(0.0f);
+        Seq<MODE> q = seq;
+        q.at(t);
+        return load_state(o.dh_last, q.s, D, w.d, w.has0, w.has1);
+    };
+    const float2 nones = pinned(-1.0f);
+    struct Turn {
+        float2 sr[S], si[S], a[S], rs[S], msi[S], x[S], g[S], h, sufA, sufK, back;      // (msi: m sigmoid(i), g: dy)
+        unsigned starts;
+    };
+
+    auto prepare = [&](int turn, Turn& q) {
+        const int chunk = turn * P + w.rank, t0 = turn * P * kChunk + first;
+        fetch(turn - kAhead);
+        q.h = chunk * kChunk < L ? load_state(ck, chunk, D, w.d, w.has0, w.has1) : f2(0.0f);
+        q.starts = 0;
+        float2 own[S], beyond[S];                 // states and back states of the sequences that start here, end before here
+        if (CUTS) {
+            if (t0 < L) seq.at(t0);
+            q.starts = starts_in<MODE, S>(seq, t0, L);
+            if (q.starts)
 #pragma unroll
-    for (int k = 1; k < ST; ++k) fetch(turns - k);
-    if (CLUSTER) cluster_sync();
-    for (int turn = turns - 1; turn >= 0; --turn) {
-        const int buf = turn & 1;
-        const int chunk = turn * P + w.rank;
-        const int t0 = chunk * kChunk + w.warp * S;
-        fetch(turn - ST + 1);
-        const float2 enter = chunk * kChunk < L ? load_state(ck, chunk, D, w.d, w.has0, w.has1) : f2(0.0f);
-        cp_wait<ST - 1>();
+                for (int j = 0; j < S; ++j)
+                    if (q.starts >> j & 1u) {
+                        own[j] = state0(t0 + j);
+                        beyond[j] = back0(t0 + j - 1);
+                    }
+        }
+        cp_wait<kAhead>();
         __syncwarp();
         const char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 4>();
-        float2 sgr[S], sgi[S], wv[S], rs[S];
         float prod = 0.0f;
 #pragma unroll
         for (int j = 0; j < S; ++j) {
-            const Gates g = gates<true>(sr.read(at, j, t0 + j, n), si.read(at, S + j, t0 + j, n), ncs, prod);
-            sgr[j] = g.sr; sgi[j] = g.si; wv[j] = g.w; rs[j] = g.rs;
+            const Gates g = gates<true>(In::read(at, ir, w, n, j, t0 + j), In::read(at, ii, w, n, S + j, t0 + j), cs, consts, prod);
+            q.sr[j] = g.sr; q.si[j] = g.si; q.a[j] = g.a; q.rs[j] = g.rs; q.msi[j] = mul(g.m, g.si);
         }
         if (!__all_sync(kFull, small && prod < kProdEnd)) {
 #pragma unroll
             for (int j = 0; j < S; ++j) {
-                const Gates g = gates<false>(sr.read(at, j, t0 + j, n), si.read(at, S + j, t0 + j, n), ncs, prod);
-                sgr[j] = g.sr; sgi[j] = g.si; wv[j] = g.w; rs[j] = g.rs;
+                const Gates g = gates<false>(In::read(at, ir, w, n, j, t0 + j), In::read(at, ii, w, n, S + j, t0 + j), cs, consts, prod);
+                q.sr[j] = g.sr; q.si[j] = g.si; q.a[j] = g.a; q.rs[j] = g.rs; q.msi[j] = mul(g.m, g.si);
             }
         }
-        if (t0 + S > L)                   // tokens past the end change nothing (their x and dy are zero)
+        if (t0 + S > L)                           // tokens past the end change nothing (their x and dy are zero)
 #pragma unroll
             for (int j = 0; j < S; ++j)
                 if (t0 + j >= L) {
-                    wv[j] = f2(0.0f);
-                    rs[j] = f2(0.0f);
-                    sgr[j] = f2(0.0f);
+                    q.a[j] = f2(1.0f);
+                    q.rs[j] = q.msi[j] = q.sr[j] = f2(0.0f);
                 }
-        float2 xv[S], G[S], a[S], msi[S], prev[S];
+        // forward composition (A, H), backward composition (A, K) of the warp's tokens
+        float2 A = f2(1.0f), H = f2(0.0f), K = f2(0.0f);
 #pragma unroll
         for (int j = 0; j < S; ++j) {
-            xv[j] = sx.read(at, 2 * S + j, t0 + j, n);
-            G[j] = sg.read(at, 3 * S + j, t0 + j, n);        // for now dy
-            a[j] = a_of(wv[j]);
-            msi[j] = mul(m_of(wv[j], rs[j]), sgi[j]);
-            prev[j] = mul(msi[j], xv[j]);                                       // for now what enters at the token
-        }
-        // forward composition (A, H), backward composition (A, K) of the warp's tokens
-        if (CUTS && t0 < L) seq.at(t0);
-        const unsigned starts = starts_in<MODE, S>(seq, t0, L);
-        auto state0 = [&](int t) -> float2 {                // the state that enters the sequence of token t
-            Seq<MODE> q = seq;
-            q.at(t);
-            return load_state(o.h0, q.s, D, w.d, w.has0, w.has1);
-        };
-        auto back0 = [&](int t) -> float2 {                 // what enters, from the right, the sequence of token t
-            if (t < 0) return f2(0.0f);
-            Seq<MODE> q = seq;
-            q.at(t);
-            return load_state(o.dh_last, q.s, D, w.d, w.has0, w.has1);
-        };
-        float2 A = f2(1.0f), H = f2(0.0f), K = f2(0.0f);
-        if (CUTS && starts) {
-#pragma unroll
-            for (int j = 0; j < S; ++j) {
-                if (starts >> j & 1u) {
-                    A = f2(kCut);
-                    H = fma(a[j], state0(t0 + j), prev[j]);
-                } else {
-                    then<CUTS>(A, H, a[j], prev[j]);
-                }
+            q.x[j] = In::read(at, ix, w, n, 2 * S + j, t0 + j);
+            q.g[j] = In::read(at, ig, w, n, 3 * S + j, t0 + j);
+            const float2 e = mul(q.msi[j], q.x[j]);
+            if (CUTS && (q.starts >> j & 1u)) {
+                A = f2(kCut);
+                H = fma(q.a[j], own[j], e);
+            } else if (CUTS && q.starts) {
+                then<CUTS>(A, H, q.a[j], e);
+            } else {
+                then<false>(A, H, q.a[j], e);
             }
-#pragma unroll
-            for (int j = S - 1; j >= 0; --j) K = starts >> j & 1u ? back0(t0 + j - 1) : mul(a[j], add(G[j], K));
-        } else {
-#pragma unroll
-            for (int j = 0; j < S; ++j) then<false>(A, H, a[j], prev[j]);
-#pragma unroll
-            for (int j = S - 1; j >= 0; --j) K = mul(a[j], add(G[j], K));
         }
-        ex[buf][w.warp][w.lane] = make_float4(A.x, A.y, K.x, K.y);
-        exh[buf][w.warp][w.lane] = H;
+#pragma unroll
+        for (int j = S - 1; j >= 0; --j) {
+            if (CUTS && (q.starts >> j & 1u)) K = beyond[j];
+            else K = mul(q.a[j], add(q.g[j], K));
+        }
+        ex[turn & 1][w.warp][w.lane] = make_float4(A.x, A.y, K.x, K.y);
+        exh[turn & 1][w.warp][w.lane] = H;
         __syncthreads();
-        float2 h = enter, back;
         for (int k = 0; k < w.warp; ++k) {
-            const float4 f = ex[buf][k][w.lane];
-            h = apply<CUTS>(make_float2(f.x, f.y), exh[buf][k][w.lane], h);
+            const float4 f = ex[turn & 1][k][w.lane];
+            q.h = apply<CUTS>(make_float2(f.x, f.y), exh[turn & 1][k][w.lane], q.h);
         }
-        if (CLUSTER) {
-            float2 tA = f2(1.0f), tK = f2(0.0f);
-            for (int k = kWarps - 1; k > w.warp; --k) {
-                const float4 f = ex[buf][k][w.lane];
-                then<CUTS>(tA, tK, make_float2(f.x, f.y), make_float2(f.z, f.w));
-            }
-            const float2 sufA = tA, sufK = tK;
-            for (int k = w.warp; k >= 0; --k) {
-                const float4 f = ex[buf][k][w.lane];
-                then<CUTS>(tA, tK, make_float2(f.x, f.y), make_float2(f.z, f.w));
-            }
-            for (int k = w.warp; k < P; k += kWarps) st_cluster(smem_addr(&pub[buf][w.rank][w.lane]), k, make_float4(tA.x, tA.y, tK.x, tK.y));
-            cluster_sync();
-            for (int k = P - 1; k > w.rank; --k) {
-                const float4 f = pub[buf][k][w.lane];
-                run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
-            }
-            back = apply<CUTS>(sufA, sufK, run);
-            for (int k = w.rank; k >= 0; --k) {
-                const float4 f = pub[buf][k][w.lane];
-                run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
-            }
-        } else {
-            for (int k = kWarps - 1; k > w.warp; --k) {
-                const float4 f = ex[buf][k][w.lane];
-                run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
-            }
-            back = run;
-            for (int k = w.warp; k >= 0; --k) {
-                const float4 f = ex[buf][k][w.lane];
-                run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
-            }
+    };
+    auto publish = [&](int turn, Turn& q) {
+        float2 tA = f2(1.0f), tK = f2(0.0f);
+        for (int k = kWarps - 1; k > w.warp; --k) {
+            const float4 f = ex[turn & 1][k][w.lane];
+            then<CUTS>(tA, tK, make_float2(f.x, f.y), make_float2(f.z, f.w));
         }
-        if (!CUTS || starts == 0) {
+        q.sufA = tA;
+        q.sufK = tK;
+        for (int k = w.warp; k >= 0; --k) {
+            const float4 f = ex[turn & 1][k][w.lane];
+            then<CUTS>(tA, tK, make_float2(f.x, f.y), make_float2(f.z, f.w));
+        }
+        if constexpr (CLUSTER)
+            if (w.warp < P) st_cluster(smem_addr(&pub.v[turn & 1][w.rank][w.lane]), w.warp, make_float4(tA.x, tA.y, tK.x, tK.y));
+    };
+    auto enter = [&](const float4 (&from)[CLUSTER ? kMaxCluster : kWarps][32], int count, int here) -> float2 {
+        for (int k = count - 1; k > here; --k) {
+            const float4 f = from[k][w.lane];
+            run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
+        }
+        const float2 back = run;
+        for (int k = here; k >= 0; --k) {
+            const float4 f = from[k][w.lane];
+            run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
+        }
+        return back;
+    };
+    auto replay = [&](int turn, Turn& q) {
+        const int t0 = turn * P * kChunk + first;
+        float2 prev[S];
+        const bool cuts = CUTS && q.starts != 0;
 #pragma unroll
-            for (int j = 0; j < S; ++j) {
-                const float2 e = prev[j];
-                prev[j] = h;
-                h = fma(a[j], h, e);
-            }
+        for (int j = 0; j < S; ++j) {
+            if (cuts && (q.starts >> j & 1u)) q.h = state0(t0 + j);
+            prev[j] = q.h;
+            q.h = fma(q.a[j], q.h, mul(q.msi[j], q.x[j]));
+        }
 #pragma unroll
-            for (int j = S - 1; j >= 0; --j) {
-                G[j] = add(G[j], back);
-                back = mul(a[j], G[j]);                 // (past the end a is 1 and dy 0)
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < S; ++j) {
-                const float2 e = prev[j];
-                if (starts >> j & 1u) h = state0(t0 + j);
-                prev[j] = h;
-                h = fma(a[j], h, e);
-            }
-#pragma unroll
-            for (int j = S - 1; j >= 0; --j) {
-                G[j] = add(G[j], back);
-                back = mul(a[j], G[j]);
-                if (starts >> j & 1u) {
-                    Seq<MODE> q = seq;
-                    q.at(t0 + j);
-                    if (o.dh0) store_state(o.dh0, q.s, D, w.d, back, w.has0, w.has1);
-                    back = back0(t0 + j - 1);
-                }
+        for (int j = S - 1; j >= 0; --j) {        // dy becomes G
+            q.g[j] = add(q.g[j], q.back);
+            q.back = mul(q.a[j], q.g[j]);         // (past the end a is 1 and dy 0)
+            if (cuts && (q.starts >> j & 1u)) {
+                Seq<MODE> z = seq;
+                z.at(t0 + j);
+                if (o.dh0) store_state(o.dh0, z.s, D, w.d, q.back, w.has0, w.has1);
+                q.back = back0(t0 + j - 1);
             }
         }
-        T *px = dx + (int64_t)t0 * D, *pr = dr + (int64_t)t0 * D, *pi = di + (int64_t)t0 * D;
+        const int64_t out = base + (int64_t)t0 * D;
+        T *px = static_cast<T*>(o.dx) + out, *pr = static_cast<T*>(o.dr) + out, *pi = static_cast<T*>(o.di) + out;
         const bool full = t0 + S <= L;
 #pragma unroll
         for (int j = 0; j < S; ++j) {
-            const float2 vx = mul(G[j], msi[j]);
-            const float2 vi = mul(mul(vx, xv[j]), fma(sgi[j], f2(-1.0f), f2(1.0f)));
+            const float2 vx = mul(q.g[j], q.msi[j]);
+            const float2 vi = mul(mul(vx, q.x[j]), fma(q.si[j], nones, consts.one));
             // du = G a (prev - (a / m) sigmoid(i) x)
-            const float2 slope = mul(mul(a[j], rs[j]), mul(sgi[j], xv[j]));
-            const float2 du = mul(mul(G[j], a[j]), fma(slope, f2(-1.0f), prev[j]));
-            const float2 ds = mul(du, sgr[j]);
-            const float2 vr = mul(mul(ds, ncs), fma(sgr[j], f2(-1.0f), f2(1.0f)));
+            const float2 slope = mul(mul(q.a[j], q.rs[j]), mul(q.si[j], q.x[j]));
+            const float2 du = mul(mul(q.g[j], q.a[j]), fma(slope, nones, prev[j]));
+            const float2 ds = mul(du, q.sr[j]);
+            const float2 vr = mul(mul(ds, cs), add(q.sr[j], nones));
             if (full || t0 + j < L) {
                 sum = add(sum, ds);
                 store_pair<T, EVEN>(px, vx, even_rows, w.has0, w.has1);
@@ -767,6 +798,24 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
             pr += D;
             pi += D;
         }
+    };
+
+    if (CLUSTER) {
+        cluster_arrive();
+        cluster_wait();
+    }
+    for (int turn = turns - 1; turn >= 0; --turn) {
+        Turn q;
+        prepare(turn, q);
+        if constexpr (CLUSTER) {
+            publish(turn, q);
+            cluster_arrive();
+            cluster_wait();
+            q.back = apply<CUTS>(q.sufA, q.sufK, enter(pub.v[turn & 1], P, w.rank));
+        } else {
+            q.back = enter(ex[turn & 1], kWarps, w.warp);
+        }
+        replay(turn, q);
     }
     __syncthreads();
     exh[0][w.warp][w.lane] = sum;
@@ -781,7 +830,7 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         if (w.warp == 0) store_state(o.dh0, w.b, D, w.d, run, w.has0, w.has1);
     } else if (MODE == kPacked) {
         for (int64_t s = w.warp; s < n.n; s += kWarps)
-            if (n.cu[s] >= n.cu[s + 1])
+            if (seq.cu[s] >= seq.cu[s + 1])
                 store_state(o.dh0, s, D, w.d, load_state(o.dh_last, s, D, w.d, w.has0, w.has1), w.has0, w.has1);
     }
 }
@@ -811,10 +860,11 @@ __global__ void rec_step_kernel(RecPtr p, int64_t B, int64_t D, const float* __r
     const int64_t n = B * D, stride = (int64_t)gridDim.x * blockDim.x;
     for (int64_t k = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; k < n; k += stride) {
         const int64_t b = k / D, d = k - b * D;
+        const Consts consts;
         float prod;
         const Gates g = gates<false>(f2(to_f32<T>(static_cast<const T*>(p.r)[b * p.rb + d])),
-                                     f2(to_f32<T>(static_cast<const T*>(p.i)[b * p.ib + d])), f2(-c * softplus_(lam[d])), prod);
-        const float v = fmaf(1.0f + g.w.x, h[k], m_of(g.w, g.rs).x * g.si.x * to_f32<T>(static_cast<const T*>(p.x)[b * p.xb + d]));
+                                     f2(to_f32<T>(static_cast<const T*>(p.i)[b * p.ib + d])), f2(c * softplus_(lam[d])), consts, prod);
+        const float v = fmaf(g.a.x, h[k], g.m.x * g.si.x * to_f32<T>(static_cast<const T*>(p.x)[b * p.xb + d]));
         h[k] = v;
         y[k] = from_f32<T>(v);
     }
@@ -901,7 +951,6 @@ bcm_status rec_launch_as(F* kernel, int smem, const bcm_gated_rec_args* a, const
     cfg.attrs = attr;
     cfg.numAttrs = pl.P > 1 ? 1 : 0;
     BCM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    if (pl.P > 8) BCM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     const RecDim n = {a->cu_seqlens, a->batch, pl.L, (int)a->seqlen, pl.per, (int)a->dim, pl.P};
     BCM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, rec_ptr(a), o, n, a->lam, a->decay_scale));
     return BCM_OK;

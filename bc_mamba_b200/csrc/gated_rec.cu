@@ -119,7 +119,8 @@ __device__ __forceinline__ Gates gates(float2 r, float2 i, float2 cs, const Cons
 //
 // Mode: kDense, one sequence per block; kGroup, a block takes `per` consecutive
 // dense sequences as one run of tokens (short sequences would leave most of a
-// chunk empty); kPacked, one run of tokens with the sequences' offsets in cu.
+// chunk empty); kPacked, the sequences' offsets stand in cu, and run g of G takes
+// the sequences that start in the g-th part of the tokens (found on the device).
 // Where a sequence starts inside a run, nothing passes and its own state enters.
 constexpr int kWarps = 8;
 constexpr int kTile = 64;                        // features of a block
@@ -140,12 +141,12 @@ struct RecOut {
     const float* dh_last; void* dx; void* dr; void* di; float* part; float* dh0;   // backward
 };
 
-// A run holds L tokens (kGroup: its last may hold fewer), a sequence Ls (kDense, kGroup), per sequences make a run
-// (kGroup); n sequences, D features, P blocks in a cluster.
+// A run holds L tokens (kGroup: its last may hold fewer; kPacked: all runs together), a sequence Ls (kDense, kGroup),
+// per sequences make a run (kGroup), runs of them (kPacked); n sequences, D features, P blocks in a cluster.
 struct RecDim {
     const int32_t* cu;
     int64_t n;
-    int L, Ls, per, D, P;
+    int L, Ls, per, runs, D, P;
 };
 
 // The sequence that holds token t: the last s with cu[s] <= t, in [0, n).  Called by whole warps; t is uniform.
@@ -166,16 +167,16 @@ __device__ __forceinline__ int seq_of(const int32_t* cu, int n, int t) {
 template <int MODE>
 struct Seq {
     const int32_t* cu;
-    int n, Ls;
+    int n, Ls, off;           // off: the run's first token (kPacked)
     int64_t s0, s;
     int beg, end;
     __device__ __forceinline__ void at(int t) {
         if (MODE == kDense || (beg <= t && t < end)) return;
         if (MODE == kPacked) {
-            const int k = seq_of(cu, n, t);
+            const int k = seq_of(cu, n, t + off);
             s = k;
-            beg = cu[k];
-            end = cu[k + 1];
+            beg = cu[k] - off;
+            end = cu[k + 1] - off;
         } else {
             const int k = t / Ls;
             s = s0 + k;
@@ -221,12 +222,14 @@ __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0
 // Where a block works.
 struct Place {
     int lane, warp, rank, tile, d, L;
-    int64_t run, b;           // the run and its first sequence
+    int off;                  // the run's first token (kPacked)
+    int64_t run, b;           // the run and its first sequence (kDense, kGroup)
     bool has0, has1;          // the lane's features exist
 };
 template <int MODE, bool CLUSTER>
-__device__ __forceinline__ Place place(const RecDim& n) {
+__device__ __forceinline__ Place place(const RecDim& n, const int32_t* cu) {
     Place q;
+    q.off = 0;
     q.lane = threadIdx.x & 31;
     q.warp = threadIdx.x >> 5;
     const int P = CLUSTER ? n.P : 1, tiles = (n.D + kTile - 1) / kTile;
@@ -238,6 +241,16 @@ __device__ __forceinline__ Place place(const RecDim& n) {
     q.d = q.tile * kTile + q.lane * 2;
     q.has0 = q.d < n.D;
     q.has1 = q.d + 1 < n.D;
+    if (MODE == kPacked && n.runs > 1) {
+        // from the first start at or after run * L / runs to that at or after (run + 1) * L / runs
+        int at[2] = {0, n.L};
+        for (int k = 0; k < 2; ++k) {
+            const int64_t edge = (q.run + k) * n.L / n.runs;
+            if (edge > 0 && edge < n.L) at[k] = min(max(cu[seq_of(cu, (int)n.n, (int)edge - 1) + 1], 0), n.L);
+        }
+        q.off = at[0];
+        q.L = max(at[1] - at[0], 0);
+    }
     return q;
 }
 
@@ -282,6 +295,7 @@ struct Stream {
     using R = Rows<T, EVEN>;
     static constexpr int kLaneRows = EVEN ? 32 / R::kGran : 1;      // rows of a warp's copy instruction
     const char* at;
+    int bytes;
     __device__ __forceinline__ static bool linear(const Input& in, const RecDim& n) { return MODE != kGroup || in.sb == in.st * n.Ls; }
     // elements from the run's first row to that of token t
     __device__ __forceinline__ static int64_t row(const Input& in, const RecDim& n, int t) {
@@ -290,16 +304,16 @@ struct Stream {
         return k * in.sb + (int64_t)(t - k * n.Ls) * in.st;
     }
     __device__ __forceinline__ static const T* base(const Input& in, const Place& w) {
-        return static_cast<const T*>(in.p) + (MODE == kPacked ? 0 : w.b * in.sb) + (int64_t)w.tile * kTile;
+        return static_cast<const T*>(in.p) + (MODE == kPacked ? w.off * in.st : w.b * in.sb) + (int64_t)w.tile * kTile;
     }
-    __device__ __forceinline__ Stream(const Input& in, const Place& w, int t0) {
+    __device__ __forceinline__ Stream(const Input& in, const Place& w, int t0, int width) {
+        bytes = max(0, min(16, width * (int)sizeof(T) - w.lane % R::kGran * 16));
         if (EVEN) at = reinterpret_cast<const char*>(base(in, w) + (int64_t)(t0 + w.lane / R::kGran) * in.st) + w.lane % R::kGran * 16;
     }
     // t0: the first row; advance: tokens from this fetch to the next; rows and features that are not there become zeros
     __device__ __forceinline__ void fetch(char* dst, const Input& in, const Place& w, const RecDim& n, int t0, int advance, int width) {
         const uint32_t to = smem_addr(dst);
         if (EVEN && t0 + S <= w.L && linear(in, n)) {
-            const int bytes = max(0, min(16, width * (int)sizeof(T) - w.lane % R::kGran * 16));
 #pragma unroll
             for (int k = 0; k < S / kLaneRows; ++k)
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + w.lane * 16 + k * 512),
@@ -367,6 +381,12 @@ __device__ __forceinline__ void store_state(float* p, int64_t row, int D, int d,
     if (has1) p[row * D + d + 1] = v.y;
 }
 
+// The run's first row of kept states.
+template <int MODE>
+__device__ __forceinline__ int64_t ckpt_row(const Place& w, const RecDim& n) {
+    return MODE == kPacked ? w.off / kCkpt + w.run : w.run * ((n.L + kCkpt - 1) / kCkpt);
+}
+
 // Bit j: a sequence starts at token t0 + j.
 template <int MODE, int S>
 __device__ __forceinline__ unsigned starts_in(const Seq<MODE>& seq, int t0, int L) {
@@ -417,19 +437,20 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
     __shared__ Pub<CLUSTER> pub;
     __shared__ int32_t cus[MODE == kPacked ? kCuMax : 1];
     extern __shared__ __align__(16) char rows[];
-    const Place w = place<MODE, CLUSTER>(n);
+    const int32_t* cu = stage_cu<MODE>(n, cus);
+    const Place w = place<MODE, CLUSTER>(n, cu);
     const int D = n.D, L = w.L, P = CLUSTER ? n.P : 1, width = min(kTile, D - w.tile * kTile);
-    T* y = static_cast<T*>(o.y) + (MODE == kPacked ? 0 : w.b * n.Ls * D) + w.d;
+    T* y = static_cast<T*>(o.y) + (MODE == kPacked ? (int64_t)w.off : w.b * n.Ls) * D + w.d;
     const bool even_rows = (D & 1) == 0 && (uintptr_t)o.y % (2 * sizeof(T)) == 0;
-    const int turns = ((n.L + kChunk - 1) / kChunk + P - 1) / P;
-    float* ck = o.ckpt ? o.ckpt + w.run * ((n.L + kCkpt - 1) / kCkpt) * D : nullptr;
+    const int turns = (((MODE == kPacked ? L : n.L) + kChunk - 1) / kChunk + P - 1) / P;
+    float* ck = o.ckpt ? o.ckpt + ckpt_row<MODE>(w, n) * D : nullptr;
     const float2 l = load_state(lam, 0, D, w.d, w.has0, w.has1);
     const float2 cs = make_float2(w.has0 ? c * softplus_(l.x) : kPolyEnd, w.has1 ? c * softplus_(l.y) : kPolyEnd);
     const bool small = __all_sync(kFull, cs.x >= kCsLow && cs.x <= kPolyEnd && cs.y >= kCsLow && cs.y <= kPolyEnd);
     const Consts consts;
     const int first = w.rank * kChunk + w.warp * S;
     const Input ix = {p.x, p.xb, p.xt}, ir = {p.r, p.rb, p.rt}, ii = {p.i, p.ib, p.it};
-    In sx(ix, w, first), sr(ir, w, first), si(ii, w, first);
+    In sx(ix, w, first, width), sr(ir, w, first, width), si(ii, w, first, width);
     char* mine = rows + w.warp * (3 * S * R::kPitch);
     auto fetch = [&](int turn) {
         if (turn < turns) {
@@ -443,7 +464,7 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
     };
 #pragma unroll
     for (int k = 0; k < ST - 1; ++k) fetch(k);
-    Seq<MODE> seq{stage_cu<MODE>(n, cus), (int)n.n, n.Ls, w.b, 0, 0, 0};
+    Seq<MODE> seq{cu, (int)n.n, n.Ls, w.off, w.b, 0, 0, 0};
     float2 run = MODE == kDense ? load_state(o.h0, w.b, D, w.d, w.has0, w.has1) : f2(0.0f);
 
     // gates and composition of a turn: h -> a_j h + e_j token by token, h -> A h + H together
@@ -526,12 +547,11 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
     };
     // the state that enters the warp's tokens; run moves on to the next turn
     auto enter = [&](const float4 (&from)[CLUSTER ? kMaxCluster : kWarps][32], int count, int here) -> float2 {
-        for (int k = 0; k < here; ++k) {
-            const float4 f = from[k][w.lane];
-            run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
-        }
-        const float2 h = run;
-        for (int k = here; k < count; ++k) {
+        float2 h = run;
+#pragma unroll
+        for (int k = 0; k < (CLUSTER ? kMaxCluster : kWarps); ++k) {
+            if (k >= count) break;
+            if (k == here) h = run;
             const float4 f = from[k][w.lane];
             run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
         }
@@ -584,7 +604,7 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         }
         replay(turn, a, e, starts, h);
     }
-    if (w.rank != 0) return;
+    if (w.rank != 0 || (MODE == kPacked && w.run != 0)) return;
     if (MODE == kDense) {
         if (w.warp == 0) store_state(o.h_last, w.b, D, w.d, run, w.has0, w.has1);
     } else if (MODE == kPacked) {
@@ -610,12 +630,13 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
     __shared__ Pub<CLUSTER> pub;
     __shared__ int32_t cus[MODE == kPacked ? kCuMax : 1];
     extern __shared__ __align__(16) char rows[];
-    const Place w = place<MODE, CLUSTER>(n);
+    const int32_t* cu = stage_cu<MODE>(n, cus);
+    const Place w = place<MODE, CLUSTER>(n, cu);
     const int D = n.D, L = w.L, P = CLUSTER ? n.P : 1, width = min(kTile, D - w.tile * kTile);
-    const int64_t base = (MODE == kPacked ? 0 : w.b * n.Ls * D) + w.d;
+    const int64_t base = (MODE == kPacked ? (int64_t)w.off : w.b * n.Ls) * D + w.d;
     const bool even_rows = (D & 1) == 0 && ((uintptr_t)o.dx | (uintptr_t)o.dr | (uintptr_t)o.di) % (2 * sizeof(T)) == 0;
-    const int turns = ((n.L + kChunk - 1) / kChunk + P - 1) / P;
-    const float* ck = o.ckpt + w.run * ((n.L + kCkpt - 1) / kCkpt) * D;
+    const int turns = (((MODE == kPacked ? L : n.L) + kChunk - 1) / kChunk + P - 1) / P;
+    const float* ck = o.ckpt + ckpt_row<MODE>(w, n) * D;
     const float2 l = load_state(lam, 0, D, w.d, w.has0, w.has1);
     const float2 cs = make_float2(w.has0 ? c * softplus_(l.x) : kPolyEnd, w.has1 ? c * softplus_(l.y) : kPolyEnd);
     const bool small = __all_sync(kFull, cs.x >= kCsLow && cs.x <= kPolyEnd && cs.y >= kCsLow && cs.y <= kPolyEnd);
@@ -623,7 +644,7 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
     const int first = w.rank * kChunk + w.warp * S, last = (turns - 1) * P * kChunk + first;
     // (without dy: rows of no width, zeros)
     const Input ix = {p.x, p.xb, p.xt}, ir = {p.r, p.rb, p.rt}, ii = {p.i, p.ib, p.it}, ig = {p.dy ? p.dy : p.x, p.gb, p.gt};
-    In sx(ix, w, last), sr(ir, w, last), si(ii, w, last), sg(ig, w, last);
+    In sx(ix, w, last, width), sr(ir, w, last, width), si(ii, w, last, width), sg(ig, w, last, p.dy ? width : 0);
     char* mine = rows + w.warp * (4 * S * R::kPitch);
     auto fetch = [&](int turn) {
         if (turn >= 0) {
@@ -639,8 +660,8 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
     constexpr int kAhead = ST - 1;                // turns in flight beyond the one being prepared
 #pragma unroll
     for (int k = 1; k <= kAhead; ++k) fetch(turns - k);
-    Seq<MODE> seq{stage_cu<MODE>(n, cus), (int)n.n, n.Ls, w.b, 0, 0, 0};
-    seq.at(L - 1);
+    Seq<MODE> seq{cu, (int)n.n, n.Ls, w.off, w.b, 0, 0, 0};
+    if (L > 0) seq.at(L - 1);
     float2 run = load_state(o.dh_last, CUTS ? seq.s : w.b, D, w.d, w.has0, w.has1), sum = f2(0.0f);
     auto state0 = [&](int t) -> float2 {          // the state that enters the sequence of token t
         Seq<MODE> q = seq;
@@ -744,12 +765,11 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
             if (w.warp < P) st_cluster(smem_addr(&pub.v[turn & 1][w.rank][w.lane]), w.warp, make_float4(tA.x, tA.y, tK.x, tK.y));
     };
     auto enter = [&](const float4 (&from)[CLUSTER ? kMaxCluster : kWarps][32], int count, int here) -> float2 {
-        for (int k = count - 1; k > here; --k) {
-            const float4 f = from[k][w.lane];
-            run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
-        }
-        const float2 back = run;
-        for (int k = here; k >= 0; --k) {
+        float2 back = run;
+#pragma unroll
+        for (int k = (CLUSTER ? kMaxCluster : kWarps) - 1; k >= 0; --k) {
+            if (k >= count) continue;
+            if (k == here) back = run;
             const float4 f = from[k][w.lane];
             run = apply<CUTS>(make_float2(f.x, f.y), make_float2(f.z, f.w), run);
         }
@@ -825,7 +845,7 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         for (int k = 0; k < kWarps; ++k) s = add(s, exh[0][k][w.lane]);
         store_state(o.part, w.run * P + w.rank, D, w.d, s, w.has0, w.has1);
     }
-    if (w.rank != 0 || !o.dh0) return;
+    if (w.rank != 0 || !o.dh0 || (MODE == kPacked && w.run != 0)) return;
     if (MODE == kDense) {
         if (w.warp == 0) store_state(o.dh0, w.b, D, w.d, run, w.has0, w.has1);
     } else if (MODE == kPacked) {
@@ -903,8 +923,11 @@ Plan rec_plan(const bcm_gated_rec_args* a) {
     constexpr int kChunk = kWarps * kStepsFwd;
     Plan pl = {kDense, 1, (int)a->seqlen, 1, a->batch, rec_parts(a->dim, kTile)};
     if (a->cu_seqlens) {
+        // Runs need no exchange, but a long sequence leaves them uneven: one for every four sequences at most, and no
+        // more than two blocks per SM take; clusters fill the rest.
         pl.mode = kPacked;
         pl.runs = 1;
+        while (pl.runs * 8 <= a->batch && pl.tiles * pl.runs <= (int64_t)sm_count() && pl.runs * 2 * kChunk <= a->seqlen) pl.runs *= 2;
     } else if (a->seqlen < 4 * kChunk && a->batch > 1) {
         // runs of about 8 chunks (an eighth of the last one empty at most), fewer where that leaves SMs without a block
         pl.mode = kGroup;
@@ -915,7 +938,7 @@ Plan rec_plan(const bcm_gated_rec_args* a) {
         pl.runs = rec_parts(a->batch, pl.per);
     }
     // blocks of a cluster: as many as the chunks allow and two blocks per SM hold at once
-    while (pl.P < kMaxCluster && pl.runs * pl.tiles * pl.P <= (int64_t)sm_count() && 2 * pl.P <= rec_parts(pl.L, kChunk)) pl.P *= 2;
+    while (pl.P < kMaxCluster && pl.runs * pl.tiles * pl.P <= (int64_t)sm_count() && 2 * pl.P <= rec_parts(pl.mode == kPacked ? pl.L / pl.runs : pl.L, kChunk)) pl.P *= 2;
     return pl;
 }
 
@@ -951,7 +974,7 @@ bcm_status rec_launch_as(F* kernel, int smem, const bcm_gated_rec_args* a, const
     cfg.attrs = attr;
     cfg.numAttrs = pl.P > 1 ? 1 : 0;
     BCM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    const RecDim n = {a->cu_seqlens, a->batch, pl.L, (int)a->seqlen, pl.per, (int)a->dim, pl.P};
+    const RecDim n = {a->cu_seqlens, a->batch, pl.L, (int)a->seqlen, pl.per, (int)pl.runs, (int)a->dim, pl.P};
     BCM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, rec_ptr(a), o, n, a->lam, a->decay_scale));
     return BCM_OK;
 }
@@ -993,7 +1016,8 @@ extern "C" size_t bcm_gated_rec_ckpt_bytes(const bcm_gated_rec_args* a) {
     if (!a || a->batch < 0 || a->seqlen < 0 || a->dim < 1) return 0;
     if (rec_rows(a) == 0) return 0;
     const Plan pl = rec_plan(a);
-    return align_up((size_t)pl.runs * (size_t)rec_parts(pl.L, kCkpt) * (size_t)a->dim * sizeof(float), 256);
+    const int64_t states = pl.mode == kPacked ? rec_parts(pl.L, kCkpt) + pl.runs + 1 : pl.runs * rec_parts(pl.L, kCkpt);
+    return align_up((size_t)states * (size_t)a->dim * sizeof(float), 256);
 }
 
 extern "C" size_t bcm_gated_rec_bwd_workspace_bytes(const bcm_gated_rec_args* a) {

@@ -101,6 +101,16 @@ def test_packed(cu, D, dtype):
     _check(_inputs(cu[-1], D, len(cu) - 1, dtype, seed=len(cu) + D), cu, None)
 
 
+@pytest.mark.parametrize("seed,n,T,D", [(0, 9, 700, 40), (1, 64, 5000, 6), (2, 200, 9000, 70), (3, 1500, 3000, 3), (4, 40, 20000, 2)])
+def test_packed_runs(seed, n, T, D):
+    """Many sequences of uneven length, cut at random (some empty), and one that takes nearly every token."""
+    rng = np.random.default_rng(seed)
+    cu = [0, *np.sort(rng.integers(0, T + 1, n - 1)).tolist(), T]
+    _check(_inputs(T, D, n, torch.float32, seed), cu, None)
+    cu = [0] * (n // 2) + [5] * (n // 4) + [T] * (n + 1 - n // 2 - n // 4)
+    _check(_inputs(T, D, n, torch.bfloat16, seed), cu, None)
+
+
 @pytest.mark.parametrize("h0,dy,dh", [(False, True, False), (True, False, True), (False, True, True)])
 def test_optional_parts(h0, dy, dh):
     _check(_inputs(2 * 150, 40, 2, torch.float32, seed=1), (0, 150, 300), (2, 150), h0, dy, dh)

@@ -1,30 +1,24 @@
-// sample.cu — one token per row from its logits and a given uniform number,
-// with temperature, top-k, top-p and min-p.
-//
-// Row b, T = temperature[b]; T <= 0 (or NaN, or so small that 1/T overflows)
-// means greedy: 1/T is taken as 1 and top_k as 1.
-//   s_v = (logit_v - max logit) * (1/T)  (fp32, 0 at the maximum; a NaN logit
-//         counts as -inf; s = -inf is never taken)
-//   e_v = exp(s_v),  w_v = floor(e_v 2^40)   (integer weight)
-// In descending order of s (equal s in ascending order of index):
-//   top-k  keeps the first k (k <= 0: all);
-//   top-p  keeps of these the tokens whose preceding weight is below
-//          ceil(p * total weight of these), the first always (p >= 1: all);
-//   min-p  keeps of these the tokens with e_v >= min(min_p, 1).
-// The token is the first, in ascending order of index, whose inclusive kept
-// weight exceeds floor(u * total kept weight).  Weights are integers, so sums
-// are exact and no order of summation changes a token.
 #include <algorithm>
+#include <cstring>
 
 #include "common.cuh"
 
 namespace bcm {
 namespace {
 
-constexpr int kThreads = 1024;
+// A cluster of C blocks keeps a row in shared memory, in 16-byte granules (rows may
+// start anywhere).  One pass counts the tokens in buckets of s; the buckets bound the
+// mass above every cut, so that one more pass leaves a short list of tokens around
+// the cut: the rest is certainly kept or certainly not.  The first block sorts the
+// list and finds the cut exactly; the warp whose tokens hold the target walks them.
+constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
+constexpr int kMaxCluster = 8;
+constexpr int kBuckets = 4096;
+constexpr int kListMax = 4096;                   // tokens around the cut
 constexpr float kInf = __builtin_huge_valf();
-constexpr float kOne = 1099511627776.0f;   // 2^40
+constexpr float kOne = 1099511627776.0f;         // 2^40
+constexpr float kEnd = 27.75f;                   // e^-27.75 2^40 < 1: further down tokens weigh nothing
 
 typedef unsigned long long u64;
 
@@ -32,15 +26,31 @@ typedef unsigned long long u64;
 __device__ __forceinline__ uint32_t key_of(float s) { return 0x7f800000u - __float_as_uint(-s); }
 __device__ __forceinline__ float from_key(uint32_t k) { return -__uint_as_float(0x7f800000u - k); }
 
-template <typename T>
-__device__ __forceinline__ float scaled(const T* x, int64_t v, float top, float it) {
-    const float l = to_f32<T>(x[v]);
+__device__ __forceinline__ float scale_logit(float l, float top, float it) {
     const float s = l == top ? 0.0f : (l - top) * it;
-    return s <= 0.0f ? fabsf(s) * -1.0f : -kInf;   // -0 for 0; NaN to -inf
+    return s <= 0.0f ? -fabsf(s) : -kInf;        // -0 for 0; NaN to -inf
 }
+template <typename T>
+__device__ __forceinline__ float scaled(const T* x, int64_t v, float top, float it) { return scale_logit(to_f32<T>(x[v]), top, it); }
 
 __device__ __forceinline__ float rel_weight(float s) { return expf(s); }
 __device__ __forceinline__ u64 weight_of(float e) { return (u64)(e * kOne); }
+
+// Sums of weights in two 32-bit limbs of 20 bits (adding 2^23 with rounding down leaves the integer in the mantissa);
+// exact for fewer than 4096 terms.
+struct Sum {
+    uint32_t hi = 0, lo = 0, n = 0;
+    __device__ __forceinline__ void add(float e) {
+        const float t = __fmaf_rd(e, 1048576.0f, 8388608.0f);                       // 2^23 + floor(e 2^20)
+        const float rest = fmaf(e, 1048576.0f, 8388608.0f - t);                     // exact, in [0, 1)
+        hi += __float_as_uint(t);
+        lo += __float_as_uint(__fmaf_rd(rest, 1048576.0f, 8388608.0f));
+        ++n;
+    }
+    __device__ __forceinline__ u64 value() const {
+        return ((u64)(hi - n * 0x4b000000u) << 20) + (u64)(lo - n * 0x4b000000u);
+    }
+};
 
 template <typename V>
 __device__ V block_sum_u(V v, V* red) {
@@ -85,14 +95,13 @@ __device__ uint32_t select_key(const T* x, int64_t V, float top, float it, u64 s
     return prefix;
 }
 
+// A row by one block that reads it again for every digit: rows whose cut falls into a bucket of more than kListMax
+// tokens (mostly equal logits), and top-k beyond the list together with top-p.  131072 equal bf16 logits: @SLOW@.
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-sample_kernel(const bcm_sample_args a) {
+__device__ void sample_by_digits(const bcm_sample_args& a, int64_t b, float top) {
     __shared__ u64 red[kWarps];
     __shared__ u64 hist[256];
-    __shared__ float fred[kWarps];
     __shared__ int64_t s_cut;
-    const int64_t b = blockIdx.x;
     const int64_t V = a.vocab;
     const T* x = static_cast<const T*>(a.logits) + b * a.logits_stride;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -106,20 +115,6 @@ sample_kernel(const bcm_sample_args a) {
     const float mp = a.min_p ? a.min_p[b] : a.min_p_all;
     const float least = mp > 0.0f ? fminf(mp, 1.0f) : 0.0f;
 
-    float top = -kInf;
-    for (int64_t v = threadIdx.x; v < V; v += kThreads) top = fmaxf(top, to_f32<T>(x[v]));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
-    if (lane == 0) fred[warp] = top;
-    __syncthreads();
-    for (int j = 0; j < kWarps; ++j) top = fmaxf(top, fred[j]);
-    if (top == -kInf) {
-        if (threadIdx.x == 0) {
-            a.tokens[b] = -1;
-            a.logprob[b] = -kInf;
-        }
-        return;
-    }
     u64 n_valid = 0;
     for (int64_t v = threadIdx.x; v < V; v += kThreads) n_valid += key_of(scaled<T>(x, v, top, it)) != 0u;
     n_valid = block_sum_u<u64>(n_valid, red);
@@ -223,6 +218,453 @@ sample_kernel(const bcm_sample_args a) {
     }
 }
 
+// ---- the cluster's shared memory --------------------------------------------------
+__device__ __forceinline__ uint32_t remote(const void* p, int rank) {
+    uint32_t a = (uint32_t)__cvta_generic_to_shared(p), r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void st_remote(uint32_t a, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
+__device__ __forceinline__ void st_remote(uint32_t a, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory"); }
+__device__ __forceinline__ uint32_t ld_remote(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t add_remote(uint32_t a, uint32_t v) {
+    uint32_t o;
+    asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(o) : "r"(a), "r"(v) : "memory");
+    return o;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+struct Shared {
+    float tops[kMaxCluster];
+    float fred[kWarps];
+    u64 red[kWarps];
+    // per warp of the cluster, at rank 0: the weight above the window, all of it and what min-p keeps, and that below it
+    u64 kept[kMaxCluster * kWarps], all[kMaxCluster * kWarps], rest[kMaxCluster * kWarps];
+    // from rank 0 to all: the window of buckets (first, end), what to do, then the cut and the target
+    uint32_t win_lo, win_hi, mode, list_n;
+    uint32_t k_left;                             // how many of the list's tokens top-k leaves (rank 0)
+    uint32_t cut_d, cut_v, seg;                  // the last kept token (-s, index); the warp that holds the target
+    u64 target, total;                           // the target within that warp's tokens; the kept weight
+};
+enum { kPlain, kWindow, kDigits };
+
+// Granule g of the row: its elements as floats, those outside the row -inf.
+template <typename T>
+struct Granule {
+    static constexpr int N = 16 / (int)sizeof(T);
+    float f[N];
+    __device__ __forceinline__ void unpack(uint4 w) {
+        T t[N];
+        memcpy(t, &w, 16);
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = to_f32<T>(t[e]);
+    }
+    __device__ __forceinline__ void trim(int64_t g, int64_t last, int shift, int64_t V) {
+        if (g == 0 || g == last)
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (g * N + e < shift || g * N + e - shift >= V) f[e] = -kInf;
+    }
+};
+
+// The list in ascending order (bitonic network over the next power of two, rest ~0).
+__device__ void sort_list(u64* list, int n) {
+    int m = 1;
+    while (m < n) m <<= 1;
+    for (int k = n + threadIdx.x; k < m; k += kThreads) list[k] = ~0ull;
+    __syncthreads();
+    for (int size = 2; size <= m; size <<= 1)
+        for (int step = size >> 1; step > 0; step >>= 1) {
+            for (int k = threadIdx.x; k < m / 2; k += kThreads) {
+                const int i = 2 * k - (k & (step - 1)), j = i + step;
+                const u64 x = list[i], y = list[j];
+                if ((x > y) == ((i & size) == 0)) {
+                    list[i] = y;
+                    list[j] = x;
+                }
+            }
+            __syncthreads();
+        }
+}
+
+// KEEP: the cluster's slices of the row stay in shared memory (otherwise every pass reads the row from L2).
+template <typename T, bool KEEP>
+__global__ void __launch_bounds__(kThreads, 2)
+sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
+    using Gr = Granule<T>;
+    extern __shared__ __align__(16) char dyn[];
+    __shared__ Shared sh;
+    u64* list = reinterpret_cast<u64*>(dyn);                         // rank 0: after the buckets are done
+    uint32_t* hist = reinterpret_cast<uint32_t*>(dyn);
+    uint4* slice = reinterpret_cast<uint4*>(dyn + kListMax * 8);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = blockIdx.x % C;
+    const int64_t b = blockIdx.x / C, V = a.vocab;
+    const T* x = static_cast<const T*>(a.logits) + b * a.logits_stride;
+    const int shift = (int)((uintptr_t)x & 15) / (int)sizeof(T);
+    const uint4* row = reinterpret_cast<const uint4*>((uintptr_t)x & ~(uintptr_t)15);
+    const int64_t grans = (shift + V + Gr::N - 1) / Gr::N, last = grans - 1;
+    const int64_t per = (grans + C - 1) / C, wper = (per + kWarps - 1) / kWarps;
+    // the warp's granules: a contiguous range, so that warps follow one another in index order
+    const int64_t g0 = rank * per + warp * wper, g1 = min(min(g0 + wper, (rank + 1) * per), grans), s0 = rank * per;
+    const float temp = a.temperature ? a.temperature[b] : a.temperature_all;
+    const float inv = 1.0f / temp;
+    const bool warm = temp > 0.0f && inv < kInf;
+    const float it = warm ? inv : 1.0f;
+    int64_t k = warm ? (a.top_k ? a.top_k[b] : a.top_k_all) : 1;
+    if (k <= 0 || k > V) k = V;
+    const float p = a.top_p ? a.top_p[b] : a.top_p_all;
+    const float mp = a.min_p ? a.min_p[b] : a.min_p_all;
+    const float least = mp > 0.0f ? fminf(mp, 1.0f) : 0.0f;
+    const bool use_k = k < V, use_p = p < 1.0f;
+
+    // the row comes in; its maximum
+    float top = -kInf;
+#pragma unroll 4
+    for (int64_t g = g0 + lane; g < g1; g += 32) {
+        const uint4 w = row[g];
+        if (KEEP) slice[g - s0] = w;
+        Gr q;
+        q.unpack(w);
+        q.trim(g, last, shift, V);
+#pragma unroll
+        for (int e = 0; e < Gr::N; ++e) top = fmaxf(top, q.f[e]);
+    }
+    for (int j = tid; j < kBuckets; j += kThreads) hist[j] = 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+    if (lane == 0) sh.fred[warp] = top;
+    if (tid == 0) sh.list_n = 0;
+    __syncthreads();
+    for (int j = 0; j < kWarps; ++j) top = fmaxf(top, sh.fred[j]);
+    if (C > 1) {
+        cluster_sync();                                   // every block runs before its shared memory is written to
+        if (tid < C) st_remote(remote(&sh.tops[rank], tid), __float_as_uint(top));
+        cluster_sync();
+        for (int j = 0; j < C; ++j) top = fmaxf(top, sh.tops[j]);
+    }
+    if (top == -kInf) {
+        if (rank == 0 && tid == 0) {
+            a.tokens[b] = -1;
+            a.logprob[b] = -kInf;
+        }
+        return;
+    }
+    auto each = [&](auto&& f) {                           // f(index of the first element, elements) over the warp's granules
+        for (int64_t g = g0 + lane; g < g1; g += 32) {
+            Gr q;
+            q.unpack(KEEP ? slice[g - s0] : row[g]);
+            q.trim(g, last, shift, V);
+            f(g * Gr::N - shift, q);
+        }
+    };
+
+    // buckets of s, counted; the first block finds the window of buckets that holds the cut
+    if (use_k || use_p) {
+        constexpr float scale = (float)kBuckets / kEnd;
+        each([&](int64_t, Gr& q) {
+#pragma unroll
+            for (int e = 0; e < Gr::N; ++e) {
+                const float d = -scale_logit(q.f[e], top, it);
+                if (d < kEnd) atomicAdd(&hist[min((int)(d * scale), kBuckets - 1)], 1u);
+            }
+        });
+        __syncthreads();
+        if (C > 1) cluster_sync();
+        if (rank == 0) {
+            constexpr int kEach = kBuckets / kThreads;
+            uint32_t n[kEach], below = 0;
+            double lo[kEach], hi[kEach], slo = 0.0, shi = 0.0;
+            const float width = kEnd / (float)kBuckets;
+            for (int j = 0; j < kEach; ++j) {
+                const int bk = tid * kEach + j;
+                n[j] = hist[bk];
+                for (int c = 1; c < C; ++c) n[j] += ld_remote(remote(&hist[bk], c));
+                below += n[j];
+                // what the bucket's tokens weigh at least and at most (1e-5 covers its rounded edges, 2^-40 the rounding down)
+                lo[j] = (double)n[j] * fmax((double)expf(-(float)(bk + 1) * width - 1e-5f) * 0.99999 - 1.0 / (double)kOne, 0.0);
+                hi[j] = (double)n[j] * (double)expf(-(float)bk * width + 1e-5f) * 1.00001;
+                slo += lo[j];
+                shi += hi[j];
+            }
+            // exclusive prefixes over the threads
+            __shared__ uint32_t pre_n[kWarps];
+            __shared__ double pre_lo[kWarps], pre_hi[kWarps];
+            uint32_t cn = below;
+            double cl = slo, ch = shi;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t vn = __shfl_up_sync(kFull, cn, o);
+                const double vl = __shfl_up_sync(kFull, cl, o), vh = __shfl_up_sync(kFull, ch, o);
+                if (lane >= o) {
+                    cn += vn;
+                    cl += vl;
+                    ch += vh;
+                }
+            }
+            if (lane == 31) {
+                pre_n[warp] = cn;
+                pre_lo[warp] = cl;
+                pre_hi[warp] = ch;
+            }
+            if (tid == 0) {
+                sh.win_lo = 0;
+                sh.win_hi = kBuckets;
+                sh.mode = kPlain;
+                sh.k_left = 0xffffffffu;
+            }
+            __syncthreads();
+            uint32_t bn = cn - below, tn = 0;
+            double bl = cl - slo, bh = ch - shi, tl = 0.0, th = 0.0;
+            for (int j = 0; j < kWarps; ++j) {
+                if (j < warp) {
+                    bn += pre_n[j];
+                    bl += pre_lo[j];
+                    bh += pre_hi[j];
+                }
+                tn += pre_n[j];
+                tl += pre_lo[j];
+                th += pre_hi[j];
+            }
+            // a k-th token beyond the last bucket weighs nothing: no cut by count
+            const bool by_k = use_k && (uint64_t)k < tn;
+            const double p_lo = (double)p * tl * 0.999999, p_hi = (double)p * th * 1.000001 + 1e-9;
+            for (int j = 0; j < kEach; ++j) {
+                const uint32_t bk = tid * kEach + j, an = bn + n[j];
+                const double al = bl + lo[j], ah = bh + hi[j];
+                if (by_k) {
+                    if (bn < k && k <= an) {
+                        // with top-p the list has to hold all of the first k
+                        const bool whole = an <= kListMax;
+                        sh.win_lo = whole ? 0 : bk;
+                        sh.win_hi = bk + 1;
+                        sh.k_left = (uint32_t)k - (whole ? 0u : bn);
+                        sh.mode = whole || (n[j] <= kListMax && !use_p) ? kWindow : kDigits;
+                    }
+                } else if (use_p) {
+                    if ((bh < p_lo || bk == 0) && ah >= p_lo) sh.win_lo = bk;
+                    if ((bl < p_hi || bk == 0) && al >= p_hi) sh.win_hi = bk + 1;
+                }
+                bn = an;
+                bl = al;
+                bh = ah;
+            }
+            __syncthreads();
+            if (!by_k && use_p && tid == 0) sh.mode = kWindow;
+            __syncthreads();
+            if (!by_k && use_p) {                          // how many tokens that window holds
+                u64 in = 0;
+                for (int j = 0; j < kEach; ++j) {
+                    const uint32_t bk = tid * kEach + j;
+                    if (bk >= sh.win_lo && bk < sh.win_hi) in += n[j];
+                }
+                in = block_sum_u<u64>(in, sh.red);
+                if (tid == 0 && in > kListMax) sh.mode = kDigits;
+            }
+            __syncthreads();
+            if (tid < C && tid > 0) {
+                st_remote(remote(&sh.win_lo, tid), sh.win_lo);
+                st_remote(remote(&sh.win_hi, tid), sh.win_hi);
+                st_remote(remote(&sh.mode, tid), sh.mode);
+                st_remote(remote(&sh.k_left, tid), sh.k_left);
+            }
+        }
+        if (C > 1) cluster_sync();
+        else __syncthreads();
+    } else {
+        if (tid == 0) {
+            sh.win_lo = sh.win_hi = kBuckets;
+            sh.mode = kPlain;
+            sh.k_left = 0xffffffffu;
+        }
+        __syncthreads();
+    }
+    if (sh.mode == kDigits) {
+        if (rank == 0) sample_by_digits<T>(a, b, top);
+        return;
+    }
+    // everything above the window is summed (all of it, and what min-p keeps); the window's tokens go to the list
+    const uint32_t win_lo = sh.mode == kWindow ? sh.win_lo : kBuckets, win_hi = sh.mode == kWindow ? sh.win_hi : kBuckets;
+    {
+        constexpr float scale = (float)kBuckets / kEnd;
+        const uint32_t list_at = remote(list, 0), count_at = remote(&sh.list_n, 0);
+        // (top-p's share is of every token's weight, or, after top-k, of the weight that top-k leaves)
+        const bool want_rest = use_p && sh.k_left == 0xffffffffu;
+        u64 kept = 0, all = 0, rest = 0;
+        Sum sk, sa, sr;
+        each([&](int64_t v0, Gr& q) {
+#pragma unroll
+            for (int e = 0; e < Gr::N; ++e) {
+                const float s = scale_logit(q.f[e], top, it);
+                const uint32_t bk = -s < kEnd ? (uint32_t)min((int)(-s * scale), kBuckets - 1) : (uint32_t)kBuckets;
+                if (bk < win_lo) {
+                    const float w = rel_weight(s);
+                    sa.add(w);
+                    if (w >= least) sk.add(w);
+                } else if (bk < win_hi) {
+                    const uint32_t at = add_remote(count_at, 1u);
+                    if (at < kListMax) st_remote(list_at + at * 8, ((u64)__float_as_uint(-s) << 32) | (u64)(uint32_t)(v0 + e));
+                } else if (want_rest && bk < kBuckets) {
+                    sr.add(rel_weight(s));
+                }
+            }
+            if (sa.n > 4000u || sr.n > 4000u) {
+                kept += sk.value();
+                all += sa.value();
+                rest += sr.value();
+                sk = sa = sr = Sum();
+            }
+        });
+        kept += sk.value();
+        all += sa.value();
+        rest += sr.value();
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            kept += __shfl_xor_sync(kFull, kept, o);
+            all += __shfl_xor_sync(kFull, all, o);
+            rest += __shfl_xor_sync(kFull, rest, o);
+        }
+        if (lane == 0) {
+            st_remote(remote(&sh.rest[rank * kWarps + warp], 0), rest);
+            st_remote(remote(&sh.kept[rank * kWarps + warp], 0), kept);
+            st_remote(remote(&sh.all[rank * kWarps + warp], 0), all);
+        }
+    }
+    if (C > 1) cluster_sync();
+    else __syncthreads();
+    if (rank == 0) {
+        const int n = min((int)sh.list_n, kListMax), nk = (int)min((uint32_t)n, sh.k_left), segs = C * kWarps;
+        u64 above = 0, rest = 0;
+        for (int j = tid; j < segs; j += kThreads) {
+            above += sh.all[j];
+            rest += sh.rest[j];
+        }
+        above = block_sum_u<u64>(above, sh.red);
+        rest = block_sum_u<u64>(rest, sh.red);
+        if (tid == 0) {
+            sh.cut_d = 0x7f7fffffu;                       // without a list everything is kept
+            sh.cut_v = 0xffffffffu;
+        }
+        if (n > 0) {
+            sort_list(list, n);
+            // a thread takes consecutive entries of the first nk; prefix sums of their weights
+            constexpr int kEach = kListMax / kThreads;
+            const int each_n = (nk + kThreads - 1) / kThreads, e0 = min(tid * each_n, nk), e1 = min(e0 + each_n, nk);
+            u64 w[kEach], mine = 0;
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) {
+                w[j] = e0 + j < e1 ? weight_of(rel_weight(-__uint_as_float((uint32_t)(list[e0 + j] >> 32)))) : 0ull;
+                mine += w[j];
+            }
+            u64 run = warp_inclusive_sum<u64>(mine);
+            __syncthreads();
+            if (lane == 31) sh.red[warp] = run;
+            __syncthreads();
+            u64 in_list = 0;
+            run -= mine;
+            for (int j = 0; j < kWarps; ++j) {
+                if (j < warp) run += sh.red[j];
+                in_list += sh.red[j];
+            }
+            u64 most = ~0ull;
+            if (use_p) {
+                const double lim = ceil((double)p * (double)(above + in_list + rest));
+                most = lim >= 1.0 ? (u64)lim : 1ull;
+            }
+            run += above;
+#pragma unroll
+            for (int j = 0; j < kEach; ++j)
+                if (e0 + j < e1) {
+                    const u64 at = list[e0 + j], next = run + w[j];
+                    if (run < most) {                     // kept: its weight goes to its warp
+                        const uint32_t d = (uint32_t)(at >> 32), v = (uint32_t)at;
+                        if (e0 + j + 1 == nk || next >= most) {
+                            sh.cut_d = d;
+                            sh.cut_v = v;
+                        }
+                        if (rel_weight(-__uint_as_float(d)) >= least) {
+                            const int64_t g = ((int64_t)v + shift) / Gr::N, r = g / per;
+                            atomicAdd(&sh.kept[r * kWarps + (g - r * per) / wper], w[j]);
+                        }
+                    }
+                    run = next;
+                }
+        }
+        __syncthreads();
+        if (warp == 0) {                                  // the target and the warp that holds it: 4 warps' sums a lane
+            u64 part[kMaxCluster * kWarps / 32], mine = 0;
+#pragma unroll
+            for (int j = 0; j < kMaxCluster * kWarps / 32; ++j) {
+                const int q = lane * (kMaxCluster * kWarps / 32) + j;
+                part[j] = q < segs ? sh.kept[q] : 0ull;
+                mine += part[j];
+            }
+            const u64 upto = warp_inclusive_sum<u64>(mine), total = __shfl_sync(kFull, upto, 31);
+            const double want = floor((double)a.u[b] * (double)total);
+            u64 target = want > 0.0 ? (u64)want : 0ull;
+            if (target >= total) target = total - 1;
+            u64 run = upto - mine;
+#pragma unroll
+            for (int j = 0; j < kMaxCluster * kWarps / 32; ++j) {
+                if (run <= target && target < run + part[j]) {
+                    const int q = lane * (kMaxCluster * kWarps / 32) + j, r = q / kWarps;
+                    st_remote(remote(&sh.cut_d, r), sh.cut_d);
+                    st_remote(remote(&sh.cut_v, r), sh.cut_v);
+                    st_remote(remote(&sh.target, r), target - run);
+                    st_remote(remote(&sh.total, r), total);
+                    for (int c = 0; c < C; ++c) st_remote(remote(&sh.seg, c), (uint32_t)q);
+                }
+                run += part[j];
+            }
+        }
+    }
+    if (C > 1) cluster_sync();
+    else __syncthreads();
+    // the warp that holds the target walks its tokens in index order
+    if ((int)sh.seg != rank * kWarps + warp) return;
+    const u64 cut = ((u64)sh.cut_d << 32) | sh.cut_v;
+    u64 before = 0;
+    for (int64_t gb = g0; gb < g1; gb += 32) {
+        const int64_t g = gb + lane;
+        Gr q;
+        u64 w[Gr::N], mine = 0;
+        if (g < g1) {
+            q.unpack(KEEP ? slice[g - s0] : row[g]);
+            q.trim(g, last, shift, V);
+        }
+#pragma unroll
+        for (int e = 0; e < Gr::N; ++e) {
+            w[e] = 0;
+            if (g < g1) {
+                const float s = scale_logit(q.f[e], top, it), r = rel_weight(s);
+                const u64 at = ((u64)__float_as_uint(-s) << 32) | (u64)(uint32_t)(g * Gr::N - shift + e);
+                if (at <= cut && r >= least) w[e] = weight_of(r);
+            }
+            mine += w[e];
+        }
+        const u64 upto = before + warp_inclusive_sum<u64>(mine);
+        u64 run = upto - mine;
+        if (run <= sh.target && sh.target < upto)
+#pragma unroll
+            for (int e = 0; e < Gr::N; ++e) {
+                if (run <= sh.target && sh.target < run + w[e]) {
+                    a.tokens[b] = g * Gr::N - shift + e;
+                    a.logprob[b] = scale_logit(q.f[e], top, it) - (float)log((double)sh.total / (double)kOne);
+                }
+                run += w[e];
+            }
+        before = __shfl_sync(kFull, upto, 31);
+        if (before > sh.target) return;
+    }
+}
+
 }  // namespace
 }  // namespace bcm
 
@@ -236,10 +678,32 @@ extern "C" bcm_status bcm_sample_tokens(const bcm_sample_args* a, cudaStream_t s
                 "sample_tokens: vocab must be in [1, %d], batch below 2^31", BCM_SAMPLE_MAX_VOCAB);
     if (a->batch == 0) return BCM_OK;
     BCM_REQUIRE(a->logits && a->u && a->tokens && a->logprob, "sample_tokens: null pointer");
+    // Blocks of a row: few enough that a slice of at most 64 KB leaves room for two blocks per SM, and more where the
+    // batch would leave SMs empty (down to slices of 4 KB).  A row past 8 slices of 160 KB is read from L2 every pass.
+    const int64_t bytes = a->vocab * (int64_t)dtype_size(a->dtype) + 32;
+    int C = 1;
+    while (C < kMaxCluster && (bytes / C > 65536 || (a->batch * C < sm_count() && bytes / C > 4096))) C *= 2;
+    const int64_t grans = (bytes + 15) / 16, slice = (grans + C - 1) / C * 16;
+    const bool keep = slice <= 160 * 1024;
+    const int smem = kListMax * 8 + (keep ? (int)slice : 0);
+    BCM_REQUIRE(a->batch * C < (1ll << 31), "sample_tokens: batch too large");
     return dispatch_dtype(a->dtype, [&](auto tag) -> bcm_status {
         using T = decltype(tag);
-        sample_kernel<T><<<(unsigned)a->batch, kThreads, 0, stream>>>(*a);
-        BCM_LAUNCH_CHECK();
+        auto kernel = keep ? sample_kernel<T, true> : sample_kernel<T, false>;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(a->batch * C));
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = (size_t)smem;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)C;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = C > 1 ? 1 : 0;
+        BCM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        BCM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, *a, C));
         return BCM_OK;
     });
 }

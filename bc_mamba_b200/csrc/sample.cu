@@ -11,6 +11,9 @@ namespace {
 // mass above every cut, so that one more pass leaves a short list of tokens around
 // the cut: the rest is certainly kept or certainly not.  The first block sorts the
 // list and finds the cut exactly; the warp whose tokens hold the target walks them.
+// Where more than kListMax tokens lie around the cut (equal or close logits, top-k
+// beyond the list together with top-p), the buckets are narrowed instead until one
+// value is left: a few more passes over shared memory.
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
@@ -22,16 +25,10 @@ constexpr float kEnd = 27.75f;                   // e^-27.75 2^40 < 1: further d
 
 typedef unsigned long long u64;
 
-// Order-preserving key of s <= 0 (larger s, larger key); 0 for -inf.
-__device__ __forceinline__ uint32_t key_of(float s) { return 0x7f800000u - __float_as_uint(-s); }
-__device__ __forceinline__ float from_key(uint32_t k) { return -__uint_as_float(0x7f800000u - k); }
-
 __device__ __forceinline__ float scale_logit(float l, float top, float it) {
     const float s = l == top ? 0.0f : (l - top) * it;
     return s <= 0.0f ? -fabsf(s) : -kInf;        // -0 for 0; NaN to -inf
 }
-template <typename T>
-__device__ __forceinline__ float scaled(const T* x, int64_t v, float top, float it) { return scale_logit(to_f32<T>(x[v]), top, it); }
 
 __device__ __forceinline__ float rel_weight(float s) { return expf(s); }
 __device__ __forceinline__ u64 weight_of(float e) { return (u64)(e * kOne); }
@@ -64,160 +61,6 @@ __device__ V block_sum_u(V v, V* red) {
     return v;
 }
 
-// The largest key whose keys-at-or-above hold more than `skip` of what count
-// (or, BY_WEIGHT, weight) adds up over the tokens with key > lo_key, or key ==
-// lo_key (whose tokens count `lo_ties` times).  above: what lies above that key.
-template <typename T, bool BY_WEIGHT>
-__device__ uint32_t select_key(const T* x, int64_t V, float top, float it, u64 skip, uint32_t lo_key, u64* above_out, u64* hist) {
-    uint32_t prefix = 0, mask = 0;
-    u64 above = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        __syncthreads();
-        for (int k = threadIdx.x; k < 256; k += kThreads) hist[k] = 0;
-        __syncthreads();
-        for (int64_t v = threadIdx.x; v < V; v += kThreads) {
-            const float s = scaled<T>(x, v, top, it);
-            const uint32_t key = key_of(s);
-            if (key == 0u || key < lo_key || (key & mask) != prefix) continue;
-            atomicAdd(&hist[(key >> shift) & 255u], BY_WEIGHT ? weight_of(rel_weight(s)) : 1ull);
-        }
-        __syncthreads();
-        int digit = 255;
-        for (; digit > 0; --digit) {
-            if (above + hist[digit] > skip) break;
-            above += hist[digit];
-        }
-        prefix |= (uint32_t)digit << shift;
-        mask |= 255u << shift;
-    }
-    __syncthreads();
-    *above_out = above;
-    return prefix;
-}
-
-// A row by one block that reads it again for every digit: rows whose cut falls into a bucket of more than kListMax
-// tokens (mostly equal logits), and top-k beyond the list together with top-p.  131072 equal bf16 logits: @SLOW@.
-template <typename T>
-__device__ void sample_by_digits(const bcm_sample_args& a, int64_t b, float top) {
-    __shared__ u64 red[kWarps];
-    __shared__ u64 hist[256];
-    __shared__ int64_t s_cut;
-    const int64_t V = a.vocab;
-    const T* x = static_cast<const T*>(a.logits) + b * a.logits_stride;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const float temp = a.temperature ? a.temperature[b] : a.temperature_all;
-    const float inv = 1.0f / temp;
-    const bool warm = temp > 0.0f && inv < kInf;
-    const float it = warm ? inv : 1.0f;
-    int64_t k = warm ? (a.top_k ? a.top_k[b] : a.top_k_all) : 1;
-    if (k <= 0 || k > V) k = V;
-    const float p = a.top_p ? a.top_p[b] : a.top_p_all;
-    const float mp = a.min_p ? a.min_p[b] : a.min_p_all;
-    const float least = mp > 0.0f ? fminf(mp, 1.0f) : 0.0f;
-
-    u64 n_valid = 0;
-    for (int64_t v = threadIdx.x; v < V; v += kThreads) n_valid += key_of(scaled<T>(x, v, top, it)) != 0u;
-    n_valid = block_sum_u<u64>(n_valid, red);
-    // kept so far: key > cut, or key == cut and among the first `ties` of its equals by index
-    uint32_t cut = 1u;
-    u64 ties = (u64)V;
-    if ((u64)k < n_valid) {
-        u64 above;
-        cut = select_key<T, false>(x, V, top, it, (u64)k - 1, 1u, &above, hist);
-        ties = (u64)k - above;
-    }
-    if (p < 1.0f) {
-        u64 sum = 0, at_cut = 0;
-        for (int64_t v = threadIdx.x; v < V; v += kThreads) {
-            const float s = scaled<T>(x, v, top, it);
-            const uint32_t key = key_of(s);
-            if (key > cut) sum += weight_of(rel_weight(s));
-            else if (key == cut) ++at_cut;
-        }
-        sum = block_sum_u<u64>(sum, red);
-        at_cut = block_sum_u<u64>(at_cut, red);
-        const u64 w_cut = weight_of(rel_weight(from_key(cut)));
-        const u64 total = sum + (at_cut < ties ? at_cut : ties) * (cut == 1u ? 0ull : w_cut);
-        const double lim = ceil((double)p * (double)total);
-        const u64 most = lim >= 1.0 ? (u64)lim : 1ull;
-        // the last kept token in descending order is the one holding weight unit most - 1
-        u64 above;
-        const uint32_t pk = select_key<T, true>(x, V, top, it, most - 1, cut, &above, hist);
-        const u64 wp = weight_of(rel_weight(from_key(pk)));
-        const u64 pt = wp ? (most - above + wp - 1) / wp : (u64)V;
-        if (pk > cut) {
-            cut = pk;
-            ties = pt;
-        } else if (pt < ties) {
-            ties = pt;
-        }
-    }
-    // the index of the last kept token among those at the cut
-    const int64_t seg = ((V + kWarps - 1) / kWarps + 31) / 32 * 32;
-    const int64_t lo = warp * seg < V ? warp * seg : V, hi = lo + seg < V ? lo + seg : V;
-    if (threadIdx.x == 0) s_cut = V;
-    u64 mine = 0;
-    for (int64_t v = lo + lane; v < hi; v += 32) mine += key_of(scaled<T>(x, v, top, it)) == cut;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(kFull, mine, o);
-    __syncthreads();
-    if (lane == 0) red[warp] = mine;
-    __syncthreads();
-    u64 before = 0;
-    for (int j = 0; j < warp; ++j) before += red[j];
-    if (before < ties && before + mine >= ties) {
-        for (int64_t v0 = lo; v0 < hi; v0 += 32) {
-            const int64_t v = v0 + lane;
-            const bool at = v < hi && key_of(scaled<T>(x, v, top, it)) == cut;
-            const unsigned m = __ballot_sync(kFull, at);
-            if (at && before + __popc(m & ((2u << lane) - 1u)) == ties) s_cut = v;
-            before += __popc(m);
-        }
-    }
-    __syncthreads();
-    const int64_t last = s_cut;
-    // integer prefix sums in index order: one contiguous segment per warp
-    auto kept = [&](int64_t v, float& s) -> u64 {
-        s = scaled<T>(x, v, top, it);
-        const uint32_t key = key_of(s);
-        if (key < cut || (key == cut && v > last)) return 0ull;
-        const float e = rel_weight(s);
-        return e >= least ? weight_of(e) : 0ull;
-    };
-    u64 sum = 0;
-    for (int64_t v = lo + lane; v < hi; v += 32) {
-        float s;
-        sum += kept(v, s);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-    __syncthreads();
-    if (lane == 0) red[warp] = sum;
-    __syncthreads();
-    u64 total = 0, start = 0;
-    for (int j = 0; j < kWarps; ++j) {
-        if (j == warp) start = total;
-        total += red[j];
-    }
-    const double want = floor((double)a.u[b] * (double)total);
-    u64 target = want > 0.0 ? (u64)want : 0ull;
-    if (target >= total) target = total - 1;
-    if (start <= target && target < start + sum) {
-        for (int64_t v0 = lo; v0 < hi; v0 += 32) {
-            const int64_t v = v0 + lane;
-            float s = 0.0f;
-            const u64 w = v < hi ? kept(v, s) : 0ull;
-            const u64 run = warp_inclusive_sum<u64>(w);
-            if (start + run > target && start + run - w <= target) {
-                a.tokens[b] = v;
-                a.logprob[b] = s - (float)log((double)total / (double)kOne);
-            }
-            start += __shfl_sync(kFull, run, 31);
-            if (start > target) break;
-        }
-    }
-}
-
 // ---- the cluster's shared memory --------------------------------------------------
 __device__ __forceinline__ uint32_t remote(const void* p, int rank) {
     uint32_t a = (uint32_t)__cvta_generic_to_shared(p), r;
@@ -226,11 +69,7 @@ __device__ __forceinline__ uint32_t remote(const void* p, int rank) {
 }
 __device__ __forceinline__ void st_remote(uint32_t a, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
 __device__ __forceinline__ void st_remote(uint32_t a, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory"); }
-__device__ __forceinline__ uint32_t ld_remote(uint32_t a) {
-    uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-    return v;
-}
+__device__ __forceinline__ void red_remote(uint32_t a, uint32_t v) { asm volatile("red.shared::cluster.add.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
 __device__ __forceinline__ uint32_t add_remote(uint32_t a, uint32_t v) {
     uint32_t o;
     asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(o) : "r"(a), "r"(v) : "memory");
@@ -249,11 +88,13 @@ struct Shared {
     u64 kept[kMaxCluster * kWarps], all[kMaxCluster * kWarps], rest[kMaxCluster * kWarps];
     // from rank 0 to all: the window of buckets (first, end), what to do, then the cut and the target
     uint32_t win_lo, win_hi, mode, list_n;
+    uint32_t nar_lo, nar_hi;                     // the narrowed range of -s (as bits), the count or weight above it,
+    u64 nar_base, nar_goal;                      // and which one of them, from 1, is the last kept
     uint32_t k_left;                             // how many of the list's tokens top-k leaves (rank 0)
     uint32_t cut_d, cut_v, seg;                  // the last kept token (-s, index); the warp that holds the target
     u64 target, total;                           // the target within that warp's tokens; the kept weight
 };
-enum { kPlain, kWindow, kDigits };
+enum { kPlain, kWindow, kNarrow };
 
 // Granule g of the row: its elements as floats, those outside the row -inf.
 template <typename T>
@@ -293,6 +134,52 @@ __device__ void sort_list(u64* list, int n) {
             __syncthreads();
         }
 }
+
+// Exclusive prefixes of a thread's counts and bounds over the block, and their totals.
+struct Prefix {
+    uint32_t n, tn;
+    float lo, hi, tl, th;
+};
+__device__ Prefix block_prefix(uint32_t n, float lo, float hi) {
+    __shared__ uint32_t pn[kWarps];
+    __shared__ float pl[kWarps], ph[kWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t cn = n;
+    float cl = lo, ch = hi;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t vn = __shfl_up_sync(kFull, cn, o);
+        const float vl = __shfl_up_sync(kFull, cl, o), vh = __shfl_up_sync(kFull, ch, o);
+        if (lane >= o) {
+            cn += vn;
+            cl += vl;
+            ch += vh;
+        }
+    }
+    __syncthreads();
+    if (lane == 31) {
+        pn[warp] = cn;
+        pl[warp] = cl;
+        ph[warp] = ch;
+    }
+    __syncthreads();
+    Prefix r = {cn - n, 0, cl - lo, ch - hi, 0.0f, 0.0f};
+    for (int j = 0; j < kWarps; ++j) {
+        if (j < warp) {
+            r.n += pn[j];
+            r.lo += pl[j];
+            r.hi += ph[j];
+        }
+        r.tn += pn[j];
+        r.tl += pl[j];
+        r.th += ph[j];
+    }
+    return r;
+}
+// What n tokens with -s in [from, to) weigh at least and at most, over 2^40.  1e-5 covers rounded edges and 2^-40 the
+// rounding down; the sums of up to 4096 fp32 terms, added in blocks, are within 1e-5 too.
+__device__ __forceinline__ float weighs_least(uint32_t n, float to) { return (float)n * fmaxf(expf(-to - 1e-5f) - 1.0f / kOne, 0.0f) * (1.0f - 4e-5f); }
+__device__ __forceinline__ float weighs_most(uint32_t n, float from) { return (float)n * expf(-from + 1e-5f) * (1.0f + 4e-5f); }
 
 // KEEP: the cluster's slices of the row stay in shared memory (otherwise every pass reads the row from L2).
 template <typename T, bool KEEP>
@@ -377,42 +264,26 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
             }
         });
         __syncthreads();
-        if (C > 1) cluster_sync();
+        if (C > 1) {
+            if (rank != 0)
+                for (int j = tid; j < kBuckets; j += kThreads)
+                    if (hist[j]) red_remote(remote(&hist[j], 0), hist[j]);
+            cluster_sync();
+        }
         if (rank == 0) {
             constexpr int kEach = kBuckets / kThreads;
             uint32_t n[kEach], below = 0;
-            double lo[kEach], hi[kEach], slo = 0.0, shi = 0.0;
+            float lo[kEach], hi[kEach], slo = 0.0f, shi = 0.0f;
             const float width = kEnd / (float)kBuckets;
+#pragma unroll
             for (int j = 0; j < kEach; ++j) {
                 const int bk = tid * kEach + j;
                 n[j] = hist[bk];
-                for (int c = 1; c < C; ++c) n[j] += ld_remote(remote(&hist[bk], c));
                 below += n[j];
-                // what the bucket's tokens weigh at least and at most (1e-5 covers its rounded edges, 2^-40 the rounding down)
-                lo[j] = (double)n[j] * fmax((double)expf(-(float)(bk + 1) * width - 1e-5f) * 0.99999 - 1.0 / (double)kOne, 0.0);
-                hi[j] = (double)n[j] * (double)expf(-(float)bk * width + 1e-5f) * 1.00001;
+                lo[j] = weighs_least(n[j], (float)(bk + 1) * width);
+                hi[j] = weighs_most(n[j], (float)bk * width);
                 slo += lo[j];
                 shi += hi[j];
-            }
-            // exclusive prefixes over the threads
-            __shared__ uint32_t pre_n[kWarps];
-            __shared__ double pre_lo[kWarps], pre_hi[kWarps];
-            uint32_t cn = below;
-            double cl = slo, ch = shi;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t vn = __shfl_up_sync(kFull, cn, o);
-                const double vl = __shfl_up_sync(kFull, cl, o), vh = __shfl_up_sync(kFull, ch, o);
-                if (lane >= o) {
-                    cn += vn;
-                    cl += vl;
-                    ch += vh;
-                }
-            }
-            if (lane == 31) {
-                pre_n[warp] = cn;
-                pre_lo[warp] = cl;
-                pre_hi[warp] = ch;
             }
             if (tid == 0) {
                 sh.win_lo = 0;
@@ -420,25 +291,17 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
                 sh.mode = kPlain;
                 sh.k_left = 0xffffffffu;
             }
-            __syncthreads();
-            uint32_t bn = cn - below, tn = 0;
-            double bl = cl - slo, bh = ch - shi, tl = 0.0, th = 0.0;
-            for (int j = 0; j < kWarps; ++j) {
-                if (j < warp) {
-                    bn += pre_n[j];
-                    bl += pre_lo[j];
-                    bh += pre_hi[j];
-                }
-                tn += pre_n[j];
-                tl += pre_lo[j];
-                th += pre_hi[j];
-            }
+            const Prefix pre = block_prefix(below, slo, shi);
+            uint32_t bn = pre.n;
+            const uint32_t tn = pre.tn;
+            float bl = pre.lo, bh = pre.hi;
+            const float tl = pre.tl, th = pre.th;
             // a k-th token beyond the last bucket weighs nothing: no cut by count
             const bool by_k = use_k && (uint64_t)k < tn;
-            const double p_lo = (double)p * tl * 0.999999, p_hi = (double)p * th * 1.000001 + 1e-9;
+            const float p_lo = p * tl * (1.0f - 2e-5f), p_hi = p * th * (1.0f + 2e-5f) + 1e-9f;
             for (int j = 0; j < kEach; ++j) {
                 const uint32_t bk = tid * kEach + j, an = bn + n[j];
-                const double al = bl + lo[j], ah = bh + hi[j];
+                const float al = bl + lo[j], ah = bh + hi[j];
                 if (by_k) {
                     if (bn < k && k <= an) {
                         // with top-p the list has to hold all of the first k
@@ -446,7 +309,7 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
                         sh.win_lo = whole ? 0 : bk;
                         sh.win_hi = bk + 1;
                         sh.k_left = (uint32_t)k - (whole ? 0u : bn);
-                        sh.mode = whole || (n[j] <= kListMax && !use_p) ? kWindow : kDigits;
+                        sh.mode = whole || (n[j] <= kListMax && !use_p) ? kWindow : kNarrow;
                     }
                 } else if (use_p) {
                     if ((bh < p_lo || bk == 0) && ah >= p_lo) sh.win_lo = bk;
@@ -466,7 +329,7 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
                     if (bk >= sh.win_lo && bk < sh.win_hi) in += n[j];
                 }
                 in = block_sum_u<u64>(in, sh.red);
-                if (tid == 0 && in > kListMax) sh.mode = kDigits;
+                if (tid == 0 && in > kListMax) sh.mode = kNarrow;
             }
             __syncthreads();
             if (tid < C && tid > 0) {
@@ -486,17 +349,220 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
         }
         __syncthreads();
     }
-    if (sh.mode == kDigits) {
-        if (rank == 0) sample_by_digits<T>(a, b, top);
-        return;
+    uint32_t win_lo = sh.mode == kWindow ? sh.win_lo : kBuckets, win_hi = sh.mode == kWindow ? sh.win_hi : kBuckets;
+    u64 limit = 0x7f7fffffffffffffull;                    // (-s, index) of the last token that is still in
+    if (sh.mode == kNarrow) {
+        const uint32_t end = __float_as_uint(kEnd);
+        auto sync = [&]() {
+            if (C > 1) cluster_sync();
+            else __syncthreads();
+        };
+        auto token_of = [&](float l, int64_t v) -> u64 { return ((u64)__float_as_uint(-scale_logit(l, top, it)) << 32) | (u64)(uint32_t)v; };
+        // weight of the tokens with -s in [from, to) that are still in, at rank 0 (over every warp, through sh.all)
+        auto weigh = [&](uint32_t from, uint32_t to) -> u64 {
+            Sum some;
+            u64 all = 0;
+            each([&](int64_t v0, Gr& q) {
+#pragma unroll
+                for (int e = 0; e < Gr::N; ++e) {
+                    const u64 at = token_of(q.f[e], v0 + e);
+                    const uint32_t d = (uint32_t)(at >> 32);
+                    if (d >= from && d < to && at <= limit) some.add(rel_weight(-__uint_as_float(d)));
+                }
+                if (some.n > 4000u) {
+                    all += some.value();
+                    some = Sum();
+                }
+            });
+            all += some.value();
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(kFull, all, o);
+            if (lane == 0) st_remote(remote(&sh.all[rank * kWarps + warp], 0), all);
+            sync();
+            u64 sum = 0;
+            if (rank == 0) {
+                for (int j = tid; j < C * kWarps; j += kThreads) sum += sh.all[j];
+                sum = block_sum_u<u64>(sum, sh.red);
+            }
+            sync();
+            return sum;
+        };
+        for (int by_weight = 0; by_weight < 2; ++by_weight) {
+            if (by_weight ? !use_p : sh.k_left == 0xffffffffu) continue;
+            // rank 0 keeps the range [nar_lo, nar_hi) of -s that holds the last kept token, and tells the others
+            const u64 whole = by_weight ? weigh(0, end) : 0;
+            if (rank == 0 && tid == 0) {
+                sh.nar_lo = 0;
+                sh.nar_hi = end;
+                sh.nar_base = 0;
+                const double lim = ceil((double)p * (double)whole);
+                sh.nar_goal = by_weight ? (lim >= 1.0 ? (u64)lim : 1ull) : (u64)k;
+            }
+            for (int round = 0; round < 64; ++round) {    // (each narrows a thousandfold; 64 only bounds the loop)
+                for (int j = tid; j < kBuckets; j += kThreads) hist[j] = 0;
+                if (rank == 0) {
+                    __syncthreads();
+                    if (tid < C && tid > 0) {
+                        st_remote(remote(&sh.nar_lo, tid), sh.nar_lo);
+                        st_remote(remote(&sh.nar_hi, tid), sh.nar_hi);
+                    }
+                }
+                sync();
+                const uint32_t from = sh.nar_lo, span = sh.nar_hi - from;
+                if (span == 1) break;
+                const int cut = max(0, 32 - __clz((span - 1) >> 12));      // buckets of 2^cut values
+                each([&](int64_t v0, Gr& q) {
+#pragma unroll
+                    for (int e = 0; e < Gr::N; ++e) {
+                        const u64 at = token_of(q.f[e], v0 + e);
+                        const uint32_t d = (uint32_t)(at >> 32) - from;
+                        if (d < span && at <= limit) atomicAdd(&hist[d >> cut], 1u);
+                    }
+                });
+                __syncthreads();
+                if (C > 1) {
+                    if (rank != 0)
+                        for (int j = tid; j < kBuckets; j += kThreads)
+                            if (hist[j]) red_remote(remote(&hist[j], 0), hist[j]);
+                    cluster_sync();
+                }
+                uint32_t first = from, next = from;                        // the bucket that may hold the token first
+                if (rank == 0) {
+                    constexpr int kEach = kBuckets / kThreads;
+                    uint32_t n[kEach], below = 0;
+                    float lo[kEach], hi[kEach], slo = 0.0f, shi = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < kEach; ++j) {
+                        const uint32_t bk = tid * kEach + j;
+                        n[j] = hist[bk];
+                        below += n[j];
+                        lo[j] = hi[j] = 0.0f;
+                        if (by_weight && n[j]) {
+                            lo[j] = weighs_least(n[j], __uint_as_float(from + ((bk + 1) << cut)));
+                            hi[j] = weighs_most(n[j], __uint_as_float(from + (bk << cut)));
+                        }
+                        slo += lo[j];
+                        shi += hi[j];
+                    }
+                    const Prefix pre = block_prefix(below, slo, shi);
+                    uint32_t bn = pre.n;
+                    float bl = pre.lo, bh = pre.hi;
+                    // (float differences of 64-bit weights: 2^-24 of the goal, in both directions)
+                    const float left = (float)((double)(sh.nar_goal - sh.nar_base) / (double)kOne);
+                    const u64 count_left = sh.nar_goal - sh.nar_base;
+                    if (tid == 0) {
+                        sh.win_lo = 0xffffffffu;
+                        sh.win_hi = (span - 1) >> cut;
+                    }
+                    __syncthreads();
+#pragma unroll
+                    for (int j = 0; j < kEach; ++j) {
+                        const uint32_t bk = tid * kEach + j;
+                        if (n[j]) {
+                            if (!by_weight && bn < count_left && count_left <= (u64)bn + n[j]) {
+                                sh.win_lo = sh.win_hi = bk;
+                                sh.nar_base += bn;
+                            }
+                            if (by_weight && bh + hi[j] >= left * (1.0f - 2e-5f)) atomicMin(&sh.win_lo, bk);
+                            if (by_weight && bl + lo[j] >= left * (1.0f + 2e-5f)) atomicMin(&sh.win_hi, bk);
+                        }
+                        bn += n[j];
+                        bl += lo[j];
+                        bh += hi[j];
+                    }
+                    __syncthreads();
+                    if (tid == 0) {
+                        first = from + ((sh.win_lo == 0xffffffffu ? 0u : sh.win_lo) << cut);
+                        sh.nar_lo = first;
+                        sh.nar_hi = min(sh.nar_hi, from + ((sh.win_hi + 1) << cut));
+                    }
+                    __syncthreads();
+                    first = sh.nar_lo;
+                }
+                if (by_weight) {
+                    // exactly: the weight above that bucket and in it
+                    if (rank == 0 && tid < C && tid > 0) st_remote(remote(&sh.nar_lo, tid), first);
+                    sync();
+                    first = sh.nar_lo;
+                    next = first + (1u << cut);
+                    const u64 above = weigh(from, first), in = weigh(first, next);
+                    if (rank == 0 && tid == 0) {
+                        sh.nar_base += above;
+                        if (sh.nar_base + in >= sh.nar_goal) {
+                            sh.nar_hi = min(sh.nar_hi, next);
+                        } else {
+                            sh.nar_base += in;
+                            sh.nar_lo = next;
+                            sh.nar_hi = max(sh.nar_hi, next + 1);
+                        }
+                    }
+                }
+            }
+            // one value is left: of the tokens that have it, the first ones by index
+            const uint32_t value = sh.nar_lo;
+            u64 mine = 0;
+            each([&](int64_t v0, Gr& q) {
+#pragma unroll
+                for (int e = 0; e < Gr::N; ++e) {
+                    const u64 at = token_of(q.f[e], v0 + e);
+                    mine += (uint32_t)(at >> 32) == value && at <= limit;
+                }
+            });
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(kFull, mine, o);
+            if (lane == 0) st_remote(remote(&sh.all[rank * kWarps + warp], 0), mine);
+            sync();
+            if (rank == 0 && tid == 0) {
+                const u64 w = by_weight ? max(weight_of(rel_weight(-__uint_as_float(value))), 1ull) : 1ull;
+                u64 left = (sh.nar_goal - sh.nar_base + w - 1) / w;
+                int q = 0;
+                while (q < C * kWarps - 1 && left > sh.all[q]) left -= sh.all[q++];
+                for (int c = 0; c < C; ++c) {
+                    st_remote(remote(&sh.seg, c), (uint32_t)q);
+                    st_remote(remote(&sh.target, c), left);
+                }
+            }
+            sync();
+            if ((int)sh.seg == rank * kWarps + warp) {    // that warp finds it
+                u64 before = 0;
+                for (int64_t gb = g0; gb < g1; gb += 32) {
+                    const int64_t g = gb + lane;
+                    Gr q;
+                    uint32_t here = 0;
+                    if (g < g1) {
+                        q.unpack(KEEP ? slice[g - s0] : row[g]);
+                        q.trim(g, last, shift, V);
+#pragma unroll
+                        for (int e = 0; e < Gr::N; ++e) {
+                            const u64 at = token_of(q.f[e], g * Gr::N - shift + e);
+                            here |= ((uint32_t)(at >> 32) == value && at <= limit ? 1u : 0u) << e;
+                        }
+                    }
+                    const u64 upto = before + warp_inclusive_sum<u64>((u64)__popc(here));
+                    u64 run = upto - __popc(here);
+                    if (run < sh.target && sh.target <= upto)
+#pragma unroll
+                        for (int e = 0; e < Gr::N; ++e)
+                            if ((here >> e & 1u) && ++run == sh.target)
+                                for (int c = 0; c < C; ++c) {
+                                    st_remote(remote(&sh.cut_d, c), value);
+                                    st_remote(remote(&sh.cut_v, c), (uint32_t)(g * Gr::N - shift + e));
+                                }
+                    before = __shfl_sync(kFull, upto, 31);
+                }
+            }
+            sync();
+            limit = ((u64)sh.cut_d << 32) | sh.cut_v;
+            sync();
+        }
+        win_lo = win_hi = kBuckets;                       // what is in is known: no list
     }
     // everything above the window is summed (all of it, and what min-p keeps); the window's tokens go to the list
-    const uint32_t win_lo = sh.mode == kWindow ? sh.win_lo : kBuckets, win_hi = sh.mode == kWindow ? sh.win_hi : kBuckets;
     {
         constexpr float scale = (float)kBuckets / kEnd;
         const uint32_t list_at = remote(list, 0), count_at = remote(&sh.list_n, 0);
         // (top-p's share is of every token's weight, or, after top-k, of the weight that top-k leaves)
-        const bool want_rest = use_p && sh.k_left == 0xffffffffu;
+        const bool want_rest = use_p && sh.k_left == 0xffffffffu && sh.mode == kWindow;
         u64 kept = 0, all = 0, rest = 0;
         Sum sk, sa, sr;
         each([&](int64_t v0, Gr& q) {
@@ -504,13 +570,14 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
             for (int e = 0; e < Gr::N; ++e) {
                 const float s = scale_logit(q.f[e], top, it);
                 const uint32_t bk = -s < kEnd ? (uint32_t)min((int)(-s * scale), kBuckets - 1) : (uint32_t)kBuckets;
-                if (bk < win_lo) {
+                const u64 at = ((u64)__float_as_uint(-s) << 32) | (u64)(uint32_t)(v0 + e);
+                if (bk < win_lo && at <= limit) {
                     const float w = rel_weight(s);
                     sa.add(w);
                     if (w >= least) sk.add(w);
-                } else if (bk < win_hi) {
-                    const uint32_t at = add_remote(count_at, 1u);
-                    if (at < kListMax) st_remote(list_at + at * 8, ((u64)__float_as_uint(-s) << 32) | (u64)(uint32_t)(v0 + e));
+                } else if (bk >= win_lo && bk < win_hi) {
+                    const uint32_t slot = add_remote(count_at, 1u);
+                    if (slot < kListMax) st_remote(list_at + slot * 8, at);
                 } else if (want_rest && bk < kBuckets) {
                     sr.add(rel_weight(s));
                 }
@@ -549,8 +616,8 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
         above = block_sum_u<u64>(above, sh.red);
         rest = block_sum_u<u64>(rest, sh.red);
         if (tid == 0) {
-            sh.cut_d = 0x7f7fffffu;                       // without a list everything is kept
-            sh.cut_v = 0xffffffffu;
+            sh.cut_d = (uint32_t)(limit >> 32);           // without a list everything up to the limit is kept
+            sh.cut_v = (uint32_t)limit;
         }
         if (n > 0) {
             sort_list(list, n);
@@ -678,11 +745,11 @@ extern "C" bcm_status bcm_sample_tokens(const bcm_sample_args* a, cudaStream_t s
                 "sample_tokens: vocab must be in [1, %d], batch below 2^31", BCM_SAMPLE_MAX_VOCAB);
     if (a->batch == 0) return BCM_OK;
     BCM_REQUIRE(a->logits && a->u && a->tokens && a->logprob, "sample_tokens: null pointer");
-    // Blocks of a row: few enough that a slice of at most 64 KB leaves room for two blocks per SM, and more where the
+    // Blocks of a row: few enough that a slice of at most 68 KB leaves room for two blocks per SM, and more where the
     // batch would leave SMs empty (down to slices of 4 KB).  A row past 8 slices of 160 KB is read from L2 every pass.
     const int64_t bytes = a->vocab * (int64_t)dtype_size(a->dtype) + 32;
     int C = 1;
-    while (C < kMaxCluster && (bytes / C > 65536 || (a->batch * C < sm_count() && bytes / C > 4096))) C *= 2;
+    while (C < kMaxCluster && (bytes / C > 69632 || (a->batch * C < sm_count() && bytes / C > 4096))) C *= 2;
     const int64_t grans = (bytes + 15) / 16, slice = (grans + C - 1) / C * 16;
     const bool keep = slice <= 160 * 1024;
     const int smem = kListMax * 8 + (keep ? (int)slice : 0);
@@ -703,6 +770,7 @@ extern "C" bcm_status bcm_sample_tokens(const bcm_sample_args* a, cudaStream_t s
         cfg.attrs = attr;
         cfg.numAttrs = C > 1 ? 1 : 0;
         BCM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        BCM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
         BCM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, *a, C));
         return BCM_OK;
     });

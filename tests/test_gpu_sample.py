@@ -101,6 +101,18 @@ def test_all_equal(V):
     assert tok.tolist() == [0, V // 2 - 1]
 
 
+@pytest.mark.parametrize("V,spread,dtype", [(60000, 0.3, torch.float32), (60000, 1.0, torch.bfloat16), (150000, 0.05, torch.float16),
+                                            (20000, 0.5, torch.float32)])
+def test_cuts_among_many_close_tokens(V, spread, dtype):
+    """More tokens around the cut than the list holds: flat rows, top-p alone, top-k in the thousands with and without top-p."""
+    x = _logits(3, V, dtype, seed=V, spread=spread)
+    xs = x.float().cpu().numpy()
+    for k in (0, V // 3, V - 5):
+        _run(x, 3, top_k=k, temperature=0.9)
+        for p in (0.2, 0.97):
+            _run(x, 3, top_p=[_clear_p(xs[b], 0.9, k, p) for b in range(3)], temperature=0.9, top_k=k, min_p=0.3 if k else 0.0)
+
+
 @pytest.mark.parametrize("m", [0.01, 0.1, 0.5, 1.0, 3.0])
 def test_min_p(m):
     x = _logits(3, 30000, torch.float32, seed=4)

@@ -12,8 +12,9 @@ namespace {
 // the cut: the rest is certainly kept or certainly not.  The first block sorts the
 // list and finds the cut exactly; the warp whose tokens hold the target walks them.
 // Where more than kListMax tokens lie around the cut (equal or close logits, top-k
-// beyond the list together with top-p), the buckets are narrowed instead until one
-// value is left: a few more passes over shared memory.
+// beyond the list together with top-p), the range of s is narrowed, by buckets of
+// its bits and exact sums above them, until the list takes what it holds or one
+// value is left.
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
@@ -94,7 +95,7 @@ struct Shared {
     uint32_t cut_d, cut_v, seg;                  // the last kept token (-s, index); the warp that holds the target
     u64 target, total;                           // the target within that warp's tokens; the kept weight
 };
-enum { kPlain, kWindow, kNarrow };
+enum { kPlain, kWindow, kNarrow, kRange };      // kRange: a window of -s, [nar_lo, nar_hi), in place of buckets
 
 // Granule g of the row: its elements as floats, those outside the row -inf.
 template <typename T>
@@ -245,10 +246,15 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
         return;
     }
     auto each = [&](auto&& f) {                           // f(index of the first element, elements) over the warp's granules
-        for (int64_t g = g0 + lane; g < g1; g += 32) {
+        for (int64_t g = g0 + lane; g - lane < g1; g += 32) {      // (the whole warp; no element past the last: -inf)
             Gr q;
-            q.unpack(KEEP ? slice[g - s0] : row[g]);
-            q.trim(g, last, shift, V);
+            if (g < g1) {
+                q.unpack(KEEP ? slice[g - s0] : row[g]);
+                q.trim(g, last, shift, V);
+            } else {
+#pragma unroll
+                for (int e = 0; e < Gr::N; ++e) q.f[e] = -kInf;
+            }
             f(g * Gr::N - shift, q);
         }
     };
@@ -358,44 +364,68 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
             else __syncthreads();
         };
         auto token_of = [&](float l, int64_t v) -> u64 { return ((u64)__float_as_uint(-scale_logit(l, top, it)) << 32) | (u64)(uint32_t)v; };
-        // weight of the tokens with -s in [from, to) that are still in, at rank 0 (over every warp, through sh.all)
-        auto weigh = [&](uint32_t from, uint32_t to) -> u64 {
-            Sum some;
-            u64 all = 0;
+        // weight of the tokens that are still in with -s in [from, mid) and in [mid, to), at rank 0 (through sh.all, sh.rest)
+        u64 front = 0, back = 0;
+        auto weigh = [&](uint32_t from, uint32_t mid, uint32_t to) {
+            Sum sf, sb;
+            front = back = 0;
             each([&](int64_t v0, Gr& q) {
 #pragma unroll
                 for (int e = 0; e < Gr::N; ++e) {
                     const u64 at = token_of(q.f[e], v0 + e);
                     const uint32_t d = (uint32_t)(at >> 32);
-                    if (d >= from && d < to && at <= limit) some.add(rel_weight(-__uint_as_float(d)));
+                    if (d >= from && d < to && at <= limit) {
+                        const float r = rel_weight(-__uint_as_float(d));
+                        if (d < mid) sf.add(r);
+                        else sb.add(r);
+                    }
                 }
-                if (some.n > 4000u) {
-                    all += some.value();
-                    some = Sum();
+                if (sf.n > 4000u || sb.n > 4000u) {
+                    front += sf.value();
+                    back += sb.value();
+                    sf = sb = Sum();
                 }
             });
-            all += some.value();
+            front += sf.value();
+            back += sb.value();
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(kFull, all, o);
-            if (lane == 0) st_remote(remote(&sh.all[rank * kWarps + warp], 0), all);
-            sync();
-            u64 sum = 0;
-            if (rank == 0) {
-                for (int j = tid; j < C * kWarps; j += kThreads) sum += sh.all[j];
-                sum = block_sum_u<u64>(sum, sh.red);
+            for (int o = 16; o > 0; o >>= 1) {
+                front += __shfl_xor_sync(kFull, front, o);
+                back += __shfl_xor_sync(kFull, back, o);
+            }
+            if (lane == 0) {
+                st_remote(remote(&sh.all[rank * kWarps + warp], 0), front);
+                st_remote(remote(&sh.rest[rank * kWarps + warp], 0), back);
             }
             sync();
-            return sum;
+            if (rank == 0) {
+                front = back = 0;
+                for (int j = tid; j < C * kWarps; j += kThreads) {
+                    front += sh.all[j];
+                    back += sh.rest[j];
+                }
+                front = block_sum_u<u64>(front, sh.red);
+                back = block_sum_u<u64>(back, sh.red);
+            }
+            sync();
         };
         for (int by_weight = 0; by_weight < 2; ++by_weight) {
             if (by_weight ? !use_p : sh.k_left == 0xffffffffu) continue;
             // rank 0 keeps the range [nar_lo, nar_hi) of -s that holds the last kept token, and tells the others
-            const u64 whole = by_weight ? weigh(0, end) : 0;
+            uint32_t lo0 = 0, hi0 = end;
+            if (by_weight) {
+                if (sh.k_left == 0xffffffffu) {           // the window of buckets, widened by their edges' rounding
+                    const float width = kEnd / (float)kBuckets;
+                    lo0 = __float_as_uint((float)sh.win_lo * width * (1.0f - 1e-6f));
+                    hi0 = min(end, __float_as_uint((float)sh.win_hi * width * (1.0f + 1e-6f)) + 1u);
+                }
+                weigh(0, lo0, end);
+            }
             if (rank == 0 && tid == 0) {
-                sh.nar_lo = 0;
-                sh.nar_hi = end;
-                sh.nar_base = 0;
-                const double lim = ceil((double)p * (double)whole);
+                sh.nar_lo = lo0;
+                sh.nar_hi = hi0;
+                sh.nar_base = front;
+                const double lim = ceil((double)p * (double)(front + back));
                 sh.nar_goal = by_weight ? (lim >= 1.0 ? (u64)lim : 1ull) : (u64)k;
             }
             for (int round = 0; round < 64; ++round) {    // (each narrows a thousandfold; 64 only bounds the loop)
@@ -405,11 +435,12 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
                     if (tid < C && tid > 0) {
                         st_remote(remote(&sh.nar_lo, tid), sh.nar_lo);
                         st_remote(remote(&sh.nar_hi, tid), sh.nar_hi);
+                        st_remote(remote(&sh.mode, tid), sh.mode);
                     }
                 }
                 sync();
                 const uint32_t from = sh.nar_lo, span = sh.nar_hi - from;
-                if (span == 1) break;
+                if (span == 1 || sh.mode == kRange) break;
                 const int cut = max(0, 32 - __clz((span - 1) >> 12));      // buckets of 2^cut values
                 each([&](int64_t v0, Gr& q) {
 #pragma unroll
@@ -471,7 +502,16 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
                         bh += hi[j];
                     }
                     __syncthreads();
+                    u64 in = 0;                           // tokens in what is left: enough for the list to take over?
+#pragma unroll
+                    for (int j = 0; j < kEach; ++j)
+                        if (tid * kEach + j >= sh.win_lo && tid * kEach + j <= sh.win_hi) in += n[j];
+                    in = block_sum_u<u64>(in, sh.red);
                     if (tid == 0) {
+                        if (in <= kListMax && sh.win_lo != 0xffffffffu && (by_weight || !use_p)) {
+                            sh.mode = kRange;
+                            sh.k_left = by_weight ? 0xffffffffu : (uint32_t)(sh.nar_goal - sh.nar_base);
+                        }
                         first = from + ((sh.win_lo == 0xffffffffu ? 0u : sh.win_lo) << cut);
                         sh.nar_lo = first;
                         sh.nar_hi = min(sh.nar_hi, from + ((sh.win_hi + 1) << cut));
@@ -480,24 +520,29 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
                     first = sh.nar_lo;
                 }
                 if (by_weight) {
-                    // exactly: the weight above that bucket and in it
-                    if (rank == 0 && tid < C && tid > 0) st_remote(remote(&sh.nar_lo, tid), first);
+                    if (rank == 0 && tid < C && tid > 0) {
+                        st_remote(remote(&sh.nar_lo, tid), first);
+                        st_remote(remote(&sh.mode, tid), sh.mode);
+                    }
                     sync();
+                    if (sh.mode == kRange) continue;
+                    // exactly: the weight above that bucket and in it
                     first = sh.nar_lo;
                     next = first + (1u << cut);
-                    const u64 above = weigh(from, first), in = weigh(first, next);
+                    weigh(from, first, next);
                     if (rank == 0 && tid == 0) {
-                        sh.nar_base += above;
-                        if (sh.nar_base + in >= sh.nar_goal) {
+                        sh.nar_base += front;
+                        if (sh.nar_base + back >= sh.nar_goal) {
                             sh.nar_hi = min(sh.nar_hi, next);
                         } else {
-                            sh.nar_base += in;
+                            sh.nar_base += back;
                             sh.nar_lo = next;
                             sh.nar_hi = max(sh.nar_hi, next + 1);
                         }
                     }
                 }
             }
+            if (sh.mode == kRange) break;
             // one value is left: of the tokens that have it, the first ones by index
             const uint32_t value = sh.nar_lo;
             u64 mine = 0;
@@ -555,32 +600,56 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
             limit = ((u64)sh.cut_d << 32) | sh.cut_v;
             sync();
         }
-        win_lo = win_hi = kBuckets;                       // what is in is known: no list
+        if (sh.mode != kRange) win_lo = win_hi = kBuckets;      // what is in is known: no list
+        else {
+            win_lo = 1;                                   // (the list pass numbers what lies above the range, in it and below)
+            win_hi = 2;
+        }
     }
     // everything above the window is summed (all of it, and what min-p keeps); the window's tokens go to the list
     {
         constexpr float scale = (float)kBuckets / kEnd;
         const uint32_t list_at = remote(list, 0), count_at = remote(&sh.list_n, 0);
         // (top-p's share is of every token's weight, or, after top-k, of the weight that top-k leaves)
-        const bool want_rest = use_p && sh.k_left == 0xffffffffu && sh.mode == kWindow;
+        const bool range = sh.mode == kRange;
+        const uint32_t range_lo = sh.nar_lo, range_hi = sh.nar_hi;
+        // (broadcast: the list was cut by count where k_left says so)
+        const bool want_rest = use_p && (range || (sh.mode == kWindow && sh.k_left == 0xffffffffu));
         u64 kept = 0, all = 0, rest = 0;
         Sum sk, sa, sr;
         each([&](int64_t v0, Gr& q) {
+            uint32_t to_list = 0;
 #pragma unroll
             for (int e = 0; e < Gr::N; ++e) {
                 const float s = scale_logit(q.f[e], top, it);
-                const uint32_t bk = -s < kEnd ? (uint32_t)min((int)(-s * scale), kBuckets - 1) : (uint32_t)kBuckets;
-                const u64 at = ((u64)__float_as_uint(-s) << 32) | (u64)(uint32_t)(v0 + e);
-                if (bk < win_lo && at <= limit) {
+                uint32_t bk = -s < kEnd ? (uint32_t)min((int)(-s * scale), kBuckets - 1) : (uint32_t)kBuckets;
+                const uint32_t d = __float_as_uint(-s);
+                const u64 at = ((u64)d << 32) | (u64)(uint32_t)(v0 + e);
+                if (range) bk = -s < kEnd ? (d >= range_lo) + (d >= range_hi) : (uint32_t)kBuckets;
+                if (at > limit) bk = kBuckets;
+                if (bk < win_lo) {
                     const float w = rel_weight(s);
                     sa.add(w);
                     if (w >= least) sk.add(w);
-                } else if (bk >= win_lo && bk < win_hi) {
-                    const uint32_t slot = add_remote(count_at, 1u);
-                    if (slot < kListMax) st_remote(list_at + slot * 8, at);
+                } else if (bk < win_hi) {
+                    to_list |= 1u << e;
                 } else if (want_rest && bk < kBuckets) {
                     sr.add(rel_weight(s));
                 }
+            }
+            // the warp's tokens of the window go to consecutive places of the list
+            if (__any_sync(kFull, to_list != 0)) {
+                const uint32_t mine = __popc(to_list), upto = warp_inclusive_sum<uint32_t>(mine);
+                uint32_t slot = 0;
+                if (lane == 31) slot = add_remote(count_at, upto);
+                slot = __shfl_sync(kFull, slot, 31) + upto - mine;
+#pragma unroll
+                for (int e = 0; e < Gr::N; ++e)
+                    if (to_list >> e & 1u) {
+                        if (slot < kListMax)
+                            st_remote(list_at + slot * 8, ((u64)__float_as_uint(-scale_logit(q.f[e], top, it)) << 32) | (u64)(uint32_t)(v0 + e));
+                        ++slot;
+                    }
             }
             if (sa.n > 4000u || sr.n > 4000u) {
                 kept += sk.value();

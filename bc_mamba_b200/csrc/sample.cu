@@ -23,32 +23,41 @@ constexpr int kListMax = 4096;                   // tokens around the cut
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kOne = 1099511627776.0f;         // 2^40
 constexpr float kEnd = 27.75f;                   // e^-27.75 2^40 < 1: further down tokens weigh nothing
+constexpr float kTop = 3.402823466e38f;
 
 typedef unsigned long long u64;
 
-__device__ __forceinline__ float scale_logit(float l, float top, float it) {
-    const float s = l == top ? 0.0f : (l - top) * it;
-    return s <= 0.0f ? -fabsf(s) : -kInf;        // -0 for 0; NaN to -inf
+__device__ __forceinline__ int bucket_of(float d) { return min((int)(d * ((float)kBuckets / kEnd)), kBuckets - 1); }
+// The smallest distance, as bits, whose bucket is at least bk.
+__device__ uint32_t bucket_edge(uint32_t bk) {
+    uint32_t lo = 0, hi = __float_as_uint(kEnd);          // the answer lies in [lo, hi]; distances from kEnd on have no bucket
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (bucket_of(__uint_as_float(mid)) >= (int)bk) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
 }
-
 __device__ __forceinline__ float rel_weight(float s) { return expf(s); }
 __device__ __forceinline__ u64 weight_of(float e) { return (u64)(e * kOne); }
 
 // Sums of weights in two 32-bit limbs of 20 bits (adding 2^23 with rounding down leaves the integer in the mantissa);
-// exact for fewer than 4096 terms.
+// exact for fewer than 4096 terms.  The n terms include those that weigh nothing.
 struct Sum {
-    uint32_t hi = 0, lo = 0, n = 0;
+    uint32_t hi = 0, lo = 0;
     __device__ __forceinline__ void add(float e) {
         const float t = __fmaf_rd(e, 1048576.0f, 8388608.0f);                       // 2^23 + floor(e 2^20)
         const float rest = fmaf(e, 1048576.0f, 8388608.0f - t);                     // exact, in [0, 1)
         hi += __float_as_uint(t);
         lo += __float_as_uint(__fmaf_rd(rest, 1048576.0f, 8388608.0f));
-        ++n;
     }
-    __device__ __forceinline__ u64 value() const {
-        return ((u64)(hi - n * 0x4b000000u) << 20) + (u64)(lo - n * 0x4b000000u);
+    __device__ __forceinline__ u64 take(uint32_t n) {
+        const u64 v = ((u64)(hi - n * 0x4b000000u) << 20) + (u64)(lo - n * 0x4b000000u);
+        hi = lo = 0;
+        return v;
     }
 };
+constexpr uint32_t kSumMax = 4000;
 
 template <typename V>
 __device__ V block_sum_u(V v, V* red) {
@@ -95,9 +104,9 @@ struct Shared {
     uint32_t cut_d, cut_v, seg;                  // the last kept token (-s, index); the warp that holds the target
     u64 target, total;                           // the target within that warp's tokens; the kept weight
 };
-enum { kPlain, kWindow, kNarrow, kRange };      // kRange: a window of -s, [nar_lo, nar_hi), in place of buckets
+enum { kSet, kNarrow };                          // whether [nar_lo, nar_hi) is the list's range already
 
-// Granule g of the row: its elements as floats, those outside the row -inf.
+// Granule g of the row: its elements as floats, those outside the row -inf; then their distances -s from the maximum.
 template <typename T>
 struct Granule {
     static constexpr int N = 16 / (int)sizeof(T);
@@ -113,6 +122,15 @@ struct Granule {
 #pragma unroll
             for (int e = 0; e < N; ++e)
                 if (g * N + e < shift || g * N + e - shift >= V) f[e] = -kInf;
+    }
+    // (a NaN, or -inf at 1/T = 0, becomes a NaN: its bits lie above every distance that counts)
+    __device__ __forceinline__ void distances(float top, float it) {
+        if (top > kTop)                                  // +inf: its equals at 0, the rest far away
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[e] = f[e] == top ? 0.0f : kInf;
+        else
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[e] = (top - f[e]) * it;
     }
 };
 
@@ -245,15 +263,16 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
         }
         return;
     }
-    auto each = [&](auto&& f) {                           // f(index of the first element, elements) over the warp's granules
-        for (int64_t g = g0 + lane; g - lane < g1; g += 32) {      // (the whole warp; no element past the last: -inf)
+    auto each = [&](auto&& f) {                           // f(index of the first element, distances) over the warp's granules
+        for (int64_t g = g0 + lane; g - lane < g1; g += 32) {      // (the whole warp)
             Gr q;
             if (g < g1) {
                 q.unpack(KEEP ? slice[g - s0] : row[g]);
                 q.trim(g, last, shift, V);
+                q.distances(top, it);
             } else {
 #pragma unroll
-                for (int e = 0; e < Gr::N; ++e) q.f[e] = -kInf;
+                for (int e = 0; e < Gr::N; ++e) q.f[e] = kInf;
             }
             f(g * Gr::N - shift, q);
         }
@@ -261,12 +280,10 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
 
     // buckets of s, counted; the first block finds the window of buckets that holds the cut
     if (use_k || use_p) {
-        constexpr float scale = (float)kBuckets / kEnd;
         each([&](int64_t, Gr& q) {
 #pragma unroll
             for (int e = 0; e < Gr::N; ++e) {
-                const float d = -scale_logit(q.f[e], top, it);
-                if (d < kEnd) atomicAdd(&hist[min((int)(d * scale), kBuckets - 1)], 1u);
+                if (q.f[e] < kEnd) atomicAdd(&hist[bucket_of(q.f[e])], 1u);
             }
         });
         __syncthreads();
@@ -286,15 +303,15 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
                 const int bk = tid * kEach + j;
                 n[j] = hist[bk];
                 below += n[j];
-                lo[j] = weighs_least(n[j], (float)(bk + 1) * width);
-                hi[j] = weighs_most(n[j], (float)bk * width);
+                lo[j] = use_p ? weighs_least(n[j], (float)(bk + 1) * width) : 0.0f;
+                hi[j] = use_p ? weighs_most(n[j], (float)bk * width) : 0.0f;
                 slo += lo[j];
                 shi += hi[j];
             }
             if (tid == 0) {
                 sh.win_lo = 0;
                 sh.win_hi = kBuckets;
-                sh.mode = kPlain;
+                sh.mode = kSet;
                 sh.k_left = 0xffffffffu;
             }
             const Prefix pre = block_prefix(below, slo, shi);
@@ -315,7 +332,7 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
                         sh.win_lo = whole ? 0 : bk;
                         sh.win_hi = bk + 1;
                         sh.k_left = (uint32_t)k - (whole ? 0u : bn);
-                        sh.mode = whole || (n[j] <= kListMax && !use_p) ? kWindow : kNarrow;
+                        sh.mode = whole || (n[j] <= kListMax && !use_p) ? kSet : kNarrow;
                     }
                 } else if (use_p) {
                     if ((bh < p_lo || bk == 0) && ah >= p_lo) sh.win_lo = bk;
@@ -326,21 +343,21 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
                 bh = ah;
             }
             __syncthreads();
-            if (!by_k && use_p && tid == 0) sh.mode = kWindow;
-            __syncthreads();
             if (!by_k && use_p) {                          // how many tokens that window holds
                 u64 in = 0;
-                for (int j = 0; j < kEach; ++j) {
-                    const uint32_t bk = tid * kEach + j;
-                    if (bk >= sh.win_lo && bk < sh.win_hi) in += n[j];
-                }
+#pragma unroll
+                for (int j = 0; j < kEach; ++j)
+                    if (tid * kEach + j >= sh.win_lo && tid * kEach + j < sh.win_hi) in += n[j];
                 in = block_sum_u<u64>(in, sh.red);
                 if (tid == 0 && in > kListMax) sh.mode = kNarrow;
             }
             __syncthreads();
+            if (warp == 0 && lane < 2) {                   // the window's edges
+                const bool any = by_k || use_p;
+                const uint32_t edge = !any ? __float_as_uint(kEnd) : bucket_edge(lane ? sh.win_hi : sh.win_lo);
+                for (int c = 0; c < C; ++c) st_remote(remote(lane ? &sh.nar_hi : &sh.nar_lo, c), edge);
+            }
             if (tid < C && tid > 0) {
-                st_remote(remote(&sh.win_lo, tid), sh.win_lo);
-                st_remote(remote(&sh.win_hi, tid), sh.win_hi);
                 st_remote(remote(&sh.mode, tid), sh.mode);
                 st_remote(remote(&sh.k_left, tid), sh.k_left);
             }
@@ -349,45 +366,44 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
         else __syncthreads();
     } else {
         if (tid == 0) {
-            sh.win_lo = sh.win_hi = kBuckets;
-            sh.mode = kPlain;
+            sh.nar_lo = sh.nar_hi = __float_as_uint(kEnd);
+            sh.mode = kSet;
             sh.k_left = 0xffffffffu;
         }
         __syncthreads();
     }
-    uint32_t win_lo = sh.mode == kWindow ? sh.win_lo : kBuckets, win_hi = sh.mode == kWindow ? sh.win_hi : kBuckets;
     u64 limit = 0x7f7fffffffffffffull;                    // (-s, index) of the last token that is still in
+    auto token_of = [&](float d, int64_t v) -> u64 { return ((u64)__float_as_uint(d) << 32) | (u64)(uint32_t)v; };
     if (sh.mode == kNarrow) {
         const uint32_t end = __float_as_uint(kEnd);
         auto sync = [&]() {
             if (C > 1) cluster_sync();
             else __syncthreads();
         };
-        auto token_of = [&](float l, int64_t v) -> u64 { return ((u64)__float_as_uint(-scale_logit(l, top, it)) << 32) | (u64)(uint32_t)v; };
         // weight of the tokens that are still in with -s in [from, mid) and in [mid, to), at rank 0 (through sh.all, sh.rest)
         u64 front = 0, back = 0;
         auto weigh = [&](uint32_t from, uint32_t mid, uint32_t to) {
             Sum sf, sb;
+            uint32_t terms = 0;
             front = back = 0;
             each([&](int64_t v0, Gr& q) {
 #pragma unroll
                 for (int e = 0; e < Gr::N; ++e) {
                     const u64 at = token_of(q.f[e], v0 + e);
                     const uint32_t d = (uint32_t)(at >> 32);
-                    if (d >= from && d < to && at <= limit) {
-                        const float r = rel_weight(-__uint_as_float(d));
-                        if (d < mid) sf.add(r);
-                        else sb.add(r);
-                    }
+                    const float r = d >= from && d < to && at <= limit ? rel_weight(-q.f[e]) : 0.0f;
+                    sf.add(d < mid ? r : 0.0f);
+                    sb.add(d < mid ? 0.0f : r);
                 }
-                if (sf.n > 4000u || sb.n > 4000u) {
-                    front += sf.value();
-                    back += sb.value();
-                    sf = sb = Sum();
+                terms += Gr::N;
+                if (terms > kSumMax) {
+                    front += sf.take(terms);
+                    back += sb.take(terms);
+                    terms = 0;
                 }
             });
-            front += sf.value();
-            back += sb.value();
+            front += sf.take(terms);
+            back += sb.take(terms);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) {
                 front += __shfl_xor_sync(kFull, front, o);
@@ -414,10 +430,9 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
             // rank 0 keeps the range [nar_lo, nar_hi) of -s that holds the last kept token, and tells the others
             uint32_t lo0 = 0, hi0 = end;
             if (by_weight) {
-                if (sh.k_left == 0xffffffffu) {           // the window of buckets, widened by their edges' rounding
-                    const float width = kEnd / (float)kBuckets;
-                    lo0 = __float_as_uint((float)sh.win_lo * width * (1.0f - 1e-6f));
-                    hi0 = min(end, __float_as_uint((float)sh.win_hi * width * (1.0f + 1e-6f)) + 1u);
+                if (sh.k_left == 0xffffffffu) {           // (without top-k the window of buckets holds it)
+                    lo0 = sh.nar_lo;
+                    hi0 = sh.nar_hi;
                 }
                 weigh(0, lo0, end);
             }
@@ -436,11 +451,12 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
                         st_remote(remote(&sh.nar_lo, tid), sh.nar_lo);
                         st_remote(remote(&sh.nar_hi, tid), sh.nar_hi);
                         st_remote(remote(&sh.mode, tid), sh.mode);
+                        st_remote(remote(&sh.k_left, tid), sh.k_left);
                     }
                 }
                 sync();
                 const uint32_t from = sh.nar_lo, span = sh.nar_hi - from;
-                if (span == 1 || sh.mode == kRange) break;
+                if (span == 1 || sh.mode == kSet) break;
                 const int cut = max(0, 32 - __clz((span - 1) >> 12));      // buckets of 2^cut values
                 each([&](int64_t v0, Gr& q) {
 #pragma unroll
@@ -509,7 +525,7 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
                     in = block_sum_u<u64>(in, sh.red);
                     if (tid == 0) {
                         if (in <= kListMax && sh.win_lo != 0xffffffffu && (by_weight || !use_p)) {
-                            sh.mode = kRange;
+                            sh.mode = kSet;
                             sh.k_left = by_weight ? 0xffffffffu : (uint32_t)(sh.nar_goal - sh.nar_base);
                         }
                         first = from + ((sh.win_lo == 0xffffffffu ? 0u : sh.win_lo) << cut);
@@ -525,7 +541,7 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
                         st_remote(remote(&sh.mode, tid), sh.mode);
                     }
                     sync();
-                    if (sh.mode == kRange) continue;
+                    if (sh.mode == kSet) continue;
                     // exactly: the weight above that bucket and in it
                     first = sh.nar_lo;
                     next = first + (1u << cut);
@@ -542,7 +558,7 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
                     }
                 }
             }
-            if (sh.mode == kRange) break;
+            if (sh.mode == kSet) break;
             // one value is left: of the tokens that have it, the first ones by index
             const uint32_t value = sh.nar_lo;
             u64 mine = 0;
@@ -577,6 +593,7 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
                     if (g < g1) {
                         q.unpack(KEEP ? slice[g - s0] : row[g]);
                         q.trim(g, last, shift, V);
+                        q.distances(top, it);
 #pragma unroll
                         for (int e = 0; e < Gr::N; ++e) {
                             const u64 at = token_of(q.f[e], g * Gr::N - shift + e);
@@ -600,67 +617,63 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
             limit = ((u64)sh.cut_d << 32) | sh.cut_v;
             sync();
         }
-        if (sh.mode != kRange) win_lo = win_hi = kBuckets;      // what is in is known: no list
-        else {
-            win_lo = 1;                                   // (the list pass numbers what lies above the range, in it and below)
-            win_hi = 2;
-        }
     }
-    // everything above the window is summed (all of it, and what min-p keeps); the window's tokens go to the list
+    // (a cut that is known needs no list: everything up to the limit)
+    const uint32_t list_lo = sh.mode == kSet ? sh.nar_lo : __float_as_uint(kEnd), list_hi = sh.mode == kSet ? sh.nar_hi : __float_as_uint(kEnd);
+    // what lies above the list's range is summed (all of it, and what min-p keeps), what lies in it goes to the list
     {
-        constexpr float scale = (float)kBuckets / kEnd;
-        const uint32_t list_at = remote(list, 0), count_at = remote(&sh.list_n, 0);
-        // (top-p's share is of every token's weight, or, after top-k, of the weight that top-k leaves)
-        const bool range = sh.mode == kRange;
-        const uint32_t range_lo = sh.nar_lo, range_hi = sh.nar_hi;
-        // (broadcast: the list was cut by count where k_left says so)
-        const bool want_rest = use_p && (range || (sh.mode == kWindow && sh.k_left == 0xffffffffu));
+        const uint32_t list_at = remote(list, 0), count_at = remote(&sh.list_n, 0), end = __float_as_uint(kEnd);
+        // top-p's share is of every token's weight, or, after top-k, of the weight that top-k leaves
+        const bool some_above = list_lo > 0, want_all = use_p && least > 0.0f, limited = limit != 0x7f7fffffffffffffull;
+        const bool want_rest = use_p && list_hi > list_lo && sh.k_left == 0xffffffffu, listed = list_hi > list_lo;
         u64 kept = 0, all = 0, rest = 0;
         Sum sk, sa, sr;
+        uint32_t terms = 0;
         each([&](int64_t v0, Gr& q) {
             uint32_t to_list = 0;
+            if (some_above || want_rest) {
 #pragma unroll
-            for (int e = 0; e < Gr::N; ++e) {
-                const float s = scale_logit(q.f[e], top, it);
-                uint32_t bk = -s < kEnd ? (uint32_t)min((int)(-s * scale), kBuckets - 1) : (uint32_t)kBuckets;
-                const uint32_t d = __float_as_uint(-s);
-                const u64 at = ((u64)d << 32) | (u64)(uint32_t)(v0 + e);
-                if (range) bk = -s < kEnd ? (d >= range_lo) + (d >= range_hi) : (uint32_t)kBuckets;
-                if (at > limit) bk = kBuckets;
-                if (bk < win_lo) {
-                    const float w = rel_weight(s);
-                    sa.add(w);
-                    if (w >= least) sk.add(w);
-                } else if (bk < win_hi) {
-                    to_list |= 1u << e;
-                } else if (want_rest && bk < kBuckets) {
-                    sr.add(rel_weight(s));
+                for (int e = 0; e < Gr::N; ++e) {
+                    const uint32_t d = __float_as_uint(q.f[e]);
+                    float w = d < end ? rel_weight(-q.f[e]) : 0.0f;
+                    if (limited && token_of(q.f[e], v0 + e) > limit) w = 0.0f;
+                    sk.add(d < list_lo && w >= least ? w : 0.0f);
+                    if (want_all) sa.add(d < list_lo ? w : 0.0f);
+                    if (want_rest) sr.add(d >= list_hi ? w : 0.0f);
+                }
+                terms += Gr::N;
+                if (terms > kSumMax) {
+                    kept += sk.take(terms);
+                    if (want_all) all += sa.take(terms);
+                    if (want_rest) rest += sr.take(terms);
+                    terms = 0;
                 }
             }
-            // the warp's tokens of the window go to consecutive places of the list
-            if (__any_sync(kFull, to_list != 0)) {
-                const uint32_t mine = __popc(to_list), upto = warp_inclusive_sum<uint32_t>(mine);
-                uint32_t slot = 0;
-                if (lane == 31) slot = add_remote(count_at, upto);
-                slot = __shfl_sync(kFull, slot, 31) + upto - mine;
+            if (listed) {
 #pragma unroll
-                for (int e = 0; e < Gr::N; ++e)
-                    if (to_list >> e & 1u) {
-                        if (slot < kListMax)
-                            st_remote(list_at + slot * 8, ((u64)__float_as_uint(-scale_logit(q.f[e], top, it)) << 32) | (u64)(uint32_t)(v0 + e));
-                        ++slot;
-                    }
-            }
-            if (sa.n > 4000u || sr.n > 4000u) {
-                kept += sk.value();
-                all += sa.value();
-                rest += sr.value();
-                sk = sa = sr = Sum();
+                for (int e = 0; e < Gr::N; ++e) {
+                    const uint32_t d = __float_as_uint(q.f[e]);
+                    if (d >= list_lo && d < list_hi && (!limited || token_of(q.f[e], v0 + e) <= limit)) to_list |= 1u << e;
+                }
+                // the warp's tokens go to consecutive places
+                if (__any_sync(kFull, to_list != 0)) {
+                    const uint32_t mine = __popc(to_list), upto = warp_inclusive_sum<uint32_t>(mine);
+                    uint32_t slot = 0;
+                    if (lane == 31) slot = add_remote(count_at, upto);
+                    slot = __shfl_sync(kFull, slot, 31) + upto - mine;
+#pragma unroll
+                    for (int e = 0; e < Gr::N; ++e)
+                        if (to_list >> e & 1u) {
+                            if (slot < kListMax) st_remote(list_at + slot * 8, token_of(q.f[e], v0 + e));
+                            ++slot;
+                        }
+                }
             }
         });
-        kept += sk.value();
-        all += sa.value();
-        rest += sr.value();
+        kept += sk.take(terms);
+        if (want_all) all += sa.take(terms);
+        else all = kept;                                  // (without min-p the same; not asked for without top-p)
+        if (want_rest) rest += sr.take(terms);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             kept += __shfl_xor_sync(kFull, kept, o);
@@ -774,14 +787,14 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
         if (g < g1) {
             q.unpack(KEEP ? slice[g - s0] : row[g]);
             q.trim(g, last, shift, V);
+            q.distances(top, it);
         }
 #pragma unroll
         for (int e = 0; e < Gr::N; ++e) {
             w[e] = 0;
             if (g < g1) {
-                const float s = scale_logit(q.f[e], top, it), r = rel_weight(s);
-                const u64 at = ((u64)__float_as_uint(-s) << 32) | (u64)(uint32_t)(g * Gr::N - shift + e);
-                if (at <= cut && r >= least) w[e] = weight_of(r);
+                const float r = rel_weight(-q.f[e]);
+                if (token_of(q.f[e], g * Gr::N - shift + e) <= cut && r >= least) w[e] = weight_of(r);
             }
             mine += w[e];
         }
@@ -792,7 +805,7 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
             for (int e = 0; e < Gr::N; ++e) {
                 if (run <= sh.target && sh.target < run + w[e]) {
                     a.tokens[b] = g * Gr::N - shift + e;
-                    a.logprob[b] = scale_logit(q.f[e], top, it) - (float)log((double)sh.total / (double)kOne);
+                    a.logprob[b] = -q.f[e] - (float)log((double)sh.total / (double)kOne);
                 }
                 run += w[e];
             }

@@ -8,15 +8,27 @@
 // A row without teacher entries, or with w = 0, has loss 0 and gradient 0
 // whatever its logits hold.
 #include <algorithm>
+#include <cstring>
 
 #include "common.cuh"
 
 namespace bcm {
 namespace {
 
+// C blocks of a cluster share a row, in 16-byte granules (rows may start anywhere).
+// The forward is one pass with a running maximum and sum; the backward one pass that
+// writes.  Loss and gradient in one call keep the row in the cluster's shared memory
+// in between (KEEP), so that memory is read once.  The teacher's entries are one
+// warp's work meanwhile; the K places of the gradient that they touch are written
+// again at the end.
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kMaxCluster = 8;
+constexpr int kBatch = 4;                        // granules a thread has in flight
 constexpr float kInf = __builtin_huge_valf();
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2_(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
 
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
@@ -29,129 +41,270 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// Block reductions: every thread gets the result; red holds kWarps floats.
-__device__ float block_max(float v, float* red) {
-    v = warp_max(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = red[0];
-    for (int k = 1; k < kWarps; ++k) v = fmaxf(v, red[k]);
-    return v;
-}
-__device__ float block_sum(float v, float* red) {
-    v = warp_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = red[0];
-    for (int k = 1; k < kWarps; ++k) v += red[k];
-    return v;
-}
-
 __device__ __forceinline__ int64_t load_id(const void* ids, int wide, int64_t k) {
     return wide ? static_cast<const int64_t*>(ids)[k] : (int64_t) static_cast<const int32_t*>(ids)[k];
 }
 
-// The row's teacher distribution: s_id[k] (-1: absent) and s_p[k]; returns the
-// logarithm of the normaliser plus the maximum, -inf for an empty row.
+// The row's teacher distribution, by one warp: s_id[k] (-1: absent) and s_p[k]; returns the logarithm of the normaliser
+// plus the maximum, -inf for an empty row.
 template <typename TQ>
-__device__ float teacher_row(const TQ* q, const void* ids, int wide, int64_t off, int K, int64_t V, float itau, int* s_id,
-                             float* s_p, float* red) {
+__device__ float teacher_row(const TQ* q, const void* ids, int wide, int64_t off, int K, int64_t V, float itau, int* s_id, float* s_p) {
+    const int lane = threadIdx.x & 31;
     float top = -kInf;
-    for (int k = threadIdx.x; k < K; k += kThreads) {
+    bool nan = false;
+    for (int k = lane; k < K; k += 32) {
         const int64_t id = load_id(ids, wide, off + k);
         const float v = to_f32<TQ>(q[k]) * itau;
         const bool there = id >= 0 && id < V && v != -kInf;
         s_id[k] = there ? (int)id : -1;
         s_p[k] = v;
-        if (there) top = v > top || isnan(v) ? v : top;
+        if (there) {
+            top = fmaxf(top, v);
+            nan |= isnan(v);
+        }
     }
-    float any = block_sum(isnan(top) ? 1.0f : 0.0f, red);
-    top = block_max(top, red);
-    if (any > 0.0f) top = __int_as_float(0x7fffffff);
+    top = warp_max(top);
+    if (__any_sync(kFull, nan)) top = __int_as_float(0x7fffffff);
     if (top == -kInf) return -kInf;
     float sum = 0.0f;
-    for (int k = threadIdx.x; k < K; k += kThreads)
+    for (int k = lane; k < K; k += 32)
         if (s_id[k] >= 0) sum += expf(s_p[k] - top);
-    sum = block_sum(sum, red);
-    const float lg = logf(sum);
-    for (int k = threadIdx.x; k < K; k += kThreads) s_p[k] = s_id[k] >= 0 ? expf(s_p[k] - top) / sum : 0.0f;
-    __syncthreads();
-    return top + lg;
+    sum = warp_sum(sum);
+    for (int k = lane; k < K; k += 32) s_p[k] = s_id[k] >= 0 ? expf(s_p[k] - top) / sum : 0.0f;
+    return top + logf(sum);
 }
 
-// stats[2t] = max of z/tau, stats[2t+1] = sum of exp(z/tau - max).
 template <typename T>
-__device__ float2 row_stats(const T* z, int64_t V, float itau, float* red) {
-    float m = -kInf, s = 0.0f;
-    for (int64_t v = threadIdx.x; v < V; v += kThreads) {
-        const float x = to_f32<T>(z[v]) * itau;
-        if (x > m) {
-            s = s * expf(m - x) + 1.0f;
-            m = x;
-        } else if (x != -kInf) {
-            s += expf(x - m);
+struct Granule {
+    static constexpr int N = 16 / (int)sizeof(T);
+    float f[N];
+    __device__ __forceinline__ void unpack(uint4 w) {
+        T t[N];
+        memcpy(t, &w, 16);
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = to_f32<T>(t[e]);
+    }
+    // exp2((f - m) c): the difference first, so that large logits lose nothing; packed, two elements an instruction
+    __device__ __forceinline__ void exponentials(float m, float c) {
+        const float2 nm = m == -kInf ? make_float2(0.0f, 0.0f) : make_float2(-m, -m), cc = make_float2(c, c);
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+            const float2 v = __fmul2_rn(__fadd2_rn(make_float2(f[e], f[e + 1]), nm), cc);
+            f[e] = ex2_(v.x);
+            f[e + 1] = ex2_(v.y);
         }
     }
-    const float top = block_max(m, red);
-    s = block_sum(m == top ? s : (m == -kInf && !isnan(s) ? 0.0f : s * expf(m - top)), red);
-    return make_float2(top, s);
+    __device__ __forceinline__ uint4 pack() const {
+        T t[N];
+        uint4 w;
+#pragma unroll
+        for (int e = 0; e < N; ++e) t[e] = from_f32<T>(f[e]);
+        memcpy(&w, t, 16);
+        return w;
+    }
+};
+
+// A row of V elements at x as 16-byte granules: the first holds `shift` foreign elements in front.
+template <typename T>
+struct RowOf {
+    static constexpr int N = 16 / (int)sizeof(T);
+    const uint4* at;
+    int shift;
+    int64_t grans;
+    __device__ __forceinline__ RowOf(const T* x, int64_t V)
+        : at(reinterpret_cast<const uint4*>((uintptr_t)x & ~(uintptr_t)15)), shift((int)((uintptr_t)x & 15) / (int)sizeof(T)),
+          grans((shift + V + N - 1) / N) {}
+};
+
+// Sum of exp2(c (f - m)) with its maximum m; c > 0 is log2(e) / tau.
+struct Soft {
+    float m, s;
+    __device__ __forceinline__ void join(float m2, float s2, float c) {
+        const float top = fmaxf(m, m2);
+        if (top == -kInf) {
+            s += s2;                             // (0, or NaN)
+            return;
+        }
+        s = (m == top ? s : (m == -kInf && s == 0.0f ? 0.0f : s * ex2_((m - top) * c))) +
+            (m2 == top ? s2 : (m2 == -kInf && s2 == 0.0f ? 0.0f : s2 * ex2_((m2 - top) * c)));
+        m = top;
+    }
+};
+
+__device__ __forceinline__ uint32_t remote(const void* p, int rank) {
+    uint32_t a = (uint32_t)__cvta_generic_to_shared(p), r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <typename T, typename TQ, bool FWD, bool GRAD>
-__global__ void __launch_bounds__(kThreads)
-distill_kernel(const T* __restrict__ z, int64_t z_stride, const TQ* __restrict__ q, const void* __restrict__ ids, int wide,
-               int64_t V, int K, const float* __restrict__ weight, float itau, float tau, float* __restrict__ loss,
-               float2* __restrict__ stats, const float* __restrict__ dloss, T* __restrict__ dz) {
-    extern __shared__ float smem[];
-    __shared__ float red[kWarps];
-    int* s_id = reinterpret_cast<int*>(smem);
-    float* s_p = smem + K;
-    const int64_t t = blockIdx.x;
-    const T* zr = z + t * z_stride;
-    T* dr = GRAD ? dz + t * V : nullptr;
-    const float w = weight ? weight[t] : 1.0f;
-    const float lse_q = w != 0.0f ? teacher_row<TQ>(q + t * K, ids, wide, t * K, K, V, itau, s_id, s_p, red) : -kInf;
-    if (lse_q == -kInf) {
-        if (FWD && threadIdx.x == 0) {
-            loss[t] = 0.0f;
-            stats[t] = make_float2(0.0f, 1.0f);
-        }
-        if (GRAD)
-            for (int64_t v = threadIdx.x; v < V; v += kThreads) dr[v] = from_f32<T>(0.0f);
-        return;
+template <typename T, typename TQ, bool FWD, bool GRAD, bool KEEP>
+__global__ void __launch_bounds__(kThreads, GRAD && FWD ? 3 : 4)
+distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
+    using Gr = Granule<T>;
+    constexpr int N = Gr::N;
+    extern __shared__ __align__(16) char dyn[];
+    __shared__ float wm[kWarps], ws[kWarps];
+    __shared__ float2 parts[kMaxCluster];
+    __shared__ float s_lse_q;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = (int)a.k;
+    int* s_id = reinterpret_cast<int*>(dyn);
+    float* s_p = reinterpret_cast<float*>(dyn) + K;
+    uint4* slice = reinterpret_cast<uint4*>(dyn + (K * 8 + 15) / 16 * 16);
+    const int rank = blockIdx.x % C;
+    const int64_t t = blockIdx.x / C, V = a.vocab;
+    const T* z = static_cast<const T*>(a.logits) + t * a.logits_stride;
+    const TQ* q = static_cast<const TQ*>(a.teacher_logits) + t * K;
+    const float w = a.weight ? a.weight[t] : 1.0f;
+    const float tau = a.temperature, itau = 1.0f / tau, c = kLog2e * itau;
+    const RowOf<T> row(z, V);
+    const int64_t per = (row.grans + C - 1) / C, g0 = rank * per, g1 = min(g0 + per, row.grans);
+    auto trim = [&](int64_t g, Gr& x) {          // elements outside the row
+        if (g == 0 || g == row.grans - 1)
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (g * N + e < row.shift || g * N + e - row.shift >= V) x.f[e] = -kInf;
+    };
+    bool live = w != 0.0f;
+    Soft soft = {-kInf, 0.0f};
+    if (!FWD) {
+        const float2 st = reinterpret_cast<const float2*>(a.stats)[t];
+        soft = {st.x, st.y};
+        live = st.y >= 0.0f || isnan(st.y);      // (the forward marks rows without a target)
     }
-    const float2 st = FWD ? row_stats<T>(zr, V, itau, red) : stats[t];
-    if (FWD) {
-        const float lse = st.x + logf(st.y);
-        float sum = 0.0f;
-        for (int k = threadIdx.x; k < K; k += kThreads)
-            if (s_p[k] > 0.0f || isnan(s_p[k]))
-                sum += s_p[k] * (to_f32<TQ>(q[t * K + k]) * itau - lse_q - to_f32<T>(zr[s_id[k]]) * itau + lse);
-        sum = block_sum(sum, red);
-        if (threadIdx.x == 0) {
-            loss[t] = w * tau * tau * sum;
-            stats[t] = st;
+    if (live) {
+        if (warp == 0) {
+            const float l = teacher_row<TQ>(q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p);
+            if (lane == 0) s_lse_q = l;
         }
-    }
-    if (GRAD) {
-        const float scale = (dloss ? dloss[t] : 1.0f) * w * tau, inv = 1.0f / st.y;
-        for (int64_t v = threadIdx.x; v < V; v += kThreads)
-            dr[v] = from_f32<T>(expf(to_f32<T>(zr[v]) * itau - st.x) * inv * scale);
-        __syncthreads();
-        for (int k = threadIdx.x; k < K; k += kThreads) {
-            const int id = s_id[k];
-            if (id < 0) continue;
-            bool first = true;
-            float p = s_p[k];
-            for (int j = 0; j < K; ++j)
-                if (j != k && s_id[j] == id) {
-                    if (j < k) { first = false; break; }
-                    p += s_p[j];
+        if (FWD) {
+            for (int64_t gb = g0 + tid; gb < g1; gb += kBatch * kThreads) {
+                uint4 in[kBatch];
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j)
+                    if (gb + j * kThreads < g1) in[j] = row.at[gb + j * kThreads];
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) {
+                    const int64_t g = gb + j * kThreads;
+                    if (g >= g1) break;
+                    if (KEEP) slice[g - g0] = in[j];
+                    Gr x;
+                    x.unpack(in[j]);
+                    trim(g, x);
+                    float top = x.f[0];
+#pragma unroll
+                    for (int e = 1; e < N; ++e) top = fmaxf(top, x.f[e]);
+                    if (top > soft.m) {
+                        if (soft.m != -kInf) soft.s *= ex2_((soft.m - top) * c);
+                        soft.m = top;
+                    }
+                    x.exponentials(soft.m, c);
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) sum += x.f[e];
+                    soft.s += sum;
                 }
-            if (first) dr[id] = from_f32<T>((expf(to_f32<T>(zr[id]) * itau - st.x) * inv - p) * scale);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+                soft.join(__shfl_xor_sync(kFull, soft.m, o), __shfl_xor_sync(kFull, soft.s, o), c);
+            if (lane == 0) {
+                wm[warp] = soft.m;
+                ws[warp] = soft.s;
+            }
+            __syncthreads();
+            soft = {wm[0], ws[0]};
+            for (int k = 1; k < kWarps; ++k) soft.join(wm[k], ws[k], c);
+            if (C > 1) {
+                cluster_sync();                  // every block runs before its shared memory is written to
+                if (tid < C) {
+                    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(remote(&parts[rank], tid)), "f"(soft.m), "f"(soft.s) : "memory");
+                }
+                cluster_sync();
+                soft = {parts[0].x, parts[0].y};
+                for (int k = 1; k < C; ++k) soft.join(parts[k].x, parts[k].y, c);
+            }
+            live = s_lse_q != -kInf;
+            if (rank == 0 && warp == 0) {
+                const float lse = soft.m * itau + logf(soft.s), lse_q = s_lse_q;
+                float sum = 0.0f;
+                if (live)
+                    for (int k = lane; k < K; k += 32)
+                        if (s_p[k] > 0.0f || isnan(s_p[k])) sum += s_p[k] * (to_f32<TQ>(q[k]) * itau - lse_q - to_f32<T>(z[s_id[k]]) * itau + lse);
+                sum = warp_sum(sum);
+                if (lane == 0) {
+                    a.loss[t] = live ? w * tau * tau * sum : 0.0f;
+                    reinterpret_cast<float2*>(a.stats)[t] = live ? make_float2(soft.m, soft.s) : make_float2(0.0f, -1.0f);
+                }
+            }
         }
+    } else if (FWD && rank == 0 && tid == 0) {
+        a.loss[t] = 0.0f;
+        reinterpret_cast<float2*>(a.stats)[t] = make_float2(0.0f, -1.0f);
+    }
+    if (!GRAD) return;
+    // the gradient by granules of its own row, which may lie differently from the logits'
+    T* d = static_cast<T*>(a.dlogits) + t * V;
+    const RowOf<T> out(d, V);
+    const bool alike = out.shift == row.shift;
+    const int64_t oper = alike ? per : (out.grans + C - 1) / C, o0 = rank * oper, o1 = min(o0 + oper, out.grans);
+    const float scale = live ? (a.dloss ? a.dloss[t] : 1.0f) * w * tau : 0.0f, k_out = scale / soft.s;
+    for (int64_t gb = o0 + tid; gb < o1; gb += kBatch * kThreads) {
+        uint4 in[kBatch];
+        if (alike && live)
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j)
+                if (gb + j * kThreads < o1) in[j] = KEEP ? slice[gb + j * kThreads - o0] : row.at[gb + j * kThreads];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const int64_t g = gb + j * kThreads;
+            if (g >= o1) break;
+            const int64_t v0 = g * N - out.shift;
+            Gr x;
+            if (!live) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) x.f[e] = 0.0f;
+            } else {
+                if (alike) {
+                    x.unpack(in[j]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) x.f[e] = v0 + e >= 0 && v0 + e < V ? to_f32<T>(z[v0 + e]) : 0.0f;
+                }
+                x.exponentials(soft.m, c);
+#pragma unroll
+                for (int e = 0; e < N; ++e) x.f[e] *= k_out;
+            }
+            if (v0 >= 0 && v0 + N <= V) {
+                __stcs(const_cast<uint4*>(out.at) + g, x.pack());
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (v0 + e >= 0 && v0 + e < V) d[v0 + e] = from_f32<T>(x.f[e]);
+            }
+        }
+    }
+    if (!live) return;
+    // the teacher's tokens among this block's: the first entry of a token takes its later ones' shares too
+    __syncthreads();
+    for (int k = tid; k < K; k += kThreads) {
+        const int id = s_id[k];
+        const int64_t g = ((int64_t)id + out.shift) / N;
+        if (id < 0 || g < o0 || g >= o1) continue;
+        bool first = true;
+        float p = s_p[k];
+        for (int j = 0; j < K; ++j)
+            if (j != k && s_id[j] == id) {
+                if (j < k) {
+                    first = false;
+                    break;
+                }
+                p += s_p[j];
+            }
+        if (first) d[id] = from_f32<T>((ex2_((to_f32<T>(z[id]) - soft.m) * c) / soft.s - p) * scale);
     }
 }
 
@@ -166,18 +319,44 @@ bcm_status distill_validate(const bcm_distill_args* a, const char* what) {
     return BCM_OK;
 }
 
+template <typename F>
+bcm_status distill_launch_as(F* kernel, const bcm_distill_args* a, int C, int smem, cudaStream_t stream) {
+    BCM_REQUIRE(a->rows * C < (1ll << 31), "distill: too many rows");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a->rows * C));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)C;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = C > 1 ? 1 : 0;
+    BCM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    BCM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, *a, C));
+    return BCM_OK;
+}
+
 template <bool FWD, bool GRAD>
 bcm_status distill_launch(const bcm_distill_args* a, cudaStream_t stream) {
+    // Blocks of a row: with both directions, slices that let three blocks share an SM's shared memory; otherwise one, and
+    // more where the rows leave SMs without a block (down to slices of 8 KB).
+    const int64_t bytes = a->vocab * (int64_t)dtype_size(a->dtype) + 32;
+    const int lists = (int)(a->k * 8 + 15) / 16 * 16, room = 72 * 1024 - lists;
+    int C = 1;
+    while (C < kMaxCluster && ((FWD && GRAD && bytes / C > room) || (a->rows * C < 2 * (int64_t)sm_count() && bytes / C > 8192))) C *= 2;
+    const int64_t slice = ((bytes + 15) / 16 + C - 1) / C * 16;
+    const bool keep = FWD && GRAD && slice <= room;
+    const int smem = lists + (keep ? (int)slice : 0);
     return dispatch_dtype(a->dtype, [&](auto tag) -> bcm_status {
         using T = decltype(tag);
         return dispatch_dtype(a->teacher_dtype, [&](auto qtag) -> bcm_status {
             using TQ = decltype(qtag);
-            distill_kernel<T, TQ, FWD, GRAD><<<(unsigned)a->rows, kThreads, (size_t)a->k * 8, stream>>>(
-                static_cast<const T*>(a->logits), a->logits_stride, static_cast<const TQ*>(a->teacher_logits), a->teacher_ids,
-                a->ids_are_int64, a->vocab, (int)a->k, a->weight, 1.0f / a->temperature, a->temperature, a->loss,
-                reinterpret_cast<float2*>(a->stats), a->dloss, static_cast<T*>(a->dlogits));
-            BCM_LAUNCH_CHECK();
-            return BCM_OK;
+            if constexpr (FWD && GRAD)
+                if (keep) return distill_launch_as(distill_kernel<T, TQ, FWD, GRAD, true>, a, C, smem, stream);
+            return distill_launch_as(distill_kernel<T, TQ, FWD, GRAD, false>, a, C, smem, stream);
         });
     });
 }

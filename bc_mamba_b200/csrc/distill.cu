@@ -17,14 +17,15 @@ namespace {
 
 // C blocks of a cluster share a row, in 16-byte granules (rows may start anywhere).
 // The forward is one pass with a running maximum and sum; the backward one pass that
-// writes.  Loss and gradient in one call keep the row in the cluster's shared memory
-// in between (KEEP), so that memory is read once.  The teacher's entries are one
-// warp's work meanwhile; the K places of the gradient that they touch are written
-// again at the end.
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+// writes; loss and gradient in one call are both by the same block, the second from
+// L2.  (Keeping rows in a cluster's shared memory in between measured slower, 1545
+// against @@ us at 8192 x 131072 bf16: it leaves fewer warps for the exponentials.)
+// Granules arrive by cyclic cp.async buffers of each thread's own.  The teacher's
+// entries are one warp's work meanwhile; the K places of the gradient that they
+// touch are written again at the end.
 constexpr int kMaxCluster = 8;
-constexpr int kBatch = 4;                        // granules a thread has in flight
+constexpr int kBatch = 4, kStages = 3;           // granules a thread takes at a time; batches in flight or in use
+constexpr int kShortRow = 24 * 1024;             // bytes of a row up to which a block has 64 threads, not 256
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -141,9 +142,45 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <typename T, typename TQ, bool FWD, bool GRAD, bool KEEP>
-__global__ void __launch_bounds__(kThreads, GRAD && FWD ? 3 : 4)
+// Granules g, g + kThreads, ... of a thread, in order.
+template <int kThreads>
+struct Feed {
+    uint4* ring;
+    const uint4* at;
+    int64_t end;
+    __device__ __forceinline__ Feed(uint4* room, const uint4* from, int64_t begin, int64_t end_) : ring(room + threadIdx.x), at(from), end(end_) {
+#pragma unroll
+        for (int k = 0; k < kStages - 1; ++k) issue(begin + threadIdx.x + (int64_t)k * kBatch * kThreads, k);
+    }
+    __device__ __forceinline__ void issue(int64_t g, int stage) {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+            if (g + j * kThreads < end)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(ring + (stage * kBatch + j) * kThreads)),
+                             "l"(at + g + j * kThreads)
+                             : "memory");
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    // f(granule, its 16 bytes) for every granule of the thread from g on
+    template <typename F>
+    __device__ __forceinline__ void run(int64_t g, F&& f) {
+        int stage = 0;
+        for (; g < end; g += kBatch * kThreads) {
+            issue(g + (int64_t)(kStages - 1) * kBatch * kThreads, stage == 0 ? kStages - 1 : stage - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j)
+                if (g + j * kThreads < end) f(g + j * kThreads, ring[(stage * kBatch + j) * kThreads]);
+            stage = stage == kStages - 1 ? 0 : stage + 1;
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+};
+
+template <typename T, typename TQ, bool FWD, bool GRAD, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
 distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
+    constexpr int kWarps = kThreads / 32;
     using Gr = Granule<T>;
     constexpr int N = Gr::N;
     extern __shared__ __align__(16) char dyn[];
@@ -153,7 +190,7 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = (int)a.k;
     int* s_id = reinterpret_cast<int*>(dyn);
     float* s_p = reinterpret_cast<float*>(dyn) + K;
-    uint4* slice = reinterpret_cast<uint4*>(dyn + (K * 8 + 15) / 16 * 16);
+    uint4* ring = reinterpret_cast<uint4*>(dyn + (K * 8 + 15) / 16 * 16);
     const int rank = blockIdx.x % C;
     const int64_t t = blockIdx.x / C, V = a.vocab;
     const T* z = static_cast<const T*>(a.logits) + t * a.logits_stride;
@@ -176,38 +213,30 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
         live = st.y >= 0.0f || isnan(st.y);      // (the forward marks rows without a target)
     }
     if (live) {
-        if (warp == 0) {
-            const float l = teacher_row<TQ>(q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p);
-            if (lane == 0) s_lse_q = l;
-        }
         if (FWD) {
-            for (int64_t gb = g0 + tid; gb < g1; gb += kBatch * kThreads) {
-                uint4 in[kBatch];
-#pragma unroll
-                for (int j = 0; j < kBatch; ++j)
-                    if (gb + j * kThreads < g1) in[j] = row.at[gb + j * kThreads];
-#pragma unroll
-                for (int j = 0; j < kBatch; ++j) {
-                    const int64_t g = gb + j * kThreads;
-                    if (g >= g1) break;
-                    if (KEEP) slice[g - g0] = in[j];
-                    Gr x;
-                    x.unpack(in[j]);
-                    trim(g, x);
-                    float top = x.f[0];
-#pragma unroll
-                    for (int e = 1; e < N; ++e) top = fmaxf(top, x.f[e]);
-                    if (top > soft.m) {
-                        if (soft.m != -kInf) soft.s *= ex2_((soft.m - top) * c);
-                        soft.m = top;
-                    }
-                    x.exponentials(soft.m, c);
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < N; ++e) sum += x.f[e];
-                    soft.s += sum;
-                }
+            Feed<kThreads> feed(ring, row.at, g0, g1);
+            if (warp == 0) {
+                const float l = teacher_row<TQ>(q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p);
+                if (lane == 0) s_lse_q = l;
             }
+            feed.run(g0 + tid, [&](int64_t g, uint4 in) {
+                Gr x;
+                x.unpack(in);
+                trim(g, x);
+                float top = x.f[0];
+#pragma unroll
+                for (int e = 1; e < N; ++e) top = fmaxf(top, x.f[e]);
+                if (top > soft.m) {
+                    if (soft.m != -kInf) soft.s *= ex2_((soft.m - top) * c);
+                    soft.m = top;
+                }
+                x.exponentials(soft.m, c);
+#pragma unroll
+                for (int step = 1; step < N; step <<= 1)
+#pragma unroll
+                    for (int e = 0; e < N; e += 2 * step) x.f[e] += x.f[e + step];
+                soft.s += x.f[0];
+            });
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1)
                 soft.join(__shfl_xor_sync(kFull, soft.m, o), __shfl_xor_sync(kFull, soft.s, o), c);
@@ -252,39 +281,44 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
     const bool alike = out.shift == row.shift;
     const int64_t oper = alike ? per : (out.grans + C - 1) / C, o0 = rank * oper, o1 = min(o0 + oper, out.grans);
     const float scale = live ? (a.dloss ? a.dloss[t] : 1.0f) * w * tau : 0.0f, k_out = scale / soft.s;
-    for (int64_t gb = o0 + tid; gb < o1; gb += kBatch * kThreads) {
-        uint4 in[kBatch];
-        if (alike && live)
+    auto put = [&](int64_t g, const Gr& x) {
+        const int64_t v0 = g * N - out.shift;
+        if (v0 >= 0 && v0 + N <= V) {
+            __stcs(const_cast<uint4*>(out.at) + g, x.pack());
+        } else {
 #pragma unroll
-            for (int j = 0; j < kBatch; ++j)
-                if (gb + j * kThreads < o1) in[j] = KEEP ? slice[gb + j * kThreads - o0] : row.at[gb + j * kThreads];
+            for (int e = 0; e < N; ++e)
+                if (v0 + e >= 0 && v0 + e < V) d[v0 + e] = from_f32<T>(x.f[e]);
+        }
+    };
+    auto gradient = [&](Gr& x) {
+        x.exponentials(soft.m, c);
+        const float2 k2 = make_float2(k_out, k_out);
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-            const int64_t g = gb + j * kThreads;
-            if (g >= o1) break;
+        for (int e = 0; e < N; e += 2) {
+            const float2 v = __fmul2_rn(make_float2(x.f[e], x.f[e + 1]), k2);
+            x.f[e] = v.x;
+            x.f[e + 1] = v.y;
+        }
+    };
+    if (live && alike) {
+        Feed<kThreads> feed(ring, row.at, o0, o1);
+        if (!FWD && warp == 0) teacher_row<TQ>(q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p);
+        feed.run(o0 + tid, [&](int64_t g, uint4 in) {
+            Gr x;
+            x.unpack(in);
+            gradient(x);
+            put(g, x);
+        });
+    } else {
+        if (!FWD && live && warp == 0) teacher_row<TQ>(q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p);
+        for (int64_t g = o0 + tid; g < o1; g += kThreads) {
             const int64_t v0 = g * N - out.shift;
             Gr x;
-            if (!live) {
 #pragma unroll
-                for (int e = 0; e < N; ++e) x.f[e] = 0.0f;
-            } else {
-                if (alike) {
-                    x.unpack(in[j]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < N; ++e) x.f[e] = v0 + e >= 0 && v0 + e < V ? to_f32<T>(z[v0 + e]) : 0.0f;
-                }
-                x.exponentials(soft.m, c);
-#pragma unroll
-                for (int e = 0; e < N; ++e) x.f[e] *= k_out;
-            }
-            if (v0 >= 0 && v0 + N <= V) {
-                __stcs(const_cast<uint4*>(out.at) + g, x.pack());
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (v0 + e >= 0 && v0 + e < V) d[v0 + e] = from_f32<T>(x.f[e]);
-            }
+            for (int e = 0; e < N; ++e) x.f[e] = live && v0 + e >= 0 && v0 + e < V ? to_f32<T>(z[v0 + e]) : 0.0f;
+            if (live) gradient(x);
+            put(g, x);
         }
     }
     if (!live) return;
@@ -320,11 +354,16 @@ bcm_status distill_validate(const bcm_distill_args* a, const char* what) {
 }
 
 template <typename F>
-bcm_status distill_launch_as(F* kernel, const bcm_distill_args* a, int C, int smem, cudaStream_t stream) {
+bcm_status distill_launch_as(F* kernel, const bcm_distill_args* a, int threads, cudaStream_t stream) {
+    // one block a row, and more where the rows leave SMs without a block (down to slices of 8 KB)
+    const int64_t bytes = a->vocab * (int64_t)dtype_size(a->dtype);
+    int C = 1;
+    while (C < kMaxCluster && a->rows * C < 2 * (int64_t)sm_count() && bytes / C > 8192) C *= 2;
     BCM_REQUIRE(a->rows * C < (1ll << 31), "distill: too many rows");
+    const int smem = (int)(a->k * 8 + 15) / 16 * 16 + kStages * kBatch * threads * 16;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a->rows * C));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -341,22 +380,13 @@ bcm_status distill_launch_as(F* kernel, const bcm_distill_args* a, int C, int sm
 
 template <bool FWD, bool GRAD>
 bcm_status distill_launch(const bcm_distill_args* a, cudaStream_t stream) {
-    // Blocks of a row: with both directions, slices that let three blocks share an SM's shared memory; otherwise one, and
-    // more where the rows leave SMs without a block (down to slices of 8 KB).
-    const int64_t bytes = a->vocab * (int64_t)dtype_size(a->dtype) + 32;
-    const int lists = (int)(a->k * 8 + 15) / 16 * 16, room = 72 * 1024 - lists;
-    int C = 1;
-    while (C < kMaxCluster && ((FWD && GRAD && bytes / C > room) || (a->rows * C < 2 * (int64_t)sm_count() && bytes / C > 8192))) C *= 2;
-    const int64_t slice = ((bytes + 15) / 16 + C - 1) / C * 16;
-    const bool keep = FWD && GRAD && slice <= room;
-    const int smem = lists + (keep ? (int)slice : 0);
+    const bool small = a->vocab * (int64_t)dtype_size(a->dtype) <= kShortRow;
     return dispatch_dtype(a->dtype, [&](auto tag) -> bcm_status {
         using T = decltype(tag);
         return dispatch_dtype(a->teacher_dtype, [&](auto qtag) -> bcm_status {
             using TQ = decltype(qtag);
-            if constexpr (FWD && GRAD)
-                if (keep) return distill_launch_as(distill_kernel<T, TQ, FWD, GRAD, true>, a, C, smem, stream);
-            return distill_launch_as(distill_kernel<T, TQ, FWD, GRAD, false>, a, C, smem, stream);
+            return small ? distill_launch_as(distill_kernel<T, TQ, FWD, GRAD, 64>, a, 64, stream)
+                         : distill_launch_as(distill_kernel<T, TQ, FWD, GRAD, 256>, a, 256, stream);
         });
     });
 }

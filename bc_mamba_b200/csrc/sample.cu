@@ -6,11 +6,14 @@
 namespace bcm {
 namespace {
 
-// A cluster of C blocks keeps a row in shared memory, in 16-byte granules (rows may
-// start anywhere).  One pass counts the tokens in buckets of s; the buckets bound the
-// mass above every cut, so that one more pass leaves a short list of tokens around
-// the cut: the rest is certainly kept or certainly not.  The first block sorts the
-// list and finds the cut exactly; the warp whose tokens hold the target walks them.
+// A block, or a cluster of C blocks, has a row, in 16-byte granules (rows may start
+// anywhere); each pass reads it again, from L2 (keeping it in a cluster's shared
+// memory left fewer rows in flight and measured slower: 264 against 191 us at 512 x
+// 131072 bf16, top-k 50).  One pass finds the maximum, one counts the tokens in
+// buckets of s; the buckets bound the mass above every cut, so that one more pass
+// leaves a short list of tokens around the cut: the rest is certainly kept or
+// certainly not.  The first block sorts the list and finds the cut exactly; the block
+// whose tokens hold the target walks them.
 // Where more than kListMax tokens lie around the cut (equal or close logits, top-k
 // beyond the list together with top-p), the range of s is narrowed, by buckets of
 // its bits and exact sums above them, until the list takes what it holds or one
@@ -45,11 +48,13 @@ __device__ __forceinline__ u64 weight_of(float e) { return (u64)(e * kOne); }
 // exact for fewer than 4096 terms.  The n terms include those that weigh nothing.
 struct Sum {
     uint32_t hi = 0, lo = 0;
-    __device__ __forceinline__ void add(float e) {
-        const float t = __fmaf_rd(e, 1048576.0f, 8388608.0f);                       // 2^23 + floor(e 2^20)
-        const float rest = fmaf(e, 1048576.0f, 8388608.0f - t);                     // exact, in [0, 1)
-        hi += __float_as_uint(t);
-        lo += __float_as_uint(__fmaf_rd(rest, 1048576.0f, 8388608.0f));
+    __device__ __forceinline__ void add(float2 e) {
+        const float2 big = make_float2(8388608.0f, 8388608.0f), scale = make_float2(1048576.0f, 1048576.0f);
+        const float2 t = __ffma2_rd(e, scale, big);                                 // 2^23 + floor(e 2^20)
+        const float2 rest = __ffma2_rn(e, scale, __fadd2_rn(big, make_float2(-t.x, -t.y)));   // exact, in [0, 1)
+        const float2 r = __ffma2_rd(rest, scale, big);
+        hi += __float_as_uint(t.x) + __float_as_uint(t.y);
+        lo += __float_as_uint(r.x) + __float_as_uint(r.y);
     }
     __device__ __forceinline__ u64 take(uint32_t n) {
         const u64 v = ((u64)(hi - n * 0x4b000000u) << 20) + (u64)(lo - n * 0x4b000000u);
@@ -200,8 +205,7 @@ __device__ Prefix block_prefix(uint32_t n, float lo, float hi) {
 __device__ __forceinline__ float weighs_least(uint32_t n, float to) { return (float)n * fmaxf(expf(-to - 1e-5f) - 1.0f / kOne, 0.0f) * (1.0f - 4e-5f); }
 __device__ __forceinline__ float weighs_most(uint32_t n, float from) { return (float)n * expf(-from + 1e-5f) * (1.0f + 4e-5f); }
 
-// KEEP: the cluster's slices of the row stay in shared memory (otherwise every pass reads the row from L2).
-template <typename T, bool KEEP>
+template <typename T>
 __global__ void __launch_bounds__(kThreads, 2)
 sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
     using Gr = Granule<T>;
@@ -209,7 +213,6 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
     __shared__ Shared sh;
     u64* list = reinterpret_cast<u64*>(dyn);                         // rank 0: after the buckets are done
     uint32_t* hist = reinterpret_cast<uint32_t*>(dyn);
-    uint4* slice = reinterpret_cast<uint4*>(dyn + kListMax * 8);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = blockIdx.x % C;
     const int64_t b = blockIdx.x / C, V = a.vocab;
@@ -219,7 +222,7 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
     const int64_t grans = (shift + V + Gr::N - 1) / Gr::N, last = grans - 1;
     const int64_t per = (grans + C - 1) / C, wper = (per + kWarps - 1) / kWarps;
     // the warp's granules: a contiguous range, so that warps follow one another in index order
-    const int64_t g0 = rank * per + warp * wper, g1 = min(min(g0 + wper, (rank + 1) * per), grans), s0 = rank * per;
+    const int64_t g0 = rank * per + warp * wper, g1 = min(min(g0 + wper, (rank + 1) * per), grans);
     const float temp = a.temperature ? a.temperature[b] : a.temperature_all;
     const float inv = 1.0f / temp;
     const bool warm = temp > 0.0f && inv < kInf;
@@ -236,7 +239,6 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
 #pragma unroll 4
     for (int64_t g = g0 + lane; g < g1; g += 32) {
         const uint4 w = row[g];
-        if (KEEP) slice[g - s0] = w;
         Gr q;
         q.unpack(w);
         q.trim(g, last, shift, V);
@@ -267,7 +269,7 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
         for (int64_t g = g0 + lane; g - lane < g1; g += 32) {      // (the whole warp)
             Gr q;
             if (g < g1) {
-                q.unpack(KEEP ? slice[g - s0] : row[g]);
+                q.unpack(row[g]);
                 q.trim(g, last, shift, V);
                 q.distances(top, it);
             } else {
@@ -388,12 +390,18 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
             front = back = 0;
             each([&](int64_t v0, Gr& q) {
 #pragma unroll
-                for (int e = 0; e < Gr::N; ++e) {
-                    const u64 at = token_of(q.f[e], v0 + e);
-                    const uint32_t d = (uint32_t)(at >> 32);
-                    const float r = d >= from && d < to && at <= limit ? rel_weight(-q.f[e]) : 0.0f;
-                    sf.add(d < mid ? r : 0.0f);
-                    sb.add(d < mid ? 0.0f : r);
+                for (int e0 = 0; e0 < Gr::N; e0 += 2) {
+                    float in_front[2], behind[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const u64 at = token_of(q.f[e0 + j], v0 + e0 + j);
+                        const uint32_t d = (uint32_t)(at >> 32);
+                        const float r = d >= from && d < to && at <= limit ? rel_weight(-q.f[e0 + j]) : 0.0f;
+                        in_front[j] = d < mid ? r : 0.0f;
+                        behind[j] = d < mid ? 0.0f : r;
+                    }
+                    sf.add(make_float2(in_front[0], in_front[1]));
+                    sb.add(make_float2(behind[0], behind[1]));
                 }
                 terms += Gr::N;
                 if (terms > kSumMax) {
@@ -591,7 +599,7 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
                     Gr q;
                     uint32_t here = 0;
                     if (g < g1) {
-                        q.unpack(KEEP ? slice[g - s0] : row[g]);
+                        q.unpack(row[g]);
                         q.trim(g, last, shift, V);
                         q.distances(top, it);
 #pragma unroll
@@ -633,13 +641,20 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
             uint32_t to_list = 0;
             if (some_above || want_rest) {
 #pragma unroll
-                for (int e = 0; e < Gr::N; ++e) {
-                    const uint32_t d = __float_as_uint(q.f[e]);
-                    float w = d < end ? rel_weight(-q.f[e]) : 0.0f;
-                    if (limited && token_of(q.f[e], v0 + e) > limit) w = 0.0f;
-                    sk.add(d < list_lo && w >= least ? w : 0.0f);
-                    if (want_all) sa.add(d < list_lo ? w : 0.0f);
-                    if (want_rest) sr.add(d >= list_hi ? w : 0.0f);
+                for (int e0 = 0; e0 < Gr::N; e0 += 2) {
+                    float wk[2], wa[2], wr[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t d = __float_as_uint(q.f[e0 + j]);
+                        float w = d < end ? rel_weight(-q.f[e0 + j]) : 0.0f;
+                        if (limited && token_of(q.f[e0 + j], v0 + e0 + j) > limit) w = 0.0f;
+                        wa[j] = d < list_lo ? w : 0.0f;
+                        wk[j] = wa[j] >= least ? wa[j] : 0.0f;
+                        wr[j] = d >= list_hi ? w : 0.0f;
+                    }
+                    sk.add(make_float2(wk[0], wk[1]));
+                    if (want_all) sa.add(make_float2(wa[0], wa[1]));
+                    if (want_rest) sr.add(make_float2(wr[0], wr[1]));
                 }
                 terms += Gr::N;
                 if (terms > kSumMax) {
@@ -776,28 +791,42 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
     }
     if (C > 1) cluster_sync();
     else __syncthreads();
-    // the warp that holds the target walks its tokens in index order
-    if ((int)sh.seg != rank * kWarps + warp) return;
+    // The block that holds the target walks that warp's tokens in index order: every warp sums a part of them, the one
+    // whose part holds the target finds it.
+    if ((int)sh.seg / kWarps != rank) return;
     const u64 cut = ((u64)sh.cut_d << 32) | sh.cut_v;
-    u64 before = 0;
-    for (int64_t gb = g0; gb < g1; gb += 32) {
-        const int64_t g = gb + lane;
-        Gr q;
-        u64 w[Gr::N], mine = 0;
-        if (g < g1) {
-            q.unpack(KEEP ? slice[g - s0] : row[g]);
+    const int64_t w0 = rank * per + sh.seg % kWarps * wper, w1 = min(min(w0 + wper, (rank + 1) * per), grans), part = (wper + kWarps - 1) / kWarps;
+    const int64_t p0 = min(w0 + warp * part, w1), p1 = min(p0 + part, w1);
+    auto kept_in = [&](int64_t g, Gr& q, u64 (&w)[Gr::N]) -> u64 {
+        u64 mine = 0;
+#pragma unroll
+        for (int e = 0; e < Gr::N; ++e) w[e] = 0;
+        if (g < p1) {
+            q.unpack(row[g]);
             q.trim(g, last, shift, V);
             q.distances(top, it);
-        }
 #pragma unroll
-        for (int e = 0; e < Gr::N; ++e) {
-            w[e] = 0;
-            if (g < g1) {
+            for (int e = 0; e < Gr::N; ++e) {
                 const float r = rel_weight(-q.f[e]);
                 if (token_of(q.f[e], g * Gr::N - shift + e) <= cut && r >= least) w[e] = weight_of(r);
+                mine += w[e];
             }
-            mine += w[e];
         }
+        return mine;
+    };
+    Gr q;
+    u64 w[Gr::N], sum = 0;
+    for (int64_t g = p0 + lane; g < p1; g += 32) sum += kept_in(g, q, w);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+    if (lane == 0) sh.red[warp] = sum;
+    __syncthreads();
+    u64 before = 0;
+    for (int j = 0; j < warp; ++j) before += sh.red[j];
+    if (!(before <= sh.target && sh.target < before + sum)) return;
+    for (int64_t gb = p0; gb < p1; gb += 32) {
+        const int64_t g = gb + lane;
+        const u64 mine = kept_in(g, q, w);
         const u64 upto = before + warp_inclusive_sum<u64>(mine);
         u64 run = upto - mine;
         if (run <= sh.target && sh.target < upto)
@@ -827,22 +856,17 @@ extern "C" bcm_status bcm_sample_tokens(const bcm_sample_args* a, cudaStream_t s
                 "sample_tokens: vocab must be in [1, %d], batch below 2^31", BCM_SAMPLE_MAX_VOCAB);
     if (a->batch == 0) return BCM_OK;
     BCM_REQUIRE(a->logits && a->u && a->tokens && a->logprob, "sample_tokens: null pointer");
-    // Blocks of a row: few enough that a slice of at most 68 KB leaves room for two blocks per SM, and more where the
-    // batch would leave SMs empty (down to slices of 4 KB).  A row past 8 slices of 160 KB is read from L2 every pass.
-    const int64_t bytes = a->vocab * (int64_t)dtype_size(a->dtype) + 32;
+    // Blocks of a row: one where the batch fills the GPU (two blocks per SM), more below (down to slices of 4 KB).
+    const int64_t bytes = a->vocab * (int64_t)dtype_size(a->dtype);
     int C = 1;
-    while (C < kMaxCluster && (bytes / C > 69632 || (a->batch * C < sm_count() && bytes / C > 4096))) C *= 2;
-    const int64_t grans = (bytes + 15) / 16, slice = (grans + C - 1) / C * 16;
-    const bool keep = slice <= 160 * 1024;
-    const int smem = kListMax * 8 + (keep ? (int)slice : 0);
-    BCM_REQUIRE(a->batch * C < (1ll << 31), "sample_tokens: batch too large");
+    while (C < kMaxCluster && a->batch * C <= sm_count() && bytes / C > 4096) C *= 2;
     return dispatch_dtype(a->dtype, [&](auto tag) -> bcm_status {
         using T = decltype(tag);
-        auto kernel = keep ? sample_kernel<T, true> : sample_kernel<T, false>;
+        auto kernel = sample_kernel<T>;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)(a->batch * C));
         cfg.blockDim = dim3(kThreads);
-        cfg.dynamicSmemBytes = (size_t)smem;
+        cfg.dynamicSmemBytes = kListMax * 8;
         cfg.stream = stream;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -851,8 +875,6 @@ extern "C" bcm_status bcm_sample_tokens(const bcm_sample_args* a, cudaStream_t s
         attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = C > 1 ? 1 : 0;
-        BCM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        BCM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
         BCM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, *a, C));
         return BCM_OK;
     });

@@ -102,7 +102,7 @@ struct Shared {
     // per warp of the cluster, at rank 0: the weight above the window, all of it and what min-p keeps, and that below it
     u64 kept[kMaxCluster * kWarps], all[kMaxCluster * kWarps], rest[kMaxCluster * kWarps];
     // from rank 0 to all: the window of buckets (first, end), what to do, then the cut and the target
-    uint32_t win_lo, win_hi, mode, list_n;
+    uint32_t win_lo, win_hi, mode, list_n, list_at;
     uint32_t nar_lo, nar_hi;                     // the narrowed range of -s (as bits), the count or weight above it,
     u64 nar_base, nar_goal;                      // and which one of them, from 1, is the last kept
     uint32_t k_left;                             // how many of the list's tokens top-k leaves (rank 0)
@@ -139,15 +139,17 @@ struct Granule {
     }
 };
 
-// The list in ascending order (bitonic network over the next power of two, rest ~0).
+// The list in ascending order (bitonic network over the next power of two, rest ~0).  A warp takes consecutive pairs:
+// steps within its own elements need no block barrier.
 __device__ void sort_list(u64* list, int n) {
     int m = 1;
     while (m < n) m <<= 1;
     for (int k = n + threadIdx.x; k < m; k += kThreads) list[k] = ~0ull;
     __syncthreads();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, own = max(m / 2 / kWarps, 32);   // pairs of a warp
     for (int size = 2; size <= m; size <<= 1)
         for (int step = size >> 1; step > 0; step >>= 1) {
-            for (int k = threadIdx.x; k < m / 2; k += kThreads) {
+            for (int k = warp * own + lane; k < min((warp + 1) * own, m / 2); k += 32) {
                 const int i = 2 * k - (k & (step - 1)), j = i + step;
                 const u64 x = list[i], y = list[j];
                 if ((x > y) == ((i & size) == 0)) {
@@ -155,8 +157,12 @@ __device__ void sort_list(u64* list, int n) {
                     list[j] = x;
                 }
             }
-            __syncthreads();
+            // what comes next reads other warps' elements when this step or the next one leaves the warp's own
+            const int next = step > 1 ? step >> 1 : size;
+            if (max(step, next) > own) __syncthreads();
+            else __syncwarp();
         }
+    __syncthreads();
 }
 
 // Exclusive prefixes of a thread's counts and bounds over the block, and their totals.
@@ -211,7 +217,7 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
     using Gr = Granule<T>;
     extern __shared__ __align__(16) char dyn[];
     __shared__ Shared sh;
-    u64* list = reinterpret_cast<u64*>(dyn);                         // rank 0: after the buckets are done
+    u64* list = reinterpret_cast<u64*>(dyn);                         // after the buckets are done
     uint32_t* hist = reinterpret_cast<uint32_t*>(dyn);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = blockIdx.x % C;
@@ -630,7 +636,7 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
     const uint32_t list_lo = sh.mode == kSet ? sh.nar_lo : __float_as_uint(kEnd), list_hi = sh.mode == kSet ? sh.nar_hi : __float_as_uint(kEnd);
     // what lies above the list's range is summed (all of it, and what min-p keeps), what lies in it goes to the list
     {
-        const uint32_t list_at = remote(list, 0), count_at = remote(&sh.list_n, 0), end = __float_as_uint(kEnd);
+        const uint32_t end = __float_as_uint(kEnd);
         // top-p's share is of every token's weight, or, after top-k, of the weight that top-k leaves
         const bool some_above = list_lo > 0, want_all = use_p && least > 0.0f, limited = limit != 0x7f7fffffffffffffull;
         const bool want_rest = use_p && list_hi > list_lo && sh.k_left == 0xffffffffu, listed = list_hi > list_lo;
@@ -674,12 +680,12 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
                 if (__any_sync(kFull, to_list != 0)) {
                     const uint32_t mine = __popc(to_list), upto = warp_inclusive_sum<uint32_t>(mine);
                     uint32_t slot = 0;
-                    if (lane == 31) slot = add_remote(count_at, upto);
+                    if (lane == 31) slot = atomicAdd(&sh.list_n, upto);
                     slot = __shfl_sync(kFull, slot, 31) + upto - mine;
 #pragma unroll
                     for (int e = 0; e < Gr::N; ++e)
                         if (to_list >> e & 1u) {
-                            if (slot < kListMax) st_remote(list_at + slot * 8, token_of(q.f[e], v0 + e));
+                            if (slot < kListMax) list[slot] = token_of(q.f[e], v0 + e);
                             ++slot;
                         }
                 }
@@ -701,8 +707,19 @@ sample_kernel(const __grid_constant__ bcm_sample_args a, int C) {
             st_remote(remote(&sh.all[rank * kWarps + warp], 0), all);
         }
     }
-    if (C > 1) cluster_sync();
-    else __syncthreads();
+    if (C > 1) {                                          // the other blocks' lists go behind the first one's
+        cluster_sync();
+        if (rank != 0) {
+            const uint32_t n = min(sh.list_n, (uint32_t)kListMax);
+            if (tid == 0) sh.list_at = n ? add_remote(remote(&sh.list_n, 0), n) : 0;
+            __syncthreads();
+            for (uint32_t j = tid; j < n; j += kThreads)
+                if (sh.list_at + j < kListMax) st_remote(remote(list + sh.list_at + j, 0), list[j]);
+        }
+        cluster_sync();
+    } else {
+        __syncthreads();
+    }
     if (rank == 0) {
         const int n = min((int)sh.list_n, kListMax), nk = (int)min((uint32_t)n, sh.k_left), segs = C * kWarps;
         u64 above = 0, rest = 0;

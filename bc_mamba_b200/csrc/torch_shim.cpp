@@ -1281,37 +1281,49 @@ bcm_dtype float_dtype(const Tensor& t, const char* name) {
     return to_bcm(t.scalar_type(), name);
 }
 
-// x, r, i (or dy): (B, L, D), packed (T, D), or one token (B, D); unit stride of the features
-void check_rows(const char* what, const Tensor& t, const char* name, const Tensor& like) {
+// t, copied only where its last dimension is strided
+Tensor unit_last(const Tensor& t) { return t.dim() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+// x, r, i (or dy): (B, L, D), packed (T, D), or one token (B, D) -> the tensor with unit stride of the features
+Tensor check_rows(const char* what, const Tensor& t, const char* name, const Tensor& like) {
     TORCH_CHECK(t.is_cuda() && t.device() == like.device(), what, ": ", name, " must be on the device of x");
     TORCH_CHECK(t.scalar_type() == like.scalar_type(), what, ": ", name, " must have the dtype of x");
     TORCH_CHECK(t.sizes() == like.sizes(), what, ": ", name, " must have the shape of x");
-    TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1, what, ": ", name, " must have unit stride in its last dimension");
+    return unit_last(t);
 }
 
-const float* fp32_ptr(const char* what, const Tensor& t, const char* name, const Tensor& like, c10::IntArrayRef shape) {
-    TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == at::ScalarType::Float && t.is_contiguous(),
-                what, ": ", name, " must be a contiguous float32 tensor on the device of the input");
+Tensor fp32_like(const char* what, const Tensor& t, const char* name, const Tensor& like, c10::IntArrayRef shape) {
+    TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == at::ScalarType::Float, what, ": ", name,
+                " must be a float32 tensor on the device of the input");
     TORCH_CHECK(t.sizes() == shape, what, ": ", name, " has the wrong shape");
-    return t.data_ptr<float>();
+    return t.contiguous();
 }
+
+// Copies that a call reads through raw pointers, alive until it has launched.
+struct Held {
+    std::vector<Tensor> all;
+    const Tensor& operator()(Tensor t) {
+        all.push_back(std::move(t));
+        return all.back();
+    }
+    const float* fp32(const char* what, const Tensor& t, const char* name, const Tensor& like, c10::IntArrayRef shape) {
+        return (*this)(fp32_like(what, t, name, like, shape)).data_ptr<float>();
+    }
+};
 
 // Sizes, input pointers and strides of a gated recurrence (forward and backward).
 bcm_gated_rec_args gated_rec_args(const char* what, const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& lam,
-                                  const optional<Tensor>& h0, const optional<Tensor>& cu_seqlens, double decay_scale) {
+                                  const optional<Tensor>& h0, const optional<Tensor>& cu_seqlens, double decay_scale, Held& held) {
     TORCH_CHECK(x.is_cuda(), what, ": x must be on CUDA");
     const bool packed = cu_seqlens.has_value();
     TORCH_CHECK(x.dim() == (packed ? 2 : 3), what, ": x must be (B, L, D), or (T, D) with cu_seqlens");
     bcm_gated_rec_args a{};
     a.dtype = float_dtype(x, "x");
-    check_rows(what, x, "x", x);
-    check_rows(what, r, "r", x);
-    check_rows(what, i, "i", x);
     if (packed) {
-        const Tensor& cu = *cu_seqlens;
-        TORCH_CHECK(cu.is_cuda() && cu.device() == x.device() && cu.scalar_type() == at::ScalarType::Int &&
-                        cu.is_contiguous() && cu.dim() == 1 && cu.size(0) >= 1,
-                    what, ": cu_seqlens must be a contiguous 1-D int32 tensor on the device of x");
+        TORCH_CHECK(cu_seqlens->is_cuda() && cu_seqlens->device() == x.device() &&
+                        cu_seqlens->scalar_type() == at::ScalarType::Int && cu_seqlens->dim() == 1 && cu_seqlens->size(0) >= 1,
+                    what, ": cu_seqlens must be a 1-D int32 tensor on the device of x");
+        const Tensor cu = held(cu_seqlens->contiguous());
         a.batch = cu.size(0) - 1;
         a.seqlen = x.size(0);
         a.cu_seqlens = cu.data_ptr<int32_t>();
@@ -1322,16 +1334,17 @@ bcm_gated_rec_args gated_rec_args(const char* what, const Tensor& x, const Tenso
     }
     a.dim = x.size(-1);
     TORCH_CHECK(a.dim >= 1, what, ": x must have features");
-    auto set = [&](const Tensor& t, const void*& p, int64_t& sb, int64_t& st) {
+    auto set = [&](const Tensor& from, const char* name, const void*& p, int64_t& sb, int64_t& st) {
+        const Tensor& t = held(check_rows(what, from, name, x));
         p = t.data_ptr();
         sb = packed ? 0 : t.stride(0);
         st = t.stride(packed ? 0 : 1);
     };
-    set(x, a.x, a.x_stride_b, a.x_stride_t);
-    set(r, a.r, a.r_stride_b, a.r_stride_t);
-    set(i, a.i, a.i_stride_b, a.i_stride_t);
-    a.lam = fp32_ptr(what, lam, "lam", x, {a.dim});
-    a.h0 = h0.has_value() ? fp32_ptr(what, *h0, "h0", x, {a.batch, a.dim}) : nullptr;
+    set(x, "x", a.x, a.x_stride_b, a.x_stride_t);
+    set(r, "r", a.r, a.r_stride_b, a.r_stride_t);
+    set(i, "i", a.i, a.i_stride_b, a.i_stride_t);
+    a.lam = held.fp32(what, lam, "lam", x, {a.dim});
+    a.h0 = h0.has_value() ? held.fp32(what, *h0, "h0", x, {a.batch, a.dim}) : nullptr;
     a.decay_scale = (float)decay_scale;
     return a;
 }
@@ -1339,7 +1352,8 @@ bcm_gated_rec_args gated_rec_args(const char* what, const Tensor& x, const Tenso
 std::vector<Tensor> gated_rec_fwd(const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& lam,
                                   const optional<Tensor>& h0, const optional<Tensor>& cu_seqlens, double decay_scale,
                                   bool keep_ckpt) {
-    bcm_gated_rec_args a = gated_rec_args("gated_rec_fwd", x, r, i, lam, h0, cu_seqlens, decay_scale);
+    Held held;
+    bcm_gated_rec_args a = gated_rec_args("gated_rec_fwd", x, r, i, lam, h0, cu_seqlens, decay_scale, held);
     c10::cuda::CUDAGuard guard(x.device());
     auto y = torch::empty(x.sizes(), x.options());
     auto h_last = torch::empty({a.batch, a.dim}, lam.options());
@@ -1359,14 +1373,15 @@ std::vector<Tensor> gated_rec_fwd(const Tensor& x, const Tensor& r, const Tensor
 std::vector<Tensor> gated_rec_bwd(const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& lam,
                                   const optional<Tensor>& h0, const optional<Tensor>& cu_seqlens, double decay_scale,
                                   const Tensor& ckpt, const optional<Tensor>& dy, const optional<Tensor>& dh_last) {
-    bcm_gated_rec_args a = gated_rec_args("gated_rec_bwd", x, r, i, lam, h0, cu_seqlens, decay_scale);
+    Held held;
+    bcm_gated_rec_args a = gated_rec_args("gated_rec_bwd", x, r, i, lam, h0, cu_seqlens, decay_scale, held);
     if (dy.has_value()) {
-        check_rows("gated_rec_bwd", *dy, "dy", x);
-        a.dy = dy->data_ptr();
-        a.dy_stride_b = a.cu_seqlens ? 0 : dy->stride(0);
-        a.dy_stride_t = dy->stride(a.cu_seqlens ? 0 : 1);
+        const Tensor& g = held(check_rows("gated_rec_bwd", *dy, "dy", x));
+        a.dy = g.data_ptr();
+        a.dy_stride_b = a.cu_seqlens ? 0 : g.stride(0);
+        a.dy_stride_t = g.stride(a.cu_seqlens ? 0 : 1);
     }
-    if (dh_last.has_value()) a.dh_last = fp32_ptr("gated_rec_bwd", *dh_last, "dh_last", x, {a.batch, a.dim});
+    if (dh_last.has_value()) a.dh_last = held.fp32("gated_rec_bwd", *dh_last, "dh_last", x, {a.batch, a.dim});
     TORCH_CHECK(ckpt.is_cuda() && ckpt.device() == x.device() && ckpt.is_contiguous(),
                 "gated_rec_bwd: ckpt must be the buffer gated_rec_fwd returned for these inputs");
     c10::cuda::CUDAGuard guard(x.device());
@@ -1394,53 +1409,53 @@ Tensor gated_rec_step(const Tensor& x, const Tensor& r, const Tensor& i, const T
     const char* what = "gated_rec_step";
     TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.size(1) >= 1, what, ": x must be a CUDA tensor (B, D)");
     const bcm_dtype dt = float_dtype(x, "x");
-    check_rows(what, x, "x", x);
-    check_rows(what, r, "r", x);
-    check_rows(what, i, "i", x);
-    fp32_ptr(what, lam, "lam", x, {x.size(1)});
-    fp32_ptr(what, h, "h", x, {x.size(0), x.size(1)});
+    const Tensor xs = check_rows(what, x, "x", x), rs = check_rows(what, r, "r", x), is = check_rows(what, i, "i", x);
+    const Tensor l = fp32_like(what, lam, "lam", x, {x.size(1)});
+    TORCH_CHECK(h.is_contiguous(), what, ": h must be a contiguous float32 tensor (it is updated in place)");
+    fp32_like(what, h, "h", x, {x.size(0), x.size(1)});
     c10::cuda::CUDAGuard guard(x.device());
     auto y = torch::empty(x.sizes(), x.options());
-    check_status(bcm_gated_rec_step(x.data_ptr(), x.stride(0), r.data_ptr(), r.stride(0), i.data_ptr(), i.stride(0), dt,
-                                    x.size(0), x.size(1), lam.data_ptr<float>(), (float)decay_scale, h.data_ptr<float>(),
+    check_status(bcm_gated_rec_step(xs.data_ptr(), xs.stride(0), rs.data_ptr(), rs.stride(0), is.data_ptr(), is.stride(0), dt,
+                                    x.size(0), x.size(1), l.data_ptr<float>(), (float)decay_scale, h.data_ptr<float>(),
                                     y.data_ptr(), cur_stream()),
                  what);
     return y;
 }
 
 bcm_distill_args distill_args(const char* what, const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_ids,
-                              const optional<Tensor>& weight, double temperature) {
+                              const optional<Tensor>& weight, double temperature, Held& held) {
     TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, what, ": logits must be a CUDA tensor (T, V)");
     bcm_distill_args a{};
     a.dtype = float_dtype(logits, "logits");
-    TORCH_CHECK(logits.size(1) >= 1 && (logits.size(1) == 1 || logits.stride(1) == 1), what,
-                ": logits must have unit stride in their last dimension");
+    TORCH_CHECK(logits.size(1) >= 1, what, ": logits of an empty vocabulary");
     TORCH_CHECK(teacher_logits.is_cuda() && teacher_logits.device() == logits.device() && teacher_logits.dim() == 2 &&
-                    teacher_logits.size(0) == logits.size(0) && teacher_logits.is_contiguous(),
-                what, ": teacher_logits must be a contiguous (T, K) tensor on the device of the logits");
+                    teacher_logits.size(0) == logits.size(0),
+                what, ": teacher_logits must be a (T, K) tensor on the device of the logits");
     a.teacher_dtype = float_dtype(teacher_logits, "teacher_logits");
     const bool wide = teacher_ids.scalar_type() == at::ScalarType::Long;
     TORCH_CHECK(wide || teacher_ids.scalar_type() == at::ScalarType::Int, what, ": teacher_ids must be int32 or int64");
     TORCH_CHECK(teacher_ids.is_cuda() && teacher_ids.device() == logits.device() &&
-                    teacher_ids.sizes() == teacher_logits.sizes() && teacher_ids.is_contiguous(),
-                what, ": teacher_ids must be contiguous, of the shape of teacher_logits, on the device of the logits");
+                    teacher_ids.sizes() == teacher_logits.sizes(),
+                what, ": teacher_ids must have the shape of teacher_logits and be on the device of the logits");
     a.rows = logits.size(0);
     a.vocab = logits.size(1);
     a.k = teacher_logits.size(1);
     a.ids_are_int64 = wide ? 1 : 0;
     a.temperature = (float)temperature;
-    a.logits = logits.data_ptr();
-    a.logits_stride = logits.stride(0);
-    a.teacher_logits = teacher_logits.data_ptr();
-    a.teacher_ids = teacher_ids.data_ptr();
-    a.weight = weight.has_value() ? fp32_ptr(what, *weight, "weight", logits, {a.rows}) : nullptr;
+    const Tensor z = held(unit_last(logits));
+    a.logits = z.data_ptr();
+    a.logits_stride = z.stride(0);
+    a.teacher_logits = held(teacher_logits.contiguous()).data_ptr();
+    a.teacher_ids = held(teacher_ids.contiguous()).data_ptr();
+    a.weight = weight.has_value() ? held.fp32(what, *weight, "weight", logits, {a.rows}) : nullptr;
     return a;
 }
 
 // -> [loss, stats], with grad also [dlogits] for an upstream gradient of one
 std::vector<Tensor> distill_fwd(const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_ids,
                                 const optional<Tensor>& weight, double temperature, bool grad) {
-    bcm_distill_args a = distill_args("distill_fwd", logits, teacher_logits, teacher_ids, weight, temperature);
+    Held held;
+    bcm_distill_args a = distill_args("distill_fwd", logits, teacher_logits, teacher_ids, weight, temperature, held);
     c10::cuda::CUDAGuard guard(logits.device());
     auto opt = logits.options().dtype(at::ScalarType::Float);
     auto loss = torch::empty({a.rows}, opt), stats = torch::empty({a.rows, 2}, opt);
@@ -1460,12 +1475,11 @@ Tensor distill_bwd(const Tensor& logits, const Tensor& teacher_logits, const Ten
                    const optional<Tensor>& weight, double temperature, const Tensor& loss, const Tensor& stats,
                    const Tensor& dloss) {
     const char* what = "distill_bwd";
-    bcm_distill_args a = distill_args(what, logits, teacher_logits, teacher_ids, weight, temperature);
-    fp32_ptr(what, loss, "loss", logits, {a.rows});
-    fp32_ptr(what, stats, "stats", logits, {a.rows, 2});
-    a.loss = loss.data_ptr<float>();
-    a.stats = stats.data_ptr<float>();
-    a.dloss = fp32_ptr(what, dloss, "dloss", logits, {a.rows});
+    Held held;
+    bcm_distill_args a = distill_args(what, logits, teacher_logits, teacher_ids, weight, temperature, held);
+    a.loss = const_cast<float*>(held.fp32(what, loss, "loss", logits, {a.rows}));
+    a.stats = const_cast<float*>(held.fp32(what, stats, "stats", logits, {a.rows, 2}));
+    a.dloss = held.fp32(what, dloss, "dloss", logits, {a.rows});
     c10::cuda::CUDAGuard guard(logits.device());
     auto dlogits = torch::empty({a.rows, a.vocab}, logits.options());
     a.dlogits = dlogits.data_ptr();
@@ -1481,27 +1495,27 @@ std::vector<Tensor> sample_tokens(const Tensor& logits, const Tensor& u, double 
     TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, what, ": logits must be a CUDA tensor (B, V)");
     bcm_sample_args a{};
     a.dtype = float_dtype(logits, "logits");
-    TORCH_CHECK(logits.size(1) >= 1 && (logits.size(1) == 1 || logits.stride(1) == 1), what,
-                ": logits must have unit stride in their last dimension");
+    TORCH_CHECK(logits.size(1) >= 1, what, ": logits of an empty vocabulary");
     const int64_t B = logits.size(0);
     a.batch = B;
     a.vocab = logits.size(1);
-    a.logits = logits.data_ptr();
-    a.logits_stride = logits.stride(0);
-    a.u = fp32_ptr(what, u, "u", logits, {B});
+    Held held;
+    const Tensor z = held(unit_last(logits));
+    a.logits = z.data_ptr();
+    a.logits_stride = z.stride(0);
+    a.u = held.fp32(what, u, "u", logits, {B});
     a.temperature_all = (float)temperature;
     a.top_k_all = (int32_t)std::min<int64_t>(std::max<int64_t>(top_k, 0), INT32_MAX);
     a.top_p_all = (float)top_p;
     a.min_p_all = (float)min_p;
-    if (temperatures.has_value()) a.temperature = fp32_ptr(what, *temperatures, "temperature", logits, {B});
-    if (top_ps.has_value()) a.top_p = fp32_ptr(what, *top_ps, "top_p", logits, {B});
-    if (min_ps.has_value()) a.min_p = fp32_ptr(what, *min_ps, "min_p", logits, {B});
+    if (temperatures.has_value()) a.temperature = held.fp32(what, *temperatures, "temperature", logits, {B});
+    if (top_ps.has_value()) a.top_p = held.fp32(what, *top_ps, "top_p", logits, {B});
+    if (min_ps.has_value()) a.min_p = held.fp32(what, *min_ps, "min_p", logits, {B});
     if (top_ks.has_value()) {
         TORCH_CHECK(top_ks->is_cuda() && top_ks->device() == logits.device() &&
-                        top_ks->scalar_type() == at::ScalarType::Int && top_ks->is_contiguous() && top_ks->dim() == 1 &&
-                        top_ks->size(0) == B,
-                    what, ": top_k must be a contiguous int32 tensor (B) on the device of the logits");
-        a.top_k = top_ks->data_ptr<int32_t>();
+                        top_ks->scalar_type() == at::ScalarType::Int && top_ks->dim() == 1 && top_ks->size(0) == B,
+                    what, ": top_k must be an int32 tensor (B) on the device of the logits");
+        a.top_k = held(top_ks->contiguous()).data_ptr<int32_t>();
     }
     c10::cuda::CUDAGuard guard(logits.device());
     auto tokens = torch::empty({B}, logits.options().dtype(at::ScalarType::Long));

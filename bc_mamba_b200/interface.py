@@ -57,27 +57,33 @@ def stage_timing():
         _stage_log = prev
 
 
-@contextlib.contextmanager
-def cuda_stage(name: str):
+class cuda_stage:
     """NVTX range named like the reference's profiling stages
     (spike_mamba/runtime_breakdown.py:12-15), timed with CUDA events while
     stage_timing() is open."""
-    if torch.cuda.is_available():
-        log = _stage_log
-        torch.cuda.nvtx.range_push(name)
-        if log is not None:
-            start = torch.cuda.Event(enable_timing=True)
-            start.record()
-        try:
-            yield
-        finally:
-            if log is not None:
+
+    __slots__ = ("name", "on", "log", "start")
+
+    def __init__(self, name: str):
+        self.name = name
+
+    def __enter__(self):
+        self.on = torch.cuda.is_available()
+        if self.on:
+            self.log = _stage_log
+            torch.cuda.nvtx.range_push(self.name)
+            if self.log is not None:
+                self.start = torch.cuda.Event(enable_timing=True)
+                self.start.record()
+
+    def __exit__(self, *exc):
+        if self.on:
+            if self.log is not None:
                 end = torch.cuda.Event(enable_timing=True)
                 end.record()
-                log.append((name, start, end))
+                self.log.append((self.name, self.start, end))
             torch.cuda.nvtx.range_pop()
-    else:
-        yield
+        return False
 
 
 class SelectiveScanFlatChFn(torch.autograd.Function):
@@ -421,21 +427,11 @@ class EventDecoder:
 # token sampler for models built on this package's scans)
 
 
-def _unit(t):
-    """t, copied only where its last dimension is strided."""
-    return t if t is None or t.size(-1) <= 1 or t.stride(-1) == 1 else t.contiguous()
-
-
-def _flat(t):
-    return None if t is None else t.contiguous()
-
-
 class GatedRecurrenceFn(torch.autograd.Function):
     """Gated linear recurrence; see gated_recurrence."""
 
     @staticmethod
     def forward(ctx, x, r, i, lam, h0, cu_seqlens, decay_scale):
-        x, r, i, lam, h0, cu_seqlens = _unit(x), _unit(r), _unit(i), _flat(lam), _flat(h0), _flat(cu_seqlens)
         keep = any(ctx.needs_input_grad[:5])
         with cuda_stage("gated_recurrence_forward"):
             res = load_ops().gated_rec_fwd(x, r, i, lam, h0, cu_seqlens, decay_scale, keep)
@@ -452,8 +448,7 @@ class GatedRecurrenceFn(torch.autograd.Function):
             return (None,) * 7
         x, r, i, lam, h0, cu_seqlens, ckpt = ctx.saved_tensors
         with cuda_stage("gated_recurrence_backward"):
-            dx, dr, di, dlam, dh0 = load_ops().gated_rec_bwd(x, r, i, lam, h0, cu_seqlens, ctx.decay_scale, ckpt,
-                                                             _unit(dy), _flat(dh_last))
+            dx, dr, di, dlam, dh0 = load_ops().gated_rec_bwd(x, r, i, lam, h0, cu_seqlens, ctx.decay_scale, ckpt, dy, dh_last)
         return dx, dr, di, dlam, dh0 if h0 is not None else None, None, None
 
 
@@ -475,7 +470,7 @@ def gated_recurrence(x, r, i, lam, h0=None, cu_seqlens=None, decay_scale: float 
 def gated_recurrence_step(x, r, i, lam, h, decay_scale: float = 8.0):
     """One token of gated_recurrence for every sequence: x, r, i (B, D), the
     state h (B, D) float32 contiguous, updated in place.  Returns y (B, D)."""
-    return load_ops().gated_rec_step(_unit(x), _unit(r), _unit(i), lam.contiguous(), h, float(decay_scale))
+    return load_ops().gated_rec_step(x, r, i, lam, h, decay_scale)
 
 
 class DistillTopkFn(torch.autograd.Function):
@@ -483,7 +478,6 @@ class DistillTopkFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, teacher_logits, teacher_ids, weight, temperature):
-        logits, teacher_logits, teacher_ids, weight = _unit(logits), _flat(teacher_logits), _flat(teacher_ids), _flat(weight)
         with cuda_stage("distill_forward"):
             loss, stats = load_ops().distill_fwd(logits, teacher_logits, teacher_ids, weight, temperature)
         if ctx.needs_input_grad[0]:
@@ -496,8 +490,7 @@ class DistillTopkFn(torch.autograd.Function):
     def backward(ctx, dloss):
         logits, teacher_logits, teacher_ids, weight, loss, stats = ctx.saved_tensors
         with cuda_stage("distill_backward"):
-            dz = load_ops().distill_bwd(logits, teacher_logits, teacher_ids, weight, ctx.temperature, loss, stats,
-                                        dloss.contiguous())
+            dz = load_ops().distill_bwd(logits, teacher_logits, teacher_ids, weight, ctx.temperature, loss, stats, dloss)
         return dz, None, None, None, None
 
 
@@ -519,8 +512,7 @@ def distill_topk_with_grad(logits, teacher_logits, teacher_ids, weight=None, tem
     scale, into weight).  It reads the logits from memory once where the
     autograd pair reads them twice."""
     with torch.no_grad(), cuda_stage("distill_forward"):
-        loss, _, dz = load_ops().distill_fwd(_unit(logits.detach()), _flat(teacher_logits.detach()), _flat(teacher_ids),
-                                             _flat(weight), float(temperature), True)
+        loss, _, dz = load_ops().distill_fwd(logits, teacher_logits, teacher_ids, weight, float(temperature), True)
     return loss, dz
 
 
@@ -530,7 +522,7 @@ def _per_row(value, off, dtype):
         return (off if value is None else value), None
     if dtype == torch.int32 and value.dtype != dtype:
         value = value.clamp(0, 2 ** 31 - 1)
-    return off, value.to(dtype).contiguous()
+    return off, value if value.dtype == dtype else value.to(dtype)
 
 
 def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -548,5 +540,5 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     p, ps = _per_row(top_p, 1.0, torch.float32)
     m, ms = _per_row(min_p, 0.0, torch.float32)
     with torch.no_grad(), cuda_stage("sample_tokens"):
-        tokens, logprob = load_ops().sample_tokens(_unit(logits.detach()), u.contiguous(), t, k, p, m, ts, ks, ps, ms)
+        tokens, logprob = load_ops().sample_tokens(logits, u, t, k, p, m, ts, ks, ps, ms)
     return tokens, logprob

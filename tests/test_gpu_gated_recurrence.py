@@ -101,6 +101,23 @@ def test_packed(cu, D, dtype):
     _check(_inputs(cu[-1], D, len(cu) - 1, dtype, seed=len(cu) + D), cu, None)
 
 
+@pytest.mark.parametrize("B,L,D,dtype", [(1800, 9, 30, torch.float32), (900, 70, 130, torch.bfloat16), (2000, 3, 7, torch.float16), (5000, 8, 64, torch.float32),
+                                         (600, 33, 161, torch.float32), (20000, 1, 6, torch.float32)])
+def test_a_warp_for_each_sequence(B, L, D, dtype):
+    _check(_inputs(B * L, D, B, dtype, seed=B + L), range(0, B * L + 1, L), (B, L))
+    if B == 1800:
+        for h0, dy, dh in ((False, True, False), (True, False, True)):
+            _check(_inputs(B * L, D, B, dtype, seed=3), range(0, B * L + 1, L), (B, L), h0, dy, dh)
+        t = _inputs(B * L, 3 * D, B, dtype, seed=4)        # sequences apart from one another, rows off 16 bytes
+        wide = [torch.zeros(B, L + 2, 3 * D + 1, device=dev)[:, 1:L + 1, 1:] for _ in range(3)]
+        for v, k in zip(wide, ("x", "r", "i")):
+            v.copy_(t[k].reshape(B, L, 3 * D))
+        y, h = itf.gated_recurrence(*wide, t["lam"], h0=t["h0"])
+        want = itf.gated_recurrence(*(v.contiguous() for v in wide), t["lam"], h0=t["h0"])
+        assert_exact(y, want[0], "y")
+        assert_exact(h, want[1], "h_last")
+
+
 @pytest.mark.parametrize("seed,n,T,D", [(0, 9, 700, 40), (1, 64, 5000, 6), (2, 200, 9000, 70), (3, 1500, 3000, 3), (4, 40, 20000, 2)])
 def test_packed_runs(seed, n, T, D):
     """Many sequences of uneven length, cut at random (some empty), and one that takes nearly every token."""

@@ -244,7 +244,7 @@ def test_refusals():
     for args, kw, match in [((x.double(), u), {}, "float32, float16 or bfloat16"), ((x[0], u), {}, "\\(B, V\\)"), ((x, u[:1]), {}, "u has the wrong shape"),
                             ((x, u.half()), {}, "u must be"), ((x.cpu(), u), {}, "CUDA"), ((x, u), dict(top_p=u[:1]), "top_p has the wrong shape"),
                             ((x, u), dict(top_k=torch.zeros(3, dtype=torch.int32, device=dev)), "top_k"),
-                            ((x, u), dict(temperature=torch.ones(2)), "temperature must be"), ((x[:, :0], u), {}, "unit stride")]:
+                            ((x, u), dict(temperature=torch.ones(2)), "temperature must be"), ((x[:, :0], u), {}, "empty vocabulary")]:
         with pytest.raises(RuntimeError, match=match):
             itf.sample_tokens(*args, **kw)
     with pytest.raises(RuntimeError, match="vocab must be"):

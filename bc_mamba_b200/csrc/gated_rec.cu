@@ -271,14 +271,13 @@ struct Rows {
             if (EVEN) return *reinterpret_cast<const float2*>(p);
             return make_float2(*reinterpret_cast<const float*>(p), *reinterpret_cast<const float*>(p + 4));
         } else {
-            const T *e = reinterpret_cast<const T*>(p);
-            if (EVEN) {
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
-                T v[2];
-                memcpy(v, &w, 4);
-                return make_float2(to_f32<T>(v[0]), to_f32<T>(v[1]));
-            }
-            return make_float2(to_f32<T>(e[0]), to_f32<T>(e[1]));
+            // (a row that starts between two words: both words of the pair)
+            const uint32_t* q = reinterpret_cast<const uint32_t*>(EVEN ? p : p - (off & 2));
+            uint32_t w = q[0];
+            if (!EVEN && (off & 2)) w = __funnelshift_r(w, q[1], 16);
+            T v[2];
+            memcpy(v, &w, 4);
+            return make_float2(to_f32<T>(v[0]), to_f32<T>(v[1]));
         }
     }
 };
@@ -293,9 +292,10 @@ struct Input {
 template <typename T, int MODE, bool EVEN, int S>
 struct Stream {
     using R = Rows<T, EVEN>;
-    static constexpr int kLaneRows = EVEN ? 32 / R::kGran : 1;      // rows of a warp's copy instruction
+    static constexpr int kLaneRows = 32 / R::kGran;      // rows of a warp's copy instruction
     const char* at;
     int bytes;
+    uint32_t low, step;                                  // the run's first row and the distance of rows, in bytes, mod 2^32
     __device__ __forceinline__ static bool linear(const Input& in, const RecDim& n) { return MODE != kGroup || in.sb == in.st * n.Ls; }
     // elements from the run's first row to that of token t
     __device__ __forceinline__ static int64_t row(const Input& in, const RecDim& n, int t) {
@@ -308,7 +308,10 @@ struct Stream {
     }
     __device__ __forceinline__ Stream(const Input& in, const Place& w, int t0, int width) {
         bytes = max(0, min(16, width * (int)sizeof(T) - w.lane % R::kGran * 16));
-        if (EVEN) at = reinterpret_cast<const char*>(base(in, w) + (int64_t)(t0 + w.lane / R::kGran) * in.st) + w.lane % R::kGran * 16;
+        low = (uint32_t)(uintptr_t)base(in, w);
+        step = (uint32_t)(in.st * (int)sizeof(T));
+        at = reinterpret_cast<const char*>(base(in, w) + (int64_t)(t0 + w.lane / R::kGran) * in.st);
+        if (EVEN) at += w.lane % R::kGran * 16;          // (otherwise the row's start: its granules move with it)
     }
     // t0: the first row; advance: tokens from this fetch to the next; rows and features that are not there become zeros
     __device__ __forceinline__ void fetch(char* dst, const Input& in, const Place& w, const RecDim& n, int t0, int advance, int width) {
@@ -319,6 +322,19 @@ struct Stream {
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + w.lane * 16 + k * 512),
                              "l"(at + (int64_t)(k * kLaneRows) * in.st * (int)sizeof(T)), "r"(bytes)
                              : "memory");
+        } else if (!EVEN && t0 + S <= w.L && linear(in, n)) {
+            const int j0 = w.lane / R::kGran, g = w.lane - j0 * R::kGran;
+            const char* first = at;
+#pragma unroll
+            for (int j = 0; j < S; j += kLaneRows) {
+                const uintptr_t from = ((uintptr_t)first & ~(uintptr_t)15) + g * 16;
+                const int left = (int)((int64_t)((uintptr_t)first + width * sizeof(T)) - (int64_t)from);
+                if (j0 < kLaneRows && j0 + j < S)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + (j0 + j) * R::kPitch + g * 16),
+                                 "l"(left > 0 ? from : (uintptr_t)first & ~(uintptr_t)15), "r"(max(0, min(16, left)))
+                                 : "memory");
+                first += (int64_t)kLaneRows * in.st * (int)sizeof(T);
+            }
         } else {
             const T* from0 = base(in, w);
             for (int q = w.lane; q < S * R::kGran; q += 32) {
@@ -336,12 +352,12 @@ struct Stream {
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + j * R::kPitch + g * 16), "l"(src), "r"(bytes) : "memory");
             }
         }
-        if (EVEN) at += (int64_t)advance * in.st * (int)sizeof(T);
+        at += (int64_t)advance * in.st * (int)sizeof(T);
     }
     // the lane's two features of token t, in slot j of the fetched rows
-    __device__ __forceinline__ static float2 read(const char* from, const Input& in, const Place& w, const RecDim& n, int j, int t) {
+    __device__ __forceinline__ float2 read(const char* from, const Input& in, const RecDim& n, int j, int t) const {
         uint32_t off = 0;
-        if (!EVEN) off = ((uint32_t)(uintptr_t)base(in, w) + (uint32_t)row(in, n, t) * (uint32_t)sizeof(T)) & 15u;
+        if (!EVEN) off = (low + (linear(in, n) ? (uint32_t)t * step : (uint32_t)row(in, n, t) * (uint32_t)sizeof(T))) & 15u;
         return R::read(from + j * R::kPitch, (int)off);
     }
 };
@@ -366,6 +382,8 @@ template <typename T, bool EVEN>
 __device__ __forceinline__ void store_pair(T* p, float2 v, bool even_rows, bool has0, bool has1) {
     if (EVEN || even_rows) {
         store_row<T>(p, v, has0, false);
+    } else if (((uintptr_t)p & (2 * sizeof(T) - 1)) == 0) {      // (every other row of an odd number of features)
+        store_row<T>(p, v, has1, has0);
     } else {
         if (has0) p[0] = from_f32<T>(v.x);
         if (has1) p[1] = from_f32<T>(v.y);
@@ -491,16 +509,16 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         float prod = 0.0f;
 #pragma unroll
         for (int j = 0; j < S; ++j) {
-            const Gates g = gates<true>(In::read(at, ir, w, n, j, t0 + j), In::read(at, ii, w, n, S + j, t0 + j), cs, consts, prod);
+            const Gates g = gates<true>(sr.read(at, ir, n, j, t0 + j), si.read(at, ii, n, S + j, t0 + j), cs, consts, prod);
             a[j] = g.a;
-            e[j] = mul(mul(g.m, g.si), In::read(at, ix, w, n, 2 * S + j, t0 + j));
+            e[j] = mul(mul(g.m, g.si), sx.read(at, ix, n, 2 * S + j, t0 + j));
         }
         if (!__all_sync(kFull, small && prod < kProdEnd)) {
 #pragma unroll
             for (int j = 0; j < S; ++j) {
-                const Gates g = gates<false>(In::read(at, ir, w, n, j, t0 + j), In::read(at, ii, w, n, S + j, t0 + j), cs, consts, prod);
+                const Gates g = gates<false>(sr.read(at, ir, n, j, t0 + j), si.read(at, ii, n, S + j, t0 + j), cs, consts, prod);
                 a[j] = g.a;
-                e[j] = mul(mul(g.m, g.si), In::read(at, ix, w, n, 2 * S + j, t0 + j));
+                e[j] = mul(mul(g.m, g.si), sx.read(at, ix, n, 2 * S + j, t0 + j));
             }
         }
         if (t0 + S > L)                   // tokens past the end change nothing
@@ -703,13 +721,13 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         float prod = 0.0f;
 #pragma unroll
         for (int j = 0; j < S; ++j) {
-            const Gates g = gates<true>(In::read(at, ir, w, n, j, t0 + j), In::read(at, ii, w, n, S + j, t0 + j), cs, consts, prod);
+            const Gates g = gates<true>(sr.read(at, ir, n, j, t0 + j), si.read(at, ii, n, S + j, t0 + j), cs, consts, prod);
             q.sr[j] = g.sr; q.si[j] = g.si; q.a[j] = g.a; q.rs[j] = g.rs; q.msi[j] = mul(g.m, g.si);
         }
         if (!__all_sync(kFull, small && prod < kProdEnd)) {
 #pragma unroll
             for (int j = 0; j < S; ++j) {
-                const Gates g = gates<false>(In::read(at, ir, w, n, j, t0 + j), In::read(at, ii, w, n, S + j, t0 + j), cs, consts, prod);
+                const Gates g = gates<false>(sr.read(at, ir, n, j, t0 + j), si.read(at, ii, n, S + j, t0 + j), cs, consts, prod);
                 q.sr[j] = g.sr; q.si[j] = g.si; q.a[j] = g.a; q.rs[j] = g.rs; q.msi[j] = mul(g.m, g.si);
             }
         }
@@ -724,8 +742,8 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         float2 A = f2(1.0f), H = f2(0.0f), K = f2(0.0f);
 #pragma unroll
         for (int j = 0; j < S; ++j) {
-            q.x[j] = In::read(at, ix, w, n, 2 * S + j, t0 + j);
-            q.g[j] = In::read(at, ig, w, n, 3 * S + j, t0 + j);
+            q.x[j] = sx.read(at, ix, n, 2 * S + j, t0 + j);
+            q.g[j] = sg.read(at, ig, n, 3 * S + j, t0 + j);
             const float2 e = mul(q.msi[j], q.x[j]);
             if (CUTS && (q.starts >> j & 1u)) {
                 A = f2(kCut);
@@ -936,16 +954,16 @@ rec_fwd_serial(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         float prod = 0.0f;
 #pragma unroll
         for (int j = 0; j < S; ++j) {
-            const Gates g = gates<true>(In::read(at, ir, w, n, j, t0 + j), In::read(at, ii, w, n, S + j, t0 + j), cs, consts, prod);
+            const Gates g = gates<true>(sr.read(at, ir, n, j, t0 + j), si.read(at, ii, n, S + j, t0 + j), cs, consts, prod);
             a[j] = g.a;
-            e[j] = mul(mul(g.m, g.si), In::read(at, ix, w, n, 2 * S + j, t0 + j));
+            e[j] = mul(mul(g.m, g.si), sx.read(at, ix, n, 2 * S + j, t0 + j));
         }
         if (!__all_sync(kFull, small && prod < kProdEnd)) {
 #pragma unroll
             for (int j = 0; j < S; ++j) {
-                const Gates g = gates<false>(In::read(at, ir, w, n, j, t0 + j), In::read(at, ii, w, n, S + j, t0 + j), cs, consts, prod);
+                const Gates g = gates<false>(sr.read(at, ir, n, j, t0 + j), si.read(at, ii, n, S + j, t0 + j), cs, consts, prod);
                 a[j] = g.a;
-                e[j] = mul(mul(g.m, g.si), In::read(at, ix, w, n, 2 * S + j, t0 + j));
+                e[j] = mul(mul(g.m, g.si), sx.read(at, ix, n, 2 * S + j, t0 + j));
             }
         }
         int64_t ended = seq0 - 1;
@@ -1035,20 +1053,20 @@ rec_bwd_serial(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         float prod = 0.0f;
 #pragma unroll
         for (int j = 0; j < S; ++j) {
-            const Gates g = gates<true>(In::read(at, ir, w, n, j, t0 + j), In::read(at, ii, w, n, S + j, t0 + j), cs, consts, prod);
+            const Gates g = gates<true>(sr.read(at, ir, n, j, t0 + j), si.read(at, ii, n, S + j, t0 + j), cs, consts, prod);
             sgr[j] = g.sr; sgi[j] = g.si; a[j] = g.a; rs[j] = g.rs; msi[j] = mul(g.m, g.si);
         }
         if (!__all_sync(kFull, small && prod < kProdEnd)) {
 #pragma unroll
             for (int j = 0; j < S; ++j) {
-                const Gates g = gates<false>(In::read(at, ir, w, n, j, t0 + j), In::read(at, ii, w, n, S + j, t0 + j), cs, consts, prod);
+                const Gates g = gates<false>(sr.read(at, ir, n, j, t0 + j), si.read(at, ii, n, S + j, t0 + j), cs, consts, prod);
                 sgr[j] = g.sr; sgi[j] = g.si; a[j] = g.a; rs[j] = g.rs; msi[j] = mul(g.m, g.si);
             }
         }
         float2 prev[S], xv[S];
 #pragma unroll
         for (int j = 0; j < S; ++j) {
-            xv[j] = In::read(at, ix, w, n, 2 * S + j, t0 + j);
+            xv[j] = sx.read(at, ix, n, 2 * S + j, t0 + j);
             if (starts >> j & 1u) h = own[j];
             prev[j] = h;
             h = fma(a[j], h, mul(msi[j], xv[j]));
@@ -1059,7 +1077,7 @@ rec_bwd_serial(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
 #pragma unroll
         for (int j = S - 1; j >= 0; --j) {
             if (t0 + j < L) {
-                const float2 G = add(In::read(at, ig, w, n, 3 * S + j, t0 + j), back);
+                const float2 G = add(sg.read(at, ig, n, 3 * S + j, t0 + j), back);
                 back = mul(a[j], G);
                 const float2 vx = mul(G, msi[j]);
                 const float2 vi = mul(mul(vx, xv[j]), fma(sgi[j], nones, consts.one));

@@ -255,12 +255,16 @@ __device__ __forceinline__ Place place(const RecDim& n, const int32_t* cu) {
 }
 
 // ---- rows in shared memory -----------------------------------------------------
-// A row of a tile is 64 elements from the tile's first feature on.  EVEN: every
-// row starts on 16 bytes.  Otherwise the copy starts at the 16-byte granule that
-// holds the row's first element and takes one granule more; it reads no granule
-// without an element of the row in it.
-template <typename T, bool EVEN>
+// A row of a tile is 64 elements from the tile's first feature on.  kRows16: every
+// row starts on 16 bytes and arrives by 16-byte copies.  kRows4: on 4 bytes, every
+// lane copies its own two features.  kRows2 (16-bit types): the copy starts at the
+// 16-byte granule that holds the row's first element and takes one granule more; it
+// reads no granule without an element of the row in it.  400 x 300 x 300 bf16
+// backward: 236 us by 4-byte copies, 290 us by granules.
+enum Form { kRows2, kRows4, kRows16 };
+template <typename T, int FORM>
 struct Rows {
+    static constexpr bool EVEN = FORM != kRows2;
     static constexpr int kGran = kTile * (int)sizeof(T) / 16 + (EVEN ? 0 : 1);
     static constexpr int kPitch = kGran * 16;
 
@@ -284,14 +288,15 @@ struct Rows {
 
 // One input of a warp: fetches S rows a turn, reads them back.  Where a row of the run follows the one before it by st
 // elements (kDense, kPacked, and kGroup without gaps between sequences) and all S rows are there, the lane's granule
-// (EVEN) only moves along.
+// (kRows16) only moves along.
 struct Input {
     const void* p;
     int64_t sb, st;
 };
-template <typename T, int MODE, bool EVEN, int S>
+template <typename T, int MODE, int FORM, int S>
 struct Stream {
-    using R = Rows<T, EVEN>;
+    using R = Rows<T, FORM>;
+    static constexpr bool EVEN = FORM == kRows16;
     static constexpr int kLaneRows = 32 / R::kGran;      // rows of a warp's copy instruction
     const char* at;
     int bytes;
@@ -311,18 +316,36 @@ struct Stream {
         low = (uint32_t)(uintptr_t)base(in, w);
         step = (uint32_t)(in.st * (int)sizeof(T));
         at = reinterpret_cast<const char*>(base(in, w) + (int64_t)(t0 + w.lane / R::kGran) * in.st);
-        if (EVEN) at += w.lane % R::kGran * 16;          // (otherwise the row's start: its granules move with it)
+        if (EVEN) at += w.lane % R::kGran * 16;          // (kRows2: the row's start, its granules move with it)
+        if (FORM == kRows4) {
+            at = reinterpret_cast<const char*>(base(in, w) + (int64_t)t0 * in.st + w.lane * 2);
+            bytes = max(0, min(2, width - w.lane * 2)) * (int)sizeof(T);
+        }
     }
     // t0: the first row; advance: tokens from this fetch to the next; rows and features that are not there become zeros
     __device__ __forceinline__ void fetch(char* dst, const Input& in, const Place& w, const RecDim& n, int t0, int advance, int width) {
         const uint32_t to = smem_addr(dst);
-        if (EVEN && t0 + S <= w.L && linear(in, n)) {
+        if constexpr (FORM == kRows4) {
+            const bool straight = linear(in, n);
+            const char* none = reinterpret_cast<const char*>(base(in, w));
+#pragma unroll
+            for (int j = 0; j < S; ++j) {
+                const char* src = at + (int64_t)j * in.st * (int)sizeof(T);
+                if (!straight && t0 + j < w.L) src = reinterpret_cast<const char*>(base(in, w) + row(in, n, t0 + j) + w.lane * 2);
+                const int size = t0 + j < w.L ? bytes : 0;
+                if (size == 0) src = none;
+                const uint32_t d = to + j * R::kPitch + w.lane * 2 * (int)sizeof(T);
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"(src), "r"(min(size, 4)) : "memory");
+                if (sizeof(T) == 4)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d + 4), "l"(size > 4 ? src + 4 : none), "r"(max(size - 4, 0)) : "memory");
+            }
+        } else if (EVEN && t0 + S <= w.L && linear(in, n)) {
 #pragma unroll
             for (int k = 0; k < S / kLaneRows; ++k)
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + w.lane * 16 + k * 512),
                              "l"(at + (int64_t)(k * kLaneRows) * in.st * (int)sizeof(T)), "r"(bytes)
                              : "memory");
-        } else if (!EVEN && t0 + S <= w.L && linear(in, n)) {
+        } else if (FORM == kRows2 && t0 + S <= w.L && linear(in, n)) {
             const int j0 = w.lane / R::kGran, g = w.lane - j0 * R::kGran;
             const char* first = at;
 #pragma unroll
@@ -357,7 +380,7 @@ struct Stream {
     // the lane's two features of token t, in slot j of the fetched rows
     __device__ __forceinline__ float2 read(const char* from, const Input& in, const RecDim& n, int j, int t) const {
         uint32_t off = 0;
-        if (!EVEN) off = (low + (linear(in, n) ? (uint32_t)t * step : (uint32_t)row(in, n, t) * (uint32_t)sizeof(T))) & 15u;
+        if (FORM == kRows2) off = (low + (linear(in, n) ? (uint32_t)t * step : (uint32_t)row(in, n, t) * (uint32_t)sizeof(T))) & 15u;
         return R::read(from + j * R::kPitch, (int)off);
     }
 };
@@ -428,8 +451,8 @@ __device__ __forceinline__ const int32_t* stage_cu(const RecDim& n, int32_t* roo
     return room;
 }
 
-template <typename T, int S, bool EVEN, int ARRAYS>
-constexpr int stage_bytes() { return kWarps * ARRAYS * S * Rows<T, EVEN>::kPitch; }
+template <typename T, int S, int FORM, int ARRAYS>
+constexpr int stage_bytes() { return kWarps * ARRAYS * S * Rows<T, FORM>::kPitch; }
 // turns of rows in shared memory, as many as let two blocks share an SM
 template <typename T>
 constexpr int stages_fwd() { return sizeof(T) == 4 ? 2 : 3; }
@@ -443,14 +466,14 @@ struct Pub {
     float4 v[CLUSTER ? 2 : 1][CLUSTER ? kMaxCluster : 1][CLUSTER ? 32 : 1];
 };
 
-template <typename T, int MODE, bool EVEN, bool CLUSTER>
+template <typename T, int MODE, int FORM, bool CLUSTER>
 __global__ void __launch_bounds__(kWarps * 32, 2)
 rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut o, const __grid_constant__ RecDim n,
                const float* __restrict__ lam, float c) {
     constexpr bool CUTS = MODE != kDense;
     constexpr int S = kStepsFwd, kChunk = kWarps * S, ST = stages_fwd<T>();
-    using In = Stream<T, MODE, EVEN, S>;
-    using R = Rows<T, EVEN>;
+    using In = Stream<T, MODE, FORM, S>;
+    using R = Rows<T, FORM>;
     __shared__ float4 ex[2][kWarps][32];
     __shared__ Pub<CLUSTER> pub;
     __shared__ int32_t cus[MODE == kPacked ? kCuMax : 1];
@@ -472,7 +495,7 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
     char* mine = rows + w.warp * (3 * S * R::kPitch);
     auto fetch = [&](int turn) {
         if (turn < turns) {
-            char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 3>();
+            char* at = mine + (turn % ST) * stage_bytes<T, S, FORM, 3>();
             const int t0 = turn * P * kChunk + first;
             sr.fetch(at, ir, w, n, t0, P * kChunk, width);
             si.fetch(at + S * R::kPitch, ii, w, n, t0, P * kChunk, width);
@@ -505,7 +528,7 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         }
         cp_wait<ST - 1>();
         __syncwarp();
-        const char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 3>();
+        const char* at = mine + (turn % ST) * stage_bytes<T, S, FORM, 3>();
         float prod = 0.0f;
 #pragma unroll
         for (int j = 0; j < S; ++j) {
@@ -585,7 +608,7 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
 #pragma unroll
             for (int j = 0; j < S; ++j) {
                 h = fma(a[j], h, e[j]);
-                store_pair<T, EVEN>(out, h, even_rows, w.has0, w.has1);
+                store_pair<T, FORM == kRows16>(out, h, even_rows, w.has0, w.has1);
                 out += D;
             }
         } else {
@@ -594,7 +617,7 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
                 const int t = t0 + j;
                 h = CUTS && (starts >> j & 1u) ? e[j] : fma(a[j], h, e[j]);
                 if (t < L) {
-                    store_pair<T, EVEN>(out, h, even_rows, w.has0, w.has1);
+                    store_pair<T, FORM == kRows16>(out, h, even_rows, w.has0, w.has1);
                     if (CUTS) q.at(t);
                     if (CUTS && t == q.end - 1) store_state(o.h_last, q.s, D, w.d, h, w.has0, w.has1);
                 }
@@ -635,14 +658,14 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
 // Chunks from the last to the first.  The states that enter a chunk come from
 // the forward; back_t = a_t G_t passes from right to left by the same products
 // of decays, back -> A back + K.
-template <typename T, int MODE, bool EVEN, bool CLUSTER>
+template <typename T, int MODE, int FORM, bool CLUSTER>
 __global__ void __launch_bounds__(kWarps * 32, 2)
 rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut o, const __grid_constant__ RecDim n,
                const float* __restrict__ lam, float c) {
     constexpr bool CUTS = MODE != kDense;
     constexpr int S = kStepsBwd, kChunk = kWarps * S, ST = stages_bwd<T>();
-    using In = Stream<T, MODE, EVEN, S>;
-    using R = Rows<T, EVEN>;
+    using In = Stream<T, MODE, FORM, S>;
+    using R = Rows<T, FORM>;
     __shared__ float4 ex[2][kWarps][32];          // (A, K)
     __shared__ float2 exh[2][kWarps][32];         // H
     __shared__ Pub<CLUSTER> pub;
@@ -666,7 +689,7 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
     char* mine = rows + w.warp * (4 * S * R::kPitch);
     auto fetch = [&](int turn) {
         if (turn >= 0) {
-            char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 4>();
+            char* at = mine + (turn % ST) * stage_bytes<T, S, FORM, 4>();
             const int t0 = turn * P * kChunk + first;
             sr.fetch(at, ir, w, n, t0, -P * kChunk, width);
             si.fetch(at + S * R::kPitch, ii, w, n, t0, -P * kChunk, width);
@@ -717,7 +740,7 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         }
         cp_wait<kAhead>();
         __syncwarp();
-        const char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 4>();
+        const char* at = mine + (turn % ST) * stage_bytes<T, S, FORM, 4>();
         float prod = 0.0f;
 #pragma unroll
         for (int j = 0; j < S; ++j) {
@@ -828,9 +851,9 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
             const float2 vr = mul(mul(ds, cs), add(q.sr[j], nones));
             if (full || t0 + j < L) {
                 sum = add(sum, ds);
-                store_pair<T, EVEN>(px, vx, even_rows, w.has0, w.has1);
-                store_pair<T, EVEN>(pr, vr, even_rows, w.has0, w.has1);
-                store_pair<T, EVEN>(pi, vi, even_rows, w.has0, w.has1);
+                store_pair<T, FORM == kRows16>(px, vx, even_rows, w.has0, w.has1);
+                store_pair<T, FORM == kRows16>(pr, vr, even_rows, w.has0, w.has1);
+                store_pair<T, FORM == kRows16>(pi, vi, even_rows, w.has0, w.has1);
             }
             px += D;
             pr += D;
@@ -895,13 +918,13 @@ __device__ __forceinline__ bool place_serial(const RecDim& n, Place& q) {
     return q.run < n.runs;
 }
 
-template <typename T, bool EVEN>
+template <typename T, int FORM>
 __global__ void __launch_bounds__(kWarps * 32, 2)
 rec_fwd_serial(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut o, const __grid_constant__ RecDim n,
                const float* __restrict__ lam, float c) {
     constexpr int S = kStepsFwd, ST = stages_fwd<T>();
-    using In = Stream<T, kGroup, EVEN, S>;
-    using R = Rows<T, EVEN>;
+    using In = Stream<T, kGroup, FORM, S>;
+    using R = Rows<T, FORM>;
     extern __shared__ __align__(16) char rows[];
     Place w;
     if (!place_serial(n, w)) return;
@@ -914,7 +937,7 @@ rec_fwd_serial(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
     char* mine = rows + w.warp * (3 * S * R::kPitch);
     auto fetch = [&](int turn) {
         if (turn < turns) {
-            char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 3>();
+            char* at = mine + (turn % ST) * stage_bytes<T, S, FORM, 3>();
             sr.fetch(at, ir, w, n, turn * S, S, width);
             si.fetch(at + S * R::kPitch, ii, w, n, turn * S, S, width);
             sx.fetch(at + 2 * S * R::kPitch, ix, w, n, turn * S, S, width);
@@ -949,7 +972,7 @@ rec_fwd_serial(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         }
         cp_wait<ST - 1>();
         __syncwarp();
-        const char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 3>();
+        const char* at = mine + (turn % ST) * stage_bytes<T, S, FORM, 3>();
         float2 a[S], e[S];
         float prod = 0.0f;
 #pragma unroll
@@ -977,7 +1000,7 @@ rec_fwd_serial(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
             }
             if (t0 + j < L) {
                 h = fma(a[j], h, e[j]);
-                store_pair<T, EVEN>(out, h, even_rows, w.has0, w.has1);
+                store_pair<T, FORM == kRows16>(out, h, even_rows, w.has0, w.has1);
             }
             out += D;
         }
@@ -986,13 +1009,13 @@ rec_fwd_serial(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
     store_state(o.h_last, w.b + L / n.Ls - 1, D, w.d, h, w.has0, w.has1);
 }
 
-template <typename T, bool EVEN>
+template <typename T, int FORM>
 __global__ void __launch_bounds__(kWarps * 32, 2)
 rec_bwd_serial(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut o, const __grid_constant__ RecDim n,
                const float* __restrict__ lam, float c) {
     constexpr int S = kStepsBwd, ST = stages_bwd<T>();
-    using In = Stream<T, kGroup, EVEN, S>;
-    using R = Rows<T, EVEN>;
+    using In = Stream<T, kGroup, FORM, S>;
+    using R = Rows<T, FORM>;
     extern __shared__ __align__(16) char rows[];
     Place w;
     if (!place_serial(n, w)) return;
@@ -1006,7 +1029,7 @@ rec_bwd_serial(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
     char* mine = rows + w.warp * (4 * S * R::kPitch);
     auto fetch = [&](int turn) {
         if (turn >= 0) {
-            char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 4>();
+            char* at = mine + (turn % ST) * stage_bytes<T, S, FORM, 4>();
             sr.fetch(at, ir, w, n, turn * S, -S, width);
             si.fetch(at + S * R::kPitch, ii, w, n, turn * S, -S, width);
             sx.fetch(at + 2 * S * R::kPitch, ix, w, n, turn * S, -S, width);
@@ -1048,7 +1071,7 @@ rec_bwd_serial(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         }
         cp_wait<ST - 1>();
         __syncwarp();
-        const char* at = mine + (turn % ST) * stage_bytes<T, S, EVEN, 4>();
+        const char* at = mine + (turn % ST) * stage_bytes<T, S, FORM, 4>();
         float2 sgr[S], sgi[S], a[S], rs[S], msi[S];
         float prod = 0.0f;
 #pragma unroll
@@ -1087,9 +1110,9 @@ rec_bwd_serial(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
                 const float2 ds = mul(du, sgr[j]);
                 const float2 vr = mul(mul(ds, cs), add(sgr[j], nones));
                 sum = add(sum, ds);
-                store_pair<T, EVEN>(px + (int64_t)j * D, vx, even_rows, w.has0, w.has1);
-                store_pair<T, EVEN>(pr + (int64_t)j * D, vr, even_rows, w.has0, w.has1);
-                store_pair<T, EVEN>(pi + (int64_t)j * D, vi, even_rows, w.has0, w.has1);
+                store_pair<T, FORM == kRows16>(px + (int64_t)j * D, vx, even_rows, w.has0, w.has1);
+                store_pair<T, FORM == kRows16>(pr + (int64_t)j * D, vr, even_rows, w.has0, w.has1);
+                store_pair<T, FORM == kRows16>(pi + (int64_t)j * D, vi, even_rows, w.has0, w.has1);
             }
             if (starts >> j & 1u) {
                 if (o.dh0) store_state(o.dh0, q, D, w.d, back, w.has0, w.has1);
@@ -1231,8 +1254,8 @@ Plan rec_plan(const bcm_gated_rec_args* a) {
     return pl;
 }
 
-// Whether every row of every input starts on 16 bytes (and the outputs' rows on two features).
-bool rec_even(const bcm_gated_rec_args* a, bool bwd) {
+// What every row of every input starts on (and, for 16 bytes, the outputs' rows on two features).
+int rec_form(const bcm_gated_rec_args* a, bool bwd) {
     const int64_t s = (int64_t)dtype_size(a->dtype);
     int64_t bits = 0;
     auto see = [&](const void* p, int64_t sb, int64_t st) {
@@ -1242,8 +1265,9 @@ bool rec_even(const bcm_gated_rec_args* a, bool bwd) {
     see(a->r, a->r_stride_b, a->r_stride_t);
     see(a->i, a->i_stride_b, a->i_stride_t);
     if (bwd && a->dy) see(a->dy, a->dy_stride_b, a->dy_stride_t);
+    if ((bits & 3) != 0 || (s == 2 && a->dim % 2 != 0)) return kRows2;
     bits |= (int64_t)(bwd ? (uintptr_t)a->dx | (uintptr_t)a->dr | (uintptr_t)a->di : (uintptr_t)a->y);
-    return (bits & 15) == 0 && a->dim % 2 == 0;
+    return (bits & 15) == 0 && a->dim % 2 == 0 ? kRows16 : kRows4;
 }
 
 template <typename F>
@@ -1268,35 +1292,39 @@ bcm_status rec_launch_as(F* kernel, int smem, const bcm_gated_rec_args* a, const
     return BCM_OK;
 }
 
-template <bool BWD, typename T, int MODE, bool EVEN>
+template <bool BWD, typename T, int MODE, int FORM>
 bcm_status rec_launch_p(const bcm_gated_rec_args* a, const RecOut& o, const Plan& pl, cudaStream_t stream) {
     if constexpr (BWD) {
-        constexpr int smem = stages_bwd<T>() * stage_bytes<T, kStepsBwd, EVEN, 4>();
+        constexpr int smem = stages_bwd<T>() * stage_bytes<T, kStepsBwd, FORM, 4>();
         if constexpr (MODE == kGroup)
-            if (pl.serial) return rec_launch_as(rec_bwd_serial<T, EVEN>, smem, a, o, pl, stream);
-        return pl.P > 1 ? rec_launch_as(rec_bwd_kernel<T, MODE, EVEN, true>, smem, a, o, pl, stream)
-                        : rec_launch_as(rec_bwd_kernel<T, MODE, EVEN, false>, smem, a, o, pl, stream);
+            if (pl.serial) return rec_launch_as(rec_bwd_serial<T, FORM>, smem, a, o, pl, stream);
+        return pl.P > 1 ? rec_launch_as(rec_bwd_kernel<T, MODE, FORM, true>, smem, a, o, pl, stream)
+                        : rec_launch_as(rec_bwd_kernel<T, MODE, FORM, false>, smem, a, o, pl, stream);
     } else {
-        constexpr int smem = stages_fwd<T>() * stage_bytes<T, kStepsFwd, EVEN, 3>();
+        constexpr int smem = stages_fwd<T>() * stage_bytes<T, kStepsFwd, FORM, 3>();
         if constexpr (MODE == kGroup)
-            if (pl.serial) return rec_launch_as(rec_fwd_serial<T, EVEN>, smem, a, o, pl, stream);
-        return pl.P > 1 ? rec_launch_as(rec_fwd_kernel<T, MODE, EVEN, true>, smem, a, o, pl, stream)
-                        : rec_launch_as(rec_fwd_kernel<T, MODE, EVEN, false>, smem, a, o, pl, stream);
+            if (pl.serial) return rec_launch_as(rec_fwd_serial<T, FORM>, smem, a, o, pl, stream);
+        return pl.P > 1 ? rec_launch_as(rec_fwd_kernel<T, MODE, FORM, true>, smem, a, o, pl, stream)
+                        : rec_launch_as(rec_fwd_kernel<T, MODE, FORM, false>, smem, a, o, pl, stream);
     }
 }
 
-template <bool BWD, typename T, bool EVEN>
+template <bool BWD, typename T, int FORM>
 bcm_status rec_launch_m(const bcm_gated_rec_args* a, const RecOut& o, const Plan& pl, cudaStream_t stream) {
-    if (pl.mode == kDense) return rec_launch_p<BWD, T, kDense, EVEN>(a, o, pl, stream);
-    if (pl.mode == kGroup) return rec_launch_p<BWD, T, kGroup, EVEN>(a, o, pl, stream);
-    return rec_launch_p<BWD, T, kPacked, EVEN>(a, o, pl, stream);
+    if (pl.mode == kDense) return rec_launch_p<BWD, T, kDense, FORM>(a, o, pl, stream);
+    if (pl.mode == kGroup) return rec_launch_p<BWD, T, kGroup, FORM>(a, o, pl, stream);
+    return rec_launch_p<BWD, T, kPacked, FORM>(a, o, pl, stream);
 }
 
 template <bool BWD>
 bcm_status rec_launch(const bcm_gated_rec_args* a, const RecOut& o, const Plan& pl, cudaStream_t stream) {
     return dispatch_dtype(a->dtype, [&](auto tag) -> bcm_status {
         using T = decltype(tag);
-        return rec_even(a, BWD) ? rec_launch_m<BWD, T, true>(a, o, pl, stream) : rec_launch_m<BWD, T, false>(a, o, pl, stream);
+        const int form = rec_form(a, BWD);
+        if (form == kRows16) return rec_launch_m<BWD, T, kRows16>(a, o, pl, stream);
+        if constexpr (sizeof(T) == 2)
+            if (form == kRows2) return rec_launch_m<BWD, T, kRows2>(a, o, pl, stream);
+        return rec_launch_m<BWD, T, kRows4>(a, o, pl, stream);
     });
 }
 

@@ -18,8 +18,10 @@ namespace {
 // C blocks of a cluster share a row, in 16-byte granules (rows may start anywhere).
 // The forward is one pass with a running maximum and sum; the backward one pass that
 // writes; loss and gradient in one call are both by the same block, the second from
-// L2.  (Keeping rows in a cluster's shared memory in between measured slower, 1545
-// against @@ us at 8192 x 131072 bf16: it leaves fewer warps for the exponentials.)
+// L2 as far as it holds.  (Keeping rows in a cluster's shared memory in between
+// measured slower, 1545 against 1045 us at 8192 x 131072 bf16, and so did clusters of
+// four that leave few enough rows in flight for L2, 1368 us: a block's fixed work -
+// teacher, reductions, the places written again - then recurs for every part.)
 // Granules arrive by cyclic cp.async buffers of each thread's own.  The teacher's
 // entries are one warp's work meanwhile; the K places of the gradient that they
 // touch are written again at the end.
@@ -46,19 +48,24 @@ __device__ __forceinline__ int64_t load_id(const void* ids, int wide, int64_t k)
     return wide ? static_cast<const int64_t*>(ids)[k] : (int64_t) static_cast<const int32_t*>(ids)[k];
 }
 
-// The row's teacher distribution, by one warp: s_id[k] (-1: absent) and s_p[k]; returns the logarithm of the normaliser
-// plus the maximum, -inf for an empty row.
-template <typename TQ>
-__device__ float teacher_row(const TQ* q, const void* ids, int wide, int64_t off, int K, int64_t V, float itau, int* s_id, float* s_p) {
+__host__ __device__ __forceinline__ int list_len(int K) { return (K + 3) / 4 * 4; }
+
+// The row's teacher distribution, by one warp: s_id[k] (-1: absent, up to a multiple of 4), s_p[k] and the student's
+// logit s_z[k]; returns the logarithm of the normaliser plus the maximum, -inf for an empty row.
+template <typename T, typename TQ>
+__device__ float teacher_row(const T* z, const TQ* q, const void* ids, int wide, int64_t off, int K, int64_t V, float itau, int* s_id, float* s_p,
+                             float* s_z) {
     const int lane = threadIdx.x & 31;
     float top = -kInf;
     bool nan = false;
+    if (lane < 4 && K + lane < list_len(K)) s_id[K + lane] = -1;
     for (int k = lane; k < K; k += 32) {
         const int64_t id = load_id(ids, wide, off + k);
         const float v = to_f32<TQ>(q[k]) * itau;
         const bool there = id >= 0 && id < V && v != -kInf;
         s_id[k] = there ? (int)id : -1;
         s_p[k] = v;
+        s_z[k] = there ? to_f32<T>(z[id]) : 0.0f;
         if (there) {
             top = fmaxf(top, v);
             nan |= isnan(v);
@@ -189,8 +196,8 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
     __shared__ float s_lse_q;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = (int)a.k;
     int* s_id = reinterpret_cast<int*>(dyn);
-    float* s_p = reinterpret_cast<float*>(dyn) + K;
-    uint4* ring = reinterpret_cast<uint4*>(dyn + (K * 8 + 15) / 16 * 16);
+    float *s_p = reinterpret_cast<float*>(dyn) + list_len(K), *s_z = s_p + list_len(K);
+    uint4* ring = reinterpret_cast<uint4*>(s_z + list_len(K));
     const int rank = blockIdx.x % C;
     const int64_t t = blockIdx.x / C, V = a.vocab;
     const T* z = static_cast<const T*>(a.logits) + t * a.logits_stride;
@@ -216,7 +223,7 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
         if (FWD) {
             Feed<kThreads> feed(ring, row.at, g0, g1);
             if (warp == 0) {
-                const float l = teacher_row<TQ>(q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p);
+                const float l = teacher_row<T, TQ>(z, q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p, s_z);
                 if (lane == 0) s_lse_q = l;
             }
             feed.run(g0 + tid, [&](int64_t g, uint4 in) {
@@ -262,7 +269,7 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
                 float sum = 0.0f;
                 if (live)
                     for (int k = lane; k < K; k += 32)
-                        if (s_p[k] > 0.0f || isnan(s_p[k])) sum += s_p[k] * (to_f32<TQ>(q[k]) * itau - lse_q - to_f32<T>(z[s_id[k]]) * itau + lse);
+                        if (s_p[k] > 0.0f || isnan(s_p[k])) sum += s_p[k] * (to_f32<TQ>(q[k]) * itau - lse_q - s_z[k] * itau + lse);
                 sum = warp_sum(sum);
                 if (lane == 0) {
                     a.loss[t] = live ? w * tau * tau * sum : 0.0f;
@@ -303,7 +310,7 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
     };
     if (live && alike) {
         Feed<kThreads> feed(ring, row.at, o0, o1);
-        if (!FWD && warp == 0) teacher_row<TQ>(q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p);
+        if (!FWD && warp == 0) teacher_row<T, TQ>(z, q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p, s_z);
         feed.run(o0 + tid, [&](int64_t g, uint4 in) {
             Gr x;
             x.unpack(in);
@@ -311,7 +318,7 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
             put(g, x);
         });
     } else {
-        if (!FWD && live && warp == 0) teacher_row<TQ>(q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p);
+        if (!FWD && live && warp == 0) teacher_row<T, TQ>(z, q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p, s_z);
         for (int64_t g = o0 + tid; g < o1; g += kThreads) {
             const int64_t v0 = g * N - out.shift;
             Gr x;
@@ -330,15 +337,18 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
         if (id < 0 || g < o0 || g >= o1) continue;
         bool first = true;
         float p = s_p[k];
-        for (int j = 0; j < K; ++j)
-            if (j != k && s_id[j] == id) {
-                if (j < k) {
-                    first = false;
-                    break;
+        for (int j = 0; j < K; j += 4) {
+            const int4 at = reinterpret_cast<const int4*>(s_id)[j / 4];
+            if (at.x != id && at.y != id && at.z != id && at.w != id) continue;
+            const int who[4] = {at.x, at.y, at.z, at.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (who[e] == id && j + e != k) {
+                    first = first && j + e > k;
+                    p += s_p[j + e];
                 }
-                p += s_p[j];
-            }
-        if (first) d[id] = from_f32<T>((ex2_((to_f32<T>(z[id]) - soft.m) * c) / soft.s - p) * scale);
+        }
+        if (first) d[id] = from_f32<T>((ex2_((s_z[k] - soft.m) * c) / soft.s - p) * scale);
     }
 }
 
@@ -360,7 +370,7 @@ bcm_status distill_launch_as(F* kernel, const bcm_distill_args* a, int threads, 
     int C = 1;
     while (C < kMaxCluster && a->rows * C < 2 * (int64_t)sm_count() && bytes / C > 8192) C *= 2;
     BCM_REQUIRE(a->rows * C < (1ll << 31), "distill: too many rows");
-    const int smem = (int)(a->k * 8 + 15) / 16 * 16 + kStages * kBatch * threads * 16;
+    const int smem = list_len((int)a->k) * 12 + kStages * kBatch * threads * 16;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a->rows * C));
     cfg.blockDim = dim3((unsigned)threads);

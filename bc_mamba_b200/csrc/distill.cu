@@ -23,8 +23,8 @@ namespace {
 // four that leave few enough rows in flight for L2, 1368 us: a block's fixed work -
 // teacher, reductions, the places written again - then recurs for every part.)
 // Granules arrive by cyclic cp.async buffers of each thread's own.  The teacher's
-// entries are one warp's work meanwhile; the K places of the gradient that they
-// touch are written again at the end.
+// entries and the loss are the work of a warp of their own meanwhile; the K places
+// of the gradient that they touch are written again at the end.
 constexpr int kMaxCluster = 8;
 constexpr int kBatch = 4, kStages = 3;           // granules a thread takes at a time; batches in flight or in use
 constexpr int kShortRow = 24 * 1024;             // bytes of a row up to which a block has 64 threads, not 256
@@ -185,9 +185,9 @@ struct Feed {
 };
 
 template <typename T, typename TQ, bool FWD, bool GRAD, int kThreads>
-__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
+__global__ void __launch_bounds__(kThreads + 32, kThreads == 64 ? 12 : 4)
 distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
-    constexpr int kWarps = kThreads / 32;
+    constexpr int kWarps = kThreads / 32;        // that stream the row; one more is the teacher's
     using Gr = Granule<T>;
     constexpr int N = Gr::N;
     extern __shared__ __align__(16) char dyn[];
@@ -198,6 +198,7 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
     int* s_id = reinterpret_cast<int*>(dyn);
     float *s_p = reinterpret_cast<float*>(dyn) + list_len(K), *s_z = s_p + list_len(K);
     uint4* ring = reinterpret_cast<uint4*>(s_z + list_len(K));
+    const bool teacher = warp == kWarps;
     const int rank = blockIdx.x % C;
     const int64_t t = blockIdx.x / C, V = a.vocab;
     const T* z = static_cast<const T*>(a.logits) + t * a.logits_stride;
@@ -221,35 +222,36 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
     }
     if (live) {
         if (FWD) {
-            Feed<kThreads> feed(ring, row.at, g0, g1);
-            if (warp == 0) {
+            if (teacher) {
                 const float l = teacher_row<T, TQ>(z, q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p, s_z);
                 if (lane == 0) s_lse_q = l;
-            }
-            feed.run(g0 + tid, [&](int64_t g, uint4 in) {
-                Gr x;
-                x.unpack(in);
-                trim(g, x);
-                float top = x.f[0];
+            } else {
+                Feed<kThreads> feed(ring, row.at, g0, g1);
+                feed.run(g0 + tid, [&](int64_t g, uint4 in) {
+                    Gr x;
+                    x.unpack(in);
+                    trim(g, x);
+                    float top = x.f[0];
 #pragma unroll
-                for (int e = 1; e < N; ++e) top = fmaxf(top, x.f[e]);
-                if (top > soft.m) {
-                    if (soft.m != -kInf) soft.s *= ex2_((soft.m - top) * c);
-                    soft.m = top;
+                    for (int e = 1; e < N; ++e) top = fmaxf(top, x.f[e]);
+                    if (top > soft.m) {
+                        if (soft.m != -kInf) soft.s *= ex2_((soft.m - top) * c);
+                        soft.m = top;
+                    }
+                    x.exponentials(soft.m, c);
+#pragma unroll
+                    for (int step = 1; step < N; step <<= 1)
+#pragma unroll
+                        for (int e = 0; e < N; e += 2 * step) x.f[e] += x.f[e + step];
+                    soft.s += x.f[0];
+                });
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1)
+                    soft.join(__shfl_xor_sync(kFull, soft.m, o), __shfl_xor_sync(kFull, soft.s, o), c);
+                if (lane == 0) {
+                    wm[warp] = soft.m;
+                    ws[warp] = soft.s;
                 }
-                x.exponentials(soft.m, c);
-#pragma unroll
-                for (int step = 1; step < N; step <<= 1)
-#pragma unroll
-                    for (int e = 0; e < N; e += 2 * step) x.f[e] += x.f[e + step];
-                soft.s += x.f[0];
-            });
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1)
-                soft.join(__shfl_xor_sync(kFull, soft.m, o), __shfl_xor_sync(kFull, soft.s, o), c);
-            if (lane == 0) {
-                wm[warp] = soft.m;
-                ws[warp] = soft.s;
             }
             __syncthreads();
             soft = {wm[0], ws[0]};
@@ -264,7 +266,7 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
                 for (int k = 1; k < C; ++k) soft.join(parts[k].x, parts[k].y, c);
             }
             live = s_lse_q != -kInf;
-            if (rank == 0 && warp == 0) {
+            if (rank == 0 && teacher) {
                 const float lse = soft.m * itau + logf(soft.s), lse_q = s_lse_q;
                 float sum = 0.0f;
                 if (live)
@@ -309,17 +311,20 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
         }
     };
     if (live && alike) {
-        Feed<kThreads> feed(ring, row.at, o0, o1);
-        if (!FWD && warp == 0) teacher_row<T, TQ>(z, q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p, s_z);
-        feed.run(o0 + tid, [&](int64_t g, uint4 in) {
+        if (teacher) {
+            if (!FWD) teacher_row<T, TQ>(z, q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p, s_z);
+        } else {
+            Feed<kThreads> feed(ring, row.at, o0, o1);
+            feed.run(o0 + tid, [&](int64_t g, uint4 in) {
             Gr x;
             x.unpack(in);
             gradient(x);
             put(g, x);
         });
+        }
     } else {
-        if (!FWD && live && warp == 0) teacher_row<T, TQ>(z, q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p, s_z);
-        for (int64_t g = o0 + tid; g < o1; g += kThreads) {
+        if (!FWD && live && teacher) teacher_row<T, TQ>(z, q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p, s_z);
+        for (int64_t g = o0 + tid; g < o1; g += kThreads + 32) {
             const int64_t v0 = g * N - out.shift;
             Gr x;
 #pragma unroll
@@ -331,7 +336,7 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
     if (!live) return;
     // the teacher's tokens among this block's: the first entry of a token takes its later ones' shares too
     __syncthreads();
-    for (int k = tid; k < K; k += kThreads) {
+    for (int k = tid; k < K; k += kThreads + 32) {
         const int id = s_id[k];
         const int64_t g = ((int64_t)id + out.shift) / N;
         if (id < 0 || g < o0 || g >= o1) continue;
@@ -373,7 +378,7 @@ bcm_status distill_launch_as(F* kernel, const bcm_distill_args* a, int threads, 
     const int smem = list_len((int)a->k) * 12 + kStages * kBatch * threads * 16;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a->rows * C));
-    cfg.blockDim = dim3((unsigned)threads);
+    cfg.blockDim = dim3((unsigned)threads + 32);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];

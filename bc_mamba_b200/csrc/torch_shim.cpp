@@ -1526,6 +1526,81 @@ std::vector<Tensor> sample_tokens(const Tensor& logits, const Tensor& u, double 
     return {tokens, logprob};
 }
 
+// ---- autograd ----
+// C++ functions: the backward runs on the engine's thread without entering Python (forward and backward of a small
+// batch take about half the host time).  The gradients themselves are not differentiable.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+optional<Tensor> given(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : optional<Tensor>(); }
+
+void once(const char* what) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), what, ": the gradient is not differentiable (create_graph)");
+}
+
+struct GatedRecurrence : public torch::autograd::Function<GatedRecurrence> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& lam,
+                                 const optional<Tensor>& h0, const optional<Tensor>& cu_seqlens, double decay_scale, bool keep) {
+        std::vector<Tensor> res = gated_rec_fwd(x, r, i, lam, h0, cu_seqlens, decay_scale, keep);
+        if (keep) {
+            ctx->save_for_backward({x, r, i, lam, h0.value_or(Tensor()), cu_seqlens.value_or(Tensor()), res[2]});
+            ctx->saved_data["decay_scale"] = decay_scale;
+        }
+        ctx->set_materialize_grads(false);   // an output without a gradient reaches the kernel as NULL
+        return {res[0], res[1]};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list out(8);
+        if (!grads[0].defined() && !grads[1].defined()) return out;
+        once("gated_recurrence");
+        const variable_list v = ctx->get_saved_variables();
+        std::vector<Tensor> d = gated_rec_bwd(v[0], v[1], v[2], v[3], given(v[4]), given(v[5]),
+                                              ctx->saved_data["decay_scale"].toDouble(), v[6], given(grads[0]), given(grads[1]));
+        for (int k = 0; k < 4; ++k) out[k] = d[k];
+        if (v[4].defined()) out[4] = d[4];
+        return out;
+    }
+};
+
+struct DistillTopk : public torch::autograd::Function<DistillTopk> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_ids,
+                          const optional<Tensor>& weight, double temperature, bool keep) {
+        std::vector<Tensor> res = distill_fwd(logits, teacher_logits, teacher_ids, weight, temperature, false);
+        if (keep) {
+            ctx->save_for_backward({logits, teacher_logits, teacher_ids, weight.value_or(Tensor()), res[0], res[1]});
+            ctx->saved_data["temperature"] = temperature;
+        }
+        return res[0];
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once("distill_topk");
+        const variable_list v = ctx->get_saved_variables();
+        variable_list out(6);
+        out[0] = distill_bwd(v[0], v[1], v[2], given(v[3]), ctx->saved_data["temperature"].toDouble(), v[4], v[5], grads[0]);
+        return out;
+    }
+};
+
+bool any_grad(std::initializer_list<const Tensor*> all) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : all)
+        if (t->defined() && t->requires_grad()) return true;
+    return false;
+}
+
+std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& lam,
+                                            const optional<Tensor>& h0, const optional<Tensor>& cu_seqlens, double decay_scale) {
+    const Tensor h = h0.value_or(Tensor());
+    variable_list out = GatedRecurrence::apply(x, r, i, lam, h0, cu_seqlens, decay_scale, any_grad({&x, &r, &i, &lam, &h}));
+    return {out[0], out[1]};
+}
+
+Tensor distill_topk(const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_ids, const optional<Tensor>& weight,
+                    double temperature) {
+    const optional<Tensor> w = weight.has_value() ? optional<Tensor>(weight->detach()) : optional<Tensor>();
+    return DistillTopk::apply(logits, teacher_logits.detach(), teacher_ids, w, temperature, any_grad({&logits}));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1626,6 +1701,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("gated_rec_bwd", &gated_rec_bwd, py::arg("x"), py::arg("r"), py::arg("i"), py::arg("lam"), py::arg("h0"),
           py::arg("cu_seqlens"), py::arg("decay_scale"), py::arg("ckpt"), py::arg("dy"), py::arg("dh_last"),
           "Backward of gated_rec_fwd (dy or dh_last None: zero) -> [dx, dr, di, dlam, dh0]");
+    m.def("gated_recurrence", &gated_recurrence, py::arg("x"), py::arg("r"), py::arg("i"), py::arg("lam"),
+          py::arg("h0") = py::none(), py::arg("cu_seqlens") = py::none(), py::arg("decay_scale") = 8.0,
+          "gated_rec_fwd with autograd in x, r, i, lam and h0 -> (y, h_last)");
+    m.def("distill_topk", &distill_topk, py::arg("logits"), py::arg("teacher_logits"), py::arg("teacher_ids"),
+          py::arg("weight") = py::none(), py::arg("temperature") = 1.0, "distill_fwd with autograd in logits -> loss (T)");
     m.def("gated_rec_step", &gated_rec_step, py::arg("x"), py::arg("r"), py::arg("i"), py::arg("lam"), py::arg("h"),
           py::arg("decay_scale") = 8.0, "One token of every sequence; the state h (B, D) is updated in place -> y (B, D)");
     m.def("distill_fwd", &distill_fwd, py::arg("logits"), py::arg("teacher_logits"), py::arg("teacher_ids"),

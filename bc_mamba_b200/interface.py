@@ -424,32 +424,8 @@ class EventDecoder:
 
 # ------------------------------------------------ language-model operators ----
 # (no counterpart in the reference: a sequence mixer, a training loss and a
-# token sampler for models built on this package's scans)
-
-
-class GatedRecurrenceFn(torch.autograd.Function):
-    """Gated linear recurrence; see gated_recurrence."""
-
-    @staticmethod
-    def forward(ctx, x, r, i, lam, h0, cu_seqlens, decay_scale):
-        keep = any(ctx.needs_input_grad[:5])
-        with cuda_stage("gated_recurrence_forward"):
-            res = load_ops().gated_rec_fwd(x, r, i, lam, h0, cu_seqlens, decay_scale, keep)
-        if keep:
-            ctx.save_for_backward(x, r, i, lam, h0, cu_seqlens, res[2])
-            ctx.decay_scale = decay_scale
-        ctx.set_materialize_grads(False)   # an output without a gradient reaches the kernel as NULL
-        return res[0], res[1]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, dh_last):
-        if dy is None and dh_last is None:
-            return (None,) * 7
-        x, r, i, lam, h0, cu_seqlens, ckpt = ctx.saved_tensors
-        with cuda_stage("gated_recurrence_backward"):
-            dx, dr, di, dlam, dh0 = load_ops().gated_rec_bwd(x, r, i, lam, h0, cu_seqlens, ctx.decay_scale, ckpt, dy, dh_last)
-        return dx, dr, di, dlam, dh0 if h0 is not None else None, None, None
+# token sampler for models built on this package's scans; their autograd
+# functions are C++, in the shim, and their gradients not differentiable)
 
 
 def gated_recurrence(x, r, i, lam, h0=None, cu_seqlens=None, decay_scale: float = 8.0):
@@ -464,34 +440,14 @@ def gated_recurrence(x, r, i, lam, h0=None, cu_seqlens=None, decay_scale: float 
     sequence's last token, which continue it as h0 of a next call or as the
     state of gated_recurrence_step.  Differentiable in x, r, i, lam and h0; the
     state is float32 throughout and gradients are the same from run to run."""
-    return GatedRecurrenceFn.apply(x, r, i, lam, h0, cu_seqlens, float(decay_scale))
+    with cuda_stage("gated_recurrence_forward"):
+        return load_ops().gated_recurrence(x, r, i, lam, h0, cu_seqlens, decay_scale)
 
 
 def gated_recurrence_step(x, r, i, lam, h, decay_scale: float = 8.0):
     """One token of gated_recurrence for every sequence: x, r, i (B, D), the
     state h (B, D) float32 contiguous, updated in place.  Returns y (B, D)."""
     return load_ops().gated_rec_step(x, r, i, lam, h, decay_scale)
-
-
-class DistillTopkFn(torch.autograd.Function):
-    """Distillation loss on a teacher's top logits; see distill_topk."""
-
-    @staticmethod
-    def forward(ctx, logits, teacher_logits, teacher_ids, weight, temperature):
-        with cuda_stage("distill_forward"):
-            loss, stats = load_ops().distill_fwd(logits, teacher_logits, teacher_ids, weight, temperature)
-        if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(logits, teacher_logits, teacher_ids, weight, loss, stats)
-            ctx.temperature = temperature
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dloss):
-        logits, teacher_logits, teacher_ids, weight, loss, stats = ctx.saved_tensors
-        with cuda_stage("distill_backward"):
-            dz = load_ops().distill_bwd(logits, teacher_logits, teacher_ids, weight, ctx.temperature, loss, stats, dloss)
-        return dz, None, None, None, None
 
 
 def distill_topk(logits, teacher_logits, teacher_ids, weight=None, temperature: float = 1.0):
@@ -503,7 +459,8 @@ def distill_topk(logits, teacher_logits, teacher_ids, weight=None, temperature: 
     early); a row without entries, or of weight 0, has loss and gradient 0
     whatever its logits hold.  weight (T,) float32.  Differentiable in logits.
     Returns the losses (T,) float32."""
-    return DistillTopkFn.apply(logits, teacher_logits, teacher_ids, weight, float(temperature))
+    with cuda_stage("distill_forward"):
+        return load_ops().distill_topk(logits, teacher_logits, teacher_ids, weight, temperature)
 
 
 def distill_topk_with_grad(logits, teacher_logits, teacher_ids, weight=None, temperature: float = 1.0):
@@ -512,7 +469,7 @@ def distill_topk_with_grad(logits, teacher_logits, teacher_ids, weight=None, tem
     scale, into weight).  It reads the logits from memory once where the
     autograd pair reads them twice."""
     with torch.no_grad(), cuda_stage("distill_forward"):
-        loss, _, dz = load_ops().distill_fwd(logits, teacher_logits, teacher_ids, weight, float(temperature), True)
+        loss, _, dz = load_ops().distill_fwd(logits, teacher_logits, teacher_ids, weight, temperature, True)
     return loss, dz
 
 

@@ -196,3 +196,10 @@ def test_refusals():
         for f in (itf.distill_topk, itf.distill_topk_with_grad):
             with pytest.raises(RuntimeError, match=match):
                 f(**{**ok, **bad})
+
+
+def test_second_derivatives_are_refused():
+    z, q, ids, w, up = _inputs(2, 50, 3, torch.float32, seed=11)
+    z.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(itf.distill_topk(z, q, ids).sum(), z, create_graph=True)

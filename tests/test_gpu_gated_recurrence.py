@@ -347,3 +347,21 @@ def test_refusals():
     for bad, match in [(dict(h=h.half()), "h must be"), (dict(h=h[:1]), "h has the wrong shape"), (dict(x=x), "\\(B, D\\)")]:
         with pytest.raises(RuntimeError, match=match):
             itf.gated_recurrence_step(**{**dict(x=x[:, 0], r=x[:, 0], i=x[:, 0], lam=lam, h=h), **bad})
+
+
+def test_second_derivatives_are_refused_and_unused_outputs_cost_nothing():
+    x = torch.randn(1, 5, 4, device=dev, requires_grad=True)
+    lam = torch.zeros(4, device=dev)
+    y, h = itf.gated_recurrence(x, x.detach(), x.detach(), lam)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+    y, h = itf.gated_recurrence(x, x.detach(), x.detach(), lam)
+    g, = torch.autograd.grad(h.sum(), x)                   # y takes no part
+    assert torch.isfinite(g).all() and not itf.gated_recurrence(x.detach(), x.detach(), x.detach(), lam)[0].requires_grad
+    with torch.no_grad():
+        assert not itf.gated_recurrence(x, x, x, lam)[0].requires_grad
+    z = torch.randn(1, 5, 4, device=dev, requires_grad=True)
+    y, _ = itf.gated_recurrence(z * 1, x.detach(), x.detach(), lam)
+    w = y.detach()
+    y.sum().backward()
+    assert z.grad is not None and w.shape == y.shape

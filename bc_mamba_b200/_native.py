@@ -55,6 +55,7 @@ ABI_SYMBOLS = (
     "bcm_event_params_fwd",
     "bcm_event_params_bwd",
     "bcm_gated_rec_ckpt_bytes",
+    "bcm_gated_rec_fwd_workspace_bytes",
     "bcm_gated_rec_bwd_workspace_bytes",
     "bcm_gated_rec_fwd",
     "bcm_gated_rec_bwd",

@@ -122,6 +122,11 @@ __device__ __forceinline__ Gates gates(float2 r, float2 i, float2 cs, const Cons
 // chunk empty); kPacked, the sequences' offsets stand in cu, and run g of G takes
 // the sequences that start in the g-th part of the tokens (found on the device).
 // Where a sequence starts inside a run, nothing passes and its own state enters.
+//
+// Few features with long sequences: a sequence (kDense) or the whole packed run is
+// cut into segments of fixed length.  A first launch (SUM) only composes every
+// segment, a small kernel carries the state over them, and the second launch starts
+// each segment from its own.
 constexpr int kWarps = 8;
 constexpr int kTile = 64;                        // features of a block
 constexpr int kStepsFwd = 8, kStepsBwd = 4;      // tokens of a warp's turn (the backward keeps 7 values a token)
@@ -139,6 +144,7 @@ struct RecPtr {
 struct RecOut {
     const float* h0; void* y; float* h_last; float* ckpt;                          // forward
     const float* dh_last; void* dx; void* dr; void* di; float* part; float* dh0;   // backward
+    const float* seg; float* sum;                  // segments: what enters each of them; their compositions [2] (SUM)
 };
 
 // A run holds L tokens (kGroup: its last may hold fewer; kPacked: all runs together), a sequence Ls (kDense, kGroup),
@@ -147,6 +153,7 @@ struct RecDim {
     const int32_t* cu;
     int64_t n;
     int L, Ls, per, runs, D, P;
+    int segs, seg;            // segments of a sequence (1: none) and their length
 };
 
 // The sequence that holds token t: the last s with cu[s] <= t, in [0, n).  Called by whole warps; t is uniform.
@@ -222,7 +229,7 @@ __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0
 // Where a block works.
 struct Place {
     int lane, warp, rank, tile, d, L;
-    int off;                  // the run's first token (kPacked)
+    int off;                  // the run's first token (kPacked, segments)
     int64_t run, b;           // the run and its first sequence (kDense, kGroup)
     bool has0, has1;          // the lane's features exist
 };
@@ -236,8 +243,12 @@ __device__ __forceinline__ Place place(const RecDim& n, const int32_t* cu) {
     q.rank = CLUSTER ? blockIdx.x % P : 0;
     q.run = blockIdx.x / P / tiles;
     q.tile = (int)(blockIdx.x / P - q.run * tiles);
-    q.b = MODE == kGroup ? q.run * n.per : q.run;
+    q.b = MODE == kGroup ? q.run * n.per : q.run / n.segs;
     q.L = MODE == kGroup ? (int)min((int64_t)n.per, n.n - q.b) * n.Ls : n.L;
+    if (MODE != kGroup && n.segs > 1) {
+        q.off = (int)min((q.run - q.b * n.segs) * n.seg, (int64_t)n.L);
+        q.L = min(n.L - q.off, n.seg);
+    }
     q.d = q.tile * kTile + q.lane * 2;
     q.has0 = q.d < n.D;
     q.has1 = q.d + 1 < n.D;
@@ -309,7 +320,7 @@ struct Stream {
         return k * in.sb + (int64_t)(t - k * n.Ls) * in.st;
     }
     __device__ __forceinline__ static const T* base(const Input& in, const Place& w) {
-        return static_cast<const T*>(in.p) + (MODE == kPacked ? w.off * in.st : w.b * in.sb) + (int64_t)w.tile * kTile;
+        return static_cast<const T*>(in.p) + (MODE == kPacked ? 0 : w.b * in.sb) + w.off * in.st + (int64_t)w.tile * kTile;
     }
     __device__ __forceinline__ Stream(const Input& in, const Place& w, int t0, int width) {
         bytes = max(0, min(16, width * (int)sizeof(T) - w.lane % R::kGran * 16));
@@ -425,7 +436,7 @@ __device__ __forceinline__ void store_state(float* p, int64_t row, int D, int d,
 // The run's first row of kept states.
 template <int MODE>
 __device__ __forceinline__ int64_t ckpt_row(const Place& w, const RecDim& n) {
-    return MODE == kPacked ? w.off / kCkpt + w.run : w.run * ((n.L + kCkpt - 1) / kCkpt);
+    return MODE == kPacked ? w.off / kCkpt + w.run : (MODE == kDense ? w.b : w.run) * ((n.L + kCkpt - 1) / kCkpt) + w.off / kCkpt;
 }
 
 // Bit j: a sequence starts at token t0 + j.
@@ -466,7 +477,7 @@ struct Pub {
     float4 v[CLUSTER ? 2 : 1][CLUSTER ? kMaxCluster : 1][CLUSTER ? 32 : 1];
 };
 
-template <typename T, int MODE, int FORM, bool CLUSTER>
+template <typename T, int MODE, int FORM, bool CLUSTER, bool SUM>
 __global__ void __launch_bounds__(kWarps * 32, 2)
 rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut o, const __grid_constant__ RecDim n,
                const float* __restrict__ lam, float c) {
@@ -481,9 +492,9 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
     const int32_t* cu = stage_cu<MODE>(n, cus);
     const Place w = place<MODE, CLUSTER>(n, cu);
     const int D = n.D, L = w.L, P = CLUSTER ? n.P : 1, width = min(kTile, D - w.tile * kTile);
-    T* y = static_cast<T*>(o.y) + (MODE == kPacked ? (int64_t)w.off : w.b * n.Ls) * D + w.d;
+    T* y = static_cast<T*>(o.y) + ((MODE == kPacked ? 0 : w.b * n.Ls) + w.off) * D + w.d;
     const bool even_rows = (D & 1) == 0 && (uintptr_t)o.y % (2 * sizeof(T)) == 0;
-    const int turns = (((MODE == kPacked ? L : n.L) + kChunk - 1) / kChunk + P - 1) / P;
+    const int turns = (((MODE == kGroup ? n.L : L) + kChunk - 1) / kChunk + P - 1) / P;
     float* ck = o.ckpt ? o.ckpt + ckpt_row<MODE>(w, n) * D : nullptr;
     const float2 l = load_state(lam, 0, D, w.d, w.has0, w.has1);
     const float2 cs = make_float2(w.has0 ? c * softplus_(l.x) : kPolyEnd, w.has1 ? c * softplus_(l.y) : kPolyEnd);
@@ -506,7 +517,8 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
 #pragma unroll
     for (int k = 0; k < ST - 1; ++k) fetch(k);
     Seq<MODE> seq{cu, (int)n.n, n.Ls, w.off, w.b, 0, 0, 0};
-    float2 run = MODE == kDense ? load_state(o.h0, w.b, D, w.d, w.has0, w.has1) : f2(0.0f);
+    float2 run = MODE == kDense && !SUM ? load_state(o.h0, w.b, D, w.d, w.has0, w.has1) : f2(0.0f), runA = f2(1.0f);
+    if (!SUM && o.seg) run = load_state(o.seg, w.run, D, w.d, w.has0, w.has1);
 
     // gates and composition of a turn: h -> a_j h + e_j token by token, h -> A h + H together
     auto prepare = [&](int turn, float2 (&a)[S], float2 (&e)[S], unsigned& starts) {
@@ -639,15 +651,29 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
             publish(turn, preA, preH);
             cluster_arrive();
             cluster_wait();
+            if constexpr (SUM) {
+                for (int k = 0; k < P; ++k) {
+                    const float4 f = pub.v[turn & 1][k][w.lane];
+                    then<CUTS>(runA, run, make_float2(f.x, f.y), make_float2(f.z, f.w));
+                }
+                continue;
+            }
             h = apply<CUTS>(preA, preH, enter(pub.v[turn & 1], P, w.rank));
         } else {
             h = enter(ex[turn & 1], kWarps, w.warp);
         }
         replay(turn, a, e, starts, h);
     }
+    if (SUM) {
+        if (w.rank == 0 && w.warp == 0) {
+            store_state(o.sum, w.run * 2, D, w.d, runA, w.has0, w.has1);
+            store_state(o.sum, w.run * 2 + 1, D, w.d, run, w.has0, w.has1);
+        }
+        return;
+    }
     if (w.rank != 0 || (MODE == kPacked && w.run != 0)) return;
     if (MODE == kDense) {
-        if (w.warp == 0) store_state(o.h_last, w.b, D, w.d, run, w.has0, w.has1);
+        if (w.warp == 0 && L > 0 && w.off + L == n.L) store_state(o.h_last, w.b, D, w.d, run, w.has0, w.has1);
     } else if (MODE == kPacked) {
         for (int64_t s = w.warp; s < n.n; s += kWarps)       // empty sequences keep their state
             if (seq.cu[s] >= seq.cu[s + 1])
@@ -658,7 +684,7 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
 // Chunks from the last to the first.  The states that enter a chunk come from
 // the forward; back_t = a_t G_t passes from right to left by the same products
 // of decays, back -> A back + K.
-template <typename T, int MODE, int FORM, bool CLUSTER>
+template <typename T, int MODE, int FORM, bool CLUSTER, bool SUM>
 __global__ void __launch_bounds__(kWarps * 32, 2)
 rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut o, const __grid_constant__ RecDim n,
                const float* __restrict__ lam, float c) {
@@ -674,9 +700,9 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
     const int32_t* cu = stage_cu<MODE>(n, cus);
     const Place w = place<MODE, CLUSTER>(n, cu);
     const int D = n.D, L = w.L, P = CLUSTER ? n.P : 1, width = min(kTile, D - w.tile * kTile);
-    const int64_t base = (MODE == kPacked ? (int64_t)w.off : w.b * n.Ls) * D + w.d;
+    const int64_t base = ((MODE == kPacked ? 0 : w.b * n.Ls) + w.off) * D + w.d;
     const bool even_rows = (D & 1) == 0 && ((uintptr_t)o.dx | (uintptr_t)o.dr | (uintptr_t)o.di) % (2 * sizeof(T)) == 0;
-    const int turns = (((MODE == kPacked ? L : n.L) + kChunk - 1) / kChunk + P - 1) / P;
+    const int turns = (((MODE == kGroup ? n.L : L) + kChunk - 1) / kChunk + P - 1) / P;
     const float* ck = o.ckpt + ckpt_row<MODE>(w, n) * D;
     const float2 l = load_state(lam, 0, D, w.d, w.has0, w.has1);
     const float2 cs = make_float2(w.has0 ? c * softplus_(l.x) : kPolyEnd, w.has1 ? c * softplus_(l.y) : kPolyEnd);
@@ -703,14 +729,15 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
     for (int k = 1; k <= kAhead; ++k) fetch(turns - k);
     Seq<MODE> seq{cu, (int)n.n, n.Ls, w.off, w.b, 0, 0, 0};
     if (L > 0) seq.at(L - 1);
-    float2 run = load_state(o.dh_last, CUTS ? seq.s : w.b, D, w.d, w.has0, w.has1), sum = f2(0.0f);
+    float2 run = load_state(SUM ? nullptr : o.dh_last, CUTS ? seq.s : w.b, D, w.d, w.has0, w.has1), sum = f2(0.0f), runA = f2(1.0f);
+    if (!SUM && o.seg) run = load_state(o.seg, w.run, D, w.d, w.has0, w.has1);
     auto state0 = [&](int t) -> float2 {          // the state that enters the sequence of token t
         Seq<MODE> q = seq;
         q.at(t);
         return load_state(o.h0, q.s, D, w.d, w.has0, w.has1);
     };
     auto back0 = [&](int t) -> float2 {           // what enters, from the right, the sequence of token t
-        if (t < 0) return f2(0.0f);
+        if (t + w.off < 0) return f2(0.0f);
         Seq<MODE> q = seq;
         q.at(t);
         return load_state(o.dh_last, q.s, D, w.d, w.has0, w.has1);
@@ -872,11 +899,25 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
             publish(turn, q);
             cluster_arrive();
             cluster_wait();
+            if constexpr (SUM) {
+                for (int k = P - 1; k >= 0; --k) {
+                    const float4 f = pub.v[turn & 1][k][w.lane];
+                    then<CUTS>(runA, run, make_float2(f.x, f.y), make_float2(f.z, f.w));
+                }
+                continue;
+            }
             q.back = apply<CUTS>(q.sufA, q.sufK, enter(pub.v[turn & 1], P, w.rank));
         } else {
             q.back = enter(ex[turn & 1], kWarps, w.warp);
         }
         replay(turn, q);
+    }
+    if (SUM) {
+        if (w.rank == 0 && w.warp == 0) {
+            store_state(o.sum, w.run * 2, D, w.d, runA, w.has0, w.has1);
+            store_state(o.sum, w.run * 2 + 1, D, w.d, run, w.has0, w.has1);
+        }
+        return;
     }
     __syncthreads();
     exh[0][w.warp][w.lane] = sum;
@@ -888,7 +929,7 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
     }
     if (w.rank != 0 || !o.dh0 || (MODE == kPacked && w.run != 0)) return;
     if (MODE == kDense) {
-        if (w.warp == 0) store_state(o.dh0, w.b, D, w.d, run, w.has0, w.has1);
+        if (w.warp == 0 && w.off == 0) store_state(o.dh0, w.b, D, w.d, run, w.has0, w.has1);
     } else if (MODE == kPacked) {
         for (int64_t s = w.warp; s < n.n; s += kWarps)
             if (seq.cu[s] >= seq.cu[s + 1])
@@ -1125,6 +1166,32 @@ rec_bwd_serial(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
     store_state(o.part, w.run, D, w.d, sum, w.has0, w.has1);
 }
 
+// What enters every segment of a sequence (blockIdx.y; packed: of all), from the first on or (REVERSE) from the last on.
+template <bool REVERSE>
+__global__ void rec_join_kernel(const float* __restrict__ sum, const float* __restrict__ init, RecDim n, float* __restrict__ state) {
+    const int d = blockIdx.x * blockDim.x + threadIdx.x;
+    if (d >= n.D) return;
+    const int64_t first = (int64_t)blockIdx.y * n.segs;
+    float h = 0.0f;
+    if (n.cu == nullptr) {
+        if (init) h = init[(int64_t)blockIdx.y * n.D + d];
+    } else if (REVERSE && init) {                 // the last token's sequence
+        int64_t lo = 0, hi = n.n - 1;
+        while (lo < hi) {
+            const int64_t mid = (lo + hi + 1) / 2;
+            if (n.cu[mid] <= n.L - 1) lo = mid;
+            else hi = mid - 1;
+        }
+        h = init[lo * n.D + d];
+    }
+    for (int k = 0; k < n.segs; ++k) {
+        const int64_t run = first + (REVERSE ? n.segs - 1 - k : k);
+        state[run * n.D + d] = h;
+        const float A = sum[run * 2 * n.D + d], H = sum[(run * 2 + 1) * n.D + d];
+        h = A < 0.0f ? H : fmaf(A, h, H);
+    }
+}
+
 // dlam[d] = -c sigmoid(lam[d]) * sum of the n partials of feature d: a block takes
 // 32 features, a warp every 32nd partial, then the warps' sums in order.
 __global__ void __launch_bounds__(1024)
@@ -1218,11 +1285,12 @@ struct Plan {
     int mode, per, L, P;
     int64_t runs, tiles;
     bool serial;
+    int segs, seg;
 };
 
 Plan rec_plan(const bcm_gated_rec_args* a) {
     constexpr int kChunk = kWarps * kStepsFwd;
-    Plan pl = {kDense, 1, (int)a->seqlen, 1, a->batch, rec_parts(a->dim, kTile), false};
+    Plan pl = {kDense, 1, (int)a->seqlen, 1, a->batch, rec_parts(a->dim, kTile), false, 1, 0};
     if (a->cu_seqlens) {
         // Runs need no exchange, but a long sequence leaves them uneven: one for every four sequences at most, and no
         // more than two blocks per SM take; clusters fill the rest.
@@ -1251,6 +1319,14 @@ Plan rec_plan(const bcm_gated_rec_args* a) {
     }
     // blocks of a cluster: as many as the chunks allow and two blocks per SM hold at once
     while (pl.P < kMaxCluster && pl.runs * pl.tiles * pl.P <= (int64_t)sm_count() && 2 * pl.P <= rec_parts(pl.mode == kPacked ? pl.L / pl.runs : pl.L, kChunk)) pl.P *= 2;
+    // Segments where full clusters still leave most of the GPU empty: they take their tokens twice, so three at least,
+    // of four turns or more.
+    const int64_t room = 2 * (int64_t)sm_count() / (pl.runs * pl.tiles * pl.P), turns = rec_parts(pl.L, kChunk * kMaxCluster);
+    if (pl.P == kMaxCluster && pl.mode != kGroup && (pl.mode == kDense || pl.runs == 1) && std::min(room, turns / 4) >= 3) {
+        pl.seg = (int)rec_parts(rec_parts(pl.L, (int)std::min(room, turns / 4)), kChunk) * kChunk;
+        pl.segs = (int)rec_parts(pl.L, pl.seg);
+        pl.runs *= pl.segs;
+    }
     return pl;
 }
 
@@ -1270,6 +1346,10 @@ int rec_form(const bcm_gated_rec_args* a, bool bwd) {
     return (bits & 15) == 0 && a->dim % 2 == 0 ? kRows16 : kRows4;
 }
 
+RecDim rec_dim(const bcm_gated_rec_args* a, const Plan& pl) {
+    return {a->cu_seqlens, a->batch, pl.L, (int)a->seqlen, pl.per, pl.segs > 1 ? 1 : (int)pl.runs, (int)a->dim, pl.P, pl.segs, pl.seg};
+}
+
 template <typename F>
 bcm_status rec_launch_as(F* kernel, int smem, const bcm_gated_rec_args* a, const RecOut& o, const Plan& pl, cudaStream_t stream) {
     const int64_t blocks = pl.serial ? rec_parts(pl.tiles * pl.runs, kWarps) : pl.tiles * pl.runs * pl.P;
@@ -1287,7 +1367,7 @@ bcm_status rec_launch_as(F* kernel, int smem, const bcm_gated_rec_args* a, const
     cfg.attrs = attr;
     cfg.numAttrs = pl.P > 1 ? 1 : 0;
     BCM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    const RecDim n = {a->cu_seqlens, a->batch, pl.L, (int)a->seqlen, pl.per, (int)pl.runs, (int)a->dim, pl.P};
+    const RecDim n = rec_dim(a, pl);
     BCM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, rec_ptr(a), o, n, a->lam, a->decay_scale));
     return BCM_OK;
 }
@@ -1298,14 +1378,18 @@ bcm_status rec_launch_p(const bcm_gated_rec_args* a, const RecOut& o, const Plan
         constexpr int smem = stages_bwd<T>() * stage_bytes<T, kStepsBwd, FORM, 4>();
         if constexpr (MODE == kGroup)
             if (pl.serial) return rec_launch_as(rec_bwd_serial<T, FORM>, smem, a, o, pl, stream);
-        return pl.P > 1 ? rec_launch_as(rec_bwd_kernel<T, MODE, FORM, true>, smem, a, o, pl, stream)
-                        : rec_launch_as(rec_bwd_kernel<T, MODE, FORM, false>, smem, a, o, pl, stream);
+        if constexpr (MODE != kGroup)
+            if (o.sum) return rec_launch_as(rec_bwd_kernel<T, MODE, FORM, true, true>, smem, a, o, pl, stream);
+        return pl.P > 1 ? rec_launch_as(rec_bwd_kernel<T, MODE, FORM, true, false>, smem, a, o, pl, stream)
+                        : rec_launch_as(rec_bwd_kernel<T, MODE, FORM, false, false>, smem, a, o, pl, stream);
     } else {
         constexpr int smem = stages_fwd<T>() * stage_bytes<T, kStepsFwd, FORM, 3>();
         if constexpr (MODE == kGroup)
             if (pl.serial) return rec_launch_as(rec_fwd_serial<T, FORM>, smem, a, o, pl, stream);
-        return pl.P > 1 ? rec_launch_as(rec_fwd_kernel<T, MODE, FORM, true>, smem, a, o, pl, stream)
-                        : rec_launch_as(rec_fwd_kernel<T, MODE, FORM, false>, smem, a, o, pl, stream);
+        if constexpr (MODE != kGroup)
+            if (o.sum) return rec_launch_as(rec_fwd_kernel<T, MODE, FORM, true, true>, smem, a, o, pl, stream);
+        return pl.P > 1 ? rec_launch_as(rec_fwd_kernel<T, MODE, FORM, true, false>, smem, a, o, pl, stream)
+                        : rec_launch_as(rec_fwd_kernel<T, MODE, FORM, false, false>, smem, a, o, pl, stream);
     }
 }
 
@@ -1317,7 +1401,7 @@ bcm_status rec_launch_m(const bcm_gated_rec_args* a, const RecOut& o, const Plan
 }
 
 template <bool BWD>
-bcm_status rec_launch(const bcm_gated_rec_args* a, const RecOut& o, const Plan& pl, cudaStream_t stream) {
+bcm_status rec_launch_form(const bcm_gated_rec_args* a, const RecOut& o, const Plan& pl, cudaStream_t stream) {
     return dispatch_dtype(a->dtype, [&](auto tag) -> bcm_status {
         using T = decltype(tag);
         const int form = rec_form(a, BWD);
@@ -1326,6 +1410,22 @@ bcm_status rec_launch(const bcm_gated_rec_args* a, const RecOut& o, const Plan& 
             if (form == kRows2) return rec_launch_m<BWD, T, kRows2>(a, o, pl, stream);
         return rec_launch_m<BWD, T, kRows4>(a, o, pl, stream);
     });
+}
+
+template <bool BWD>
+bcm_status rec_launch(const bcm_gated_rec_args* a, const RecOut& o, const Plan& pl, cudaStream_t stream) {
+    if (pl.segs > 1 && o.sum) {                   // compose the segments, join them, then start each from its own state
+        if (bcm_status st = rec_launch_form<BWD>(a, o, pl, stream); st != BCM_OK) return st;
+        float* state = o.sum + 2 * pl.runs * a->dim;
+        const dim3 grid((unsigned)ceil_div(a->dim, 64), (unsigned)(pl.runs / pl.segs));
+        rec_join_kernel<BWD><<<grid, 64, 0, stream>>>(o.sum, BWD ? a->dh_last : a->h0, rec_dim(a, pl), state);
+        BCM_LAUNCH_CHECK();
+        RecOut next = o;
+        next.sum = nullptr;
+        next.seg = state;
+        return rec_launch_form<BWD>(a, next, pl, stream);
+    }
+    return rec_launch_form<BWD>(a, o, pl, stream);
 }
 
 }  // namespace
@@ -1337,15 +1437,23 @@ extern "C" size_t bcm_gated_rec_ckpt_bytes(const bcm_gated_rec_args* a) {
     if (!a || a->batch < 0 || a->seqlen < 0 || a->dim < 1) return 0;
     if (rec_rows(a) == 0) return 0;
     const Plan pl = rec_plan(a);
-    const int64_t states = pl.mode == kPacked ? rec_parts(pl.L, kCkpt) + pl.runs + 1 : pl.runs * rec_parts(pl.L, pl.serial ? kCkptSerial : kCkpt);
+    const int64_t states = pl.mode == kPacked ? rec_parts(pl.L, kCkpt) + pl.runs + 1 : pl.runs / pl.segs * rec_parts(pl.L, pl.serial ? kCkptSerial : kCkpt);
     return align_up((size_t)states * (size_t)a->dim * sizeof(float), 256);
 }
 
+static size_t rec_segment_bytes(const bcm_gated_rec_args* a, const Plan& pl) {
+    return pl.segs > 1 ? align_up((size_t)pl.runs * (size_t)a->dim * 3 * sizeof(float), 256) : 0;
+}
+
+extern "C" size_t bcm_gated_rec_fwd_workspace_bytes(const bcm_gated_rec_args* a) {
+    if (!a || a->batch < 0 || a->seqlen < 0 || a->dim < 1 || rec_rows(a) == 0) return 0;
+    return rec_segment_bytes(a, rec_plan(a));
+}
+
 extern "C" size_t bcm_gated_rec_bwd_workspace_bytes(const bcm_gated_rec_args* a) {
-    if (!a || a->batch < 0 || a->seqlen < 0 || a->dim < 1) return 0;
-    if (rec_rows(a) == 0) return 0;
+    if (!a || a->batch < 0 || a->seqlen < 0 || a->dim < 1 || rec_rows(a) == 0) return 0;
     const Plan pl = rec_plan(a);
-    return align_up((size_t)pl.runs * (size_t)pl.P * (size_t)a->dim * sizeof(float), 256);
+    return align_up((size_t)pl.runs * (size_t)pl.P * (size_t)a->dim * sizeof(float), 256) + rec_segment_bytes(a, pl);
 }
 
 extern "C" bcm_status bcm_gated_rec_fwd(const bcm_gated_rec_args* a, cudaStream_t stream) {
@@ -1365,7 +1473,15 @@ extern "C" bcm_status bcm_gated_rec_fwd(const bcm_gated_rec_args* a, cudaStream_
     }
     RecOut o = {};
     o.h0 = a->h0; o.y = a->y; o.h_last = a->h_last; o.ckpt = static_cast<float*>(a->ckpt);
-    return rec_launch<false>(a, o, rec_plan(a), stream);
+    const Plan pl = rec_plan(a);
+    if (pl.segs > 1) {
+        if (!a->workspace || a->workspace_bytes < rec_segment_bytes(a, pl)) {
+            set_error("gated_rec_fwd: workspace of %zu bytes < required %zu", a->workspace_bytes, rec_segment_bytes(a, pl));
+            return BCM_ERR_WORKSPACE;
+        }
+        o.sum = static_cast<float*>(a->workspace);
+    }
+    return rec_launch<false>(a, o, pl, stream);
 }
 
 extern "C" bcm_status bcm_gated_rec_bwd(const bcm_gated_rec_args* a, cudaStream_t stream) {
@@ -1391,6 +1507,7 @@ extern "C" bcm_status bcm_gated_rec_bwd(const bcm_gated_rec_args* a, cudaStream_
     o.dh_last = a->dh_last; o.dx = a->dx; o.dr = a->dr; o.di = a->di;
     o.part = static_cast<float*>(a->workspace); o.dh0 = a->dh0;
     const Plan pl = rec_plan(a);
+    if (pl.segs > 1) o.sum = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + need - rec_segment_bytes(a, pl));
     if (bcm_status st = rec_launch<true>(a, o, pl, stream); st != BCM_OK) return st;
     rec_dlam_kernel<<<(unsigned)ceil_div(a->dim, 32), 1024, 0, stream>>>(o.part, pl.runs * pl.P, a->dim, a->lam, a->decay_scale,
                                                                         a->dlam);

@@ -1366,6 +1366,11 @@ std::vector<Tensor> gated_rec_fwd(const Tensor& x, const Tensor& r, const Tensor
         a.ckpt_bytes = (size_t)ckpt.numel();
         out.push_back(ckpt);
     }
+    if (const size_t bytes = bcm_gated_rec_fwd_workspace_bytes(&a)) {
+        const Tensor& ws = held(workspace((int64_t)bytes, x.device()));
+        a.workspace = ws.data_ptr();
+        a.workspace_bytes = bytes;
+    }
     check_status(bcm_gated_rec_fwd(&a, cur_stream()), "gated_rec_fwd");
     return out;
 }

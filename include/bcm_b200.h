@@ -616,6 +616,7 @@ typedef struct bcm_gated_rec_args {
 } bcm_gated_rec_args;
 
 BCM_API size_t bcm_gated_rec_ckpt_bytes(const bcm_gated_rec_args* args);
+BCM_API size_t bcm_gated_rec_fwd_workspace_bytes(const bcm_gated_rec_args* args);   /* 0 for most sizes */
 BCM_API size_t bcm_gated_rec_bwd_workspace_bytes(const bcm_gated_rec_args* args);
 BCM_API bcm_status bcm_gated_rec_fwd(const bcm_gated_rec_args* args, cudaStream_t stream);
 BCM_API bcm_status bcm_gated_rec_bwd(const bcm_gated_rec_args* args, cudaStream_t stream);

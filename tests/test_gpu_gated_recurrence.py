@@ -118,6 +118,33 @@ def test_a_warp_for_each_sequence(B, L, D, dtype):
         assert_exact(h, want[1], "h_last")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_sequences_in_segments(dtype):
+    """Few features and long sequences: segments of the tokens with their states joined, dense and packed; sequences
+    that start at a segment's first token, end at its last, and span several."""
+    _check(_inputs(2 * 9000, 70, 2, dtype, seed=1), (0, 9000, 18000), (2, 9000))
+    _check(_inputs(8191, 3, 1, dtype, seed=2), (0, 8191), (1, 8191))
+    for cu in ((0, 2048, 4096, 4096, 9000, 20000), (0, 1, 2047, 2048, 19999, 20000), (0, 20000), (0, 0, 20000, 20000)):
+        _check(_inputs(20000, 5, len(cu) - 1, dtype, seed=len(cu)), cu, None)
+    t = _inputs(20000, 5, 3, dtype, seed=9)
+    _check(t, (0, 6000, 12288, 20000), None, False, True, False)
+    _check(t, (0, 6000, 12288, 20000), None, True, False, True)
+
+
+def test_nan_stays_in_its_sequence_across_segments():
+    cu = torch.tensor([0, 4096, 9000, 20000], dtype=torch.int32, device=dev)
+    t = _inputs(20000, 6, 3, torch.float32, seed=12)
+    clean, _ = itf.gated_recurrence(t["x"], t["r"], t["i"], t["lam"], h0=t["h0"], cu_seqlens=cu)
+    x = t["x"].clone()
+    x[4097, 2] = math.nan
+    y, h = itf.gated_recurrence(x, t["r"], t["i"], t["lam"], h0=t["h0"], cu_seqlens=cu)
+    bad = torch.zeros(20000, 6, dtype=torch.bool, device=dev)
+    bad[4097:9000, 2] = True
+    assert_exact(torch.isnan(y), bad, "NaN region")
+    assert_exact(y[~bad], clean[~bad], "clean region")
+    assert torch.isnan(h).sum() == 1 and torch.isnan(h[1, 2])
+
+
 @pytest.mark.parametrize("seed,n,T,D", [(0, 9, 700, 40), (1, 64, 5000, 6), (2, 200, 9000, 70), (3, 1500, 3000, 3), (4, 40, 20000, 2)])
 def test_packed_runs(seed, n, T, D):
     """Many sequences of uneven length, cut at random (some empty), and one that takes nearly every token."""

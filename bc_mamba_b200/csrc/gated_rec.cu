@@ -337,18 +337,26 @@ struct Stream {
     __device__ __forceinline__ void fetch(char* dst, const Input& in, const Place& w, const RecDim& n, int t0, int advance, int width) {
         const uint32_t to = smem_addr(dst);
         if constexpr (FORM == kRows4) {
-            const bool straight = linear(in, n);
-            const char* none = reinterpret_cast<const char*>(base(in, w));
-#pragma unroll
-            for (int j = 0; j < S; ++j) {
-                const char* src = at + (int64_t)j * in.st * (int)sizeof(T);
-                if (!straight && t0 + j < w.L) src = reinterpret_cast<const char*>(base(in, w) + row(in, n, t0 + j) + w.lane * 2);
-                const int size = t0 + j < w.L ? bytes : 0;
-                if (size == 0) src = none;
+            auto copy = [&](int j, const char* src, int size) {
                 const uint32_t d = to + j * R::kPitch + w.lane * 2 * (int)sizeof(T);
                 asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"(src), "r"(min(size, 4)) : "memory");
                 if (sizeof(T) == 4)
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d + 4), "l"(size > 4 ? src + 4 : none), "r"(max(size - 4, 0)) : "memory");
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d + 4), "l"(size > 4 ? src + 4 : src), "r"(max(size - 4, 0)) : "memory");
+            };
+            if (t0 + S <= w.L && linear(in, n)) {
+                const char* src = at;
+#pragma unroll
+                for (int j = 0; j < S; ++j) {
+                    copy(j, src, bytes);
+                    src += in.st * (int)sizeof(T);
+                }
+            } else {
+                const T* from0 = base(in, w);
+#pragma unroll 1
+                for (int j = 0; j < S; ++j) {
+                    const bool there = t0 + j < w.L && bytes > 0;
+                    copy(j, reinterpret_cast<const char*>(there ? from0 + row(in, n, t0 + j) + w.lane * 2 : from0), there ? bytes : 0);
+                }
             }
         } else if (EVEN && t0 + S <= w.L && linear(in, n)) {
 #pragma unroll
@@ -371,6 +379,7 @@ struct Stream {
             }
         } else {
             const T* from0 = base(in, w);
+#pragma unroll 1
             for (int q = w.lane; q < S * R::kGran; q += 32) {
                 const int j = q / R::kGran, g = q - j * R::kGran;
                 int bytes = 0;
@@ -514,7 +523,7 @@ rec_fwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         }
         cp_commit();
     };
-#pragma unroll
+#pragma unroll 1
     for (int k = 0; k < ST - 1; ++k) fetch(k);
     Seq<MODE> seq{cu, (int)n.n, n.Ls, w.off, w.b, 0, 0, 0};
     float2 run = MODE == kDense && !SUM ? load_state(o.h0, w.b, D, w.d, w.has0, w.has1) : f2(0.0f), runA = f2(1.0f);
@@ -725,7 +734,7 @@ rec_bwd_kernel(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         cp_commit();
     };
     constexpr int kAhead = ST - 1;                // turns in flight beyond the one being prepared
-#pragma unroll
+#pragma unroll 1
     for (int k = 1; k <= kAhead; ++k) fetch(turns - k);
     Seq<MODE> seq{cu, (int)n.n, n.Ls, w.off, w.b, 0, 0, 0};
     if (L > 0) seq.at(L - 1);
@@ -985,7 +994,7 @@ rec_fwd_serial(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         }
         cp_commit();
     };
-#pragma unroll
+#pragma unroll 1
     for (int k = 0; k < ST - 1; ++k) fetch(k);
     const float2 l = load_state(lam, 0, D, w.d, w.has0, w.has1);
     const float2 cs = make_float2(w.has0 ? c * softplus_(l.x) : kPolyEnd, w.has1 ? c * softplus_(l.y) : kPolyEnd);
@@ -1078,7 +1087,7 @@ rec_bwd_serial(const __grid_constant__ RecPtr p, const __grid_constant__ RecOut 
         }
         cp_commit();
     };
-#pragma unroll
+#pragma unroll 1
     for (int k = 1; k < ST; ++k) fetch(turns - k);
     const float2 l = load_state(lam, 0, D, w.d, w.has0, w.has1);
     const float2 cs = make_float2(w.has0 ? c * softplus_(l.x) : kPolyEnd, w.has1 ? c * softplus_(l.y) : kPolyEnd);

@@ -286,10 +286,10 @@ struct Rows {
             if (EVEN) return *reinterpret_cast<const float2*>(p);
             return make_float2(*reinterpret_cast<const float*>(p), *reinterpret_cast<const float*>(p + 4));
         } else {
-            // (a row that starts between two words: both words of the pair)
+            // (a row may start between two words: both words of the pair, without a branch)
             const uint32_t* q = reinterpret_cast<const uint32_t*>(EVEN ? p : p - (off & 2));
             uint32_t w = q[0];
-            if (!EVEN && (off & 2)) w = __funnelshift_r(w, q[1], 16);
+            if (!EVEN) w = __funnelshift_r(w, q[1], (off & 2) * 8);
             T v[2];
             memcpy(v, &w, 4);
             return make_float2(to_f32<T>(v[0]), to_f32<T>(v[1]));

@@ -26,9 +26,11 @@ __device__ __forceinline__ float softplus_(float v) { return v > 20.0f ? v : log
 // results an instruction).  What bounds it then is the special-function unit
 // (8 cycles a warp instruction), so:
 //  * v = 1 - a = -expm1(u) is a polynomial for U = -u <= kPolyEnd (degree 4 times
-//    U, interpolated at Chebyshev nodes, relative error 1.4e-8).  It also gives
+//    U, interpolated at Chebyshev nodes, relative error 2.5e-8).  It also gives
 //    1 - a^2 = v + v a without cancellation and a correctly rounded a = 1 - v, so
-//    that a memory of a thousand tokens does not add up a biased decay;
+//    that a memory of a thousand tokens does not add up a biased decay.  Beyond, a
+//    is the exponential itself and v = 1 - a: gradients are proportional to a, and
+//    1 - v would leave it a multiple of 2^-24, 0 from U = 17 on;
 //  * FAST shares one reciprocal between the four sigmoids of a pair and needs no
 //    exponential for a: 7 special functions a pair instead of 12.  It holds where
 //    every c s lies in [kCsLow, kPolyEnd] and the product of a pair's four
@@ -89,11 +91,17 @@ __device__ __forceinline__ Gates gates(float2 r, float2 i, float2 cs, const Cons
     q = fma(U, q, k.c2);
     q = fma(U, q, k.c1);
     float2 v = fma(mul(U, U), q, U);
-    if (!FAST) {
-        if (!(U.x <= kPolyEnd)) v.x = 1.0f - ex2_(U.x * -kLog2e);
-        if (!(U.y <= kPolyEnd)) v.y = 1.0f - ex2_(U.y * -kLog2e);
-    }
     g.a = make_float2(1.0f - v.x, 1.0f - v.y);
+    if (!FAST) {
+        if (!(U.x <= kPolyEnd)) {
+            g.a.x = ex2_(U.x * -kLog2e);
+            v.x = 1.0f - g.a.x;
+        }
+        if (!(U.y <= kPolyEnd)) {
+            g.a.y = ex2_(U.y * -kLog2e);
+            v.y = 1.0f - g.a.y;
+        }
+    }
     const float2 m2 = fma(v, g.a, v);
     g.rs = make_float2(rsqrt_(m2.x), rsqrt_(m2.y));
     if (!FAST) {

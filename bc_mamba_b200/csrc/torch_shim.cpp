@@ -1409,6 +1409,14 @@ std::vector<Tensor> gated_rec_bwd(const Tensor& x, const Tensor& r, const Tensor
     return {dx, dr, di, dlam, dh0};
 }
 
+// whether a graph is recorded and one of them is part of it
+bool any_grad(std::initializer_list<const Tensor*> all) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : all)
+        if (t->defined() && t->requires_grad()) return true;
+    return false;
+}
+
 Tensor gated_rec_step(const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& lam, const Tensor& h,
                       double decay_scale) {
     const char* what = "gated_rec_step";
@@ -1418,8 +1426,12 @@ Tensor gated_rec_step(const Tensor& x, const Tensor& r, const Tensor& i, const T
     const Tensor l = fp32_like(what, lam, "lam", x, {x.size(1)});
     TORCH_CHECK(h.is_contiguous(), what, ": h must be a contiguous float32 tensor (it is updated in place)");
     fp32_like(what, h, "h", x, {x.size(0), x.size(1)});
+    TORCH_CHECK(!any_grad({&x, &r, &i, &lam, &h}), what,
+                ": no gradient passes through the step (it updates h in place); call it under torch.no_grad(), or on detached tensors");
     c10::cuda::CUDAGuard guard(x.device());
     auto y = torch::empty(x.sizes(), x.options());
+    // graphs that saved h learn of the change (inference tensors have no version, and no graph saves them)
+    if (!h.is_inference()) h.unsafeGetTensorImpl()->bump_version();
     check_status(bcm_gated_rec_step(xs.data_ptr(), xs.stride(0), rs.data_ptr(), rs.stride(0), is.data_ptr(), is.stride(0), dt,
                                     x.size(0), x.size(1), l.data_ptr<float>(), (float)decay_scale, h.data_ptr<float>(),
                                     y.data_ptr(), cur_stream()),
@@ -1585,13 +1597,6 @@ struct DistillTopk : public torch::autograd::Function<DistillTopk> {
         return out;
     }
 };
-
-bool any_grad(std::initializer_list<const Tensor*> all) {
-    if (!at::GradMode::is_enabled()) return false;
-    for (const Tensor* t : all)
-        if (t->defined() && t->requires_grad()) return true;
-    return false;
-}
 
 std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& lam,
                                             const optional<Tensor>& h0, const optional<Tensor>& cu_seqlens, double decay_scale) {

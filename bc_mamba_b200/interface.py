@@ -446,7 +446,9 @@ def gated_recurrence(x, r, i, lam, h0=None, cu_seqlens=None, decay_scale: float 
 
 def gated_recurrence_step(x, r, i, lam, h, decay_scale: float = 8.0):
     """One token of gated_recurrence for every sequence: x, r, i (B, D), the
-    state h (B, D) float32 contiguous, updated in place.  Returns y (B, D)."""
+    state h (B, D) float32 contiguous, updated in place.  Returns y (B, D).  No
+    gradient passes through it: while gradients are recorded, inputs that
+    require them are refused, and a graph that saved h finds it modified."""
     return load_ops().gated_rec_step(x, r, i, lam, h, decay_scale)
 
 

@@ -48,6 +48,7 @@ class RecurrentLM:
             out.append(h)
         return F.linear(F.rms_norm(v, v.shape[-1:]), self.head), out
 
+    @torch.no_grad()
     def step_logits(self, tokens, states):
         """One token of every sequence: tokens (B,) -> logits (B, vocab); states are updated in place."""
         v = F.embedding(tokens, self.embed)

@@ -51,17 +51,21 @@ __device__ __forceinline__ int64_t load_id(const void* ids, int wide, int64_t k)
 __host__ __device__ __forceinline__ int list_len(int K) { return (K + 3) / 4 * 4; }
 
 // The row's teacher distribution, by one warp: s_id[k] (-1: absent, up to a multiple of 4), s_p[k] and the student's
-// logit s_z[k]; returns the logarithm of the normaliser plus the maximum, -inf for an empty row.
+// logit s_z[k].  Returns its largest logit (-inf for an empty row) and the logarithm of the sum of exp((q - top) / tau).
+// The difference comes before the factor 1 / tau: an offset of the row loses no digits, and no finite logit becomes -inf.
+struct Teacher {
+    float top, lsum;
+};
 template <typename T, typename TQ>
-__device__ float teacher_row(const T* z, const TQ* q, const void* ids, int wide, int64_t off, int K, int64_t V, float itau, int* s_id, float* s_p,
-                             float* s_z) {
+__device__ Teacher teacher_row(const T* z, const TQ* q, const void* ids, int wide, int64_t off, int K, int64_t V, float itau, int* s_id,
+                               float* s_p, float* s_z) {
     const int lane = threadIdx.x & 31;
     float top = -kInf;
     bool nan = false;
     if (lane < 4 && K + lane < list_len(K)) s_id[K + lane] = -1;
     for (int k = lane; k < K; k += 32) {
         const int64_t id = load_id(ids, wide, off + k);
-        const float v = to_f32<TQ>(q[k]) * itau;
+        const float v = to_f32<TQ>(q[k]);
         const bool there = id >= 0 && id < V && v != -kInf;
         s_id[k] = there ? (int)id : -1;
         s_p[k] = v;
@@ -73,13 +77,13 @@ __device__ float teacher_row(const T* z, const TQ* q, const void* ids, int wide,
     }
     top = warp_max(top);
     if (__any_sync(kFull, nan)) top = __int_as_float(0x7fffffff);
-    if (top == -kInf) return -kInf;
+    if (top == -kInf) return {-kInf, 0.0f};
     float sum = 0.0f;
     for (int k = lane; k < K; k += 32)
-        if (s_id[k] >= 0) sum += expf(s_p[k] - top);
+        if (s_id[k] >= 0) sum += expf((s_p[k] - top) * itau);
     sum = warp_sum(sum);
-    for (int k = lane; k < K; k += 32) s_p[k] = s_id[k] >= 0 ? expf(s_p[k] - top) / sum : 0.0f;
-    return top + logf(sum);
+    for (int k = lane; k < K; k += 32) s_p[k] = s_id[k] >= 0 ? expf((s_p[k] - top) * itau) / sum : 0.0f;
+    return {top, logf(sum)};
 }
 
 template <typename T>
@@ -194,7 +198,7 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
     extern __shared__ __align__(16) char dyn[];
     __shared__ float wm[kWarps], ws[kWarps];
     __shared__ float2 parts[kMaxCluster];
-    __shared__ float s_lse_q;
+    __shared__ Teacher s_teacher;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = (int)a.k;
     int* s_id = reinterpret_cast<int*>(dyn);
     float *s_p = reinterpret_cast<float*>(dyn) + list_len(K), *s_z = s_p + list_len(K);
@@ -224,8 +228,8 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
     if (live) {
         if (FWD) {
             if (teacher) {
-                const float l = teacher_row<T, TQ>(z, q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p, s_z);
-                if (lane == 0) s_lse_q = l;
+                const Teacher l = teacher_row<T, TQ>(z, q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p, s_z);
+                if (lane == 0) s_teacher = l;
             } else {
                 Feed<kThreads> feed(ring, row.at, g0, g1);
                 feed.run(g0 + tid, [&](int64_t g, uint4 in) {
@@ -266,13 +270,15 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
                 soft = {parts[0].x, parts[0].y};
                 for (int k = 1; k < C; ++k) soft.join(parts[k].x, parts[k].y, c);
             }
-            live = s_lse_q != -kInf;
+            live = s_teacher.top != -kInf;
             if (rank == 0 && teacher) {
-                const float lse = soft.m * itau + logf(soft.s), lse_q = s_lse_q;
+                // ln p - ln s, both from differences to their maxima: logits with a common offset lose no digits
+                const float lsum = logf(soft.s), top_q = s_teacher.top, lsum_q = s_teacher.lsum;
                 float sum = 0.0f;
                 if (live)
                     for (int k = lane; k < K; k += 32)
-                        if (s_p[k] > 0.0f || isnan(s_p[k])) sum += s_p[k] * (to_f32<TQ>(q[k]) * itau - lse_q - s_z[k] * itau + lse);
+                        if (s_p[k] > 0.0f || isnan(s_p[k]))
+                            sum += s_p[k] * (((to_f32<TQ>(q[k]) - top_q) * itau - lsum_q) + ((soft.m - s_z[k]) * itau + lsum));
                 sum = warp_sum(sum);
                 if (lane == 0) {
                     a.loss[t] = live ? w * tau * tau * sum : 0.0f;

@@ -4,9 +4,10 @@ from __future__ import annotations
 import numpy as np
 
 
-def _softmax(v):
-    e = np.exp(v - v.max())
-    return e / e.sum(), v.max() + np.log(e.sum())
+def _softmax(v, tau):
+    """softmax(v / tau) and its logarithm, from differences to the maximum."""
+    d = (v - v.max()) / tau
+    return np.exp(d) / np.exp(d).sum(), d - np.log(np.exp(d).sum())
 
 
 def loss_and_grad(z, q, ids, weight=None, tau=1.0, dloss=None):
@@ -19,13 +20,13 @@ def loss_and_grad(z, q, ids, weight=None, tau=1.0, dloss=None):
         at = [k for k in range(q.shape[1]) if 0 <= ids[t, k] < V and q[t, k] != -np.inf]
         if w == 0 or not at:
             continue
-        p, lse_q = _softmax(q[t, at] / tau)
-        s, lse = _softmax(z[t] / tau)
+        p, logp = _softmax(q[t, at], tau)
+        s, logs = _softmax(z[t], tau)
         g = s.copy()
-        for pk, k in zip(p, at):
+        for pk, lk, k in zip(p, logp, at):
             v = ids[t, k]
             if pk > 0:
-                loss[t] += pk * (q[t, k] / tau - lse_q - z[t, v] / tau + lse)
+                loss[t] += pk * (lk - logs[v])
             g[v] -= pk
         loss[t] *= w * tau * tau
         dz[t] = (1.0 if dloss is None else float(dloss[t])) * w * tau * g

@@ -480,7 +480,9 @@ def _per_row(value, off, dtype):
     if not isinstance(value, torch.Tensor):
         return (off if value is None else value), None
     if dtype == torch.int32 and value.dtype != dtype:
-        value = value.clamp(0, 2 ** 31 - 1)
+        # (in a type that holds both ends; a NaN is off, as in the other settings)
+        wide = value.double().nan_to_num(0.0) if value.is_floating_point() else value.to(torch.int64)
+        value = wide.clamp(0, 2 ** 31 - 1)
     return off, value if value.dtype == dtype else value.to(dtype)
 
 

@@ -71,13 +71,14 @@ def distill_step(model: RecurrentLM, optimizer, tokens, cu_seqlens, teacher_logi
 
 @torch.no_grad()
 def generate(model: RecurrentLM, prompts, u, **settings):
-    """prompts (B, L), u (B, n) uniform numbers -> tokens (B, n), their log-probabilities (B, n)."""
+    """prompts (B, L), u (B, n) uniform numbers -> tokens (B, n), their log-probabilities (B, n).  A row whose logits
+    are all NaN or -inf has token -1 there (log-probability -inf); its next step takes token 0."""
     logits, states = model.logits(prompts)
     logits = logits[:, -1]
     tokens, logps = [], []
     for k in range(u.shape[1]):
         if k:
-            logits = model.step_logits(tokens[-1], states)
+            logits = model.step_logits(tokens[-1].clamp(min=0), states)
         token, logp = itf.sample_tokens(logits, u[:, k], **settings)
         tokens.append(token)
         logps.append(logp)

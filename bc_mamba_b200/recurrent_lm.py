@@ -60,9 +60,12 @@ class RecurrentLM:
 
 def distill_step(model: RecurrentLM, optimizer, tokens, cu_seqlens, teacher_logits, teacher_ids, weight, temperature: float = 2.0):
     """One training step on packed documents (T,): the teacher's K top logits and ids per token, weight (T,) with 0
-    for padding.  The head's gradient comes from the one-call form of the loss.  Returns the mean loss (a tensor)."""
+    for padding (all of it: loss and gradients are 0).  The head's gradient comes from the one-call form of the loss.
+    Returns the mean loss (a tensor)."""
     logits, _ = model.logits(tokens, cu_seqlens=cu_seqlens)
-    loss, dlogits = itf.distill_topk_with_grad(logits, teacher_logits, teacher_ids, weight=weight / weight.sum(), temperature=temperature)
+    total = weight.sum()
+    loss, dlogits = itf.distill_topk_with_grad(logits, teacher_logits, teacher_ids, weight=weight / torch.where(total == 0, 1.0, total),
+                                               temperature=temperature)
     optimizer.zero_grad(set_to_none=True)
     logits.backward(dlogits)
     optimizer.step()

@@ -221,9 +221,8 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
     bool live = w != 0.0f;
     Soft soft = {-kInf, 0.0f};
     if (!FWD) {
-        const float2 st = reinterpret_cast<const float2*>(a.stats)[t];
-        soft = {st.x, st.y};
-        live = st.y >= 0.0f || isnan(st.y);      // (the forward marks rows without a target)
+        soft = {a.stats[2 * t], a.stats[2 * t + 1]};
+        live = soft.s >= 0.0f || isnan(soft.s);  // (the forward marks rows without a target)
     }
     if (live) {
         if (FWD) {
@@ -282,13 +281,15 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
                 sum = warp_sum(sum);
                 if (lane == 0) {
                     a.loss[t] = live ? w * tau * tau * sum : 0.0f;
-                    reinterpret_cast<float2*>(a.stats)[t] = live ? make_float2(soft.m, soft.s) : make_float2(0.0f, -1.0f);
+                    a.stats[2 * t] = live ? soft.m : 0.0f;
+                    a.stats[2 * t + 1] = live ? soft.s : -1.0f;
                 }
             }
         }
     } else if (FWD && rank == 0 && tid == 0) {
         a.loss[t] = 0.0f;
-        reinterpret_cast<float2*>(a.stats)[t] = make_float2(0.0f, -1.0f);
+        a.stats[2 * t] = 0.0f;
+        a.stats[2 * t + 1] = -1.0f;
     }
     if (!GRAD) return;
     // the gradient by granules of its own row, which may lie differently from the logits'

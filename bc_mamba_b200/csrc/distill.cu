@@ -365,13 +365,13 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
     }
 }
 
-bcm_status distill_validate(const bcm_distill_args* a, const char* what) {
+bcm_status distill_validate(const bcm_distill_args* a, const char* what, bool fwd) {
     BCM_REQUIRE(a != nullptr, "%s: null arguments", what);
     BCM_REQUIRE(dtype_ok(a->dtype) && dtype_ok(a->teacher_dtype), "%s: unsupported dtype", what);
     BCM_REQUIRE(a->rows >= 0 && a->rows < (1ll << 31) && a->vocab >= 1 && a->vocab < (1ll << 31), "%s: bad sizes", what);
     BCM_REQUIRE(a->k >= 1 && a->k <= BCM_DISTILL_MAX_K, "%s: k must be in [1, %d]", what, BCM_DISTILL_MAX_K);
     BCM_REQUIRE(a->temperature > 0.0f && a->temperature < kInf, "%s: temperature must be positive and finite", what);
-    BCM_REQUIRE(a->rows == 0 || (a->logits && a->teacher_logits && a->teacher_ids && a->loss && a->stats),
+    BCM_REQUIRE(a->rows == 0 || (a->logits && a->teacher_logits && a->teacher_ids && (a->loss || !fwd) && a->stats),
                 "%s: null pointer", what);
     return BCM_OK;
 }
@@ -421,14 +421,14 @@ using namespace bcm;
 
 extern "C" bcm_status bcm_distill_fwd(const bcm_distill_args* a, cudaStream_t stream) {
     clear_error();
-    if (bcm_status st = distill_validate(a, "distill_fwd"); st != BCM_OK) return st;
+    if (bcm_status st = distill_validate(a, "distill_fwd", true); st != BCM_OK) return st;
     if (a->rows == 0) return BCM_OK;
     return distill_launch<true, false>(a, stream);
 }
 
 extern "C" bcm_status bcm_distill_bwd(const bcm_distill_args* a, cudaStream_t stream) {
     clear_error();
-    if (bcm_status st = distill_validate(a, "distill_bwd"); st != BCM_OK) return st;
+    if (bcm_status st = distill_validate(a, "distill_bwd", false); st != BCM_OK) return st;
     if (a->rows == 0) return BCM_OK;
     BCM_REQUIRE(a->dlogits && a->dloss, "distill_bwd: null pointer");
     return distill_launch<false, true>(a, stream);
@@ -436,7 +436,7 @@ extern "C" bcm_status bcm_distill_bwd(const bcm_distill_args* a, cudaStream_t st
 
 extern "C" bcm_status bcm_distill_fwd_grad(const bcm_distill_args* a, cudaStream_t stream) {
     clear_error();
-    if (bcm_status st = distill_validate(a, "distill_fwd_grad"); st != BCM_OK) return st;
+    if (bcm_status st = distill_validate(a, "distill_fwd_grad", true); st != BCM_OK) return st;
     if (a->rows == 0) return BCM_OK;
     BCM_REQUIRE(a->dlogits, "distill_fwd_grad: null pointer");
     return distill_launch<true, true>(a, stream);

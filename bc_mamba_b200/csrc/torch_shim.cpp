@@ -1489,12 +1489,13 @@ std::vector<Tensor> distill_fwd(const Tensor& logits, const Tensor& teacher_logi
 }
 
 Tensor distill_bwd(const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_ids,
-                   const optional<Tensor>& weight, double temperature, const Tensor& loss, const Tensor& stats,
+                   const optional<Tensor>& weight, double temperature, const optional<Tensor>& loss, const Tensor& stats,
                    const Tensor& dloss) {
     const char* what = "distill_bwd";
     Held held;
     bcm_distill_args a = distill_args(what, logits, teacher_logits, teacher_ids, weight, temperature, held);
-    a.loss = const_cast<float*>(held.fp32(what, loss, "loss", logits, {a.rows}));
+    // (the gradient takes nothing of the loss, which its caller may have changed)
+    a.loss = loss.has_value() ? const_cast<float*>(held.fp32(what, *loss, "loss", logits, {a.rows})) : nullptr;
     a.stats = const_cast<float*>(held.fp32(what, stats, "stats", logits, {a.rows, 2}));
     a.dloss = held.fp32(what, dloss, "dloss", logits, {a.rows});
     c10::cuda::CUDAGuard guard(logits.device());
@@ -1584,7 +1585,7 @@ struct DistillTopk : public torch::autograd::Function<DistillTopk> {
                           const optional<Tensor>& weight, double temperature, bool keep) {
         std::vector<Tensor> res = distill_fwd(logits, teacher_logits, teacher_ids, weight, temperature, false);
         if (keep) {
-            ctx->save_for_backward({logits, teacher_logits, teacher_ids, weight.value_or(Tensor()), res[0], res[1]});
+            ctx->save_for_backward({logits, teacher_logits, teacher_ids, weight.value_or(Tensor()), res[1]});
             ctx->saved_data["temperature"] = temperature;
         }
         return res[0];
@@ -1593,7 +1594,7 @@ struct DistillTopk : public torch::autograd::Function<DistillTopk> {
         once("distill_topk");
         const variable_list v = ctx->get_saved_variables();
         variable_list out(6);
-        out[0] = distill_bwd(v[0], v[1], v[2], given(v[3]), ctx->saved_data["temperature"].toDouble(), v[4], v[5], grads[0]);
+        out[0] = distill_bwd(v[0], v[1], v[2], given(v[3]), ctx->saved_data["temperature"].toDouble(), c10::nullopt, v[4], grads[0]);
         return out;
     }
 };
@@ -1724,7 +1725,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "upstream gradient of one");
     m.def("distill_bwd", &distill_bwd, py::arg("logits"), py::arg("teacher_logits"), py::arg("teacher_ids"),
           py::arg("weight"), py::arg("temperature"), py::arg("loss"), py::arg("stats"), py::arg("dloss"),
-          "Backward of distill_fwd -> dlogits (T, V)");
+          "Backward of distill_fwd (its loss may be None) -> dlogits (T, V)");
     m.def("sample_tokens", &sample_tokens, py::arg("logits"), py::arg("u"), py::arg("temperature") = 1.0,
           py::arg("top_k") = 0, py::arg("top_p") = 1.0, py::arg("min_p") = 0.0, py::arg("temperatures") = py::none(),
           py::arg("top_ks") = py::none(), py::arg("top_ps") = py::none(), py::arg("min_ps") = py::none(),

@@ -642,8 +642,8 @@ BCM_API bcm_status bcm_gated_rec_step(const void* x, int64_t x_stride_b, const v
  * where its logits are NaN.  An id that occurs twice adds up.
  * loss [rows] fp32; stats [rows, 2] fp32 carries (max, sum of exp) of z / tau
  * from the forward to the backward; dlogits [rows, vocab] contiguous, must not
- * overlap the logits.  fwd_grad is forward and backward in one call (dloss
- * NULL: 1).
+ * overlap the logits.  The backward takes nothing of loss, which may be NULL
+ * there.  fwd_grad is forward and backward in one call (dloss NULL: 1).
  * ------------------------------------------------------------------------- */
 #define BCM_DISTILL_MAX_K 1024
 

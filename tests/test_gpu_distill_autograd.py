@@ -20,3 +20,15 @@ def test_stats_lie_on_any_float():
     odd.copy_(stats)
     assert odd.data_ptr() % 8 == 4
     assert_exact(ops.distill_bwd(z, q, ids, w, 2.0, loss, odd, up), want, "gradient")
+
+
+def test_the_loss_may_be_changed_in_place():
+    """The backward reads nothing of the loss: masking it in place is a caller's right."""
+    z, q, ids, w, up = _inputs(5, 700, 9, torch.float32, seed=31)
+    mask = torch.tensor([1.0, 0.0, 1.0, 0.5, 1.0], device="cuda")
+    leaf = z.clone().requires_grad_(True)
+    want, = torch.autograd.grad(itf.distill_topk(leaf, q, ids, weight=w), leaf, mask)
+    loss = itf.distill_topk(leaf, q, ids, weight=w)
+    loss *= mask
+    got, = torch.autograd.grad(loss.sum(), leaf)
+    assert_exact(got, want, "gradient")

@@ -370,7 +370,9 @@ bcm_status distill_validate(const bcm_distill_args* a, const char* what, bool fw
     BCM_REQUIRE(dtype_ok(a->dtype) && dtype_ok(a->teacher_dtype), "%s: unsupported dtype", what);
     BCM_REQUIRE(a->rows >= 0 && a->rows < (1ll << 31) && a->vocab >= 1 && a->vocab < (1ll << 31), "%s: bad sizes", what);
     BCM_REQUIRE(a->k >= 1 && a->k <= BCM_DISTILL_MAX_K, "%s: k must be in [1, %d]", what, BCM_DISTILL_MAX_K);
-    BCM_REQUIRE(a->temperature > 0.0f && a->temperature < kInf, "%s: temperature must be positive and finite", what);
+    // (of a smaller one every exponent would be a difference, 0 among them, times infinity)
+    BCM_REQUIRE(a->temperature > 0.0f && a->temperature < kInf && kLog2e / a->temperature < kInf,
+                "%s: temperature must be positive and finite, and its reciprocal a float32", what);
     BCM_REQUIRE(a->rows == 0 || (a->logits && a->teacher_logits && a->teacher_ids && (a->loss || !fwd) && a->stats),
                 "%s: null pointer", what);
     return BCM_OK;

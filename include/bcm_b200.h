@@ -633,7 +633,7 @@ BCM_API bcm_status bcm_gated_rec_step(const void* x, int64_t x_stride_b, const v
  * Row t of the student's logits z [rows, vocab] (dtype, row stride, unit
  * stride of v), the teacher's k logits q [rows, k] (teacher_dtype) with token
  * ids [rows, k] (int32, or int64 with ids_are_int64), w = weight[t] (NULL: 1),
- * tau the temperature:
+ * tau the temperature (log2(e) / tau finite in fp32):
  *   p = softmax(q / tau) over the entries whose id lies in [0, vocab) and
  *       whose logit is not -inf,   s = softmax(z / tau),
  *   loss[t] = w tau^2 sum_j p_j (ln p_j - ln s_{id_j})      (p_j = 0: no term),

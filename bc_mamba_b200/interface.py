@@ -57,15 +57,16 @@ def stage_timing():
         _stage_log = prev
 
 
-class cuda_stage:
+class cuda_stage(contextlib.ContextDecorator):
     """NVTX range named like the reference's profiling stages
     (spike_mamba/runtime_breakdown.py:12-15), timed with CUDA events while
-    stage_timing() is open."""
-
-    __slots__ = ("name", "on", "log", "start")
+    stage_timing() is open.  A context, or a decorator of functions."""
 
     def __init__(self, name: str):
         self.name = name
+
+    def _recreate_cm(self):
+        return cuda_stage(self.name)      # a decorated function's calls may be nested
 
     def __enter__(self):
         self.on = torch.cuda.is_available()

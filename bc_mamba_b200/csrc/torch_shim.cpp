@@ -15,8 +15,10 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <nvtx3/nvToolsExt.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdlib>
 #include <map>
 #include <mutex>
@@ -1409,6 +1411,51 @@ std::vector<Tensor> gated_rec_bwd(const Tensor& x, const Tensor& r, const Tensor
     return {dx, dr, di, dlam, dh0};
 }
 
+// A stage of interface.cuda_stage around work that no Python surrounds.  Its NVTX range, and, while stage_timing() is
+// open, the interface's own stage in its place, whose class time_stages then holds.
+std::atomic<bool> g_timing{false};
+py::object& stage_class() {
+    static py::object* held = new py::object();      // (never destroyed: the interpreter may be gone by then)
+    return *held;
+}
+
+void time_stages(const py::object& cls) {
+    stage_class() = cls;
+    g_timing = !cls.is_none();
+}
+
+class Stage {
+  public:
+    explicit Stage(const char* name) {
+        if (g_timing) {
+            py::gil_scoped_acquire gil;
+            if (stage_class() && !stage_class().is_none()) {
+                timed_ = stage_class()(name).release();
+                timed_.attr("__enter__")();
+            }
+        }
+        if (!timed_) nvtxRangePushA(name);
+    }
+    ~Stage() {
+        if (!timed_) {
+            nvtxRangePop();
+            return;
+        }
+        py::gil_scoped_acquire gil;
+        try {
+            timed_.attr("__exit__")(py::none(), py::none(), py::none());
+        } catch (py::error_already_set& e) {
+            e.discard_as_unraisable("cuda_stage");
+        }
+        timed_.dec_ref();
+    }
+    Stage(const Stage&) = delete;
+    Stage& operator=(const Stage&) = delete;
+
+  private:
+    py::handle timed_;
+};
+
 // whether a graph is recorded and one of them is part of it
 bool any_grad(std::initializer_list<const Tensor*> all) {
     if (!at::GradMode::is_enabled()) return false;
@@ -1430,6 +1477,7 @@ Tensor gated_rec_step(const Tensor& x, const Tensor& r, const Tensor& i, const T
                 ": no gradient passes through the step (it updates h in place); call it under torch.no_grad(), or on detached tensors");
     c10::cuda::CUDAGuard guard(x.device());
     auto y = torch::empty(x.sizes(), x.options());
+    const Stage stage("gated_recurrence_step");
     // graphs that saved h learn of the change (inference tensors have no version, and no graph saves them)
     if (!h.is_inference()) h.unsafeGetTensorImpl()->bump_version();
     check_status(bcm_gated_rec_step(xs.data_ptr(), xs.stride(0), rs.data_ptr(), rs.stride(0), is.data_ptr(), is.stride(0), dt,
@@ -1572,6 +1620,7 @@ struct GatedRecurrence : public torch::autograd::Function<GatedRecurrence> {
         if (!grads[0].defined() && !grads[1].defined()) return out;
         once("gated_recurrence");
         const variable_list v = ctx->get_saved_variables();
+        const Stage stage("gated_recurrence_backward");
         std::vector<Tensor> d = gated_rec_bwd(v[0], v[1], v[2], v[3], given(v[4]), given(v[5]),
                                               ctx->saved_data["decay_scale"].toDouble(), v[6], given(grads[0]), given(grads[1]));
         for (int k = 0; k < 4; ++k) out[k] = d[k];
@@ -1594,6 +1643,7 @@ struct DistillTopk : public torch::autograd::Function<DistillTopk> {
         once("distill_topk");
         const variable_list v = ctx->get_saved_variables();
         variable_list out(6);
+        const Stage stage("distill_backward");
         out[0] = distill_bwd(v[0], v[1], v[2], given(v[3]), ctx->saved_data["temperature"].toDouble(), c10::nullopt, v[4], grads[0]);
         return out;
     }
@@ -1704,6 +1754,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("dW_B"), py::arg("dW_C"), py::arg("ddt_idle"), py::arg("ddt_active"),
           "backward of event_params_fwd (None gradients are zero) -> [dA_log, dW_BC, da0, da1]");
     // language-model operators (no reference bindings)
+    m.def("time_stages", &time_stages, py::arg("stage"),
+          "While not None: the context class, taking a name, that times the stages which run without Python");
     m.def("gated_rec_fwd", &gated_rec_fwd, py::arg("x"), py::arg("r"), py::arg("i"), py::arg("lam"),
           py::arg("h0") = py::none(), py::arg("cu_seqlens") = py::none(), py::arg("decay_scale") = 8.0,
           py::arg("keep_ckpt") = false,

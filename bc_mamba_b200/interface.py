@@ -50,11 +50,14 @@ def stage_timing():
     included).  Yields the list of (name, start_event, end_event); read the
     times after a synchronize."""
     global _stage_log
+    ops = load_ops()
     prev, _stage_log = _stage_log, []
+    ops.time_stages(cuda_stage)           # backward passes in C++ are stages too
     try:
         yield _stage_log
     finally:
         _stage_log = prev
+        ops.time_stages(None if prev is None else cuda_stage)
 
 
 class cuda_stage(contextlib.ContextDecorator):

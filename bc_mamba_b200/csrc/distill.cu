@@ -271,16 +271,16 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
             }
             live = s_teacher.top != -kInf;
             if (rank == 0 && teacher) {
-                // ln p - ln s, both from differences to their maxima: logits with a common offset lose no digits
-                const float lsum = logf(soft.s), top_q = s_teacher.top, lsum_q = s_teacher.lsum;
+                // tau (ln p - ln s), both from differences to their maxima: logits with a common offset lose no digits, and
+                // nothing on the way is larger than the difference of a logit and its maximum
+                const float lsum = tau * (logf(soft.s) - s_teacher.lsum), top_q = s_teacher.top;
                 float sum = 0.0f;
                 if (live)
                     for (int k = lane; k < K; k += 32)
-                        if (s_p[k] > 0.0f || isnan(s_p[k]))
-                            sum += s_p[k] * (((to_f32<TQ>(q[k]) - top_q) * itau - lsum_q) + ((soft.m - s_z[k]) * itau + lsum));
+                        if (s_p[k] > 0.0f || isnan(s_p[k])) sum += s_p[k] * ((to_f32<TQ>(q[k]) - top_q) + (soft.m - s_z[k]) + lsum);
                 sum = warp_sum(sum);
                 if (lane == 0) {
-                    a.loss[t] = live ? w * tau * tau * sum : 0.0f;
+                    a.loss[t] = live ? w * tau * sum : 0.0f;
                     a.stats[2 * t] = live ? soft.m : 0.0f;
                     a.stats[2 * t + 1] = live ? soft.s : -1.0f;
                 }

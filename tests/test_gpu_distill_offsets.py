@@ -41,3 +41,14 @@ def test_finite_teacher_logits_are_never_absent(tau):
     assert (np.abs(_np(loss) - want) <= 1e-5 * np.maximum(1.0, np.abs(want)) * max(1.0, tau * tau)).all()
     assert np.abs(_np(dz) - dwant).max() <= 1e-5 * np.abs(dwant).max()
     assert (want != 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tau", [0.25, 0.5])
+def test_a_target_masked_by_the_lowest_value(dtype, tau):
+    """The loss is as large as the mask times tau, which the type of the loss holds: no step on the way is larger."""
+    z, q, ids, w, up = _inputs(4, 700, 6, dtype, seed=24)
+    z.scatter_(1, ids[:, :1], torch.finfo(dtype).min)
+    w.clamp_(max=1.0)
+    assert torch.isfinite(itf.distill_topk(z, q, ids, weight=w, temperature=tau)).all()
+    _check(z, q, ids, w, tau, up)

@@ -18,10 +18,11 @@ namespace {
 // C blocks of a cluster share a row, in 16-byte granules (rows may start anywhere).
 // The forward is one pass with a running maximum and sum; the backward one pass that
 // writes; loss and gradient in one call are both by the same block, the second from
-// L2 as far as it holds.  (Keeping rows in a cluster's shared memory in between
-// measured slower, 1545 against 1045 us at 8192 x 131072 bf16, and so did clusters of
-// four that leave few enough rows in flight for L2, 1368 us: a block's fixed work -
-// teacher, reductions, the places written again - then recurs for every part.)
+// L2 as far as it holds.  (8192 x 131072 bf16: clusters of four, which leave few
+// enough rows in flight for L2, take 1110 against 991 us, since a block's fixed work -
+// teacher, reductions, the places written again - then recurs for every part.  A row
+// kept in a cluster's shared memory in between was only measured with granules loaded
+// straight into registers, 1545 us, not with the rings below.)
 // Granules arrive by cyclic cp.async buffers of each thread's own.  The teacher's
 // entries and the loss are the work of a warp of their own meanwhile; the K places
 // of the gradient that they touch are written again at the end.
@@ -188,7 +189,8 @@ struct Feed {
     }
 };
 
-// 8192 x 131072 bf16: forward 410 us (5.2 TB/s), backward 684 us (6.3 TB/s of reads and writes, memory's rate), both in one call 999 us.
+// 8192 x 131072 bf16: forward 407 us (5.3 TB/s), backward 674 us (6.4 TB/s of reads and writes, memory's rate), both in one call 991 us;
+// 4096 x 50257 bf16: forward 106 us, bound by instructions (issue slots 78 % busy), backward 137 us (6.0 TB/s), one call 188 us.
 template <typename T, typename TQ, bool FWD, bool GRAD, int kThreads>
 __global__ void __launch_bounds__(kThreads + 32, kThreads == 64 ? 12 : 4)
 distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
@@ -331,6 +333,8 @@ distill_kernel(const __grid_constant__ bcm_distill_args a, int C) {
         });
         }
     } else {
+        // Rows without a target, and logits whose rows lie differently on 16 bytes than the gradient's (columns of a wider
+        // buffer): element by element, 4096 x 50257 of 50304 bf16 backward 270 us against 137.
         if (!FWD && live && teacher) teacher_row<T, TQ>(z, q, a.teacher_ids, a.ids_are_int64, t * K, K, V, itau, s_id, s_p, s_z);
         for (int64_t g = o0 + tid; g < o1; g += kThreads + 32) {
             const int64_t v0 = g * N - out.shift;

@@ -36,7 +36,10 @@ __device__ __forceinline__ float softplus_(float v) { return v > 20.0f ? v : log
 //    every c s lies in [kCsLow, kPolyEnd] and the product of a pair's four
 //    denominators (1 + e^-r)(1 + e^-i) stays below kProdEnd (U is a normal number
 //    then); a warp that finds a larger one (gates below about -10, infinite, NaN)
-//    computes its batch again in the long form.
+//    computes its batch again in the long form.  One feature in 64 outside the range
+//    (an open gate's decay below 0.705 a token) costs its warp as much as all of them:
+//    128 x 4000 x 256 bf16 forward 261 -> 385 us, backward 540 -> 640 us, fp32 348 ->
+//    410 and 620 -> 658 us.
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPolyEnd = 0.35f, kCsLow = 1e-18f;
 constexpr float kProdEnd = 1e18f;

@@ -575,8 +575,9 @@ BCM_API bcm_status bcm_event_params_bwd(const float* A, const float* a0, const f
                                         float* da1, cudaStream_t stream);
 
 /* ---------------------------------------------------------------------------
- * Gated linear recurrence.  No reference binding: a sequence mixer beside the
- * event scan and the dense S6 scan.  Per feature d, c = decay_scale,
+ * Gated linear recurrence (published as the real-gated linear recurrent unit).
+ * No reference binding: a sequence mixer beside the event scan and the dense S6
+ * scan.  Per feature d, c = decay_scale,
  * s = softplus(lam[d]) (identity above 20):
  *   u_t = -c s sigmoid(r_t),  a_t = exp(u_t),  m_t = sqrt(1 - a_t^2),
  *   h_t = a_t h_{t-1} + m_t sigmoid(i_t) x_t,  y_t = h_t,
@@ -640,8 +641,9 @@ BCM_API bcm_status bcm_gated_rec_step(const void* x, int64_t x_stride_b, const v
  *   dlogits[t, v] = dloss[t] w tau (s_v - sum over {j: id_j = v} of p_j).
  * A row without such entries, or with w = 0, has loss 0 and gradient 0 even
  * where its logits are NaN.  An id that occurs twice adds up.
- * loss [rows] fp32; stats [rows, 2] fp32 carries (max, sum of exp) of z / tau
- * from the forward to the backward; dlogits [rows, vocab] contiguous, must not
+ * loss [rows] fp32; stats [rows, 2] fp32 carries the maximum of z (not of
+ * z / tau) and the sum of exp((z - max) / tau) from the forward to the backward,
+ * (0, -1) for a row without a target; dlogits [rows, vocab] contiguous, must not
  * overlap the logits.  The backward takes nothing of loss, which may be NULL
  * there.  fwd_grad is forward and backward in one call (dloss NULL: 1).
  * ------------------------------------------------------------------------- */

@@ -64,6 +64,18 @@ ABI_SYMBOLS = (
     "bcm_distill_bwd",
     "bcm_distill_fwd_grad",
     "bcm_sample_tokens",
+    "bcm_decay_attn_ckpt_bytes",
+    "bcm_decay_attn_fwd_workspace_bytes",
+    "bcm_decay_attn_bwd_workspace_bytes",
+    "bcm_decay_attn_fwd",
+    "bcm_decay_attn_bwd",
+    "bcm_decay_attn_step",
+    "bcm_gated_norm_fwd",
+    "bcm_gated_norm_bwd_workspace_bytes",
+    "bcm_gated_norm_bwd",
+    "bcm_add_norm_fwd",
+    "bcm_add_norm_bwd_workspace_bytes",
+    "bcm_add_norm_bwd",
 )
 
 _ops = None

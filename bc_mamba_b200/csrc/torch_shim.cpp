@@ -1592,6 +1592,276 @@ std::vector<Tensor> sample_tokens(const Tensor& logits, const Tensor& u, double 
     return {tokens, logprob};
 }
 
+// ---- linear attention with a decay for each head ----
+// Sizes, input pointers and strides: q, k (.., Hk, N), v (.., H, P), log_decay (.., H) or (H) with .. = (B, L), packed
+// (T) with cu_seqlens, or (B) for one token.
+bcm_decay_attn_args decay_attn_args(const char* what, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
+                                    const optional<Tensor>& h0, const optional<Tensor>& cu_seqlens, bool step, Held& held) {
+    const bool packed = cu_seqlens.has_value();
+    const int64_t lead = step || packed ? 1 : 2;
+    TORCH_CHECK(v.is_cuda(), what, ": v must be on CUDA");
+    TORCH_CHECK(v.dim() == lead + 2, what, step ? ": v must be (B, H, P)" : ": v must be (B, L, H, P), or (T, H, P) with cu_seqlens");
+    bcm_decay_attn_args a{};
+    a.dtype = float_dtype(v, "v");
+    for (const Tensor* t : {&q, &k}) {
+        TORCH_CHECK(t->is_cuda() && t->device() == v.device() && t->scalar_type() == v.scalar_type(), what,
+                    ": q and k must have the device and dtype of v");
+        TORCH_CHECK(t->dim() == v.dim() && t->sizes().slice(0, lead) == v.sizes().slice(0, lead) && t->sizes() == q.sizes(), what,
+                    ": q and k must be one shape, with the batch and tokens of v");
+    }
+    a.heads = v.size(-2);
+    a.dim_v = v.size(-1);
+    a.qk_heads = q.size(-2);
+    a.dim_k = q.size(-1);
+    TORCH_CHECK(a.heads >= 1 && a.dim_v >= 1 && a.qk_heads >= 1 && a.dim_k >= 1, what, ": heads and features must not be empty");
+    TORCH_CHECK(a.heads % a.qk_heads == 0, what, ": the heads of v must be a multiple of those of q and k");
+    if (packed) {
+        TORCH_CHECK(cu_seqlens->is_cuda() && cu_seqlens->device() == v.device() &&
+                        cu_seqlens->scalar_type() == at::ScalarType::Int && cu_seqlens->dim() == 1 && cu_seqlens->size(0) >= 1,
+                    what, ": cu_seqlens must be a 1-D int32 tensor on the device of v");
+        const Tensor cu = held(cu_seqlens->contiguous());
+        a.batch = cu.size(0) - 1;
+        a.seqlen = v.size(0);
+        a.cu_seqlens = cu.data_ptr<int32_t>();
+        TORCH_CHECK(a.batch >= 1 || a.seqlen == 0, what, ": cu_seqlens of no sequence with tokens");
+    } else {
+        a.batch = v.size(0);
+        a.seqlen = step ? 1 : v.size(1);
+    }
+    auto set = [&](const Tensor& from, const void*& p, int64_t& sb, int64_t& st, int64_t& sh) {
+        const Tensor& t = held(unit_last(from));
+        p = t.data_ptr();
+        sb = packed ? 0 : t.stride(0);
+        st = step ? 0 : t.stride(packed ? 0 : 1);
+        sh = t.stride(-2);
+    };
+    set(q, a.q, a.q_stride_b, a.q_stride_t, a.q_stride_h);
+    set(k, a.k, a.k_stride_b, a.k_stride_t, a.k_stride_h);
+    set(v, a.v, a.v_stride_b, a.v_stride_t, a.v_stride_h);
+    TORCH_CHECK(log_decay.is_cuda() && log_decay.device() == v.device() && log_decay.scalar_type() == at::ScalarType::Float, what,
+                ": log_decay must be a float32 tensor on the device of v");
+    a.fixed_decay = log_decay.dim() == 1;
+    if (a.fixed_decay) {
+        TORCH_CHECK(log_decay.size(0) == a.heads, what, ": log_decay has the wrong shape");
+        a.g_stride_h = log_decay.stride(0);
+    } else {
+        TORCH_CHECK(log_decay.dim() == lead + 1 && log_decay.sizes() == v.sizes().slice(0, lead + 1), what, ": log_decay has the wrong shape");
+        a.g_stride_b = packed ? 0 : log_decay.stride(0);
+        a.g_stride_t = step ? 0 : log_decay.stride(packed ? 0 : 1);
+        a.g_stride_h = log_decay.stride(-1);
+    }
+    a.log_decay = log_decay.data_ptr<float>();
+    if (h0.has_value()) a.h0 = held.fp32(what, *h0, "h0", v, {a.batch, a.heads, a.dim_k, a.dim_v});
+    return a;
+}
+
+std::vector<Tensor> decay_attn_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const optional<Tensor>& h0,
+                                   const optional<Tensor>& cu_seqlens, bool keep_ckpt) {
+    Held held;
+    bcm_decay_attn_args a = decay_attn_args("decay_attn_fwd", q, k, v, log_decay, h0, cu_seqlens, false, held);
+    c10::cuda::CUDAGuard guard(v.device());
+    auto y = torch::empty(v.sizes(), v.options());
+    auto h_last = torch::empty({a.batch, a.heads, a.dim_k, a.dim_v}, log_decay.options());
+    a.y = y.data_ptr();
+    a.h_last = h_last.data_ptr<float>();
+    std::vector<Tensor> out = {y, h_last};
+    if (keep_ckpt) {
+        auto ckpt = workspace((int64_t)bcm_decay_attn_ckpt_bytes(&a), v.device());
+        a.ckpt = ckpt.data_ptr();
+        a.ckpt_bytes = (size_t)ckpt.numel();
+        out.push_back(ckpt);
+    }
+    if (const size_t bytes = bcm_decay_attn_fwd_workspace_bytes(&a)) {
+        const Tensor& ws = held(workspace((int64_t)bytes, v.device()));
+        a.workspace = ws.data_ptr();
+        a.workspace_bytes = bytes;
+    }
+    check_status(bcm_decay_attn_fwd(&a, cur_stream()), "decay_attn_fwd");
+    return out;
+}
+
+std::vector<Tensor> decay_attn_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
+                                   const optional<Tensor>& cu_seqlens, const Tensor& ckpt, const optional<Tensor>& dy,
+                                   const optional<Tensor>& dh_last) {
+    const char* what = "decay_attn_bwd";
+    Held held;
+    bcm_decay_attn_args a = decay_attn_args(what, q, k, v, log_decay, c10::nullopt, cu_seqlens, false, held);
+    if (dy.has_value()) {
+        const Tensor& g = held(check_rows(what, *dy, "dy", v));
+        a.dy = g.data_ptr();
+        a.dy_stride_b = a.cu_seqlens ? 0 : g.stride(0);
+        a.dy_stride_t = g.stride(a.cu_seqlens ? 0 : 1);
+        a.dy_stride_h = g.stride(-2);
+    }
+    if (dh_last.has_value()) a.dh_last = held.fp32(what, *dh_last, "dh_last", v, {a.batch, a.heads, a.dim_k, a.dim_v});
+    TORCH_CHECK(ckpt.is_cuda() && ckpt.device() == v.device() && ckpt.is_contiguous(), what,
+                ": ckpt must be the buffer decay_attn_fwd returned for these inputs");
+    c10::cuda::CUDAGuard guard(v.device());
+    auto dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), k.options()), dv = torch::empty(v.sizes(), v.options());
+    auto dg = torch::empty(log_decay.sizes(), log_decay.options());
+    auto dh0 = torch::empty({a.batch, a.heads, a.dim_k, a.dim_v}, log_decay.options());
+    if (a.batch == 0) dg.zero_();            // (of a fixed decay; there is no token)
+    a.dq = dq.data_ptr();
+    a.dk = dk.data_ptr();
+    a.dv = dv.data_ptr();
+    a.dlog_decay = dg.data_ptr<float>();
+    a.dh0 = dh0.data_ptr<float>();
+    a.ckpt = ckpt.data_ptr();
+    a.ckpt_bytes = ckpt.nbytes();
+    if (const size_t bytes = bcm_decay_attn_bwd_workspace_bytes(&a)) {
+        const Tensor& ws = held(workspace((int64_t)bytes, v.device()));
+        a.workspace = ws.data_ptr();
+        a.workspace_bytes = bytes;
+    }
+    check_status(bcm_decay_attn_bwd(&a, cur_stream()), what);
+    return {dq, dk, dv, dg, dh0};
+}
+
+Tensor decay_attn_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& h) {
+    const char* what = "decay_attn_step";
+    Held held;
+    bcm_decay_attn_args a = decay_attn_args(what, q, k, v, log_decay, c10::nullopt, c10::nullopt, true, held);
+    TORCH_CHECK(h.is_contiguous(), what, ": h must be a contiguous float32 tensor (it is updated in place)");
+    fp32_like(what, h, "h", v, {a.batch, a.heads, a.dim_k, a.dim_v});
+    TORCH_CHECK(!any_grad({&q, &k, &v, &log_decay, &h}), what,
+                ": no gradient passes through the step (it updates h in place); call it under torch.no_grad(), or on detached tensors");
+    c10::cuda::CUDAGuard guard(v.device());
+    auto y = torch::empty(v.sizes(), v.options());
+    a.y = y.data_ptr();
+    const Stage stage("decay_attention_step");
+    if (!h.is_inference()) h.unsafeGetTensorImpl()->bump_version();
+    check_status(bcm_decay_attn_step(&a, h.data_ptr<float>(), cur_stream()), what);
+    return y;
+}
+
+// ---- norms of a block ----
+// t (.., D) as rows of unit stride of the features, of one stride apart
+Tensor norm_rows(const char* what, const Tensor& t, const char* name, const Tensor& like, at::ScalarType dtype) {
+    TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == dtype, what, ": ", name,
+                " has the wrong device or dtype");
+    TORCH_CHECK(t.sizes() == like.sizes(), what, ": ", name, " has the wrong shape");
+    return unit_last(t.reshape({like.numel() / like.size(-1), like.size(-1)}));
+}
+
+void check_features(const char* what, const Tensor& x, const char* name) {
+    TORCH_CHECK(x.is_cuda() && x.dim() >= 1 && x.size(-1) >= 1, what, ": ", name, " must be a CUDA tensor (.., D)");
+}
+
+bcm_gated_norm_args gated_norm_args(const char* what, const Tensor& x, const Tensor& gate, const Tensor& weight, int64_t groups, double eps,
+                                    Held& held) {
+    check_features(what, x, "x");
+    bcm_gated_norm_args a{};
+    a.dtype = float_dtype(x, "x");
+    a.dim = x.size(-1);
+    a.rows = x.numel() / a.dim;
+    a.groups = groups;
+    TORCH_CHECK(groups >= 1 && a.dim % groups == 0, what, ": the features must be a multiple of the groups");
+    a.eps = (float)eps;
+    const Tensor xs = held(norm_rows(what, x, "x", x, x.scalar_type())), gs = held(norm_rows(what, gate, "gate", x, x.scalar_type()));
+    a.x = xs.data_ptr();
+    a.x_stride = xs.stride(0);
+    a.gate = gs.data_ptr();
+    a.gate_stride = gs.stride(0);
+    a.weight = held.fp32(what, weight, "weight", x, {a.dim});
+    return a;
+}
+
+Tensor gated_norm_fwd(const Tensor& x, const Tensor& gate, const Tensor& weight, int64_t groups, double eps) {
+    Held held;
+    bcm_gated_norm_args a = gated_norm_args("gated_norm_fwd", x, gate, weight, groups, eps, held);
+    c10::cuda::CUDAGuard guard(x.device());
+    auto out = torch::empty(x.sizes(), x.options());
+    a.out = out.data_ptr();
+    check_status(bcm_gated_norm_fwd(&a, cur_stream()), "gated_norm_fwd");
+    return out;
+}
+
+std::vector<Tensor> gated_norm_bwd(const Tensor& x, const Tensor& gate, const Tensor& weight, int64_t groups, double eps, const Tensor& dout) {
+    const char* what = "gated_norm_bwd";
+    Held held;
+    bcm_gated_norm_args a = gated_norm_args(what, x, gate, weight, groups, eps, held);
+    const Tensor d = held(norm_rows(what, dout, "dout", x, x.scalar_type()));
+    a.dout = d.data_ptr();
+    a.dout_stride = d.stride(0);
+    c10::cuda::CUDAGuard guard(x.device());
+    auto dx = torch::empty(x.sizes(), x.options()), dgate = torch::empty(x.sizes(), x.options());
+    auto dw = torch::empty(weight.sizes(), weight.options());
+    a.dx = dx.data_ptr();
+    a.dgate = dgate.data_ptr();
+    a.dweight = dw.data_ptr<float>();
+    const Tensor& ws = held(workspace((int64_t)bcm_gated_norm_bwd_workspace_bytes(&a), x.device()));
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = (size_t)ws.numel();
+    check_status(bcm_gated_norm_bwd(&a, cur_stream()), what);
+    return {dx, dgate, dw};
+}
+
+bcm_add_norm_args add_norm_args(const char* what, const Tensor& residual, const Tensor& branch, const Tensor& weight,
+                                const optional<Tensor>& scale, double eps, Held& held) {
+    check_features(what, branch, "branch");
+    bcm_add_norm_args a{};
+    a.dtype = float_dtype(branch, "branch");
+    TORCH_CHECK(residual.scalar_type() == branch.scalar_type() || residual.scalar_type() == at::ScalarType::Float, what,
+                ": residual must have the dtype of branch or be float32");
+    a.residual_dtype = float_dtype(residual, "residual");
+    a.dim = branch.size(-1);
+    a.rows = branch.numel() / a.dim;
+    a.eps = (float)eps;
+    const Tensor r = held(norm_rows(what, residual, "residual", branch, residual.scalar_type()));
+    const Tensor b = held(norm_rows(what, branch, "branch", branch, branch.scalar_type()));
+    a.residual = r.data_ptr();
+    a.residual_stride = r.stride(0);
+    a.branch = b.data_ptr();
+    a.branch_stride = b.stride(0);
+    a.weight = held.fp32(what, weight, "weight", branch, {a.dim});
+    a.scale = scale.has_value() ? held.fp32(what, *scale, "scale", branch, {a.dim}) : nullptr;
+    return a;
+}
+
+std::vector<Tensor> add_norm_fwd(const Tensor& residual, const Tensor& branch, const Tensor& weight, const optional<Tensor>& scale, double eps) {
+    Held held;
+    bcm_add_norm_args a = add_norm_args("add_norm_fwd", residual, branch, weight, scale, eps, held);
+    c10::cuda::CUDAGuard guard(branch.device());
+    auto v = torch::empty(residual.sizes(), residual.options()), out = torch::empty(branch.sizes(), branch.options());
+    a.residual_out = v.data_ptr();
+    a.out = out.data_ptr();
+    check_status(bcm_add_norm_fwd(&a, cur_stream()), "add_norm_fwd");
+    return {v, out};
+}
+
+// -> [dresidual, dbranch, dweight(, dscale)]; without a scale and in one dtype the first two are one tensor
+std::vector<Tensor> add_norm_bwd(const Tensor& residual, const Tensor& branch, const Tensor& weight, const optional<Tensor>& scale, double eps,
+                                 const optional<Tensor>& dresidual_out, const optional<Tensor>& dout) {
+    const char* what = "add_norm_bwd";
+    Held held;
+    bcm_add_norm_args a = add_norm_args(what, residual, branch, weight, scale, eps, held);
+    auto set = [&](const optional<Tensor>& g, const char* name, at::ScalarType dtype, const void*& p, int64_t& st) {
+        if (!g.has_value()) return;
+        const Tensor t = held(norm_rows(what, *g, name, branch, dtype));
+        p = t.data_ptr();
+        st = t.stride(0);
+    };
+    set(dresidual_out, "dresidual_out", residual.scalar_type(), a.dresidual_out, a.dresidual_out_stride);
+    set(dout, "dout", branch.scalar_type(), a.dout, a.dout_stride);
+    c10::cuda::CUDAGuard guard(branch.device());
+    const bool one = !scale.has_value() && residual.scalar_type() == branch.scalar_type();
+    auto dr = torch::empty(residual.sizes(), residual.options()), db = one ? dr : torch::empty(branch.sizes(), branch.options());
+    auto dw = torch::empty(weight.sizes(), weight.options());
+    a.dresidual = dr.data_ptr();
+    a.dbranch = one ? nullptr : db.data_ptr();
+    a.dweight = dw.data_ptr<float>();
+    std::vector<Tensor> out = {dr, db, dw};
+    if (scale.has_value()) {
+        out.push_back(torch::empty(scale->sizes(), scale->options()));
+        a.dscale = out.back().data_ptr<float>();
+    }
+    const Tensor& ws = held(workspace((int64_t)bcm_add_norm_bwd_workspace_bytes(&a), branch.device()));
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = (size_t)ws.numel();
+    check_status(bcm_add_norm_bwd(&a, cur_stream()), what);
+    return out;
+}
+
 // ---- autograd ----
 // C++ functions: the backward runs on the engine's thread without entering Python (forward and backward of a small
 // batch take about half the host time).  The gradients themselves are not differentiable.
@@ -1648,6 +1918,89 @@ struct DistillTopk : public torch::autograd::Function<DistillTopk> {
         return out;
     }
 };
+
+struct DecayAttention : public torch::autograd::Function<DecayAttention> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay,
+                                 const optional<Tensor>& h0, const optional<Tensor>& cu_seqlens, bool keep) {
+        std::vector<Tensor> res = decay_attn_fwd(q, k, v, log_decay, h0, cu_seqlens, keep);
+        if (keep) {
+            ctx->save_for_backward({q, k, v, log_decay, cu_seqlens.value_or(Tensor()), res[2]});
+            ctx->saved_data["h0"] = h0.has_value();
+        }
+        ctx->set_materialize_grads(false);
+        return {res[0], res[1]};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list out(7);
+        if (!grads[0].defined() && !grads[1].defined()) return out;
+        once("decay_attention");
+        const variable_list s = ctx->get_saved_variables();
+        const Stage stage("decay_attention_backward");
+        std::vector<Tensor> d = decay_attn_bwd(s[0], s[1], s[2], s[3], given(s[4]), s[5], given(grads[0]), given(grads[1]));
+        for (int n = 0; n < 4; ++n) out[n] = d[n];
+        if (ctx->saved_data["h0"].toBool()) out[4] = d[4];
+        return out;
+    }
+};
+
+struct GatedNorm : public torch::autograd::Function<GatedNorm> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& gate, const Tensor& weight, int64_t groups, double eps, bool keep) {
+        Tensor out = gated_norm_fwd(x, gate, weight, groups, eps);
+        if (keep) {
+            ctx->save_for_backward({x, gate, weight});
+            ctx->saved_data["groups"] = groups;
+            ctx->saved_data["eps"] = eps;
+        }
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once("gated_norm");
+        const variable_list s = ctx->get_saved_variables();
+        const Stage stage("gated_norm_backward");
+        std::vector<Tensor> d = gated_norm_bwd(s[0], s[1], s[2], ctx->saved_data["groups"].toInt(), ctx->saved_data["eps"].toDouble(), grads[0]);
+        return {d[0], d[1], d[2], Tensor(), Tensor(), Tensor()};
+    }
+};
+
+struct AddNorm : public torch::autograd::Function<AddNorm> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& residual, const Tensor& branch, const Tensor& weight,
+                                 const optional<Tensor>& scale, double eps, bool keep) {
+        std::vector<Tensor> res = add_norm_fwd(residual, branch, weight, scale, eps);
+        if (keep) {
+            ctx->save_for_backward({residual, branch, weight, scale.value_or(Tensor())});
+            ctx->saved_data["eps"] = eps;
+        }
+        ctx->set_materialize_grads(false);
+        return {res[0], res[1]};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list out(6);
+        if (!grads[0].defined() && !grads[1].defined()) return out;
+        once("add_norm");
+        const variable_list s = ctx->get_saved_variables();
+        const Stage stage("add_norm_backward");
+        std::vector<Tensor> d = add_norm_bwd(s[0], s[1], s[2], given(s[3]), ctx->saved_data["eps"].toDouble(), given(grads[0]), given(grads[1]));
+        for (int n = 0; n < (int)d.size(); ++n) out[n] = d[n];
+        return out;
+    }
+};
+
+std::tuple<Tensor, Tensor> decay_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const optional<Tensor>& h0,
+                                           const optional<Tensor>& cu_seqlens) {
+    const Tensor h = h0.value_or(Tensor());
+    variable_list out = DecayAttention::apply(q, k, v, log_decay, h0, cu_seqlens, any_grad({&q, &k, &v, &log_decay, &h}));
+    return {out[0], out[1]};
+}
+
+Tensor gated_norm(const Tensor& x, const Tensor& gate, const Tensor& weight, int64_t groups, double eps) {
+    return GatedNorm::apply(x, gate, weight, groups, eps, any_grad({&x, &gate, &weight}));
+}
+
+std::tuple<Tensor, Tensor> add_norm(const Tensor& residual, const Tensor& branch, const Tensor& weight, const optional<Tensor>& scale, double eps) {
+    const Tensor s = scale.value_or(Tensor());
+    variable_list out = AddNorm::apply(residual, branch, weight, scale, eps, any_grad({&residual, &branch, &weight, &s}));
+    return {out[0], out[1]};
+}
 
 std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& lam,
                                             const optional<Tensor>& h0, const optional<Tensor>& cu_seqlens, double decay_scale) {
@@ -1783,4 +2136,27 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("top_ks") = py::none(), py::arg("top_ps") = py::none(), py::arg("min_ps") = py::none(),
           "One token per row from given uniforms -> [tokens (B) int64, logprob (B)]; a tensor of one setting per row takes "
           "the place of the number");
+    m.def("decay_attn_fwd", &decay_attn_fwd, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("log_decay"), py::arg("h0") = py::none(),
+          py::arg("cu_seqlens") = py::none(), py::arg("keep_ckpt") = false,
+          "Linear attention with a decay for each head -> [y, h_last], with keep_ckpt also the buffer decay_attn_bwd reads");
+    m.def("decay_attn_bwd", &decay_attn_bwd, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("log_decay"), py::arg("cu_seqlens"),
+          py::arg("ckpt"), py::arg("dy"), py::arg("dh_last"),
+          "Backward of decay_attn_fwd (dy or dh_last None: zero) -> [dq, dk, dv, dlog_decay, dh0]");
+    m.def("decay_attention", &decay_attention, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("log_decay"), py::arg("h0") = py::none(),
+          py::arg("cu_seqlens") = py::none(), "decay_attn_fwd with autograd in q, k, v, log_decay and h0 -> (y, h_last)");
+    m.def("decay_attn_step", &decay_attn_step, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("log_decay"), py::arg("h"),
+          "One token of every sequence; the states h (B, H, N, P) are updated in place -> y (B, H, P)");
+    m.def("gated_norm_fwd", &gated_norm_fwd, py::arg("x"), py::arg("gate"), py::arg("weight"), py::arg("groups") = 1, py::arg("eps") = 1e-6,
+          "Norm of x by groups of features, times weight and silu(gate) -> out");
+    m.def("gated_norm_bwd", &gated_norm_bwd, py::arg("x"), py::arg("gate"), py::arg("weight"), py::arg("groups"), py::arg("eps"), py::arg("dout"),
+          "Backward of gated_norm_fwd -> [dx, dgate, dweight]");
+    m.def("gated_norm", &gated_norm, py::arg("x"), py::arg("gate"), py::arg("weight"), py::arg("groups") = 1, py::arg("eps") = 1e-6,
+          "gated_norm_fwd with autograd in x, gate and weight -> out");
+    m.def("add_norm_fwd", &add_norm_fwd, py::arg("residual"), py::arg("branch"), py::arg("weight"), py::arg("scale") = py::none(),
+          py::arg("eps") = 1e-6, "residual + scale * branch and its norm times weight -> [residual, normed]");
+    m.def("add_norm_bwd", &add_norm_bwd, py::arg("residual"), py::arg("branch"), py::arg("weight"), py::arg("scale"), py::arg("eps"),
+          py::arg("dresidual_out"), py::arg("dout"),
+          "Backward of add_norm_fwd (an upstream gradient None: zero) -> [dresidual, dbranch, dweight(, dscale)]");
+    m.def("add_norm", &add_norm, py::arg("residual"), py::arg("branch"), py::arg("weight"), py::arg("scale") = py::none(), py::arg("eps") = 1e-6,
+          "add_norm_fwd with autograd in residual, branch, weight and scale -> (residual, normed)");
 }

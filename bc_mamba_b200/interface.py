@@ -12,7 +12,9 @@ reference's Python layer so callers switch without edits:
 and, without a counterpart there, operators of language models: the gated
 linear recurrence (``gated_recurrence``, ``gated_recurrence_step``), the
 distillation loss on a teacher's top logits (``distill_topk``,
-``distill_topk_with_grad``) and token sampling (``sample_tokens``).
+``distill_topk_with_grad``), token sampling (``sample_tokens``), and the
+parts of a linear-attention block: ``decay_attention``,
+``decay_attention_step``, ``gated_norm`` and ``add_norm``.
 
 All device work goes through the native shim (``bc_mamba_b200._native``);
 there is no Python or CPU fallback.  ``install_shim()`` puts the drop-in
@@ -454,6 +456,59 @@ def gated_recurrence_step(x, r, i, lam, h, decay_scale: float = 8.0):
     gradient passes through it: while gradients are recorded, inputs that
     require them are refused, and a graph that saved h finds it modified."""
     return load_ops().gated_rec_step(x, r, i, lam, h, decay_scale)
+
+
+def decay_attention(q, k, v, log_decay, h0=None, cu_seqlens=None):
+    """Linear attention with a decay for each head: with a_t = exp(log_decay_t),
+    S_t = a_t S_(t-1) + k_t v_t^T (N x P) and y_t = S_t^T q_t.
+
+    v (B, L, H, P), q and k (B, L, Hk, N), or packed (T, ..) with cu_seqlens
+    (n + 1,) int32, ascending from 0 (sequences may be empty; rows behind the
+    last one have y and gradients 0); float32, float16 or bfloat16, any strides
+    of the batch, the tokens and the heads.  Hk divides H: head h reads query
+    and key h // (H / Hk); N is 128 at most.  log_decay is float32, at most 0
+    (-inf drops the state): one per token and head (B, L, H) (packed (T, H)),
+    or one constant for each head (H,).  The entering states h0 (B, H, N, P)
+    (None: zeros) are float32.
+    Returns (y, h_last): y in v's dtype, and the float32 states after each
+    sequence's last token, which continue it as h0 of a next call or as the
+    states of decay_attention_step.  Differentiable in q, k, v, log_decay and
+    h0; gradients are the same from run to run.  States are float32; between
+    them products run on the tensor cores, with masked scores, states and
+    decayed keys as sums of two bfloat16 numbers for 16-bit inputs (relative
+    2^-18) and of three for float32.  A value that is not finite reaches no
+    token before its own."""
+    with cuda_stage("decay_attention_forward"):
+        return load_ops().decay_attention(q, k, v, log_decay, h0, cu_seqlens)
+
+
+def decay_attention_step(q, k, v, log_decay, h):
+    """One token of decay_attention for every sequence: v (B, H, P), q and k
+    (B, Hk, N), log_decay (B, H) or (H,), the states h (B, H, N, P) float32
+    contiguous, updated in place.  Returns y (B, H, P).  No gradient passes
+    through it, as in gated_recurrence_step."""
+    return load_ops().decay_attn_step(q, k, v, log_decay, h)
+
+
+def gated_norm(x, gate, weight, groups: int = 1, eps: float = 1e-6):
+    """The norm of a mixer's output with its gate, per row of x (.., D) and
+    group of D / groups features (a head each, 8192 features at most):
+    x / sqrt(mean(x^2) + eps) * weight * silu(gate).  gate has the shape and
+    dtype of x (float32, float16 or bfloat16, any row stride), weight (D,) is
+    float32.  Differentiable in all three; sums are float32, in a fixed order."""
+    with cuda_stage("gated_norm_forward"):
+        return load_ops().gated_norm(x, gate, weight, groups, eps)
+
+
+def add_norm(residual, branch, weight, scale=None, eps: float = 1e-6):
+    """The residual addition of a block's output and the norm before the next
+    block: v = residual + scale * branch, normed = v / sqrt(mean(v^2) + eps) *
+    weight, over the last dimension (8192 at most).  branch (.., D) is float32,
+    float16 or bfloat16, residual of its dtype or float32, weight and scale (D,)
+    (None: 1) float32.  Returns (v in residual's dtype, normed in branch's); the
+    norm is that of v before it is rounded.  Differentiable in all."""
+    with cuda_stage("add_norm_forward"):
+        return load_ops().add_norm(residual, branch, weight, scale, eps)
 
 
 def distill_topk(logits, teacher_logits, teacher_ids, weight=None, temperature: float = 1.0):

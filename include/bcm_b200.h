@@ -702,6 +702,118 @@ typedef struct bcm_sample_args {
 
 BCM_API bcm_status bcm_sample_tokens(const bcm_sample_args* args, cudaStream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Linear attention with a decay for each head.  No reference binding: the
+ * matrix-state form of the scans above.  Per sequence and head, with
+ * a_t = exp(log_decay_t):
+ *   S_t = a_t S_(t-1) + k_t v_t^T (dim_k x dim_v),   y_t = S_t^T q_t,
+ * S_0 from h0 (NULL: zeros), the state after the last token to h_last.
+ * q, k [batch, seqlen, qk_heads, dim_k], v, y [batch, seqlen, heads, dim_v] in dtype,
+ * log_decay [batch, seqlen, heads] fp32 (at most 0; -inf drops the state); head h
+ * reads query and key h / (heads / qk_heads).  Any strides of b, t and h, unit
+ * stride of the features (stride 0 of b and t in log_decay: one decay for each
+ * head); h0, h_last [batch, heads, dim_k, dim_v] fp32 contiguous; dim_k <= 128.
+ * Packed (cu_seqlens [batch + 1] int32 on the device, ascending from 0): batch
+ * sequences, some of them possibly empty, in seqlen rows; the b strides are not
+ * used.  Rows behind the last sequence have y and gradients 0.  Offsets that are
+ * not ascending or leave [0, seqlen] give undefined values, no access out of range.
+ * States and sums are fp32.  A value that is not finite reaches no token before
+ * its own.
+ * ckpt (bcm_decay_attn_ckpt_bytes): the states that the backward restarts from;
+ * NULL in a forward without a backward.  Backward: dy or dh_last NULL is a zero
+ * gradient; dq, dk, dv [as q, k, v] contiguous in dtype, dlog_decay
+ * [batch, seqlen, heads] fp32 contiguous, with fixed_decay [heads] (sums over
+ * the tokens), dh0 as h0; every output is written, not accumulated, and sums run
+ * in a fixed order.
+ * The step takes one token of every sequence (seqlen 1, t strides not used) and
+ * updates the states h [batch, heads, dim_k, dim_v] in place.
+ * ------------------------------------------------------------------------- */
+#define BCM_DECAY_ATTN_MAX_DIM_K 128
+
+typedef struct bcm_decay_attn_args {
+    int64_t batch, seqlen, heads, qk_heads, dim_k, dim_v;
+    const int32_t* cu_seqlens;
+    bcm_dtype dtype;
+    int fixed_decay;
+    const void* q; int64_t q_stride_b, q_stride_t, q_stride_h;
+    const void* k; int64_t k_stride_b, k_stride_t, k_stride_h;
+    const void* v; int64_t v_stride_b, v_stride_t, v_stride_h;
+    const float* log_decay; int64_t g_stride_b, g_stride_t, g_stride_h;
+    const float* h0;
+    /* forward outputs */
+    void* y; float* h_last;
+    void* ckpt; size_t ckpt_bytes;      /* written by the forward, read by the backward */
+    /* backward */
+    const void* dy; int64_t dy_stride_b, dy_stride_t, dy_stride_h;
+    const float* dh_last;
+    void* dq; void* dk; void* dv; float* dlog_decay; float* dh0;
+    void* workspace; size_t workspace_bytes;
+} bcm_decay_attn_args;
+
+BCM_API size_t bcm_decay_attn_ckpt_bytes(const bcm_decay_attn_args* args);
+BCM_API size_t bcm_decay_attn_fwd_workspace_bytes(const bcm_decay_attn_args* args);
+BCM_API size_t bcm_decay_attn_bwd_workspace_bytes(const bcm_decay_attn_args* args);
+BCM_API bcm_status bcm_decay_attn_fwd(const bcm_decay_attn_args* args, cudaStream_t stream);
+BCM_API bcm_status bcm_decay_attn_bwd(const bcm_decay_attn_args* args, cudaStream_t stream);
+BCM_API bcm_status bcm_decay_attn_step(const bcm_decay_attn_args* args, float* h, cudaStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Norm of a mixer's output with its gate.  No reference binding.
+ * x, gate [rows, dim] in dtype (row strides, unit stride of the features), the
+ * features in `groups` of equal width W (a head each), weight [dim] fp32:
+ *   out = x (mean of the group's x^2 + eps)^(-1/2) weight silu(gate).
+ * W <= 8192, eps > 0.  out, dx, dgate contiguous in dtype; dweight [dim] fp32,
+ * written, summed in a fixed order (rows 0: zeros).
+ * ------------------------------------------------------------------------- */
+typedef struct bcm_gated_norm_args {
+    int64_t rows, dim, groups;
+    bcm_dtype dtype;
+    float eps;
+    const void* x; int64_t x_stride;
+    const void* gate; int64_t gate_stride;
+    const float* weight;
+    void* out;
+    /* backward */
+    const void* dout; int64_t dout_stride;
+    void* dx; void* dgate; float* dweight;
+    void* workspace; size_t workspace_bytes;
+} bcm_gated_norm_args;
+
+BCM_API bcm_status bcm_gated_norm_fwd(const bcm_gated_norm_args* args, cudaStream_t stream);
+BCM_API size_t bcm_gated_norm_bwd_workspace_bytes(const bcm_gated_norm_args* args);
+BCM_API bcm_status bcm_gated_norm_bwd(const bcm_gated_norm_args* args, cudaStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Residual addition with the norm before the next block.  No reference binding.
+ * residual [rows, dim] in residual_dtype (dtype, or fp32), branch [rows, dim] in
+ * dtype (row strides, unit stride of the features), weight [dim] and scale [dim]
+ * (NULL: 1) fp32:
+ *   residual_out = v = residual + scale branch,
+ *   out = v (mean v^2 + eps)^(-1/2) weight, of v before it is rounded.
+ * dim <= 8192, eps > 0.  Backward: the gradients dresidual_out and dout of the
+ * two outputs may be NULL (zero); dresidual in residual_dtype, dbranch in dtype
+ * (NULL where it equals dresidual: no scale, one dtype), dweight, dscale [dim]
+ * fp32, written, summed in a fixed order (rows 0: zeros).  Outputs contiguous.
+ * ------------------------------------------------------------------------- */
+typedef struct bcm_add_norm_args {
+    int64_t rows, dim;
+    bcm_dtype dtype, residual_dtype;
+    float eps;
+    const void* residual; int64_t residual_stride;
+    const void* branch; int64_t branch_stride;
+    const float* weight; const float* scale;
+    void* residual_out; void* out;
+    /* backward */
+    const void* dresidual_out; int64_t dresidual_out_stride;
+    const void* dout; int64_t dout_stride;
+    void* dresidual; void* dbranch; float* dweight; float* dscale;
+    void* workspace; size_t workspace_bytes;
+} bcm_add_norm_args;
+
+BCM_API bcm_status bcm_add_norm_fwd(const bcm_add_norm_args* args, cudaStream_t stream);
+BCM_API size_t bcm_add_norm_bwd_workspace_bytes(const bcm_add_norm_args* args);
+BCM_API bcm_status bcm_add_norm_bwd(const bcm_add_norm_args* args, cudaStream_t stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

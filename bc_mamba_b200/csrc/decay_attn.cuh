@@ -7,10 +7,12 @@
 //
 // Numbers.  The products run on the tensor cores in bf16 with fp32 sums.  An operand of more bits is a sum of bf16
 // pieces, each the rounding of what the pieces before it left: float32 is three pieces (exact), float16 two (exact),
-// and what a kernel computes itself (masked scores, states, keys times decays) is rounded to two for 16-bit inputs
-// (relative 2^-18) and to three for float32.  Products of pieces whose weight is below that are left out.  States are
-// float32 between chunks.  G is summed in float64 and kept as two floats, so that a difference of two of its values
-// keeps full precision after a decay of any size.
+// and what a kernel computes itself (masked scores, states, keys times decays) has as many as its products need: two
+// (relative 2^-18) where they end in 16 bits, three where they end in float32.  Of the pieces' products those whose
+// weight lies below that are left out, and the small ones are added up first: the tensor cores cut sums off instead of
+// rounding them, so that only few additions may be made at the full sum.  States are float32 between chunks.  G is
+// summed in float64 and kept as two floats, so that a difference of two of its values keeps full precision after a
+// decay of any size.
 #pragma once
 
 #include <algorithm>
@@ -24,13 +26,13 @@ namespace decay_attn {
 using bf16 = __nv_bfloat16;
 
 constexpr int kChunk = 64;
-constexpr int kThreads = 128;
 
-// input pieces and pieces of computed operands
+// pieces of an input, and of what is computed for products that end in T; for those that end in float32 there are three
 template <typename T> struct Pieces;
-template <> struct Pieces<float> { static constexpr int in = 3, mid = 3; };
-template <> struct Pieces<__half> { static constexpr int in = 2, mid = 2; };
-template <> struct Pieces<bf16> { static constexpr int in = 1, mid = 2; };
+template <> struct Pieces<float> { static constexpr int in = 3, out = 3; };
+template <> struct Pieces<__half> { static constexpr int in = 2, out = 2; };
+template <> struct Pieces<bf16> { static constexpr int in = 1, out = 2; };
+constexpr int kFull3 = 3;
 
 // ------------------------------------------------------------ matrix products ----
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -110,6 +112,41 @@ __device__ __forceinline__ void split_a(const float (&c0)[4], const float (&c1)[
     }
 }
 
+// acc[2 i], acc[2 i + 1] += A B over K16 steps of 16 and the N16 blocks of 16 columns.  la(regs, piece, step) loads A's
+// NA pieces; B's NB pieces lie `piece` elements apart, stored m[k][n] (BK) or m[n][k].  Products (s, u) of pieces with
+// s + u < D.  With many products to a step all but the largest go in a pass of their own.
+template <int NA, int NB, int D, int K16, int N16, bool BK, typename LA>
+__device__ __forceinline__ void gemm(float (&acc)[2 * N16][4], LA&& la, const bf16* b, int ldb, int piece, int k0, int n0) {
+    constexpr bool two = NA * NB > 4;
+#pragma unroll
+    for (int pass = two ? 0 : 1; pass < 2; ++pass) {
+#pragma unroll
+        for (int kk = 0; kk < K16; ++kk) {
+            uint32_t a[NA][4];
+#pragma unroll
+            for (int s = 0; s < NA; ++s)
+                if (!(two && pass == 1 && s > 0)) la(a[s], s, kk);
+#pragma unroll
+            for (int nb = 0; nb < N16; ++nb)
+#pragma unroll
+                for (int u = NB - 1; u >= 0; --u) {
+                    if (two && pass == 1 && u > 0) continue;
+                    if (u >= D) continue;
+                    uint32_t r[4];
+                    if (BK) load_bk(r, b + u * piece, ldb, k0 + kk * 16, n0 + nb * 16);
+                    else load_bn(r, b + u * piece, ldb, n0 + nb * 16, k0 + kk * 16);
+#pragma unroll
+                    for (int s = NA - 1; s >= 0; --s) {
+                        if (s + u >= D) continue;
+                        if (two && (pass == 1) != (s + u == 0)) continue;
+                        mma(acc[2 * nb], a[s], r[0], r[1]);
+                        mma(acc[2 * nb + 1], a[s], r[2], r[3]);
+                    }
+                }
+        }
+    }
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -119,7 +156,7 @@ __device__ __forceinline__ float ex2(float x) {
 // ------------------------------------------------------------------- decays ----
 // Of one chunk: the running sums of g log2(e) as two floats, what has decayed since the chunk's start and what will
 // until its end, and the decay of the whole chunk.
-struct Decays {
+struct alignas(16) Decays {
     float hi[kChunk], lo[kChunk], since[kChunk], until[kChunk];
     float whole, pad[3];
 };
@@ -205,21 +242,22 @@ __device__ __forceinline__ const T* row_ptr(const Rows& r, const Sizes& z, int s
 }
 
 // ---------------------------------------------------------------------- tiles ----
-template <typename T> __device__ __forceinline__ bool not_finite(T v) { return !(fabsf(to_f32(v)) <= 3.4028234e38f); }
+// whether v's pieces are not finite
+__device__ __forceinline__ bool not_finite(float v) { return !(fabsf(v) <= 3.38e38f); }
 
 template <typename T> struct alignas(16) Eight { T v[8]; };
 
-// A tile of 64 tokens x W columns on its way to shared memory: every thread of the block has W / 16 groups of eight
-// columns.  Rows behind the last token and columns behind the last are 0.
-template <typename T, int W>
+// A tile of R rows x W columns on its way to shared memory: each of TH threads has groups of eight columns.  Rows and
+// columns behind the last are 0.
+template <typename T, int R, int W, int TH>
 struct Pending {
-    static constexpr int n = kChunk * W / 8 / kThreads;
+    static constexpr int all = R * W / 8, n = (all + TH - 1) / TH;
     Eight<T> g[n];
 
     __device__ __forceinline__ void fetch(const T* src, int64_t stride, int rows, int cols, bool vec) {
 #pragma unroll
         for (int i = 0; i < n; ++i) {
-            const int at = threadIdx.x + i * kThreads, row = at / (W / 8), col = at % (W / 8) * 8;
+            const int at = threadIdx.x + i * TH, row = at / (W / 8), col = at % (W / 8) * 8;
             const T* p = src + row * stride + col;
             if (row < rows && vec && col + 8 <= cols) {
                 const uint4* q = (const uint4*)p;
@@ -231,26 +269,48 @@ struct Pending {
             }
         }
     }
-    // writes the pieces; whether a value was not finite
-    __device__ __forceinline__ bool put(bf16* dst, int ld, int rows_of_piece) const {
+    // writes the pieces, R rows of ld each; whether a value was not finite
+    __device__ __forceinline__ bool put(bf16* dst, int ld) const {
         constexpr int NS = Pieces<T>::in;
         bool bad = false;
 #pragma unroll
         for (int i = 0; i < n; ++i) {
-            const int at = threadIdx.x + i * kThreads, row = at / (W / 8), col = at % (W / 8) * 8;
-            uint32_t r[4][NS];
+            const int at = threadIdx.x + i * TH, row = at / (W / 8), col = at % (W / 8) * 8;
+            if (all % TH != 0 && at >= all) continue;
+            if constexpr (std::is_same<T, bf16>::value) {
+                const uint4 q = *(const uint4*)&g[i];
+                const uint32_t e = 0x7f807f80u;
+                // exponents of all ones
+                bad |= (__vcmpeq2(q.x & e, e) | __vcmpeq2(q.y & e, e) | __vcmpeq2(q.z & e, e) | __vcmpeq2(q.w & e, e)) != 0;
+                *(uint4*)(dst + row * ld + col) = q;
+            } else {
+                uint32_t r[4][NS];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                split<NS>(to_f32(g[i].v[2 * u]), to_f32(g[i].v[2 * u + 1]), r[u]);
-                bad |= not_finite(g[i].v[2 * u]) | not_finite(g[i].v[2 * u + 1]);
+                for (int u = 0; u < 4; ++u) {
+                    const float x = to_f32(g[i].v[2 * u]), y = to_f32(g[i].v[2 * u + 1]);
+                    split<NS>(x, y, r[u]);
+                    bad |= not_finite(x) | not_finite(y);
+                }
+#pragma unroll
+                for (int s = 0; s < NS; ++s) *(uint4*)(dst + (s * R + row) * ld + col) = make_uint4(r[0][s], r[1][s], r[2][s], r[3][s]);
             }
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-                *(uint4*)(dst + (s * rows_of_piece + row) * ld + col) = make_uint4(r[0][s], r[1][s], r[2][s], r[3][s]);
         }
         return bad;
     }
 };
+
+// two neighbouring values from their pieces
+template <int NS>
+__device__ __forceinline__ float2 from_pieces(const bf16* m, int piece) {
+    float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int s = NS - 1; s >= 0; --s) {
+        const uint32_t r = *(const uint32_t*)(m + s * piece);
+        v.x += low_f(r);
+        v.y += high_f(r);
+    }
+    return v;
+}
 
 template <typename T>
 __device__ __forceinline__ bool on_16(const T* p, int64_t stride) {
@@ -258,7 +318,7 @@ __device__ __forceinline__ bool on_16(const T* p, int64_t stride) {
 }
 
 // ---------------------------------------------------------------------- state ----
-// An NT x PT state in the registers of four warps, in the accumulators' layout.
+// An NT x PT state in the registers of four warps (which begin at a multiple of four), in the accumulators' layout.
 template <int NT, int PT>
 struct State {
     static constexpr int rows16 = NT / 16;
@@ -268,11 +328,11 @@ struct State {
     float s[M][C][4];
 
     __device__ __forceinline__ static int row(int m) {                 // first of the tile's rows
-        const int w = threadIdx.x >> 5;
+        const int w = (threadIdx.x >> 5) & 3;
         return rows16 >= 4 ? (w * M + m) * 16 : w / across * 16;
     }
     __device__ __forceinline__ static int col(int c) {
-        const int w = threadIdx.x >> 5;
+        const int w = (threadIdx.x >> 5) & 3;
         return ((rows16 >= 4 ? 0 : w % across * C) + c) * 8;
     }
     // calls f(value, row, column) for pairs of neighbouring columns
@@ -325,20 +385,21 @@ struct State {
     // its pieces to shared memory [M][NT][PT + 8]; whether a value was not finite
     template <int MS>
     __device__ __forceinline__ bool put(bf16* dst) {
-        float bad = 0.0f;
+        bool bad = false;
         pairs([&](float& x, float& y, int r, int c) {
             uint32_t q[MS];
             split<MS>(x, y, q);
-            bad = fmaf(x, 0.0f, fmaf(y, 0.0f, bad));
+            bad |= not_finite(x) | not_finite(y);
 #pragma unroll
             for (int k = 0; k < MS; ++k) *(uint32_t*)(dst + (k * NT + r) * (PT + 8) + c) = q[k];
         });
-        return bad != 0.0f;                                            // (0 times what is not finite is NaN)
+        return bad;
     }
-    // s = whole s + sum over the 64 tokens of weight[t] a[t] b[t]^T
-    template <int NS, int MS>
+    // s = whole s + sum over the 64 tokens of weight[t] a[t] b[t]^T; weighted a in three pieces.  Half of the tokens at
+    // a time is added up from 0 and then to the state, whose own roundings stay those of float32.
+    template <int NS>
     __device__ __forceinline__ void advance(const bf16* a, const bf16* b, const float* weight, float whole) {
-        constexpr int lda = NT + 8, ldb = PT + 8;
+        constexpr int lda = NT + 8, ldb = PT + 8, MS = kFull3;
         const int l = lane_id();
         pairs([&](float& x, float& y, int, int) {
             x *= whole;
@@ -356,7 +417,7 @@ struct State {
                     for (int q = 0; q < NS; ++q) load_at(raw[q], a + q * kChunk * lda, lda, row(m), k + 16 * h);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const int t = k + 16 * h + 2 * (l & 3) + 8 * (r >> 1);
+                        const float2 w2 = *(const float2*)(weight + k + 16 * h + 2 * (l & 3) + 8 * (r >> 1));
                         float x = 0.0f, y = 0.0f;
 #pragma unroll
                         for (int q = NS - 1; q >= 0; --q) {
@@ -364,25 +425,32 @@ struct State {
                             y += high_f(raw[q][r]);
                         }
                         uint32_t w[MS];
-                        split<MS>(x * weight[t], y * weight[t + 1], w);
+                        split<MS>(x * w2.x, y * w2.y, w);
 #pragma unroll
                         for (int q = 0; q < MS; ++q) f[m][h][q][r] = w[q];
                     }
                 }
 #pragma unroll
-            for (int c = 0; c < C; ++c)
+            for (int c = 0; c < C; ++c) {
+                float sum[M][4] = {};
+                uint32_t v[NS][4];
 #pragma unroll
-                for (int u = 0; u < NS; ++u) {
-                    uint32_t v[4];
-                    load_bk32(v, b + u * kChunk * ldb, ldb, k, col(c));
+                for (int u = NS - 1; u >= 0; --u) load_bk32(v[u], b + u * kChunk * ldb, ldb, k, col(c));
+                // pieces of small weight first
 #pragma unroll
-                    for (int m = 0; m < M; ++m)
+                for (int order = MS - 1; order >= 0; --order)
 #pragma unroll
-                        for (int q = 0; q < MS - u; ++q) {
-                            mma(s[m][c], f[m][0][q], v[0], v[1]);
-                            mma(s[m][c], f[m][1][q], v[2], v[3]);
+                    for (int u = 0; u < NS && u <= order; ++u)
+#pragma unroll
+                        for (int m = 0; m < M; ++m) {
+                            mma(sum[m], f[m][0][order - u], v[u][0], v[u][1]);
+                            mma(sum[m], f[m][1][order - u], v[u][2], v[u][3]);
                         }
-                }
+#pragma unroll
+                for (int m = 0; m < M; ++m)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[m][c][r] += sum[m][r];
+            }
         }
     }
 };
@@ -468,8 +536,10 @@ struct PartSmem {
     Decays d;
 };
 
+constexpr int kPartThreads = 128;
+
 template <typename T, int NT, int PT, bool BACK>
-__global__ void __launch_bounds__(kThreads) part_kernel(const __grid_constant__ PartArgs p) {
+__global__ void __launch_bounds__(kPartThreads) part_kernel(const __grid_constant__ PartArgs p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     PartSmem<T, NT, PT>& sm = *(PartSmem<T, NT, PT>*)smem_raw;
     const Sizes& z = p.z;
@@ -486,24 +556,28 @@ __global__ void __launch_bounds__(kThreads) part_kernel(const __grid_constant__ 
     st.zero();
     double all = 0.0;
     const int len = it.t1 - it.t0, nc = (len + kChunk - 1) / kChunk, l = lane_id();
-    Pending<T, NT> pa;
-    Pending<T, PT> pb;
-    for (int i = 0; i < nc; ++i) {
+    Pending<T, kChunk, NT, kPartThreads> pa;
+    Pending<T, kChunk, PT, kPartThreads> pb;
+    float g0 = 0.0f, g1 = 0.0f;
+    auto fetch = [&](int i) {                             // the i-th chunk of the walk
         const int t = (BACK ? nc - 1 - i : i) * kChunk, rows = min(kChunk, len - t);
         pa.fetch(a + t * p.a.st, p.a.st, rows, z.n, va);
         pb.fetch(b + t * p.b.st, p.b.st, p.b.p ? rows : 0, cols, vb);
-        float g0 = 0.0f, g1 = 0.0f;
         if (threadIdx.x < 32) {
-            if (2 * l < rows) g0 = g[(int64_t)(t + 2 * l) * p.g_st];
-            if (2 * l + 1 < rows) g1 = g[(int64_t)(t + 2 * l + 1) * p.g_st];
+            g0 = 2 * l < rows ? g[(int64_t)(t + 2 * l) * p.g_st] : 0.0f;
+            g1 = 2 * l + 1 < rows ? g[(int64_t)(t + 2 * l + 1) * p.g_st] : 0.0f;
         }
+    };
+    if (nc > 0) fetch(0);
+    for (int i = 0; i < nc; ++i) {
         __syncthreads();
         if (threadIdx.x < 32) all += decays_of(sm.d, g0, g1);
         // (what is not finite stays so in the sums, and the walk takes such chunks token by token)
-        pa.put(&sm.a[0][0][0], NT + 8, kChunk);
-        pb.put(&sm.b[0][0][0], PT + 8, kChunk);
+        pa.put(&sm.a[0][0][0], NT + 8);
+        pb.put(&sm.b[0][0][0], PT + 8);
         __syncthreads();
-        st.template advance<Pieces<T>::in, Pieces<T>::mid>(&sm.a[0][0][0], &sm.b[0][0][0], BACK ? sm.d.since : sm.d.until, sm.d.whole);
+        if (i + 1 < nc) fetch(i + 1);
+        st.template advance<Pieces<T>::in>(&sm.a[0][0][0], &sm.b[0][0][0], BACK ? sm.d.since : sm.d.until, sm.d.whole);
     }
     const int64_t at = (int64_t)item * z.heads + h;
     st.store(p.parts.state + at * z.n * z.p + col, z.n, z.p - col, z.p);
@@ -516,7 +590,7 @@ bcm_status launch_part(const PartArgs& p, cudaStream_t stream) {
     auto kernel = part_kernel<T, NT, PT, BACK>;
     bcm_status st = allow_smem(kernel, smem);
     if (st != BCM_OK) return st;
-    kernel<<<(unsigned)(p.z.items * p.z.heads * p.z.slices), kThreads, smem, stream>>>(p);
+    kernel<<<(unsigned)(p.z.items * p.z.heads * p.z.slices), kPartThreads, smem, stream>>>(p);
     BCM_LAUNCH_CHECK();
     return BCM_OK;
 }

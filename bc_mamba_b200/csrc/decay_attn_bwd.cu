@@ -28,17 +28,23 @@ struct BwdArgs {
     int shares;
 };
 
+// Four groups of four warps: dv and dg's pairs; dk; dq; the state's gradient.  The first three take 16 tokens a warp.
+// Where there is room for it the pieces of the next chunk's gradient go to a second buffer.
+constexpr int kBwdThreads = 512;
+
 template <typename T, int NT, int PT>
 struct BwdSmem {
-    static constexpr int NS = Pieces<T>::in, MS = Pieces<T>::mid;
+    static constexpr int NS = Pieces<T>::in, MS = Pieces<T>::out;
     struct Tiles {
         bf16 q[NS][kChunk][NT + 8], k[NS][kChunk][NT + 8], v[NS][kChunk][PT + 8], dy[NS][kChunk][PT + 8];
-        bf16 s[MS][NT][PT + 8], ds[MS][NT][PT + 8];
+        bf16 s[kFull3][NT][PT + 8];
     } tiles;
+    static constexpr int buffers = sizeof(Tiles) + 2 * sizeof(bf16[kFull3][NT][PT + 8]) <= 222 * 1024 ? 2 : 1;
+    bf16 ds[buffers][kFull3][NT][PT + 8];
     Decays d;
     float pairs[4][kChunk];    // sum over i >= t, j < t of W_ij, j of one warp
     float of_q[kChunk], of_k[kChunk];
-    float across[2][4];        // <S_in, dS> of the warps, two chunks
+    float across[4];           // <S_in, dS> of the warps
 };
 
 // where a block's rows of dq and dk go
@@ -76,12 +82,12 @@ template <typename T, int NT, int PT>
 __device__ __noinline__ void back_tokens(const BwdArgs& p, const T* q, const T* k, const T* v, const T* dy, const float* g, const float* s_in,
                                          const RowsOut<T>& dq, const RowsOut<T>& dk, T* dv, int64_t dv_st, float* dg, int64_t dg_st,
                                          int rows, int cols, int64_t row0, float* f) {
-    constexpr int parts = kThreads / PT, warps = PT / 32;
+    constexpr int parts = kBwdThreads / PT, warps = PT / 32, all_warps = kBwdThreads / 32;
     const int c = threadIdx.x % PT, part = threadIdx.x / PT, w = threadIdx.x >> 5, l = lane_id();
     float* const sq = f + NT * PT;                 // [warps][NT]
     float* const sk = sq + 2 * NT;
-    float* const sv = sk + 2 * NT;                 // [kThreads]
-    float* const sg = sv + kThreads;               // [4]
+    float* const sv = sk + 2 * NT;                 // [kBwdThreads]
+    float* const sg = sv + kBwdThreads;            // [all_warps]
     const bool in = c < cols;
     for (int t = rows - 1; t >= 0; --t) {
         const float a = expf(g[t * p.g_st]);
@@ -113,7 +119,7 @@ __device__ __noinline__ void back_tokens(const BwdArgs& p, const T* q, const T* 
         if (l == 0) sg[w] = gg;
         sv[threadIdx.x] = gv;
         __syncthreads();
-        for (int n = threadIdx.x; n < p.z.n; n += kThreads) {
+        for (int n = threadIdx.x; n < p.z.n; n += kBwdThreads) {
             float x0 = sq[n], x1 = sk[n];
             if (warps > 1) {
                 x0 += sq[NT + n];
@@ -126,16 +132,20 @@ __device__ __noinline__ void back_tokens(const BwdArgs& p, const T* q, const T* 
             for (int r = 1; r < parts; ++r) gv += sv[r * PT + c];
             dv[t * dv_st + c] = from_f32<T>(gv);
         }
-        if (threadIdx.x == 0) dg[t * dg_st] = (sg[0] + sg[1]) + (sg[2] + sg[3]);
+        if (threadIdx.x == 0) {
+            for (int r = 1; r < all_warps; ++r) gg += sg[r];
+            dg[t * dg_st] = gg;
+        }
         __syncthreads();
     }
 }
 
 template <typename T, int NT, int PT>
-__global__ void __launch_bounds__(kThreads) bwd_kernel(const __grid_constant__ BwdArgs p) {
+__global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant__ BwdArgs p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    BwdSmem<T, NT, PT>& sm = *(BwdSmem<T, NT, PT>*)smem_raw;
-    constexpr int NS = Pieces<T>::in, MS = Pieces<T>::mid, LN = NT + 8, LP = PT + 8;
+    using Smem = BwdSmem<T, NT, PT>;
+    Smem& sm = *(Smem*)smem_raw;
+    constexpr int NS = Smem::NS, MS = Smem::MS, LN = NT + 8, LP = PT + 8;
     const Sizes& z = p.z;
     const int across = z.heads * z.slices, share = z.heads / z.qk_heads;
     const int item = blockIdx.x / across, hs = blockIdx.x % across, h = hs / z.slices, slice = hs % z.slices, col = slice * PT;
@@ -174,168 +184,166 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const __grid_constant__ B
     const bool vq = on_16(q, p.q.st), vk = on_16(k, p.k.st), vv = on_16(v, p.v.st), vy = dy && on_16(dy, p.dy.st);
     const bool pair_v = (((uintptr_t)dv | (uintptr_t)(v_st * sizeof(T))) & (2 * sizeof(T) - 1)) == 0, pair_qk = dq.pairs() && dk.pairs();
     const int np = z.n * z.p;
-    State<NT, PT> ds;
-    const float* from = it.last ? (p.dh_last ? p.dh_last + ((int64_t)it.seq * z.heads + h) * np : nullptr)
-                                : p.enter + ((int64_t)item * z.heads + h) * np;
-    if (from) ds.load(from + col, z.n, z.p - col, z.p);
-    else ds.zero();
     const int len = it.t1 - it.t0, nc = (len + kChunk - 1) / kChunk;
-    const int l = lane_id(), w = threadIdx.x >> 5, row = w * 16 + (l >> 2), lq = l & 3;
+    const int l = lane_id(), group = threadIdx.x >> 7, w = (threadIdx.x >> 5) & 3, row = w * 16 + (l >> 2), lq = l & 3;
+    const bool decay_warp = threadIdx.x >= 384 && threadIdx.x < 416;
     bf16* const tq = &sm.tiles.q[0][0][0];
     bf16* const tk = &sm.tiles.k[0][0][0];
     bf16* const tv = &sm.tiles.v[0][0][0];
     bf16* const ty = &sm.tiles.dy[0][0][0];
     bf16* const ts = &sm.tiles.s[0][0][0];
-    bf16* const tds = &sm.tiles.ds[0][0][0];
+    constexpr int piece_n = kChunk * LN, piece_p = kChunk * LP, piece_s = NT * LP;
 
-    // dg of chunk c from what its walk left in shared memory (one warp)
-    auto finish_dg = [&](int c) {
-        const int t = 2 * l, rows = min(kChunk, len - c * kChunk);
-        const float q0 = sm.of_q[t], q1 = sm.of_q[t + 1], k0 = sm.of_k[t], k1 = sm.of_k[t + 1];
-        float behind = q0 + q1, before = k0 + k1;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const float a = __shfl_down_sync(kFull, behind, off), b = __shfl_up_sync(kFull, before, off);
-            if (l + off < 32) behind += a;
-            if (l >= off) before += b;
+    Pending<T, kChunk, NT, kBwdThreads> pq, pk;
+    Pending<T, kChunk, PT, kBwdThreads> pv, py;
+    Pending<float, NT, PT, kBwdThreads> ps;
+    float g0 = 0.0f, g1 = 0.0f;
+    const bool vs = (z.p & 3) == 0 && (col & 3) == 0 && ((uintptr_t)p.ckpt & 15) == 0;
+    auto state_in = [&](int c) { return p.ckpt + ((int64_t)(it.chunk + c) * z.heads + h) * np + col; };
+    auto fetch = [&](int c) {
+        const int t = c * kChunk, rows = min(kChunk, len - t);
+        pq.fetch(q + t * p.q.st, p.q.st, rows, z.n, vq);
+        pk.fetch(k + t * p.k.st, p.k.st, rows, z.n, vk);
+        pv.fetch(v + t * p.v.st, p.v.st, rows, cols, vv);
+        py.fetch(dy + t * p.dy.st, p.dy.st, dy ? rows : 0, cols, vy);
+        ps.fetch(state_in(c), z.p, z.n, cols, vs);
+        if (decay_warp) {
+            g0 = 2 * l < rows ? g[(int64_t)(t + 2 * l) * p.g_st] : 0.0f;
+            g1 = 2 * l + 1 < rows ? g[(int64_t)(t + 2 * l + 1) * p.g_st] : 0.0f;
         }
-        float rest = __shfl_down_sync(kFull, behind, 1), past = __shfl_up_sync(kFull, before, 1);
-        if (l == 31) rest = 0.0f;
-        if (l == 0) past = 0.0f;
-        const float* x = sm.across[c & 1];
-        const float through = sm.d.whole * ((x[0] + x[1]) + (x[2] + x[3]));
-        float d0 = 0.0f, d1 = 0.0f;
-        for (int k2 = 0; k2 <= t / 16; ++k2) {
-            d0 += sm.pairs[k2][t];
-            d1 += sm.pairs[k2][t + 1];
-        }
-        d0 += (rest + q1 + q0) + past + through;
-        d1 += (rest + q1) + (past + k0) + through;
-        if (t < rows) dg[(int64_t)(c * kChunk + t) * z.heads] = d0;
-        if (t + 1 < rows) dg[(int64_t)(c * kChunk + t + 1) * z.heads] = d1;
     };
+    auto put = [&]() {
+        bool bad = pq.put(tq, LN);
+        bad |= pk.put(tk, LN);
+        bad |= pv.put(tv, LP);
+        bad |= py.put(ty, LP);
+        bad |= ps.put(ts, LP);
+        if (decay_warp) {
+            bad |= !(g0 <= 3.38e38f && g1 <= 3.38e38f);
+            decays_of(sm.d, g0, g1);
+        }
+        return bad;
+    };
+    auto walk = [&](int c) {
+        const int t = c * kChunk;
+        back_tokens<T, NT, PT>(p, q + t * p.q.st, k + t * p.k.st, v + t * p.v.st, dy ? dy + t * p.dy.st : nullptr, g + t * p.g_st, state_in(c), dq, dk,
+                               dv + t * v_st, v_st, dg + (int64_t)t * z.heads, z.heads, min(kChunk, len - t), cols, row_at + t, (float*)&sm.tiles);
+    };
+    if (nc > 0) fetch(nc - 1);
 
-    bool pending = false;      // whether the chunk behind has its dg still to be finished
+    if (group == 3) {
+        // dg of chunk c from what its walk left in shared memory (one warp)
+        auto finish_dg = [&](int c) {
+            const int t = 2 * l, rows = min(kChunk, len - c * kChunk);
+            const float q0 = sm.of_q[t], q1 = sm.of_q[t + 1], k0 = sm.of_k[t], k1 = sm.of_k[t + 1];
+            float behind = q0 + q1, before = k0 + k1;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const float a = __shfl_down_sync(kFull, behind, off), b = __shfl_up_sync(kFull, before, off);
+                if (l + off < 32) behind += a;
+                if (l >= off) before += b;
+            }
+            float rest = __shfl_down_sync(kFull, behind, 1), past = __shfl_up_sync(kFull, before, 1);
+            if (l == 31) rest = 0.0f;
+            if (l == 0) past = 0.0f;
+            const float through = sm.d.whole * ((sm.across[0] + sm.across[1]) + (sm.across[2] + sm.across[3]));
+            float d0 = 0.0f, d1 = 0.0f;
+            for (int k2 = 0; k2 <= t / 16; ++k2) {
+                d0 += sm.pairs[k2][t];
+                d1 += sm.pairs[k2][t + 1];
+            }
+            d0 += (rest + q1 + q0) + past + through;
+            d1 += (rest + q1) + (past + k0) + through;
+            if (t < rows) dg[(int64_t)(c * kChunk + t) * z.heads] = d0;
+            if (t + 1 < rows) dg[(int64_t)(c * kChunk + t + 1) * z.heads] = d1;
+        };
+        State<NT, PT> ds;
+        const float* from = it.last ? (p.dh_last ? p.dh_last + ((int64_t)it.seq * z.heads + h) * np : nullptr)
+                                    : p.enter + ((int64_t)item * z.heads + h) * np;
+        if (from) ds.load(from + col, z.n, z.p - col, z.p);
+        else ds.zero();
+        bool bad = false, pending = false;                    // pending: the chunk behind has its dg still to be finished
+        if (Smem::buffers > 1) bad = ds.template put<kFull3>(&sm.ds[(nc - 1) & 1 & (Smem::buffers - 1)][0][0][0]);
+        for (int c = nc - 1; c >= 0; --c) {
+            __syncthreads();                                  // the chunk behind is done with the tiles
+            if (pending && decay_warp) finish_dg(c + 1);
+            bad |= put();
+            if (Smem::buffers == 1) bad |= ds.template put<kFull3>(&sm.ds[0][0][0][0]);
+            const bool slow = __syncthreads_or(bad);
+            if (c > 0) fetch(c - 1);
+            pending = !slow;
+            if (slow) {
+                float* f = (float*)&sm.tiles;
+                ds.pairs([&](float& x0, float& x1, int r, int cc) {
+                    f[r * PT + cc] = x0;
+                    f[r * PT + cc + 1] = x1;
+                });
+                __syncthreads();
+                walk(c);
+                ds.pairs([&](float& x0, float& x1, int r, int cc) {
+                    x0 = f[r * PT + cc];
+                    x1 = f[r * PT + cc + 1];
+                });
+            } else {
+                float x = 0.0f;
+                ds.pairs([&](float& x0, float& x1, int r, int cc) {
+                    const float2 in = from_pieces<kFull3>(ts + r * LP + cc, piece_s);
+                    x = fmaf(in.x, x0, fmaf(in.y, x1, x));
+                });
+#pragma unroll
+                for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(kFull, x, o);
+                if (l == 0) sm.across[w] = x;
+                ds.template advance<NS>(tq, ty, sm.d.since, sm.d.whole);
+            }
+            bad = false;
+            if (Smem::buffers > 1) bad = ds.template put<kFull3>(&sm.ds[(c + 1) & 1 & (Smem::buffers - 1)][0][0][0]);
+        }
+        __syncthreads();
+        if (pending && decay_warp) finish_dg(0);
+        if (it.first) ds.store(p.dh0 + ((int64_t)it.seq * z.heads + h) * np + col, z.n, z.p - col, z.p);
+        return;
+    }
+
     for (int c = nc - 1; c >= 0; --c) {
         const int t = c * kChunk, rows = min(kChunk, len - t);
-        const float* s_in = p.ckpt + ((int64_t)(it.chunk + c) * z.heads + h) * np + col;
-        bool bad = false;
-        float x = 0.0f;
-        {
-            Pending<T, NT> pq, pk;
-            Pending<T, PT> pv, py;
-            pq.fetch(q + t * p.q.st, p.q.st, rows, z.n, vq);
-            pk.fetch(k + t * p.k.st, p.k.st, rows, z.n, vk);
-            pv.fetch(v + t * p.v.st, p.v.st, rows, cols, vv);
-            py.fetch(dy + t * p.dy.st, p.dy.st, dy ? rows : 0, cols, vy);
-            float g0 = 0.0f, g1 = 0.0f;
-            if (w == 0) {
-                if (2 * l < rows) g0 = g[(int64_t)(t + 2 * l) * p.g_st];
-                if (2 * l + 1 < rows) g1 = g[(int64_t)(t + 2 * l + 1) * p.g_st];
-                bad = !(g0 <= 3.4028234e38f && g1 <= 3.4028234e38f);
-            }
-            __syncthreads();                                  // the chunk behind is done with the tiles
-            if (w == 0) {
-                if (pending) finish_dg(c + 1);
-                decays_of(sm.d, g0, g1);
-            }
-            bad |= pq.put(tq, LN, kChunk);
-            bad |= pk.put(tk, LN, kChunk);
-            bad |= pv.put(tv, LP, kChunk);
-            bad |= py.put(ty, LP, kChunk);
-            State<NT, PT> in;
-            in.load(s_in, z.n, z.p - col, z.p);
-#pragma unroll
-            for (int m = 0; m < ds.M; ++m)
-#pragma unroll
-                for (int e = 0; e < ds.C; ++e)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) x = fmaf(in.s[m][e][r], ds.s[m][e][r], x);
-            bad |= in.template put<MS>(ts);
-            bad |= ds.template put<MS>(tds);
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(kFull, x, o);
-        if (l == 0) sm.across[c & 1][w] = x;
-        pending = true;
-        if (__syncthreads_or(bad)) {
-            float* f = (float*)&sm.tiles;
-            ds.pairs([&](float& x0, float& x1, int r, int cc) {
-                f[r * PT + cc] = x0;
-                f[r * PT + cc + 1] = x1;
-            });
+        __syncthreads();
+        const bool bad = put();
+        const bool slow = __syncthreads_or(bad);
+        if (c > 0) fetch(c - 1);
+        if (slow) {
             __syncthreads();
-            back_tokens<T, NT, PT>(p, q + t * p.q.st, k + t * p.k.st, v + t * p.v.st, dy ? dy + t * p.dy.st : nullptr, g + t * p.g_st, s_in, dq, dk,
-                                   dv + t * v_st, v_st, dg + (int64_t)t * z.heads, z.heads, rows, cols, row_at + t, f);
-            ds.pairs([&](float& x0, float& x1, int r, int cc) {
-                x0 = f[r * PT + cc];
-                x1 = f[r * PT + cc + 1];
-            });
-            pending = false;
+            walk(c);
             continue;
         }
+        const bf16* tds = &sm.ds[c & 1 & (Smem::buffers - 1)][0][0][0];
         const float hi0 = sm.d.hi[row], lo0 = sm.d.lo[row], hi1 = sm.d.hi[row + 8], lo1 = sm.d.lo[row + 8];
-        // ---- this warp's 16 tokens as keys and values
-        {
-            float gv[PT / 8][4] = {}, gk[NT / 8][4] = {};
+        auto keys = [&](uint32_t(&a)[4], int s, int kk) { load_a(a, tk + s * piece_n, LN, w * 16, kk * 16); };
+        auto values = [&](uint32_t(&a)[4], int s, int kk) { load_a(a, tv + s * piece_p, LP, w * 16, kk * 16); };
+        auto ups = [&](uint32_t(&a)[4], int s, int kk) { load_a(a, ty + s * piece_p, LP, w * 16, kk * 16); };
+        // x D of 16 rows by 16 columns: rows as the earlier tokens (keys) or as the later ones (queries)
+        auto decayed = [&](float(&x)[2][4], int block, bool as_keys) {
 #pragma unroll
-            for (int kk = 0; kk < NT; kk += 16) {
-                uint32_t a[NS][4];
+            for (int q2 = 0; q2 < 2; ++q2) {
+                const int o = block * 16 + q2 * 8 + 2 * lq;
+                const float2 h2 = *(const float2*)&sm.d.hi[o], l2 = *(const float2*)&sm.d.lo[o];
 #pragma unroll
-                for (int s = 0; s < NS; ++s) load_a(a[s], tk + s * kChunk * LN, LN, w * 16, kk);
-#pragma unroll
-                for (int pb = 0; pb < PT / 16; ++pb)
-#pragma unroll
-                    for (int u = 0; u < MS; ++u) {
-                        uint32_t b[4];
-                        load_bk(b, tds + u * NT * LP, LP, kk, pb * 16);
-#pragma unroll
-                        for (int s = 0; s < NS && s + u < MS; ++s) {
-                            mma(gv[2 * pb], a[s], b[0], b[1]);
-                            mma(gv[2 * pb + 1], a[s], b[2], b[3]);
-                        }
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    const int i = o + (e & 1), r = row + (e & 2) * 4;
+                    const float ho = e & 1 ? h2.y : h2.x, lo = e & 1 ? l2.y : l2.x, hr = e & 2 ? hi1 : hi0, lr = e & 2 ? lo1 : lo0;
+                    if (as_keys) x[q2][e] = i >= r ? x[q2][e] * between(ho, lo, hr, lr) : 0.0f;
+                    else x[q2][e] = i <= r ? x[q2][e] * between(hr, lr, ho, lo) : 0.0f;
+                }
             }
-#pragma unroll
-            for (int kk = 0; kk < PT; kk += 16) {
-                uint32_t a[NS][4];
-#pragma unroll
-                for (int s = 0; s < NS; ++s) load_a(a[s], tv + s * kChunk * LP, LP, w * 16, kk);
-#pragma unroll
-                for (int nb = 0; nb < NT / 16; ++nb)
-#pragma unroll
-                    for (int u = 0; u < MS; ++u) {
-                        uint32_t b[4];
-                        load_bn(b, tds + u * NT * LP, LP, nb * 16, kk);
-#pragma unroll
-                        for (int s = 0; s < NS && s + u < MS; ++s) {
-                            mma(gk[2 * nb], a[s], b[0], b[1]);
-                            mma(gk[2 * nb + 1], a[s], b[2], b[3]);
-                        }
-                    }
-            }
-            const float u0 = sm.d.until[row], u1 = sm.d.until[row + 8];
+        };
+        // a row's dot with `tile`'s, into out[row]
+        auto dots = [&](float(&x)[NT / 8][4], const bf16* tile, float* out) {
             float dot0 = 0.0f, dot1 = 0.0f;
 #pragma unroll
-            for (int pb = 0; pb < PT / 8; ++pb) {
-                gv[pb][0] *= u0;
-                gv[pb][1] *= u0;
-                gv[pb][2] *= u1;
-                gv[pb][3] *= u1;
-            }
-#pragma unroll
             for (int nb = 0; nb < NT / 8; ++nb) {
-                gk[nb][0] *= u0;
-                gk[nb][1] *= u0;
-                gk[nb][2] *= u1;
-                gk[nb][3] *= u1;
-#pragma unroll
-                for (int s = 0; s < NS; ++s) {
-                    const uint32_t k0 = *(const uint32_t*)(tk + (s * kChunk + row) * LN + nb * 8 + 2 * lq);
-                    const uint32_t k1 = *(const uint32_t*)(tk + (s * kChunk + row + 8) * LN + nb * 8 + 2 * lq);
-                    dot0 = fmaf(low_f(k0), gk[nb][0], fmaf(high_f(k0), gk[nb][1], dot0));
-                    dot1 = fmaf(low_f(k1), gk[nb][2], fmaf(high_f(k1), gk[nb][3], dot1));
-                }
+                const float2 k0 = from_pieces<NS>(tile + row * LN + nb * 8 + 2 * lq, piece_n);
+                const float2 k1 = from_pieces<NS>(tile + (row + 8) * LN + nb * 8 + 2 * lq, piece_n);
+                dot0 = fmaf(k0.x, x[nb][0], fmaf(k0.y, x[nb][1], dot0));
+                dot1 = fmaf(k1.x, x[nb][2], fmaf(k1.y, x[nb][3], dot1));
             }
 #pragma unroll
             for (int o = 1; o < 4; o <<= 1) {
@@ -343,69 +351,39 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const __grid_constant__ B
                 dot1 += __shfl_xor_sync(kFull, dot1, o);
             }
             if (lq == 0) {
-                sm.of_k[row] = dot0;
-                sm.of_k[row + 8] = dot1;
+                out[row] = dot0;
+                out[row + 8] = dot1;
+            }
+        };
+        if (group == 0) {
+            // dv of 16 tokens, and the sums of W
+            float gv[PT / 8][4] = {};
+            gemm<NS, MS, MS, NT / 16, PT / 16, true>(gv, keys, tds, LP, piece_s, 0, 0);
+            const float u0 = sm.d.until[row], u1 = sm.d.until[row + 8];
+#pragma unroll
+            for (int pb = 0; pb < PT / 8; ++pb) {
+                gv[pb][0] *= u0;
+                gv[pb][1] *= u0;
+                gv[pb][2] *= u1;
+                gv[pb][3] *= u1;
             }
             float run[2] = {0.0f, 0.0f};                      // sums of W over the queries behind the block
 #pragma unroll 1
             for (int ib = 3; ib >= w; --ib) {
                 float at[2][4] = {}, dt[2][4] = {};
-#pragma unroll
-                for (int kk = 0; kk < NT; kk += 16) {
-                    uint32_t a[NS][4];
-#pragma unroll
-                    for (int s = 0; s < NS; ++s) load_a(a[s], tk + s * kChunk * LN, LN, w * 16, kk);
-#pragma unroll
-                    for (int u = 0; u < NS; ++u) {
-                        uint32_t b[4];
-                        load_bn(b, tq + u * kChunk * LN, LN, ib * 16, kk);
-#pragma unroll
-                        for (int s = 0; s < NS && s + u < MS; ++s) {
-                            mma(at[0], a[s], b[0], b[1]);
-                            mma(at[1], a[s], b[2], b[3]);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int kk = 0; kk < PT; kk += 16) {
-                    uint32_t a[NS][4];
-#pragma unroll
-                    for (int s = 0; s < NS; ++s) load_a(a[s], tv + s * kChunk * LP, LP, w * 16, kk);
-#pragma unroll
-                    for (int u = 0; u < NS; ++u) {
-                        uint32_t b[4];
-                        load_bn(b, ty + u * kChunk * LP, LP, ib * 16, kk);
-#pragma unroll
-                        for (int s = 0; s < NS && s + u < MS; ++s) {
-                            mma(dt[0], a[s], b[0], b[1]);
-                            mma(dt[1], a[s], b[2], b[3]);
-                        }
-                    }
-                }
+                gemm<NS, NS, kFull3, NT / 16, 1, false>(at, keys, tq, LN, piece_n, 0, ib * 16);
+                gemm<NS, NS, kFull3, PT / 16, 1, false>(dt, values, ty, LP, piece_p, 0, ib * 16);
+                decayed(at, ib, true);
                 float sum[2][2] = {};                         // of the four columns, over this warp's keys before them
-                float W[2][2][2];
-#pragma unroll
-                for (int q2 = 0; q2 < 2; ++q2)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int i = ib * 16 + q2 * 8 + 2 * lq + e;
-                        const float hi = sm.d.hi[i], lo = sm.d.lo[i];
-                        const float d0 = between(hi, lo, hi0, lo0), d1 = between(hi, lo, hi1, lo1);
-                        const float a0 = at[q2][e], a1 = at[q2][2 + e], b0 = dt[q2][e], b1 = dt[q2][2 + e];
-                        at[q2][e] = i >= row ? a0 * d0 : 0.0f;
-                        at[q2][2 + e] = i >= row + 8 ? a1 * d1 : 0.0f;
-                        dt[q2][e] = i >= row ? b0 * d0 : 0.0f;
-                        dt[q2][2 + e] = i >= row + 8 ? b1 * d1 : 0.0f;
-                        W[0][q2][e] = at[q2][e] * b0;
-                        W[1][q2][e] = at[q2][2 + e] * b1;
-                    }
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const int j = row + 8 * half;
-                    float ex[2], all[2];
+                    float W[2][2], ex[2], all[2];
 #pragma unroll
                     for (int q2 = 0; q2 < 2; ++q2) {
-                        float s = W[half][q2][0] + W[half][q2][1];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) W[q2][e] = at[q2][2 * half + e] * dt[q2][2 * half + e];
+                        float s = W[q2][0] + W[q2][1];
                         float o = __shfl_down_sync(kFull, s, 1, 4);
                         if (lq < 3) s += o;
                         o = __shfl_down_sync(kFull, s, 2, 4);
@@ -414,14 +392,14 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const __grid_constant__ B
                         ex[q2] = lq < 3 ? o : 0.0f;
                         all[q2] = __shfl_sync(kFull, s, 0, 4);
                     }
-                    float u = run[half] + ex[1] + W[half][1][1];
+                    float u = run[half] + ex[1] + W[1][1];
                     const int i = ib * 16 + 2 * lq;
                     if (j < i + 9) sum[1][1] += u;
-                    u += W[half][1][0];
+                    u += W[1][0];
                     if (j < i + 8) sum[1][0] += u;
-                    u = run[half] + all[1] + ex[0] + W[half][0][1];
+                    u = run[half] + all[1] + ex[0] + W[0][1];
                     if (j < i + 1) sum[0][1] += u;
-                    u += W[half][0][0];
+                    u += W[0][0];
                     if (j < i) sum[0][0] += u;
                     run[half] += all[1] + all[0];
                 }
@@ -435,159 +413,72 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const __grid_constant__ B
                     }
                 uint32_t a[MS][4];
                 split_a<MS>(at[0], at[1], a);
+                gemm<MS, NS, MS, 1, PT / 16, true>(gv, [&](uint32_t(&r)[4], int s, int) {
 #pragma unroll
-                for (int pb = 0; pb < PT / 16; ++pb)
-#pragma unroll
-                    for (int u = 0; u < NS; ++u) {
-                        uint32_t b[4];
-                        load_bk(b, ty + u * kChunk * LP, LP, ib * 16, pb * 16);
-#pragma unroll
-                        for (int s = 0; s < MS - u; ++s) {
-                            mma(gv[2 * pb], a[s], b[0], b[1]);
-                            mma(gv[2 * pb + 1], a[s], b[2], b[3]);
-                        }
-                    }
-                split_a<MS>(dt[0], dt[1], a);
-#pragma unroll
-                for (int nb = 0; nb < NT / 16; ++nb)
-#pragma unroll
-                    for (int u = 0; u < NS; ++u) {
-                        uint32_t b[4];
-                        load_bk(b, tq + u * kChunk * LN, LN, ib * 16, nb * 16);
-#pragma unroll
-                        for (int s = 0; s < MS - u; ++s) {
-                            mma(gk[2 * nb], a[s], b[0], b[1]);
-                            mma(gk[2 * nb + 1], a[s], b[2], b[3]);
-                        }
-                    }
+                    for (int e = 0; e < 4; ++e) r[e] = a[s][e];
+                }, ty, LP, piece_p, ib * 16, 0);
             }
+            const RowsOut<T> ov{dv + t * v_st, nullptr, v_st};
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int r = row + 8 * half;
-                if (r < rows) {
-                    RowsOut<T> ov{dv, nullptr, v_st};
+            for (int half = 0; half < 2; ++half)
+                if (row + 8 * half < rows)
 #pragma unroll
-                    for (int pb = 0; pb < PT / 8; ++pb) ov.put2(t + r, pb * 8 + 2 * lq, cols, gv[pb][2 * half], gv[pb][2 * half + 1], pair_v);
-#pragma unroll
-                    for (int nb = 0; nb < NT / 8; ++nb)
-                        dk.put2(row_at + t + r, nb * 8 + 2 * lq, z.n, gk[nb][2 * half], gk[nb][2 * half + 1], pair_qk);
-                }
-            }
-        }
-        // ---- as queries
-        {
-            float gq[NT / 8][4] = {};
-#pragma unroll
-            for (int kk = 0; kk < PT; kk += 16) {
-                uint32_t a[NS][4];
-#pragma unroll
-                for (int s = 0; s < NS; ++s) load_a(a[s], ty + s * kChunk * LP, LP, w * 16, kk);
-#pragma unroll
-                for (int nb = 0; nb < NT / 16; ++nb)
-#pragma unroll
-                    for (int u = 0; u < MS; ++u) {
-                        uint32_t b[4];
-                        load_bn(b, ts + u * NT * LP, LP, nb * 16, kk);
-#pragma unroll
-                        for (int s = 0; s < NS && s + u < MS; ++s) {
-                            mma(gq[2 * nb], a[s], b[0], b[1]);
-                            mma(gq[2 * nb + 1], a[s], b[2], b[3]);
-                        }
-                    }
-            }
-            const float e0 = sm.d.since[row], e1 = sm.d.since[row + 8];
-            float dot0 = 0.0f, dot1 = 0.0f;
+                    for (int pb = 0; pb < PT / 8; ++pb)
+                        ov.put2(row + 8 * half, pb * 8 + 2 * lq, cols, gv[pb][2 * half], gv[pb][2 * half + 1], pair_v);
+        } else {
+            // dk (rows as keys) and dq (rows as queries) are one form:  (dP o D) X + decay (V or dY) times the state's
+            // gradient or the state; the far part's dot with the row itself is its share of dg
+            const bool as_keys = group == 1;
+            float gx[NT / 8][4] = {};
+            const bf16* const own = as_keys ? tv : ty;
+            const bf16* const other = as_keys ? ty : tv;
+            const bf16* const mate = as_keys ? tq : tk;
+            auto lines = [&](uint32_t(&a)[4], int s, int kk) { load_a(a, own + s * piece_p, LP, w * 16, kk * 16); };
+            gemm<NS, kFull3, kFull3, PT / 16, NT / 16, false>(gx, lines, as_keys ? tds : ts, LP, piece_s, 0, 0);
+            const float* decay = as_keys ? sm.d.until : sm.d.since;
+            const float u0 = decay[row], u1 = decay[row + 8];
 #pragma unroll
             for (int nb = 0; nb < NT / 8; ++nb) {
-                gq[nb][0] *= e0;
-                gq[nb][1] *= e0;
-                gq[nb][2] *= e1;
-                gq[nb][3] *= e1;
-#pragma unroll
-                for (int s = 0; s < NS; ++s) {
-                    const uint32_t q0 = *(const uint32_t*)(tq + (s * kChunk + row) * LN + nb * 8 + 2 * lq);
-                    const uint32_t q1 = *(const uint32_t*)(tq + (s * kChunk + row + 8) * LN + nb * 8 + 2 * lq);
-                    dot0 = fmaf(low_f(q0), gq[nb][0], fmaf(high_f(q0), gq[nb][1], dot0));
-                    dot1 = fmaf(low_f(q1), gq[nb][2], fmaf(high_f(q1), gq[nb][3], dot1));
-                }
+                gx[nb][0] *= u0;
+                gx[nb][1] *= u0;
+                gx[nb][2] *= u1;
+                gx[nb][3] *= u1;
             }
-#pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
-                dot0 += __shfl_xor_sync(kFull, dot0, o);
-                dot1 += __shfl_xor_sync(kFull, dot1, o);
-            }
-            if (lq == 0) {
-                sm.of_q[row] = dot0;
-                sm.of_q[row + 8] = dot1;
-            }
+            dots(gx, as_keys ? tk : tq, as_keys ? sm.of_k : sm.of_q);
+            const int from = as_keys ? w : 0, to = as_keys ? 4 : w + 1;
 #pragma unroll 1
-            for (int jb = 0; jb <= w; ++jb) {
+            for (int b = from; b < to; ++b) {
                 float dt[2][4] = {};
-#pragma unroll
-                for (int kk = 0; kk < PT; kk += 16) {
-                    uint32_t a[NS][4];
-#pragma unroll
-                    for (int s = 0; s < NS; ++s) load_a(a[s], ty + s * kChunk * LP, LP, w * 16, kk);
-#pragma unroll
-                    for (int u = 0; u < NS; ++u) {
-                        uint32_t b[4];
-                        load_bn(b, tv + u * kChunk * LP, LP, jb * 16, kk);
-#pragma unroll
-                        for (int s = 0; s < NS && s + u < MS; ++s) {
-                            mma(dt[0], a[s], b[0], b[1]);
-                            mma(dt[1], a[s], b[2], b[3]);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int q2 = 0; q2 < 2; ++q2)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int j = jb * 16 + q2 * 8 + 2 * lq + e;
-                        const float hj = sm.d.hi[j], lj = sm.d.lo[j];
-                        dt[q2][e] = j <= row ? dt[q2][e] * between(hi0, lo0, hj, lj) : 0.0f;
-                        dt[q2][2 + e] = j <= row + 8 ? dt[q2][2 + e] * between(hi1, lo1, hj, lj) : 0.0f;
-                    }
+                gemm<NS, NS, MS, PT / 16, 1, false>(dt, lines, other, LP, piece_p, 0, b * 16);
+                decayed(dt, b, as_keys);
                 uint32_t a[MS][4];
                 split_a<MS>(dt[0], dt[1], a);
+                gemm<MS, NS, MS, 1, NT / 16, true>(gx, [&](uint32_t(&r)[4], int s, int) {
 #pragma unroll
-                for (int nb = 0; nb < NT / 16; ++nb)
-#pragma unroll
-                    for (int u = 0; u < NS; ++u) {
-                        uint32_t b[4];
-                        load_bk(b, tk + u * kChunk * LN, LN, jb * 16, nb * 16);
-#pragma unroll
-                        for (int s = 0; s < MS - u; ++s) {
-                            mma(gq[2 * nb], a[s], b[0], b[1]);
-                            mma(gq[2 * nb + 1], a[s], b[2], b[3]);
-                        }
-                    }
+                    for (int e = 0; e < 4; ++e) r[e] = a[s][e];
+                }, mate, LN, piece_n, b * 16, 0);
             }
+            const RowsOut<T>& out = as_keys ? dk : dq;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int r = row + 8 * half;
-                if (r < rows)
+            for (int half = 0; half < 2; ++half)
+                if (row + 8 * half < rows)
 #pragma unroll
                     for (int nb = 0; nb < NT / 8; ++nb)
-                        dq.put2(row_at + t + r, nb * 8 + 2 * lq, z.n, gq[nb][2 * half], gq[nb][2 * half + 1], pair_qk);
-            }
+                        out.put2(row_at + t + row + 8 * half, nb * 8 + 2 * lq, z.n, gx[nb][2 * half], gx[nb][2 * half + 1], pair_qk);
         }
-        ds.template advance<NS, MS>(tq, ty, sm.d.since, sm.d.whole);
     }
     __syncthreads();
-    if (pending && w == 0) finish_dg(0);
-    if (it.first) ds.store(p.dh0 + ((int64_t)it.seq * z.heads + h) * np + col, z.n, z.p - col, z.p);
 }
 
 template <typename T, int NT, int PT>
 bcm_status launch_bwd(const BwdArgs& p, cudaStream_t stream) {
     using Smem = BwdSmem<T, NT, PT>;
     static_assert(sizeof(Smem) <= 227 * 1024, "shared memory of a block");
-    static_assert(sizeof(typename Smem::Tiles) >= sizeof(float) * (NT * PT + 4 * NT + kThreads + 4), "the state of back_tokens");
+    static_assert(sizeof(typename Smem::Tiles) >= sizeof(float) * (NT * PT + 4 * NT + kBwdThreads + kBwdThreads / 32), "the state of back_tokens");
     auto kernel = bwd_kernel<T, NT, PT>;
     bcm_status st = allow_smem(kernel, sizeof(Smem));
     if (st != BCM_OK) return st;
-    kernel<<<(unsigned)(p.z.items * p.z.heads * p.z.slices), kThreads, sizeof(Smem), stream>>>(p);
+    kernel<<<(unsigned)(p.z.items * p.z.heads * p.z.slices), kBwdThreads, sizeof(Smem), stream>>>(p);
     BCM_LAUNCH_CHECK();
     return BCM_OK;
 }

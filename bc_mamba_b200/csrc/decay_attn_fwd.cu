@@ -181,22 +181,27 @@ struct FwdArgs {
     float* ckpt;               // [chunks][heads][n][p] states that enter each chunk, or NULL
 };
 
+// Warps 0 to 3 form the outputs of 16 tokens each, warps 4 to 7 hold the state and advance it meanwhile.  Where there is
+// room for it the pieces of the next chunk's entering state go to a second buffer.
+constexpr int kFwdThreads = 256;
+
 template <typename T, int NT, int PT>
 struct FwdSmem {
-    static constexpr int NS = Pieces<T>::in, MS = Pieces<T>::mid;
+    static constexpr int NS = Pieces<T>::in, MS = Pieces<T>::out;
     struct Tiles {
         bf16 q[NS][kChunk][NT + 8], k[NS][kChunk][NT + 8], v[NS][kChunk][PT + 8];
     } tiles;
-    bf16 s[MS][NT][PT + 8];
+    static constexpr int buffers = sizeof(Tiles) + 2 * sizeof(bf16[MS][NT][PT + 8]) <= 110 * 1024 ? 2 : 1;
+    bf16 s[buffers][MS][NT][PT + 8];
     Decays d;
 };
 
 // A chunk with a value that is not finite, token by token: 0 times such a value would spread it to tokens before it.
-// `s` (shared, NT x PT) holds the state before and after, `sum` 128 floats.
+// `s` (shared, NT x PT) holds the state before and after, `sum` a float for each thread.
 template <typename T, int NT, int PT>
 __device__ __noinline__ void walk_tokens(const FwdArgs& p, const T* q, const T* k, const T* v, const float* g, T* y, int rows, int cols,
                                          float* s, float* sum) {
-    constexpr int parts = kThreads / PT;
+    constexpr int parts = kFwdThreads / PT;
     const int c = threadIdx.x % PT, part = threadIdx.x / PT;
     for (int t = 0; t < rows; ++t) {
         const float a = expf(g[(int64_t)t * p.g_st]), x = c < cols ? to_f32(v[(int64_t)t * p.v.st + c]) : 0.0f;
@@ -217,10 +222,11 @@ __device__ __noinline__ void walk_tokens(const FwdArgs& p, const T* q, const T* 
 }
 
 template <typename T, int NT, int PT>
-__global__ void __launch_bounds__(kThreads) fwd_kernel(const __grid_constant__ FwdArgs p) {
+__global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT, PT>::buffers) fwd_kernel(const __grid_constant__ FwdArgs p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    FwdSmem<T, NT, PT>& sm = *(FwdSmem<T, NT, PT>*)smem_raw;
-    constexpr int NS = Pieces<T>::in, MS = Pieces<T>::mid, LN = NT + 8, LP = PT + 8;
+    using Smem = FwdSmem<T, NT, PT>;
+    Smem& sm = *(Smem*)smem_raw;
+    constexpr int NS = Smem::NS, MS = Smem::MS, LN = NT + 8, LP = PT + 8;
     const Sizes& z = p.z;
     const int across = z.heads * z.slices;
     const int item = blockIdx.x / across, hs = blockIdx.x % across, h = hs / z.slices, col = hs % z.slices * PT;
@@ -238,88 +244,98 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const __grid_constant__ F
     const bool vq = on_16(q, p.q.st), vk = on_16(k, p.k.st), vv = on_16(v, p.v.st);
     const bool pair_y = (((uintptr_t)y | (uintptr_t)(y_st * sizeof(T))) & (2 * sizeof(T) - 1)) == 0;
     const int np = z.n * z.p;
-    State<NT, PT> st;
-    const float* from = it.first ? (p.h0 ? p.h0 + ((int64_t)it.seq * z.heads + h) * np : nullptr)
-                                 : p.enter + ((int64_t)item * z.heads + h) * np;
-    if (from) st.load(from + col, z.n, z.p - col, z.p);
-    else st.zero();
     const int len = it.t1 - it.t0, nc = (len + kChunk - 1) / kChunk;
-    const int l = lane_id(), w = threadIdx.x >> 5, row = w * 16 + (l >> 2);
+    const int l = lane_id(), w = (threadIdx.x >> 5) & 3, row = w * 16 + (l >> 2);
+    const bool state_warp = threadIdx.x >= 128, decay_warp = threadIdx.x >= 128 && threadIdx.x < 160;
     bf16* const tq = &sm.tiles.q[0][0][0];
     bf16* const tk = &sm.tiles.k[0][0][0];
     bf16* const tv = &sm.tiles.v[0][0][0];
-    bf16* const ts = &sm.s[0][0][0];
+
+    Pending<T, kChunk, NT, kFwdThreads> pq, pk;
+    Pending<T, kChunk, PT, kFwdThreads> pv;
+    float g0 = 0.0f, g1 = 0.0f;
+    auto fetch = [&](int c) {
+        const int t = c * kChunk, rows = min(kChunk, len - t);
+        pq.fetch(q + t * p.q.st, p.q.st, rows, z.n, vq);
+        pk.fetch(k + t * p.k.st, p.k.st, rows, z.n, vk);
+        pv.fetch(v + t * p.v.st, p.v.st, rows, cols, vv);
+        if (decay_warp) {
+            g0 = 2 * l < rows ? g[(int64_t)(t + 2 * l) * p.g_st] : 0.0f;
+            g1 = 2 * l + 1 < rows ? g[(int64_t)(t + 2 * l + 1) * p.g_st] : 0.0f;
+        }
+    };
+    // the tiles of the fetched chunk; whether a value was not finite
+    auto put = [&]() {
+        bool bad = pq.put(tq, LN);
+        bad |= pk.put(tk, LN);
+        bad |= pv.put(tv, LP);
+        if (decay_warp) {
+            bad |= !(g0 <= 3.38e38f && g1 <= 3.38e38f);
+            decays_of(sm.d, g0, g1);
+        }
+        return bad;
+    };
+    // token by token, the state through shared memory
+    auto walk = [&](int c) {
+        const int t = c * kChunk;
+        float* f = (float*)&sm.tiles;
+        walk_tokens<T, NT, PT>(p, q + t * p.q.st, k + t * p.k.st, v + t * p.v.st, g + t * p.g_st, y + t * y_st, min(kChunk, len - t), cols, f,
+                               f + NT * PT);
+    };
+    if (nc > 0) fetch(0);
+
+    if (state_warp) {
+        State<NT, PT> st;
+        const float* from = it.first ? (p.h0 ? p.h0 + ((int64_t)it.seq * z.heads + h) * np : nullptr)
+                                     : p.enter + ((int64_t)item * z.heads + h) * np;
+        if (from) st.load(from + col, z.n, z.p - col, z.p);
+        else st.zero();
+        bool bad = false;
+        if (Smem::buffers > 1) bad = st.template put<MS>(&sm.s[0][0][0][0]);
+        for (int c = 0; c < nc; ++c) {
+            if (p.ckpt) st.store(p.ckpt + ((int64_t)(it.chunk + c) * z.heads + h) * np + col, z.n, z.p - col, z.p);
+            __syncthreads();
+            bad |= put();
+            if (Smem::buffers == 1) bad |= st.template put<MS>(&sm.s[0][0][0][0]);
+            const bool slow = __syncthreads_or(bad);
+            if (c + 1 < nc) fetch(c + 1);
+            if (slow) {
+                float* f = (float*)&sm.tiles;
+                st.pairs([&](float& x, float& x1, int r, int cc) {
+                    f[r * PT + cc] = x;
+                    f[r * PT + cc + 1] = x1;
+                });
+                __syncthreads();
+                walk(c);
+                st.pairs([&](float& x, float& x1, int r, int cc) {
+                    x = f[r * PT + cc];
+                    x1 = f[r * PT + cc + 1];
+                });
+            } else {
+                st.template advance<NS>(tk, tv, sm.d.until, sm.d.whole);
+            }
+            bad = false;
+            if (Smem::buffers > 1) bad = st.template put<MS>(&sm.s[(c + 1) % Smem::buffers][0][0][0]);
+        }
+        if (it.last) st.store(p.h_last + ((int64_t)it.seq * z.heads + h) * np + col, z.n, z.p - col, z.p);
+        return;
+    }
     for (int c = 0; c < nc; ++c) {
         const int t = c * kChunk, rows = min(kChunk, len - t);
-        bool bad = false;
-        {
-            Pending<T, NT> pq, pk;
-            Pending<T, PT> pv;
-            pq.fetch(q + t * p.q.st, p.q.st, rows, z.n, vq);
-            pk.fetch(k + t * p.k.st, p.k.st, rows, z.n, vk);
-            pv.fetch(v + t * p.v.st, p.v.st, rows, cols, vv);
-            float g0 = 0.0f, g1 = 0.0f;
-            if (w == 0) {
-                if (2 * l < rows) g0 = g[(int64_t)(t + 2 * l) * p.g_st];
-                if (2 * l + 1 < rows) g1 = g[(int64_t)(t + 2 * l + 1) * p.g_st];
-                bad = !(g0 <= 3.4028234e38f && g1 <= 3.4028234e38f);
-            }
-            if (p.ckpt) st.store(p.ckpt + ((int64_t)(it.chunk + c) * z.heads + h) * np + col, z.n, z.p - col, z.p);
-            __syncthreads();                                  // the chunk before is done with the tiles
-            if (w == 0) decays_of(sm.d, g0, g1);
-            bad |= st.template put<MS>(ts);
-            bad |= pq.put(tq, LN, kChunk);
-            bad |= pk.put(tk, LN, kChunk);
-            bad |= pv.put(tv, LP, kChunk);
-        }
-        if (__syncthreads_or(bad)) {
-            float* f = (float*)&sm.tiles;
-            st.pairs([&](float& x, float& x1, int r, int cc) {
-                f[r * PT + cc] = x;
-                f[r * PT + cc + 1] = x1;
-            });
+        __syncthreads();                                      // the chunk before is done with the tiles
+        const bool bad = put();
+        const bool slow = __syncthreads_or(bad);
+        if (c + 1 < nc) fetch(c + 1);
+        if (slow) {
             __syncthreads();
-            walk_tokens<T, NT, PT>(p, q + t * p.q.st, k + t * p.k.st, v + t * p.v.st, g + t * p.g_st, y + t * y_st, rows, cols, f, f + NT * PT);
-            st.pairs([&](float& x, float& x1, int r, int cc) {
-                x = f[r * PT + cc];
-                x1 = f[r * PT + cc + 1];
-            });
+            walk(c);
             continue;
         }
-        // this warp's 16 queries: products with the keys up to their own, and with the entering state
-        float sc[kChunk / 8][4] = {}, acc[PT / 8][4] = {};
-#pragma unroll
-        for (int kk = 0; kk < NT; kk += 16) {
-            uint32_t qa[NS][4];
-#pragma unroll
-            for (int s = 0; s < NS; ++s) load_a(qa[s], tq + s * kChunk * LN, LN, w * 16, kk);
-#pragma unroll
-            for (int jb = 0; jb < 4; ++jb)
-                if (jb <= w) {
-#pragma unroll
-                    for (int u = 0; u < NS; ++u) {
-                        uint32_t b[4];
-                        load_bn(b, tk + u * kChunk * LN, LN, jb * 16, kk);
-#pragma unroll
-                        for (int s = 0; s < NS && s + u < MS; ++s) {
-                            mma(sc[2 * jb], qa[s], b[0], b[1]);
-                            mma(sc[2 * jb + 1], qa[s], b[2], b[3]);
-                        }
-                    }
-                }
-#pragma unroll
-            for (int pb = 0; pb < PT / 16; ++pb)
-#pragma unroll
-                for (int u = 0; u < MS; ++u) {
-                    uint32_t b[4];
-                    load_bk(b, ts + u * NT * LP, LP, kk, pb * 16);
-#pragma unroll
-                    for (int s = 0; s < NS && s + u < MS; ++s) {
-                        mma(acc[2 * pb], qa[s], b[0], b[1]);
-                        mma(acc[2 * pb + 1], qa[s], b[2], b[3]);
-                    }
-                }
-        }
+        // 16 queries: the entering state's part, then those of the keys up to their own
+        float acc[PT / 8][4] = {};
+        const bf16* ts = &sm.s[c % Smem::buffers][0][0][0];
+        auto queries = [&](uint32_t(&a)[4], int s, int kk) { load_a(a, tq + s * kChunk * LN, LN, w * 16, kk * 16); };
+        gemm<NS, MS, MS, NT / 16, PT / 16, true>(acc, queries, ts, LP, NT * LP, 0, 0);
         const float since0 = sm.d.since[row], since1 = sm.d.since[row + 8];
 #pragma unroll
         for (int pb = 0; pb < PT / 8; ++pb) {
@@ -329,35 +345,26 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const __grid_constant__ F
             acc[pb][3] *= since1;
         }
         const float hi0 = sm.d.hi[row], lo0 = sm.d.lo[row], hi1 = sm.d.hi[row + 8], lo1 = sm.d.lo[row + 8];
+#pragma unroll 1
+        for (int jb = 0; jb <= w; ++jb) {
+            float sc[2][4] = {};
+            gemm<NS, NS, MS, NT / 16, 1, false>(sc, queries, tk, LN, kChunk * LN, 0, jb * 16);
 #pragma unroll
-        for (int jb = 0; jb < 4; ++jb)
-            if (jb <= w) {
-#pragma unroll
-                for (int q2 = 0; q2 < 2; ++q2)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int j = jb * 16 + q2 * 8 + 2 * (l & 3) + e;
-                        const float hj = sm.d.hi[j], lj = sm.d.lo[j];
-                        float(&x)[4] = sc[2 * jb + q2];
-                        x[e] = j <= row ? x[e] * between(hi0, lo0, hj, lj) : 0.0f;
-                        x[2 + e] = j <= row + 8 ? x[2 + e] * between(hi1, lo1, hj, lj) : 0.0f;
-                    }
-                uint32_t a[MS][4];
-                split_a<MS>(sc[2 * jb], sc[2 * jb + 1], a);
-#pragma unroll
-                for (int pb = 0; pb < PT / 16; ++pb)
-#pragma unroll
-                    for (int u = 0; u < NS; ++u) {
-                        uint32_t b[4];
-                        load_bk(b, tv + u * kChunk * LP, LP, jb * 16, pb * 16);
-#pragma unroll
-                        for (int s = 0; s < MS - u; ++s) {
-                            mma(acc[2 * pb], a[s], b[0], b[1]);
-                            mma(acc[2 * pb + 1], a[s], b[2], b[3]);
-                        }
-                    }
+            for (int q2 = 0; q2 < 2; ++q2) {
+                const int j = jb * 16 + q2 * 8 + 2 * (l & 3);
+                const float2 hj = *(const float2*)&sm.d.hi[j], lj = *(const float2*)&sm.d.lo[j];
+                sc[q2][0] = j <= row ? sc[q2][0] * between(hi0, lo0, hj.x, lj.x) : 0.0f;
+                sc[q2][1] = j + 1 <= row ? sc[q2][1] * between(hi0, lo0, hj.y, lj.y) : 0.0f;
+                sc[q2][2] = j <= row + 8 ? sc[q2][2] * between(hi1, lo1, hj.x, lj.x) : 0.0f;
+                sc[q2][3] = j + 1 <= row + 8 ? sc[q2][3] * between(hi1, lo1, hj.y, lj.y) : 0.0f;
             }
-        st.template advance<NS, MS>(tk, tv, sm.d.until, sm.d.whole);
+            uint32_t a[MS][4];
+            split_a<MS>(sc[0], sc[1], a);
+            gemm<MS, NS, MS, 1, PT / 16, true>(acc, [&](uint32_t(&r)[4], int s, int) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) r[e] = a[s][e];
+            }, tv, LP, kChunk * LP, jb * 16, 0);
+        }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int r = row + 8 * half;
@@ -378,17 +385,17 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const __grid_constant__ F
             }
         }
     }
-    if (it.last) st.store(p.h_last + ((int64_t)it.seq * z.heads + h) * np + col, z.n, z.p - col, z.p);
 }
 
 template <typename T, int NT, int PT>
 bcm_status launch_fwd(const FwdArgs& p, cudaStream_t stream) {
     constexpr size_t smem = sizeof(FwdSmem<T, NT, PT>);
-    static_assert(sizeof(typename FwdSmem<T, NT, PT>::Tiles) >= sizeof(float) * (NT * PT + kThreads), "the state of walk_tokens");
+    static_assert(smem <= 227 * 1024, "shared memory of a block");
+    static_assert(sizeof(typename FwdSmem<T, NT, PT>::Tiles) >= sizeof(float) * (NT * PT + kFwdThreads), "the state of walk_tokens");
     auto kernel = fwd_kernel<T, NT, PT>;
     bcm_status st = allow_smem(kernel, smem);
     if (st != BCM_OK) return st;
-    kernel<<<(unsigned)(p.z.items * p.z.heads * p.z.slices), kThreads, smem, stream>>>(p);
+    kernel<<<(unsigned)(p.z.items * p.z.heads * p.z.slices), kFwdThreads, smem, stream>>>(p);
     BCM_LAUNCH_CHECK();
     return BCM_OK;
 }

@@ -1,24 +1,26 @@
-// decay_attn.cuh — what the kernels of the linear attention with a decay for each head share: tiles in shared memory,
-// their matrix products, the decays' running sums, and the work items that sequences are cut into.
+// decay_attn.cuh — what the kernels of the linear attention with a decay for each head share: tiles and their products,
+// the decays' running sums, the state, and the work items that sequences are cut into.
 //
 // Per head, a_t = exp(g_t):  S_t = a_t S_(t-1) + k_t v_t^T (N x P),  y_t = S_t^T q_t.
 // In chunks of 64 tokens with G the running sum of g inside the chunk, D_ij = exp(G_i - G_j) for j <= i, 0 elsewhere:
 //   Y = ((Q K^T) o D) V + diag(exp G) Q S_in,    S_out = exp(G_64) S_in + sum_j exp(G_64 - G_j) k_j v_j^T.
+// All products are of 64 rows and run on the tensor cores; a block walks the chunks of its item, 64 columns of the
+// values wide.
 //
-// Numbers.  The products run on the tensor cores in bf16 with fp32 sums.  An operand of more bits is a sum of bf16
-// pieces, each the rounding of what the pieces before it left: float32 is three pieces (exact), float16 two (exact),
-// and what a kernel computes itself (masked scores, states, keys times decays) has as many as its products need: two
-// (relative 2^-18) where they end in 16 bits, three where they end in float32.  Of the pieces' products those whose
-// weight lies below that are left out, and the small ones are added up first: the tensor cores cut sums off instead of
-// rounding them, so that only few additions may be made at the full sum.  States are float32 between chunks.  G is
-// summed in float64 and kept as two floats, so that a difference of two of its values keeps full precision after a
-// decay of any size.
+// Numbers.  The products are of bf16 with fp32 sums.  An operand of more bits is a sum of bf16 pieces, each the rounding
+// of what the pieces before it left: float32 is three pieces (exact), float16 two (exact), and what a kernel computes
+// itself (masked scores, states, values times decays) has as many as its products need: two (relative 2^-18) where
+// they end in 16 bits, three where they end in float32.  Of the pieces' products those whose weight lies below that are
+// left out, and the small ones are added up first: the tensor cores cut sums off instead of rounding them, so that few
+// additions may be made at the full sum.  States are float32 between chunks.  G is summed in float64 and kept as two
+// floats, so that a difference of two of its values keeps full precision after a decay of any size.
 #pragma once
 
 #include <algorithm>
 #include <type_traits>
 
 #include "common.cuh"
+#include "tensor5.cuh"
 
 namespace bcm {
 namespace decay_attn {
@@ -26,6 +28,7 @@ namespace decay_attn {
 using bf16 = __nv_bfloat16;
 
 constexpr int kChunk = 64;
+constexpr int kP = 64;        // columns of the values that a block takes
 
 // pieces of an input, and of what is computed for products that end in T; for those that end in float32 there are three
 template <typename T> struct Pieces;
@@ -34,50 +37,14 @@ template <> struct Pieces<__half> { static constexpr int in = 2, out = 2; };
 template <> struct Pieces<bf16> { static constexpr int in = 1, out = 2; };
 constexpr int kFull3 = 3;
 
-// ------------------------------------------------------------ matrix products ----
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const bf16* p) {
-    const uint32_t s = (uint32_t)__cvta_generic_to_shared(p);
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s) : "memory");
-}
-
-__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const bf16* p) {
-    const uint32_t s = (uint32_t)__cvta_generic_to_shared(p);
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s) : "memory");
-}
-
-// A of 16 rows x 16: stored by rows
-__device__ __forceinline__ void load_a(uint32_t (&r)[4], const bf16* m, int ld, int row, int col) {
-    const int l = lane_id();
-    ldsm4(r, m + (row + (l & 15)) * ld + col + 8 * (l >> 4));
-}
-// A of 16 rows x 16, stored transposed (m[k][row])
-__device__ __forceinline__ void load_at(uint32_t (&r)[4], const bf16* m, int ld, int row, int k) {
-    const int l = lane_id();
-    ldsm4t(r, m + (k + (l & 7) + 8 * (l >> 4)) * ld + row + 8 * ((l >> 3) & 1));
-}
-// B of 16 (k) x 16 (n), stored m[n][k]: r[0], r[1] the first eight n, r[2], r[3] the others
-__device__ __forceinline__ void load_bn(uint32_t (&r)[4], const bf16* m, int ld, int n, int k) {
-    const int l = lane_id();
-    ldsm4(r, m + (n + (l & 7) + 8 * (l >> 4)) * ld + k + 8 * ((l >> 3) & 1));
-}
-// B of 16 (k) x 16 (n), stored m[k][n]
-__device__ __forceinline__ void load_bk(uint32_t (&r)[4], const bf16* m, int ld, int k, int n) {
-    const int l = lane_id();
-    ldsm4t(r, m + (k + (l & 15)) * ld + n + 8 * (l >> 4));
-}
-// B of 32 (k) x 8 (n), stored m[k][n]: r[0], r[1] the first sixteen k, r[2], r[3] the others
-__device__ __forceinline__ void load_bk32(uint32_t (&r)[4], const bf16* m, int ld, int k, int n) {
-    ldsm4t(r, m + (k + lane_id()) * ld + n);
-}
+// Tiles of 64 rows and NT columns (of queries, keys, states): one of up to 64 columns, or two of 64
+template <int NT>
+struct Wide {
+    static constexpr int W = NT < 64 ? NT : 64;
+    using Tile = t5::Tile<W>;
+    static constexpr int elements = 64 * NT, bytes = 2 * elements;     // of a piece
+    __device__ __forceinline__ static int at(int row, int col) { return col / W * Tile::elements + Tile::at(row, col % W); }
+};
 
 __device__ __forceinline__ float low_f(uint32_t r) { return __uint_as_float(r << 16); }
 __device__ __forceinline__ float high_f(uint32_t r) { return __uint_as_float(r & 0xffff0000u); }
@@ -94,55 +61,9 @@ __device__ __forceinline__ void split(float x, float y, uint32_t (&r)[M]) {
 #pragma unroll
     for (int m = 0; m < M; ++m) {
         r[m] = pack(x, y);
-        x -= low_f(r[m]);
-        y -= high_f(r[m]);
-    }
-}
-
-// the four registers of an A operand as M pieces, from the two accumulator tiles that cover its 16 columns
-template <int M>
-__device__ __forceinline__ void split_a(const float (&c0)[4], const float (&c1)[4], uint32_t (&a)[M][4]) {
-    uint32_t r[M];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const float(&c)[4] = q < 2 ? c0 : c1;
-        split<M>(c[2 * (q & 1)], c[2 * (q & 1) + 1], r);
-#pragma unroll
-        for (int m = 0; m < M; ++m) a[m][q] = r[m];
-    }
-}
-
-// acc[2 i], acc[2 i + 1] += A B over K16 steps of 16 and the N16 blocks of 16 columns.  la(regs, piece, step) loads A's
-// NA pieces; B's NB pieces lie `piece` elements apart, stored m[k][n] (BK) or m[n][k].  Products (s, u) of pieces with
-// s + u < D.  With many products to a step all but the largest go in a pass of their own.
-template <int NA, int NB, int D, int K16, int N16, bool BK, typename LA>
-__device__ __forceinline__ void gemm(float (&acc)[2 * N16][4], LA&& la, const bf16* b, int ldb, int piece, int k0, int n0) {
-    constexpr bool two = NA * NB > 4;
-#pragma unroll
-    for (int pass = two ? 0 : 1; pass < 2; ++pass) {
-#pragma unroll
-        for (int kk = 0; kk < K16; ++kk) {
-            uint32_t a[NA][4];
-#pragma unroll
-            for (int s = 0; s < NA; ++s)
-                if (!(two && pass == 1 && s > 0)) la(a[s], s, kk);
-#pragma unroll
-            for (int nb = 0; nb < N16; ++nb)
-#pragma unroll
-                for (int u = NB - 1; u >= 0; --u) {
-                    if (two && pass == 1 && u > 0) continue;
-                    if (u >= D) continue;
-                    uint32_t r[4];
-                    if (BK) load_bk(r, b + u * piece, ldb, k0 + kk * 16, n0 + nb * 16);
-                    else load_bn(r, b + u * piece, ldb, n0 + nb * 16, k0 + kk * 16);
-#pragma unroll
-                    for (int s = NA - 1; s >= 0; --s) {
-                        if (s + u >= D) continue;
-                        if (two && (pass == 1) != (s + u == 0)) continue;
-                        mma(acc[2 * nb], a[s], r[0], r[1]);
-                        mma(acc[2 * nb + 1], a[s], r[2], r[3]);
-                    }
-                }
+        if (m + 1 < M) {
+            x -= low_f(r[m]);
+            y -= high_f(r[m]);
         }
     }
 }
@@ -152,6 +73,41 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+// --------------------------------------------------------------------- products ----
+// An operand of NT columns at a shared address, its pieces one behind the other; K: columns along the sum, else rows.
+template <int NT, bool K>
+struct Operand {
+    using X = Wide<NT>;
+    uint32_t addr;
+    __device__ __forceinline__ uint64_t desc(int piece, int step) const {
+        constexpr int in_tile = X::W / 16;
+        const uint32_t off = piece * X::bytes + (K ? step / in_tile * X::Tile::bytes + step % in_tile * X::Tile::step_k : step * X::Tile::step_mn);
+        return X::Tile::desc(addr + off, X::Tile::bytes);
+    }
+};
+
+// d (+)= A B over `steps` of 16, products (s, u) of A's NA and B's NB pieces with s + u < D, small ones first; one thread.
+// a(s, step), b(u, step): descriptors (or A's address in tensor memory)
+template <int NA, int NB, int D, typename FA, typename FB>
+__device__ __forceinline__ void products(uint32_t d, FA&& a, FB&& b, int steps, uint32_t idesc, bool add) {
+#pragma unroll
+    for (int order = (NA + NB - 2 < D - 1 ? NA + NB - 2 : D - 1); order >= 0; --order)
+#pragma unroll
+        for (int s = 0; s < NA; ++s) {
+            const int u = order - s;
+            if (u < 0 || u >= NB) continue;
+#pragma unroll 1
+            for (int k = 0; k < steps; ++k) {
+                const auto x = a(s, k);
+                if constexpr (sizeof(x) == 4) t5::mma_ts(d, x, b(u, k), idesc, add);
+                else t5::mma_ss(d, x, b(u, k), idesc, add);
+                add = true;
+            }
+        }
+}
+
+__device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 // ------------------------------------------------------------------- decays ----
 // Of one chunk: the running sums of g log2(e) as two floats, what has decayed since the chunk's start and what will
@@ -211,8 +167,8 @@ struct Tables {               // of a packed batch, in the workspace
 struct Sizes {
     int batch, heads, qk_heads, n, p, seqlen;
     int span, items, per_seq; // items in all (packed: at most), per sequence (dense)
-    int chunks;               // kept states in all (packed: at most)
-    int slices;               // of PT columns of the values
+    int chunks;               // kept states of a head in all (packed: at most)
+    int slices;               // of kP columns of the values
     const int32_t* cu;
     Tables tables;
 };
@@ -247,57 +203,109 @@ __device__ __forceinline__ bool not_finite(float v) { return !(fabsf(v) <= 3.38e
 
 template <typename T> struct alignas(16) Eight { T v[8]; };
 
-// A tile of R rows x W columns on its way to shared memory: each of TH threads has groups of eight columns.  Rows and
-// columns behind the last are 0.
-template <typename T, int R, int W, int TH>
+// 64 rows x W columns on their way to shared memory: each of TH threads has groups of eight columns.  Rows and columns
+// behind the last are 0.
+template <typename T, int W, int TH>
 struct Pending {
-    static constexpr int all = R * W / 8, n = (all + TH - 1) / TH;
+    static constexpr int all = 64 * W / 8, n = (all + TH - 1) / TH;
     Eight<T> g[n];
 
-    __device__ __forceinline__ void fetch(const T* src, int64_t stride, int rows, int cols, bool vec) {
+    __device__ __forceinline__ static int row(int i) { return (threadIdx.x + i * TH) / (W / 8); }
+    __device__ __forceinline__ static int col(int i) { return (threadIdx.x + i * TH) % (W / 8) * 8; }
+
+    // how: elements at a time that the rows' alignment allows (8, 2 or 1)
+    __device__ __forceinline__ void fetch(const T* src, int64_t stride, int rows, int cols, int how) {
+        if (how == 8) {
+#pragma unroll
+            for (int i = 0; i < n; ++i) {
+                const T* p = src + row(i) * stride + col(i);
+                if (row(i) < rows && col(i) + 8 <= cols) {
+#pragma unroll
+                    for (int u = 0; u < (int)sizeof(T) / 2; ++u) ((uint4*)&g[i])[u] = ((const uint4*)p)[u];
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) g[i].v[u] = row(i) < rows && col(i) + u < cols ? p[u] : from_f32<T>(0.0f);
+                }
+            }
+            return;
+        }
+        using Two = typename std::conditional<sizeof(T) == 4, uint2, uint32_t>::type;
 #pragma unroll
         for (int i = 0; i < n; ++i) {
-            const int at = threadIdx.x + i * TH, row = at / (W / 8), col = at % (W / 8) * 8;
-            const T* p = src + row * stride + col;
-            if (row < rows && vec && col + 8 <= cols) {
-                const uint4* q = (const uint4*)p;
+            const T* p = src + row(i) * stride + col(i);
+            const int in = row(i) < rows ? cols - col(i) : 0;
+            if (how == 2) {
 #pragma unroll
-                for (int u = 0; u < (int)sizeof(T) / 2; ++u) ((uint4*)&g[i])[u] = q[u];
+                for (int u = 0; u < 8; u += 2) {
+                    if (u + 2 <= in) {
+                        *(Two*)&g[i].v[u] = *(const Two*)(p + u);
+                    } else {
+                        g[i].v[u] = u < in ? p[u] : from_f32<T>(0.0f);
+                        g[i].v[u + 1] = from_f32<T>(0.0f);
+                    }
+                }
             } else {
 #pragma unroll
-                for (int u = 0; u < 8; ++u) g[i].v[u] = row < rows && col + u < cols ? p[u] : from_f32<T>(0.0f);
+                for (int u = 0; u < 8; ++u) g[i].v[u] = u < in ? p[u] : from_f32<T>(0.0f);
             }
         }
     }
-    // writes the pieces, R rows of ld each; whether a value was not finite
-    __device__ __forceinline__ bool put(bf16* dst, int ld) const {
-        constexpr int NS = Pieces<T>::in;
-        bool bad = false;
+    __device__ __forceinline__ bool bad() const {
+        bool b = false;
 #pragma unroll
         for (int i = 0; i < n; ++i) {
-            const int at = threadIdx.x + i * TH, row = at / (W / 8), col = at % (W / 8) * 8;
-            if (all % TH != 0 && at >= all) continue;
+            if (all % TH != 0 && threadIdx.x + i * TH >= all) continue;
             if constexpr (std::is_same<T, bf16>::value) {
                 const uint4 q = *(const uint4*)&g[i];
-                const uint32_t e = 0x7f807f80u;
-                // exponents of all ones
-                bad |= (__vcmpeq2(q.x & e, e) | __vcmpeq2(q.y & e, e) | __vcmpeq2(q.z & e, e) | __vcmpeq2(q.w & e, e)) != 0;
-                *(uint4*)(dst + row * ld + col) = q;
+                const uint32_t e = 0x7f807f80u;                        // exponents of all ones
+                b |= (__vcmpeq2(q.x & e, e) | __vcmpeq2(q.y & e, e) | __vcmpeq2(q.z & e, e) | __vcmpeq2(q.w & e, e)) != 0;
+            } else {
+#pragma unroll
+                for (int u = 0; u < 8; ++u) b |= not_finite(to_f32(g[i].v[u]));
+            }
+        }
+        return b;
+    }
+    // the values' pieces
+    __device__ __forceinline__ void put(bf16* dst) const {
+        constexpr int NS = Pieces<T>::in;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            if (all % TH != 0 && threadIdx.x + i * TH >= all) continue;
+            bf16* to = dst + Wide<W>::at(row(i), col(i));
+            if constexpr (NS == 1) {
+                *(uint4*)to = *(const uint4*)&g[i];
             } else {
                 uint32_t r[4][NS];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const float x = to_f32(g[i].v[2 * u]), y = to_f32(g[i].v[2 * u + 1]);
-                    split<NS>(x, y, r[u]);
-                    bad |= not_finite(x) | not_finite(y);
-                }
+                for (int u = 0; u < 4; ++u) split<NS>(to_f32(g[i].v[2 * u]), to_f32(g[i].v[2 * u + 1]), r[u]);
 #pragma unroll
-                for (int s = 0; s < NS; ++s) *(uint4*)(dst + (s * R + row) * ld + col) = make_uint4(r[0][s], r[1][s], r[2][s], r[3][s]);
+                for (int s = 0; s < NS; ++s) *(uint4*)(to + s * Wide<W>::elements) = make_uint4(r[0][s], r[1][s], r[2][s], r[3][s]);
             }
         }
-        return bad;
+    }
+    // three pieces of the values times their row's weight
+    __device__ __forceinline__ void put_weighted(bf16* dst, const float* weight) const {
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            if (all % TH != 0 && threadIdx.x + i * TH >= all) continue;
+            bf16* to = dst + Wide<W>::at(row(i), col(i));
+            const float w = weight[row(i)];
+            uint32_t r[4][kFull3];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) split<kFull3>(to_f32(g[i].v[2 * u]) * w, to_f32(g[i].v[2 * u + 1]) * w, r[u]);
+#pragma unroll
+            for (int s = 0; s < kFull3; ++s) *(uint4*)(to + s * Wide<W>::elements) = make_uint4(r[0][s], r[1][s], r[2][s], r[3][s]);
+        }
     }
 };
+
+// elements at a time for rows that start at p and lie `stride` apart
+template <typename T>
+__device__ __forceinline__ int alignment(const T* p, int64_t stride) {
+    const uint64_t x = (uint64_t)(uintptr_t)p | (uint64_t)(stride * (int64_t)sizeof(T));
+    return (x & 15) == 0 ? 8 : (x & (2 * sizeof(T) - 1)) == 0 ? 2 : 1;
+}
 
 // two neighbouring values from their pieces
 template <int NS>
@@ -312,148 +320,154 @@ __device__ __forceinline__ float2 from_pieces(const bf16* m, int piece) {
     return v;
 }
 
+// Writes a warp's 16 x 16 fragment (rows r0 and r0 + 8 of this lane) to rows of `st` elements; `how` as in alignment().
+// 16-bit values of four lanes are brought together, so that a lane stores 16 bytes.
 template <typename T>
-__device__ __forceinline__ bool on_16(const T* p, int64_t stride) {
-    return (((uintptr_t)p | (uintptr_t)(stride * (int64_t)sizeof(T))) & 15) == 0;
+__device__ __forceinline__ void store_rows(T* out, int64_t st, int rows, int cols, int r0, int c0, const float (&x)[2][4], int how) {
+    const int lq = lane_id() & 3;
+    if (sizeof(T) == 2 && how == 8 && c0 + 16 <= cols) {
+        // two tiles of 8 columns, rows r0 and r0 + 8: lane lq gathers tile lq & 1 of row r0 + 8 (lq >> 1)
+        uint32_t v[4];                                                 // [tile + 2 half]
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                struct alignas(4) Two { T a, b; } t{from_f32<T>(x[q][2 * h]), from_f32<T>(x[q][2 * h + 1])};
+                v[q + 2 * h] = *(uint32_t*)&t;
+            }
+        uint32_t a = lq & 1 ? v[0] : v[1], b = lq & 1 ? v[2] : v[3];
+        a = __shfl_xor_sync(kFull, a, 1);
+        b = __shfl_xor_sync(kFull, b, 1);
+        // now this lane and its neighbour hold tile lq & 1 of both rows: (mine, the neighbour's) words
+        uint32_t m0 = lq & 1 ? v[1] : v[0], m1 = lq & 1 ? v[3] : v[2];
+        uint32_t lo0 = lq & 1 ? a : m0, hi0 = lq & 1 ? m0 : a, lo1 = lq & 1 ? b : m1, hi1 = lq & 1 ? m1 : b;
+        const bool up = lq >> 1;
+        uint32_t s0 = up ? lo0 : lo1, s1 = up ? hi0 : hi1;
+        s0 = __shfl_xor_sync(kFull, s0, 2);
+        s1 = __shfl_xor_sync(kFull, s1, 2);
+        const uint32_t k0 = up ? lo1 : lo0, k1 = up ? hi1 : hi0;
+        const uint4 all = up ? make_uint4(s0, s1, k0, k1) : make_uint4(k0, k1, s0, s1);
+        const int r = r0 + 8 * (lq >> 1);
+        if (r < rows) *(uint4*)(out + r * st + c0 + 8 * (lq & 1)) = all;
+        return;
+    }
+    struct alignas(2 * sizeof(T)) Two { T a, b; };
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = r0 + 8 * h;
+        if (r < rows)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int c = c0 + 8 * q + 2 * lq;
+                const T a = from_f32<T>(x[q][2 * h]), b = from_f32<T>(x[q][2 * h + 1]);
+                T* to = out + r * st + c;
+                if (how > 1 && c + 1 < cols) {
+                    *(Two*)to = Two{a, b};
+                } else {
+                    if (c < cols) to[0] = a;
+                    if (c + 1 < cols) to[1] = b;
+                }
+            }
+    }
 }
 
 // ---------------------------------------------------------------------- state ----
-// An NT x PT state in the registers of four warps (which begin at a multiple of four), in the accumulators' layout.
-template <int NT, int PT>
+// The transposed state (64 columns of the values by NT of the keys) in the registers of four warps (which begin at a
+// multiple of four), in the accumulators' layout.
+template <int NT>
 struct State {
-    static constexpr int rows16 = NT / 16;
-    static constexpr int M = rows16 >= 4 ? rows16 / 4 : 1;             // 16-row tiles of a warp
-    static constexpr int across = rows16 >= 4 ? 1 : 4 / rows16;        // warps side by side over the columns
-    static constexpr int C = PT / 8 / across;                          // 8-column tiles of a warp
-    float s[M][C][4];
+    float s[NT / 8][4];
 
-    __device__ __forceinline__ static int row(int m) {                 // first of the tile's rows
-        const int w = (threadIdx.x >> 5) & 3;
-        return rows16 >= 4 ? (w * M + m) * 16 : w / across * 16;
-    }
-    __device__ __forceinline__ static int col(int c) {
-        const int w = (threadIdx.x >> 5) & 3;
-        return ((rows16 >= 4 ? 0 : w % across * C) + c) * 8;
-    }
-    // calls f(value, row, column) for pairs of neighbouring columns
+    __device__ __forceinline__ static int p(int half) { return ((threadIdx.x >> 5) & 3) * 16 + (lane_id() >> 2) + 8 * half; }
+    __device__ __forceinline__ static int n(int c) { return 8 * c + 2 * (lane_id() & 3); }
+
+    // calls f(value, value, p, n) for pairs of neighbouring n
     template <typename F>
     __device__ __forceinline__ void pairs(F&& f) {
-        const int l = lane_id();
 #pragma unroll
-        for (int m = 0; m < M; ++m)
+        for (int c = 0; c < NT / 8; ++c)
 #pragma unroll
-            for (int c = 0; c < C; ++c)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    f(s[m][c][2 * h], s[m][c][2 * h + 1], row(m) + (l >> 2) + 8 * h, col(c) + 2 * (l & 3));
+            for (int h = 0; h < 2; ++h) f(s[c][2 * h], s[c][2 * h + 1], p(h), n(c));
     }
     __device__ __forceinline__ void zero() {
         pairs([](float& x, float& y, int, int) { x = y = 0.0f; });
     }
-    // from rows of `stride` floats, n x p of them
-    __device__ __forceinline__ void load(const float* src, int n, int p, int stride) {
-        const bool even = ((stride & 1) | ((uintptr_t)src & 7)) == 0;
-        pairs([&](float& x, float& y, int r, int c) {
-            x = y = 0.0f;
-            if (r < n && c < p) {
-                const float* q = src + (int64_t)r * stride + c;
-                if (even && c + 1 < p) {
-                    const float2 v = *(const float2*)q;
-                    x = v.x;
-                    y = v.y;
-                } else {
-                    x = q[0];
-                    if (c + 1 < p) y = q[1];
-                }
-            }
+    // from (n, p) of rows of `stride` floats
+    __device__ __forceinline__ void load(const float* src, int rows, int cols, int stride) {
+        pairs([&](float& x, float& y, int p, int n) {
+            x = p < cols && n < rows ? src[(int64_t)n * stride + p] : 0.0f;
+            y = p < cols && n + 1 < rows ? src[(int64_t)(n + 1) * stride + p] : 0.0f;
         });
     }
-    __device__ __forceinline__ void store(float* dst, int n, int p, int stride) {
-        const bool even = ((stride & 1) | ((uintptr_t)dst & 7)) == 0;
-        pairs([&](float& x, float& y, int r, int c) {
-            if (r < n && c < p) {
-                float* q = dst + (int64_t)r * stride + c;
-                if (even && c + 1 < p) {
-                    *(float2*)q = make_float2(x, y);
-                } else {
-                    q[0] = x;
-                    if (c + 1 < p) q[1] = y;
-                }
-            }
+    __device__ __forceinline__ void store(float* dst, int rows, int cols, int stride) {
+        pairs([&](float& x, float& y, int p, int n) {
+            if (p < cols && n < rows) dst[(int64_t)n * stride + p] = x;
+            if (p < cols && n + 1 < rows) dst[(int64_t)(n + 1) * stride + p] = y;
         });
     }
-    // its pieces to shared memory [M][NT][PT + 8]; whether a value was not finite
+    // its pieces to shared memory; whether a value was not finite
     template <int MS>
     __device__ __forceinline__ bool put(bf16* dst) {
         bool bad = false;
-        pairs([&](float& x, float& y, int r, int c) {
+        pairs([&](float& x, float& y, int p, int n) {
             uint32_t q[MS];
             split<MS>(x, y, q);
             bad |= not_finite(x) | not_finite(y);
+            bf16* to = dst + Wide<NT>::at(p, n);
 #pragma unroll
-            for (int k = 0; k < MS; ++k) *(uint32_t*)(dst + (k * NT + r) * (PT + 8) + c) = q[k];
+            for (int k = 0; k < MS; ++k) *(uint32_t*)(to + k * Wide<NT>::elements) = q[k];
         });
         return bad;
     }
-    // s = whole s + sum over the 64 tokens of weight[t] a[t] b[t]^T; weighted a in three pieces.  Half of the tokens at
-    // a time is added up from 0 and then to the state, whose own roundings stay those of float32.
-    template <int NS>
-    __device__ __forceinline__ void advance(const bf16* a, const bf16* b, const float* weight, float whole) {
-        constexpr int lda = NT + 8, ldb = PT + 8, MS = kFull3;
-        const int l = lane_id();
-        pairs([&](float& x, float& y, int, int) {
-            x *= whole;
-            y *= whole;
-        });
+    // s = whole s + the accumulator at addr (this warp's lanes)
+    __device__ __forceinline__ void advance(uint32_t addr, float whole) {
 #pragma unroll
-        for (int k = 0; k < kChunk; k += 32) {
-            uint32_t f[M][2][MS][4];
+        for (int c = 0; c < NT / 16; ++c) {
+            float x[2][4];
+            t5::ld16(x, addr + 16 * c);
+            t5::wait_ld();
 #pragma unroll
-            for (int m = 0; m < M; ++m)
+            for (int q = 0; q < 2; ++q)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t raw[NS][4];
-#pragma unroll
-                    for (int q = 0; q < NS; ++q) load_at(raw[q], a + q * kChunk * lda, lda, row(m), k + 16 * h);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float2 w2 = *(const float2*)(weight + k + 16 * h + 2 * (l & 3) + 8 * (r >> 1));
-                        float x = 0.0f, y = 0.0f;
-#pragma unroll
-                        for (int q = NS - 1; q >= 0; --q) {
-                            x += low_f(raw[q][r]);
-                            y += high_f(raw[q][r]);
-                        }
-                        uint32_t w[MS];
-                        split<MS>(x * w2.x, y * w2.y, w);
-#pragma unroll
-                        for (int q = 0; q < MS; ++q) f[m][h][q][r] = w[q];
-                    }
-                }
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                float sum[M][4] = {};
-                uint32_t v[NS][4];
-#pragma unroll
-                for (int u = NS - 1; u >= 0; --u) load_bk32(v[u], b + u * kChunk * ldb, ldb, k, col(c));
-                // pieces of small weight first
-#pragma unroll
-                for (int order = MS - 1; order >= 0; --order)
-#pragma unroll
-                    for (int u = 0; u < NS && u <= order; ++u)
-#pragma unroll
-                        for (int m = 0; m < M; ++m) {
-                            mma(sum[m], f[m][0][order - u], v[u][0], v[u][1]);
-                            mma(sum[m], f[m][1][order - u], v[u][2], v[u][3]);
-                        }
-#pragma unroll
-                for (int m = 0; m < M; ++m)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) s[m][c][r] += sum[m][r];
-            }
+                for (int e = 0; e < 4; ++e) s[2 * c + q][e] = fmaf(whole, s[2 * c + q][e], x[q][e]);
         }
     }
 };
+
+// What has to be initialised and awaited: barriers of the tensor cores' work, the tensor memory's address, and whether
+// a wait has run out of time, after which no wait is made any more and results are NaN.
+template <int BARS>
+struct Sync {
+    uint64_t bars[BARS];
+    uint32_t tmem;
+    int failed;
+
+    __device__ __forceinline__ void init(uint32_t cols) {
+        if (threadIdx.x < 32) t5::alloc(&tmem, cols);
+        if (threadIdx.x == 0) {
+            failed = 0;
+            for (int i = 0; i < BARS; ++i) t5::bar_init(&bars[i], 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        t5::fence_before();
+        __syncthreads();
+        t5::fence_after();
+    }
+    __device__ __forceinline__ void wait(int bar, uint32_t phase) {
+        if (!*(volatile int*)&failed && !t5::bar_wait(&bars[bar], phase)) *(volatile int*)&failed = 1;
+        t5::fence_after();
+    }
+    // the whole block, all products awaited
+    __device__ __forceinline__ void end(uint32_t cols) {
+        t5::fence_before();
+        __syncthreads();
+        t5::fence_after();
+        if (threadIdx.x < 32) t5::dealloc(tmem, cols);
+    }
+};
+
+// dynamic shared memory from the next multiple of 1024 bytes (tiles want it)
+__device__ __forceinline__ unsigned char* tiles_base(unsigned char* raw) { return raw + ((1024 - (t5::smem_u32(raw) & 1023)) & 1023); }
 
 // The rows of a packed batch behind its last sequence are written as zeros: each block has its share of them.
 template <typename T>
@@ -479,12 +493,10 @@ struct Parts {
 // Sizes and tables of a call; what it takes of the workspace (offsets from its start, 0 bytes where there is none)
 struct Plan {
     Sizes z;
-    int pt;                   // columns of a block's tile
     size_t items_at, seq_at, state_at, whole_at, bytes;
     bool cut;                 // some sequence may have more than one item
 };
 
-int padded_n(int64_t n);
 bcm_status check(const bcm_decay_attn_args* a, const char* what);
 Plan plan_of(const bcm_decay_attn_args* a, bool backward);
 bcm_status fill_tables(Plan& plan, void* workspace, cudaStream_t stream);
@@ -494,20 +506,14 @@ bcm_status join(const Plan& plan, const Parts& parts, const float* end, bool bac
 
 inline Rows rows_of(const void* p, int64_t sb, int64_t st, int64_t sh) { return Rows{p, sb, st, sh}; }
 
-// calls f(T, NT, PT as integral constants)
+// calls f(T, NT as an integral constant)
 template <typename F>
-bcm_status dispatch(bcm_dtype t, int nt, int pt, F&& f) {
+bcm_status dispatch(bcm_dtype t, int64_t n, F&& f) {
     return dispatch_dtype(t, [&](auto type) -> bcm_status {
-        auto by_pt = [&](auto n) -> bcm_status {
-            if (pt == 32) return f(type, n, std::integral_constant<int, 32>());
-            return f(type, n, std::integral_constant<int, 64>());
-        };
-        switch (nt) {
-            case 16: return by_pt(std::integral_constant<int, 16>());
-            case 32: return by_pt(std::integral_constant<int, 32>());
-            case 64: return by_pt(std::integral_constant<int, 64>());
-            default: return by_pt(std::integral_constant<int, 128>());
-        }
+        if (n <= 16) return f(type, std::integral_constant<int, 16>());
+        if (n <= 32) return f(type, std::integral_constant<int, 32>());
+        if (n <= 64) return f(type, std::integral_constant<int, 64>());
+        return f(type, std::integral_constant<int, 128>());
     });
 }
 
@@ -529,35 +535,38 @@ struct PartArgs {
     Parts parts;
 };
 
-template <typename T, int NT, int PT>
+template <typename T, int NT>
 struct PartSmem {
-    bf16 a[Pieces<T>::in][kChunk][NT + 8];
-    bf16 b[Pieces<T>::in][kChunk][PT + 8];
-    Decays d;
+    bf16 a[Pieces<T>::in][Wide<NT>::elements];
+    bf16 bw[kFull3][Wide<kP>::elements];
+    Decays d[2];
+    Sync<1> sync;
 };
 
 constexpr int kPartThreads = 128;
 
-template <typename T, int NT, int PT, bool BACK>
+template <typename T, int NT, bool BACK>
 __global__ void __launch_bounds__(kPartThreads) part_kernel(const __grid_constant__ PartArgs p) {
-    extern __shared__ __align__(16) unsigned char smem_raw[];
-    PartSmem<T, NT, PT>& sm = *(PartSmem<T, NT, PT>*)smem_raw;
+    extern __shared__ unsigned char smem_raw[];
+    PartSmem<T, NT>& sm = *(PartSmem<T, NT>*)tiles_base(smem_raw);
+    constexpr int NS = Pieces<T>::in;
+    constexpr uint32_t kCols = NT < 32 ? 32 : NT;
     const Sizes& z = p.z;
     const int across = z.heads * z.slices;
-    const int item = blockIdx.x / across, hs = blockIdx.x % across, h = hs / z.slices, col = hs % z.slices * PT;
+    const int item = blockIdx.x / across, hs = blockIdx.x % across, h = hs / z.slices, col = hs % z.slices * kP;
     const Item it = item_of(z, item);
     if (it.seq < 0 || (BACK ? it.first : it.last)) return;
-    const int cols = min(PT, z.p - col), ha = h / (z.heads / z.qk_heads);
+    const int cols = min(kP, z.p - col), ha = h / (z.heads / z.qk_heads);
     const T* a = row_ptr<T>(p.a, z, it.seq, it.t0, ha);
     const T* b = row_ptr<T>(p.b, z, it.seq, it.t0, h) + col;
     const float* g = p.g + (z.cu ? 0 : it.seq * p.g_sb) + it.t0 * p.g_st + h * p.g_sh;
-    const bool va = on_16(a, p.a.st), vb = on_16(b, p.b.st);
-    State<NT, PT> st;
+    const int va = alignment(a, p.a.st), vb = alignment(b, p.b.st);
+    const int len = it.t1 - it.t0, nc = (len + kChunk - 1) / kChunk, l = lane_id();
+    State<NT> st;
     st.zero();
     double all = 0.0;
-    const int len = it.t1 - it.t0, nc = (len + kChunk - 1) / kChunk, l = lane_id();
-    Pending<T, kChunk, NT, kPartThreads> pa;
-    Pending<T, kChunk, PT, kPartThreads> pb;
+    Pending<T, NT, kPartThreads> pa;
+    Pending<T, kP, kPartThreads> pb;
     float g0 = 0.0f, g1 = 0.0f;
     auto fetch = [&](int i) {                             // the i-th chunk of the walk
         const int t = (BACK ? nc - 1 - i : i) * kChunk, rows = min(kChunk, len - t);
@@ -569,25 +578,46 @@ __global__ void __launch_bounds__(kPartThreads) part_kernel(const __grid_constan
         }
     };
     if (nc > 0) fetch(0);
+    sm.sync.init(kCols);
+    if (threadIdx.x < 32) all += decays_of(sm.d[0], g0, g1);
+    const uint32_t acc = sm.sync.tmem;
     for (int i = 0; i < nc; ++i) {
         __syncthreads();
-        if (threadIdx.x < 32) all += decays_of(sm.d, g0, g1);
         // (what is not finite stays so in the sums, and the walk takes such chunks token by token)
-        pa.put(&sm.a[0][0][0], NT + 8);
-        pb.put(&sm.b[0][0][0], PT + 8);
+        const Decays& d = sm.d[i & 1];
+        pa.put(sm.a[0]);
+        pb.put_weighted(sm.bw[0], BACK ? d.since : d.until);
+        t5::fence_smem();
+        t5::fence_before();
         __syncthreads();
-        if (i + 1 < nc) fetch(i + 1);
-        st.template advance<Pieces<T>::in>(&sm.a[0][0][0], &sm.b[0][0][0], BACK ? sm.d.since : sm.d.until, sm.d.whole);
+        if (threadIdx.x == 0) {
+            t5::fence_after();
+            const Operand<kP, false> A{t5::smem_u32(sm.bw)};
+            const Operand<NT, false> B{t5::smem_u32(sm.a)};
+            products<kFull3, NS, kFull3>(acc, [&](int s, int k) { return A.desc(s, k); }, [&](int u, int k) { return B.desc(u, k); },
+                                         kChunk / 16, t5::instr(NT, true, true), false);
+            t5::commit(&sm.sync.bars[0]);
+        }
+        __syncwarp();
+        if (i + 1 < nc) {
+            fetch(i + 1);
+            if (threadIdx.x < 32) all += decays_of(sm.d[(i + 1) & 1], g0, g1);
+        }
+        sm.sync.wait(0, i & 1);
+        st.advance(acc + ((threadIdx.x >> 5) << 21), d.whole);
+        t5::fence_before();
     }
+    if (sm.sync.failed) st.pairs([](float& x, float& y, int, int) { x = y = __int_as_float(0x7fc00000); });
     const int64_t at = (int64_t)item * z.heads + h;
-    st.store(p.parts.state + at * z.n * z.p + col, z.n, z.p - col, z.p);
+    st.store(p.parts.state + at * z.n * z.p + col, z.n, cols, z.p);
     if (threadIdx.x == 0 && col == 0) p.parts.whole[at] = exp2f((float)all);
+    sm.sync.end(kCols);
 }
 
-template <typename T, int NT, int PT, bool BACK>
+template <typename T, int NT, bool BACK>
 bcm_status launch_part(const PartArgs& p, cudaStream_t stream) {
-    constexpr size_t smem = sizeof(PartSmem<T, NT, PT>);
-    auto kernel = part_kernel<T, NT, PT, BACK>;
+    constexpr size_t smem = sizeof(PartSmem<T, NT>) + 1024;
+    auto kernel = part_kernel<T, NT, BACK>;
     bcm_status st = allow_smem(kernel, smem);
     if (st != BCM_OK) return st;
     kernel<<<(unsigned)(p.z.items * p.z.heads * p.z.slices), kPartThreads, smem, stream>>>(p);

@@ -17,7 +17,7 @@ struct BwdArgs {
     Rows q, k, v, dy;          // dy.p NULL: zeros
     const float* g;
     int64_t g_sb, g_st, g_sh;
-    const float* ckpt;         // states that enter the chunks, from the forward
+    const float* ckpt;         // [chunks][heads][slices][64][NT] transposed states that enter the chunks
     const float* dh_last;      // or NULL
     const float* enter;        // gradients of the states behind the items, where sequences are cut
     void* dq;                  // contiguous; of `shares` blocks a float32 part each where there is more than one
@@ -28,23 +28,36 @@ struct BwdArgs {
     int shares;
 };
 
-// Four groups of four warps: dv and dg's pairs; dk; dq; the state's gradient.  The first three take 16 tokens a warp.
-// Where there is room for it the pieces of the next chunk's gradient go to a second buffer.
+// Four groups of four warps.  The first takes 16 keys a warp: it decays both products of scores, puts the pieces of
+// (Q K^T o D)^T into tensor memory and those of (dY V^T o D)^T into shared memory (where they serve dk by rows and dq by
+// columns), sums W for dg, and writes dv.  The second and third write dk and dq; the fourth holds the state's gradient.
 constexpr int kBwdThreads = 512;
 
-template <typename T, int NT, int PT>
+template <typename T, int NT>
 struct BwdSmem {
     static constexpr int NS = Pieces<T>::in, MS = Pieces<T>::out;
+    // Keys of 128 leave no room in tensor memory for the state's increase beside the other sums: there it is formed last,
+    // in the scores' place, and its operand takes the place of the scores' pieces.
+    static constexpr bool late = NT > 64;
+    // and in float32 the state takes the place of its gradient once that has been read
+    static constexpr bool one_state = late && NS == 3;
     struct Tiles {
-        bf16 q[NS][kChunk][NT + 8], k[NS][kChunk][NT + 8], v[NS][kChunk][PT + 8], dy[NS][kChunk][PT + 8];
-        bf16 s[kFull3][NT][PT + 8];
+        bf16 q[NS][Wide<NT>::elements], k[NS][Wide<NT>::elements], v[NS][Wide<kP>::elements], dy[NS][Wide<kP>::elements];
+        bf16 ds[kFull3][Wide<NT>::elements], dyw[kFull3][Wide<kP>::elements];
+        bf16 s[one_state ? 1 : kFull3][one_state ? 8 : Wide<NT>::elements], dp[late ? 1 : MS][late ? 8 : Wide<kP>::elements];
+        __device__ __forceinline__ bf16* state() { return one_state ? ds[0] : s[0]; }
+        __device__ __forceinline__ bf16* scores() { return late ? dyw[0] : dp[0]; }
     } tiles;
-    static constexpr int buffers = sizeof(Tiles) + 2 * sizeof(bf16[kFull3][NT][PT + 8]) <= 222 * 1024 ? 2 : 1;
-    bf16 ds[buffers][kFull3][NT][PT + 8];
-    Decays d;
+    Decays d[2];
     float pairs[4][kChunk];    // sum over i >= t, j < t of W_ij, j of one warp
     float of_q[kChunk], of_k[kChunk];
     float across[4];           // <S_in, dS> of the warps
+    Sync<7> sync;
+
+    static constexpr uint32_t at = 0, dt = 64, gv = 128, gk = 192, gq = gk + NT, inc = late ? 0 : gq + NT, cols = 512;
+    // a piece of the keys' decayed scores: blocks of 16 queries are taken from the last, and the 8 columns that a block's
+    // piece needs lie in blocks of both scores which have been read
+    __device__ __forceinline__ static uint32_t piece(int m) { return m == 0 ? at + 32 : m == 1 ? dt + 32 : 480; }
 };
 
 // where a block's rows of dq and dk go
@@ -57,34 +70,17 @@ struct RowsOut {
         if (part) part[row * st + c] = x;
         else whole[row * st + c] = from_f32<T>(x);
     }
-    __device__ __forceinline__ void put2(int64_t row, int c, int cols, float x, float y, bool pair) const {
-        if (c + 1 < cols && pair) {
-            if (part) {
-                *(float2*)(part + row * st + c) = make_float2(x, y);
-            } else {
-                struct alignas(2 * sizeof(T)) Two { T x, y; };
-                *(Two*)(whole + row * st + c) = Two{from_f32<T>(x), from_f32<T>(y)};
-            }
-        } else {
-            if (c < cols) put(row, c, x);
-            if (c + 1 < cols) put(row, c + 1, y);
-        }
-    }
-    __device__ __forceinline__ bool pairs() const {
-        return part ? (((uintptr_t)part | (uintptr_t)(st * 4)) & 7) == 0
-                    : (((uintptr_t)whole | (uintptr_t)(st * sizeof(T))) & (2 * sizeof(T) - 1)) == 0;
-    }
 };
 
 // A chunk with a value that is not finite, token by token from its last: a state is run up anew for each.
-// `f` (shared): the state's gradient NT x PT, then sums.
-template <typename T, int NT, int PT>
+// `f` (shared): the state's gradient NT x kP, then sums.
+template <typename T, int NT>
 __device__ __noinline__ void back_tokens(const BwdArgs& p, const T* q, const T* k, const T* v, const T* dy, const float* g, const float* s_in,
                                          const RowsOut<T>& dq, const RowsOut<T>& dk, T* dv, int64_t dv_st, float* dg, int64_t dg_st,
                                          int rows, int cols, int64_t row0, float* f) {
-    constexpr int parts = kBwdThreads / PT, warps = PT / 32, all_warps = kBwdThreads / 32;
-    const int c = threadIdx.x % PT, part = threadIdx.x / PT, w = threadIdx.x >> 5, l = lane_id();
-    float* const sq = f + NT * PT;                 // [warps][NT]
+    constexpr int parts = kBwdThreads / kP, warps = kP / 32, all_warps = kBwdThreads / 32;
+    const int c = threadIdx.x % kP, part = threadIdx.x / kP, w = threadIdx.x >> 5, l = lane_id();
+    float* const sq = f + NT * kP;                 // [warps][NT]
     float* const sk = sq + 2 * NT;
     float* const sv = sk + 2 * NT;                 // [kBwdThreads]
     float* const sg = sv + kBwdThreads;            // [all_warps]
@@ -94,16 +90,16 @@ __device__ __noinline__ void back_tokens(const BwdArgs& p, const T* q, const T* 
         const float gy = in && dy ? to_f32(dy[t * p.dy.st + c]) : 0.0f, x = in ? to_f32(v[t * p.v.st + c]) : 0.0f;
         float gv = 0.0f, gg = 0.0f;
         for (int n = part; n < p.z.n; n += parts) {
-            float s = in ? s_in[(int64_t)n * p.z.p + c] : 0.0f;
+            float s = in ? s_in[c * NT + n] : 0.0f;
             if (in)
                 for (int u = 0; u < t; ++u) s = fmaf(expf(g[u * p.g_st]), s, to_f32(k[u * p.k.st + n]) * to_f32(v[u * p.v.st + c]));
             const float kn = to_f32(k[t * p.k.st + n]), now = fmaf(a, s, kn * x);
-            const float ds = f[n * PT + c] + (dy ? to_f32(q[t * p.q.st + n]) * gy : 0.0f);
+            const float ds = f[n * kP + c] + (dy ? to_f32(q[t * p.q.st + n]) * gy : 0.0f);
             float gq = in ? now * gy : 0.0f, gk = in ? ds * x : 0.0f;
             gv = fmaf(ds, kn, gv);
             const float back = a * ds;
             gg += in ? back * s : 0.0f;
-            f[n * PT + c] = in ? back : 0.0f;
+            f[n * kP + c] = in ? back : 0.0f;
 #pragma unroll
             for (int o = 16; o; o >>= 1) {
                 gq += __shfl_xor_sync(kFull, gq, o);
@@ -129,7 +125,7 @@ __device__ __noinline__ void back_tokens(const BwdArgs& p, const T* q, const T* 
             dk.put(row0 + t, n, x1);
         }
         if (part == 0 && in) {
-            for (int r = 1; r < parts; ++r) gv += sv[r * PT + c];
+            for (int r = 1; r < parts; ++r) gv += sv[r * kP + c];
             dv[t * dv_st + c] = from_f32<T>(gv);
         }
         if (threadIdx.x == 0) {
@@ -140,23 +136,23 @@ __device__ __noinline__ void back_tokens(const BwdArgs& p, const T* q, const T* 
     }
 }
 
-template <typename T, int NT, int PT>
+template <typename T, int NT>
 __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant__ BwdArgs p) {
-    extern __shared__ __align__(16) unsigned char smem_raw[];
-    using Smem = BwdSmem<T, NT, PT>;
-    Smem& sm = *(Smem*)smem_raw;
-    constexpr int NS = Smem::NS, MS = Smem::MS, LN = NT + 8, LP = PT + 8;
+    extern __shared__ unsigned char smem_raw[];
+    using Smem = BwdSmem<T, NT>;
+    Smem& sm = *(Smem*)tiles_base(smem_raw);
+    constexpr int NS = Smem::NS, MS = Smem::MS;
     const Sizes& z = p.z;
     const int across = z.heads * z.slices, share = z.heads / z.qk_heads;
-    const int item = blockIdx.x / across, hs = blockIdx.x % across, h = hs / z.slices, slice = hs % z.slices, col = slice * PT;
-    const int cols = min(PT, z.p - col), hq = h / share;
+    const int item = blockIdx.x / across, hs = blockIdx.x % across, h = hs / z.slices, slice = hs % z.slices, col = slice * kP;
+    const int cols = min(kP, z.p - col), hq = h / share;
     const int64_t rows_all = (z.cu ? 1 : (int64_t)z.batch) * z.seqlen;
     const int64_t qk_st = (int64_t)z.qk_heads * z.n, v_st = (int64_t)z.heads * z.p;
-    const int mine = h % share * z.slices + slice;            // of the blocks that share a row of dq
+    const int part = h % share * z.slices + slice;            // of the blocks that share a row of dq
     RowsOut<T> dq{(T*)p.dq + (int64_t)hq * z.n, nullptr, qk_st}, dk{(T*)p.dk + (int64_t)hq * z.n, nullptr, qk_st};
     if (p.shares > 1) {
-        dq.part = (float*)p.dq + mine * rows_all * qk_st + (int64_t)hq * z.n;
-        dk.part = (float*)p.dk + mine * rows_all * qk_st + (int64_t)hq * z.n;
+        dq.part = (float*)p.dq + part * rows_all * qk_st + (int64_t)hq * z.n;
+        dk.part = (float*)p.dk + part * rows_all * qk_st + (int64_t)hq * z.n;
     }
     float* const dg_all = p.dg + slice * rows_all * z.heads + h;
     if (z.cu) {
@@ -181,55 +177,66 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
     const int64_t row_at = (z.cu ? 0 : (int64_t)it.seq * z.seqlen) + it.t0;
     T* const dv = (T*)p.dv + row_at * v_st + (int64_t)h * z.p + col;
     float* const dg = dg_all + row_at * z.heads;
-    const bool vq = on_16(q, p.q.st), vk = on_16(k, p.k.st), vv = on_16(v, p.v.st), vy = dy && on_16(dy, p.dy.st);
-    const bool pair_v = (((uintptr_t)dv | (uintptr_t)(v_st * sizeof(T))) & (2 * sizeof(T) - 1)) == 0, pair_qk = dq.pairs() && dk.pairs();
+    const int vq = alignment(q, p.q.st), vk = alignment(k, p.k.st), vv = alignment(v, p.v.st), vy = dy ? alignment(dy, p.dy.st) : 1;
     const int np = z.n * z.p;
     const int len = it.t1 - it.t0, nc = (len + kChunk - 1) / kChunk;
     const int l = lane_id(), group = threadIdx.x >> 7, w = (threadIdx.x >> 5) & 3, row = w * 16 + (l >> 2), lq = l & 3;
     const bool decay_warp = threadIdx.x >= 384 && threadIdx.x < 416;
-    bf16* const tq = &sm.tiles.q[0][0][0];
-    bf16* const tk = &sm.tiles.k[0][0][0];
-    bf16* const tv = &sm.tiles.v[0][0][0];
-    bf16* const ty = &sm.tiles.dy[0][0][0];
-    bf16* const ts = &sm.tiles.s[0][0][0];
-    constexpr int piece_n = kChunk * LN, piece_p = kChunk * LP, piece_s = NT * LP;
+    const int p16 = (cols + 15) / 16, n16 = (z.n + 15) / 16;
 
-    Pending<T, kChunk, NT, kBwdThreads> pq, pk;
-    Pending<T, kChunk, PT, kBwdThreads> pv, py;
-    Pending<float, NT, PT, kBwdThreads> ps;
+    Pending<T, NT, kBwdThreads> pq, pk;
+    Pending<T, kP, kBwdThreads> pv, py;
+    Pending<float, NT, kBwdThreads> ps;
     float g0 = 0.0f, g1 = 0.0f;
-    const bool vs = (z.p & 3) == 0 && (col & 3) == 0 && ((uintptr_t)p.ckpt & 15) == 0;
-    auto state_in = [&](int c) { return p.ckpt + ((int64_t)(it.chunk + c) * z.heads + h) * np + col; };
+    auto state_in = [&](int c) { return p.ckpt + (((int64_t)(it.chunk + c) * z.heads + h) * z.slices + slice) * (NT * kP); };
     auto fetch = [&](int c) {
         const int t = c * kChunk, rows = min(kChunk, len - t);
         pq.fetch(q + t * p.q.st, p.q.st, rows, z.n, vq);
         pk.fetch(k + t * p.k.st, p.k.st, rows, z.n, vk);
         pv.fetch(v + t * p.v.st, p.v.st, rows, cols, vv);
         py.fetch(dy + t * p.dy.st, p.dy.st, dy ? rows : 0, cols, vy);
-        ps.fetch(state_in(c), z.p, z.n, cols, vs);
+        ps.fetch(state_in(c), NT, cols, NT, 8);
         if (decay_warp) {
             g0 = 2 * l < rows ? g[(int64_t)(t + 2 * l) * p.g_st] : 0.0f;
             g1 = 2 * l + 1 < rows ? g[(int64_t)(t + 2 * l + 1) * p.g_st] : 0.0f;
         }
     };
-    auto put = [&]() {
-        bool bad = pq.put(tq, LN);
-        bad |= pk.put(tk, LN);
-        bad |= pv.put(tv, LP);
-        bad |= py.put(ty, LP);
-        bad |= ps.put(ts, LP);
-        if (decay_warp) {
-            bad |= !(g0 <= 3.38e38f && g1 <= 3.38e38f);
-            decays_of(sm.d, g0, g1);
-        }
+    auto put = [&](int c) {
+        bool bad = pq.bad() | pk.bad() | pv.bad() | py.bad() | ps.bad();
+        if (decay_warp) bad |= !(g0 <= 3.38e38f && g1 <= 3.38e38f);
+        pq.put(sm.tiles.q[0]);
+        pk.put(sm.tiles.k[0]);
+        pv.put(sm.tiles.v[0]);
+        py.put(sm.tiles.dy[0]);
+        if (!Smem::one_state) ps.put(sm.tiles.state());
+        if (!Smem::late) py.put_weighted(sm.tiles.dyw[0], sm.d[c & 1].since);
+        t5::fence_smem();
+        t5::fence_before();
         return bad;
+    };
+    // (float32 keys of 128) the state in the place of its gradient, which all have read by then
+    auto put_state = [&](uint32_t phase) {
+        if (!Smem::one_state) return;
+        sm.sync.wait(1, phase);
+        ps.put(sm.tiles.state());
+        t5::fence_smem();
+        t5::fence_before();
+        __syncthreads();
     };
     auto walk = [&](int c) {
         const int t = c * kChunk;
-        back_tokens<T, NT, PT>(p, q + t * p.q.st, k + t * p.k.st, v + t * p.v.st, dy ? dy + t * p.dy.st : nullptr, g + t * p.g_st, state_in(c), dq, dk,
-                               dv + t * v_st, v_st, dg + (int64_t)t * z.heads, z.heads, min(kChunk, len - t), cols, row_at + t, (float*)&sm.tiles);
+        back_tokens<T, NT>(p, q + t * p.q.st, k + t * p.k.st, v + t * p.v.st, dy ? dy + t * p.dy.st : nullptr, g + t * p.g_st, state_in(c), dq, dk,
+                           dv + t * v_st, v_st, dg + (int64_t)t * z.heads, z.heads, min(kChunk, len - t), cols, row_at + t, (float*)&sm.tiles);
     };
     if (nc > 0) fetch(nc - 1);
+    sm.sync.init(Smem::cols);
+    const uint32_t tm = sm.sync.tmem, lanes = (uint32_t)w << 21;
+    uint32_t phase = 0;
+    const Operand<NT, true> Q{t5::smem_u32(sm.tiles.q)}, K{t5::smem_u32(sm.tiles.k)}, Sk{t5::smem_u32(sm.tiles.ds)};
+    const Operand<NT, false> Qt{t5::smem_u32(sm.tiles.q)}, Kt{t5::smem_u32(sm.tiles.k)}, dS{t5::smem_u32(sm.tiles.ds)}, S{t5::smem_u32(sm.tiles.state())};
+    const Operand<kP, true> V{t5::smem_u32(sm.tiles.v)}, Y{t5::smem_u32(sm.tiles.dy)}, P{t5::smem_u32(sm.tiles.scores())};
+    const Operand<kP, false> Yt{t5::smem_u32(sm.tiles.dy)}, Yw{t5::smem_u32(sm.tiles.dyw)}, Pt{t5::smem_u32(sm.tiles.scores())};
+    auto of = [](const auto& o) { return [&o](int s, int i) { return o.desc(s, i); }; };
 
     if (group == 3) {
         // dg of chunk c from what its walk left in shared memory (one warp)
@@ -246,7 +253,7 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
             float rest = __shfl_down_sync(kFull, behind, 1), past = __shfl_up_sync(kFull, before, 1);
             if (l == 31) rest = 0.0f;
             if (l == 0) past = 0.0f;
-            const float through = sm.d.whole * ((sm.across[0] + sm.across[1]) + (sm.across[2] + sm.across[3]));
+            const float through = sm.d[c & 1].whole * ((sm.across[0] + sm.across[1]) + (sm.across[2] + sm.across[3]));
             float d0 = 0.0f, d1 = 0.0f;
             for (int k2 = 0; k2 <= t / 16; ++k2) {
                 d0 += sm.pairs[k2][t];
@@ -257,93 +264,260 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
             if (t < rows) dg[(int64_t)(c * kChunk + t) * z.heads] = d0;
             if (t + 1 < rows) dg[(int64_t)(c * kChunk + t + 1) * z.heads] = d1;
         };
-        State<NT, PT> ds;
+        State<NT> ds;
         const float* from = it.last ? (p.dh_last ? p.dh_last + ((int64_t)it.seq * z.heads + h) * np : nullptr)
                                     : p.enter + ((int64_t)item * z.heads + h) * np;
-        if (from) ds.load(from + col, z.n, z.p - col, z.p);
+        if (decay_warp && nc > 0) decays_of(sm.d[(nc - 1) & 1], g0, g1);
+        if (from) ds.load(from + col, z.n, cols, z.p);
         else ds.zero();
-        bool bad = false, pending = false;                    // pending: the chunk behind has its dg still to be finished
-        if (Smem::buffers > 1) bad = ds.template put<kFull3>(&sm.ds[(nc - 1) & 1 & (Smem::buffers - 1)][0][0][0]);
+        bool bad = ds.template put<kFull3>(sm.tiles.ds[0]);
+        bool pending = false;                                 // the chunk behind has its dg still to be finished
         for (int c = nc - 1; c >= 0; --c) {
-            __syncthreads();                                  // the chunk behind is done with the tiles
+            __syncthreads();                                  // decays are there; the chunk behind is done with the tiles
             if (pending && decay_warp) finish_dg(c + 1);
-            bad |= put();
-            if (Smem::buffers == 1) bad |= ds.template put<kFull3>(&sm.ds[0][0][0][0]);
+            bad |= put(c);
             const bool slow = __syncthreads_or(bad);
-            if (c > 0) fetch(c - 1);
+            const float whole = sm.d[c & 1].whole;
+            if (!slow) put_state(phase);
+            if (c > 0) {
+                fetch(c - 1);
+                if (decay_warp) decays_of(sm.d[(c - 1) & 1], g0, g1);
+            }
             pending = !slow;
             if (slow) {
                 float* f = (float*)&sm.tiles;
-                ds.pairs([&](float& x0, float& x1, int r, int cc) {
-                    f[r * PT + cc] = x0;
-                    f[r * PT + cc + 1] = x1;
+                ds.pairs([&](float& x0, float& x1, int pp, int n) {
+                    f[n * kP + pp] = x0;
+                    f[(n + 1) * kP + pp] = x1;
                 });
                 __syncthreads();
                 walk(c);
-                ds.pairs([&](float& x0, float& x1, int r, int cc) {
-                    x0 = f[r * PT + cc];
-                    x1 = f[r * PT + cc + 1];
+                ds.pairs([&](float& x0, float& x1, int pp, int n) {
+                    x0 = f[n * kP + pp];
+                    x1 = f[(n + 1) * kP + pp];
                 });
+                __syncthreads();                              // all have theirs back before the pieces take the place
             } else {
                 float x = 0.0f;
-                ds.pairs([&](float& x0, float& x1, int r, int cc) {
-                    const float2 in = from_pieces<kFull3>(ts + r * LP + cc, piece_s);
+                ds.pairs([&](float& x0, float& x1, int pp, int n) {
+                    const float2 in = from_pieces<kFull3>(sm.tiles.state() + Wide<NT>::at(pp, n), Wide<NT>::elements);
                     x = fmaf(in.x, x0, fmaf(in.y, x1, x));
                 });
 #pragma unroll
                 for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(kFull, x, o);
                 if (l == 0) sm.across[w] = x;
-                ds.template advance<NS>(tq, ty, sm.d.since, sm.d.whole);
+                if (Smem::late) {
+                    // behind all other products of the chunk
+                    for (int b = 4; b < 7; ++b) sm.sync.wait(b, phase);
+                    const float* since = sm.d[c & 1].since;
+                    for (int i = threadIdx.x - 384; i < 64 * 8; i += 128) {
+                        const int r = i / 8, u = i % 8 * 8, e = Wide<kP>::at(r, u);
+                        uint32_t a[4][kFull3];
+#pragma unroll
+                        for (int k2 = 0; k2 < 4; ++k2) {
+                            const float2 in = from_pieces<NS>(sm.tiles.dy[0] + e + 2 * k2, Wide<kP>::elements);
+                            split<kFull3>(in.x * since[r], in.y * since[r], a[k2]);
+                        }
+#pragma unroll
+                        for (int s = 0; s < kFull3; ++s) *(uint4*)(sm.tiles.dyw[s] + e) = make_uint4(a[0][s], a[1][s], a[2][s], a[3][s]);
+                    }
+                    t5::fence_smem();
+                    t5::fence_before();
+                    named_sync(2, 128);
+                    if (threadIdx.x == 384) {
+                        t5::fence_after();
+                        products<kFull3, NS, kFull3>(tm + Smem::inc, of(Yw), of(Qt), kChunk / 16, t5::instr(NT, true, true), false);
+                        t5::commit(&sm.sync.bars[3]);
+                    }
+                    __syncwarp();
+                }
+                sm.sync.wait(3, phase);
+                ds.advance(tm + Smem::inc + lanes, whole);
+                sm.sync.wait(1, phase);                       // the products with the gradient (and the state) have read it
+                if (Smem::one_state) sm.sync.wait(2, phase);
+                t5::fence_before();
+                named_sync(2, 128);                           // (and this group the state, for its dot)
+                phase ^= 1;
             }
-            bad = false;
-            if (Smem::buffers > 1) bad = ds.template put<kFull3>(&sm.ds[(c + 1) & 1 & (Smem::buffers - 1)][0][0][0]);
+            bad = ds.template put<kFull3>(sm.tiles.ds[0]);
         }
         __syncthreads();
         if (pending && decay_warp) finish_dg(0);
-        if (it.first) ds.store(p.dh0 + ((int64_t)it.seq * z.heads + h) * np + col, z.n, z.p - col, z.p);
+        if (sm.sync.failed) ds.pairs([](float& x, float& y1, int, int) { x = y1 = __int_as_float(0x7fc00000); });
+        if (it.first) ds.store(p.dh0 + ((int64_t)it.seq * z.heads + h) * np + col, z.n, cols, z.p);
+        sm.sync.end(Smem::cols);
         return;
     }
 
     for (int c = nc - 1; c >= 0; --c) {
         const int t = c * kChunk, rows = min(kChunk, len - t);
         __syncthreads();
-        const bool bad = put();
-        const bool slow = __syncthreads_or(bad);
-        if (c > 0) fetch(c - 1);
+        const bool slow = __syncthreads_or(put(c));
         if (slow) {
+            if (c > 0) fetch(c - 1);
             __syncthreads();
             walk(c);
+            __syncthreads();
             continue;
         }
-        const bf16* tds = &sm.ds[c & 1 & (Smem::buffers - 1)][0][0][0];
-        const float hi0 = sm.d.hi[row], lo0 = sm.d.lo[row], hi1 = sm.d.hi[row + 8], lo1 = sm.d.lo[row + 8];
-        auto keys = [&](uint32_t(&a)[4], int s, int kk) { load_a(a, tk + s * piece_n, LN, w * 16, kk * 16); };
-        auto values = [&](uint32_t(&a)[4], int s, int kk) { load_a(a, tv + s * piece_p, LP, w * 16, kk * 16); };
-        auto ups = [&](uint32_t(&a)[4], int s, int kk) { load_a(a, ty + s * piece_p, LP, w * 16, kk * 16); };
-        // x D of 16 rows by 16 columns: rows as the earlier tokens (keys) or as the later ones (queries)
-        auto decayed = [&](float(&x)[2][4], int block, bool as_keys) {
+        if (threadIdx.x == 0) {
+            t5::fence_after();
+            products<NS, NS, kFull3>(tm + Smem::at, of(K), of(Q), n16, t5::instr(kChunk, false, false), false);
+            products<NS, NS, kFull3>(tm + Smem::dt, of(V), of(Y), p16, t5::instr(kChunk, false, false), false);
+            t5::commit(&sm.sync.bars[0]);
+            products<NS, MS, MS>(tm + Smem::gv, of(K), of(Sk), n16, t5::instr(p16 * 16, false, false), false);
+            products<NS, kFull3, kFull3>(tm + Smem::gk, of(V), of(dS), p16, t5::instr(n16 * 16, false, true), false);
+            t5::commit(&sm.sync.bars[1]);
+            if (!Smem::one_state) {
+                products<NS, kFull3, kFull3>(tm + Smem::gq, of(Y), of(S), p16, t5::instr(n16 * 16, false, true), false);
+                t5::commit(&sm.sync.bars[2]);
+            }
+            if (!Smem::late) {
+                products<kFull3, NS, kFull3>(tm + Smem::inc, of(Yw), of(Qt), kChunk / 16, t5::instr(NT, true, true), false);
+                t5::commit(&sm.sync.bars[3]);
+            }
+        }
+        __syncwarp();
+        put_state(phase);
+        if (Smem::one_state && threadIdx.x == 0) {
+            t5::fence_after();
+            products<NS, kFull3, kFull3>(tm + Smem::gq, of(Y), of(S), p16, t5::instr(n16 * 16, false, true), false);
+            t5::commit(&sm.sync.bars[2]);
+        }
+        __syncwarp();
+        if (c > 0) fetch(c - 1);
+        const Decays& d = sm.d[c & 1];
+        if (group == 0) {
+            const float hi0 = d.hi[row], lo0 = d.lo[row], hi1 = d.hi[row + 8], lo1 = d.lo[row + 8], u0 = d.until[row], u1 = d.until[row + 8];
+            sm.sync.wait(0, phase);
+            bf16* const dp = sm.tiles.scores();
+            float run[2] = {0.0f, 0.0f};                      // sums of W over the queries behind the block
+#pragma unroll 1
+            for (int ib = 3; ib >= 0; --ib) {
+                uint32_t r[2][2][MS] = {}, r2[2][2][MS] = {};
+                if (ib >= w) {
+                    float at[2][4], dt[2][4];
+                    t5::ld16(at, tm + Smem::at + lanes + 16 * ib);
+                    t5::ld16(dt, tm + Smem::dt + lanes + 16 * ib);
+                    t5::wait_ld();
+                    float W[2][2][2], sum[2][2] = {};         // sum: of the four columns, over this warp's keys before them
 #pragma unroll
-            for (int q2 = 0; q2 < 2; ++q2) {
-                const int o = block * 16 + q2 * 8 + 2 * lq;
-                const float2 h2 = *(const float2*)&sm.d.hi[o], l2 = *(const float2*)&sm.d.lo[o];
+                    for (int q2 = 0; q2 < 2; ++q2) {
+                        const int i = ib * 16 + q2 * 8 + 2 * lq;
+                        const float2 hi = *(const float2*)&d.hi[i], lo = *(const float2*)&d.lo[i];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int i = o + (e & 1), r = row + (e & 2) * 4;
-                    const float ho = e & 1 ? h2.y : h2.x, lo = e & 1 ? l2.y : l2.x, hr = e & 2 ? hi1 : hi0, lr = e & 2 ? lo1 : lo0;
-                    if (as_keys) x[q2][e] = i >= r ? x[q2][e] * between(ho, lo, hr, lr) : 0.0f;
-                    else x[q2][e] = i <= r ? x[q2][e] * between(hr, lr, ho, lo) : 0.0f;
+                        for (int e = 0; e < 4; ++e) {
+                            const bool in = i + (e & 1) >= row + (e & 2) * 4;
+                            const float f = between(e & 1 ? hi.y : hi.x, e & 1 ? lo.y : lo.x, e & 2 ? hi1 : hi0, e & 2 ? lo1 : lo0);
+                            float &a = at[q2][e], &b = dt[q2][e];
+                            a = in ? a * f : 0.0f;
+                            W[e >> 1][q2][e & 1] = in ? a * b : 0.0f;
+                            b = in ? b * f : 0.0f;
+                        }
+                        split<MS>(at[q2][0], at[q2][1], r[q2][0]);
+                        split<MS>(at[q2][2], at[q2][3], r[q2][1]);
+                        split<MS>(dt[q2][0], dt[q2][1], r2[q2][0]);
+                        split<MS>(dt[q2][2], dt[q2][3], r2[q2][1]);
+                    }
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const int j = row + 8 * half, i = ib * 16 + 2 * lq;
+                        float ex[2], all[2];
+#pragma unroll
+                        for (int q2 = 0; q2 < 2; ++q2) {
+                            float s = W[half][q2][0] + W[half][q2][1];
+                            float o = __shfl_down_sync(kFull, s, 1, 4);
+                            if (lq < 3) s += o;
+                            o = __shfl_down_sync(kFull, s, 2, 4);
+                            if (lq < 2) s += o;
+                            o = __shfl_down_sync(kFull, s, 1, 4);
+                            ex[q2] = lq < 3 ? o : 0.0f;
+                            all[q2] = __shfl_sync(kFull, s, 0, 4);
+                        }
+                        float u = run[half] + ex[1] + W[half][1][1];
+                        if (j < i + 9) sum[1][1] += u;
+                        u += W[half][1][0];
+                        if (j < i + 8) sum[1][0] += u;
+                        u = run[half] + all[1] + ex[0] + W[half][0][1];
+                        if (j < i + 1) sum[0][1] += u;
+                        u += W[half][0][0];
+                        if (j < i) sum[0][0] += u;
+                        run[half] += all[1] + all[0];
+                    }
+#pragma unroll
+                    for (int q2 = 0; q2 < 2; ++q2)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                            for (int o = 4; o < 32; o <<= 1) sum[q2][e] += __shfl_xor_sync(kFull, sum[q2][e], o);
+                            if (l < 4) sm.pairs[w][ib * 16 + q2 * 8 + 2 * lq + e] = sum[q2][e];
+                        }
+                }
+#pragma unroll
+                for (int m = 0; m < MS; ++m) {
+                    t5::st16(tm + Smem::piece(m) + lanes + 8 * ib, r[0][0][m], r[0][1][m], r[1][0][m], r[1][1][m]);
+#pragma unroll
+                    for (int q2 = 0; q2 < 2; ++q2)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half)
+                            *(uint32_t*)(dp + m * Wide<kP>::elements + Wide<kP>::at(row + 8 * half, ib * 16 + q2 * 8 + 2 * lq)) = r2[q2][half][m];
                 }
             }
-        };
-        // a row's dot with `tile`'s, into out[row]
-        auto dots = [&](float(&x)[NT / 8][4], const bf16* tile, float* out) {
-            float dot0 = 0.0f, dot1 = 0.0f;
+            t5::fence_smem();
+            sm.sync.wait(1, phase);
+            for (int pb = 0; pb < p16; ++pb) {
+                float x[2][4];
+                t5::ld16(x, tm + Smem::gv + lanes + 16 * pb);
+                t5::wait_ld();
 #pragma unroll
-            for (int nb = 0; nb < NT / 8; ++nb) {
-                const float2 k0 = from_pieces<NS>(tile + row * LN + nb * 8 + 2 * lq, piece_n);
-                const float2 k1 = from_pieces<NS>(tile + (row + 8) * LN + nb * 8 + 2 * lq, piece_n);
-                dot0 = fmaf(k0.x, x[nb][0], fmaf(k0.y, x[nb][1], dot0));
-                dot1 = fmaf(k1.x, x[nb][2], fmaf(k1.y, x[nb][3], dot1));
+                for (int q2 = 0; q2 < 2; ++q2)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[q2][e] *= e < 2 ? u0 : u1;
+                t5::st_acc16(tm + Smem::gv + lanes + 16 * pb, x);
+            }
+            t5::wait_st();
+            t5::fence_before();
+            named_sync(1, 384);
+            if (threadIdx.x == 0) {
+                t5::fence_after();
+                products<MS, NS, MS>(tm + Smem::gv, [&](int s, int i) { return tm + Smem::piece(s) + 8 * i; }, of(Yt), kChunk / 16,
+                                     t5::instr(p16 * 16, false, true), true);
+                t5::commit(&sm.sync.bars[4]);
+            }
+            __syncwarp();
+            sm.sync.wait(4, phase);
+            const int how = alignment(dv, v_st);
+            for (int pb = 0; pb < p16; ++pb) {
+                float x[2][4];
+                t5::ld16(x, tm + Smem::gv + lanes + 16 * pb);
+                t5::wait_ld();
+                store_rows(dv + t * v_st, v_st, rows, cols, row, 16 * pb, x, how);
+            }
+        } else {
+            // dk (rows as keys) and dq (rows as queries): the far part, decayed in place, whose dot with the row itself is
+            // its share of dg; then the near part on top of it
+            const bool as_keys = group == 1;
+            const float* decay = as_keys ? d.until : d.since;
+            const float u0 = decay[row], u1 = decay[row + 8];
+            const uint32_t acc = tm + (as_keys ? Smem::gk : Smem::gq) + lanes;
+            const bf16* const self = as_keys ? sm.tiles.k[0] : sm.tiles.q[0];
+            float dot0 = 0.0f, dot1 = 0.0f;
+            sm.sync.wait(as_keys ? 1 : 2, phase);
+            for (int nb = 0; nb < n16; ++nb) {
+                float x[2][4];
+                t5::ld16(x, acc + 16 * nb);
+                t5::wait_ld();
+#pragma unroll
+                for (int q2 = 0; q2 < 2; ++q2) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[q2][e] *= e < 2 ? u0 : u1;
+                    const int n = 16 * nb + 8 * q2 + 2 * lq;
+                    const float2 k0 = from_pieces<NS>(self + Wide<NT>::at(row, n), Wide<NT>::elements);
+                    const float2 k1 = from_pieces<NS>(self + Wide<NT>::at(row + 8, n), Wide<NT>::elements);
+                    dot0 = fmaf(k0.x, x[q2][0], fmaf(k0.y, x[q2][1], dot0));
+                    dot1 = fmaf(k1.x, x[q2][2], fmaf(k1.y, x[q2][3], dot1));
+                }
+                t5::st_acc16(acc + 16 * nb, x);
             }
 #pragma unroll
             for (int o = 1; o < 4; o <<= 1) {
@@ -351,134 +525,49 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
                 dot1 += __shfl_xor_sync(kFull, dot1, o);
             }
             if (lq == 0) {
+                float* out = as_keys ? sm.of_k : sm.of_q;
                 out[row] = dot0;
                 out[row + 8] = dot1;
             }
-        };
-        if (group == 0) {
-            // dv of 16 tokens, and the sums of W
-            float gv[PT / 8][4] = {};
-            gemm<NS, MS, MS, NT / 16, PT / 16, true>(gv, keys, tds, LP, piece_s, 0, 0);
-            const float u0 = sm.d.until[row], u1 = sm.d.until[row + 8];
-#pragma unroll
-            for (int pb = 0; pb < PT / 8; ++pb) {
-                gv[pb][0] *= u0;
-                gv[pb][1] *= u0;
-                gv[pb][2] *= u1;
-                gv[pb][3] *= u1;
+            t5::wait_st();
+            t5::fence_before();
+            named_sync(1, 384);
+            if (threadIdx.x % 128 == 0) {
+                t5::fence_after();
+                if (as_keys) products<MS, NS, MS>(tm + Smem::gk, of(P), of(Qt), kChunk / 16, t5::instr(n16 * 16, false, true), true);
+                else products<MS, NS, MS>(tm + Smem::gq, of(Pt), of(Kt), kChunk / 16, t5::instr(n16 * 16, true, true), true);
+                t5::commit(&sm.sync.bars[4 + group]);
             }
-            float run[2] = {0.0f, 0.0f};                      // sums of W over the queries behind the block
-#pragma unroll 1
-            for (int ib = 3; ib >= w; --ib) {
-                float at[2][4] = {}, dt[2][4] = {};
-                gemm<NS, NS, kFull3, NT / 16, 1, false>(at, keys, tq, LN, piece_n, 0, ib * 16);
-                gemm<NS, NS, kFull3, PT / 16, 1, false>(dt, values, ty, LP, piece_p, 0, ib * 16);
-                decayed(at, ib, true);
-                float sum[2][2] = {};                         // of the four columns, over this warp's keys before them
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int j = row + 8 * half;
-                    float W[2][2], ex[2], all[2];
-#pragma unroll
-                    for (int q2 = 0; q2 < 2; ++q2) {
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) W[q2][e] = at[q2][2 * half + e] * dt[q2][2 * half + e];
-                        float s = W[q2][0] + W[q2][1];
-                        float o = __shfl_down_sync(kFull, s, 1, 4);
-                        if (lq < 3) s += o;
-                        o = __shfl_down_sync(kFull, s, 2, 4);
-                        if (lq < 2) s += o;
-                        o = __shfl_down_sync(kFull, s, 1, 4);
-                        ex[q2] = lq < 3 ? o : 0.0f;
-                        all[q2] = __shfl_sync(kFull, s, 0, 4);
-                    }
-                    float u = run[half] + ex[1] + W[1][1];
-                    const int i = ib * 16 + 2 * lq;
-                    if (j < i + 9) sum[1][1] += u;
-                    u += W[1][0];
-                    if (j < i + 8) sum[1][0] += u;
-                    u = run[half] + all[1] + ex[0] + W[0][1];
-                    if (j < i + 1) sum[0][1] += u;
-                    u += W[0][0];
-                    if (j < i) sum[0][0] += u;
-                    run[half] += all[1] + all[0];
-                }
-#pragma unroll
-                for (int q2 = 0; q2 < 2; ++q2)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) sum[q2][e] += __shfl_xor_sync(kFull, sum[q2][e], o);
-                        if (l < 4) sm.pairs[w][ib * 16 + q2 * 8 + 2 * lq + e] = sum[q2][e];
-                    }
-                uint32_t a[MS][4];
-                split_a<MS>(at[0], at[1], a);
-                gemm<MS, NS, MS, 1, PT / 16, true>(gv, [&](uint32_t(&r)[4], int s, int) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) r[e] = a[s][e];
-                }, ty, LP, piece_p, ib * 16, 0);
-            }
-            const RowsOut<T> ov{dv + t * v_st, nullptr, v_st};
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-                if (row + 8 * half < rows)
-#pragma unroll
-                    for (int pb = 0; pb < PT / 8; ++pb)
-                        ov.put2(row + 8 * half, pb * 8 + 2 * lq, cols, gv[pb][2 * half], gv[pb][2 * half + 1], pair_v);
-        } else {
-            // dk (rows as keys) and dq (rows as queries) are one form:  (dP o D) X + decay (V or dY) times the state's
-            // gradient or the state; the far part's dot with the row itself is its share of dg
-            const bool as_keys = group == 1;
-            float gx[NT / 8][4] = {};
-            const bf16* const own = as_keys ? tv : ty;
-            const bf16* const other = as_keys ? ty : tv;
-            const bf16* const mate = as_keys ? tq : tk;
-            auto lines = [&](uint32_t(&a)[4], int s, int kk) { load_a(a, own + s * piece_p, LP, w * 16, kk * 16); };
-            gemm<NS, kFull3, kFull3, PT / 16, NT / 16, false>(gx, lines, as_keys ? tds : ts, LP, piece_s, 0, 0);
-            const float* decay = as_keys ? sm.d.until : sm.d.since;
-            const float u0 = decay[row], u1 = decay[row + 8];
-#pragma unroll
-            for (int nb = 0; nb < NT / 8; ++nb) {
-                gx[nb][0] *= u0;
-                gx[nb][1] *= u0;
-                gx[nb][2] *= u1;
-                gx[nb][3] *= u1;
-            }
-            dots(gx, as_keys ? tk : tq, as_keys ? sm.of_k : sm.of_q);
-            const int from = as_keys ? w : 0, to = as_keys ? 4 : w + 1;
-#pragma unroll 1
-            for (int b = from; b < to; ++b) {
-                float dt[2][4] = {};
-                gemm<NS, NS, MS, PT / 16, 1, false>(dt, lines, other, LP, piece_p, 0, b * 16);
-                decayed(dt, b, as_keys);
-                uint32_t a[MS][4];
-                split_a<MS>(dt[0], dt[1], a);
-                gemm<MS, NS, MS, 1, NT / 16, true>(gx, [&](uint32_t(&r)[4], int s, int) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) r[e] = a[s][e];
-                }, mate, LN, piece_n, b * 16, 0);
-            }
+            __syncwarp();
+            sm.sync.wait(4 + group, phase);
             const RowsOut<T>& out = as_keys ? dk : dq;
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-                if (row + 8 * half < rows)
-#pragma unroll
-                    for (int nb = 0; nb < NT / 8; ++nb)
-                        out.put2(row_at + t + row + 8 * half, nb * 8 + 2 * lq, z.n, gx[nb][2 * half], gx[nb][2 * half + 1], pair_qk);
+            const int how = out.part ? alignment(out.part, qk_st) : alignment(out.whole, qk_st);
+            for (int nb = 0; nb < n16; ++nb) {
+                float x[2][4];
+                t5::ld16(x, acc + 16 * nb);
+                t5::wait_ld();
+                if (out.part) store_rows(out.part + (row_at + t) * qk_st, qk_st, rows, z.n, row, 16 * nb, x, how);
+                else store_rows(out.whole + (row_at + t) * qk_st, qk_st, rows, z.n, row, 16 * nb, x, how);
+            }
         }
+        t5::fence_before();
+        phase ^= 1;
     }
     __syncthreads();
+    sm.sync.end(Smem::cols);
 }
 
-template <typename T, int NT, int PT>
+template <typename T, int NT>
 bcm_status launch_bwd(const BwdArgs& p, cudaStream_t stream) {
-    using Smem = BwdSmem<T, NT, PT>;
-    static_assert(sizeof(Smem) <= 227 * 1024, "shared memory of a block");
-    static_assert(sizeof(typename Smem::Tiles) >= sizeof(float) * (NT * PT + 4 * NT + kBwdThreads + kBwdThreads / 32), "the state of back_tokens");
-    auto kernel = bwd_kernel<T, NT, PT>;
-    bcm_status st = allow_smem(kernel, sizeof(Smem));
+    using Smem = BwdSmem<T, NT>;
+    constexpr size_t smem = sizeof(Smem) + 1024;
+    static_assert(smem <= 227 * 1024, "shared memory of a block");
+    static_assert(sizeof(typename Smem::Tiles) >= sizeof(float) * (NT * kP + 4 * NT + kBwdThreads + kBwdThreads / 32), "the state of back_tokens");
+    static_assert(Smem::gq + NT <= 512 && (Smem::late || Smem::inc + NT <= 512), "tensor memory of a block");
+    auto kernel = bwd_kernel<T, NT>;
+    bcm_status st = allow_smem(kernel, smem);
     if (st != BCM_OK) return st;
-    kernel<<<(unsigned)(p.z.items * p.z.heads * p.z.slices), kBwdThreads, sizeof(Smem), stream>>>(p);
+    kernel<<<(unsigned)(p.z.items * p.z.heads * p.z.slices), kBwdThreads, smem, stream>>>(p);
     BCM_LAUNCH_CHECK();
     return BCM_OK;
 }
@@ -592,23 +681,19 @@ extern "C" bcm_status bcm_decay_attn_bwd(const bcm_decay_attn_args* a, cudaStrea
                v = rows_of(a->v, a->v_stride_b, a->v_stride_t, a->v_stride_h), dy = rows_of(a->dy, a->dy_stride_b, a->dy_stride_t, a->dy_stride_h);
     const bool apart = room.shares > 1, dg_parts = z.slices > 1 || room.fixed;
     const int64_t tokens = (int64_t)(z.cu ? 1 : z.batch) * z.seqlen;
-    return dispatch(a->dtype, padded_n(a->dim_k), plan.pt, [&](auto type, auto n, auto pt) -> bcm_status {
+    return dispatch(a->dtype, a->dim_k, [&](auto type, auto n) -> bcm_status {
         using T = decltype(type);
         bcm_status r = BCM_OK;
-        if constexpr (sizeof(T) == 4 && n == 128 && pt == 64) {
-            set_error("decay_attn_bwd: unplanned tile");
-            return BCM_ERR_INVALID_ARGUMENT;
-        } else {
             if (plan.cut) {
                 // without dy an item's own part is 0: its rows count as none
                 PartArgs pa{plan.z, q, dy, a->log_decay, a->g_stride_b, a->g_stride_t, a->g_stride_h, parts};
-                if ((r = launch_part<T, n, pt, true>(pa, stream)) != BCM_OK) return r;
+                if ((r = launch_part<T, n, true>(pa, stream)) != BCM_OK) return r;
                 if ((r = join(plan, parts, a->dh_last, true, stream)) != BCM_OK) return r;
             }
             const BwdArgs ba{plan.z, q, k, v, dy, a->log_decay, a->g_stride_b, a->g_stride_t, a->g_stride_h, (const float*)a->ckpt,
                              a->dh_last, parts.state, apart ? (void*)(ws + room.dq) : a->dq, apart ? (void*)(ws + room.dk) : a->dk,
                              a->dv, dg_parts ? (float*)(ws + room.dg) : a->dlog_decay, a->dh0, room.shares};
-            if ((r = launch_bwd<T, n, pt>(ba, stream)) != BCM_OK) return r;
+            if ((r = launch_bwd<T, n>(ba, stream)) != BCM_OK) return r;
             if (apart) {
                 const int64_t count = tokens * z.qk_heads * z.n;
                 if ((r = add_parts((const float*)(ws + room.dq), room.shares, count, (T*)a->dq, stream)) != BCM_OK) return r;
@@ -628,6 +713,5 @@ extern "C" bcm_status bcm_decay_attn_bwd(const bcm_decay_attn_args* a, cudaStrea
                 BCM_LAUNCH_CHECK();
             }
             return BCM_OK;
-        }
     });
 }

@@ -4,8 +4,6 @@
 namespace bcm {
 namespace decay_attn {
 
-int padded_n(int64_t n) { return n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 128; }
-
 bcm_status check(const bcm_decay_attn_args* a, const char* what) {
     BCM_REQUIRE(a != nullptr, "%s: null arguments", what);
     BCM_REQUIRE(dtype_ok(a->dtype), "%s: unsupported dtype %d", what, (int)a->dtype);
@@ -19,8 +17,8 @@ bcm_status check(const bcm_decay_attn_args* a, const char* what) {
 }
 
 // Blocks are (item, head, 64 columns of the values) and walk their item's chunks one after another.  Sequences are cut
-// into items only where whole ones leave the GPU short of blocks: an item costs one more pass over two inputs and
-// states to join.  An item has 256 tokens at least.
+// into items only where whole ones leave much of the GPU without a block: an item costs one more pass over two inputs
+// and states to join.  An item has 256 tokens at least.
 Plan plan_of(const bcm_decay_attn_args* a, bool backward) {
     Plan plan{};
     Sizes& z = plan.z;
@@ -31,23 +29,19 @@ Plan plan_of(const bcm_decay_attn_args* a, bool backward) {
     z.p = (int)a->dim_v;
     z.seqlen = (int)a->seqlen;
     z.cu = a->cu_seqlens;
-    // shared memory of the backward walk: two tiles of 128 x 64 in three pieces do not fit beside the others
-    const bool narrow = z.p <= 32 || (backward && a->dtype == BCM_F32 && z.n > 64);
-    plan.pt = narrow ? 32 : 64;
-    z.slices = ceil_div(z.p, plan.pt);
-    const int64_t across = (int64_t)z.heads * z.slices, want = 4 * sm_count();
+    z.slices = ceil_div(z.p, kP);
+    const int64_t across = (int64_t)z.heads * z.slices, room = (backward ? 1 : 2) * sm_count();
     const int64_t tokens = a->seqlen;
     auto chunks_up = [](int64_t v) { return std::max<int64_t>(256, (v + kChunk - 1) / kChunk * kChunk); };
     if (!z.cu) {
-        const int64_t blocks = std::max<int64_t>(1, z.batch * across);
-        const int64_t segs = blocks >= 2 * sm_count() ? 1 : (want + blocks - 1) / blocks;
-        z.span = (int)chunks_up((tokens + segs - 1) / std::max<int64_t>(1, segs));
+        const int64_t blocks = std::max<int64_t>(1, z.batch * across), segs = std::max<int64_t>(1, room / blocks);
+        z.span = (int)chunks_up((tokens + segs - 1) / segs);
         z.per_seq = std::max(1, ceil_div(tokens, z.span));
         z.items = z.batch * z.per_seq;
         z.chunks = z.batch * ceil_div(tokens, kChunk);
         plan.cut = z.per_seq > 1;
     } else {
-        z.span = (int)chunks_up((tokens * across + want - 1) / want);
+        z.span = (int)chunks_up((tokens * across + 2 * room - 1) / (2 * room));
         z.per_seq = 0;
         z.items = z.batch + (int)(tokens / z.span);
         z.chunks = z.batch + (int)(tokens / kChunk);
@@ -178,60 +172,70 @@ struct FwdArgs {
     const float* enter;        // [items][heads][n][p], or NULL where items are whole sequences
     void* y;                   // contiguous
     float* h_last;
-    float* ckpt;               // [chunks][heads][n][p] states that enter each chunk, or NULL
+    float* ckpt;               // [chunks][heads][slices][64][NT] transposed states that enter each chunk, or NULL
 };
 
-// Warps 0 to 3 form the outputs of 16 tokens each, warps 4 to 7 hold the state and advance it meanwhile.  Where there is
-// room for it the pieces of the next chunk's entering state go to a second buffer.
+// One thread issues all products of a chunk that need no other: Q K^T, Q S, and the state's V'^T K (V' the values times
+// their decays until the chunk's end).  Warps 0 to 3 take 16 queries each: they mask and decay the scores, put their
+// pieces back into tensor memory as an operand, and add the two parts of y.  Warps 4 to 7 hold the state and advance it
+// meanwhile.  The next chunk's tiles are on their way to registers during all of that.
 constexpr int kFwdThreads = 256;
 
-template <typename T, int NT, int PT>
+template <typename T, int NT>
 struct FwdSmem {
     static constexpr int NS = Pieces<T>::in, MS = Pieces<T>::out;
     struct Tiles {
-        bf16 q[NS][kChunk][NT + 8], k[NS][kChunk][NT + 8], v[NS][kChunk][PT + 8];
+        bf16 q[NS][Wide<NT>::elements], k[NS][Wide<NT>::elements], v[NS][Wide<kP>::elements];
+        bf16 vw[kFull3][Wide<kP>::elements];
     } tiles;
-    static constexpr int buffers = sizeof(Tiles) + 2 * sizeof(bf16[MS][NT][PT + 8]) <= 110 * 1024 ? 2 : 1;
-    bf16 s[buffers][MS][NT][PT + 8];
-    Decays d;
+    bf16 s[MS][Wide<NT>::elements];
+    Decays d[2];
+    Sync<4> sync;
+
+    // tensor memory: scores, then their pieces (32 columns each); the near and the far part of y; the state's increase.
+    // Beside a state of 128 there is no room for both parts: the far one is decayed in place and the near one added to it.
+    static constexpr bool apart = NT <= 64;
+    static constexpr uint32_t scores = 0, near = MS > 2 ? 96 : 64, far = apart ? near + 64 : near, inc = far + 64;
+    static constexpr uint32_t cols = inc + NT <= 256 ? 256 : 512;
+    static constexpr int resident = cols == 256 && sizeof(Tiles) + sizeof(bf16[MS][Wide<NT>::elements]) <= 108 * 1024 ? 2 : 1;   // blocks on an SM
 };
 
 // A chunk with a value that is not finite, token by token: 0 times such a value would spread it to tokens before it.
-// `s` (shared, NT x PT) holds the state before and after, `sum` a float for each thread.
-template <typename T, int NT, int PT>
+// `s` (shared, NT x kP) holds the state before and after, `sum` a float for each thread.
+template <typename T>
 __device__ __noinline__ void walk_tokens(const FwdArgs& p, const T* q, const T* k, const T* v, const float* g, T* y, int rows, int cols,
                                          float* s, float* sum) {
-    constexpr int parts = kFwdThreads / PT;
-    const int c = threadIdx.x % PT, part = threadIdx.x / PT;
+    constexpr int parts = kFwdThreads / kP;
+    const int c = threadIdx.x % kP, part = threadIdx.x / kP;
     for (int t = 0; t < rows; ++t) {
         const float a = expf(g[(int64_t)t * p.g_st]), x = c < cols ? to_f32(v[(int64_t)t * p.v.st + c]) : 0.0f;
         float got = 0.0f;
         for (int n = part; n < p.z.n; n += parts) {
-            const float now = fmaf(a, s[n * PT + c], to_f32(k[(int64_t)t * p.k.st + n]) * x);
-            s[n * PT + c] = now;
+            const float now = fmaf(a, s[n * kP + c], to_f32(k[(int64_t)t * p.k.st + n]) * x);
+            s[n * kP + c] = now;
             got = fmaf(to_f32(q[(int64_t)t * p.q.st + n]), now, got);
         }
         sum[threadIdx.x] = got;
         __syncthreads();
         if (part == 0 && c < cols) {
-            for (int k2 = 1; k2 < parts; ++k2) got += sum[k2 * PT + c];
+            for (int k2 = 1; k2 < parts; ++k2) got += sum[k2 * kP + c];
             y[(int64_t)t * p.z.heads * p.z.p + c] = from_f32<T>(got);
         }
         __syncthreads();
     }
 }
 
-template <typename T, int NT, int PT>
-__global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT, PT>::buffers) fwd_kernel(const __grid_constant__ FwdArgs p) {
-    extern __shared__ __align__(16) unsigned char smem_raw[];
-    using Smem = FwdSmem<T, NT, PT>;
-    Smem& sm = *(Smem*)smem_raw;
-    constexpr int NS = Smem::NS, MS = Smem::MS, LN = NT + 8, LP = PT + 8;
+template <typename T, int NT>
+__global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_kernel(const __grid_constant__ FwdArgs p) {
+    extern __shared__ unsigned char smem_raw[];
+    using Smem = FwdSmem<T, NT>;
+    Smem& sm = *(Smem*)tiles_base(smem_raw);
+    constexpr int NS = Smem::NS, MS = Smem::MS;
     const Sizes& z = p.z;
     const int across = z.heads * z.slices;
-    const int item = blockIdx.x / across, hs = blockIdx.x % across, h = hs / z.slices, col = hs % z.slices * PT;
+    const int item = blockIdx.x / across, hs = blockIdx.x % across, h = hs / z.slices, col = hs % z.slices * kP;
     const int64_t y_st = (int64_t)z.heads * z.p;
-    const int cols = min(PT, z.p - col), hq = h / (z.heads / z.qk_heads);
+    const int cols = min(kP, z.p - col), hq = h / (z.heads / z.qk_heads);
     if (z.cu)
         zero_rows((T*)p.y + (int64_t)h * z.p + col, z.tables.seq_item[z.batch + 1], z.seqlen, y_st, cols, item, z.items);
     const Item it = item_of(z, item);
@@ -241,18 +245,15 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT, PT>::buffers) fwd_
     const T* v = row_ptr<T>(p.v, z, it.seq, it.t0, h) + col;
     const float* g = p.g + (z.cu ? 0 : it.seq * p.g_sb) + it.t0 * p.g_st + h * p.g_sh;
     T* y = (T*)p.y + ((z.cu ? 0 : (int64_t)it.seq * z.seqlen) + it.t0) * y_st + (int64_t)h * z.p + col;
-    const bool vq = on_16(q, p.q.st), vk = on_16(k, p.k.st), vv = on_16(v, p.v.st);
-    const bool pair_y = (((uintptr_t)y | (uintptr_t)(y_st * sizeof(T))) & (2 * sizeof(T) - 1)) == 0;
+    const int vq = alignment(q, p.q.st), vk = alignment(k, p.k.st), vv = alignment(v, p.v.st), vy = alignment(y, y_st);
     const int np = z.n * z.p;
     const int len = it.t1 - it.t0, nc = (len + kChunk - 1) / kChunk;
     const int l = lane_id(), w = (threadIdx.x >> 5) & 3, row = w * 16 + (l >> 2);
     const bool state_warp = threadIdx.x >= 128, decay_warp = threadIdx.x >= 128 && threadIdx.x < 160;
-    bf16* const tq = &sm.tiles.q[0][0][0];
-    bf16* const tk = &sm.tiles.k[0][0][0];
-    bf16* const tv = &sm.tiles.v[0][0][0];
+    const int p16 = (cols + 15) / 16;
 
-    Pending<T, kChunk, NT, kFwdThreads> pq, pk;
-    Pending<T, kChunk, PT, kFwdThreads> pv;
+    Pending<T, NT, kFwdThreads> pq, pk;
+    Pending<T, kP, kFwdThreads> pv;
     float g0 = 0.0f, g1 = 0.0f;
     auto fetch = [&](int c) {
         const int t = c * kChunk, rows = min(kChunk, len - t);
@@ -265,134 +266,186 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT, PT>::buffers) fwd_
         }
     };
     // the tiles of the fetched chunk; whether a value was not finite
-    auto put = [&]() {
-        bool bad = pq.put(tq, LN);
-        bad |= pk.put(tk, LN);
-        bad |= pv.put(tv, LP);
-        if (decay_warp) {
-            bad |= !(g0 <= 3.38e38f && g1 <= 3.38e38f);
-            decays_of(sm.d, g0, g1);
-        }
+    auto put = [&](int c) {
+        bool bad = pq.bad() | pk.bad() | pv.bad();
+        if (decay_warp) bad |= !(g0 <= 3.38e38f && g1 <= 3.38e38f);
+        pq.put(sm.tiles.q[0]);
+        pk.put(sm.tiles.k[0]);
+        pv.put(sm.tiles.v[0]);
+        pv.put_weighted(sm.tiles.vw[0], sm.d[c & 1].until);
+        t5::fence_smem();
+        t5::fence_before();
         return bad;
     };
     // token by token, the state through shared memory
     auto walk = [&](int c) {
         const int t = c * kChunk;
         float* f = (float*)&sm.tiles;
-        walk_tokens<T, NT, PT>(p, q + t * p.q.st, k + t * p.k.st, v + t * p.v.st, g + t * p.g_st, y + t * y_st, min(kChunk, len - t), cols, f,
-                               f + NT * PT);
+        walk_tokens<T>(p, q + t * p.q.st, k + t * p.k.st, v + t * p.v.st, g + t * p.g_st, y + t * y_st, min(kChunk, len - t), cols, f, f + NT * kP);
     };
     if (nc > 0) fetch(0);
+    sm.sync.init(Smem::cols);
+    const uint32_t tm = sm.sync.tmem, lanes = (uint32_t)w << 21;
+    uint32_t phase = 0;
 
     if (state_warp) {
-        State<NT, PT> st;
+        State<NT> st;
         const float* from = it.first ? (p.h0 ? p.h0 + ((int64_t)it.seq * z.heads + h) * np : nullptr)
                                      : p.enter + ((int64_t)item * z.heads + h) * np;
-        if (from) st.load(from + col, z.n, z.p - col, z.p);
+        if (decay_warp) decays_of(sm.d[0], g0, g1);
+        if (from) st.load(from + col, z.n, cols, z.p);
         else st.zero();
-        bool bad = false;
-        if (Smem::buffers > 1) bad = st.template put<MS>(&sm.s[0][0][0][0]);
+        bool bad = st.template put<MS>(sm.s[0]);
         for (int c = 0; c < nc; ++c) {
-            if (p.ckpt) st.store(p.ckpt + ((int64_t)(it.chunk + c) * z.heads + h) * np + col, z.n, z.p - col, z.p);
-            __syncthreads();
-            bad |= put();
-            if (Smem::buffers == 1) bad |= st.template put<MS>(&sm.s[0][0][0][0]);
+            if (p.ckpt) {
+                float* to = p.ckpt + (((int64_t)(it.chunk + c) * z.heads + h) * z.slices + hs % z.slices) * (NT * kP);
+                st.pairs([&](float& x, float& y1, int pp, int n) {
+                    if (pp < cols) *(float2*)(to + pp * NT + n) = make_float2(x, y1);
+                });
+            }
+            __syncthreads();                                  // decays are there; the chunk before is done with the tiles
+            bad |= put(c);
             const bool slow = __syncthreads_or(bad);
-            if (c + 1 < nc) fetch(c + 1);
+            const float whole = sm.d[c & 1].whole;
+            if (c + 1 < nc) {
+                fetch(c + 1);
+                if (decay_warp) decays_of(sm.d[(c + 1) & 1], g0, g1);
+            }
             if (slow) {
                 float* f = (float*)&sm.tiles;
-                st.pairs([&](float& x, float& x1, int r, int cc) {
-                    f[r * PT + cc] = x;
-                    f[r * PT + cc + 1] = x1;
+                st.pairs([&](float& x, float& x1, int pp, int n) {
+                    f[n * kP + pp] = x;
+                    f[(n + 1) * kP + pp] = x1;
                 });
                 __syncthreads();
                 walk(c);
-                st.pairs([&](float& x, float& x1, int r, int cc) {
-                    x = f[r * PT + cc];
-                    x1 = f[r * PT + cc + 1];
+                st.pairs([&](float& x, float& x1, int pp, int n) {
+                    x = f[n * kP + pp];
+                    x1 = f[(n + 1) * kP + pp];
                 });
             } else {
-                st.template advance<NS>(tk, tv, sm.d.until, sm.d.whole);
+                sm.sync.wait(2, phase);
+                st.advance(tm + Smem::inc + lanes, whole);
+                sm.sync.wait(1, phase);                       // the products with the entering state have read it
+                t5::fence_before();
+                phase ^= 1;
             }
-            bad = false;
-            if (Smem::buffers > 1) bad = st.template put<MS>(&sm.s[(c + 1) % Smem::buffers][0][0][0]);
+            bad = st.template put<MS>(sm.s[0]);
         }
-        if (it.last) st.store(p.h_last + ((int64_t)it.seq * z.heads + h) * np + col, z.n, z.p - col, z.p);
+        if (sm.sync.failed) st.pairs([](float& x, float& y1, int, int) { x = y1 = __int_as_float(0x7fc00000); });
+        if (it.last) st.store(p.h_last + ((int64_t)it.seq * z.heads + h) * np + col, z.n, cols, z.p);
+        sm.sync.end(Smem::cols);
         return;
     }
     for (int c = 0; c < nc; ++c) {
         const int t = c * kChunk, rows = min(kChunk, len - t);
-        __syncthreads();                                      // the chunk before is done with the tiles
-        const bool bad = put();
-        const bool slow = __syncthreads_or(bad);
-        if (c + 1 < nc) fetch(c + 1);
+        __syncthreads();
+        const bool slow = __syncthreads_or(put(c));
         if (slow) {
+            if (c + 1 < nc) fetch(c + 1);
             __syncthreads();
             walk(c);
             continue;
         }
-        // 16 queries: the entering state's part, then those of the keys up to their own
-        float acc[PT / 8][4] = {};
-        const bf16* ts = &sm.s[c % Smem::buffers][0][0][0];
-        auto queries = [&](uint32_t(&a)[4], int s, int kk) { load_a(a, tq + s * kChunk * LN, LN, w * 16, kk * 16); };
-        gemm<NS, MS, MS, NT / 16, PT / 16, true>(acc, queries, ts, LP, NT * LP, 0, 0);
-        const float since0 = sm.d.since[row], since1 = sm.d.since[row + 8];
-#pragma unroll
-        for (int pb = 0; pb < PT / 8; ++pb) {
-            acc[pb][0] *= since0;
-            acc[pb][1] *= since0;
-            acc[pb][2] *= since1;
-            acc[pb][3] *= since1;
+        if (threadIdx.x == 0) {
+            t5::fence_after();
+            const Operand<NT, true> Q{t5::smem_u32(sm.tiles.q)}, K{t5::smem_u32(sm.tiles.k)}, S{t5::smem_u32(sm.s)};
+            const Operand<NT, false> Kt{t5::smem_u32(sm.tiles.k)};
+            const Operand<kP, false> V{t5::smem_u32(sm.tiles.vw)};
+            auto fq = [&](int s, int i) { return Q.desc(s, i); };
+            const int n16 = (z.n + 15) / 16;
+            products<NS, NS, MS>(tm + Smem::scores, fq, [&](int u, int i) { return K.desc(u, i); }, n16, t5::instr(kChunk, false, false), false);
+            t5::commit(&sm.sync.bars[0]);
+            products<NS, MS, MS>(tm + Smem::far, fq, [&](int u, int i) { return S.desc(u, i); }, n16, t5::instr(p16 * 16, false, false), false);
+            t5::commit(&sm.sync.bars[1]);
+            products<kFull3, NS, kFull3>(tm + Smem::inc, [&](int s, int i) { return V.desc(s, i); }, [&](int u, int i) { return Kt.desc(u, i); },
+                                         kChunk / 16, t5::instr(NT, true, true), false);
+            t5::commit(&sm.sync.bars[2]);
         }
-        const float hi0 = sm.d.hi[row], lo0 = sm.d.lo[row], hi1 = sm.d.hi[row + 8], lo1 = sm.d.lo[row + 8];
-#pragma unroll 1
-        for (int jb = 0; jb <= w; ++jb) {
-            float sc[2][4] = {};
-            gemm<NS, NS, MS, NT / 16, 1, false>(sc, queries, tk, LN, kChunk * LN, 0, jb * 16);
+        __syncwarp();
+        if (c + 1 < nc) fetch(c + 1);
+        const Decays& d = sm.d[c & 1];
+        const float hi0 = d.hi[row], lo0 = d.lo[row], hi1 = d.hi[row + 8], lo1 = d.lo[row + 8], since0 = d.since[row], since1 = d.since[row + 8];
+        sm.sync.wait(0, phase);
+        float sc[4][2][4];
 #pragma unroll
-            for (int q2 = 0; q2 < 2; ++q2) {
-                const int j = jb * 16 + q2 * 8 + 2 * (l & 3);
-                const float2 hj = *(const float2*)&sm.d.hi[j], lj = *(const float2*)&sm.d.lo[j];
-                sc[q2][0] = j <= row ? sc[q2][0] * between(hi0, lo0, hj.x, lj.x) : 0.0f;
-                sc[q2][1] = j + 1 <= row ? sc[q2][1] * between(hi0, lo0, hj.y, lj.y) : 0.0f;
-                sc[q2][2] = j <= row + 8 ? sc[q2][2] * between(hi1, lo1, hj.x, lj.x) : 0.0f;
-                sc[q2][3] = j + 1 <= row + 8 ? sc[q2][3] * between(hi1, lo1, hj.y, lj.y) : 0.0f;
-            }
-            uint32_t a[MS][4];
-            split_a<MS>(sc[0], sc[1], a);
-            gemm<MS, NS, MS, 1, PT / 16, true>(acc, [&](uint32_t(&r)[4], int s, int) {
+        for (int jb = 0; jb < 4; ++jb)
+            if (jb <= w) t5::ld16(sc[jb], tm + Smem::scores + lanes + 16 * jb);
+        t5::wait_ld();
 #pragma unroll
-                for (int e = 0; e < 4; ++e) r[e] = a[s][e];
-            }, tv, LP, kChunk * LP, jb * 16, 0);
-        }
+        for (int jb = 0; jb < 4; ++jb) {
+            uint32_t r[2][2][MS] = {};                        // [tile][half]
+            if (jb <= w)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int r = row + 8 * half;
-            if (r < rows) {
-                T* out = y + (int64_t)(t + r) * y_st;
-#pragma unroll
-                for (int pb = 0; pb < PT / 8; ++pb) {
-                    const int cc = pb * 8 + 2 * (l & 3);
-                    struct alignas(2 * sizeof(T)) Two { T x, y; };
-                    const T x0 = from_f32<T>(acc[pb][2 * half]), x1 = from_f32<T>(acc[pb][2 * half + 1]);
-                    if (pair_y && cc + 1 < cols) {
-                        *(Two*)(out + cc) = Two{x0, x1};
-                    } else {
-                        if (cc < cols) out[cc] = x0;
-                        if (cc + 1 < cols) out[cc + 1] = x1;
-                    }
+                for (int q2 = 0; q2 < 2; ++q2) {
+                    const int j = jb * 16 + q2 * 8 + 2 * (l & 3);
+                    const float2 hj = *(const float2*)&d.hi[j], lj = *(const float2*)&d.lo[j];
+                    float(&x)[4] = sc[jb][q2];
+                    x[0] = j <= row ? x[0] * between(hi0, lo0, hj.x, lj.x) : 0.0f;
+                    x[1] = j + 1 <= row ? x[1] * between(hi0, lo0, hj.y, lj.y) : 0.0f;
+                    x[2] = j <= row + 8 ? x[2] * between(hi1, lo1, hj.x, lj.x) : 0.0f;
+                    x[3] = j + 1 <= row + 8 ? x[3] * between(hi1, lo1, hj.y, lj.y) : 0.0f;
+                    split<MS>(x[0], x[1], r[q2][0]);
+                    split<MS>(x[2], x[3], r[q2][1]);
                 }
+#pragma unroll
+            for (int m = 0; m < MS; ++m) t5::st16(tm + Smem::scores + lanes + 32 * m + 8 * jb, r[0][0][m], r[0][1][m], r[1][0][m], r[1][1][m]);
+        }
+        if (!Smem::apart) {
+            sm.sync.wait(1, phase);
+            for (int pb = 0; pb < p16; ++pb) {
+                float x[2][4];
+                t5::ld16(x, tm + Smem::far + lanes + 16 * pb);
+                t5::wait_ld();
+#pragma unroll
+                for (int q2 = 0; q2 < 2; ++q2)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[q2][e] *= e < 2 ? since0 : since1;
+                t5::st_acc16(tm + Smem::far + lanes + 16 * pb, x);
             }
         }
+        t5::wait_st();
+        t5::fence_before();
+        named_sync(1, 128);
+        if (threadIdx.x == 0) {
+            t5::fence_after();
+            const Operand<kP, false> V{t5::smem_u32(sm.tiles.v)};
+            products<MS, NS, MS>(tm + Smem::near, [&](int s, int i) { return tm + Smem::scores + 32 * s + 8 * i; },
+                                 [&](int u, int i) { return V.desc(u, i); }, kChunk / 16, t5::instr(p16 * 16, false, true), !Smem::apart);
+            t5::commit(&sm.sync.bars[3]);
+        }
+        __syncwarp();
+        sm.sync.wait(3, phase);                               // (and with it the far part)
+        T* const out = y + (int64_t)t * y_st;
+        for (int pb = 0; pb < p16; ++pb) {
+            float x[2][4];
+            t5::ld16(x, tm + Smem::near + lanes + 16 * pb);
+            if (Smem::apart) {
+                float f[2][4];
+                t5::ld16(f, tm + Smem::far + lanes + 16 * pb);
+                t5::wait_ld();
+#pragma unroll
+                for (int q2 = 0; q2 < 2; ++q2)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[q2][e] = fmaf(e < 2 ? since0 : since1, f[q2][e], x[q2][e]);
+            } else {
+                t5::wait_ld();
+            }
+            store_rows(out, y_st, rows, cols, row, 16 * pb, x, vy);
+        }
+        t5::fence_before();
+        phase ^= 1;
     }
+    sm.sync.end(Smem::cols);
 }
 
-template <typename T, int NT, int PT>
+template <typename T, int NT>
 bcm_status launch_fwd(const FwdArgs& p, cudaStream_t stream) {
-    constexpr size_t smem = sizeof(FwdSmem<T, NT, PT>);
+    using Smem = FwdSmem<T, NT>;
+    constexpr size_t smem = sizeof(Smem) + 1024;
     static_assert(smem <= 227 * 1024, "shared memory of a block");
-    static_assert(sizeof(typename FwdSmem<T, NT, PT>::Tiles) >= sizeof(float) * (NT * PT + kFwdThreads), "the state of walk_tokens");
-    auto kernel = fwd_kernel<T, NT, PT>;
+    static_assert(sizeof(typename Smem::Tiles) >= sizeof(float) * (NT * kP + kFwdThreads), "the state of walk_tokens");
+    auto kernel = fwd_kernel<T, NT>;
     bcm_status st = allow_smem(kernel, smem);
     if (st != BCM_OK) return st;
     kernel<<<(unsigned)(p.z.items * p.z.heads * p.z.slices), kFwdThreads, smem, stream>>>(p);
@@ -475,7 +528,8 @@ using namespace bcm::decay_attn;
 extern "C" size_t bcm_decay_attn_ckpt_bytes(const bcm_decay_attn_args* a) {
     if (check(a, "decay_attn") != BCM_OK) return 0;
     const Plan plan = plan_of(a, false);
-    return sizeof(float) * (size_t)plan.z.chunks * plan.z.heads * plan.z.n * plan.z.p;
+    const int nt = plan.z.n <= 16 ? 16 : plan.z.n <= 32 ? 32 : plan.z.n <= 64 ? 64 : 128;
+    return sizeof(float) * (size_t)plan.z.chunks * plan.z.heads * plan.z.slices * kP * nt;
 }
 
 extern "C" size_t bcm_decay_attn_fwd_workspace_bytes(const bcm_decay_attn_args* a) {
@@ -498,17 +552,17 @@ extern "C" bcm_status bcm_decay_attn_fwd(const bcm_decay_attn_args* a, cudaStrea
     const Parts parts = parts_of(plan, a->workspace);
     const Rows q = rows_of(a->q, a->q_stride_b, a->q_stride_t, a->q_stride_h), k = rows_of(a->k, a->k_stride_b, a->k_stride_t, a->k_stride_h),
                v = rows_of(a->v, a->v_stride_b, a->v_stride_t, a->v_stride_h);
-    return dispatch(a->dtype, padded_n(a->dim_k), plan.pt, [&](auto type, auto n, auto p) -> bcm_status {
+    return dispatch(a->dtype, a->dim_k, [&](auto type, auto n) -> bcm_status {
         using T = decltype(type);
         if (plan.cut) {
             const PartArgs pa{plan.z, k, v, a->log_decay, a->g_stride_b, a->g_stride_t, a->g_stride_h, parts};
-            bcm_status r = launch_part<T, n, p, false>(pa, stream);
+            bcm_status r = launch_part<T, n, false>(pa, stream);
             if (r != BCM_OK) return r;
             if ((r = join(plan, parts, a->h0, false, stream)) != BCM_OK) return r;
         }
         const FwdArgs fa{plan.z, q, k, v, a->log_decay, a->g_stride_b, a->g_stride_t, a->g_stride_h, a->h0, parts.state,
                          a->y, a->h_last, (float*)a->ckpt};
-        return launch_fwd<T, n, p>(fa, stream);
+        return launch_fwd<T, n>(fa, stream);
     });
 }
 

@@ -75,33 +75,35 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // --------------------------------------------------------------------- products ----
-// An operand of NT columns at a shared address, its pieces one behind the other; K: columns along the sum, else rows.
+// An operand of NT columns, its pieces one behind the other; K: columns along the sum, else rows.
 template <int NT, bool K>
 struct Operand {
     using X = Wide<NT>;
-    uint32_t addr;
-    __device__ __forceinline__ uint64_t desc(int piece, int step) const {
+    uint32_t base;
+    __device__ __forceinline__ explicit Operand(const void* m) {
+        base = X::Tile::low(t5::smem_u32(m), X::Tile::bytes);
+    }
+    // of a piece's step of 16 along the sum (constants once loops are unrolled; shared addresses do not leave the field)
+    __device__ __forceinline__ t5::Desc operator()(int piece, int step) const {
         constexpr int in_tile = X::W / 16;
-        const uint32_t off = piece * X::bytes + (K ? step / in_tile * X::Tile::bytes + step % in_tile * X::Tile::step_k : step * X::Tile::step_mn);
-        return X::Tile::desc(addr + off, X::Tile::bytes);
+        const int off = piece * X::bytes + (K ? step / in_tile * X::Tile::bytes + step % in_tile * X::Tile::step_k : step * X::Tile::step_mn);
+        return t5::Desc{base + (uint32_t)(off >> 4), X::Tile::high};
     }
 };
 
-// d (+)= A B over `steps` of 16, products (s, u) of A's NA and B's NB pieces with s + u < D, small ones first; one thread.
+// d (+)= A B over STEPS of 16, products (s, u) of A's NA and B's NB pieces with s + u < D, small ones first; one thread.
 // a(s, step), b(u, step): descriptors (or A's address in tensor memory)
-template <int NA, int NB, int D, typename FA, typename FB>
-__device__ __forceinline__ void products(uint32_t d, FA&& a, FB&& b, int steps, uint32_t idesc, bool add) {
+template <int NA, int NB, int D, int STEPS, typename FA, typename FB>
+__device__ __forceinline__ void products(uint32_t d, FA&& a, FB&& b, uint32_t idesc, bool add) {
 #pragma unroll
     for (int order = (NA + NB - 2 < D - 1 ? NA + NB - 2 : D - 1); order >= 0; --order)
 #pragma unroll
         for (int s = 0; s < NA; ++s) {
             const int u = order - s;
             if (u < 0 || u >= NB) continue;
-#pragma unroll 1
-            for (int k = 0; k < steps; ++k) {
-                const auto x = a(s, k);
-                if constexpr (sizeof(x) == 4) t5::mma_ts(d, x, b(u, k), idesc, add);
-                else t5::mma_ss(d, x, b(u, k), idesc, add);
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) {
+                t5::mma(d, a(s, k), b(u, k), idesc, add);
                 add = true;
             }
         }
@@ -198,114 +200,116 @@ __device__ __forceinline__ const T* row_ptr(const Rows& r, const Sizes& z, int s
 }
 
 // ---------------------------------------------------------------------- tiles ----
-// whether v's pieces are not finite
-__device__ __forceinline__ bool not_finite(float v) { return !(fabsf(v) <= 3.38e38f); }
-
-template <typename T> struct alignas(16) Eight { T v[8]; };
+// 0 as long as every value seen has finite pieces (those of a float32 next to the largest round up to infinity)
+__device__ __forceinline__ float seen(float v, float so_far) { return fmaf(v * 1.00390625f, 0.0f, so_far); }
 
 // 64 rows x W columns on their way to shared memory: each of TH threads has groups of eight columns.  Rows and columns
-// behind the last are 0.
-template <typename T, int W, int TH>
+// behind the last are 0.  VEC: rows on 16 bytes, a multiple of 8 columns.  What is loaded is not touched before put(), so
+// that nothing waits for it earlier.
+template <typename T, int W, int TH, bool VEC>
 struct Pending {
-    static constexpr int all = 64 * W / 8, n = (all + TH - 1) / TH;
-    Eight<T> g[n];
+    static constexpr int all = 64 * W / 8, n = (all + TH - 1) / TH, step = TH / (W / 8);    // rows between a thread's groups
+    static_assert(TH % (W / 8) == 0 && step % 8 == 0, "a thread's groups lie in one column, alike in the swizzle");
+    using Word = typename std::conditional<sizeof(T) == 4, float, typename std::conditional<VEC, uint32_t, unsigned short>::type>::type;
+    static constexpr int words = VEC ? 2 * (int)sizeof(T) : 8;
+    Word g[n][words];
 
-    __device__ __forceinline__ static int row(int i) { return (threadIdx.x + i * TH) / (W / 8); }
-    __device__ __forceinline__ static int col(int i) { return (threadIdx.x + i * TH) % (W / 8) * 8; }
+    __device__ __forceinline__ static int row0() { return threadIdx.x / (W / 8); }
+    __device__ __forceinline__ static int col() { return threadIdx.x % (W / 8) * 8; }
+    __device__ __forceinline__ static bool mine(int i) { return all % TH == 0 || threadIdx.x + i * TH < all; }
 
-    // how: elements at a time that the rows' alignment allows (8, 2 or 1)
-    __device__ __forceinline__ void fetch(const T* src, int64_t stride, int rows, int cols, int how) {
-        if (how == 8) {
+    __device__ __forceinline__ void fetch(const T* src, int64_t stride, int rows, int cols) {
+        const T* p = src + row0() * stride + col();
+        const int in = cols - col();
 #pragma unroll
-            for (int i = 0; i < n; ++i) {
-                const T* p = src + row(i) * stride + col(i);
-                if (row(i) < rows && col(i) + 8 <= cols) {
+        for (int i = 0; i < n; ++i, p += step * stride) {
+            const bool here = row0() + i * step < rows;
+            if (VEC) {
 #pragma unroll
-                    for (int u = 0; u < (int)sizeof(T) / 2; ++u) ((uint4*)&g[i])[u] = ((const uint4*)p)[u];
-                } else {
-#pragma unroll
-                    for (int u = 0; u < 8; ++u) g[i].v[u] = row(i) < rows && col(i) + u < cols ? p[u] : from_f32<T>(0.0f);
-                }
-            }
-            return;
-        }
-        using Two = typename std::conditional<sizeof(T) == 4, uint2, uint32_t>::type;
-#pragma unroll
-        for (int i = 0; i < n; ++i) {
-            const T* p = src + row(i) * stride + col(i);
-            const int in = row(i) < rows ? cols - col(i) : 0;
-            if (how == 2) {
-#pragma unroll
-                for (int u = 0; u < 8; u += 2) {
-                    if (u + 2 <= in) {
-                        *(Two*)&g[i].v[u] = *(const Two*)(p + u);
-                    } else {
-                        g[i].v[u] = u < in ? p[u] : from_f32<T>(0.0f);
-                        g[i].v[u + 1] = from_f32<T>(0.0f);
-                    }
+                for (int u = 0; u < (int)sizeof(T) / 2; ++u) {
+                    uint4 q = make_uint4(0, 0, 0, 0);
+                    if (here && in > 0) q = ((const uint4*)p)[u];
+                    ((uint32_t*)g[i])[4 * u] = q.x;
+                    ((uint32_t*)g[i])[4 * u + 1] = q.y;
+                    ((uint32_t*)g[i])[4 * u + 2] = q.z;
+                    ((uint32_t*)g[i])[4 * u + 3] = q.w;
                 }
             } else {
 #pragma unroll
-                for (int u = 0; u < 8; ++u) g[i].v[u] = u < in ? p[u] : from_f32<T>(0.0f);
+                for (int u = 0; u < 8; ++u) {
+                    Word x = 0;
+                    if (here && u < in) x = ((const Word*)p)[u];
+                    g[i][u] = x;
+                }
             }
         }
     }
+    // two of a group's values, as loaded (16-bit types)
+    __device__ __forceinline__ uint32_t pair(int i, int u) const {
+        if constexpr (sizeof(T) == 4) return 0;
+        else return VEC ? (uint32_t)g[i][u] : (uint32_t)g[i][2 * u] | (uint32_t)g[i][2 * u + 1] << 16;
+    }
+    __device__ __forceinline__ float2 two(int i, int u) const {
+        if constexpr (sizeof(T) == 4) {
+            return make_float2(g[i][2 * u], g[i][2 * u + 1]);
+        } else {
+            const uint32_t r = pair(i, u);
+            if constexpr (std::is_same<T, bf16>::value) return make_float2(low_f(r), high_f(r));
+            else return __half22float2(*(const __half2*)&r);
+        }
+    }
+    // whether a value is not finite
     __device__ __forceinline__ bool bad() const {
-        bool b = false;
+        if constexpr (std::is_same<T, bf16>::value) {
+            __nv_bfloat162 sum = __float2bfloat162_rn(0.0f);
 #pragma unroll
-        for (int i = 0; i < n; ++i) {
-            if (all % TH != 0 && threadIdx.x + i * TH >= all) continue;
-            if constexpr (std::is_same<T, bf16>::value) {
-                const uint4 q = *(const uint4*)&g[i];
-                const uint32_t e = 0x7f807f80u;                        // exponents of all ones
-                b |= (__vcmpeq2(q.x & e, e) | __vcmpeq2(q.y & e, e) | __vcmpeq2(q.z & e, e) | __vcmpeq2(q.w & e, e)) != 0;
-            } else {
+            for (int i = 0; i < n; ++i)
 #pragma unroll
-                for (int u = 0; u < 8; ++u) b |= not_finite(to_f32(g[i].v[u]));
+                for (int u = 0; u < 4; ++u) {
+                    const uint32_t r = pair(i, u);
+                    sum = __hfma2(*(const __nv_bfloat162*)&r, __float2bfloat162_rn(0.0f), sum);
+                }
+            return (*(const uint32_t*)&sum & 0x7fff7fffu) != 0;        // (0 times what is not finite is NaN)
+        } else {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < n; ++i)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const float2 v = two(i, u);
+                    sum = seen(v.x, seen(v.y, sum));
+                }
+            return sum != 0.0f;
+        }
+    }
+    // M pieces of the values, or of the values times their row's weight
+    template <int M, bool WEIGHTED>
+    __device__ __forceinline__ void put(bf16* dst, const float* weight) const {
+        bf16* to = dst + Wide<W>::at(row0(), col());
+#pragma unroll
+        for (int i = 0; i < n; ++i, to += step * Wide<W>::W) {
+            if (!mine(i)) continue;
+            const float w = WEIGHTED ? weight[row0() + i * step] : 1.0f;
+            uint32_t r[4][M];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if constexpr (std::is_same<T, bf16>::value && M == 1) {
+                    r[u][0] = pair(i, u);
+                } else {
+                    const float2 v = two(i, u);
+                    split<M>(WEIGHTED ? v.x * w : v.x, WEIGHTED ? v.y * w : v.y, r[u]);
+                }
             }
-        }
-        return b;
-    }
-    // the values' pieces
-    __device__ __forceinline__ void put(bf16* dst) const {
-        constexpr int NS = Pieces<T>::in;
 #pragma unroll
-        for (int i = 0; i < n; ++i) {
-            if (all % TH != 0 && threadIdx.x + i * TH >= all) continue;
-            bf16* to = dst + Wide<W>::at(row(i), col(i));
-            if constexpr (NS == 1) {
-                *(uint4*)to = *(const uint4*)&g[i];
-            } else {
-                uint32_t r[4][NS];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) split<NS>(to_f32(g[i].v[2 * u]), to_f32(g[i].v[2 * u + 1]), r[u]);
-#pragma unroll
-                for (int s = 0; s < NS; ++s) *(uint4*)(to + s * Wide<W>::elements) = make_uint4(r[0][s], r[1][s], r[2][s], r[3][s]);
-            }
+            for (int s = 0; s < M; ++s) *(uint4*)(to + s * Wide<W>::elements) = make_uint4(r[0][s], r[1][s], r[2][s], r[3][s]);
         }
     }
-    // three pieces of the values times their row's weight
-    __device__ __forceinline__ void put_weighted(bf16* dst, const float* weight) const {
-#pragma unroll
-        for (int i = 0; i < n; ++i) {
-            if (all % TH != 0 && threadIdx.x + i * TH >= all) continue;
-            bf16* to = dst + Wide<W>::at(row(i), col(i));
-            const float w = weight[row(i)];
-            uint32_t r[4][kFull3];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) split<kFull3>(to_f32(g[i].v[2 * u]) * w, to_f32(g[i].v[2 * u + 1]) * w, r[u]);
-#pragma unroll
-            for (int s = 0; s < kFull3; ++s) *(uint4*)(to + s * Wide<W>::elements) = make_uint4(r[0][s], r[1][s], r[2][s], r[3][s]);
-        }
-    }
+    __device__ __forceinline__ void put(bf16* dst) const { put<Pieces<T>::in, false>(dst, nullptr); }
+    __device__ __forceinline__ void put_weighted(bf16* dst, const float* weight) const { put<kFull3, true>(dst, weight); }
 };
 
-// elements at a time for rows that start at p and lie `stride` apart
-template <typename T>
-__device__ __forceinline__ int alignment(const T* p, int64_t stride) {
-    const uint64_t x = (uint64_t)(uintptr_t)p | (uint64_t)(stride * (int64_t)sizeof(T));
-    return (x & 15) == 0 ? 8 : (x & (2 * sizeof(T) - 1)) == 0 ? 2 : 1;
-}
+// whether rows that start at p and lie `stride` apart are on 16 bytes
+inline bool on_16(const void* p, int64_t stride_bytes) { return (((uintptr_t)p | (uintptr_t)stride_bytes) & 15) == 0; }
 
 // two neighbouring values from their pieces
 template <int NS>
@@ -320,54 +324,46 @@ __device__ __forceinline__ float2 from_pieces(const bf16* m, int piece) {
     return v;
 }
 
-// Writes a warp's 16 x 16 fragment (rows r0 and r0 + 8 of this lane) to rows of `st` elements; `how` as in alignment().
-// 16-bit values of four lanes are brought together, so that a lane stores 16 bytes.
-template <typename T>
-__device__ __forceinline__ void store_rows(T* out, int64_t st, int rows, int cols, int r0, int c0, const float (&x)[2][4], int how) {
+// Writes a warp's 16 x 16 fragment (rows r0 and r0 + 8 of this lane) to rows of `st` elements.  VEC: rows on 16 bytes, a
+// multiple of 8 columns; 16-bit values of four lanes are brought together, so that a lane stores 16 bytes.
+template <bool VEC, typename T>
+__device__ __forceinline__ void store_rows(T* out, int64_t st, int rows, int cols, int r0, int c0, const float (&x0)[4], const float (&x1)[4]) {
     const int lq = lane_id() & 3;
-    if (sizeof(T) == 2 && how == 8 && c0 + 16 <= cols) {
+    if constexpr (VEC && sizeof(T) == 2) {
         // two tiles of 8 columns, rows r0 and r0 + 8: lane lq gathers tile lq & 1 of row r0 + 8 (lq >> 1)
         uint32_t v[4];                                                 // [tile + 2 half]
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                struct alignas(4) Two { T a, b; } t{from_f32<T>(x[q][2 * h]), from_f32<T>(x[q][2 * h + 1])};
-                v[q + 2 * h] = *(uint32_t*)&t;
-            }
-        uint32_t a = lq & 1 ? v[0] : v[1], b = lq & 1 ? v[2] : v[3];
-        a = __shfl_xor_sync(kFull, a, 1);
-        b = __shfl_xor_sync(kFull, b, 1);
-        // now this lane and its neighbour hold tile lq & 1 of both rows: (mine, the neighbour's) words
-        uint32_t m0 = lq & 1 ? v[1] : v[0], m1 = lq & 1 ? v[3] : v[2];
-        uint32_t lo0 = lq & 1 ? a : m0, hi0 = lq & 1 ? m0 : a, lo1 = lq & 1 ? b : m1, hi1 = lq & 1 ? m1 : b;
+        for (int h = 0; h < 2; ++h) {
+            struct alignas(4) Two { T a, b; } t{from_f32<T>(x0[2 * h]), from_f32<T>(x0[2 * h + 1])}, t2{from_f32<T>(x1[2 * h]), from_f32<T>(x1[2 * h + 1])};
+            v[2 * h] = *(uint32_t*)&t;
+            v[1 + 2 * h] = *(uint32_t*)&t2;
+        }
+        const uint32_t a = __shfl_xor_sync(kFull, lq & 1 ? v[0] : v[1], 1), b = __shfl_xor_sync(kFull, lq & 1 ? v[2] : v[3], 1);
+        // this lane and its neighbour now hold tile lq & 1 of both rows
+        const uint32_t m0 = lq & 1 ? v[1] : v[0], m1 = lq & 1 ? v[3] : v[2];
+        const uint32_t lo0 = lq & 1 ? a : m0, hi0 = lq & 1 ? m0 : a, lo1 = lq & 1 ? b : m1, hi1 = lq & 1 ? m1 : b;
         const bool up = lq >> 1;
-        uint32_t s0 = up ? lo0 : lo1, s1 = up ? hi0 : hi1;
-        s0 = __shfl_xor_sync(kFull, s0, 2);
-        s1 = __shfl_xor_sync(kFull, s1, 2);
+        const uint32_t s0 = __shfl_xor_sync(kFull, up ? lo0 : lo1, 2), s1 = __shfl_xor_sync(kFull, up ? hi0 : hi1, 2);
         const uint32_t k0 = up ? lo1 : lo0, k1 = up ? hi1 : hi0;
-        const uint4 all = up ? make_uint4(s0, s1, k0, k1) : make_uint4(k0, k1, s0, s1);
-        const int r = r0 + 8 * (lq >> 1);
-        if (r < rows) *(uint4*)(out + r * st + c0 + 8 * (lq & 1)) = all;
-        return;
-    }
-    struct alignas(2 * sizeof(T)) Two { T a, b; };
+        const int r = r0 + 8 * (lq >> 1), c = c0 + 8 * (lq & 1);
+        if (r < rows && c < cols) *(uint4*)(out + r * st + c) = up ? make_uint4(s0, s1, k0, k1) : make_uint4(k0, k1, s0, s1);
+    } else {
+        struct alignas(2 * sizeof(T)) Two { T a, b; };
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int r = r0 + 8 * h;
-        if (r < rows)
+        for (int h = 0; h < 2; ++h) {
+            T* to = out + (r0 + 8 * h) * st + c0 + 2 * lq;
+            const int in = r0 + 8 * h < rows ? cols - c0 - 2 * lq : 0;
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                const int c = c0 + 8 * q + 2 * lq;
-                const T a = from_f32<T>(x[q][2 * h]), b = from_f32<T>(x[q][2 * h + 1]);
-                T* to = out + r * st + c;
-                if (how > 1 && c + 1 < cols) {
-                    *(Two*)to = Two{a, b};
+                const T a = from_f32<T>(q ? x1[2 * h] : x0[2 * h]), b = from_f32<T>(q ? x1[2 * h + 1] : x0[2 * h + 1]);
+                if (VEC) {
+                    if (8 * q < in) *(Two*)(to + 8 * q) = Two{a, b};
                 } else {
-                    if (c < cols) to[0] = a;
-                    if (c + 1 < cols) to[1] = b;
+                    if (8 * q < in) to[8 * q] = a;
+                    if (8 * q + 1 < in) to[8 * q + 1] = b;
                 }
             }
+        }
     }
 }
 
@@ -408,30 +404,57 @@ struct State {
     // its pieces to shared memory; whether a value was not finite
     template <int MS>
     __device__ __forceinline__ bool put(bf16* dst) {
-        bool bad = false;
+        float bad = 0.0f;
         pairs([&](float& x, float& y, int p, int n) {
             uint32_t q[MS];
             split<MS>(x, y, q);
-            bad |= not_finite(x) | not_finite(y);
+            bad = fmaf(x, 0.0f, fmaf(y, 0.0f, bad));
             bf16* to = dst + Wide<NT>::at(p, n);
 #pragma unroll
             for (int k = 0; k < MS; ++k) *(uint32_t*)(to + k * Wide<NT>::elements) = q[k];
         });
-        return bad;
+        return bad != 0.0f;
     }
     // s = whole s + the accumulator at addr (this warp's lanes)
     __device__ __forceinline__ void advance(uint32_t addr, float whole) {
+        if constexpr (NT >= 64) {
 #pragma unroll
-        for (int c = 0; c < NT / 16; ++c) {
-            float x[2][4];
-            t5::ld16(x, addr + 16 * c);
-            t5::wait_ld();
+            for (int c = 0; c < NT / 8; c += 8) {
+                float x[4][4], y[4][4];
+                t5::ld32x2(x, addr + 8 * c, y, addr + 8 * c + 32);
 #pragma unroll
-            for (int q = 0; q < 2; ++q)
+                for (int q = 0; q < 4; ++q)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[2 * c + q][e] = fmaf(whole, s[2 * c + q][e], x[q][e]);
+                    for (int e = 0; e < 4; ++e) {
+                        s[c + q][e] = fmaf(whole, s[c + q][e], x[q][e]);
+                        s[c + 4 + q][e] = fmaf(whole, s[c + 4 + q][e], y[q][e]);
+                    }
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < NT / 8; c += 2) {
+                float x[2][4];
+                t5::ld16(x, addr + 8 * c);
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[c + q][e] = fmaf(whole, s[c + q][e], x[q][e]);
+            }
         }
     }
+};
+
+// The logarithms of a chunk's decays on their way (one warp), two chunks ahead of the walk.
+struct Logs {
+    const float* g;
+    int64_t st;
+    float a, b;                  // of token 2 lane and 2 lane + 1
+    __device__ __forceinline__ void fetch(int t, int len) {
+        const int l = lane_id();
+        a = t + 2 * l < len && t >= 0 ? g[(int64_t)(t + 2 * l) * st] : 0.0f;
+        b = t + 2 * l + 1 < len && t >= 0 ? g[(int64_t)(t + 2 * l + 1) * st] : 0.0f;
+    }
+    __device__ __forceinline__ bool bad() const { return !(a <= 3.38e38f && b <= 3.38e38f); }
 };
 
 // What has to be initialised and awaited: barriers of the tensor cores' work, the tensor memory's address, and whether
@@ -442,11 +465,12 @@ struct Sync {
     uint32_t tmem;
     int failed;
 
-    __device__ __forceinline__ void init(uint32_t cols) {
+    // the first barrier awaits `first` arrivals, the others one
+    __device__ __forceinline__ void init(uint32_t cols, int first = 1) {
         if (threadIdx.x < 32) t5::alloc(&tmem, cols);
         if (threadIdx.x == 0) {
             failed = 0;
-            for (int i = 0; i < BARS; ++i) t5::bar_init(&bars[i], 1);
+            for (int i = 0; i < BARS; ++i) t5::bar_init(&bars[i], i == 0 ? first : 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         t5::fence_before();
@@ -455,6 +479,7 @@ struct Sync {
     }
     __device__ __forceinline__ void wait(int bar, uint32_t phase) {
         if (!*(volatile int*)&failed && !t5::bar_wait(&bars[bar], phase)) *(volatile int*)&failed = 1;
+        __syncwarp();                                         // threads leave a wait at their own times
         t5::fence_after();
     }
     // the whole block, all products awaited
@@ -504,6 +529,9 @@ Parts parts_of(const Plan& plan, void* workspace);
 // entering states along each sequence, from `end` (nullptr: zeros) at its first (backwards: last) item
 bcm_status join(const Plan& plan, const Parts& parts, const float* end, bool backward, cudaStream_t stream);
 
+// whether all rows of a call are on 16 bytes (NULL pointers count)
+bool aligned(const bcm_decay_attn_args* a, bool backward);
+
 inline Rows rows_of(const void* p, int64_t sb, int64_t st, int64_t sh) { return Rows{p, sb, st, sh}; }
 
 // calls f(T, NT as an integral constant)
@@ -545,7 +573,7 @@ struct PartSmem {
 
 constexpr int kPartThreads = 128;
 
-template <typename T, int NT, bool BACK>
+template <typename T, int NT, bool BACK, bool VEC>
 __global__ void __launch_bounds__(kPartThreads) part_kernel(const __grid_constant__ PartArgs p) {
     extern __shared__ unsigned char smem_raw[];
     PartSmem<T, NT>& sm = *(PartSmem<T, NT>*)tiles_base(smem_raw);
@@ -560,51 +588,54 @@ __global__ void __launch_bounds__(kPartThreads) part_kernel(const __grid_constan
     const T* a = row_ptr<T>(p.a, z, it.seq, it.t0, ha);
     const T* b = row_ptr<T>(p.b, z, it.seq, it.t0, h) + col;
     const float* g = p.g + (z.cu ? 0 : it.seq * p.g_sb) + it.t0 * p.g_st + h * p.g_sh;
-    const int va = alignment(a, p.a.st), vb = alignment(b, p.b.st);
     const int len = it.t1 - it.t0, nc = (len + kChunk - 1) / kChunk, l = lane_id();
     State<NT> st;
     st.zero();
     double all = 0.0;
-    Pending<T, NT, kPartThreads> pa;
-    Pending<T, kP, kPartThreads> pb;
-    float g0 = 0.0f, g1 = 0.0f;
-    auto fetch = [&](int i) {                             // the i-th chunk of the walk
-        const int t = (BACK ? nc - 1 - i : i) * kChunk, rows = min(kChunk, len - t);
-        pa.fetch(a + t * p.a.st, p.a.st, rows, z.n, va);
-        pb.fetch(b + t * p.b.st, p.b.st, p.b.p ? rows : 0, cols, vb);
-        if (threadIdx.x < 32) {
-            g0 = 2 * l < rows ? g[(int64_t)(t + 2 * l) * p.g_st] : 0.0f;
-            g1 = 2 * l + 1 < rows ? g[(int64_t)(t + 2 * l + 1) * p.g_st] : 0.0f;
-        }
+    Pending<T, NT, kPartThreads, VEC> pa;
+    Pending<T, kP, kPartThreads, VEC> pb;
+    Logs logs{g, p.g_st};
+    const bool decay_warp = threadIdx.x < 32;
+    auto start = [&](int i) { return (BACK ? nc - 1 - i : i) * kChunk; };      // of the i-th chunk of the walk
+    auto fetch = [&](int i) {
+        const int t = start(i), rows = min(kChunk, len - t);
+        pa.fetch(a + t * p.a.st, p.a.st, rows, z.n);
+        pb.fetch(b + t * p.b.st, p.b.st, p.b.p ? rows : 0, cols);
     };
-    if (nc > 0) fetch(0);
     sm.sync.init(kCols);
-    if (threadIdx.x < 32) all += decays_of(sm.d[0], g0, g1);
-    const uint32_t acc = sm.sync.tmem;
-    for (int i = 0; i < nc; ++i) {
-        __syncthreads();
-        // (what is not finite stays so in the sums, and the walk takes such chunks token by token)
-        const Decays& d = sm.d[i & 1];
-        pa.put(sm.a[0]);
-        pb.put_weighted(sm.bw[0], BACK ? d.since : d.until);
-        t5::fence_smem();
-        t5::fence_before();
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            t5::fence_after();
-            const Operand<kP, false> A{t5::smem_u32(sm.bw)};
-            const Operand<NT, false> B{t5::smem_u32(sm.a)};
-            products<kFull3, NS, kFull3>(acc, [&](int s, int k) { return A.desc(s, k); }, [&](int u, int k) { return B.desc(u, k); },
-                                         kChunk / 16, t5::instr(NT, true, true), false);
-            t5::commit(&sm.sync.bars[0]);
+    if (decay_warp) {
+        logs.fetch(start(0), len);
+        all += decays_of(sm.d[0], logs.a, logs.b);
+        logs.fetch(nc > 1 ? start(1) : -1, len);
+    }
+    const uint32_t acc = __shfl_sync(kFull, sm.sync.tmem, 0);
+    const int warp = t5::warp_id();
+    for (int i = -1; i < nc; ++i) {
+        if (i >= 0) {
+            __syncthreads();
+            // (what is not finite stays so in the sums, and the walk takes such chunks token by token)
+            pa.put(sm.a[0]);
+            pb.put_weighted(sm.bw[0], BACK ? sm.d[i & 1].since : sm.d[i & 1].until);
+            t5::fence_smem();
+            t5::fence_before();
+            __syncthreads();
+            if (warp == 0 && t5::elect()) {
+                t5::fence_after();
+                const Operand<kP, false> A(sm.bw);
+                const Operand<NT, false> B(sm.a);
+                products<kFull3, NS, kFull3, kChunk / 16>(acc, A, B, t5::instr(NT, true, true), false);
+                t5::commit(&sm.sync.bars[0]);
+            }
+            __syncwarp();
         }
-        __syncwarp();
-        if (i + 1 < nc) {
-            fetch(i + 1);
-            if (threadIdx.x < 32) all += decays_of(sm.d[(i + 1) & 1], g0, g1);
+        if (i + 1 < nc) fetch(i + 1);
+        if (i < 0) continue;
+        if (decay_warp && i + 1 < nc) {
+            all += decays_of(sm.d[(i + 1) & 1], logs.a, logs.b);
+            logs.fetch(i + 2 < nc ? start(i + 2) : -1, len);
         }
         sm.sync.wait(0, i & 1);
-        st.advance(acc + ((threadIdx.x >> 5) << 21), d.whole);
+        st.advance(acc + (warp << 21), sm.d[i & 1].whole);
         t5::fence_before();
     }
     if (sm.sync.failed) st.pairs([](float& x, float& y, int, int) { x = y = __int_as_float(0x7fc00000); });
@@ -615,9 +646,9 @@ __global__ void __launch_bounds__(kPartThreads) part_kernel(const __grid_constan
 }
 
 template <typename T, int NT, bool BACK>
-bcm_status launch_part(const PartArgs& p, cudaStream_t stream) {
+bcm_status launch_part(const PartArgs& p, bool vec, cudaStream_t stream) {
     constexpr size_t smem = sizeof(PartSmem<T, NT>) + 1024;
-    auto kernel = part_kernel<T, NT, BACK>;
+    auto kernel = vec ? part_kernel<T, NT, BACK, true> : part_kernel<T, NT, BACK, false>;
     bcm_status st = allow_smem(kernel, smem);
     if (st != BCM_OK) return st;
     kernel<<<(unsigned)(p.z.items * p.z.heads * p.z.slices), kPartThreads, smem, stream>>>(p);

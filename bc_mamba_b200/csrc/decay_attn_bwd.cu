@@ -28,9 +28,11 @@ struct BwdArgs {
     int shares;
 };
 
-// Four groups of four warps.  The first takes 16 keys a warp: it decays both products of scores, puts the pieces of
-// (Q K^T o D)^T into tensor memory and those of (dY V^T o D)^T into shared memory (where they serve dk by rows and dq by
-// columns), sums W for dg, and writes dv.  The second and third write dk and dq; the fourth holds the state's gradient.
+// Four groups of four warps; a warp takes 16 keys (or queries).  The first three decay both products of scores, blocks of
+// 16 queries dealt among them, put the pieces of (Q K^T o D)^T into tensor memory and those of (dY V^T o D)^T into shared
+// memory (where they serve dk by rows and dq by columns) and sum W for dg; then they finish dv, dk and dq: the far part
+// of each is decayed in place and the near part added on top.  The fourth holds the state's gradient and advances it
+// meanwhile.  The next chunk's tiles are on their way to registers during all of that.
 constexpr int kBwdThreads = 512;
 
 template <typename T, int NT>
@@ -49,15 +51,19 @@ struct BwdSmem {
         __device__ __forceinline__ bf16* scores() { return late ? dyw[0] : dp[0]; }
     } tiles;
     Decays d[2];
-    float pairs[4][kChunk];    // sum over i >= t, j < t of W_ij, j of one warp
-    float of_q[kChunk], of_k[kChunk];
-    float across[4];           // <S_in, dS> of the warps
-    Sync<7> sync;
+    // of two chunks
+    float pairs[2][4][kChunk]; // [key block][query t]: sum over i >= t in t's block, j < t of W_ij
+    float rows[2][4][kChunk];  // [query block][key j]: sum over i of W_ij, blocks behind j's own
+    float of_q[2][kChunk], of_k[2][kChunk];
+    float across[2][4];        // <S_in, dS> of the warps
+    float across_whole[2];     // the chunks' decays (those of the chunk before take their place early)
+    Sync<8> sync;
 
-    static constexpr uint32_t at = 0, dt = 64, gv = 128, gk = 192, gq = gk + NT, inc = late ? 0 : gq + NT, cols = 512;
-    // a piece of the keys' decayed scores: blocks of 16 queries are taken from the last, and the 8 columns that a block's
-    // piece needs lie in blocks of both scores which have been read
-    __device__ __forceinline__ static uint32_t piece(int m) { return m == 0 ? at + 32 : m == 1 ? dt + 32 : 480; }
+    // tensor memory: both scores, dv, dk, dq, the state's increase, the pieces of the keys' decayed scores (32 columns
+    // each).  In float32 with keys of 128 the pieces have to take the scores' place.
+    static constexpr bool over = late && MS == 3;
+    static constexpr uint32_t at = 0, dt = 64, gv = 128, gk = 192, gq = gk + NT, inc = late ? 0 : gq + NT;
+    static constexpr uint32_t piece = over ? 0 : late ? gq + NT : inc + NT, cols = 512;
 };
 
 // where a block's rows of dq and dk go
@@ -76,8 +82,8 @@ struct RowsOut {
 // `f` (shared): the state's gradient NT x kP, then sums.
 template <typename T, int NT>
 __device__ __noinline__ void back_tokens(const BwdArgs& p, const T* q, const T* k, const T* v, const T* dy, const float* g, const float* s_in,
-                                         const RowsOut<T>& dq, const RowsOut<T>& dk, T* dv, int64_t dv_st, float* dg, int64_t dg_st,
-                                         int rows, int cols, int64_t row0, float* f) {
+                                         const RowsOut<T> dq, const RowsOut<T> dk, T* dv, int64_t dv_st, float* dg, int64_t dg_st,
+                                         int rows, int cols, float* f) {
     constexpr int parts = kBwdThreads / kP, warps = kP / 32, all_warps = kBwdThreads / 32;
     const int c = threadIdx.x % kP, part = threadIdx.x / kP, w = threadIdx.x >> 5, l = lane_id();
     float* const sq = f + NT * kP;                 // [warps][NT]
@@ -121,8 +127,8 @@ __device__ __noinline__ void back_tokens(const BwdArgs& p, const T* q, const T* 
                 x0 += sq[NT + n];
                 x1 += sk[NT + n];
             }
-            dq.put(row0 + t, n, x0);
-            dk.put(row0 + t, n, x1);
+            dq.put(t, n, x0);
+            dk.put(t, n, x1);
         }
         if (part == 0 && in) {
             for (int r = 1; r < parts; ++r) gv += sv[r * kP + c];
@@ -136,7 +142,7 @@ __device__ __noinline__ void back_tokens(const BwdArgs& p, const T* q, const T* 
     }
 }
 
-template <typename T, int NT>
+template <typename T, int NT, bool VEC>
 __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant__ BwdArgs p) {
     extern __shared__ unsigned char smem_raw[];
     using Smem = BwdSmem<T, NT>;
@@ -149,22 +155,21 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
     const int64_t rows_all = (z.cu ? 1 : (int64_t)z.batch) * z.seqlen;
     const int64_t qk_st = (int64_t)z.qk_heads * z.n, v_st = (int64_t)z.heads * z.p;
     const int part = h % share * z.slices + slice;            // of the blocks that share a row of dq
-    RowsOut<T> dq{(T*)p.dq + (int64_t)hq * z.n, nullptr, qk_st}, dk{(T*)p.dk + (int64_t)hq * z.n, nullptr, qk_st};
-    if (p.shares > 1) {
-        dq.part = (float*)p.dq + part * rows_all * qk_st + (int64_t)hq * z.n;
-        dk.part = (float*)p.dk + part * rows_all * qk_st + (int64_t)hq * z.n;
-    }
+    // rows of dq or dk from `row` on, whole or this block's part of them
+    auto rows_out = [&](void* all, int64_t row) {
+        RowsOut<T> o{(T*)all + row * qk_st + (int64_t)hq * z.n, nullptr, qk_st};
+        if (p.shares > 1) o.part = (float*)all + (part * rows_all + row) * qk_st + (int64_t)hq * z.n;
+        return o;
+    };
     float* const dg_all = p.dg + slice * rows_all * z.heads + h;
     if (z.cu) {
         const int end = z.tables.seq_item[z.batch + 1];
         zero_rows((T*)p.dv + (int64_t)h * z.p + col, end, z.seqlen, v_st, cols, item, z.items);
         zero_rows(dg_all, end, z.seqlen, z.heads, 1, item, z.items);
-        if (dq.part) {
-            zero_rows(dq.part, end, z.seqlen, qk_st, z.n, item, z.items);
-            zero_rows(dk.part, end, z.seqlen, qk_st, z.n, item, z.items);
-        } else {
-            zero_rows(dq.whole, end, z.seqlen, qk_st, z.n, item, z.items);
-            zero_rows(dk.whole, end, z.seqlen, qk_st, z.n, item, z.items);
+        for (void* all : {p.dq, p.dk}) {
+            const RowsOut<T> o = rows_out(all, 0);
+            if (o.part) zero_rows(o.part, end, z.seqlen, qk_st, z.n, item, z.items);
+            else zero_rows(o.whole, end, z.seqlen, qk_st, z.n, item, z.items);
         }
     }
     const Item it = item_of(z, item);
@@ -177,114 +182,183 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
     const int64_t row_at = (z.cu ? 0 : (int64_t)it.seq * z.seqlen) + it.t0;
     T* const dv = (T*)p.dv + row_at * v_st + (int64_t)h * z.p + col;
     float* const dg = dg_all + row_at * z.heads;
-    const int vq = alignment(q, p.q.st), vk = alignment(k, p.k.st), vv = alignment(v, p.v.st), vy = dy ? alignment(dy, p.dy.st) : 1;
     const int np = z.n * z.p;
     const int len = it.t1 - it.t0, nc = (len + kChunk - 1) / kChunk;
-    const int l = lane_id(), group = threadIdx.x >> 7, w = (threadIdx.x >> 5) & 3, row = w * 16 + (l >> 2), lq = l & 3;
-    const bool decay_warp = threadIdx.x >= 384 && threadIdx.x < 416;
+    const int warp = t5::warp_id(), l = lane_id(), group = warp >> 2, w = warp & 3, row = w * 16 + (l >> 2), lq = l & 3;
+    const bool decay_warp = warp == 12, dg_warp = warp == 13;
     const int p16 = (cols + 15) / 16, n16 = (z.n + 15) / 16;
 
-    Pending<T, NT, kBwdThreads> pq, pk;
-    Pending<T, kP, kBwdThreads> pv, py;
-    Pending<float, NT, kBwdThreads> ps;
-    float g0 = 0.0f, g1 = 0.0f;
-    auto state_in = [&](int c) { return p.ckpt + (((int64_t)(it.chunk + c) * z.heads + h) * z.slices + slice) * (NT * kP); };
-    auto fetch = [&](int c) {
-        const int t = c * kChunk, rows = min(kChunk, len - t);
-        pq.fetch(q + t * p.q.st, p.q.st, rows, z.n, vq);
-        pk.fetch(k + t * p.k.st, p.k.st, rows, z.n, vk);
-        pv.fetch(v + t * p.v.st, p.v.st, rows, cols, vv);
-        py.fetch(dy + t * p.dy.st, p.dy.st, dy ? rows : 0, cols, vy);
-        ps.fetch(state_in(c), NT, cols, NT, 8);
-        if (decay_warp) {
-            g0 = 2 * l < rows ? g[(int64_t)(t + 2 * l) * p.g_st] : 0.0f;
-            g1 = 2 * l + 1 < rows ? g[(int64_t)(t + 2 * l + 1) * p.g_st] : 0.0f;
+    const float* const ckpt = p.ckpt + (((int64_t)it.chunk * z.heads + h) * z.slices + slice) * (NT * kP);
+    const int64_t ckpt_st = (int64_t)z.heads * z.slices * (NT * kP);
+    Pending<T, NT, kBwdThreads, VEC> pq, pk;
+    Pending<T, kP, kBwdThreads, VEC> pv, py;
+    Pending<float, NT, kBwdThreads, true> ps;
+    Logs logs{g, p.g_st};
+    sm.sync.init(Smem::cols, 2);
+    const uint32_t tm = __shfl_sync(kFull, sm.sync.tmem, 0), lanes = (uint32_t)w << 21;
+    enum { kScores, kFarV, kFarK, kFarQ, kInc, kNearV, kNearK, kNearQ };
+
+    // dg of chunk c from what its walk left in shared memory (one warp, tokens 2 lane and 2 lane + 1)
+    auto finish_dg = [&](int c) {
+        const int t = 2 * l, block = t / 16, rows = min(kChunk, len - c * kChunk);
+        const float q0 = sm.of_q[c & 1][t], q1 = sm.of_q[c & 1][t + 1], k0 = sm.of_k[c & 1][t], k1 = sm.of_k[c & 1][t + 1];
+        float behind = q0 + q1, before = k0 + k1;
+        float r[3];                                           // of the keys up to these two, over a block of queries
+#pragma unroll
+        for (int ib = 1; ib < 4; ++ib) r[ib - 1] = block < ib ? sm.rows[c & 1][ib][t] + sm.rows[c & 1][ib][t + 1] : 0.0f;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const float a = __shfl_down_sync(kFull, behind, off), b = __shfl_up_sync(kFull, before, off);
+            if (l + off < 32) behind += a;
+            if (l >= off) before += b;
+#pragma unroll
+            for (int ib = 0; ib < 3; ++ib) {
+                const float e = __shfl_up_sync(kFull, r[ib], off);
+                if (l >= off) r[ib] += e;
+            }
+        }
+        float rest = __shfl_down_sync(kFull, behind, 1), past = __shfl_up_sync(kFull, before, 1);
+        if (l == 31) rest = 0.0f;
+        if (l == 0) past = 0.0f;
+        const float through = sm.across_whole[c & 1] * ((sm.across[c & 1][0] + sm.across[c & 1][1]) + (sm.across[c & 1][2] + sm.across[c & 1][3]));
+        float d0 = 0.0f, d1 = 0.0f;
+        for (int k2 = 0; k2 <= block; ++k2) {
+            d0 += sm.pairs[c & 1][k2][t];
+            d1 += sm.pairs[c & 1][k2][t + 1];
+        }
+#pragma unroll
+        for (int ib = 1; ib < 4; ++ib) {
+            float e = __shfl_up_sync(kFull, r[ib - 1], 1);
+            if (l == 0) e = 0.0f;
+            if (ib > block) {
+                d0 += e;
+                d1 += e + sm.rows[c & 1][ib][t];
+            }
+        }
+        d0 += (rest + q1 + q0) + past + through;
+        d1 += (rest + q1) + (past + k0) + through;
+        if (t < rows) dg[(int64_t)(c * kChunk + t) * z.heads] = d0;
+        if (t + 1 < rows) dg[(int64_t)(c * kChunk + t + 1) * z.heads] = d1;
+    };
+    // a far part: 16 rows of an accumulator times their decays, in place
+    auto decay_far = [&](uint32_t acc, int blocks, float f0, float f1, auto&& each) {
+#pragma unroll 1
+        for (int nb = 0; nb < blocks; ++nb) {
+            float x[2][4];
+            t5::ld16(x, acc + 16 * nb);
+#pragma unroll
+            for (int q2 = 0; q2 < 2; ++q2)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[q2][e] *= e < 2 ? f0 : f1;
+            each(x, nb);
+            t5::st_acc16(acc + 16 * nb, x);
         }
     };
-    auto put = [&](int c) {
-        bool bad = pq.bad() | pk.bad() | pv.bad() | py.bad() | ps.bad();
-        if (decay_warp) bad |= !(g0 <= 3.38e38f && g1 <= 3.38e38f);
-        pq.put(sm.tiles.q[0]);
-        pk.put(sm.tiles.k[0]);
-        pv.put(sm.tiles.v[0]);
-        py.put(sm.tiles.dy[0]);
-        if (!Smem::one_state) ps.put(sm.tiles.state());
-        if (!Smem::late) py.put_weighted(sm.tiles.dyw[0], sm.d[c & 1].since);
-        t5::fence_smem();
-        t5::fence_before();
-        return bad;
-    };
-    // (float32 keys of 128) the state in the place of its gradient, which all have read by then
-    auto put_state = [&](uint32_t phase) {
-        if (!Smem::one_state) return;
-        sm.sync.wait(1, phase);
-        ps.put(sm.tiles.state());
-        t5::fence_smem();
-        t5::fence_before();
-        __syncthreads();
+
+    // Puts chunk c's tiles down, starts the products that need no other and the way of the chunk before it; whether the
+    // chunk has to be taken token by token.
+    auto start = [&](int c, bool bad, uint32_t phase) {
+        const int t = c * kChunk;
+        bool slow = false;
+        if (c < nc) {
+            __syncthreads();                                  // decays are there; the chunk behind is done with the tiles
+            bad |= pq.bad() | pk.bad() | pv.bad() | py.bad() | ps.bad();
+            pq.put(sm.tiles.q[0]);
+            pk.put(sm.tiles.k[0]);
+            pv.put(sm.tiles.v[0]);
+            py.put(sm.tiles.dy[0]);
+            if (!Smem::one_state) ps.put(sm.tiles.state());
+            if (!Smem::late) py.put_weighted(sm.tiles.dyw[0], sm.d[c & 1].since);
+            t5::fence_smem();
+            t5::fence_before();
+            slow = __syncthreads_or(bad);
+            if (!slow) {
+                if (w == 0 && t5::elect()) {
+                    t5::fence_after();
+                    const Operand<NT, true> Q(sm.tiles.q), K(sm.tiles.k), Sk(sm.tiles.ds);
+                    const Operand<NT, false> Qt(sm.tiles.q), dS(sm.tiles.ds), S(sm.tiles.state());
+                    const Operand<kP, true> V(sm.tiles.v), Y(sm.tiles.dy);
+                    const Operand<kP, false> Yw(sm.tiles.dyw);
+                    if (group == 0) {
+                        products<NS, NS, kFull3, NT / 16>(tm + Smem::at, K, Q, t5::instr(kChunk, false, false), false);
+                        t5::commit(&sm.sync.bars[kScores]);
+                        products<NS, MS, MS, NT / 16>(tm + Smem::gv, K, Sk, t5::instr(p16 * 16, false, false), false);
+                        t5::commit(&sm.sync.bars[kFarV]);
+                    } else if (group == 1) {
+                        products<NS, NS, kFull3, kP / 16>(tm + Smem::dt, V, Y, t5::instr(kChunk, false, false), false);
+                        t5::commit(&sm.sync.bars[kScores]);
+                        products<NS, kFull3, kFull3, kP / 16>(tm + Smem::gk, V, dS, t5::instr(n16 * 16, false, true), false);
+                        t5::commit(&sm.sync.bars[kFarK]);
+                    } else if (group == 2) {
+                        if (!Smem::one_state) {
+                            products<NS, kFull3, kFull3, kP / 16>(tm + Smem::gq, Y, S, t5::instr(n16 * 16, false, true), false);
+                            t5::commit(&sm.sync.bars[kFarQ]);
+                        }
+                    } else if (!Smem::late) {
+                        products<kFull3, NS, kFull3, kChunk / 16>(tm + Smem::inc, Yw, Qt, t5::instr(NT, true, true), false);
+                        t5::commit(&sm.sync.bars[kInc]);
+                    }
+                }
+                __syncwarp();
+                if (Smem::one_state) {
+                    // the state in the place of its gradient, which all products have read by then
+                    sm.sync.wait(kFarV, phase);
+                    sm.sync.wait(kFarK, phase);
+                    ps.put(sm.tiles.state());
+                    t5::fence_smem();
+                    t5::fence_before();
+                    __syncthreads();
+                    if (warp == 8 && t5::elect()) {
+                        t5::fence_after();
+                        const Operand<NT, false> S(sm.tiles.state());
+                        const Operand<kP, true> Y(sm.tiles.dy);
+                        products<NS, kFull3, kFull3, kP / 16>(tm + Smem::gq, Y, S, t5::instr(n16 * 16, false, true), false);
+                        t5::commit(&sm.sync.bars[kFarQ]);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        if (c > 0) {
+            const int t2 = t - kChunk, r2 = min(kChunk, len - t2);
+            pq.fetch(q + t2 * p.q.st, p.q.st, r2, z.n);
+            pk.fetch(k + t2 * p.k.st, p.k.st, r2, z.n);
+            pv.fetch(v + t2 * p.v.st, p.v.st, r2, cols);
+            py.fetch(dy + t2 * p.dy.st, p.dy.st, dy ? r2 : 0, cols);
+            ps.fetch(ckpt + (c - 1) * ckpt_st, NT, cols, NT);
+        }
+        return slow;
     };
     auto walk = [&](int c) {
         const int t = c * kChunk;
-        back_tokens<T, NT>(p, q + t * p.q.st, k + t * p.k.st, v + t * p.v.st, dy ? dy + t * p.dy.st : nullptr, g + t * p.g_st, state_in(c), dq, dk,
-                           dv + t * v_st, v_st, dg + (int64_t)t * z.heads, z.heads, min(kChunk, len - t), cols, row_at + t, (float*)&sm.tiles);
+        back_tokens<T, NT>(p, q + t * p.q.st, k + t * p.k.st, v + t * p.v.st, dy ? dy + t * p.dy.st : nullptr, g + t * p.g_st, ckpt + c * ckpt_st,
+                           rows_out(p.dq, row_at + t), rows_out(p.dk, row_at + t), dv + t * v_st, v_st, dg + (int64_t)t * z.heads, z.heads,
+                           min(kChunk, len - t), cols, (float*)&sm.tiles);
     };
-    if (nc > 0) fetch(nc - 1);
-    sm.sync.init(Smem::cols);
-    const uint32_t tm = sm.sync.tmem, lanes = (uint32_t)w << 21;
     uint32_t phase = 0;
-    const Operand<NT, true> Q{t5::smem_u32(sm.tiles.q)}, K{t5::smem_u32(sm.tiles.k)}, Sk{t5::smem_u32(sm.tiles.ds)};
-    const Operand<NT, false> Qt{t5::smem_u32(sm.tiles.q)}, Kt{t5::smem_u32(sm.tiles.k)}, dS{t5::smem_u32(sm.tiles.ds)}, S{t5::smem_u32(sm.tiles.state())};
-    const Operand<kP, true> V{t5::smem_u32(sm.tiles.v)}, Y{t5::smem_u32(sm.tiles.dy)}, P{t5::smem_u32(sm.tiles.scores())};
-    const Operand<kP, false> Yt{t5::smem_u32(sm.tiles.dy)}, Yw{t5::smem_u32(sm.tiles.dyw)}, Pt{t5::smem_u32(sm.tiles.scores())};
-    auto of = [](const auto& o) { return [&o](int s, int i) { return o.desc(s, i); }; };
-
     if (group == 3) {
-        // dg of chunk c from what its walk left in shared memory (one warp)
-        auto finish_dg = [&](int c) {
-            const int t = 2 * l, rows = min(kChunk, len - c * kChunk);
-            const float q0 = sm.of_q[t], q1 = sm.of_q[t + 1], k0 = sm.of_k[t], k1 = sm.of_k[t + 1];
-            float behind = q0 + q1, before = k0 + k1;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const float a = __shfl_down_sync(kFull, behind, off), b = __shfl_up_sync(kFull, before, off);
-                if (l + off < 32) behind += a;
-                if (l >= off) before += b;
-            }
-            float rest = __shfl_down_sync(kFull, behind, 1), past = __shfl_up_sync(kFull, before, 1);
-            if (l == 31) rest = 0.0f;
-            if (l == 0) past = 0.0f;
-            const float through = sm.d[c & 1].whole * ((sm.across[0] + sm.across[1]) + (sm.across[2] + sm.across[3]));
-            float d0 = 0.0f, d1 = 0.0f;
-            for (int k2 = 0; k2 <= t / 16; ++k2) {
-                d0 += sm.pairs[k2][t];
-                d1 += sm.pairs[k2][t + 1];
-            }
-            d0 += (rest + q1 + q0) + past + through;
-            d1 += (rest + q1) + (past + k0) + through;
-            if (t < rows) dg[(int64_t)(c * kChunk + t) * z.heads] = d0;
-            if (t + 1 < rows) dg[(int64_t)(c * kChunk + t + 1) * z.heads] = d1;
-        };
         State<NT> ds;
+        bool bad, bad_logs = false, pending = false;          // pending: the chunk behind has its dg still to be finished
         const float* from = it.last ? (p.dh_last ? p.dh_last + ((int64_t)it.seq * z.heads + h) * np : nullptr)
                                     : p.enter + ((int64_t)item * z.heads + h) * np;
-        if (decay_warp && nc > 0) decays_of(sm.d[(nc - 1) & 1], g0, g1);
+        if (decay_warp) logs.fetch((nc - 1) * kChunk, len);
         if (from) ds.load(from + col, z.n, cols, z.p);
         else ds.zero();
-        bool bad = ds.template put<kFull3>(sm.tiles.ds[0]);
-        bool pending = false;                                 // the chunk behind has its dg still to be finished
-        for (int c = nc - 1; c >= 0; --c) {
-            __syncthreads();                                  // decays are there; the chunk behind is done with the tiles
-            if (pending && decay_warp) finish_dg(c + 1);
-            bad |= put(c);
-            const bool slow = __syncthreads_or(bad);
-            const float whole = sm.d[c & 1].whole;
-            if (!slow) put_state(phase);
-            if (c > 0) {
-                fetch(c - 1);
-                if (decay_warp) decays_of(sm.d[(c - 1) & 1], g0, g1);
-            }
+        bad = ds.template put<kFull3>(sm.tiles.ds[0]);
+        if (decay_warp) {
+            bad_logs = logs.bad();
+            decays_of(sm.d[(nc - 1) & 1], logs.a, logs.b);
+            logs.fetch((nc - 2) * kChunk, len);
+        }
+        for (int c = nc; c >= 0; --c) {
+            const int t = c * kChunk;
+            const bool slow = start(c, bad | bad_logs, phase);
+            if (c == nc) continue;
+            if (pending && dg_warp) finish_dg(c + 1);
             pending = !slow;
+            const Decays& d = sm.d[c & 1];
             if (slow) {
+                // token by token, through shared memory
                 float* f = (float*)&sm.tiles;
                 ds.pairs([&](float& x0, float& x1, int pp, int n) {
                     f[n * kP + pp] = x0;
@@ -297,7 +371,13 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
                     x1 = f[(n + 1) * kP + pp];
                 });
                 __syncthreads();                              // all have theirs back before the pieces take the place
-            } else {
+            }
+            if (decay_warp && c > 0) {
+                bad_logs = logs.bad();
+                decays_of(sm.d[(c - 1) & 1], logs.a, logs.b);
+                logs.fetch((c - 2) * kChunk, len);
+            }
+            if (!slow) {
                 float x = 0.0f;
                 ds.pairs([&](float& x0, float& x1, int pp, int n) {
                     const float2 in = from_pieces<kFull3>(sm.tiles.state() + Wide<NT>::at(pp, n), Wide<NT>::elements);
@@ -305,18 +385,18 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
                 });
 #pragma unroll
                 for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(kFull, x, o);
-                if (l == 0) sm.across[w] = x;
+                if (l == 0) sm.across[c & 1][w] = x;
+                if (threadIdx.x == 384) sm.across_whole[c & 1] = d.whole;
                 if (Smem::late) {
                     // behind all other products of the chunk
-                    for (int b = 4; b < 7; ++b) sm.sync.wait(b, phase);
-                    const float* since = sm.d[c & 1].since;
+                    for (int b = kNearV; b <= kNearQ; ++b) sm.sync.wait(b, phase);
                     for (int i = threadIdx.x - 384; i < 64 * 8; i += 128) {
-                        const int r = i / 8, u = i % 8 * 8, e = Wide<kP>::at(r, u);
+                        const int r = i / 8, e = Wide<kP>::at(r, i % 8 * 8);
                         uint32_t a[4][kFull3];
 #pragma unroll
                         for (int k2 = 0; k2 < 4; ++k2) {
                             const float2 in = from_pieces<NS>(sm.tiles.dy[0] + e + 2 * k2, Wide<kP>::elements);
-                            split<kFull3>(in.x * since[r], in.y * since[r], a[k2]);
+                            split<kFull3>(in.x * d.since[r], in.y * d.since[r], a[k2]);
                         }
 #pragma unroll
                         for (int s = 0; s < kFull3; ++s) *(uint4*)(sm.tiles.dyw[s] + e) = make_uint4(a[0][s], a[1][s], a[2][s], a[3][s]);
@@ -324,230 +404,206 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
                     t5::fence_smem();
                     t5::fence_before();
                     named_sync(2, 128);
-                    if (threadIdx.x == 384) {
+                    if (warp == 12 && t5::elect()) {
                         t5::fence_after();
-                        products<kFull3, NS, kFull3>(tm + Smem::inc, of(Yw), of(Qt), kChunk / 16, t5::instr(NT, true, true), false);
-                        t5::commit(&sm.sync.bars[3]);
+                        const Operand<kP, false> Yw(sm.tiles.dyw);
+                        const Operand<NT, false> Qt(sm.tiles.q);
+                        products<kFull3, NS, kFull3, kChunk / 16>(tm + Smem::inc, Yw, Qt, t5::instr(NT, true, true), false);
+                        t5::commit(&sm.sync.bars[kInc]);
                     }
                     __syncwarp();
                 }
-                sm.sync.wait(3, phase);
-                ds.advance(tm + Smem::inc + lanes, whole);
-                sm.sync.wait(1, phase);                       // the products with the gradient (and the state) have read it
-                if (Smem::one_state) sm.sync.wait(2, phase);
+                sm.sync.wait(kInc, phase);
+                ds.advance(tm + Smem::inc + lanes, d.whole);
+                sm.sync.wait(kFarV, phase);                   // the products with the gradient (and the state) have read it
+                sm.sync.wait(kFarK, phase);
+                if (Smem::one_state) sm.sync.wait(kFarQ, phase);
                 t5::fence_before();
-                named_sync(2, 128);                           // (and this group the state, for its dot)
+                if (Smem::one_state) named_sync(2, 128);      // (and this group the state, for its dot)
                 phase ^= 1;
             }
             bad = ds.template put<kFull3>(sm.tiles.ds[0]);
         }
         __syncthreads();
-        if (pending && decay_warp) finish_dg(0);
+        if (pending && dg_warp) finish_dg(0);
         if (sm.sync.failed) ds.pairs([](float& x, float& y1, int, int) { x = y1 = __int_as_float(0x7fc00000); });
         if (it.first) ds.store(p.dh0 + ((int64_t)it.seq * z.heads + h) * np + col, z.n, cols, z.p);
         sm.sync.end(Smem::cols);
         return;
     }
 
-    for (int c = nc - 1; c >= 0; --c) {
+    for (int c = nc; c >= 0; --c) {
         const int t = c * kChunk, rows = min(kChunk, len - t);
-        __syncthreads();
-        const bool slow = __syncthreads_or(put(c));
+        const bool slow = start(c, false, phase);
+        if (c == nc) continue;
         if (slow) {
-            if (c > 0) fetch(c - 1);
             __syncthreads();
             walk(c);
             __syncthreads();
             continue;
         }
-        if (threadIdx.x == 0) {
-            t5::fence_after();
-            products<NS, NS, kFull3>(tm + Smem::at, of(K), of(Q), n16, t5::instr(kChunk, false, false), false);
-            products<NS, NS, kFull3>(tm + Smem::dt, of(V), of(Y), p16, t5::instr(kChunk, false, false), false);
-            t5::commit(&sm.sync.bars[0]);
-            products<NS, MS, MS>(tm + Smem::gv, of(K), of(Sk), n16, t5::instr(p16 * 16, false, false), false);
-            products<NS, kFull3, kFull3>(tm + Smem::gk, of(V), of(dS), p16, t5::instr(n16 * 16, false, true), false);
-            t5::commit(&sm.sync.bars[1]);
-            if (!Smem::one_state) {
-                products<NS, kFull3, kFull3>(tm + Smem::gq, of(Y), of(S), p16, t5::instr(n16 * 16, false, true), false);
-                t5::commit(&sm.sync.bars[2]);
-            }
-            if (!Smem::late) {
-                products<kFull3, NS, kFull3>(tm + Smem::inc, of(Yw), of(Qt), kChunk / 16, t5::instr(NT, true, true), false);
-                t5::commit(&sm.sync.bars[3]);
-            }
-        }
-        __syncwarp();
-        put_state(phase);
-        if (Smem::one_state && threadIdx.x == 0) {
-            t5::fence_after();
-            products<NS, kFull3, kFull3>(tm + Smem::gq, of(Y), of(S), p16, t5::instr(n16 * 16, false, true), false);
-            t5::commit(&sm.sync.bars[2]);
-        }
-        __syncwarp();
-        if (c > 0) fetch(c - 1);
         const Decays& d = sm.d[c & 1];
-        if (group == 0) {
-            const float hi0 = d.hi[row], lo0 = d.lo[row], hi1 = d.hi[row + 8], lo1 = d.lo[row + 8], u0 = d.until[row], u1 = d.until[row + 8];
-            sm.sync.wait(0, phase);
-            bf16* const dp = sm.tiles.scores();
-            float run[2] = {0.0f, 0.0f};                      // sums of W over the queries behind the block
-#pragma unroll 1
-            for (int ib = 3; ib >= 0; --ib) {
-                uint32_t r[2][2][MS] = {}, r2[2][2][MS] = {};
-                if (ib >= w) {
-                    float at[2][4], dt[2][4];
-                    t5::ld16(at, tm + Smem::at + lanes + 16 * ib);
-                    t5::ld16(dt, tm + Smem::dt + lanes + 16 * ib);
-                    t5::wait_ld();
-                    float W[2][2][2], sum[2][2] = {};         // sum: of the four columns, over this warp's keys before them
+        // ---- scores: this warp's block of queries, and a block of zeros before the keys
+        const float hi0 = d.hi[row], lo0 = d.lo[row], hi1 = d.hi[row + 8], lo1 = d.lo[row + 8], u0 = d.until[row], u1 = d.until[row + 8];
+        bf16* const dp = sm.tiles.scores();
+        auto put_block = [&](int ib, const uint32_t(&r)[2][2][MS], const uint32_t(&r2)[2][2][MS]) {
 #pragma unroll
-                    for (int q2 = 0; q2 < 2; ++q2) {
-                        const int i = ib * 16 + q2 * 8 + 2 * lq;
-                        const float2 hi = *(const float2*)&d.hi[i], lo = *(const float2*)&d.lo[i];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const bool in = i + (e & 1) >= row + (e & 2) * 4;
-                            const float f = between(e & 1 ? hi.y : hi.x, e & 1 ? lo.y : lo.x, e & 2 ? hi1 : hi0, e & 2 ? lo1 : lo0);
-                            float &a = at[q2][e], &b = dt[q2][e];
-                            a = in ? a * f : 0.0f;
-                            W[e >> 1][q2][e & 1] = in ? a * b : 0.0f;
-                            b = in ? b * f : 0.0f;
-                        }
-                        split<MS>(at[q2][0], at[q2][1], r[q2][0]);
-                        split<MS>(at[q2][2], at[q2][3], r[q2][1]);
-                        split<MS>(dt[q2][0], dt[q2][1], r2[q2][0]);
-                        split<MS>(dt[q2][2], dt[q2][3], r2[q2][1]);
-                    }
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const int j = row + 8 * half, i = ib * 16 + 2 * lq;
-                        float ex[2], all[2];
-#pragma unroll
-                        for (int q2 = 0; q2 < 2; ++q2) {
-                            float s = W[half][q2][0] + W[half][q2][1];
-                            float o = __shfl_down_sync(kFull, s, 1, 4);
-                            if (lq < 3) s += o;
-                            o = __shfl_down_sync(kFull, s, 2, 4);
-                            if (lq < 2) s += o;
-                            o = __shfl_down_sync(kFull, s, 1, 4);
-                            ex[q2] = lq < 3 ? o : 0.0f;
-                            all[q2] = __shfl_sync(kFull, s, 0, 4);
-                        }
-                        float u = run[half] + ex[1] + W[half][1][1];
-                        if (j < i + 9) sum[1][1] += u;
-                        u += W[half][1][0];
-                        if (j < i + 8) sum[1][0] += u;
-                        u = run[half] + all[1] + ex[0] + W[half][0][1];
-                        if (j < i + 1) sum[0][1] += u;
-                        u += W[half][0][0];
-                        if (j < i) sum[0][0] += u;
-                        run[half] += all[1] + all[0];
-                    }
-#pragma unroll
-                    for (int q2 = 0; q2 < 2; ++q2)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                            for (int o = 4; o < 32; o <<= 1) sum[q2][e] += __shfl_xor_sync(kFull, sum[q2][e], o);
-                            if (l < 4) sm.pairs[w][ib * 16 + q2 * 8 + 2 * lq + e] = sum[q2][e];
-                        }
-                }
-#pragma unroll
-                for (int m = 0; m < MS; ++m) {
-                    t5::st16(tm + Smem::piece(m) + lanes + 8 * ib, r[0][0][m], r[0][1][m], r[1][0][m], r[1][1][m]);
-#pragma unroll
-                    for (int q2 = 0; q2 < 2; ++q2)
-#pragma unroll
-                        for (int half = 0; half < 2; ++half)
-                            *(uint32_t*)(dp + m * Wide<kP>::elements + Wide<kP>::at(row + 8 * half, ib * 16 + q2 * 8 + 2 * lq)) = r2[q2][half][m];
-                }
-            }
-            t5::fence_smem();
-            sm.sync.wait(1, phase);
-            for (int pb = 0; pb < p16; ++pb) {
-                float x[2][4];
-                t5::ld16(x, tm + Smem::gv + lanes + 16 * pb);
-                t5::wait_ld();
+            for (int m = 0; m < MS; ++m) {
+                t5::st16(tm + Smem::piece + lanes + 32 * m + 8 * ib, r[0][0][m], r[0][1][m], r[1][0][m], r[1][1][m]);
 #pragma unroll
                 for (int q2 = 0; q2 < 2; ++q2)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[q2][e] *= e < 2 ? u0 : u1;
-                t5::st_acc16(tm + Smem::gv + lanes + 16 * pb, x);
+                    for (int half = 0; half < 2; ++half)
+                        *(uint32_t*)(dp + m * Wide<kP>::elements + Wide<kP>::at(row + 8 * half, ib * 16 + q2 * 8 + 2 * lq)) = r2[q2][half][m];
             }
-            t5::wait_st();
-            t5::fence_before();
-            named_sync(1, 384);
-            if (threadIdx.x == 0) {
-                t5::fence_after();
-                products<MS, NS, MS>(tm + Smem::gv, [&](int s, int i) { return tm + Smem::piece(s) + 8 * i; }, of(Yt), kChunk / 16,
-                                     t5::instr(p16 * 16, false, true), true);
-                t5::commit(&sm.sync.bars[4]);
+        };
+        auto block = [&](int ib, float(&at)[2][4], float(&dt)[2][4]) {
+            uint32_t r[2][2][MS], r2[2][2][MS];
+            float W[2][2][2], sum[2][2] = {};                 // sum: of the four columns, over this warp's keys before them
+#pragma unroll
+            for (int q2 = 0; q2 < 2; ++q2) {
+                const int i = ib * 16 + q2 * 8 + 2 * lq;
+                const float2 hi = *(const float2*)&d.hi[i], lo = *(const float2*)&d.lo[i];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool in = i + (e & 1) >= row + (e & 2) * 4;
+                    const float f = between(e & 1 ? hi.y : hi.x, e & 1 ? lo.y : lo.x, e & 2 ? hi1 : hi0, e & 2 ? lo1 : lo0);
+                    float &a = at[q2][e], &b = dt[q2][e];
+                    a = in ? a * f : 0.0f;
+                    W[e >> 1][q2][e & 1] = in ? a * b : 0.0f;
+                    b = in ? b * f : 0.0f;
+                }
+                split<MS>(at[q2][0], at[q2][1], r[q2][0]);
+                split<MS>(at[q2][2], at[q2][3], r[q2][1]);
+                split<MS>(dt[q2][0], dt[q2][1], r2[q2][0]);
+                split<MS>(dt[q2][2], dt[q2][3], r2[q2][1]);
             }
-            __syncwarp();
-            sm.sync.wait(4, phase);
-            const int how = alignment(dv, v_st);
-            for (int pb = 0; pb < p16; ++pb) {
-                float x[2][4];
-                t5::ld16(x, tm + Smem::gv + lanes + 16 * pb);
-                t5::wait_ld();
-                store_rows(dv + t * v_st, v_st, rows, cols, row, 16 * pb, x, how);
-            }
-        } else {
-            // dk (rows as keys) and dq (rows as queries): the far part, decayed in place, whose dot with the row itself is
-            // its share of dg; then the near part on top of it
-            const bool as_keys = group == 1;
-            const float* decay = as_keys ? d.until : d.since;
-            const float u0 = decay[row], u1 = decay[row + 8];
-            const uint32_t acc = tm + (as_keys ? Smem::gk : Smem::gq) + lanes;
-            const bf16* const self = as_keys ? sm.tiles.k[0] : sm.tiles.q[0];
-            float dot0 = 0.0f, dot1 = 0.0f;
-            sm.sync.wait(as_keys ? 1 : 2, phase);
-            for (int nb = 0; nb < n16; ++nb) {
-                float x[2][4];
-                t5::ld16(x, acc + 16 * nb);
-                t5::wait_ld();
+            put_block(ib, r, r2);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int j = row + 8 * half, i = ib * 16 + 2 * lq;
+                float ex[2], all[2];                          // of the lanes behind this one, of all four
 #pragma unroll
                 for (int q2 = 0; q2 < 2; ++q2) {
+                    float s = W[half][q2][0] + W[half][q2][1];
+                    float o = __shfl_down_sync(kFull, s, 1, 4);
+                    if (lq < 3) s += o;
+                    o = __shfl_down_sync(kFull, s, 2, 4);
+                    if (lq < 2) s += o;
+                    o = __shfl_down_sync(kFull, s, 1, 4);
+                    ex[q2] = lq < 3 ? o : 0.0f;
+                    all[q2] = __shfl_sync(kFull, s, 0, 4);
+                }
+                float u = ex[1] + W[half][1][1];
+                if (j < i + 9) sum[1][1] += u;
+                u += W[half][1][0];
+                if (j < i + 8) sum[1][0] += u;
+                u = all[1] + ex[0] + W[half][0][1];
+                if (j < i + 1) sum[0][1] += u;
+                u += W[half][0][0];
+                if (j < i) sum[0][0] += u;
+                if (lq == 0) sm.rows[c & 1][ib][j] = all[0] + all[1];
+            }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[q2][e] *= e < 2 ? u0 : u1;
+            for (int q2 = 0; q2 < 2; ++q2)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) sum[q2][e] += __shfl_xor_sync(kFull, sum[q2][e], o);
+                    if (l < 4) sm.pairs[c & 1][w][ib * 16 + q2 * 8 + 2 * lq + e] = sum[q2][e];
+                }
+        };
+        // the first quarter has four blocks for three warps
+        const int blocks_here = w + group > 3 ? 0 : w == 0 && group == 0 ? 2 : 1;
+        auto load = [&](int ib, float(&at)[2][4], float(&dt)[2][4]) {
+            t5::ld16x2(at, tm + Smem::at + lanes + 16 * ib, dt, tm + Smem::dt + lanes + 16 * ib);
+        };
+        sm.sync.wait(kScores, phase);
+        if constexpr (Smem::over) {
+            float at[2][4], dt[2][4], at2[2][4], dt2[2][4];
+            if (blocks_here > 0) load(w + group, at, dt);
+            if (blocks_here > 1) load(3, at2, dt2);
+            t5::fence_before();
+            named_sync(1, 384);
+            t5::fence_after();
+            if (blocks_here > 0) block(w + group, at, dt);
+            if (blocks_here > 1) block(3, at2, dt2);
+        } else {
+#pragma unroll 1
+            for (int n = 0; n < blocks_here; ++n) {
+                const int ib = n ? 3 : w + group;
+                float at[2][4], dt[2][4];
+                load(ib, at, dt);
+                block(ib, at, dt);
+            }
+        }
+        if (group < w) {
+            const uint32_t none[2][2][MS] = {};
+            put_block(group, none, none);
+        }
+        t5::fence_smem();
+
+        // ---- far parts; those of dk and dq leave their dots with the row itself for dg
+        float dot0 = 0.0f, dot1 = 0.0f;
+        const uint32_t acc = tm + (group == 0 ? Smem::gv : group == 1 ? Smem::gk : Smem::gq) + lanes;
+        sm.sync.wait(kFarV + group, phase);
+        if (group == 0) {
+            decay_far(acc, p16, u0, u1, [](float(&)[2][4], int) {});
+        } else {
+            const bf16* const self = group == 1 ? sm.tiles.k[0] : sm.tiles.q[0];
+            decay_far(acc, n16, group == 1 ? u0 : d.since[row], group == 1 ? u1 : d.since[row + 8], [&](float(&x)[2][4], int nb) {
+#pragma unroll
+                for (int q2 = 0; q2 < 2; ++q2) {
                     const int n = 16 * nb + 8 * q2 + 2 * lq;
                     const float2 k0 = from_pieces<NS>(self + Wide<NT>::at(row, n), Wide<NT>::elements);
                     const float2 k1 = from_pieces<NS>(self + Wide<NT>::at(row + 8, n), Wide<NT>::elements);
                     dot0 = fmaf(k0.x, x[q2][0], fmaf(k0.y, x[q2][1], dot0));
                     dot1 = fmaf(k1.x, x[q2][2], fmaf(k1.y, x[q2][3], dot1));
                 }
-                t5::st_acc16(acc + 16 * nb, x);
-            }
+            });
 #pragma unroll
             for (int o = 1; o < 4; o <<= 1) {
                 dot0 += __shfl_xor_sync(kFull, dot0, o);
                 dot1 += __shfl_xor_sync(kFull, dot1, o);
             }
             if (lq == 0) {
-                float* out = as_keys ? sm.of_k : sm.of_q;
+                float* out = group == 1 ? sm.of_k[c & 1] : sm.of_q[c & 1];
                 out[row] = dot0;
                 out[row + 8] = dot1;
             }
-            t5::wait_st();
-            t5::fence_before();
-            named_sync(1, 384);
-            if (threadIdx.x % 128 == 0) {
-                t5::fence_after();
-                if (as_keys) products<MS, NS, MS>(tm + Smem::gk, of(P), of(Qt), kChunk / 16, t5::instr(n16 * 16, false, true), true);
-                else products<MS, NS, MS>(tm + Smem::gq, of(Pt), of(Kt), kChunk / 16, t5::instr(n16 * 16, true, true), true);
-                t5::commit(&sm.sync.bars[4 + group]);
-            }
-            __syncwarp();
-            sm.sync.wait(4 + group, phase);
-            const RowsOut<T>& out = as_keys ? dk : dq;
-            const int how = out.part ? alignment(out.part, qk_st) : alignment(out.whole, qk_st);
-            for (int nb = 0; nb < n16; ++nb) {
-                float x[2][4];
-                t5::ld16(x, acc + 16 * nb);
-                t5::wait_ld();
-                if (out.part) store_rows(out.part + (row_at + t) * qk_st, qk_st, rows, z.n, row, 16 * nb, x, how);
-                else store_rows(out.whole + (row_at + t) * qk_st, qk_st, rows, z.n, row, 16 * nb, x, how);
+        }
+        t5::wait_st();
+        t5::fence_before();
+        named_sync(1, 384);
+        if (w == 0 && t5::elect()) {
+            t5::fence_after();
+            const Operand<NT, false> Qt(sm.tiles.q), Kt(sm.tiles.k);
+            const Operand<kP, true> P(sm.tiles.scores());
+            const Operand<kP, false> Yt(sm.tiles.dy), Pt(sm.tiles.scores());
+            if (group == 0)
+                products<MS, NS, MS, kChunk / 16>(tm + Smem::gv, [&](int s, int i) { return tm + Smem::piece + 32 * s + 8 * i; }, Yt,
+                                                  t5::instr(p16 * 16, false, true), true);
+            else if (group == 1)
+                products<MS, NS, MS, kChunk / 16>(tm + Smem::gk, P, Qt, t5::instr(n16 * 16, false, true), true);
+            else
+                products<MS, NS, MS, kChunk / 16>(tm + Smem::gq, Pt, Kt, t5::instr(n16 * 16, true, true), true);
+            t5::commit(&sm.sync.bars[kNearV + group]);
+        }
+        __syncwarp();
+        sm.sync.wait(kNearV + group, phase);
+        // ---- out: dv, or (whole or as a part) dk and dq
+        const RowsOut<T> o = group == 0 ? RowsOut<T>{dv + t * v_st, nullptr, v_st} : rows_out(group == 1 ? p.dk : p.dq, row_at + t);
+        const int width = group == 0 ? cols : z.n, blocks = group == 0 ? p16 : n16;
+#pragma unroll 1
+        for (int nb = 0; nb < blocks; nb += 2) {
+            float x[2][4], x2[2][4];
+            t5::ld16x2(x, acc + 16 * nb, x2, acc + 16 * min(nb + 1, blocks - 1));
+            if (o.part) {
+                store_rows<VEC>(o.part, o.st, rows, width, row, 16 * nb, x[0], x[1]);
+                store_rows<VEC>(o.part, o.st, rows, width, row, 16 * nb + 16, x2[0], x2[1]);
+            } else {
+                store_rows<VEC>(o.whole, o.st, rows, width, row, 16 * nb, x[0], x[1]);
+                store_rows<VEC>(o.whole, o.st, rows, width, row, 16 * nb + 16, x2[0], x2[1]);
             }
         }
         t5::fence_before();
@@ -558,13 +614,13 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
 }
 
 template <typename T, int NT>
-bcm_status launch_bwd(const BwdArgs& p, cudaStream_t stream) {
+bcm_status launch_bwd(const BwdArgs& p, bool vec, cudaStream_t stream) {
     using Smem = BwdSmem<T, NT>;
     constexpr size_t smem = sizeof(Smem) + 1024;
     static_assert(smem <= 227 * 1024, "shared memory of a block");
     static_assert(sizeof(typename Smem::Tiles) >= sizeof(float) * (NT * kP + 4 * NT + kBwdThreads + kBwdThreads / 32), "the state of back_tokens");
-    static_assert(Smem::gq + NT <= 512 && (Smem::late || Smem::inc + NT <= 512), "tensor memory of a block");
-    auto kernel = bwd_kernel<T, NT>;
+    static_assert(Smem::gq + NT <= 512 && Smem::piece + 32 * Smem::MS <= 512, "tensor memory of a block");
+    auto kernel = vec ? bwd_kernel<T, NT, true> : bwd_kernel<T, NT, false>;
     bcm_status st = allow_smem(kernel, smem);
     if (st != BCM_OK) return st;
     kernel<<<(unsigned)(p.z.items * p.z.heads * p.z.slices), kBwdThreads, smem, stream>>>(p);
@@ -681,19 +737,20 @@ extern "C" bcm_status bcm_decay_attn_bwd(const bcm_decay_attn_args* a, cudaStrea
                v = rows_of(a->v, a->v_stride_b, a->v_stride_t, a->v_stride_h), dy = rows_of(a->dy, a->dy_stride_b, a->dy_stride_t, a->dy_stride_h);
     const bool apart = room.shares > 1, dg_parts = z.slices > 1 || room.fixed;
     const int64_t tokens = (int64_t)(z.cu ? 1 : z.batch) * z.seqlen;
+    const bool vec = aligned(a, true);
     return dispatch(a->dtype, a->dim_k, [&](auto type, auto n) -> bcm_status {
         using T = decltype(type);
         bcm_status r = BCM_OK;
             if (plan.cut) {
                 // without dy an item's own part is 0: its rows count as none
                 PartArgs pa{plan.z, q, dy, a->log_decay, a->g_stride_b, a->g_stride_t, a->g_stride_h, parts};
-                if ((r = launch_part<T, n, true>(pa, stream)) != BCM_OK) return r;
+                if ((r = launch_part<T, n, true>(pa, vec, stream)) != BCM_OK) return r;
                 if ((r = join(plan, parts, a->dh_last, true, stream)) != BCM_OK) return r;
             }
             const BwdArgs ba{plan.z, q, k, v, dy, a->log_decay, a->g_stride_b, a->g_stride_t, a->g_stride_h, (const float*)a->ckpt,
                              a->dh_last, parts.state, apart ? (void*)(ws + room.dq) : a->dq, apart ? (void*)(ws + room.dk) : a->dk,
                              a->dv, dg_parts ? (float*)(ws + room.dg) : a->dlog_decay, a->dh0, room.shares};
-            if ((r = launch_bwd<T, n>(ba, stream)) != BCM_OK) return r;
+            if ((r = launch_bwd<T, n>(ba, vec, stream)) != BCM_OK) return r;
             if (apart) {
                 const int64_t count = tokens * z.qk_heads * z.n;
                 if ((r = add_parts((const float*)(ws + room.dq), room.shares, count, (T*)a->dq, stream)) != BCM_OK) return r;

@@ -65,6 +65,16 @@ Plan plan_of(const bcm_decay_attn_args* a, bool backward) {
     return plan;
 }
 
+bool aligned(const bcm_decay_attn_args* a, bool backward) {
+    const int64_t size = (int64_t)dtype_size(a->dtype);
+    auto in = [&](const void* p, int64_t sb, int64_t st, int64_t sh) { return on_16(p, sb * size) && on_16(p, st * size) && on_16(p, sh * size); };
+    if (a->dim_k % 8 || a->dim_v % 8 || !in(a->q, a->q_stride_b, a->q_stride_t, a->q_stride_h) ||
+        !in(a->k, a->k_stride_b, a->k_stride_t, a->k_stride_h) || !in(a->v, a->v_stride_b, a->v_stride_t, a->v_stride_h))
+        return false;
+    if (!backward) return on_16(a->y, 0);
+    return in(a->dy, a->dy_stride_b, a->dy_stride_t, a->dy_stride_h) && on_16(a->dq, 0) && on_16(a->dk, 0) && on_16(a->dv, 0) && on_16(a->workspace, 0);
+}
+
 Parts parts_of(const Plan& plan, void* workspace) {
     char* ws = (char*)workspace;
     return plan.cut ? Parts{(float*)(ws + plan.state_at), (float*)(ws + plan.whole_at)} : Parts{nullptr, nullptr};
@@ -225,7 +235,7 @@ __device__ __noinline__ void walk_tokens(const FwdArgs& p, const T* q, const T* 
     }
 }
 
-template <typename T, int NT>
+template <typename T, int NT, bool VEC>
 __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_kernel(const __grid_constant__ FwdArgs p) {
     extern __shared__ unsigned char smem_raw[];
     using Smem = FwdSmem<T, NT>;
@@ -245,85 +255,102 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
     const T* v = row_ptr<T>(p.v, z, it.seq, it.t0, h) + col;
     const float* g = p.g + (z.cu ? 0 : it.seq * p.g_sb) + it.t0 * p.g_st + h * p.g_sh;
     T* y = (T*)p.y + ((z.cu ? 0 : (int64_t)it.seq * z.seqlen) + it.t0) * y_st + (int64_t)h * z.p + col;
-    const int vq = alignment(q, p.q.st), vk = alignment(k, p.k.st), vv = alignment(v, p.v.st), vy = alignment(y, y_st);
     const int np = z.n * z.p;
     const int len = it.t1 - it.t0, nc = (len + kChunk - 1) / kChunk;
-    const int l = lane_id(), w = (threadIdx.x >> 5) & 3, row = w * 16 + (l >> 2);
-    const bool state_warp = threadIdx.x >= 128, decay_warp = threadIdx.x >= 128 && threadIdx.x < 160;
+    const int warp = t5::warp_id(), l = lane_id(), w = warp & 3, row = w * 16 + (l >> 2);
+    const bool state_warp = warp >= 4, decay_warp = warp == 4;
     const int p16 = (cols + 15) / 16;
 
-    Pending<T, NT, kFwdThreads> pq, pk;
-    Pending<T, kP, kFwdThreads> pv;
-    float g0 = 0.0f, g1 = 0.0f;
-    auto fetch = [&](int c) {
-        const int t = c * kChunk, rows = min(kChunk, len - t);
-        pq.fetch(q + t * p.q.st, p.q.st, rows, z.n, vq);
-        pk.fetch(k + t * p.k.st, p.k.st, rows, z.n, vk);
-        pv.fetch(v + t * p.v.st, p.v.st, rows, cols, vv);
-        if (decay_warp) {
-            g0 = 2 * l < rows ? g[(int64_t)(t + 2 * l) * p.g_st] : 0.0f;
-            g1 = 2 * l + 1 < rows ? g[(int64_t)(t + 2 * l + 1) * p.g_st] : 0.0f;
-        }
-    };
-    // the tiles of the fetched chunk; whether a value was not finite
-    auto put = [&](int c) {
-        bool bad = pq.bad() | pk.bad() | pv.bad();
-        if (decay_warp) bad |= !(g0 <= 3.38e38f && g1 <= 3.38e38f);
-        pq.put(sm.tiles.q[0]);
-        pk.put(sm.tiles.k[0]);
-        pv.put(sm.tiles.v[0]);
-        pv.put_weighted(sm.tiles.vw[0], sm.d[c & 1].until);
-        t5::fence_smem();
-        t5::fence_before();
-        return bad;
-    };
-    // token by token, the state through shared memory
-    auto walk = [&](int c) {
-        const int t = c * kChunk;
-        float* f = (float*)&sm.tiles;
-        walk_tokens<T>(p, q + t * p.q.st, k + t * p.k.st, v + t * p.v.st, g + t * p.g_st, y + t * y_st, min(kChunk, len - t), cols, f, f + NT * kP);
-    };
-    if (nc > 0) fetch(0);
+    Pending<T, NT, kFwdThreads, VEC> pq, pk;
+    Pending<T, kP, kFwdThreads, VEC> pv;
+    Logs logs{g, p.g_st};
+    State<NT> st;                                             // (warps 4 to 7)
+    bool bad = false, bad_logs = false;
     sm.sync.init(Smem::cols);
-    const uint32_t tm = sm.sync.tmem, lanes = (uint32_t)w << 21;
-    uint32_t phase = 0;
-
+    const uint32_t tm = __shfl_sync(kFull, sm.sync.tmem, 0), lanes = (uint32_t)w << 21;
     if (state_warp) {
-        State<NT> st;
         const float* from = it.first ? (p.h0 ? p.h0 + ((int64_t)it.seq * z.heads + h) * np : nullptr)
                                      : p.enter + ((int64_t)item * z.heads + h) * np;
-        if (decay_warp) decays_of(sm.d[0], g0, g1);
+        if (decay_warp) logs.fetch(0, len);
         if (from) st.load(from + col, z.n, cols, z.p);
         else st.zero();
-        bool bad = st.template put<MS>(sm.s[0]);
-        for (int c = 0; c < nc; ++c) {
-            if (p.ckpt) {
+        bad = st.template put<MS>(sm.s[0]);
+        if (decay_warp) {
+            bad_logs = logs.bad();
+            decays_of(sm.d[0], logs.a, logs.b);
+            logs.fetch(kChunk, len);
+        }
+    }
+    uint32_t phase = 0;
+    for (int c = -1; c < nc; ++c) {
+        const int t = c * kChunk, rows = min(kChunk, len - t);
+        bool slow = false;
+        if (c >= 0) {
+            if (state_warp && p.ckpt) {
                 float* to = p.ckpt + (((int64_t)(it.chunk + c) * z.heads + h) * z.slices + hs % z.slices) * (NT * kP);
                 st.pairs([&](float& x, float& y1, int pp, int n) {
                     if (pp < cols) *(float2*)(to + pp * NT + n) = make_float2(x, y1);
                 });
             }
             __syncthreads();                                  // decays are there; the chunk before is done with the tiles
-            bad |= put(c);
-            const bool slow = __syncthreads_or(bad);
-            const float whole = sm.d[c & 1].whole;
-            if (c + 1 < nc) {
-                fetch(c + 1);
-                if (decay_warp) decays_of(sm.d[(c + 1) & 1], g0, g1);
+            bad |= bad_logs | pq.bad() | pk.bad() | pv.bad();
+            pq.put(sm.tiles.q[0]);
+            pk.put(sm.tiles.k[0]);
+            pv.put(sm.tiles.v[0]);
+            pv.put_weighted(sm.tiles.vw[0], sm.d[c & 1].until);
+            t5::fence_smem();
+            t5::fence_before();
+            slow = __syncthreads_or(bad);
+            bad = false;
+            if (!slow && warp == 0 && t5::elect()) {
+                t5::fence_after();
+                const Operand<NT, true> Q(sm.tiles.q), K(sm.tiles.k), S(sm.s);
+                products<NS, NS, MS, NT / 16>(tm + Smem::scores, Q, K, t5::instr(kChunk, false, false), false);
+                t5::commit(&sm.sync.bars[0]);
+                products<NS, MS, MS, NT / 16>(tm + Smem::far, Q, S, t5::instr(p16 * 16, false, false), false);
+                t5::commit(&sm.sync.bars[1]);
             }
-            if (slow) {
-                float* f = (float*)&sm.tiles;
+            if (!slow && warp == 4 && t5::elect()) {
+                t5::fence_after();
+                const Operand<kP, false> Vw(sm.tiles.vw);
+                const Operand<NT, false> Kt(sm.tiles.k);
+                products<kFull3, NS, kFull3, kChunk / 16>(tm + Smem::inc, Vw, Kt, t5::instr(NT, true, true), false);
+                t5::commit(&sm.sync.bars[2]);
+            }
+            __syncwarp();
+        }
+        if (c + 1 < nc) {
+            const int t2 = t + kChunk, r2 = min(kChunk, len - t2);
+            pq.fetch(q + t2 * p.q.st, p.q.st, r2, z.n);
+            pk.fetch(k + t2 * p.k.st, p.k.st, r2, z.n);
+            pv.fetch(v + t2 * p.v.st, p.v.st, r2, cols);
+        }
+        if (c < 0) continue;
+        if (slow) {
+            // token by token, the state through shared memory
+            float* f = (float*)&sm.tiles;
+            if (state_warp)
                 st.pairs([&](float& x, float& x1, int pp, int n) {
                     f[n * kP + pp] = x;
                     f[(n + 1) * kP + pp] = x1;
                 });
-                __syncthreads();
-                walk(c);
+            __syncthreads();
+            walk_tokens<T>(p, q + t * p.q.st, k + t * p.k.st, v + t * p.v.st, g + t * p.g_st, y + t * y_st, rows, cols, f, f + NT * kP);
+            if (state_warp) {
                 st.pairs([&](float& x, float& x1, int pp, int n) {
                     x = f[n * kP + pp];
                     x1 = f[(n + 1) * kP + pp];
                 });
-            } else {
+            }
+        }
+        if (state_warp) {
+            if (decay_warp && c + 1 < nc) {
+                bad_logs = logs.bad();
+                decays_of(sm.d[(c + 1) & 1], logs.a, logs.b);
+                logs.fetch(t + 2 * kChunk, len);
+            }
+            if (!slow) {
+                const float whole = sm.d[c & 1].whole;
                 sm.sync.wait(2, phase);
                 st.advance(tm + Smem::inc + lanes, whole);
                 sm.sync.wait(1, phase);                       // the products with the entering state have read it
@@ -331,39 +358,9 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
                 phase ^= 1;
             }
             bad = st.template put<MS>(sm.s[0]);
-        }
-        if (sm.sync.failed) st.pairs([](float& x, float& y1, int, int) { x = y1 = __int_as_float(0x7fc00000); });
-        if (it.last) st.store(p.h_last + ((int64_t)it.seq * z.heads + h) * np + col, z.n, cols, z.p);
-        sm.sync.end(Smem::cols);
-        return;
-    }
-    for (int c = 0; c < nc; ++c) {
-        const int t = c * kChunk, rows = min(kChunk, len - t);
-        __syncthreads();
-        const bool slow = __syncthreads_or(put(c));
-        if (slow) {
-            if (c + 1 < nc) fetch(c + 1);
-            __syncthreads();
-            walk(c);
             continue;
         }
-        if (threadIdx.x == 0) {
-            t5::fence_after();
-            const Operand<NT, true> Q{t5::smem_u32(sm.tiles.q)}, K{t5::smem_u32(sm.tiles.k)}, S{t5::smem_u32(sm.s)};
-            const Operand<NT, false> Kt{t5::smem_u32(sm.tiles.k)};
-            const Operand<kP, false> V{t5::smem_u32(sm.tiles.vw)};
-            auto fq = [&](int s, int i) { return Q.desc(s, i); };
-            const int n16 = (z.n + 15) / 16;
-            products<NS, NS, MS>(tm + Smem::scores, fq, [&](int u, int i) { return K.desc(u, i); }, n16, t5::instr(kChunk, false, false), false);
-            t5::commit(&sm.sync.bars[0]);
-            products<NS, MS, MS>(tm + Smem::far, fq, [&](int u, int i) { return S.desc(u, i); }, n16, t5::instr(p16 * 16, false, false), false);
-            t5::commit(&sm.sync.bars[1]);
-            products<kFull3, NS, kFull3>(tm + Smem::inc, [&](int s, int i) { return V.desc(s, i); }, [&](int u, int i) { return Kt.desc(u, i); },
-                                         kChunk / 16, t5::instr(NT, true, true), false);
-            t5::commit(&sm.sync.bars[2]);
-        }
-        __syncwarp();
-        if (c + 1 < nc) fetch(c + 1);
+        if (slow) continue;
         const Decays& d = sm.d[c & 1];
         const float hi0 = d.hi[row], lo0 = d.lo[row], hi1 = d.hi[row + 8], lo1 = d.lo[row + 8], since0 = d.since[row], since1 = d.since[row + 8];
         sm.sync.wait(0, phase);
@@ -371,7 +368,6 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
 #pragma unroll
         for (int jb = 0; jb < 4; ++jb)
             if (jb <= w) t5::ld16(sc[jb], tm + Smem::scores + lanes + 16 * jb);
-        t5::wait_ld();
 #pragma unroll
         for (int jb = 0; jb < 4; ++jb) {
             uint32_t r[2][2][MS] = {};                        // [tile][half]
@@ -396,7 +392,6 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
             for (int pb = 0; pb < p16; ++pb) {
                 float x[2][4];
                 t5::ld16(x, tm + Smem::far + lanes + 16 * pb);
-                t5::wait_ld();
 #pragma unroll
                 for (int q2 = 0; q2 < 2; ++q2)
 #pragma unroll
@@ -407,45 +402,50 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
         t5::wait_st();
         t5::fence_before();
         named_sync(1, 128);
-        if (threadIdx.x == 0) {
+        if (warp == 0 && t5::elect()) {
             t5::fence_after();
-            const Operand<kP, false> V{t5::smem_u32(sm.tiles.v)};
-            products<MS, NS, MS>(tm + Smem::near, [&](int s, int i) { return tm + Smem::scores + 32 * s + 8 * i; },
-                                 [&](int u, int i) { return V.desc(u, i); }, kChunk / 16, t5::instr(p16 * 16, false, true), !Smem::apart);
+            const Operand<kP, false> V(sm.tiles.v);
+            products<MS, NS, MS, kChunk / 16>(tm + Smem::near, [&](int s, int i) { return tm + Smem::scores + 32 * s + 8 * i; }, V,
+                                              t5::instr(p16 * 16, false, true), !Smem::apart);
             t5::commit(&sm.sync.bars[3]);
         }
         __syncwarp();
         sm.sync.wait(3, phase);                               // (and with it the far part)
         T* const out = y + (int64_t)t * y_st;
-        for (int pb = 0; pb < p16; ++pb) {
-            float x[2][4];
-            t5::ld16(x, tm + Smem::near + lanes + 16 * pb);
-            if (Smem::apart) {
-                float f[2][4];
-                t5::ld16(f, tm + Smem::far + lanes + 16 * pb);
-                t5::wait_ld();
 #pragma unroll
-                for (int q2 = 0; q2 < 2; ++q2)
+        for (int pb = 0; pb < kP / 16; pb += 2) {
+            if (pb >= p16) break;
+            float x[4][4];
+            if constexpr (Smem::apart) {
+                float f[4][4];
+                t5::ld32x2(x, tm + Smem::near + lanes + 16 * pb, f, tm + Smem::far + lanes + 16 * pb);
+#pragma unroll
+                for (int q2 = 0; q2 < 4; ++q2)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[q2][e] = fmaf(e < 2 ? since0 : since1, f[q2][e], x[q2][e]);
             } else {
-                t5::wait_ld();
+                t5::ld16x2((float(&)[2][4])x[0], tm + Smem::near + lanes + 16 * pb, (float(&)[2][4])x[2], tm + Smem::near + lanes + 16 * pb + 16);
             }
-            store_rows(out, y_st, rows, cols, row, 16 * pb, x, vy);
+            store_rows<VEC>(out, y_st, rows, cols, row, 16 * pb, x[0], x[1]);
+            store_rows<VEC>(out, y_st, rows, cols, row, 16 * pb + 16, x[2], x[3]);
         }
         t5::fence_before();
         phase ^= 1;
+    }
+    if (state_warp) {
+        if (sm.sync.failed) st.pairs([](float& x, float& y1, int, int) { x = y1 = __int_as_float(0x7fc00000); });
+        if (it.last) st.store(p.h_last + ((int64_t)it.seq * z.heads + h) * np + col, z.n, cols, z.p);
     }
     sm.sync.end(Smem::cols);
 }
 
 template <typename T, int NT>
-bcm_status launch_fwd(const FwdArgs& p, cudaStream_t stream) {
+bcm_status launch_fwd(const FwdArgs& p, bool vec, cudaStream_t stream) {
     using Smem = FwdSmem<T, NT>;
     constexpr size_t smem = sizeof(Smem) + 1024;
     static_assert(smem <= 227 * 1024, "shared memory of a block");
     static_assert(sizeof(typename Smem::Tiles) >= sizeof(float) * (NT * kP + kFwdThreads), "the state of walk_tokens");
-    auto kernel = fwd_kernel<T, NT>;
+    auto kernel = vec ? fwd_kernel<T, NT, true> : fwd_kernel<T, NT, false>;
     bcm_status st = allow_smem(kernel, smem);
     if (st != BCM_OK) return st;
     kernel<<<(unsigned)(p.z.items * p.z.heads * p.z.slices), kFwdThreads, smem, stream>>>(p);
@@ -552,17 +552,18 @@ extern "C" bcm_status bcm_decay_attn_fwd(const bcm_decay_attn_args* a, cudaStrea
     const Parts parts = parts_of(plan, a->workspace);
     const Rows q = rows_of(a->q, a->q_stride_b, a->q_stride_t, a->q_stride_h), k = rows_of(a->k, a->k_stride_b, a->k_stride_t, a->k_stride_h),
                v = rows_of(a->v, a->v_stride_b, a->v_stride_t, a->v_stride_h);
+    const bool vec = aligned(a, false);
     return dispatch(a->dtype, a->dim_k, [&](auto type, auto n) -> bcm_status {
         using T = decltype(type);
         if (plan.cut) {
             const PartArgs pa{plan.z, k, v, a->log_decay, a->g_stride_b, a->g_stride_t, a->g_stride_h, parts};
-            bcm_status r = launch_part<T, n, false>(pa, stream);
+            bcm_status r = launch_part<T, n, false>(pa, vec, stream);
             if (r != BCM_OK) return r;
             if ((r = join(plan, parts, a->h0, false, stream)) != BCM_OK) return r;
         }
         const FwdArgs fa{plan.z, q, k, v, a->log_decay, a->g_stride_b, a->g_stride_t, a->g_stride_h, a->h0, parts.state,
                          a->y, a->h_last, (float*)a->ckpt};
-        return launch_fwd<T, n>(fa, stream);
+        return launch_fwd<T, n>(fa, vec, stream);
     });
 }
 

@@ -26,12 +26,10 @@ struct Tile {
         constexpr int units = W / 8;
         return row * W + (((col >> 3) ^ (row / (8 / units) & (units - 1))) << 3) + (col & 7);
     }
-    // the upper and lower half of a descriptor: `far` bytes to the tile that continues the rows (MN-major operands that are
-    // wider than a tile); tiles are aligned to 1024 bytes
-    __device__ __forceinline__ static uint64_t desc(uint32_t addr, uint32_t far) {
-        constexpr uint64_t swizzle = W == 64 ? 2 : W == 32 ? 4 : 6;
-        return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(far >> 4) << 16 | (uint64_t)(16 * W >> 4) << 32 | (uint64_t)1 << 46 | swizzle << 61;
-    }
+    // the lower half of the descriptor of a tile's start, `far` bytes to the tile that continues the rows (MN-major operands
+    // that are wider than a tile), and the upper half, the same for all; tiles are aligned to 1024 bytes
+    __device__ __forceinline__ static uint32_t low(uint32_t addr, uint32_t far) { return (addr & 0x3ffff) >> 4 | (far >> 4) << 16; }
+    static constexpr uint32_t high = (16 * W >> 4) | 1u << 14 | (W == 64 ? 2u : W == 32 ? 4u : 6u) << 29;
 };
 
 // bf16 x bf16 -> fp32, 64 rows, n columns; a_mn, b_mn: MN-major operands
@@ -39,15 +37,24 @@ __host__ __device__ constexpr uint32_t instr(int n, bool a_mn, bool b_mn) {
     return 1u << 4 | 1u << 7 | 1u << 10 | (a_mn ? 1u << 15 : 0) | (b_mn ? 1u << 16 : 0) | (uint32_t)(n >> 3) << 17 | (uint32_t)(64 >> 4) << 24;
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
-                 "l"(b), "r"(idesc), "r"((uint32_t)add)
-                 : "memory");
+// an operand in shared memory: the two halves of its descriptor
+struct Desc {
+    uint32_t low, high;
+};
+
+__device__ __forceinline__ void mma(uint32_t d, Desc a, Desc b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(d), "r"(a.low), "r"(a.high), "r"(b.low), "r"(b.high), "r"(idesc),
+        "r"((uint32_t)add)
+        : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
-                 "l"(b), "r"(idesc), "r"((uint32_t)add)
-                 : "memory");
+// A at an address of tensor memory
+__device__ __forceinline__ void mma(uint32_t d, uint32_t a, Desc b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d), "r"(a), "r"(b.low), "r"(b.high), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
 }
 
 // arrives at the barrier once all products issued before by this thread are done
@@ -63,7 +70,7 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t phase) {
     const long long start = clock64();
     do {
         uint32_t done;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}"
                      : "=r"(done)
                      : "r"(smem_u32(bar)), "r"(phase)
                      : "memory");
@@ -71,6 +78,15 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t phase) {
     } while (clock64() - start < (1LL << 31));
     return false;
 }
+
+// one thread of a warp (all of it, together), known to the compiler to be one: what it computes alike for the whole warp
+// (descriptors) stays in uniform registers, from which products are issued
+__device__ __forceinline__ bool elect() {
+    uint32_t is;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(is));
+    return is != 0;
+}
+__device__ __forceinline__ int warp_id() { return __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0); }
 
 // writes to shared memory become visible to the tensor cores' reads
 __device__ __forceinline__ void fence_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -86,37 +102,78 @@ __device__ __forceinline__ void dealloc(uint32_t addr, uint32_t cols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
 }
 
-// 16 rows x 8 columns of an accumulator: row l / 4 columns 2 (l % 4) and the next, then row l / 4 + 8
-__device__ __forceinline__ void ld8(float (&r)[4], uint32_t addr) {
-    uint32_t x[4];
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(addr));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = __uint_as_float(x[i]);
-}
-// 16 rows x 16 columns
+// All threads of a warp take part in what follows, together: callers bring the warp together before (a wait or a store
+// under a condition may have left its threads apart).  A load's registers hold nothing before its wait, so both are one
+// statement.
+
+// 16 rows x 16 columns of an accumulator: row l / 4, columns 2 (l % 4) and the next (+ 8: second half), then row l / 4 + 8
 __device__ __forceinline__ void ld16(float (&r)[2][4], uint32_t addr) {
     uint32_t x[8];
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+    __syncwarp();
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
                  : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7])
-                 : "r"(addr));
+                 : "r"(addr)
+                 : "memory");
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i >> 2][i & 3] = __uint_as_float(x[i]);
 }
-__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// 16 columns at each of two addresses
+__device__ __forceinline__ void ld16x2(float (&r)[2][4], uint32_t addr, float (&r2)[2][4], uint32_t addr2) {
+    uint32_t x[16];
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%16];\n\t"
+        "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%17];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]),
+          "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15])
+        : "r"(addr), "r"(addr2)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        r[i >> 2][i & 3] = __uint_as_float(x[i]);
+        r2[i >> 2][i & 3] = __uint_as_float(x[8 + i]);
+    }
+}
+// 32 columns at each of two addresses
+__device__ __forceinline__ void ld32x2(float (&r)[4][4], uint32_t addr, float (&r2)[4][4], uint32_t addr2) {
+    uint32_t x[32];
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]),
+          "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15]), "=r"(x[16]), "=r"(x[17]), "=r"(x[18]), "=r"(x[19]), "=r"(x[20]),
+          "=r"(x[21]), "=r"(x[22]), "=r"(x[23]), "=r"(x[24]), "=r"(x[25]), "=r"(x[26]), "=r"(x[27]), "=r"(x[28]), "=r"(x[29]), "=r"(x[30]),
+          "=r"(x[31])
+        : "r"(addr), "r"(addr2)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        r[i >> 2][i & 3] = __uint_as_float(x[i]);
+        r2[i >> 2][i & 3] = __uint_as_float(x[16 + i]);
+    }
+}
 
 // 16 rows x 16 bf16 columns of an A operand (8 columns of 32 bits), in the accumulators' layout: r[2 q + half] the pair
 // of columns 8 q + 2 (l % 4), half: row l / 4 + 8
 __device__ __forceinline__ void st16(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+    __syncwarp();
     asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
 }
 // 16 rows x 16 columns of an accumulator
 __device__ __forceinline__ void st_acc16(uint32_t addr, const float (&r)[2][4]) {
+    __syncwarp();
     asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(__float_as_uint(r[0][0])),
                  "r"(__float_as_uint(r[0][1])), "r"(__float_as_uint(r[0][2])), "r"(__float_as_uint(r[0][3])), "r"(__float_as_uint(r[1][0])),
                  "r"(__float_as_uint(r[1][1])), "r"(__float_as_uint(r[1][2])), "r"(__float_as_uint(r[1][3]))
                  : "memory");
 }
-__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() {
+    __syncwarp();
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
 
 }  // namespace t5
 }  // namespace bcm

@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
     const int np = z.n * z.p;
     const int len = it.t1 - it.t0, nc = (len + kChunk - 1) / kChunk;
     const int warp = t5::warp_id(), l = lane_id(), group = warp >> 2, w = warp & 3, row = w * 16 + (l >> 2), lq = l & 3;
-    const bool decay_warp = warp == 12, dg_warp = warp == 13;
+    const bool decay_warp = warp == 13, dg_warp = warp == 14;
     const int p16 = (cols + 15) / 16, n16 = (z.n + 15) / 16;
 
     const float* const ckpt = p.ckpt + (((int64_t)it.chunk * z.heads + h) * z.slices + slice) * (NT * kP);
@@ -273,30 +273,31 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
             t5::fence_before();
             slow = __syncthreads_or(bad);
             if (!slow) {
+                // (issuing takes as long as the products: the fourth group has the time for those that are needed later)
                 if (w == 0 && t5::elect()) {
                     t5::fence_after();
                     const Operand<NT, true> Q(sm.tiles.q), K(sm.tiles.k), Sk(sm.tiles.ds);
                     const Operand<NT, false> Qt(sm.tiles.q), dS(sm.tiles.ds), S(sm.tiles.state());
                     const Operand<kP, true> V(sm.tiles.v), Y(sm.tiles.dy);
-                    const Operand<kP, false> Yw(sm.tiles.dyw);
                     if (group == 0) {
                         products<NS, NS, kFull3, NT / 16>(tm + Smem::at, K, Q, t5::instr(kChunk, false, false), false);
                         t5::commit(&sm.sync.bars[kScores]);
-                        products<NS, MS, MS, NT / 16>(tm + Smem::gv, K, Sk, t5::instr(p16 * 16, false, false), false);
-                        t5::commit(&sm.sync.bars[kFarV]);
                     } else if (group == 1) {
                         products<NS, NS, kFull3, kP / 16>(tm + Smem::dt, V, Y, t5::instr(kChunk, false, false), false);
                         t5::commit(&sm.sync.bars[kScores]);
+                    } else if (group == 3) {
+                        products<NS, MS, MS, NT / 16>(tm + Smem::gv, K, Sk, t5::instr(p16 * 16, false, false), false);
+                        t5::commit(&sm.sync.bars[kFarV]);
                         products<NS, kFull3, kFull3, kP / 16>(tm + Smem::gk, V, dS, t5::instr(n16 * 16, false, true), false);
                         t5::commit(&sm.sync.bars[kFarK]);
-                    } else if (group == 2) {
                         if (!Smem::one_state) {
                             products<NS, kFull3, kFull3, kP / 16>(tm + Smem::gq, Y, S, t5::instr(n16 * 16, false, true), false);
                             t5::commit(&sm.sync.bars[kFarQ]);
                         }
-                    } else if (!Smem::late) {
-                        products<kFull3, NS, kFull3, kChunk / 16>(tm + Smem::inc, Yw, Qt, t5::instr(NT, true, true), false);
-                        t5::commit(&sm.sync.bars[kInc]);
+                        if (!Smem::late) {
+                            products<kFull3, NS, kFull3, kChunk / 16>(tm + Smem::inc, Operand<kP, false>(sm.tiles.dyw), Qt, t5::instr(NT, true, true), false);
+                            t5::commit(&sm.sync.bars[kInc]);
+                        }
                     }
                 }
                 __syncwarp();

@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
     const int np = z.n * z.p;
     const int len = it.t1 - it.t0, nc = (len + kChunk - 1) / kChunk;
     const int warp = t5::warp_id(), l = lane_id(), w = warp & 3, row = w * 16 + (l >> 2);
-    const bool state_warp = warp >= 4, decay_warp = warp == 4;
+    const bool state_warp = warp >= 4, decay_warp = warp == 5;
     const int p16 = (cols + 15) / 16;
 
     Pending<T, NT, kFwdThreads, VEC> pq, pk;
@@ -302,19 +302,20 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
             t5::fence_before();
             slow = __syncthreads_or(bad);
             bad = false;
+            // (issuing takes as long as the products: the state's warps have the time for the long ones)
             if (!slow && warp == 0 && t5::elect()) {
                 t5::fence_after();
-                const Operand<NT, true> Q(sm.tiles.q), K(sm.tiles.k), S(sm.s);
-                products<NS, NS, MS, NT / 16>(tm + Smem::scores, Q, K, t5::instr(kChunk, false, false), false);
+                products<NS, NS, MS, NT / 16>(tm + Smem::scores, Operand<NT, true>(sm.tiles.q), Operand<NT, true>(sm.tiles.k),
+                                              t5::instr(kChunk, false, false), false);
                 t5::commit(&sm.sync.bars[0]);
-                products<NS, MS, MS, NT / 16>(tm + Smem::far, Q, S, t5::instr(p16 * 16, false, false), false);
-                t5::commit(&sm.sync.bars[1]);
             }
             if (!slow && warp == 4 && t5::elect()) {
                 t5::fence_after();
-                const Operand<kP, false> Vw(sm.tiles.vw);
-                const Operand<NT, false> Kt(sm.tiles.k);
-                products<kFull3, NS, kFull3, kChunk / 16>(tm + Smem::inc, Vw, Kt, t5::instr(NT, true, true), false);
+                products<NS, MS, MS, NT / 16>(tm + Smem::far, Operand<NT, true>(sm.tiles.q), Operand<NT, true>(sm.s),
+                                              t5::instr(p16 * 16, false, false), false);
+                t5::commit(&sm.sync.bars[1]);
+                products<kFull3, NS, kFull3, kChunk / 16>(tm + Smem::inc, Operand<kP, false>(sm.tiles.vw), Operand<NT, false>(sm.tiles.k),
+                                                          t5::instr(NT, true, true), false);
                 t5::commit(&sm.sync.bars[2]);
             }
             __syncwarp();
@@ -410,7 +411,8 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
             t5::commit(&sm.sync.bars[3]);
         }
         __syncwarp();
-        sm.sync.wait(3, phase);                               // (and with it the far part)
+        sm.sync.wait(3, phase);
+        sm.sync.wait(1, phase);
         T* const out = y + (int64_t)t * y_st;
 #pragma unroll
         for (int pb = 0; pb < kP / 16; pb += 2) {

@@ -214,16 +214,14 @@ struct Pending {
     static constexpr int words = VEC ? 2 * (int)sizeof(T) : 8;
     Word g[n][words];
 
-    __device__ __forceinline__ static int row0() { return threadIdx.x / (W / 8); }
-    __device__ __forceinline__ static int col() { return threadIdx.x % (W / 8) * 8; }
     __device__ __forceinline__ static bool mine(int i) { return all % TH == 0 || threadIdx.x + i * TH < all; }
 
     __device__ __forceinline__ void fetch(const T* src, int64_t stride, int rows, int cols) {
-        const T* p = src + row0() * stride + col();
-        const int in = cols - col();
+        const int tid = threadIdx.x, row0 = tid / (W / 8), col = tid % (W / 8) * 8, in = cols - col;
+        const T* p = src + row0 * stride + col;
 #pragma unroll
         for (int i = 0; i < n; ++i, p += step * stride) {
-            const bool here = row0() + i * step < rows;
+            const bool here = row0 + i * step < rows;
             if (VEC) {
 #pragma unroll
                 for (int u = 0; u < (int)sizeof(T) / 2; ++u) {
@@ -285,11 +283,12 @@ struct Pending {
     // M pieces of the values, or of the values times their row's weight
     template <int M, bool WEIGHTED>
     __device__ __forceinline__ void put(bf16* dst, const float* weight) const {
-        bf16* to = dst + Wide<W>::at(row0(), col());
+        const int tid = threadIdx.x, row0 = tid / (W / 8);
+        bf16* to = dst + Wide<W>::at(row0, tid % (W / 8) * 8);
 #pragma unroll
         for (int i = 0; i < n; ++i, to += step * Wide<W>::W) {
             if (!mine(i)) continue;
-            const float w = WEIGHTED ? weight[row0() + i * step] : 1.0f;
+            const float w = WEIGHTED ? weight[row0 + i * step] : 1.0f;
             uint32_t r[4][M];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -368,22 +367,23 @@ __device__ __forceinline__ void store_rows(T* out, int64_t st, int rows, int col
 }
 
 // ---------------------------------------------------------------------- state ----
-// The transposed state (64 columns of the values by NT of the keys) in the registers of four warps (which begin at a
-// multiple of four), in the accumulators' layout.
-template <int NT>
+// The transposed state (64 columns of the values by NT of the keys) in the registers of PARTS groups of four warps (which
+// begin at multiples of four; each has NT / PARTS of the keys' columns), in the accumulators' layout.
+template <int NT, int PARTS>
 struct State {
-    float s[NT / 8][4];
-
-    __device__ __forceinline__ static int p(int half) { return ((threadIdx.x >> 5) & 3) * 16 + (lane_id() >> 2) + 8 * half; }
-    __device__ __forceinline__ static int n(int c) { return 8 * c + 2 * (lane_id() & 3); }
+    static constexpr int C = NT / PARTS;
+    float s[C / 8][4];
+    int first;                   // of the group's columns
+    __device__ __forceinline__ explicit State(int part) : first(part * C) {}
 
     // calls f(value, value, p, n) for pairs of neighbouring n
     template <typename F>
     __device__ __forceinline__ void pairs(F&& f) {
+        const int tid = threadIdx.x, p = (tid >> 5 & 3) * 16 + (tid >> 2 & 7), n = first + 2 * (tid & 3);
 #pragma unroll
-        for (int c = 0; c < NT / 8; ++c)
+        for (int c = 0; c < C / 8; ++c)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) f(s[c][2 * h], s[c][2 * h + 1], p(h), n(c));
+            for (int h = 0; h < 2; ++h) f(s[c][2 * h], s[c][2 * h + 1], p + 8 * h, n + 8 * c);
     }
     __device__ __forceinline__ void zero() {
         pairs([](float& x, float& y, int, int) { x = y = 0.0f; });
@@ -417,29 +417,17 @@ struct State {
     }
     // s = whole s + the accumulator at addr (this warp's lanes)
     __device__ __forceinline__ void advance(uint32_t addr, float whole) {
-        if constexpr (NT >= 64) {
+        constexpr int many = C >= 32 ? 4 : C / 8;              // 8-column tiles a load
 #pragma unroll
-            for (int c = 0; c < NT / 8; c += 8) {
-                float x[4][4], y[4][4];
-                t5::ld32x2(x, addr + 8 * c, y, addr + 8 * c + 32);
+        for (int c = 0; c < C / 8; c += many) {
+            float x[many][4];
+            if constexpr (many == 4) t5::ld32(x, addr + first + 8 * c);
+            else if constexpr (many == 2) t5::ld16(x, addr + first + 8 * c);
+            else t5::ld8(x[0], addr + first + 8 * c);
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
+            for (int q = 0; q < many; ++q)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[c + q][e] = fmaf(whole, s[c + q][e], x[q][e]);
-                        s[c + 4 + q][e] = fmaf(whole, s[c + 4 + q][e], y[q][e]);
-                    }
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < NT / 8; c += 2) {
-                float x[2][4];
-                t5::ld16(x, addr + 8 * c);
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[c + q][e] = fmaf(whole, s[c + q][e], x[q][e]);
-            }
+                for (int e = 0; e < 4; ++e) s[c + q][e] = fmaf(whole, s[c + q][e], x[q][e]);
         }
     }
 };
@@ -478,8 +466,7 @@ struct Sync {
         t5::fence_after();
     }
     __device__ __forceinline__ void wait(int bar, uint32_t phase) {
-        if (!*(volatile int*)&failed && !t5::bar_wait(&bars[bar], phase)) *(volatile int*)&failed = 1;
-        __syncwarp();                                         // threads leave a wait at their own times
+        t5::bar_wait(&bars[bar], phase, &failed);
         t5::fence_after();
     }
     // the whole block, all products awaited
@@ -571,7 +558,7 @@ struct PartSmem {
     Sync<1> sync;
 };
 
-constexpr int kPartThreads = 128;
+constexpr int kPartThreads = 256;
 
 template <typename T, int NT, bool BACK, bool VEC>
 __global__ void __launch_bounds__(kPartThreads) part_kernel(const __grid_constant__ PartArgs p) {
@@ -589,13 +576,13 @@ __global__ void __launch_bounds__(kPartThreads) part_kernel(const __grid_constan
     const T* b = row_ptr<T>(p.b, z, it.seq, it.t0, h) + col;
     const float* g = p.g + (z.cu ? 0 : it.seq * p.g_sb) + it.t0 * p.g_st + h * p.g_sh;
     const int len = it.t1 - it.t0, nc = (len + kChunk - 1) / kChunk, l = lane_id();
-    State<NT> st;
+    State<NT, 2> st(threadIdx.x >> 7);
     st.zero();
     double all = 0.0;
     Pending<T, NT, kPartThreads, VEC> pa;
     Pending<T, kP, kPartThreads, VEC> pb;
     Logs logs{g, p.g_st};
-    const bool decay_warp = threadIdx.x < 32;
+    const bool decay_warp = threadIdx.x >= 128 && threadIdx.x < 160;
     auto start = [&](int i) { return (BACK ? nc - 1 - i : i) * kChunk; };      // of the i-th chunk of the walk
     auto fetch = [&](int i) {
         const int t = start(i), rows = min(kChunk, len - t);
@@ -635,13 +622,13 @@ __global__ void __launch_bounds__(kPartThreads) part_kernel(const __grid_constan
             logs.fetch(i + 2 < nc ? start(i + 2) : -1, len);
         }
         sm.sync.wait(0, i & 1);
-        st.advance(acc + (warp << 21), sm.d[i & 1].whole);
+        st.advance(acc + ((warp & 3) << 21), sm.d[i & 1].whole);
         t5::fence_before();
     }
     if (sm.sync.failed) st.pairs([](float& x, float& y, int, int) { x = y = __int_as_float(0x7fc00000); });
     const int64_t at = (int64_t)item * z.heads + h;
     st.store(p.parts.state + at * z.n * z.p + col, z.n, cols, z.p);
-    if (threadIdx.x == 0 && col == 0) p.parts.whole[at] = exp2f((float)all);
+    if (threadIdx.x == 128 && col == 0) p.parts.whole[at] = exp2f((float)all);
     sm.sync.end(kCols);
 }
 

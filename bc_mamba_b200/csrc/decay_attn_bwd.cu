@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
     };
     uint32_t phase = 0;
     if (group == 3) {
-        State<NT> ds;
+        State<NT, 1> ds(0);
         bool bad, bad_logs = false, pending = false;          // pending: the chunk behind has its dg still to be finished
         const float* from = it.last ? (p.dh_last ? p.dh_last + ((int64_t)it.seq * z.heads + h) * np : nullptr)
                                     : p.enter + ((int64_t)item * z.heads + h) * np;
@@ -678,11 +678,21 @@ __global__ void __launch_bounds__(256) sum_blocks_kernel(const double* x, int he
     out[h] = (float)s;
 }
 
+// float32 copies of strided float16 rows (tokens, heads, width), contiguous: a thread per element
+__global__ void __launch_bounds__(256) widen_kernel(const __grid_constant__ Rows in, int64_t batch, int64_t seqlen, int heads, int width, float* out) {
+    const int64_t n = batch * seqlen * heads * width;
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
+        const int c = (int)(e % width);
+        const int64_t r = e / width, t = r / heads, h = r % heads;
+        out[e] = in.p ? to_f32(((const __half*)in.p)[t / seqlen * in.sb + t % seqlen * in.st + h * in.sh + c]) : 0.0f;
+    }
+}
+
 // What the backward keeps beside the plan's: parts of dq and dk, of dg, and the sums of a fixed decay
 struct BwdRoom {
-    size_t dq, dk, dg, rows, sums, bytes;
+    size_t dq, dk, dg, rows, sums, wide[5], bytes;
     int shares;
-    bool fixed;
+    bool fixed, widen;
 };
 
 BwdRoom room_of(const bcm_decay_attn_args* a, const Plan& plan) {
@@ -697,13 +707,20 @@ BwdRoom room_of(const bcm_decay_attn_args* a, const Plan& plan) {
         at = align_up(at + bytes, 256);
         return here;
     };
-    if (r.shares > 1) {
+    if (r.shares > 1 || (a->dtype == BCM_F16 && z.n > 64)) {
         r.dq = take(sizeof(float) * r.shares * tokens * z.qk_heads * z.n);
         r.dk = take(sizeof(float) * r.shares * tokens * z.qk_heads * z.n);
     }
     if (z.slices > 1 || r.fixed) r.dg = take(sizeof(float) * z.slices * tokens * z.heads);
     if (z.slices > 1 && r.fixed) r.rows = take(sizeof(float) * tokens * z.heads);
     if (r.fixed) r.sums = take(sizeof(double) * kDecayBlocks * z.heads);
+    // float16 keys of more than 64 features go the way of float32: two pieces of every operand beside two whole states
+    // fill a block's shared memory, and that variant has not run reliably
+    r.widen = a->dtype == BCM_F16 && z.n > 64;
+    if (r.widen) {
+        for (int i = 0; i < 2; ++i) r.wide[i] = take(sizeof(float) * tokens * z.qk_heads * z.n);
+        for (int i = 2; i < 5; ++i) r.wide[i] = take(sizeof(float) * tokens * z.heads * z.p);
+    }
     r.bytes = at;
     return r;
 }
@@ -742,34 +759,54 @@ extern "C" bcm_status bcm_decay_attn_bwd(const bcm_decay_attn_args* a, cudaStrea
     return dispatch(a->dtype, a->dim_k, [&](auto type, auto n) -> bcm_status {
         using T = decltype(type);
         bcm_status r = BCM_OK;
-            if (plan.cut) {
-                // without dy an item's own part is 0: its rows count as none
-                PartArgs pa{plan.z, q, dy, a->log_decay, a->g_stride_b, a->g_stride_t, a->g_stride_h, parts};
-                if ((r = launch_part<T, n, true>(pa, vec, stream)) != BCM_OK) return r;
-                if ((r = join(plan, parts, a->dh_last, true, stream)) != BCM_OK) return r;
+        constexpr bool widen = std::is_same<T, __half>::value && n > 64;
+        using K = typename std::conditional<widen, float, T>::type;         // what the walk reads and writes
+        Rows in[4] = {q, k, v, dy};
+        void* dv = a->dv;
+        if constexpr (widen) {
+            const int64_t batch = z.cu ? 1 : z.batch;
+            for (int i = 0; i < 4; ++i) {
+                const int heads = i < 2 ? z.qk_heads : z.heads, width = i < 2 ? z.n : z.p;
+                if (tokens > 0) {
+                    widen_kernel<<<16 * sm_count(), 256, 0, stream>>>(in[i], batch, z.seqlen, heads, width, (float*)(ws + room.wide[i]));
+                    BCM_LAUNCH_CHECK();
+                }
+                in[i] = rows_of(ws + room.wide[i], (int64_t)z.seqlen * heads * width, (int64_t)heads * width, width);
             }
-            const BwdArgs ba{plan.z, q, k, v, dy, a->log_decay, a->g_stride_b, a->g_stride_t, a->g_stride_h, (const float*)a->ckpt,
-                             a->dh_last, parts.state, apart ? (void*)(ws + room.dq) : a->dq, apart ? (void*)(ws + room.dk) : a->dk,
-                             a->dv, dg_parts ? (float*)(ws + room.dg) : a->dlog_decay, a->dh0, room.shares};
-            if ((r = launch_bwd<T, n>(ba, vec, stream)) != BCM_OK) return r;
-            if (apart) {
-                const int64_t count = tokens * z.qk_heads * z.n;
-                if ((r = add_parts((const float*)(ws + room.dq), room.shares, count, (T*)a->dq, stream)) != BCM_OK) return r;
-                if ((r = add_parts((const float*)(ws + room.dk), room.shares, count, (T*)a->dk, stream)) != BCM_OK) return r;
-            }
-            if (!dg_parts) return BCM_OK;
-            const float* rows = (const float*)(ws + room.dg);
-            if (z.slices > 1) {
-                float* to = room.fixed ? (float*)(ws + room.rows) : a->dlog_decay;
-                if ((r = add_parts(rows, z.slices, tokens * z.heads, to, stream)) != BCM_OK) return r;
-                rows = to;
-            }
-            if (room.fixed) {
-                sum_rows_kernel<<<kDecayBlocks, 256, 0, stream>>>(rows, tokens, z.heads, (double*)(ws + room.sums));
-                BCM_LAUNCH_CHECK();
-                sum_blocks_kernel<<<ceil_div(z.heads, 256), 256, 0, stream>>>((const double*)(ws + room.sums), z.heads, a->dlog_decay);
-                BCM_LAUNCH_CHECK();
-            }
-            return BCM_OK;
+            dv = ws + room.wide[4];
+        }
+        const bool in_ws = apart || widen;
+        if (plan.cut) {
+            // without dy an item's own part is 0: its rows count as none
+            PartArgs pa{plan.z, in[0], in[3], a->log_decay, a->g_stride_b, a->g_stride_t, a->g_stride_h, parts};
+            if ((r = launch_part<K, n, true>(pa, widen ? a->dim_k % 8 == 0 && a->dim_v % 8 == 0 : vec, stream)) != BCM_OK) return r;
+            if ((r = join(plan, parts, a->dh_last, true, stream)) != BCM_OK) return r;
+        }
+        const BwdArgs ba{plan.z, in[0], in[1], in[2], in[3], a->log_decay, a->g_stride_b, a->g_stride_t, a->g_stride_h, (const float*)a->ckpt,
+                         a->dh_last, parts.state, in_ws ? (void*)(ws + room.dq) : a->dq, in_ws ? (void*)(ws + room.dk) : a->dk, dv,
+                         dg_parts ? (float*)(ws + room.dg) : a->dlog_decay, a->dh0, room.shares};
+        if ((r = launch_bwd<K, n>(ba, widen ? a->dim_k % 8 == 0 && a->dim_v % 8 == 0 : vec, stream)) != BCM_OK) return r;
+        if (in_ws) {
+            const int64_t count = tokens * z.qk_heads * z.n;
+            if ((r = add_parts((const float*)(ws + room.dq), room.shares, count, (T*)a->dq, stream)) != BCM_OK) return r;
+            if ((r = add_parts((const float*)(ws + room.dk), room.shares, count, (T*)a->dk, stream)) != BCM_OK) return r;
+        }
+        if constexpr (widen) {
+            if ((r = add_parts((const float*)dv, 1, tokens * z.heads * z.p, (T*)a->dv, stream)) != BCM_OK) return r;
+        }
+        if (!dg_parts) return BCM_OK;
+        const float* rows = (const float*)(ws + room.dg);
+        if (z.slices > 1) {
+            float* to = room.fixed ? (float*)(ws + room.rows) : a->dlog_decay;
+            if ((r = add_parts(rows, z.slices, tokens * z.heads, to, stream)) != BCM_OK) return r;
+            rows = to;
+        }
+        if (room.fixed) {
+            sum_rows_kernel<<<kDecayBlocks, 256, 0, stream>>>(rows, tokens, z.heads, (double*)(ws + room.sums));
+            BCM_LAUNCH_CHECK();
+            sum_blocks_kernel<<<ceil_div(z.heads, 256), 256, 0, stream>>>((const double*)(ws + room.sums), z.heads, a->dlog_decay);
+            BCM_LAUNCH_CHECK();
+        }
+        return BCM_OK;
     });
 }

@@ -34,7 +34,7 @@ Plan plan_of(const bcm_decay_attn_args* a, bool backward) {
     const int64_t tokens = a->seqlen;
     auto chunks_up = [](int64_t v) { return std::max<int64_t>(256, (v + kChunk - 1) / kChunk * kChunk); };
     if (!z.cu) {
-        const int64_t blocks = std::max<int64_t>(1, z.batch * across), segs = std::max<int64_t>(1, room / blocks);
+        const int64_t blocks = std::max<int64_t>(1, z.batch * across), segs = blocks * 2 > sm_count() ? 1 : room / blocks;
         z.span = (int)chunks_up((tokens + segs - 1) / segs);
         z.per_seq = std::max(1, ceil_div(tokens, z.span));
         z.items = z.batch * z.per_seq;
@@ -250,21 +250,20 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
         zero_rows((T*)p.y + (int64_t)h * z.p + col, z.tables.seq_item[z.batch + 1], z.seqlen, y_st, cols, item, z.items);
     const Item it = item_of(z, item);
     if (it.seq < 0) return;
-    const T* q = row_ptr<T>(p.q, z, it.seq, it.t0, hq);
-    const T* k = row_ptr<T>(p.k, z, it.seq, it.t0, hq);
-    const T* v = row_ptr<T>(p.v, z, it.seq, it.t0, h) + col;
+    // the rows of the item's token t
+    auto rows_of_token = [&](const Rows& r, int t, int head, int c0) { return row_ptr<T>(r, z, it.seq, it.t0 + t, head) + c0; };
     const float* g = p.g + (z.cu ? 0 : it.seq * p.g_sb) + it.t0 * p.g_st + h * p.g_sh;
-    T* y = (T*)p.y + ((z.cu ? 0 : (int64_t)it.seq * z.seqlen) + it.t0) * y_st + (int64_t)h * z.p + col;
+    auto y_of_token = [&](int t) { return (T*)p.y + ((z.cu ? 0 : (int64_t)it.seq * z.seqlen) + it.t0 + t) * y_st + (int64_t)h * z.p + col; };
     const int np = z.n * z.p;
     const int len = it.t1 - it.t0, nc = (len + kChunk - 1) / kChunk;
-    const int warp = t5::warp_id(), l = lane_id(), w = warp & 3, row = w * 16 + (l >> 2);
+    const int warp = t5::warp_id(), w = warp & 3;
     const bool state_warp = warp >= 4, decay_warp = warp == 5;
     const int p16 = (cols + 15) / 16;
 
     Pending<T, NT, kFwdThreads, VEC> pq, pk;
     Pending<T, kP, kFwdThreads, VEC> pv;
     Logs logs{g, p.g_st};
-    State<NT> st;                                             // (warps 4 to 7)
+    State<NT, 1> st(0);                                       // (warps 4 to 7)
     bool bad = false, bad_logs = false;
     sm.sync.init(Smem::cols);
     const uint32_t tm = __shfl_sync(kFull, sm.sync.tmem, 0), lanes = (uint32_t)w << 21;
@@ -322,9 +321,9 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
         }
         if (c + 1 < nc) {
             const int t2 = t + kChunk, r2 = min(kChunk, len - t2);
-            pq.fetch(q + t2 * p.q.st, p.q.st, r2, z.n);
-            pk.fetch(k + t2 * p.k.st, p.k.st, r2, z.n);
-            pv.fetch(v + t2 * p.v.st, p.v.st, r2, cols);
+            pq.fetch(rows_of_token(p.q, t2, hq, 0), p.q.st, r2, z.n);
+            pk.fetch(rows_of_token(p.k, t2, hq, 0), p.k.st, r2, z.n);
+            pv.fetch(rows_of_token(p.v, t2, h, col), p.v.st, r2, cols);
         }
         if (c < 0) continue;
         if (slow) {
@@ -336,7 +335,8 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
                     f[(n + 1) * kP + pp] = x1;
                 });
             __syncthreads();
-            walk_tokens<T>(p, q + t * p.q.st, k + t * p.k.st, v + t * p.v.st, g + t * p.g_st, y + t * y_st, rows, cols, f, f + NT * kP);
+            walk_tokens<T>(p, rows_of_token(p.q, t, hq, 0), rows_of_token(p.k, t, hq, 0), rows_of_token(p.v, t, h, col), g + t * p.g_st, y_of_token(t),
+                           rows, cols, f, f + NT * kP);
             if (state_warp) {
                 st.pairs([&](float& x, float& x1, int pp, int n) {
                     x = f[n * kP + pp];
@@ -363,6 +363,7 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
         }
         if (slow) continue;
         const Decays& d = sm.d[c & 1];
+        const int l = lane_id(), row = w * 16 + (l >> 2);
         const float hi0 = d.hi[row], lo0 = d.lo[row], hi1 = d.hi[row + 8], lo1 = d.lo[row + 8], since0 = d.since[row], since1 = d.since[row + 8];
         sm.sync.wait(0, phase);
         float sc[4][2][4];
@@ -413,23 +414,22 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
         __syncwarp();
         sm.sync.wait(3, phase);
         sm.sync.wait(1, phase);
-        T* const out = y + (int64_t)t * y_st;
+        T* const out = y_of_token(t);
 #pragma unroll
-        for (int pb = 0; pb < kP / 16; pb += 2) {
+        for (int pb = 0; pb < kP / 16; ++pb) {
             if (pb >= p16) break;
-            float x[4][4];
+            float x[2][4];
             if constexpr (Smem::apart) {
-                float f[4][4];
-                t5::ld32x2(x, tm + Smem::near + lanes + 16 * pb, f, tm + Smem::far + lanes + 16 * pb);
+                float f[2][4];
+                t5::ld16x2(x, tm + Smem::near + lanes + 16 * pb, f, tm + Smem::far + lanes + 16 * pb);
 #pragma unroll
-                for (int q2 = 0; q2 < 4; ++q2)
+                for (int q2 = 0; q2 < 2; ++q2)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[q2][e] = fmaf(e < 2 ? since0 : since1, f[q2][e], x[q2][e]);
             } else {
-                t5::ld16x2((float(&)[2][4])x[0], tm + Smem::near + lanes + 16 * pb, (float(&)[2][4])x[2], tm + Smem::near + lanes + 16 * pb + 16);
+                t5::ld16(x, tm + Smem::near + lanes + 16 * pb);
             }
             store_rows<VEC>(out, y_st, rows, cols, row, 16 * pb, x[0], x[1]);
-            store_rows<VEC>(out, y_st, rows, cols, row, 16 * pb + 16, x[2], x[3]);
         }
         t5::fence_before();
         phase ^= 1;

@@ -65,18 +65,35 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
 __device__ __forceinline__ void bar_init(uint64_t* bar, int count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
 }
-// waits for the phase; after 2^31 cycles (about a second; products of a tile take microseconds) it gives up and says so
-__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t phase) {
-    const long long start = clock64();
-    do {
-        uint32_t done;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}"
-                     : "=r"(done)
-                     : "r"(smem_u32(bar)), "r"(phase)
-                     : "memory");
-        if (done) return true;
-    } while (clock64() - start < (1LL << 31));
-    return false;
+// Waits for the phase, a warp as one (its threads leave together: what follows moves all their registers to or from tensor
+// memory).  After 2^31 cycles (about a second; products of a tile take microseconds) it gives up and sets *failed, and
+// where that is set it does not wait.
+__device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t phase, int* failed) {
+    __syncwarp();
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        ".reg .b32 f;\n\t"
+        ".reg .b64 t, s;\n\t"
+        "ld.volatile.shared.b32 f, [%2];\n\t"
+        "setp.ne.b32 p, f, 0;\n\t"
+        "vote.sync.any.pred p, p, 0xffffffff;\n\t"
+        "@p bra.uni DONE;\n\t"
+        "mov.u64 s, %%clock64;\n"
+        "AGAIN:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1;\n\t"
+        "vote.sync.all.pred p, p, 0xffffffff;\n\t"
+        "@p bra.uni DONE;\n\t"
+        "mov.u64 t, %%clock64;\n\t"
+        "sub.u64 t, t, s;\n\t"
+        "setp.lt.u64 p, t, 0x80000000;\n\t"
+        "vote.sync.any.pred p, p, 0xffffffff;\n\t"
+        "@p bra.uni AGAIN;\n\t"
+        "st.volatile.shared.b32 [%2], 1;\n"
+        "DONE:\n\t"
+        "}" ::"r"(smem_u32(bar)), "r"(phase), "r"(smem_u32(failed))
+        : "memory");
+    __syncwarp();
 }
 
 // one thread of a warp (all of it, together), known to the compiler to be one: what it computes alike for the whole warp
@@ -111,11 +128,36 @@ __device__ __forceinline__ void ld16(float (&r)[2][4], uint32_t addr) {
     uint32_t x[8];
     __syncwarp();
     asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
-                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7])
+                 : "=&r"(x[0]), "=&r"(x[1]), "=&r"(x[2]), "=&r"(x[3]), "=&r"(x[4]), "=&r"(x[5]), "=&r"(x[6]), "=&r"(x[7])
                  : "r"(addr)
                  : "memory");
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i >> 2][i & 3] = __uint_as_float(x[i]);
+}
+// 16 rows x 8 columns
+__device__ __forceinline__ void ld8(float (&r)[4], uint32_t addr) {
+    uint32_t x[4];
+    __syncwarp();
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=&r"(x[0]), "=&r"(x[1]), "=&r"(x[2]), "=&r"(x[3])
+                 : "r"(addr)
+                 : "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __uint_as_float(x[i]);
+}
+// 32 columns
+__device__ __forceinline__ void ld32(float (&r)[4][4], uint32_t addr) {
+    uint32_t x[16];
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=&r"(x[0]), "=&r"(x[1]), "=&r"(x[2]), "=&r"(x[3]), "=&r"(x[4]), "=&r"(x[5]), "=&r"(x[6]), "=&r"(x[7]), "=&r"(x[8]), "=&r"(x[9]), "=&r"(x[10]),
+          "=&r"(x[11]), "=&r"(x[12]), "=&r"(x[13]), "=&r"(x[14]), "=&r"(x[15])
+        : "r"(addr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[i >> 2][i & 3] = __uint_as_float(x[i]);
 }
 // 16 columns at each of two addresses
 __device__ __forceinline__ void ld16x2(float (&r)[2][4], uint32_t addr, float (&r2)[2][4], uint32_t addr2) {
@@ -125,8 +167,8 @@ __device__ __forceinline__ void ld16x2(float (&r)[2][4], uint32_t addr, float (&
         "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%16];\n\t"
         "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%17];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]),
-          "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15])
+        : "=&r"(x[0]), "=&r"(x[1]), "=&r"(x[2]), "=&r"(x[3]), "=&r"(x[4]), "=&r"(x[5]), "=&r"(x[6]), "=&r"(x[7]), "=&r"(x[8]), "=&r"(x[9]), "=&r"(x[10]),
+          "=&r"(x[11]), "=&r"(x[12]), "=&r"(x[13]), "=&r"(x[14]), "=&r"(x[15])
         : "r"(addr), "r"(addr2)
         : "memory");
 #pragma unroll
@@ -135,27 +177,6 @@ __device__ __forceinline__ void ld16x2(float (&r)[2][4], uint32_t addr, float (&
         r2[i >> 2][i & 3] = __uint_as_float(x[8 + i]);
     }
 }
-// 32 columns at each of two addresses
-__device__ __forceinline__ void ld32x2(float (&r)[4][4], uint32_t addr, float (&r2)[4][4], uint32_t addr2) {
-    uint32_t x[32];
-    __syncwarp();
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
-        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]),
-          "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15]), "=r"(x[16]), "=r"(x[17]), "=r"(x[18]), "=r"(x[19]), "=r"(x[20]),
-          "=r"(x[21]), "=r"(x[22]), "=r"(x[23]), "=r"(x[24]), "=r"(x[25]), "=r"(x[26]), "=r"(x[27]), "=r"(x[28]), "=r"(x[29]), "=r"(x[30]),
-          "=r"(x[31])
-        : "r"(addr), "r"(addr2)
-        : "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        r[i >> 2][i & 3] = __uint_as_float(x[i]);
-        r2[i >> 2][i & 3] = __uint_as_float(x[16 + i]);
-    }
-}
-
 // 16 rows x 16 bf16 columns of an A operand (8 columns of 32 bits), in the accumulators' layout: r[2 q + half] the pair
 // of columns 8 q + 2 (l % 4), half: row l / 4 + 8
 __device__ __forceinline__ void st16(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {

@@ -12,7 +12,7 @@ bcm_status check(const bcm_decay_attn_args* a, const char* what) {
     BCM_REQUIRE(a->dim_k <= BCM_DECAY_ATTN_MAX_DIM_K, "%s: a query of more than %d features", what, BCM_DECAY_ATTN_MAX_DIM_K);
     BCM_REQUIRE(a->heads % a->qk_heads == 0, "%s: heads must be a multiple of the queries' heads", what);
     BCM_REQUIRE(a->dim_v <= (1 << 20) && a->heads <= (1 << 20) && a->batch < (1 << 24) && a->seqlen < INT32_MAX - 4096, "%s: sizes too large", what);
-    BCM_REQUIRE(a->batch == 0 || a->heads * a->dim_v <= (1 << 24), "%s: sizes too large", what);
+    BCM_REQUIRE(a->heads * a->dim_v <= (1 << 24) && a->batch * (a->seqlen / kChunk + 1) < INT32_MAX, "%s: sizes too large", what);
     return BCM_OK;
 }
 

@@ -1,15 +1,20 @@
-"""A small language model on the gated linear recurrence, trained by
-distillation from a teacher's top logits and sampled token by token.
+"""Small language models on the linear mixers, trained by distillation from a
+teacher's top logits and sampled token by token.
 
-    python -m bc_mamba_b200.recurrent_lm            # needs a CUDA device
+    python -m bc_mamba_b200.recurrent_lm [--attention]      # needs a CUDA device
 
-A layer maps the residual stream to values and two gates (one projection),
-mixes over time with ``interface.gated_recurrence`` and adds the projected
-output back.  ``distill_step`` is one training step on packed documents,
-``generate`` a prefill of prompts of one length followed by decode steps whose
-state is the recurrence's (batch, dim) per layer.
+``RecurrentLM``: a layer maps the residual stream to values and two gates (one
+projection), mixes over time with ``interface.gated_recurrence`` and adds the
+projected output back.  ``AttentionLM``: a layer mixes with
+``interface.decay_attention``, whose output passes ``gated_norm`` by heads, and
+``add_norm`` joins its scaled residual addition with the next layer's norm.
+``distill_step`` is one training step on packed documents, ``generate`` a
+prefill of prompts of one length followed by decode steps whose state is the
+mixer's, (batch, dim) or (batch, heads, features, features) per layer.
 """
 from __future__ import annotations
+
+import sys
 
 import torch
 import torch.nn.functional as F
@@ -58,6 +63,61 @@ class RecurrentLM:
         return F.linear(F.rms_norm(v, v.shape[-1:]), self.head)
 
 
+class AttentionLM(RecurrentLM):
+    """The same interface on linear attention with a decay for each head.  Queries and keys of `features` are shared by
+    all `heads` heads of values, dim / heads features each; the residual stream is float32."""
+
+    def __init__(self, vocab: int, d_model: int, dim: int, layers: int, device, dtype=torch.bfloat16, seed: int = 0, heads: int = 4,
+                 features: int = 16):
+        assert dim % heads == 0, "dim must be a multiple of heads"
+        super().__init__(vocab, d_model, dim, 0, device, dtype, seed)
+        g = torch.Generator().manual_seed(seed + 1)
+        rn = lambda *s, scale: (scale * torch.randn(*s, generator=g)).to(device=device, dtype=dtype).requires_grad_(True)
+        one = lambda n, value=1.0: torch.full((n,), value, device=device).requires_grad_(True)
+        self.heads, self.features = heads, features
+        self.norm = one(d_model)
+        for _ in range(layers):
+            # rates of 1 to 16 by heads, steps of about 0.01 at a projection of zero
+            rate = torch.log(torch.linspace(1, 16, heads)).to(device).requires_grad_(True)
+            self.layers.append(dict(w_in=rn(2 * dim + 2 * features + heads, d_model, scale=d_model ** -0.5), rate=rate,
+                                    step=one(heads, -4.6), out_norm=one(dim), w_out=rn(d_model, dim, scale=dim ** -0.5),
+                                    scale=one(d_model), norm=one(d_model)))
+
+    def parameters(self):
+        return super().parameters() + [self.norm]
+
+    def _parts(self, layer, x):
+        """Queries, keys (.., 1, features), values (.., heads, dim / heads), gate and the decays' logarithms (.., heads)."""
+        v, gate, q, k, step = F.linear(x, layer["w_in"]).split([self.dim, self.dim, self.features, self.features, self.heads], -1)
+        log_decay = -layer["rate"].exp() * F.softplus(step.float() + layer["step"])
+        q = q * self.features ** -0.5
+        return q.unsqueeze(-2), k.unsqueeze(-2), v.unflatten(-1, (self.heads, -1)), gate, log_decay
+
+    def _run(self, tokens, mix):
+        """Embedding, layers and head; mix(n, q, k, v, log_decay) is the n-th mixer."""
+        v = F.embedding(tokens, self.embed).float()
+        x = (F.rms_norm(v, v.shape[-1:], eps=1e-6) * self.norm).to(self.embed.dtype)
+        for n, layer in enumerate(self.layers):
+            q, k, values, gate, log_decay = self._parts(layer, x)
+            y = itf.gated_norm(mix(n, q, k, values, log_decay).flatten(-2), gate, layer["out_norm"], groups=self.heads)
+            v, x = itf.add_norm(v, F.linear(y, layer["w_out"]), layer["norm"], scale=layer["scale"])
+        return F.linear(x, self.head)
+
+    def logits(self, tokens, cu_seqlens=None, states=None):
+        out = []
+
+        def mix(n, q, k, v, log_decay):
+            y, h = itf.decay_attention(q, k, v, log_decay, h0=None if states is None else states[n], cu_seqlens=cu_seqlens)
+            out.append(h)
+            return y
+
+        return self._run(tokens, mix), out
+
+    @torch.no_grad()
+    def step_logits(self, tokens, states):
+        return self._run(tokens, lambda n, q, k, v, log_decay: itf.decay_attention_step(q, k, v, log_decay, states[n]))
+
+
 def distill_step(model: RecurrentLM, optimizer, tokens, cu_seqlens, teacher_logits, teacher_ids, weight, temperature: float = 2.0):
     """One training step on packed documents (T,): the teacher's K top logits and ids per token, weight (T,) with 0
     for padding (all of it: loss and gradients are 0).  The head's gradient comes from the one-call form of the loss.
@@ -88,11 +148,11 @@ def generate(model: RecurrentLM, prompts, u, **settings):
     return torch.stack(tokens, 1), torch.stack(logps, 1)
 
 
-def main(steps: int = 60) -> None:
+def main(steps: int = 60, model=RecurrentLM) -> None:
     """Distils a random teacher with the student's own architecture, then samples from the student."""
     dev, vocab, k = "cuda", 1000, 16
-    teacher = RecurrentLM(vocab, 64, 128, 2, dev, torch.float32, seed=1)
-    student = RecurrentLM(vocab, 64, 128, 2, dev, torch.float32, seed=2)
+    teacher = model(vocab, 64, 128, 2, dev, torch.float32, seed=1)
+    student = model(vocab, 64, 128, 2, dev, torch.float32, seed=2)
     opt = torch.optim.AdamW(student.parameters(), lr=3e-3)
     g = torch.Generator(device=dev).manual_seed(0)
     cu = torch.tensor([0, 300, 301, 301, 1024], dtype=torch.int32, device=dev)
@@ -109,4 +169,4 @@ def main(steps: int = 60) -> None:
 
 
 if __name__ == "__main__":
-    main()
+    main(model=AttentionLM if "--attention" in sys.argv[1:] else RecurrentLM)

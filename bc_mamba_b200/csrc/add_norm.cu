@@ -21,64 +21,81 @@ struct AddArgs {
     float *dw, *ds;                                 // [blocks][dim]
 };
 
+constexpr int kAddFwdPerSm = 1024, kAddBwdPerSm = 512;     // threads that fit with the registers they need
+
+// In both directions the next row's operands are on their way while this one's are used.  Backward the weight is read
+// again for each row, which spilled otherwise.
 template <typename R, typename T, typename G>
-__global__ void __launch_bounds__(G::threads) add_fwd_kernel(const __grid_constant__ AddArgs p) {
+__global__ void __launch_bounds__(G::threads, resident(G::threads, kAddFwdPerSm)) add_fwd_kernel(const __grid_constant__ AddArgs p) {
     __shared__ float room[2][32][2];
     int turn = 0;
-    for (int64_t base = (int64_t)blockIdx.x * G::teams; base < p.rows; base += (int64_t)gridDim.x * G::teams, turn ^= 1) {
+    float w[G::n], s[G::n];
+    typename G::template Raw<R> next_res;
+    typename G::template Raw<T> next_branch;
+    auto fetch = [&](int64_t row) {
+        const int in = row < p.rows ? p.dim : 0;
+        G::fetch((const R*)p.res + row * p.res_st, in, next_res);
+        G::fetch((const T*)p.branch + row * p.branch_st, in, next_branch);
+    };
+    const int64_t across = (int64_t)gridDim.x * G::teams;
+    fetch((int64_t)blockIdx.x * G::teams + G::id());
+    G::load(p.weight, p.dim, w);
+    if (p.scale) G::load(p.scale, p.dim, s);
+    for (int64_t base = (int64_t)blockIdx.x * G::teams; base < p.rows; base += across, turn ^= 1) {
         const int64_t row = base + G::id();
         const bool live = row < p.rows;
-        const int in = live ? p.dim : 0;
         float v[G::n], b[G::n];
-        G::load((const R*)p.res + row * p.res_st, in, v);
-        G::load((const T*)p.branch + row * p.branch_st, in, b);
-        if (p.scale) {
-            float s[G::n];
-            G::load(p.scale, p.dim, s);
+        G::values(next_res, v);
+        G::values(next_branch, b);
+        fetch(row + across);
 #pragma unroll
-            for (int j = 0; j < G::n; ++j) v[j] = fmaf(s[j], b[j], v[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < G::n; ++j) v[j] += b[j];
-        }
+        for (int j = 0; j < G::n; ++j) v[j] = p.scale ? fmaf(s[j], b[j], v[j]) : v[j] + b[j];
         if (live) G::store((R*)p.res_out + row * p.dim, p.dim, v);
         float sq = 0.0f, none = 0.0f;
 #pragma unroll
         for (int j = 0; j < G::n; ++j) sq = fmaf(v[j], v[j], sq);
-        G::load(p.weight, p.dim, b);
         G::sum(sq, none, room, turn);
         const float r = rsqrtf(sq / p.dim + p.eps);
 #pragma unroll
-        for (int j = 0; j < G::n; ++j) v[j] *= r * b[j];
+        for (int j = 0; j < G::n; ++j) v[j] *= r * w[j];
         if (live) G::store((T*)p.out + row * p.dim, p.dim, v);
     }
 }
 
 template <typename R, typename T, typename G, bool SCALED>
-__global__ void __launch_bounds__(G::threads) add_bwd_kernel(const __grid_constant__ AddArgs p) {
+__global__ void __launch_bounds__(G::threads, resident(G::threads, kAddBwdPerSm)) add_bwd_kernel(const __grid_constant__ AddArgs p) {
     extern __shared__ float cols_room[];
     __shared__ float room[2][32][2];
-    float dw[G::n] = {}, ds[SCALED ? G::n : 1] = {};
+    float dw[G::n] = {}, ds[SCALED ? G::n : 1] = {}, s[SCALED ? G::n : 1];
     int turn = 0;
-    for (int64_t base = (int64_t)blockIdx.x * G::teams; base < p.rows; base += (int64_t)gridDim.x * G::teams, turn ^= 1) {
+    typename G::template Raw<R> next_res, next_dres;
+    typename G::template Raw<T> next_branch, next_dout;
+    auto fetch = [&](int64_t row) {
+        const int in = row < p.rows ? p.dim : 0;
+        G::fetch((const R*)p.res + row * p.res_st, in, next_res);
+        G::fetch((const T*)p.branch + row * p.branch_st, in, next_branch);
+        G::fetch((const T*)p.dout + row * p.dout_st, p.dout ? in : 0, next_dout);
+        G::fetch((const R*)p.dres + row * p.dres_st, p.dres ? in : 0, next_dres);
+    };
+    const int64_t across = (int64_t)gridDim.x * G::teams;
+    if (G::ahead_back) fetch((int64_t)blockIdx.x * G::teams + G::id());
+    if constexpr (SCALED) G::load(p.scale, p.dim, s);
+    for (int64_t base = (int64_t)blockIdx.x * G::teams; base < p.rows; base += across, turn ^= 1) {
         const int64_t row = base + G::id();
         const bool live = row < p.rows;
-        const int in = live ? p.dim : 0;
-        float v[G::n], b[G::n], d[G::n], dv[G::n], s[SCALED ? G::n : 1];
-        G::load((const R*)p.res + row * p.res_st, in, v);
-        G::load((const T*)p.branch + row * p.branch_st, in, b);
-        G::load((const T*)p.dout + row * p.dout_st, p.dout ? in : 0, d);
-        G::load((const R*)p.dres + row * p.dres_st, p.dres ? in : 0, dv);
-        if constexpr (SCALED) {
-            G::load(p.scale, p.dim, s);
-#pragma unroll
-            for (int j = 0; j < G::n; ++j) v[j] = fmaf(s[j], b[j], v[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < G::n; ++j) v[j] += b[j];
-        }
-        float w[G::n];
+        float v[G::n], b[G::n], d[G::n], dv[G::n], w[G::n];
+        if (!G::ahead_back) fetch(row);
+        G::values(next_res, v);
+        G::values(next_branch, b);
+        G::values(next_dout, d);
+        G::values(next_dres, dv);
+        if (G::ahead_back) fetch(row + across);
         G::load(p.weight, p.dim, w);
+#pragma unroll
+        for (int j = 0; j < G::n; ++j) {
+            if constexpr (SCALED) v[j] = fmaf(s[j], b[j], v[j]);
+            else v[j] += b[j];
+        }
         float sq = 0.0f, dot = 0.0f;
 #pragma unroll
         for (int j = 0; j < G::n; ++j) {
@@ -155,7 +172,7 @@ extern "C" bcm_status bcm_add_norm_fwd(const bcm_add_norm_args* a, cudaStream_t 
                      on_16(p.scale, 0) && on_16(p.res_out, 0) && on_16(p.out, 0);
     return row_norm::dispatch(a, vec, [&](auto r, auto t, auto team) -> bcm_status {
         using G = decltype(team);
-        add_fwd_kernel<decltype(r), decltype(t), G><<<(unsigned)row_blocks(a->rows, 1, G::teams, G::threads), G::threads, 0, stream>>>(p);
+        add_fwd_kernel<decltype(r), decltype(t), G><<<(unsigned)row_blocks(a->rows, 1, G::teams, G::threads, kAddFwdPerSm), G::threads, 0, stream>>>(p);
         BCM_LAUNCH_CHECK();
         return BCM_OK;
     });
@@ -163,7 +180,7 @@ extern "C" bcm_status bcm_add_norm_fwd(const bcm_add_norm_args* a, cudaStream_t 
 
 extern "C" size_t bcm_add_norm_bwd_workspace_bytes(const bcm_add_norm_args* a) {
     if (check(a, "add_norm") != BCM_OK) return 0;
-    return (a->scale ? 2 : 1) * sizeof(float) * (size_t)most_row_blocks(1, 256) * a->dim;
+    return (a->scale ? 2 : 1) * sizeof(float) * (size_t)most_row_blocks(1, 256, kAddBwdPerSm) * a->dim;
 }
 
 extern "C" bcm_status bcm_add_norm_bwd(const bcm_add_norm_args* a, cudaStream_t stream) {
@@ -182,7 +199,7 @@ extern "C" bcm_status bcm_add_norm_bwd(const bcm_add_norm_args* a, cudaStream_t 
     int64_t blocks = 0;
     st = row_norm::dispatch(a, vec, [&](auto r, auto t, auto team) -> bcm_status {
         using G = decltype(team);
-        blocks = row_blocks(a->rows, 1, G::teams, G::threads);
+        blocks = row_blocks(a->rows, 1, G::teams, G::threads, kAddBwdPerSm);
         p.ds = p.dw + blocks * a->dim;
         const size_t smem = G::teams > 1 ? sizeof(float) * G::teams * a->dim : 0;
         if (p.scale) add_bwd_kernel<decltype(r), decltype(t), G, true><<<(unsigned)blocks, G::threads, smem, stream>>>(p);
@@ -191,11 +208,7 @@ extern "C" bcm_status bcm_add_norm_bwd(const bcm_add_norm_args* a, cudaStream_t 
         return BCM_OK;
     });
     if (st != BCM_OK) return st;
-    add_blocks_kernel<<<ceil_div(a->dim, 32), 256, 0, stream>>>(p.dw, (int)blocks, a->dim, a->dweight);
+    add_blocks_kernel<<<dim3(ceil_div(a->dim, 32), p.scale ? 2 : 1), 1024, 0, stream>>>(p.dw, (int)blocks, a->dim, a->dweight, a->dscale);
     BCM_LAUNCH_CHECK();
-    if (p.scale) {
-        add_blocks_kernel<<<ceil_div(a->dim, 32), 256, 0, stream>>>(p.ds, (int)blocks, a->dim, a->dscale);
-        BCM_LAUNCH_CHECK();
-    }
     return BCM_OK;
 }

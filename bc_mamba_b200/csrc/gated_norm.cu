@@ -21,29 +21,47 @@ struct GatedArgs {
 
 // silu(z) and its slope
 __device__ __forceinline__ float silu(float z, float& slope) {
-    const float s = 1.0f / (1.0f + expf(-z));
+    const float s = __fdividef(1.0f, 1.0f + expf(-z));       // 2 units in the last place; an infinite divisor gives 0
     slope = s * (1.0f + z * (1.0f - s));
     return z * s;
 }
 
+template <bool BACK>
+constexpr int kGatedPerSm = BACK ? 768 : 1024;              // threads that fit with the registers they need
+
+// The next row's operands are on their way while this one's are used.  The weight stays in registers forward; backward
+// it is read again for each row, which spilled otherwise.
 template <typename T, typename G, bool BACK>
-__global__ void __launch_bounds__(G::threads) gated_kernel(const __grid_constant__ GatedArgs p) {
+__global__ void __launch_bounds__(G::threads, resident(G::threads, kGatedPerSm<BACK>)) gated_kernel(const __grid_constant__ GatedArgs p) {
     extern __shared__ float cols_room[];
     __shared__ float room[2][32][2];
     const int group = blockIdx.x % p.groups, width = p.width;
     const int64_t block = blockIdx.x / p.groups, blocks = gridDim.x / p.groups, dim = (int64_t)p.groups * width;
     const int64_t at = (int64_t)group * width;
-    float dw[G::n] = {};
+    float dw[G::n] = {}, weight[G::n];
     int turn = 0;
+    typename G::template Raw<T> next[BACK ? 3 : 2];
+    auto fetch = [&](int64_t row) {
+        const int in = row < p.rows ? width : 0;
+        G::fetch((const T*)p.x + row * p.x_st + at, in, next[0]);
+        G::fetch((const T*)p.gate + row * p.gate_st + at, in, next[1]);
+        if constexpr (BACK) G::fetch((const T*)p.dout + row * p.dout_st + at, in, next[2]);
+    };
+    constexpr bool ahead = !BACK || G::ahead_back;
+    if (ahead) fetch(block * G::teams + G::id());
+    if (!BACK) G::load(p.weight + at, width, weight);
     for (int64_t base = block * G::teams; base < p.rows; base += blocks * G::teams, turn ^= 1) {
         const int64_t row = base + G::id();
         const bool live = row < p.rows;
         float x[G::n], z[G::n], d[G::n], w[G::n];
-        const int in = live ? width : 0;
-        G::load((const T*)p.x + row * p.x_st + at, in, x);
-        G::load((const T*)p.gate + row * p.gate_st + at, in, z);
-        if (BACK) G::load((const T*)p.dout + row * p.dout_st + at, in, d);
-        G::load(p.weight + at, width, w);
+        if (!ahead) fetch(row);
+        G::values(next[0], x);
+        G::values(next[1], z);
+        if constexpr (BACK) G::values(next[2], d);
+        if (ahead) fetch(row + blocks * G::teams);
+        if (BACK) G::load(p.weight + at, width, weight);
+#pragma unroll
+        for (int j = 0; j < G::n; ++j) w[j] = weight[j];
         float sq = 0.0f, dot = 0.0f;
 #pragma unroll
         for (int j = 0; j < G::n; ++j) {
@@ -106,7 +124,7 @@ bcm_status run(const bcm_gated_norm_args* a, cudaStream_t stream) {
         using T = decltype(type);
         auto go = [&](auto team) -> bcm_status {
             using G = decltype(team);
-            blocks = row_blocks(a->rows, a->groups, G::teams, G::threads);
+            blocks = row_blocks(a->rows, a->groups, G::teams, G::threads, kGatedPerSm<BACK>);
             const size_t smem = BACK && G::teams > 1 ? sizeof(float) * G::teams * p.width : 0;
             gated_kernel<T, G, BACK><<<(unsigned)(blocks * a->groups), G::threads, smem, stream>>>(p);
             BCM_LAUNCH_CHECK();
@@ -115,7 +133,7 @@ bcm_status run(const bcm_gated_norm_args* a, cudaStream_t stream) {
         return vec ? by_width<true>(p.width, go) : by_width<false>(p.width, go);
     });
     if (!BACK || st != BCM_OK) return st;
-    add_blocks_kernel<<<ceil_div(a->dim, 32), 256, 0, stream>>>(p.dw, (int)blocks, a->dim, a->dweight);
+    add_blocks_kernel<<<ceil_div(a->dim, 32), 1024, 0, stream>>>(p.dw, (int)blocks, a->dim, a->dweight, nullptr);
     BCM_LAUNCH_CHECK();
     return BCM_OK;
 }
@@ -136,7 +154,7 @@ extern "C" bcm_status bcm_gated_norm_fwd(const bcm_gated_norm_args* a, cudaStrea
 
 extern "C" size_t bcm_gated_norm_bwd_workspace_bytes(const bcm_gated_norm_args* a) {
     if (check(a, "gated_norm") != BCM_OK) return 0;
-    return sizeof(float) * (size_t)most_row_blocks(a->groups, 256) * a->dim;
+    return sizeof(float) * (size_t)most_row_blocks(a->groups, 256, kGatedPerSm<true>) * a->dim;
 }
 
 extern "C" bcm_status bcm_gated_norm_bwd(const bcm_gated_norm_args* a, cudaStream_t stream) {

@@ -19,29 +19,39 @@ namespace row_norm {
 template <int T, bool VEC>
 struct Team {
     static constexpr int n = 8, threads = T > 256 ? T : 256, teams = threads / T;
+    // a backward pass with 64 registers a thread has none to hold the next row
+    static constexpr bool ahead_back = T < 1024;
 
     __device__ __forceinline__ static int lane() { return threadIdx.x % T; }
     __device__ __forceinline__ static int id() { return threadIdx.x / T; }
     __device__ __forceinline__ static int col(int j) { return VEC ? lane() * 8 + j : j * T + lane(); }
 
+    // a thread's elements of a row as they lie in memory, 0 behind `width`; values() makes numbers of them
     template <typename E>
-    __device__ __forceinline__ static void load(const E* row, int width, float (&x)[n]) {
-        if (VEC) {
-            struct alignas(16) Eight { E v[8]; } raw;
+    struct Raw {
+        typename std::conditional<VEC, uint4[sizeof(E) / 2], E[8]>::type v;
+    };
+    template <typename E>
+    __device__ __forceinline__ static void fetch(const E* row, int width, Raw<E>& raw) {
+        if constexpr (VEC) {
             const int c = lane() * 8;
-            if (c < width) {
 #pragma unroll
-                for (int q = 0; q < (int)sizeof(E) / 2; ++q) ((uint4*)&raw)[q] = ((const uint4*)(row + c))[q];
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = c < width ? to_f32(raw.v[e]) : 0.0f;
+            for (int q = 0; q < (int)sizeof(E) / 2; ++q) raw.v[q] = c < width ? ((const uint4*)(row + c))[q] : make_uint4(0, 0, 0, 0);
         } else {
 #pragma unroll
-            for (int j = 0; j < n; ++j) {
-                const int c = j * T + lane();
-                x[j] = c < width ? to_f32(row[c]) : 0.0f;
-            }
+            for (int j = 0; j < n; ++j) raw.v[j] = j * T + lane() < width ? row[j * T + lane()] : from_f32<E>(0.0f);
         }
+    }
+    template <typename E>
+    __device__ __forceinline__ static void values(const Raw<E>& raw, float (&x)[n]) {
+#pragma unroll
+        for (int e = 0; e < n; ++e) x[e] = to_f32(((const E*)raw.v)[e]);
+    }
+    template <typename E>
+    __device__ __forceinline__ static void load(const E* row, int width, float (&x)[n]) {
+        Raw<E> raw;
+        fetch(row, width, raw);
+        values(raw, x);
     }
     template <typename E>
     __device__ __forceinline__ static void store(E* row, int width, const float (&x)[n]) {
@@ -116,29 +126,36 @@ bcm_status by_width(int64_t width, F&& f) {
 }
 constexpr int64_t kMostWidth = 8192;
 
-// Blocks for rows of `groups` norms each (a block keeps to one group of columns): about as many as stay resident.
-constexpr int kThreadsPerSm = 1536;
-inline int64_t most_row_blocks(int64_t groups, int threads) {
-    return std::max<int64_t>(1, (int64_t)sm_count() * std::max(1, kThreadsPerSm / threads) / groups);
+// Blocks for rows of `groups` norms each (a block keeps to one group of columns): as many as are resident at once with
+// `per_sm` threads on an SM, which the kernels' launch bounds hold to.  More blocks than that ran as one and a half waves
+// (the gated norm of 512000 x 256 bf16 took 237 us forward).
+constexpr int resident(int threads, int per_sm) { return per_sm > threads ? per_sm / threads : 1; }
+inline int64_t most_row_blocks(int64_t groups, int threads, int per_sm) {
+    return std::max<int64_t>(1, (int64_t)sm_count() * resident(threads, per_sm) / groups);
 }
-inline int64_t row_blocks(int64_t rows, int64_t groups, int teams, int threads) {
-    return std::max<int64_t>(1, std::min((rows + teams - 1) / teams, most_row_blocks(groups, threads)));
+inline int64_t row_blocks(int64_t rows, int64_t groups, int teams, int threads, int per_sm) {
+    return std::max<int64_t>(1, std::min((rows + teams - 1) / teams, most_row_blocks(groups, threads, per_sm)));
 }
 
-// out[c] = sum of part[b][c] over the blocks in their order: 32 columns a block, 8 rows of threads
-static __global__ void __launch_bounds__(256) add_blocks_kernel(const float* part, int blocks, int64_t cols, float* out) {
-    __shared__ float room[8][33];
+// out[c] = sum of part[b][c] over the blocks in an order that only their number sets: 32 columns a block, 32 rows of
+// threads, so that a thread waits for few loads in turn.  A second block row does the same for the parts behind, to `more`.
+static __global__ void __launch_bounds__(1024) add_blocks_kernel(const float* part, int blocks, int64_t cols, float* out, float* more) {
+    __shared__ float room[32][33];
     const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
     const int w = threadIdx.x >> 5;
+    if (blockIdx.y) {
+        part += (int64_t)blocks * cols;
+        out = more;
+    }
     float s = 0.0f;
     if (c < cols) {
-#pragma unroll 4
-        for (int b = w; b < blocks; b += 8) s += part[b * cols + c];
+#pragma unroll 8
+        for (int b = w; b < blocks; b += 32) s += part[b * cols + c];
     }
     room[w][threadIdx.x & 31] = s;
     __syncthreads();
     if (w == 0 && c < cols) {
-        for (int k = 1; k < 8; ++k) s += room[k][threadIdx.x & 31];
+        for (int k = 1; k < 32; ++k) s += room[k][threadIdx.x & 31];
         out[c] = s;
     }
 }

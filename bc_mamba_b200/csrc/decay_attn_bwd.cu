@@ -142,12 +142,14 @@ __device__ __noinline__ void back_tokens(const BwdArgs& p, const T* q, const T* 
     }
 }
 
-template <typename T, int NT, bool VEC>
+// HALF: float32 copies of float16 operands.  Their third pieces are 0 and dv, dk and dq are rounded to 11 bits
+// afterwards, so products with the third pieces are left out (35 of 54 in a chunk remain).
+template <typename T, int NT, bool VEC, bool HALF>
 __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant__ BwdArgs p) {
     extern __shared__ unsigned char smem_raw[];
     using Smem = BwdSmem<T, NT>;
     Smem& sm = *(Smem*)tiles_base(smem_raw);
-    constexpr int NS = Smem::NS, MS = Smem::MS;
+    constexpr int NS = Smem::NS, MS = Smem::MS, NI = HALF ? 2 : NS, MI = HALF ? 2 : MS;       // pieces; those that products take
     const Sizes& z = p.z;
     const int across = z.heads * z.slices, share = z.heads / z.qk_heads;
     const int item = blockIdx.x / across, hs = blockIdx.x % across, h = hs / z.slices, slice = hs % z.slices, col = slice * kP;
@@ -280,22 +282,22 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
                     const Operand<NT, false> Qt(sm.tiles.q), dS(sm.tiles.ds), S(sm.tiles.state());
                     const Operand<kP, true> V(sm.tiles.v), Y(sm.tiles.dy);
                     if (group == 0) {
-                        products<NS, NS, kFull3, NT / 16>(tm + Smem::at, K, Q, t5::instr(kChunk, false, false), false);
+                        products<NI, NI, kFull3, NT / 16>(tm + Smem::at, K, Q, t5::instr(kChunk, false, false), false);
                         t5::commit(&sm.sync.bars[kScores]);
                     } else if (group == 1) {
-                        products<NS, NS, kFull3, kP / 16>(tm + Smem::dt, V, Y, t5::instr(kChunk, false, false), false);
+                        products<NI, NI, kFull3, kP / 16>(tm + Smem::dt, V, Y, t5::instr(kChunk, false, false), false);
                         t5::commit(&sm.sync.bars[kScores]);
                     } else if (group == 3) {
-                        products<NS, MS, MS, NT / 16>(tm + Smem::gv, K, Sk, t5::instr(p16 * 16, false, false), false);
+                        products<NI, MI, MI, NT / 16>(tm + Smem::gv, K, Sk, t5::instr(p16 * 16, false, false), false);
                         t5::commit(&sm.sync.bars[kFarV]);
-                        products<NS, kFull3, kFull3, kP / 16>(tm + Smem::gk, V, dS, t5::instr(n16 * 16, false, true), false);
+                        products<NI, kFull3, kFull3, kP / 16>(tm + Smem::gk, V, dS, t5::instr(n16 * 16, false, true), false);
                         t5::commit(&sm.sync.bars[kFarK]);
                         if (!Smem::one_state) {
-                            products<NS, kFull3, kFull3, kP / 16>(tm + Smem::gq, Y, S, t5::instr(n16 * 16, false, true), false);
+                            products<NI, kFull3, kFull3, kP / 16>(tm + Smem::gq, Y, S, t5::instr(n16 * 16, false, true), false);
                             t5::commit(&sm.sync.bars[kFarQ]);
                         }
                         if (!Smem::late) {
-                            products<kFull3, NS, kFull3, kChunk / 16>(tm + Smem::inc, Operand<kP, false>(sm.tiles.dyw), Qt, t5::instr(NT, true, true), false);
+                            products<kFull3, NI, kFull3, kChunk / 16>(tm + Smem::inc, Operand<kP, false>(sm.tiles.dyw), Qt, t5::instr(NT, true, true), false);
                             t5::commit(&sm.sync.bars[kInc]);
                         }
                     }
@@ -313,7 +315,7 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
                         t5::fence_after();
                         const Operand<NT, false> S(sm.tiles.state());
                         const Operand<kP, true> Y(sm.tiles.dy);
-                        products<NS, kFull3, kFull3, kP / 16>(tm + Smem::gq, Y, S, t5::instr(n16 * 16, false, true), false);
+                        products<NI, kFull3, kFull3, kP / 16>(tm + Smem::gq, Y, S, t5::instr(n16 * 16, false, true), false);
                         t5::commit(&sm.sync.bars[kFarQ]);
                     }
                     __syncwarp();
@@ -409,7 +411,7 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
                         t5::fence_after();
                         const Operand<kP, false> Yw(sm.tiles.dyw);
                         const Operand<NT, false> Qt(sm.tiles.q);
-                        products<kFull3, NS, kFull3, kChunk / 16>(tm + Smem::inc, Yw, Qt, t5::instr(NT, true, true), false);
+                        products<kFull3, NI, kFull3, kChunk / 16>(tm + Smem::inc, Yw, Qt, t5::instr(NT, true, true), false);
                         t5::commit(&sm.sync.bars[kInc]);
                     }
                     __syncwarp();
@@ -582,12 +584,12 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
             const Operand<kP, true> P(sm.tiles.scores());
             const Operand<kP, false> Yt(sm.tiles.dy), Pt(sm.tiles.scores());
             if (group == 0)
-                products<MS, NS, MS, kChunk / 16>(tm + Smem::gv, [&](int s, int i) { return tm + Smem::piece + 32 * s + 8 * i; }, Yt,
+                products<MI, NI, MI, kChunk / 16>(tm + Smem::gv, [&](int s, int i) { return tm + Smem::piece + 32 * s + 8 * i; }, Yt,
                                                   t5::instr(p16 * 16, false, true), true);
             else if (group == 1)
-                products<MS, NS, MS, kChunk / 16>(tm + Smem::gk, P, Qt, t5::instr(n16 * 16, false, true), true);
+                products<MI, NI, MI, kChunk / 16>(tm + Smem::gk, P, Qt, t5::instr(n16 * 16, false, true), true);
             else
-                products<MS, NS, MS, kChunk / 16>(tm + Smem::gq, Pt, Kt, t5::instr(n16 * 16, true, true), true);
+                products<MI, NI, MI, kChunk / 16>(tm + Smem::gq, Pt, Kt, t5::instr(n16 * 16, true, true), true);
             t5::commit(&sm.sync.bars[kNearV + group]);
         }
         __syncwarp();
@@ -614,14 +616,14 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
     sm.sync.end(Smem::cols);
 }
 
-template <typename T, int NT>
+template <typename T, int NT, bool HALF>
 bcm_status launch_bwd(const BwdArgs& p, bool vec, cudaStream_t stream) {
     using Smem = BwdSmem<T, NT>;
     constexpr size_t smem = sizeof(Smem) + 1024;
     static_assert(smem <= 227 * 1024, "shared memory of a block");
     static_assert(sizeof(typename Smem::Tiles) >= sizeof(float) * (NT * kP + 4 * NT + kBwdThreads + kBwdThreads / 32), "the state of back_tokens");
     static_assert(Smem::gq + NT <= 512 && Smem::piece + 32 * Smem::MS <= 512, "tensor memory of a block");
-    auto kernel = vec ? bwd_kernel<T, NT, true> : bwd_kernel<T, NT, false>;
+    auto kernel = vec ? bwd_kernel<T, NT, true, HALF> : bwd_kernel<T, NT, false, HALF>;
     bcm_status st = allow_smem(kernel, smem);
     if (st != BCM_OK) return st;
     kernel<<<(unsigned)(p.z.items * p.z.heads * p.z.slices), kBwdThreads, smem, stream>>>(p);
@@ -629,22 +631,33 @@ bcm_status launch_bwd(const BwdArgs& p, bool vec, cudaStream_t stream) {
     return BCM_OK;
 }
 
-// out[e] = sum over the parts, in their order
-template <typename T>
+// out[e] = sum over the parts, in their order; V elements at a time
+template <typename T, int V>
 __global__ void __launch_bounds__(256) add_parts_kernel(const float* part, int parts, int64_t n, T* out) {
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
-        float s = 0.0f;
+    for (int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; e < n; e += (int64_t)gridDim.x * 256 * V) {
+        float s[V] = {};
 #pragma unroll 4
-        for (int k = 0; k < parts; ++k) s += part[k * n + e];
-        out[e] = from_f32<T>(s);
+        for (int k = 0; k < parts; ++k) {
+            float x[V];
+            if constexpr (V == 4) *(float4*)x = *(const float4*)(part + k * n + e);
+            else x[0] = part[k * n + e];
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[i] += x[i];
+        }
+        struct alignas(V * sizeof(T)) Out { T v[V]; } o;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o.v[i] = from_f32<T>(s[i]);
+        *(Out*)(out + e) = o;
     }
 }
 
 template <typename T>
 bcm_status add_parts(const float* part, int parts, int64_t n, T* out, cudaStream_t stream) {
     if (n == 0) return BCM_OK;
-    const int64_t blocks = std::min<int64_t>((n + 255) / 256, 16 * sm_count());
-    add_parts_kernel<T><<<(unsigned)blocks, 256, 0, stream>>>(part, parts, n, out);
+    const bool four = n % 4 == 0 && (((uintptr_t)part | (uintptr_t)out) & 15) == 0;
+    const int64_t turns = four ? n / 4 : n, blocks = std::min<int64_t>((turns + 255) / 256, 16 * sm_count());
+    if (four) add_parts_kernel<T, 4><<<(unsigned)blocks, 256, 0, stream>>>(part, parts, n, out);
+    else add_parts_kernel<T, 1><<<(unsigned)blocks, 256, 0, stream>>>(part, parts, n, out);
     BCM_LAUNCH_CHECK();
     return BCM_OK;
 }
@@ -678,13 +691,24 @@ __global__ void __launch_bounds__(256) sum_blocks_kernel(const double* x, int he
     out[h] = (float)s;
 }
 
-// float32 copies of strided float16 rows (tokens, heads, width), contiguous: a thread per element
-__global__ void __launch_bounds__(256) widen_kernel(const __grid_constant__ Rows in, int64_t batch, int64_t seqlen, int heads, int width, float* out) {
-    const int64_t n = batch * seqlen * heads * width;
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
-        const int c = (int)(e % width);
-        const int64_t r = e / width, t = r / heads, h = r % heads;
-        out[e] = in.p ? to_f32(((const __half*)in.p)[t / seqlen * in.sb + t % seqlen * in.st + h * in.sh + c]) : 0.0f;
+// float32 copies of strided float16 rows (tokens, heads, width), contiguous: a warp per token, V elements a lane
+template <int V>
+__global__ void __launch_bounds__(256) widen_kernel(const __grid_constant__ Rows in, int64_t tokens, int64_t seqlen, int heads, int width, float* out) {
+    const int per = width / V, n = heads * per;
+    for (int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); t < tokens; t += (int64_t)gridDim.x * 8) {
+        const int64_t b = t / seqlen;
+        const __half* from = (const __half*)in.p + b * in.sb + (t - b * seqlen) * in.st;
+        float* to = out + t * heads * width;
+#pragma unroll 4
+        for (int i = lane_id(); i < n; i += 32) {
+            const int h = i / per, c = (i - h * per) * V;
+            struct alignas(V * 2) In { __half v[V]; } x = {};
+            if (in.p) x = *(const In*)(from + h * in.sh + c);
+            struct alignas(V * 4 < 16 ? V * 4 : 16) Out { float v[V]; } y;
+#pragma unroll
+            for (int e = 0; e < V; ++e) y.v[e] = to_f32(x.v[e]);
+            *(Out*)(to + (int64_t)h * width + c) = y;
+        }
     }
 }
 
@@ -714,8 +738,8 @@ BwdRoom room_of(const bcm_decay_attn_args* a, const Plan& plan) {
     if (z.slices > 1 || r.fixed) r.dg = take(sizeof(float) * z.slices * tokens * z.heads);
     if (z.slices > 1 && r.fixed) r.rows = take(sizeof(float) * tokens * z.heads);
     if (r.fixed) r.sums = take(sizeof(double) * kDecayBlocks * z.heads);
-    // float16 keys of more than 64 features go the way of float32: two pieces of every operand beside two whole states
-    // fill a block's shared memory, and that variant has not run reliably
+    // float16 keys of more than 64 features are taken as float32, whose operands share places in shared memory: two
+    // pieces of every operand beside two whole states would take all of it
     r.widen = a->dtype == BCM_F16 && z.n > 64;
     if (r.widen) {
         for (int i = 0; i < 2; ++i) r.wide[i] = take(sizeof(float) * tokens * z.qk_heads * z.n);
@@ -764,11 +788,13 @@ extern "C" bcm_status bcm_decay_attn_bwd(const bcm_decay_attn_args* a, cudaStrea
         Rows in[4] = {q, k, v, dy};
         void* dv = a->dv;
         if constexpr (widen) {
-            const int64_t batch = z.cu ? 1 : z.batch;
             for (int i = 0; i < 4; ++i) {
                 const int heads = i < 2 ? z.qk_heads : z.heads, width = i < 2 ? z.n : z.p;
+                float* const to = (float*)(ws + room.wide[i]);
                 if (tokens > 0) {
-                    widen_kernel<<<16 * sm_count(), 256, 0, stream>>>(in[i], batch, z.seqlen, heads, width, (float*)(ws + room.wide[i]));
+                    const unsigned blocks = (unsigned)std::min<int64_t>((tokens + 7) / 8, 8 * sm_count());
+                    if (vec) widen_kernel<8><<<blocks, 256, 0, stream>>>(in[i], tokens, z.seqlen, heads, width, to);
+                    else widen_kernel<1><<<blocks, 256, 0, stream>>>(in[i], tokens, z.seqlen, heads, width, to);
                     BCM_LAUNCH_CHECK();
                 }
                 in[i] = rows_of(ws + room.wide[i], (int64_t)z.seqlen * heads * width, (int64_t)heads * width, width);
@@ -785,7 +811,7 @@ extern "C" bcm_status bcm_decay_attn_bwd(const bcm_decay_attn_args* a, cudaStrea
         const BwdArgs ba{plan.z, in[0], in[1], in[2], in[3], a->log_decay, a->g_stride_b, a->g_stride_t, a->g_stride_h, (const float*)a->ckpt,
                          a->dh_last, parts.state, in_ws ? (void*)(ws + room.dq) : a->dq, in_ws ? (void*)(ws + room.dk) : a->dk, dv,
                          dg_parts ? (float*)(ws + room.dg) : a->dlog_decay, a->dh0, room.shares};
-        if ((r = launch_bwd<K, n>(ba, widen ? a->dim_k % 8 == 0 && a->dim_v % 8 == 0 : vec, stream)) != BCM_OK) return r;
+        if ((r = launch_bwd<K, n, widen>(ba, widen ? a->dim_k % 8 == 0 && a->dim_v % 8 == 0 : vec, stream)) != BCM_OK) return r;
         if (in_ws) {
             const int64_t count = tokens * z.qk_heads * z.n;
             if ((r = add_parts((const float*)(ws + room.dq), room.shares, count, (T*)a->dq, stream)) != BCM_OK) return r;

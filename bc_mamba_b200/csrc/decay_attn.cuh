@@ -559,9 +559,11 @@ struct PartSmem {
 };
 
 constexpr int kPartThreads = 256;
+template <typename T, int NT>
+constexpr int kPartResident = sizeof(T) == 2 && NT <= 64 ? 4 : 2;          // blocks on an SM
 
 template <typename T, int NT, bool BACK, bool VEC>
-__global__ void __launch_bounds__(kPartThreads) part_kernel(const __grid_constant__ PartArgs p) {
+__global__ void __launch_bounds__(kPartThreads, kPartResident<T, NT>) part_kernel(const __grid_constant__ PartArgs p) {
     extern __shared__ unsigned char smem_raw[];
     PartSmem<T, NT>& sm = *(PartSmem<T, NT>*)tiles_base(smem_raw);
     constexpr int NS = Pieces<T>::in;

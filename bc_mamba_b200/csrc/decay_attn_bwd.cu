@@ -266,6 +266,16 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
         const int t = c * kChunk;
         bool slow = false;
         if (c < nc) {
+            if (Smem::late) {
+                // no registers hold these tiles through the chunk behind them (they spilled: training of 1 x 30011 tokens
+                // of 12 heads of 128 x 64 float16 1373 us, so 1239)
+                const int r = min(kChunk, len - t);
+                pq.fetch(q + t * p.q.st, p.q.st, r, z.n);
+                pk.fetch(k + t * p.k.st, p.k.st, r, z.n);
+                pv.fetch(v + t * p.v.st, p.v.st, r, cols);
+                py.fetch(dy + t * p.dy.st, p.dy.st, dy ? r : 0, cols);
+                ps.fetch(ckpt + c * ckpt_st, NT, cols, NT);
+            }
             __syncthreads();                                  // decays are there; the chunk behind is done with the tiles
             bad |= pq.bad() | pk.bad() | pv.bad() | py.bad() | ps.bad();
             pq.put(sm.tiles.q[0]);
@@ -325,7 +335,7 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
                 }
             }
         }
-        if (c > 0) {
+        if (!Smem::late && c > 0) {
             const int t2 = t - kChunk, r2 = min(kChunk, len - t2);
             pq.fetch(q + t2 * p.q.st, p.q.st, r2, z.n);
             pk.fetch(k + t2 * p.k.st, p.k.st, r2, z.n);

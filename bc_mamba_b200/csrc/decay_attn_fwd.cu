@@ -19,8 +19,8 @@ bcm_status check(const bcm_decay_attn_args* a, const char* what) {
 
 // Blocks are (item, head, 64 columns of the values) and walk their item's chunks one after another.  Sequences are cut
 // into items only where whole ones leave much of the GPU without a block: an item costs one more pass over two inputs
-// and states to join (16 x 4096 tokens of 8 heads of 64 x 64 bf16, 128 blocks uncut: 538 us with its backward, cut in
-// two 636).  An item has 256 tokens at least.  `room` blocks are two turns of the walks, whose blocks one or two to an SM
+// and states to join (16 x 4096 tokens of 8 heads of 64 x 64 bf16, 128 blocks uncut: 537 us with its backward, cut in
+// two 674; 12 x 4096, 96 blocks, 532 and 648).  An item has 256 tokens at least.  `room` blocks are two turns of the walks, whose blocks one or two to an SM
 // hold, and one of the parts', four to an SM (one turn of the walks against two: 1 x 65536 tokens of 32 such heads 627 and
 // 574 us, forward and backward of 1 x 30011 of 12 heads 518 and 488 us).
 Plan plan_of(const bcm_decay_attn_args* a, bool backward) {

@@ -304,6 +304,9 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
             logs.fetch(kChunk, len);
         }
     }
+    // with 128 features and 128 registers the next chunk's tiles are fetched when it begins: held through this one they
+    // spilled (1 x 65536 tokens of 16 heads of 128 x 128 bf16 1289 us, so 1100)
+    constexpr bool now = NT > 64 && Smem::resident == 2;
     uint32_t phase = 0;
     for (int c = -1; c < nc; ++c) {
         const int t = c * kChunk, rows = min(kChunk, len - t);
@@ -314,6 +317,11 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
                 st.pairs([&](float& x, float& y1, int pp, int n) {
                     if (pp < cols) *(float2*)(to + pp * NT + n) = make_float2(x, y1);
                 });
+            }
+            if (now) {
+                pq.fetch(rows_of_token(p.q, t, hq, 0), p.q.st, rows, z.n);
+                pk.fetch(rows_of_token(p.k, t, hq, 0), p.k.st, rows, z.n);
+                pv.fetch(rows_of_token(p.v, t, h, col), p.v.st, rows, cols);
             }
             __syncthreads();                                  // decays are there; the chunk before is done with the tiles
             bad |= bad_logs | pq.bad() | pk.bad() | pv.bad();
@@ -343,7 +351,7 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
             }
             __syncwarp();
         }
-        if (c + 1 < nc) {
+        if (!now && c + 1 < nc) {
             const int t2 = t + kChunk, r2 = min(kChunk, len - t2);
             pq.fetch(rows_of_token(p.q, t2, hq, 0), p.q.st, r2, z.n);
             pk.fetch(rows_of_token(p.k, t2, hq, 0), p.k.st, r2, z.n);

@@ -32,10 +32,11 @@ struct BwdArgs {
 // 16 queries dealt among them, put the pieces of (Q K^T o D)^T into tensor memory and those of (dY V^T o D)^T into shared
 // memory (where they serve dk by rows and dq by columns) and sum W for dg; then they finish dv, dk and dq: the far part
 // of each is decayed in place and the near part added on top.  The fourth holds the state's gradient and advances it
-// meanwhile.  The next chunk's tiles are on their way to registers during all of that.
+// meanwhile.
 // Bound by the chain of one chunk with one block on an SM (registers, shared and tensor memory are full): 16 x 4096 tokens
 // of 8 heads of 64 x 64 bf16 370 us, 12800 clocks a chunk, of which the tensor cores take 4600 (pipe 24 %, DRAM 18 %);
-// float32 keys of 128 features spill the tiles on their way (1 x 30011 tokens of 12 heads 820 us with HALF).
+// float32 keys of 128 features share one place for the state and its gradient, three more
+// barriers a chunk.
 constexpr int kBwdThreads = 512;
 
 template <typename T, int NT>
@@ -46,6 +47,11 @@ struct BwdSmem {
     static constexpr bool late = NT > 64;
     // and in float32 the state takes the place of its gradient once that has been read
     static constexpr bool one_state = late && NS == 3;
+    // Tiles of several pieces or of 128 features are fetched when their chunk begins; held in registers through the chunk
+    // behind it they spilled (training of 1 x 30011 tokens of 12 heads of 128 x 64 float16 1373 us, so 1241; 16 x 2048 of 8
+    // heads of 64 x 64 float32 473 and 461, float16 389 and 371).  One piece of 64 is fetched ahead (16 x 4096 tokens of
+    // such heads bf16 538 us, else 585).
+    static constexpr bool now = late || NS > 1;
     struct Tiles {
         bf16 q[NS][Wide<NT>::elements], k[NS][Wide<NT>::elements], v[NS][Wide<kP>::elements], dy[NS][Wide<kP>::elements];
         bf16 ds[kFull3][Wide<NT>::elements], dyw[kFull3][Wide<kP>::elements];
@@ -266,9 +272,7 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
         const int t = c * kChunk;
         bool slow = false;
         if (c < nc) {
-            if (Smem::late) {
-                // no registers hold these tiles through the chunk behind them (they spilled: training of 1 x 30011 tokens
-                // of 12 heads of 128 x 64 float16 1373 us, so 1239)
+            if (Smem::now) {
                 const int r = min(kChunk, len - t);
                 pq.fetch(q + t * p.q.st, p.q.st, r, z.n);
                 pk.fetch(k + t * p.k.st, p.k.st, r, z.n);
@@ -335,7 +339,7 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
                 }
             }
         }
-        if (!Smem::late && c > 0) {
+        if (!Smem::now && c > 0) {
             const int t2 = t - kChunk, r2 = min(kChunk, len - t2);
             pq.fetch(q + t2 * p.q.st, p.q.st, r2, z.n);
             pk.fetch(k + t2 * p.k.st, p.k.st, r2, z.n);

@@ -491,89 +491,118 @@ bcm_status launch_fwd(const FwdArgs& p, bool vec, cudaStream_t stream) {
 struct StepArgs {
     Rows q, k, v;
     const float* g;
-    int64_t g_sb, g_sh;
-    int heads, qk_heads, n, p;
-    float* h;
+    int64_t g_sb, g_st, g_sh;
+    int heads, qk_heads, n, p, tokens;
+    const float* from;         // states before the first token (the step: h), or NULL for zeros
+    float* h;                  // and behind the last
     void* y;
 };
 
 // A block per sequence and head: its threads hold V neighbouring columns each, and the rows of the state are dealt to
 // groups of threads, whose sums of q_n S_n meet in shared memory.  Bound by memory, the state read and written once:
-// 256 x 64 heads of 64 x 64 96 us, 86 % of a copy's bandwidth (125 us when the state was read behind the queries' barrier).
-template <typename T, int V>
+// one token of 256 x 64 heads of 64 x 64 92 us, 90 % of a copy's bandwidth (125 us when the state was read behind the
+// queries' barrier).
+// ONE: one token in place (as a token of many 104 us).
+template <typename T, int V, bool ONE>
 __global__ void __launch_bounds__(256) step_kernel(const __grid_constant__ StepArgs a) {
     constexpr int kAhead = 4;
     __shared__ float part[8][32 * V];                     // sums of a warp's rows, by columns
     __shared__ float sq[128], sk[128];
     const int b = blockIdx.x / a.heads, h = blockIdx.x % a.heads, hq = h / (a.heads / a.qk_heads), tid = threadIdx.x;
-    const T* q = (const T*)a.q.p + b * a.q.sb + hq * a.q.sh;
-    const T* k = (const T*)a.k.p + b * a.k.sb + hq * a.k.sh;
-    const T* v = (const T*)a.v.p + b * a.v.sb + h * a.v.sh;
-    float* s = a.h + (int64_t)blockIdx.x * a.n * a.p;
-    T* y = (T*)a.y + (int64_t)blockIdx.x * a.p;
+    float* const s = a.h + (int64_t)blockIdx.x * a.n * a.p;
     // threads side by side over the columns: a power of two, so that the others form whole groups
     int wide = 1;
     while (wide < 32 && wide * V < a.p) wide *= 2;
     const int rows = blockDim.x / wide, row = tid / wide, lane = tid % wide;
     float now[kAhead][V];
     // the state's rows n0, n0 + rows, .. of columns from c: under way before the queries and keys are waited for
-    auto fetch = [&](int c, int n0) {
+    auto fetch = [&](const float* from, int c, int n0) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int n = n0 + i * rows;
-            if (c < a.p && n < a.n) {
-                const float* at = s + (int64_t)n * a.p + c;
+#pragma unroll
+            for (int e = 0; !ONE && e < V; ++e) now[i][e] = 0.0f;
+            if ((ONE || from) && c < a.p && n < a.n) {
+                const float* at = from + (int64_t)n * a.p + c;
                 if constexpr (V == 4) *(float4*)now[i] = *(const float4*)at;
                 else now[i][0] = at[0];
             }
         }
     };
-    fetch(lane * V, row);
-    if (tid < a.n) {
-        sq[tid] = to_f32(q[tid]);
-        sk[tid] = to_f32(k[tid]);
-    }
-    const float decay = expf(a.g[b * a.g_sb + h * a.g_sh]);
-    for (int c0 = 0; c0 < a.p; c0 += wide * V) {
-        const int c = c0 + lane * V;
-        float x[V], sum[V] = {};
+    for (int t = 0; t < (ONE ? 1 : a.tokens); ++t) {
+        // (a thread meets its own elements of the state again with every token)
+        const float* const from = ONE || t ? s : a.from ? a.from + (int64_t)blockIdx.x * a.n * a.p : nullptr;
+        const T* q = (const T*)a.q.p + b * a.q.sb + t * a.q.st + hq * a.q.sh;
+        const T* k = (const T*)a.k.p + b * a.k.sb + t * a.k.st + hq * a.k.sh;
+        const T* v = (const T*)a.v.p + b * a.v.sb + t * a.v.st + h * a.v.sh;
+        T* y = (T*)a.y + (ONE ? (int64_t)blockIdx.x : ((int64_t)b * a.tokens + t) * a.heads + h) * a.p;
+        fetch(from, lane * V, row);
+        if (tid < a.n) {
+            sq[tid] = to_f32(q[tid]);
+            sk[tid] = to_f32(k[tid]);
+        }
+        const float decay = expf(a.g[b * a.g_sb + t * a.g_st + h * a.g_sh]);
+        for (int c0 = 0; c0 < a.p; c0 += wide * V) {
+            const int c = c0 + lane * V;
+            float x[V], sum[V] = {};
 #pragma unroll
-        for (int e = 0; e < V; ++e) x[e] = c < a.p ? to_f32(v[c + e]) : 0.0f;
-        __syncthreads();                                  // queries and keys are there; the last turn's sums are read
-        for (int n0 = row; n0 < a.n; n0 += kAhead * rows) {
-            if (c0 || n0 != row) fetch(c, n0);
+            for (int e = 0; e < V; ++e) x[e] = c < a.p ? to_f32(v[c + e]) : 0.0f;
+            __syncthreads();                                  // queries and keys are there; the last turn's sums are read
+            for (int n0 = row; n0 < a.n; n0 += kAhead * rows) {
+                if (c0 || n0 != row) fetch(from, c, n0);
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const int n = n0 + i * rows;
-                if (c < a.p && n < a.n) {
-                    float* at = s + (int64_t)n * a.p + c;
-                    const float kn = sk[n], qn = sq[n];
+                for (int i = 0; i < kAhead; ++i) {
+                    const int n = n0 + i * rows;
+                    if (c < a.p && n < a.n) {
+                        float* at = s + (int64_t)n * a.p + c;
+                        const float kn = sk[n], qn = sq[n];
 #pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        now[i][e] = fmaf(decay, now[i][e], kn * x[e]);
-                        sum[e] = fmaf(qn, now[i][e], sum[e]);
+                        for (int e = 0; e < V; ++e) {
+                            now[i][e] = fmaf(decay, now[i][e], kn * x[e]);
+                            sum[e] = fmaf(qn, now[i][e], sum[e]);
+                        }
+                        if constexpr (V == 4) *(float4*)at = *(const float4*)now[i];
+                        else at[0] = now[i][0];
                     }
-                    if constexpr (V == 4) *(float4*)at = *(const float4*)now[i];
-                    else at[0] = now[i][0];
                 }
             }
-        }
-        for (int o = 16; o >= wide; o >>= 1) {
+            for (int o = 16; o >= wide; o >>= 1) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) sum[e] += __shfl_xor_sync(kFull, sum[e], o);
-        }
-        if ((tid & 31) < wide) {
+                for (int e = 0; e < V; ++e) sum[e] += __shfl_xor_sync(kFull, sum[e], o);
+            }
+            if ((tid & 31) < wide) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) part[tid >> 5][lane * V + e] = sum[e];
-        }
-        __syncthreads();
-        if (tid < wide * V && c0 + tid < a.p) {
-            float got = 0.0f;
+                for (int e = 0; e < V; ++e) part[tid >> 5][lane * V + e] = sum[e];
+            }
+            __syncthreads();
+            if (tid < wide * V && c0 + tid < a.p) {
+                float got = 0.0f;
 #pragma unroll
-            for (int r = 0; r < 8; ++r) got += part[r][tid];
-            y[c0 + tid] = from_f32<T>(got);
+                for (int r = 0; r < 8; ++r) got += part[r][tid];
+                y[c0 + tid] = from_f32<T>(got);
+            }
         }
     }
+}
+
+// Sequences of few tokens without a backward are not worth a chunk of 64 each: 2000 of 4 heads of 64 x 64 bf16 with 2, 4 and
+// 8 tokens take 75, 129 and 235 us one by one, 203 us as chunks (float32: 8 tokens 234 and 401 us).
+constexpr int kFewTokens = 4;
+// every sequence's tokens one by one, states from `from` (NULL: zeros) to h
+bcm_status launch_step(const bcm_decay_attn_args* a, const float* from, float* h, cudaStream_t stream) {
+    const StepArgs sa{rows_of(a->q, a->q_stride_b, a->q_stride_t, a->q_stride_h), rows_of(a->k, a->k_stride_b, a->k_stride_t, a->k_stride_h),
+                      rows_of(a->v, a->v_stride_b, a->v_stride_t, a->v_stride_h), a->log_decay, a->g_stride_b, a->g_stride_t, a->g_stride_h,
+                      (int)a->heads, (int)a->qk_heads, (int)a->dim_k, (int)a->dim_v, (int)a->seqlen, from, h, a->y};
+    const bool four = a->dim_v % 4 == 0 && (((uintptr_t)h | (uintptr_t)from) & 15) == 0;
+    const unsigned blocks = (unsigned)(a->batch * a->heads);
+    return dispatch_dtype(a->dtype, [&](auto type) -> bcm_status {
+        using T = decltype(type);
+        const bool one = a->seqlen == 1 && from == h;
+        auto kernel = four ? (one ? step_kernel<T, 4, true> : step_kernel<T, 4, false>) : one ? step_kernel<T, 1, true> : step_kernel<T, 1, false>;
+        kernel<<<blocks, 256, 0, stream>>>(sa);
+        BCM_LAUNCH_CHECK();
+        return BCM_OK;
+    });
 }
 
 }  // namespace decay_attn
@@ -604,6 +633,7 @@ extern "C" bcm_status bcm_decay_attn_fwd(const bcm_decay_attn_args* a, cudaStrea
     BCM_REQUIRE(plan.bytes == 0 || (a->workspace && a->workspace_bytes >= plan.bytes), "decay_attn_fwd: workspace too small");
     BCM_REQUIRE(!a->ckpt || a->ckpt_bytes >= bcm_decay_attn_ckpt_bytes(a), "decay_attn_fwd: ckpt too small");
     BCM_REQUIRE((int64_t)plan.z.items * plan.z.heads * plan.z.slices < INT32_MAX, "decay_attn_fwd: too many blocks");
+    if (!a->cu_seqlens && !a->ckpt && a->seqlen >= 1 && a->seqlen <= kFewTokens) return launch_step(a, a->h0, a->h_last, stream);
     if ((st = fill_tables(plan, a->workspace, stream)) != BCM_OK) return st;
     const Parts parts = parts_of(plan, a->workspace);
     const Rows q = rows_of(a->q, a->q_stride_b, a->q_stride_t, a->q_stride_h), k = rows_of(a->k, a->k_stride_b, a->k_stride_t, a->k_stride_h),
@@ -631,16 +661,5 @@ extern "C" bcm_status bcm_decay_attn_step(const bcm_decay_attn_args* a, float* h
     if (a->batch == 0) return BCM_OK;
     BCM_REQUIRE(a->q && a->k && a->v && a->log_decay && a->y && h, "decay_attn_step: null pointer");
     BCM_REQUIRE(a->batch * a->heads < INT32_MAX, "decay_attn_step: too many blocks");
-    const StepArgs sa{rows_of(a->q, a->q_stride_b, 0, a->q_stride_h), rows_of(a->k, a->k_stride_b, 0, a->k_stride_h),
-                      rows_of(a->v, a->v_stride_b, 0, a->v_stride_h), a->log_decay, a->g_stride_b, a->g_stride_h, (int)a->heads,
-                      (int)a->qk_heads, (int)a->dim_k, (int)a->dim_v, h, a->y};
-    const bool four = a->dim_v % 4 == 0 && ((uintptr_t)h & 15) == 0;
-    const unsigned blocks = (unsigned)(a->batch * a->heads);
-    return dispatch_dtype(a->dtype, [&](auto type) -> bcm_status {
-        using T = decltype(type);
-        if (four) step_kernel<T, 4><<<blocks, 256, 0, stream>>>(sa);
-        else step_kernel<T, 1><<<blocks, 256, 0, stream>>>(sa);
-        BCM_LAUNCH_CHECK();
-        return BCM_OK;
-    });
+    return launch_step(a, h, h, stream);
 }

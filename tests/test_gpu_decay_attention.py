@@ -360,3 +360,21 @@ def test_refusals():
     y, _ = itf.decay_attention(q, q, x, g)
     with pytest.raises(RuntimeError, match="not differentiable"):
         torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("L", [1, 2, 7, 8, 9])
+@pytest.mark.parametrize("N,P,H,Hk", [(5, 9, 2, 1), (64, 64, 3, 3), (128, 132, 2, 2)])
+@pytest.mark.parametrize("entering", [False, True])
+def test_few_tokens_without_a_gradient(L, dtype, N, P, H, Hk, entering):
+    """Calls that record no gradient give what calls that do give: float32 sums of at most N products for the former, two
+    bfloat16 pieces of 2^-18 for the latter, so 2 half steps of the output's type and 2^-16 apart next to the largest."""
+    g = torch.Generator(device=dev).manual_seed(L)
+    rn = lambda *s: torch.randn(*s, generator=g, device=dev)
+    q, k, v = (rn(3, L, Hk, N) * N ** -0.5).to(dtype), rn(3, L, Hk, N).to(dtype), rn(3, L, H, P).to(dtype)
+    log_decay, h0 = -torch.rand(3, L, H, generator=g, device=dev), rn(3, H, N, P) if entering else None
+    y, h = itf.decay_attention(q, k, v, log_decay, h0=h0)
+    y2, h2 = itf.decay_attention(q.requires_grad_(True), k, v, log_decay, h0=h0)
+    tol = torch.finfo(dtype).eps + 2.0 ** -16
+    assert ((y - y2).abs() <= tol * (y2.abs() + y2.abs().max())).all()
+    assert ((h - h2).abs() <= 2.0 ** -16 * (h2.abs() + h2.abs().max())).all()

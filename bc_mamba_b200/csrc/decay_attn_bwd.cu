@@ -788,7 +788,7 @@ extern "C" bcm_status bcm_decay_attn_bwd(const bcm_decay_attn_args* a, cudaStrea
     const Sizes& z = plan.z;
     const BwdRoom room = room_of(a, plan);
     BCM_REQUIRE(a->seqlen == 0 || (a->q && a->k && a->v && a->log_decay && a->dq && a->dk && a->dv && a->ckpt), "decay_attn_bwd: null pointer");
-    BCM_REQUIRE(a->dh0 && a->dlog_decay, "decay_attn_bwd: null pointer");
+    BCM_REQUIRE(a->dh0 && (a->dlog_decay || (a->seqlen == 0 && !a->fixed_decay)), "decay_attn_bwd: null pointer");   // (empty: no address)
     BCM_REQUIRE(room.bytes == 0 || (a->workspace && a->workspace_bytes >= room.bytes), "decay_attn_bwd: workspace too small");
     BCM_REQUIRE(a->ckpt_bytes >= bcm_decay_attn_ckpt_bytes(a), "decay_attn_bwd: ckpt too small");
     BCM_REQUIRE((int64_t)z.items * z.heads * z.slices < INT32_MAX, "decay_attn_bwd: too many blocks");

@@ -1,0 +1,25 @@
+"""CPU tests of what the linear attention's C entries accept and refuse at the edges of their contract, before any kernel
+runs: a call that passes the checks ends with a CUDA error here, where there is no GPU."""
+import ctypes
+
+import pytest
+
+from test_attention_operators_cpu import Attn, _call
+
+
+def _some(n=4):
+    """n addresses that no check may look behind."""
+    return [ctypes.c_void_p(256 * (1 + k)) for k in range(n)]
+
+
+@pytest.mark.parametrize("heads,qk_heads", [(1, 1), (4, 2)])
+def test_sequences_without_a_token_need_no_decays_gradient(heads, qk_heads):
+    """Per-token decays of no token: their gradient is empty, and an empty tensor has no address."""
+    dh0, ws = _some(2)
+    status, text = _call("bcm_decay_attn_bwd", Attn(batch=2, seqlen=0, heads=heads, qk_heads=qk_heads, dim_k=8, dim_v=8, dh0=dh0, workspace=ws,
+                                                    workspace_bytes=1 << 20))
+    assert b"null pointer" not in text, text
+    # one decay for each head has a gradient all the same, and a token's decay too
+    for more in (dict(fixed_decay=1), dict(seqlen=1, ckpt_bytes=1 << 20, **{n: _some(1)[0] for n in ("q", "k", "v", "g", "dq", "dk", "dv", "ckpt")})):
+        a = Attn(**{**dict(batch=2, seqlen=0, heads=heads, qk_heads=qk_heads, dim_k=8, dim_v=8, dh0=dh0, workspace=ws, workspace_bytes=1 << 20), **more})
+        assert _call("bcm_decay_attn_bwd", a) == (1, b"decay_attn_bwd: null pointer")

@@ -1,0 +1,30 @@
+"""The linear attention at the edges of its contract, against the float64 oracle.  Tolerances as derived in
+test_gpu_decay_attention.py unless a test says otherwise."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from bc_mamba_b200 import interface as itf
+from helpers import assert_close
+from oracle import decay_attn as orc
+from test_gpu_decay_attention import DTYPES, F32, TOL, _check, _inputs, _np
+
+pytestmark = pytest.mark.gpu
+dev = "cuda"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradients_of_sequences_without_a_token(dtype):
+    """The state passes through, and so does its gradient, whatever form the decays have."""
+    z = lambda *s, dtype=dtype: torch.zeros(*s, device=dev, dtype=dtype)
+    for shape, cu in (((2, 0), None), ((0,), z(3, dtype=torch.int32))):
+        for decay in ((*shape, 3), (3,)):
+            leaves = [z(*shape, 1, 4), z(*shape, 1, 4), z(*shape, 3, 5), z(*decay, dtype=torch.float32), torch.randn(2, 3, 4, 5, device=dev)]
+            leaves = [x.requires_grad_(True) for x in leaves]
+            y, h = itf.decay_attention(*leaves[:4], h0=leaves[4], cu_seqlens=cu)
+            dh = torch.randn_like(h)
+            grads = torch.autograd.grad([y, h], leaves, [torch.zeros_like(y), dh])
+            assert torch.equal(grads[4], dh) and (grads[3] == 0).all()
+            assert all(g.shape == x.shape for g, x in zip(grads, leaves))

@@ -13,6 +13,7 @@ bcm_status check(const bcm_decay_attn_args* a, const char* what) {
     BCM_REQUIRE(a->batch > 0 || a->seqlen == 0 || !a->cu_seqlens, "%s: offsets of no sequence with tokens", what);
     BCM_REQUIRE(a->heads % a->qk_heads == 0, "%s: heads must be a multiple of the queries' heads", what);
     BCM_REQUIRE(a->dim_v <= (1 << 20) && a->heads <= (1 << 20) && a->batch < (1 << 24) && a->seqlen < INT32_MAX - 4096, "%s: sizes too large", what);
+    BCM_REQUIRE(on_16(a->ckpt, 0) && on_16(a->workspace, 0), "%s: ckpt and workspace must be aligned to 16 bytes", what);
     BCM_REQUIRE(a->heads * a->dim_v <= (1 << 24) && a->batch * (a->seqlen / kChunk + 1) < INT32_MAX, "%s: sizes too large", what);
     return BCM_OK;
 }
@@ -76,7 +77,7 @@ bool aligned(const bcm_decay_attn_args* a, bool backward) {
         !in(a->k, a->k_stride_b, a->k_stride_t, a->k_stride_h) || !in(a->v, a->v_stride_b, a->v_stride_t, a->v_stride_h))
         return false;
     if (!backward) return on_16(a->y, 0);
-    return in(a->dy, a->dy_stride_b, a->dy_stride_t, a->dy_stride_h) && on_16(a->dq, 0) && on_16(a->dk, 0) && on_16(a->dv, 0) && on_16(a->workspace, 0);
+    return in(a->dy, a->dy_stride_b, a->dy_stride_t, a->dy_stride_h) && on_16(a->dq, 0) && on_16(a->dk, 0) && on_16(a->dv, 0);
 }
 
 Parts parts_of(const Plan& plan, void* workspace) {

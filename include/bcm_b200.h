@@ -720,7 +720,8 @@ BCM_API bcm_status bcm_sample_tokens(const bcm_sample_args* args, cudaStream_t s
  * States and sums are fp32.  A value that is not finite reaches no token before
  * its own.
  * ckpt (bcm_decay_attn_ckpt_bytes): the states that the backward restarts from;
- * NULL in a forward without a backward.  Backward: dy or dh_last NULL is a zero
+ * NULL in a forward without a backward.  ckpt and workspace are read and written
+ * 16 bytes at a time: both must be aligned to 16 bytes.  Backward: dy or dh_last NULL is a zero
  * gradient; dq, dk, dv [as q, k, v] contiguous in dtype, dlog_decay
  * [batch, seqlen, heads] fp32 contiguous, with fixed_decay [heads] (sums over
  * the tokens), dh0 as h0; every output is written, not accumulated, and sums run

@@ -23,3 +23,14 @@ def test_sequences_without_a_token_need_no_decays_gradient(heads, qk_heads):
     for more in (dict(fixed_decay=1), dict(seqlen=1, ckpt_bytes=1 << 20, **{n: _some(1)[0] for n in ("q", "k", "v", "g", "dq", "dk", "dv", "ckpt")})):
         a = Attn(**{**dict(batch=2, seqlen=0, heads=heads, qk_heads=qk_heads, dim_k=8, dim_v=8, dh0=dh0, workspace=ws, workspace_bytes=1 << 20), **more})
         assert _call("bcm_decay_attn_bwd", a) == (1, b"decay_attn_bwd: null pointer")
+
+
+@pytest.mark.parametrize("name,more", [("bcm_decay_attn_fwd", ()), ("bcm_decay_attn_bwd", ()), ("bcm_decay_attn_step", (None,))])
+@pytest.mark.parametrize("buffer", ["ckpt", "workspace"])
+@pytest.mark.parametrize("off", [4, 8, 12])
+def test_buffers_off_16_bytes_are_refused(name, more, buffer, off):
+    """Both are read 16 bytes at a time."""
+    a = Attn(batch=0, seqlen=1, heads=4, qk_heads=2, dim_k=8, dim_v=8, **{buffer: ctypes.c_void_p(4096 + off)})
+    assert _call(name, a, *more) == (1, f"{name[4:]}: ckpt and workspace must be aligned to 16 bytes".encode())
+    setattr(a, buffer, 4096 + 16)
+    assert _call(name, a, *more) == (0, b"")

@@ -55,12 +55,20 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     return r;
 }
 
-// two values as M pieces each
+// as pack(), but what rounds beyond bf16's largest number becomes that number
+__device__ __forceinline__ uint32_t pack_within(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// Two values as M pieces each.  A float32 within 2^-9 of the largest would round up to an infinite first piece: it gets
+// bf16's largest number instead, and the next piece the rest.  An infinity stays one, in the last piece.
 template <int M>
 __device__ __forceinline__ void split(float x, float y, uint32_t (&r)[M]) {
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-        r[m] = pack(x, y);
+        r[m] = m + 1 < M ? pack_within(x, y) : pack(x, y);
         if (m + 1 < M) {
             x -= low_f(r[m]);
             y -= high_f(r[m]);
@@ -200,7 +208,8 @@ __device__ __forceinline__ const T* row_ptr(const Rows& r, const Sizes& z, int s
 }
 
 // ---------------------------------------------------------------------- tiles ----
-// 0 as long as every value seen has finite pieces (those of a float32 next to the largest round up to infinity)
+// 0 as long as every value seen is finite (or within 2^-8 of float32's largest: such a value is taken token by token too,
+// where it enters no product of scores)
 __device__ __forceinline__ float seen(float v, float so_far) { return fmaf(v * 1.00390625f, 0.0f, so_far); }
 
 // 64 rows x W columns on their way to shared memory: each of TH threads has groups of eight columns.  Rows and columns

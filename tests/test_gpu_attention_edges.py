@@ -28,3 +28,27 @@ def test_gradients_of_sequences_without_a_token(dtype):
             grads = torch.autograd.grad([y, h], leaves, [torch.zeros_like(y), dh])
             assert torch.equal(grads[4], dh) and (grads[3] == 0).all()
             assert all(g.shape == x.shape for g, x in zip(grads, leaves))
+
+
+@pytest.mark.parametrize("rows", [100, 1500])
+@pytest.mark.parametrize("which", ["v", "k", "q", "h0", "dh", "dy"])
+def test_values_next_to_the_largest_float(rows, which):
+    """3.4e38 is finite, but its nearest bf16 number is not: alone, and in a sequence that is cut into items."""
+    t = _inputs(rows, 1, 2, 1, 16, 24, torch.float32, seed=31)
+    for name in ("q", "k", "v", "dy", "h0", "dh"):
+        t[name] *= 0.05
+    for at in ((0, 1, 2, 3),) if which in ("h0", "dh") else ((rows // 3, 0, 3), (rows - 30, 0, 5)):
+        t[which][at] = 3.4e38
+    _check(t, (0, rows), (1, rows))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [3, 100, 1500])
+def test_states_next_to_the_largest_float(rows, dtype):
+    t = _inputs(rows, 1, 2, 1, 16, 24, dtype, seed=32)
+    t["q"].zero_()
+    t["g"] *= 1e-6
+    t["h0"][0, 1, 2, 3] = -3.4e38
+    y, h = itf.decay_attention(*(t[k][None] for k in ("q", "k", "v", "g")), h0=t["h0"])
+    assert (y == 0).all() and torch.isfinite(h).all()
+    assert_close(h, orc.fwd(*(_np(t[k]) for k in ("q", "k", "v", "g")), _np(t["h0"]), (0, rows))[1], F32, "h_last")

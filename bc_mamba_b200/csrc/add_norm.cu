@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(G::threads, resident(G::threads, kAddBwdPerSm)
             dot = fmaf(w[j], v[j], dot);
         }
         G::sum(sq, dot, room, turn);
-        const float r = rsqrtf(sq / p.dim + p.eps), m = r * r * (dot / p.dim);
+        const float r = rsqrtf(sq / p.dim + p.eps), m = r * (r * (dot / p.dim));       // (r r of a tiny eps alone may be infinite)
 #pragma unroll
         for (int j = 0; j < G::n; ++j) {
             dw[j] = fmaf(d[j] * v[j], r, dw[j]);

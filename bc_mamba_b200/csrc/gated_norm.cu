@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(G::threads, resident(G::threads, kGatedPerSm<B
         G::sum(sq, dot, room, turn);
         const float r = rsqrtf(sq / width + p.eps);
         if (BACK) {
-            const float m = r * r * (dot / width);
+            const float m = r * (r * (dot / width));           // (r r of a tiny eps alone may be infinite)
 #pragma unroll
             for (int j = 0; j < G::n; ++j) {
                 dw[j] = fmaf(d[j], r, dw[j]);

@@ -189,7 +189,7 @@ __device__ __forceinline__ Item item_of(const Sizes& z, int i) {
     it.seq = i / z.per_seq;
     const int s = i - it.seq * z.per_seq;
     it.t0 = s * z.span;
-    it.t1 = min(z.seqlen, it.t0 + z.span);
+    it.t1 = it.t0 + min(z.span, z.seqlen - it.t0);            // (t0 + span may pass 2^31)
     it.chunk = it.seq * ((z.seqlen + kChunk - 1) / kChunk) + it.t0 / kChunk;
     it.first = s == 0;
     it.last = s == z.per_seq - 1;

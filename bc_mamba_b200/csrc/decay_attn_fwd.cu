@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(1024) tables_kernel(Sizes z) {
         const int start = max(before, l ? up : 0);
         end = max(before, end);
         const int len = end - start;
-        const int items = in ? max(1, (len + z.span - 1) / z.span) : 0, chunks = in ? (len + kChunk - 1) / kChunk : 0;
+        const int items = in ? (len > 0 ? (len - 1) / z.span + 1 : 1) : 0, chunks = in ? (len + kChunk - 1) / kChunk : 0;
         const int si = warp_inclusive_sum(items), sc = warp_inclusive_sum(chunks);
         if (l == 31) {
             part[1][w] = si;
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(1024) tables_kernel(Sizes z) {
             z.tables.seq_item[s] = item;
             for (int k = 0; k < items; ++k) {
                 const int t0 = start + k * z.span;
-                z.tables.items[item + k] = Item{s, t0, min(end, t0 + z.span), chunk + k * (z.span / kChunk), k == 0, k == items - 1};
+                z.tables.items[item + k] = Item{s, t0, t0 + min(z.span, end - t0), chunk + k * (z.span / kChunk), k == 0, k == items - 1};
             }
         }
         __syncthreads();

@@ -52,3 +52,26 @@ def test_states_next_to_the_largest_float(rows, dtype):
     y, h = itf.decay_attention(*(t[k][None] for k in ("q", "k", "v", "g")), h0=t["h0"])
     assert (y == 0).all() and torch.isfinite(h).all()
     assert_close(h, orc.fwd(*(_np(t[k]) for k in ("q", "k", "v", "g")), _np(t["h0"]), (0, rows))[1], F32, "h_last")
+
+
+@pytest.mark.parametrize("cu", [None, (0, 5, 2147479550 - 1000, 2147479550)])
+def test_close_to_two_to_the_31_tokens(cu):
+    """The last item of a sequence ends before its span would, which passes 2^31.  One token expanded to all of them:
+    y_t = sum of a^s over s <= t, which is constant from the hundredth token on."""
+    rows = 2147479550
+    one = torch.ones(1, 1, device=dev, dtype=torch.bfloat16)
+    x = one.expand(rows, 1, 1) if cu else one.expand(1, rows, 1, 1)
+    g = torch.full((1,), -0.5, device=dev)
+    with torch.no_grad():
+        y, h = itf.decay_attention(x, x, x, g, cu_seqlens=None if cu is None else torch.tensor(cu, dtype=torch.int32, device=dev))
+    y = y.reshape(-1)
+    want = 1 / (1 - math.exp(-0.5))
+    starts = cu or (0, rows)
+    for a, b in zip(starts, starts[1:]):
+        n = min(100, b - a)
+        first = torch.tensor([want * (1 - math.exp(-0.5 * (t + 1))) for t in range(n)], device=dev)
+        assert ((y[a:a + n].float() - first).abs() <= TOL[torch.bfloat16] * want).all()
+        for lo in range(a + n, b, 1 << 28):
+            part = y[lo:min(b, lo + (1 << 28))]
+            assert abs(part.min().item() - want) <= TOL[torch.bfloat16] * want and abs(part.max().item() - want) <= TOL[torch.bfloat16] * want
+    assert abs(h[-1].item() - want) <= F32 * want

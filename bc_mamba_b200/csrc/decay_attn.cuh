@@ -455,7 +455,9 @@ struct Logs {
 };
 
 // What has to be initialised and awaited: barriers of the tensor cores' work, the tensor memory's address, and whether
-// a wait has run out of time, after which no wait is made any more and results are NaN.
+// a wait has run out of time (t5::bar_wait).  After that no wait is made any more: the walk goes to its end with whatever
+// its sums hold, the products still under way are awaited, and all that the block writes from then on, or in the end all
+// that it has written, is NaN.
 template <int BARS>
 struct Sync {
     uint64_t bars[BARS];
@@ -478,14 +480,31 @@ struct Sync {
         t5::bar_wait(&bars[bar], phase, &failed);
         t5::fence_after();
     }
-    // the whole block, all products awaited
+    // 0, or NaN once a wait has run out
+    __device__ __forceinline__ float poison() const { return __int_as_float(*(const volatile int*)&failed); }
+    // the whole block, its walk over: whether a wait ran out
+    __device__ __forceinline__ bool lost() {
+        __syncthreads();
+        return failed != 0;
+    }
+    // The whole block, all products awaited.  Where a wait ran out, products may be under way that use this block's memory:
+    // they have as long again to end.
     __device__ __forceinline__ void end(uint32_t cols) {
         t5::fence_before();
         __syncthreads();
         t5::fence_after();
-        if (threadIdx.x < 32) t5::dealloc(tmem, cols);
+        if (threadIdx.x < 32) {
+            t5::rest_if(&failed);
+            t5::dealloc(tmem, cols);
+        }
     }
 };
+
+// the rows of a block that lost a wait; all its threads
+template <typename T>
+__device__ __noinline__ void nan_rows(T* out, int64_t stride, int rows, int cols) {
+    for (int64_t e = threadIdx.x; e < (int64_t)rows * cols; e += blockDim.x) out[e / cols * stride + e % cols] = from_f32<T>(__int_as_float(0x7fc00000));
+}
 
 // dynamic shared memory from the next multiple of 1024 bytes (tiles want it)
 __device__ __forceinline__ unsigned char* tiles_base(unsigned char* raw) { return raw + ((1024 - (t5::smem_u32(raw) & 1023)) & 1023); }
@@ -638,10 +657,11 @@ __global__ void __launch_bounds__(kPartThreads, kPartResident<T, NT>) part_kerne
         st.advance(acc + ((warp & 3) << 21), sm.d[i & 1].whole);
         t5::fence_before();
     }
-    if (sm.sync.failed) st.pairs([](float& x, float& y, int, int) { x = y = __int_as_float(0x7fc00000); });
     const int64_t at = (int64_t)item * z.heads + h;
     st.store(p.parts.state + at * z.n * z.p + col, z.n, cols, z.p);
     if (threadIdx.x == 128 && col == 0) p.parts.whole[at] = exp2f((float)all);
+    // (the items behind begin with it)
+    if (sm.sync.lost()) nan_rows(p.parts.state + at * z.n * z.p + col, z.p, z.n, cols);
     sm.sync.end(kCols);
 }
 

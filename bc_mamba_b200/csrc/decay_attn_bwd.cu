@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
         if (l == 31) rest = 0.0f;
         if (l == 0) past = 0.0f;
         const float through = sm.across_whole[c & 1] * ((sm.across[c & 1][0] + sm.across[c & 1][1]) + (sm.across[c & 1][2] + sm.across[c & 1][3]));
-        float d0 = 0.0f, d1 = 0.0f;
+        float d0 = sm.sync.poison(), d1 = d0;                 // (where a wait ran out all gradients are NaN)
         for (int k2 = 0; k2 <= block; ++k2) {
             d0 += sm.pairs[c & 1][k2][t];
             d1 += sm.pairs[c & 1][k2][t + 1];
@@ -380,9 +380,10 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
             if (slow) {
                 // token by token, through shared memory
                 float* f = (float*)&sm.tiles;
+                const float none = sm.sync.poison();
                 ds.pairs([&](float& x0, float& x1, int pp, int n) {
-                    f[n * kP + pp] = x0;
-                    f[(n + 1) * kP + pp] = x1;
+                    f[n * kP + pp] = x0 + none;
+                    f[(n + 1) * kP + pp] = x1 + none;
                 });
                 __syncthreads();
                 walk(c);
@@ -611,6 +612,8 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
         }
         __syncwarp();
         sm.sync.wait(kNearV + group, phase);
+        // (a wait lost by another warp is known by now: what it held up is awaited behind the barrier above)
+        const float none = sm.sync.poison();
         // ---- out: dv, or (whole or as a part) dk and dq
         const RowsOut<T> o = group == 0 ? RowsOut<T>{dv + t * v_st, nullptr, v_st} : rows_out(group == 1 ? p.dk : p.dq, row_at + t);
         const int width = group == 0 ? cols : z.n, blocks = group == 0 ? p16 : n16;
@@ -618,6 +621,10 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
         for (int nb = 0; nb < blocks; nb += 2) {
             float x[2][4], x2[2][4];
             t5::ld16x2(x, acc + 16 * nb, x2, acc + 16 * min(nb + 1, blocks - 1));
+            if (none != 0.0f) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e >> 2][e & 3] = x2[e >> 2][e & 3] = none;
+            }
             if (o.part) {
                 store_rows<VEC>(o.part, o.st, rows, width, row, 16 * nb, x[0], x[1]);
                 store_rows<VEC>(o.part, o.st, rows, width, row, 16 * nb + 16, x2[0], x2[1]);

@@ -260,6 +260,22 @@ __device__ __noinline__ void walk_tokens(const FwdArgs& p, const T* q, const T* 
     }
 }
 
+// All that this block has written becomes NaN (of its own item: the others begin with states from elsewhere).  Finds them
+// anew, so that the walk holds nothing for it in registers.
+template <typename T, int NT>
+__device__ __noinline__ void nan_item(const FwdArgs& p) {
+    const Sizes& z = p.z;
+    const int across = z.heads * z.slices, item = blockIdx.x / across, hs = blockIdx.x % across, h = hs / z.slices, slice = hs % z.slices;
+    const Item it = item_of(z, item);
+    const int len = it.t1 - it.t0;
+    const int64_t y_st = (int64_t)z.heads * z.p, row_at = (z.cu ? 0 : (int64_t)it.seq * z.seqlen) + it.t0;
+    nan_rows((T*)p.y + row_at * y_st + (int64_t)h * z.p + slice * kP, y_st, len, min(kP, z.p - slice * kP));
+    if (p.ckpt)
+        nan_rows(p.ckpt + (((int64_t)it.chunk * z.heads + h) * z.slices + slice) * (NT * kP), (int64_t)z.heads * z.slices * (NT * kP),
+                 (len + kChunk - 1) / kChunk, NT * kP);
+    if (it.last) nan_rows(p.h_last + ((int64_t)it.seq * z.heads + h) * z.n * z.p + slice * kP, z.p, z.n, min(kP, z.p - slice * kP));
+}
+
 template <typename T, int NT, bool VEC>
 __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_kernel(const __grid_constant__ FwdArgs p) {
     extern __shared__ unsigned char smem_raw[];
@@ -467,10 +483,8 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
         t5::fence_before();
         phase ^= 1;
     }
-    if (state_warp) {
-        if (sm.sync.failed) st.pairs([](float& x, float& y1, int, int) { x = y1 = __int_as_float(0x7fc00000); });
-        if (it.last) st.store(p.h_last + ((int64_t)it.seq * z.heads + h) * np + col, z.n, cols, z.p);
-    }
+    if (state_warp && it.last) st.store(p.h_last + ((int64_t)it.seq * z.heads + h) * np + col, z.n, cols, z.p);
+    if (sm.sync.lost()) nan_item<T, NT>(p);
     sm.sync.end(Smem::cols);
 }
 

@@ -66,8 +66,8 @@ __device__ __forceinline__ void bar_init(uint64_t* bar, int count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
 }
 // Waits for the phase, a warp as one (its threads leave together: what follows moves all their registers to or from tensor
-// memory).  After 2^31 cycles (about a second; products of a tile take microseconds) it gives up and sets *failed, and
-// where that is set it does not wait.
+// memory).  After 2^31 cycles (about a second; products of a tile take microseconds) it gives up and sets *failed to the bits
+// of a NaN, and where that is set it does not wait.
 __device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t phase, int* failed) {
     __syncwarp();
     asm volatile(
@@ -89,9 +89,32 @@ __device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t phase, int* fai
         "setp.lt.u64 p, t, 0x80000000;\n\t"
         "vote.sync.any.pred p, p, 0xffffffff;\n\t"
         "@p bra.uni AGAIN;\n\t"
-        "st.volatile.shared.b32 [%2], 1;\n"
+        "st.volatile.shared.b32 [%2], 0x7fc00000;\n"
         "DONE:\n\t"
         "}" ::"r"(smem_u32(bar)), "r"(phase), "r"(smem_u32(failed))
+        : "memory");
+    __syncwarp();
+}
+
+// a warp lets 2^31 cycles pass where *failed is set (without a branch that the compiler sees: one behind a kernel's walk made
+// it hold more registers in the walk)
+__device__ __forceinline__ void rest_if(const int* failed) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        ".reg .b32 f;\n\t"
+        ".reg .b64 t, s;\n\t"
+        "ld.volatile.shared.b32 f, [%0];\n\t"
+        "setp.eq.b32 p, f, 0;\n\t"
+        "@p bra DONE;\n\t"
+        "mov.u64 s, %%clock64;\n"
+        "AGAIN:\n\t"
+        "mov.u64 t, %%clock64;\n\t"
+        "sub.u64 t, t, s;\n\t"
+        "setp.lt.u64 p, t, 0x80000000;\n\t"
+        "@p bra AGAIN;\n"
+        "DONE:\n\t"
+        "}" ::"r"(smem_u32(failed))
         : "memory");
     __syncwarp();
 }

@@ -87,7 +87,7 @@ struct RowsOut {
     }
 };
 
-// A chunk with a value that is not finite, token by token from its last: a state is run up anew for each.
+// A chunk with an input that is not finite, token by token from its last: a state is run up anew for each.
 // `f` (shared): the state's gradient NT x kP, then sums.
 template <typename T, int NT>
 __device__ __noinline__ void back_tokens(const BwdArgs& p, const T* q, const T* k, const T* v, const T* dy, const float* g, const float* s_in,
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
                 ps.fetch(ckpt + c * ckpt_st, NT, cols, NT);
             }
             __syncthreads();                                  // decays are there; the chunk behind is done with the tiles
-            bad |= pq.bad() | pk.bad() | pv.bad() | py.bad() | ps.bad();
+            bad |= pq.bad() | pk.bad() | pv.bad() | py.bad();
             pq.put(sm.tiles.q[0]);
             pk.put(sm.tiles.k[0]);
             pv.put(sm.tiles.v[0]);
@@ -358,13 +358,13 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
     uint32_t phase = 0;
     if (group == 3) {
         State<NT, 1> ds(0);
-        bool bad, bad_logs = false, pending = false;          // pending: the chunk behind has its dg still to be finished
+        bool bad_logs = false, pending = false;               // pending: the chunk behind has its dg still to be finished
         const float* from = it.last ? (p.dh_last ? p.dh_last + ((int64_t)it.seq * z.heads + h) * np : nullptr)
                                     : p.enter + ((int64_t)item * z.heads + h) * np;
         if (decay_warp) logs.fetch((nc - 1) * kChunk, len);
         if (from) ds.load(from + col, z.n, cols, z.p);
         else ds.zero();
-        bad = ds.template put<kFull3>(sm.tiles.ds[0]);
+        ds.template put<kFull3, !Smem::late>(sm.tiles.ds[0]);
         if (decay_warp) {
             bad_logs = logs.bad();
             decays_of(sm.d[(nc - 1) & 1], logs.a, logs.b);
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
         }
         for (int c = nc; c >= 0; --c) {
             const int t = c * kChunk;
-            const bool slow = start(c, bad | bad_logs, phase);
+            const bool slow = start(c, bad_logs, phase);
             if (c == nc) continue;
             if (pending && dg_warp) finish_dg(c + 1);
             pending = !slow;
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(kBwdThreads) bwd_kernel(const __grid_constant_
                 if (Smem::one_state) named_sync(2, 128);      // (and this group the state, for its dot)
                 phase ^= 1;
             }
-            bad = ds.template put<kFull3>(sm.tiles.ds[0]);
+            ds.template put<kFull3, !Smem::late>(sm.tiles.ds[0]);
         }
         __syncthreads();
         if (pending && dg_warp) finish_dg(0);

@@ -235,7 +235,7 @@ struct FwdSmem {
     static constexpr int resident = cols == 256 && sizeof(Tiles) + sizeof(bf16[MS][Wide<NT>::elements]) <= 108 * 1024 ? 2 : 1;   // blocks on an SM
 };
 
-// A chunk with a value that is not finite, token by token: 0 times such a value would spread it to tokens before it.
+// A chunk with an input that is not finite, token by token: 0 times such a value would spread it to tokens before it.
 // `s` (shared, NT x kP) holds the state before and after, `sum` a float for each thread.
 template <typename T>
 __device__ __noinline__ void walk_tokens(const FwdArgs& p, const T* q, const T* k, const T* v, const float* g, T* y, int rows, int cols,
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
     Pending<T, kP, kFwdThreads, VEC> pv;
     Logs logs{g, p.g_st};
     State<NT, 1> st(0);                                       // (warps 4 to 7)
-    bool bad = false, bad_logs = false;
+    bool bad_logs = false;
     sm.sync.init(Smem::cols);
     const uint32_t tm = __shfl_sync(kFull, sm.sync.tmem, 0), lanes = (uint32_t)w << 21;
     if (state_warp) {
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
         if (decay_warp) logs.fetch(0, len);
         if (from) st.load(from + col, z.n, cols, z.p);
         else st.zero();
-        bad = st.template put<MS>(sm.s[0]);
+        st.template put<MS, true>(sm.s[0]);
         if (decay_warp) {
             bad_logs = logs.bad();
             decays_of(sm.d[0], logs.a, logs.b);
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
                 pv.fetch(rows_of_token(p.v, t, h, col), p.v.st, rows, cols);
             }
             __syncthreads();                                  // decays are there; the chunk before is done with the tiles
-            bad |= bad_logs | pq.bad() | pk.bad() | pv.bad();
+            const bool bad = bad_logs | pq.bad() | pk.bad() | pv.bad();
             pq.put(sm.tiles.q[0]);
             pk.put(sm.tiles.k[0]);
             pv.put(sm.tiles.v[0]);
@@ -349,7 +349,6 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
             t5::fence_smem();
             t5::fence_before();
             slow = __syncthreads_or(bad);
-            bad = false;
             // (issuing takes as long as the products: the state's warps have the time for the long ones)
             if (!slow && warp == 0 && t5::elect()) {
                 t5::fence_after();
@@ -407,7 +406,7 @@ __global__ void __launch_bounds__(kFwdThreads, FwdSmem<T, NT>::resident) fwd_ker
                 t5::fence_before();
                 phase ^= 1;
             }
-            bad = st.template put<MS>(sm.s[0]);
+            st.template put<MS, true>(sm.s[0]);
             continue;
         }
         if (slow) continue;

@@ -186,3 +186,27 @@ def test_decode_equals_prefill_in_float32():
     for a, b, c in zip(states, some, packed_states):
         assert_close(b, _np(a), 16 * F32, "stepped states")
         assert_close(c, _np(a), 16 * F32, "packed states")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_an_infinite_gradient_does_not_slow_every_token_down(dtype):
+    """An overflow is an ordinary event of training with a loss scale.  The chunk that has it goes token by token, some 1.4 ms;
+    32 of them in a row would take 43 ms, where a clean backward takes 0.3 ms: 20 ms tell the two apart."""
+    t = _inputs(19 * 2048, 19, 8, 8, 64, 64, dtype, seed=81)
+    leaves = [t[k].reshape(19, 2048, *t[k].shape[1:]).requires_grad_(True) for k in ("q", "k", "v", "g")]
+    dy = t["dy"].reshape(19, 2048, 8, 64).clone()
+    dy[:, -1, :, 0] = math.inf
+    y, h = itf.decay_attention(*leaves)
+    took = []
+    for _ in range(3):
+        begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        begin.record()
+        grads = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+        end.record()
+        torch.cuda.synchronize()
+        took.append(begin.elapsed_time(end))
+    assert min(took) < 20, took
+    dq, dk, dv, dg = grads
+    assert not torch.isfinite(dq[:, -1]).any() and torch.isfinite(dq[:, :-1]).all() and torch.isfinite(dv[..., 1:]).all()
+    assert not torch.isfinite(dk).any() and not torch.isfinite(dv[..., 0]).any() and not torch.isfinite(dg[:, 1:]).any()

@@ -75,3 +75,30 @@ def test_close_to_two_to_the_31_tokens(cu):
             part = y[lo:min(b, lo + (1 << 28))]
             assert abs(part.min().item() - want) <= TOL[torch.bfloat16] * want and abs(part.max().item() - want) <= TOL[torch.bfloat16] * want
     assert abs(h[-1].item() - want) <= F32 * want
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_captured_step_goes_on_with_every_replay(dtype):
+    """A graph of one step, its inputs rewritten between the replays: what steps without a graph give, states at an offset of
+    4 bytes among others."""
+    B, H, N, P = 3, 4, 24, 40
+    t = _inputs(5 * B, B, H, 2, N, P, dtype, seed=91)
+    q, k, v, g = (t[x].reshape(5, B, *t[x].shape[1:]) for x in ("q", "k", "v", "g"))
+    for off in (0, 1):
+        room = torch.zeros(t["h0"].numel() + 4, device=dev)
+        h = room[off:off + t["h0"].numel()].view_as(t["h0"]).copy_(t["h0"])
+        plain = t["h0"].clone()
+        held = [x[0].clone() for x in (q, k, v, g)]
+        itf.decay_attention_step(*held, h.clone())
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = itf.decay_attention_step(*held, h)
+        for s in range(5):
+            for to, x in zip(held, (q, k, v, g)):
+                to.copy_(x[s])
+            graph.replay()
+            want = itf.decay_attention_step(q[s], k[s], v[s], g[s], plain)
+            assert_close(out, _np(want), TOL[dtype], "y")
+        assert_close(h, _np(plain), F32, "h")
+        assert (room[:off] == 0).all() and (room[off + h.numel():] == 0).all()

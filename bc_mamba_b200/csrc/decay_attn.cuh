@@ -9,9 +9,11 @@
 //
 // Numbers.  The products are of bf16 with fp32 sums.  An operand of more bits is a sum of bf16 pieces, each the rounding
 // of what the pieces before it left: float32 is three pieces (exact), float16 two (exact), and what a kernel computes
-// itself (masked scores, states, values times decays) has as many as its products need: two (relative 2^-18) where
-// they end in 16 bits, three where they end in float32.  Of the pieces' products those whose weight lies below that are
-// left out, and the small ones are added up first: the tensor cores cut sums off instead of rounding them, so that few
+// itself (masked scores, states, values times decays) has as many as its products need: two (within 2^-17, 2.5e-6 in the
+// root mean square) where they end in 16 bits, three where they end in float32.  Of the pieces' products those that lie
+// below that are left out: under 2^-24 of the whole product where results are float32 (a third piece times all but the
+// first), under 2^-16 where they are 16 bits wide (the two second pieces of float16 operands, or of a computed one and an
+// input).  The small ones are added up first: the tensor cores cut sums off instead of rounding them, so that few
 // additions may be made at the full sum.  States are float32 between chunks.  G is summed in float64 and kept as two
 // floats, so that a difference of two of its values keeps full precision after a decay of any size.
 #pragma once
@@ -575,7 +577,7 @@ bcm_status dispatch(bcm_dtype t, int64_t n, F&& f) {
     });
 }
 
-// a kernel's dynamic shared memory, allowed once per device; the opt-in is per kernel
+// allows a kernel its dynamic shared memory, on the current device (with every launch: the attribute is the device's)
 template <typename K>
 bcm_status allow_smem(K kernel, size_t bytes) {
     BCM_CUDA_TRY(cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));

@@ -20,10 +20,15 @@ bcm_status check(const bcm_decay_attn_args* a, const char* what) {
 
 // Blocks are (item, head, 64 columns of the values) and walk their item's chunks one after another.  Sequences are cut
 // into items only where whole ones leave much of the GPU without a block: an item costs one more pass over two inputs
-// and states to join (16 x 4096 tokens of 8 heads of 64 x 64 bf16, 128 blocks uncut: 537 us with its backward, cut in
-// two 674; 12 x 4096, 96 blocks, 532 and 648).  An item has 256 tokens at least.  `room` blocks are two turns of the walks, whose blocks one or two to an SM
-// hold, and one of the parts', four to an SM (one turn of the walks against two: 1 x 65536 tokens of 32 such heads 627 and
-// 574 us, forward and backward of 1 x 30011 of 12 heads 518 and 488 us).
+// and states to join.  The border, half a block to an SM, is that of training (16 x 4096 tokens of 8 heads of 64 x 64 bf16,
+// 128 blocks, uncut 537 us with its backward, cut in two 674; 12 x 4096, 96 blocks, 532 and 648).  A forward alone, whose
+// walks are two to an SM, loses by it behind the border: 1 x 65536 tokens of 75, 80, 112 and 148 such heads take 2610 us
+// uncut and would take 1418, 1426, 1968 and 2363 cut; 1 x 4096 tokens 178 us uncut and 133, 135, 166 and 193.  An item has
+// 256 tokens at least.  `room` blocks are two turns of the walks, whose blocks one or two to an SM hold, and one of the
+// parts', four to an SM (one turn of the walks against two: 1 x 65536 tokens of 32 such heads 627 and 574 us, forward and
+// backward of 1 x 30011 of 12 heads 518 and 488 us).  A packed batch is cut by its total, since only the device knows its
+// lengths: of many short sequences none has a second item, the parts' blocks end at once and the join copies entering
+// states that nothing reads.
 Plan plan_of(const bcm_decay_attn_args* a, bool backward) {
     Plan plan{};
     Sizes& z = plan.z;
@@ -210,9 +215,9 @@ struct FwdArgs {
 // times their decays until the chunk's end).  Warps 0 to 3 take 16 queries each: they mask and decay the scores, put their
 // pieces back into tensor memory as an operand, and add the two parts of y.  Warps 4 to 7 hold the state and advance it
 // meanwhile.  The next chunk's tiles are on their way to registers during all of that.
-// Bound by the chain of one chunk (tiles down, scores, their decay, the second product, rows out), about 4500 clocks with
-// one block on an SM, of which the tensor cores take 1850: 16 x 4096 tokens of 8 heads of 64 x 64 bf16 173 us (tensor pipe
-// 20 %, DRAM 21 %), 1 x 65536 of 32 heads, two blocks on an SM, 350 us behind 185 for the items' parts (33 and 31 %).
+// Bound by the chain of one chunk (tiles down, scores, their decay, the second product, rows out), 5300 clocks with one
+// block on an SM, of which the tensor pipe is active for 1060: 16 x 2048 tokens of 8 heads of 64 x 64 bf16 93 us (tensor
+// pipe 20 %, DRAM 22 %), 1 x 32768 of 32 heads, two blocks on an SM, 214 us behind 99 for the items' parts (32 and 30 %).
 // Twice the threads, with the rows dealt to eight warps, were slower: the barriers wait for more.
 constexpr int kFwdThreads = 256;
 
@@ -514,7 +519,7 @@ struct StepArgs {
 
 // A block per sequence and head: its threads hold V neighbouring columns each, and the rows of the state are dealt to
 // groups of threads, whose sums of q_n S_n meet in shared memory.  Bound by memory, the state read and written once:
-// one token of 256 x 64 heads of 64 x 64 92 us, 90 % of a copy's bandwidth (125 us when the state was read behind the
+// one token of 256 x 64 heads of 64 x 64 92 to 97 us, 85 to 90 % of a copy's bandwidth (125 us when the state was read behind the
 // queries' barrier).
 // ONE: one token in place (as a token of many 104 us).
 template <typename T, int V, bool ONE>
@@ -599,8 +604,9 @@ __global__ void __launch_bounds__(256) step_kernel(const __grid_constant__ StepA
     }
 }
 
-// Sequences of few tokens without a backward are not worth a chunk of 64 each: 2000 of 4 heads of 64 x 64 bf16 with 2, 4 and
-// 8 tokens take 75, 129 and 235 us one by one, 203 us as chunks (float32: 8 tokens 234 and 401 us).
+// Sequences of few tokens without a backward are not worth a chunk of 64 each: 2000 of 4 heads of 64 x 64 with 2, 4, 6, 8 and
+// 12 tokens take 78, 133, 186, 241 and 350 us one by one in every type; as chunks bf16 takes 196 us, float16 244, float32 372.
+// One border for all types, where the quickest as chunks still gains; float16 would up to 8 tokens, float32 up to 12.
 constexpr int kFewTokens = 4;
 // every sequence's tokens one by one, states from `from` (NULL: zeros) to h
 bcm_status launch_step(const bcm_decay_attn_args* a, const float* from, float* h, cudaStream_t stream) {

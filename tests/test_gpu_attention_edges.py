@@ -2,7 +2,6 @@
 test_gpu_decay_attention.py unless a test says otherwise."""
 import math
 
-import numpy as np
 import pytest
 import torch
 

@@ -634,9 +634,9 @@ __global__ void __launch_bounds__(kPartThreads, kPartResident<T, NT>) part_kerne
     const bool decay_warp = threadIdx.x >= 128 && threadIdx.x < 160;
     auto start = [&](int i) { return (BACK ? nc - 1 - i : i) * kChunk; };      // of the i-th chunk of the walk
     auto fetch = [&](int i) {
-        const int t = start(i), rows = min(kChunk, len - t);
+        const int t = start(i), rows = p.b.p ? min(kChunk, len - t) : 0;       // (no gradient: nothing, whatever q holds)
         pa.fetch(a + t * p.a.st, p.a.st, rows, z.n);
-        pb.fetch(b + t * p.b.st, p.b.st, p.b.p ? rows : 0, cols);
+        pb.fetch(b + t * p.b.st, p.b.st, rows, cols);
     };
     sm.sync.init(kCols);
     if (decay_warp) {

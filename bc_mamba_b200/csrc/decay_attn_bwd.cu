@@ -726,8 +726,8 @@ __global__ void __launch_bounds__(256) widen_kernel(const __grid_constant__ Rows
 #pragma unroll 4
         for (int i = lane_id(); i < n; i += 32) {
             const int h = i / per, c = (i - h * per) * V;
-            struct alignas(V * 2) In { __half v[V]; } x = {};
-            if (in.p) x = *(const In*)(from + h * in.sh + c);
+            struct alignas(V * 2) In { __half v[V]; };
+            const In x = *(const In*)(from + h * in.sh + c);
             struct alignas(V * 4 < 16 ? V * 4 : 16) Out { float v[V]; } y;
 #pragma unroll
             for (int e = 0; e < V; ++e) y.v[e] = to_f32(x.v[e]);
@@ -815,7 +815,7 @@ extern "C" bcm_status bcm_decay_attn_bwd(const bcm_decay_attn_args* a, cudaStrea
         Rows in[4] = {q, k, v, dy};
         void* dv = a->dv;
         if constexpr (widen) {
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < (dy.p ? 4 : 3); ++i) {                          // (no dy stays none)
                 const int heads = i < 2 ? z.qk_heads : z.heads, width = i < 2 ? z.n : z.p;
                 float* const to = (float*)(ws + room.wide[i]);
                 if (tokens > 0) {

@@ -101,3 +101,20 @@ def test_a_captured_step_goes_on_with_every_replay(dtype):
             assert_close(out, _np(want), TOL[dtype], "y")
         assert_close(h, _np(plain), F32, "h")
         assert (room[:off] == 0).all() and (room[off + h.numel():] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 100, 900])
+@pytest.mark.parametrize("N", [24, 72])
+def test_a_query_that_is_not_finite_without_a_gradient_of_y(rows, N, dtype):
+    """No gradient of y is no contribution, not zero times the query: whole sequences and cut ones alike."""
+    t = _inputs(rows, 1, 2, 1, N, 40, dtype, seed=95)
+    a = [_np(t[k]) for k in ("q", "k", "v", "g", "h0")]
+    want = orc.bwd(*a, (0, rows), None, _np(t["dh"]))
+    t["q"][rows // 3, 0, 5], t["q"][max(0, rows - 2), 0, 7] = math.nan, math.inf
+    leaves = [t[k][None].clone().requires_grad_(True) for k in ("q", "k", "v", "g")] + [t["h0"].clone().requires_grad_(True)]
+    _, h = itf.decay_attention(*leaves[:4], h0=leaves[4])
+    grads = torch.autograd.grad(h, leaves, t["dh"])
+    assert (grads[0] == 0).all()
+    for what, got, ref in zip(("dk", "dv", "dg", "dh0"), grads[1:], want[1:]):
+        assert_close(got.reshape(ref.shape), ref, TOL[dtype] if what in ("dk", "dv") else F32, what)
